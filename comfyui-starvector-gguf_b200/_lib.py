@@ -12,7 +12,7 @@ LIB_PATH = os.path.join(HERE, "libstarvector_sampling.so")
 
 SV_OK = 0
 SV_E_ARG, SV_E_DTYPE, SV_E_SHAPE, SV_E_RANGE, SV_E_ALIGN, SV_E_WORKSPACE, SV_E_CUDA = range(-1, -8, -1)
-ST_OK, ST_NAN, ST_POSINF, ST_ALLNEGINF, ST_HISTORY, ST_TIMEOUT, ST_SHARD_OVERFLOW, ST_GUARD_FULL = range(8)
+ST_OK, ST_NAN, ST_POSINF, ST_ALLNEGINF, ST_HISTORY, ST_TIMEOUT, ST_SHARD_OVERFLOW, ST_GUARD_FULL, ST_LENGTH = range(9)
 F32, F16, BF16 = 0, 1, 2
 HIST_NONE, HIST_IDS32, HIST_IDS64, HIST_MASK8, HIST_BITS32 = range(5)
 DENSE_NONE, DENSE_SCORES, DENSE_PROBS = range(3)
@@ -47,6 +47,14 @@ _SIGNATURES = {
     "sv_beam_advance": (_I32, [_P, _P, _P, _P, _I32, _I32, _I32, _I32, _I32, _P, _I32, _I64, _P, _P, _P, _P, _P, _P,
                                _P, _I64, _P, _P, _I64, _P, _P, _P, _I64, _I32, _P]),
     "sv_loop_guard_incremental": (_I32, [_P, _I64, _P, _I32, _I64, _I64, _I32, _I32, _P, _P, _P]),
+    "sv_window_attention_workspace_bytes": (_SZ, [_I32] * 10),
+    "sv_window_attention": (_I32, [_P, _I32, _I32, _I32, _I32, _I32, _I32, _I64, _I64, _I64, _P, _P, _I32, _I64, _I64,
+                                   _I64, _P, _P, _I32, _I32, _D, _P, _I64, _I64, _P, _P, _SZ, _P, _P]),
+    "sv_prefix_attention_workspace_bytes": (_SZ, [_I32] * 8),
+    "sv_prefix_attention": (_I32, [_P, _I32, _I32, _I32, _I32, _I32, _I32, _I64, _I64, _I64, _P, _P, _I32, _I64, _I64,
+                                   _P, _P, _I32, _I64, _I64, _I64, _P, _D, _P, _P, _SZ, _P, _P]),
+    "sv_kv_evict": (_I32, [_P, _P, _I32, _I32, _I32, _I32, _I32, _I32, _I64, _I64, _I64, _I64, _P, _P, _P, _I32, _I32,
+                           _I32, _P, _P, _P, _P, _P]),
     "sv_error_string": (C.c_char_p, [_I32]),
     "sv_abi_version": (_I32, []),
 }

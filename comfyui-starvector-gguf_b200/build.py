@@ -2,8 +2,8 @@
 
     python comfyui-starvector-gguf_b200/build.py [--force] [--verbose]
 
-nvcc compiles csrc/*.cu for sm_100a (-gencode arch=compute_100a,code=sm_100a) into
-libstarvector_sampling.so next to this file, with the CUDA runtime linked
+nvcc compiles csrc/*.cu for sm_100a (-gencode arch=compute_100a,code=sm_100a), the
+sources in parallel, into libstarvector_sampling.so next to this file, with the CUDA runtime linked
 statically so the library does not depend on the runtime version torch ships.
 g++ then compiles ext/sv_torch.cpp against torch's headers into the extension
 module sv_torch (next to this file), linked to that library: the tensor-level
@@ -15,10 +15,12 @@ import glob
 import os
 import subprocess
 import sys
+from concurrent.futures import ThreadPoolExecutor
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 INCLUDE = os.path.join(os.path.dirname(HERE), "include")
+OBJ = os.path.join(HERE, ".build")  # object files, one per source
 LIB = os.path.join(HERE, "libstarvector_sampling.so")
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
@@ -43,11 +45,25 @@ def up_to_date() -> bool:
 def build(force: bool = False, verbose: bool = False) -> str:
     if not force and up_to_date():
         return LIB
-    cmd = [NVCC, *ARCH, "-O3", "-lineinfo", "-std=c++17", "--shared", "-Xcompiler", "-fPIC",
-           "-cudart", "static", "-I", INCLUDE, "-o", LIB + ".tmp", *sources()]
-    if verbose:
-        cmd.insert(1, "-Xptxas=-v")
-    subprocess.run(cmd, check=True)
+    os.makedirs(OBJ, exist_ok=True)
+    headers = max(os.path.getmtime(p) for p in _deps() if not p.endswith(".cu"))
+
+    def compile_one(src):
+        """One source to an object file, unless it is newer than the source and every header."""
+        obj = os.path.join(OBJ, os.path.basename(src)[:-3] + ".o")
+        if force or not os.path.exists(obj) or os.path.getmtime(obj) < max(os.path.getmtime(src), headers):
+            cmd = [NVCC, *ARCH, "-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC", "-I", INCLUDE, "-c", src,
+                   "-o", obj + ".tmp"]
+            if verbose:
+                cmd.insert(1, "-Xptxas=-v")
+            subprocess.run(cmd, check=True)
+            os.replace(obj + ".tmp", obj)
+        return obj
+
+    with ThreadPoolExecutor(os.cpu_count() or 1) as pool:
+        objects = list(pool.map(compile_one, sources()))
+    subprocess.run([NVCC, *ARCH, "--shared", "-Xcompiler", "-fPIC", "-cudart", "static", "-o", LIB + ".tmp", *objects],
+                   check=True)
     os.replace(LIB + ".tmp", LIB)
     return LIB
 

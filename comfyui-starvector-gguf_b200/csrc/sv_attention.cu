@@ -1,0 +1,207 @@
+// sv_attention.cu -- entry points of the attention over the decoder's cache: argument
+// checks, the split of the slots over blocks, workspace layout and launches.
+#include <cmath>
+
+#include "../../include/starvector_sampling.h"
+#include "sv_attention.h"
+
+namespace sv {
+namespace {
+
+constexpr int kSMs = 148;
+
+size_t up256(size_t x) { return (x + 255) / 256 * 256; }
+
+int div_up(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
+
+// The most slots one row's query tile can see.
+int64_t most_slots(int32_t capacity, int32_t window, int32_t sinks, int64_t tile_queries) {
+  if (!window) return capacity;
+  const int64_t x = (int64_t)window + sinks + tile_queries - 1;
+  return x < capacity ? x : capacity;
+}
+
+// Splits of the slots: enough blocks for every SM twice, at least two 64-slot tiles
+// each.
+int choose_splits(int64_t blocks, int64_t slots) {
+  if (blocks >= 2 * kSMs) return 1;
+  const int64_t want = (2 * kSMs + blocks - 1) / blocks, most = (slots + 127) / 128;
+  const int64_t s = want < most ? want : most;
+  return (int)(s < 1 ? 1 : s);
+}
+
+struct Plan {
+  int p_splits, o_splits;
+  size_t o_bytes, ml_bytes, lse_bytes;
+  size_t total() const { return o_bytes + ml_bytes + lse_bytes; }
+};
+
+Plan make_plan(const AttnArgs& a) {
+  Plan p = {};
+  const int64_t nG = (int64_t)a.n * a.group, all = a.rows * a.kv_heads * nG;
+  const int64_t bm = nG <= 16 ? 16 : 64;
+  const int64_t blocks = a.rows * a.kv_heads * div_up(nG, bm);
+  p.o_splits = choose_splits(blocks, most_slots(a.capacity, a.window, a.sinks, div_up(bm, a.group)));
+  if (a.prefix) {
+    const int64_t m = a.rows * nG, pb = a.kv_heads * div_up(m, m <= 16 ? 16 : 64);
+    p.p_splits = choose_splits(pb, a.prefix);
+  } else if (p.o_splits == 1) {
+    p.o_splits = 0;
+  }
+  const int64_t slots = p.p_splits + p.o_splits;
+  p.o_bytes = up256(slots * all * a.dim * 4);
+  p.ml_bytes = up256(slots * all * 8);
+  p.lse_bytes = a.weights ? up256(all * 4) : 0;
+  return p;
+}
+
+int check_shapes(const AttnArgs& a) {
+  if (a.dtype != SV_F32 && a.dtype != SV_F16 && a.dtype != SV_BF16) return SV_E_DTYPE;
+  if (a.rows < 1 || a.n < 1 || a.heads < 1 || a.kv_heads < 1 || a.heads % a.kv_heads || a.capacity < 1)
+    return SV_E_SHAPE;
+  if (a.dim < 8 || a.dim > kAttnMaxDim || a.dim % 8) return SV_E_SHAPE;
+  if ((int64_t)a.rows * a.kv_heads > 65535 || (int64_t)a.rows * a.n * a.heads > (int64_t)1 << 30) return SV_E_SHAPE;
+  if (a.window < 0 || a.sinks < 0 || a.window > 1 << 30 || a.sinks > 1 << 30 || a.capacity > 1 << 30 ||
+      a.prefix > 1 << 30)
+    return SV_E_SHAPE;
+  return SV_OK;
+}
+
+int check_pointers(const AttnArgs& a, double scale) {
+  if (!a.q || !a.k || !a.v || !a.out || (a.prefix && (!a.pk || !a.pv))) return SV_E_ARG;
+  if (!std::isfinite(scale)) return SV_E_RANGE;
+  const int64_t e = a.dtype == SV_F32 ? 4 : 2;
+  const int64_t strides[8] = {a.q_row, a.q_tok, a.q_head, a.kv_row, a.kv_head, a.kv_slot, a.p_head, a.p_slot};
+  for (int64_t s : strides)
+    if (s < 0 || s * e % 16) return SV_E_ALIGN;
+  const void* ptrs[6] = {a.q, a.k, a.v, a.pk, a.pv, a.out};
+  for (const void* p : ptrs)
+    if (reinterpret_cast<uintptr_t>(p) % 16) return SV_E_ALIGN;
+  if (a.weights && (a.w_row < 0 || a.w_head < 0)) return SV_E_SHAPE;
+  return SV_OK;
+}
+
+int run(AttnArgs& a, void* workspace, size_t workspace_bytes, cudaStream_t stream) {
+  const Plan p = make_plan(a);
+  if (p.total() && (!workspace || workspace_bytes < p.total())) return SV_E_WORKSPACE;
+  if (reinterpret_cast<uintptr_t>(workspace) % 16) return SV_E_ALIGN;
+  unsigned char* w = static_cast<unsigned char*>(workspace);
+  a.p_splits = p.p_splits;
+  a.o_splits = p.o_splits;
+  a.part_o = reinterpret_cast<float*>(w);
+  a.part_ml = reinterpret_cast<float2*>(w + p.o_bytes);
+  a.lse = a.weights ? reinterpret_cast<float*>(w + p.o_bytes + p.ml_bytes) : nullptr;
+  if (a.prefix && launch_attn_simt(a, true, stream) != cudaSuccess) return SV_E_CUDA;
+  if (launch_attn_simt(a, false, stream) != cudaSuccess) return SV_E_CUDA;
+  if (p.o_splits && launch_attn_combine(a, stream) != cudaSuccess) return SV_E_CUDA;
+  if (a.weights && launch_attn_weights(a, stream) != cudaSuccess) return SV_E_CUDA;
+  return SV_OK;
+}
+
+AttnArgs base_args(int32_t dtype, int32_t rows, int32_t tokens, int32_t heads, int32_t kv_heads, int32_t head_dim,
+                   int32_t capacity) {
+  AttnArgs a = {};
+  a.dtype = dtype;
+  a.rows = rows;
+  a.n = tokens;
+  a.heads = heads;
+  a.kv_heads = kv_heads;
+  a.group = kv_heads > 0 ? heads / kv_heads : 0;
+  a.dim = head_dim;
+  a.capacity = capacity;
+  return a;
+}
+
+}  // namespace
+}  // namespace sv
+
+using namespace sv;
+
+extern "C" {
+
+size_t sv_window_attention_workspace_bytes(int32_t dtype, int32_t rows, int32_t tokens, int32_t heads,
+                                           int32_t kv_heads, int32_t head_dim, int32_t capacity, int32_t window,
+                                           int32_t sinks, int32_t with_weights) {
+  AttnArgs a = base_args(dtype, rows, tokens, heads, kv_heads, head_dim, capacity);
+  a.window = window;
+  a.sinks = sinks;
+  if (check_shapes(a)) return 0;
+  float dummy;
+  a.weights = with_weights ? &dummy : nullptr;
+  return make_plan(a).total();
+}
+
+int sv_window_attention(const void* q, int32_t dtype, int32_t rows, int32_t tokens, int32_t heads, int32_t kv_heads,
+                        int32_t head_dim, int64_t q_stride_row, int64_t q_stride_token, int64_t q_stride_head,
+                        const void* keys, const void* values, int32_t capacity, int64_t kv_stride_row,
+                        int64_t kv_stride_head, int64_t kv_stride_slot, const int32_t* lengths, const int32_t* starts,
+                        int32_t window, int32_t sinks, double scale, float* weights, int64_t weights_stride_row,
+                        int64_t weights_stride_head, void* out, void* workspace, size_t workspace_bytes,
+                        int32_t* out_status, void* stream) {
+  AttnArgs a = base_args(dtype, rows, tokens, heads, kv_heads, head_dim, capacity);
+  a.q = q;
+  a.q_row = q_stride_row;
+  a.q_tok = q_stride_token;
+  a.q_head = q_stride_head;
+  a.k = keys;
+  a.v = values;
+  a.kv_row = kv_stride_row;
+  a.kv_head = kv_stride_head;
+  a.kv_slot = kv_stride_slot;
+  a.lengths = lengths;
+  a.starts = starts;
+  a.window = window;
+  a.sinks = sinks;
+  a.scale = (float)(scale * 1.4426950408889634);
+  a.weights = weights;
+  a.w_row = weights_stride_row;
+  a.w_head = weights_stride_head;
+  a.out = out;
+  a.status = out_status;
+  int rc = check_shapes(a);
+  if (!rc) rc = check_pointers(a, scale);
+  return rc ? rc : run(a, workspace, workspace_bytes, static_cast<cudaStream_t>(stream));
+}
+
+size_t sv_prefix_attention_workspace_bytes(int32_t dtype, int32_t rows, int32_t tokens, int32_t heads,
+                                           int32_t kv_heads, int32_t head_dim, int32_t prefix_length,
+                                           int32_t capacity) {
+  AttnArgs a = base_args(dtype, rows, tokens, heads, kv_heads, head_dim, capacity);
+  a.prefix = prefix_length;
+  if (prefix_length < 0 || check_shapes(a)) return 0;
+  return make_plan(a).total();
+}
+
+int sv_prefix_attention(const void* q, int32_t dtype, int32_t rows, int32_t tokens, int32_t heads, int32_t kv_heads,
+                        int32_t head_dim, int64_t q_stride_row, int64_t q_stride_token, int64_t q_stride_head,
+                        const void* prefix_keys, const void* prefix_values, int32_t prefix_length,
+                        int64_t prefix_stride_head, int64_t prefix_stride_slot, const void* keys, const void* values,
+                        int32_t capacity, int64_t kv_stride_row, int64_t kv_stride_head, int64_t kv_stride_slot,
+                        const int32_t* lengths, double scale, void* out, void* workspace, size_t workspace_bytes,
+                        int32_t* out_status, void* stream) {
+  AttnArgs a = base_args(dtype, rows, tokens, heads, kv_heads, head_dim, capacity);
+  a.q = q;
+  a.q_row = q_stride_row;
+  a.q_tok = q_stride_token;
+  a.q_head = q_stride_head;
+  a.pk = prefix_keys;
+  a.pv = prefix_values;
+  a.prefix = prefix_length;
+  a.p_head = prefix_stride_head;
+  a.p_slot = prefix_stride_slot;
+  a.k = keys;
+  a.v = values;
+  a.kv_row = kv_stride_row;
+  a.kv_head = kv_stride_head;
+  a.kv_slot = kv_stride_slot;
+  a.lengths = lengths;
+  a.scale = (float)(scale * 1.4426950408889634);
+  a.out = out;
+  a.status = out_status;
+  if (prefix_length < 0) return SV_E_SHAPE;
+  int rc = check_shapes(a);
+  if (!rc) rc = check_pointers(a, scale);
+  return rc ? rc : run(a, workspace, workspace_bytes, static_cast<cudaStream_t>(stream));
+}
+
+}  // extern "C"

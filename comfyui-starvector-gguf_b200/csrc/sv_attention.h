@@ -1,0 +1,107 @@
+// sv_attention.h -- launch descriptors of the cache attention kernels, shared by the
+// entry points (sv_attention.cu) and the kernel files.
+//
+// Query rows are packed by key/value head: the n x G rows (query i, head g of the
+// group) that read one head's slots are numbered m = i * G + g, so a tile of rows
+// loads each slot once for the whole group.  Over the call a row's index is
+//   idx = (r * kv_heads + h) * n * G + m.
+// Work that is split over the slots leaves, per split and row, an unnormalised f32
+// output and its (maximum, sum) in the workspace; the maximum is in units of
+// log2 (score * scale * log2 e), so weights are exp2(s - m).
+#pragma once
+#include <cstdint>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+namespace sv {
+
+constexpr int kAttnMaxDim = 128;
+
+struct AttnArgs {
+  const void* q;
+  int64_t q_row, q_tok, q_head;  // strides in elements; head_dim is contiguous
+  const void *k, *v;             // the rows' own slots
+  int64_t kv_row, kv_head, kv_slot;
+  const void *pk, *pv;  // the shared prefix (prefix = 0: none)
+  int64_t p_head, p_slot;
+  int32_t prefix;
+  int32_t dtype, rows, n, heads, kv_heads, group, dim, capacity;
+  const int32_t *lengths, *starts;  // per row, may be null (capacity, 0)
+  int32_t window, sinks;            // window 0: none
+  float scale;                      // scale * log2 e
+  float* weights;                   // accumulated attention weights, may be null
+  int64_t w_row, w_head;
+  void* out;  // [rows, n, heads, dim]
+  int32_t* status;
+  // workspace
+  float* part_o;   // [slots][idx][dim]
+  float2* part_ml; // [slots][idx]
+  float* lse;      // [idx], with weights only: log2 of the softmax denominator, maximum included
+  int32_t p_splits, o_splits;  // workspace slots of the prefix and of the own part (0 own: written directly)
+};
+
+// The slots that row r's queries can see: queries stand at p = end - n + i, slots
+// before `start` (padding in front) are never seen.
+struct RowSpan {
+  int start, end;
+};
+
+__device__ __forceinline__ RowSpan row_span(const AttnArgs& a, int r) {
+  int end = a.lengths ? a.lengths[r] : a.capacity;
+  end = min(max(end, 0), a.capacity);
+  int start = a.starts ? a.starts[r] : 0;
+  start = min(max(start, 0), end);
+  return {start, end};
+}
+
+// First slot of the window of a query at position p.
+__device__ __forceinline__ int window_low(const AttnArgs& a, int start, int p) {
+  return a.window ? max(start, p - a.window + 1) : start;
+}
+
+// Whether the query at p (window from lo) sees slot j of a row that starts at start.
+__device__ __forceinline__ bool slot_seen(const AttnArgs& a, int start, int p, int lo, int j) {
+  return j <= p && j >= start && (j >= lo || j < start + a.sinks);
+}
+
+template <typename T> __device__ __forceinline__ T from_float(float x);
+template <> __device__ __forceinline__ float from_float<float>(float x) { return x; }
+template <> __device__ __forceinline__ __half from_float<__half>(float x) { return __float2half_rn(x); }
+template <> __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float x) {
+  return __float2bfloat16_rn(x);
+}
+
+// Eight consecutive elements as floats (16-byte aligned for the 16-bit types, two
+// such vectors for float).
+__device__ __forceinline__ void load8(const float* p, float* x) {
+  const float4 a = __ldg(reinterpret_cast<const float4*>(p)), b = __ldg(reinterpret_cast<const float4*>(p) + 1);
+  x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
+  x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+}
+__device__ __forceinline__ void load8(const __half* p, float* x) {
+  const uint4 a = __ldg(reinterpret_cast<const uint4*>(p));
+  const __half2* h = reinterpret_cast<const __half2*>(&a);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 f = __half22float2(h[i]);
+    x[2 * i] = f.x;
+    x[2 * i + 1] = f.y;
+  }
+}
+__device__ __forceinline__ void load8(const __nv_bfloat16* p, float* x) {
+  const uint4 a = __ldg(reinterpret_cast<const uint4*>(p));
+  const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&a);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 f = __bfloat1622float2(h[i]);
+    x[2 * i] = f.x;
+    x[2 * i + 1] = f.y;
+  }
+}
+
+cudaError_t launch_attn_simt(const AttnArgs& a, bool prefix, cudaStream_t stream);
+cudaError_t launch_attn_combine(const AttnArgs& a, cudaStream_t stream);
+cudaError_t launch_attn_weights(const AttnArgs& a, cudaStream_t stream);
+
+}  // namespace sv

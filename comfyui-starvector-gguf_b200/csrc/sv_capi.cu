@@ -302,7 +302,7 @@ const char* sv_error_string(int32_t code) {
     case SV_E_ARG: return "invalid argument (null pointer or inconsistent arguments)";
     case SV_E_DTYPE: return "unknown dtype, history kind or dense mode";
     case SV_E_SHAPE: return "rows, vocab, strides or capacities out of range";
-    case SV_E_RANGE: return "temperature, top_p, top_k, keep or repetition_penalty out of range";
+    case SV_E_RANGE: return "temperature, top_p, top_k, keep, repetition_penalty, scale, budget, sinks or recent out of range";
     case SV_E_ALIGN: return "pointer not aligned to its element size";
     case SV_E_WORKSPACE: return "workspace missing or too small";
     case SV_E_CUDA: return "CUDA launch failed";
@@ -313,6 +313,7 @@ const char* sv_error_string(int32_t code) {
     case SV_ST_HISTORY: return "history id outside [0, vocab)";
     case SV_ST_TIMEOUT: return "asynchronous copy wait timed out";
     case SV_ST_SHARD_OVERFLOW: return "a vocabulary slice kept more tokens than its list holds (sample unsharded)";
+    case SV_ST_LENGTH: return "a row's length or start lies outside its cache";
     case SV_ST_GUARD_FULL: return "the loop guard's window table is full";
     default: return "unknown code";
   }

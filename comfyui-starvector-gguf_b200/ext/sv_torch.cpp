@@ -6,13 +6,18 @@
 // returns its code (0 or a negative SV_E_*; ops.py turns codes into the same
 // exceptions as before).  Shapes and the history form are decided by the Python
 // wrappers (ops.py), which pass the same sizes and strides as the C signatures;
-// nothing here synchronises or allocates.
+// nothing here synchronises, and only the cache operators (window_attention,
+// prefix_attention, kv_evict) allocate: their outputs and a workspace kept per
+// device, stream and size.
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
 
+#include <cmath>
 #include <cstdint>
+#include <map>
 #include <optional>
+#include <tuple>
 
 #include "../../include/starvector_sampling.h"
 
@@ -188,6 +193,132 @@ int loop_guard_incremental(const at::Tensor& table, const at::Tensor& tokens, in
   return rc;
 }
 
+// A workspace of at least `bytes` whose first `zeroed` bytes were zero before its
+// first use, kept per device, stream and power of two for the life of the process
+// (calls on different streams may overlap).  Under a stream capture it comes from the
+// graph's own pool instead, cleared by a node of the graph: a kept one would be
+// cleared only when the graph runs, and eager calls could overlap the graph's.
+at::Tensor workspace_for(const at::Device& dev, c10::cuda::CUDAStream stream, size_t bytes, size_t zeroed) {
+  const auto opts = at::TensorOptions().dtype(at::kByte).device(dev);
+  if (bytes == 0) return at::Tensor();
+  if (c10::cuda::currentStreamCaptureStatusMayInitCtx() != c10::cuda::CaptureStatus::None) {
+    at::Tensor t = at::empty({(int64_t)bytes}, opts);
+    t.narrow(0, 0, (int64_t)std::min(bytes, zeroed)).zero_();
+    return t;
+  }
+  static auto* kept = new std::map<std::tuple<int, void*, size_t>, at::Tensor>;
+  size_t size = 1 << 16;
+  while (size < bytes) size *= 2;
+  at::Tensor& t = (*kept)[std::make_tuple((int)dev.index(), (void*)stream.stream(), size)];
+  if (!t.defined()) t = at::zeros({(int64_t)size}, opts);
+  return t;
+}
+
+// Strides of a dimension of one entry mean nothing: 0 stands for them.
+int64_t stride_of(const at::Tensor& t, int64_t d) { return t.size(d) > 1 ? t.stride(d) : 0; }
+
+at::Tensor attention_out(const OptT& out, const at::Tensor& q, const at::Device& dev) {
+  if (!out.has_value()) return at::empty(q.sizes(), q.options());
+  on_device(*out, dev, "out");
+  TORCH_CHECK(out->scalar_type() == q.scalar_type() && out->numel() == q.numel() && out->is_contiguous(),
+              "out must be a contiguous tensor of the queries' shape and dtype");
+  return *out;
+}
+
+void same_cache(const at::Tensor& k, const at::Tensor& v, const at::Tensor& q, const at::Device& dev) {
+  on_device(k, dev, "keys");
+  on_device(v, dev, "values");
+  TORCH_CHECK(k.scalar_type() == q.scalar_type() && v.scalar_type() == q.scalar_type(),
+              "queries, keys and values must have one dtype");
+}
+
+// sv_window_attention.  q [rows, tokens, heads, head_dim], keys / values [rows,
+// kv_heads, capacity, head_dim], weights [rows, kv_heads, capacity].
+std::tuple<int, at::Tensor> window_attention(const at::Tensor& q, const at::Tensor& keys, const at::Tensor& values,
+                                             const OptT& lengths, const OptT& starts, int64_t window, int64_t sinks,
+                                             double scale, const OptT& weights, const OptT& out,
+                                             const OptT& out_status) {
+  const at::Device dev = q.device();
+  on_device(q, dev, "q");
+  same_cache(keys, values, q, dev);
+  const c10::cuda::CUDAGuard guard(dev);
+  const auto stream = at::cuda::getCurrentCUDAStream(dev.index());
+  const int32_t rows = (int32_t)q.size(0), n = (int32_t)q.size(1), heads = (int32_t)q.size(2), dim = (int32_t)q.size(3);
+  const int32_t kv = (int32_t)keys.size(1), capacity = (int32_t)keys.size(2), code = logit_code(q);
+  at::Tensor o = attention_out(out, q, dev);
+  const size_t bytes = sv_window_attention_workspace_bytes(code, rows, n, heads, kv, dim, capacity, (int32_t)window,
+                                                           (int32_t)sinks, weights.has_value());
+  at::Tensor ws = workspace_for(dev, stream, bytes, 4 * (size_t)rows * kv);
+  const int rc = sv_window_attention(
+      q.data_ptr(), code, rows, n, heads, kv, dim, stride_of(q, 0), stride_of(q, 1), stride_of(q, 2), keys.data_ptr(),
+      values.data_ptr(), capacity, stride_of(keys, 0), stride_of(keys, 1), stride_of(keys, 2),
+      optptr<int32_t>(lengths, dev, "lengths", at::kInt, rows), optptr<int32_t>(starts, dev, "starts", at::kInt, rows),
+      (int32_t)window, (int32_t)sinks, scale, optptr<float>(weights, dev, "weights", at::kFloat),
+      weights.has_value() ? stride_of(*weights, 0) : 0, weights.has_value() ? stride_of(*weights, 1) : 0,
+      o.data_ptr(), ws.defined() ? ws.data_ptr() : nullptr, ws.defined() ? (size_t)ws.numel() : 0,
+      optptr<int32_t>(out_status, dev, "status", at::kInt, rows), stream.stream());
+  return {rc, o};
+}
+
+// sv_prefix_attention.  prefix_keys / prefix_values [kv_heads, prefix_length, head_dim].
+std::tuple<int, at::Tensor> prefix_attention(const at::Tensor& q, const at::Tensor& prefix_keys,
+                                             const at::Tensor& prefix_values, const at::Tensor& keys,
+                                             const at::Tensor& values, const OptT& lengths, double scale,
+                                             const OptT& out, const OptT& out_status) {
+  const at::Device dev = q.device();
+  on_device(q, dev, "q");
+  same_cache(keys, values, q, dev);
+  same_cache(prefix_keys, prefix_values, q, dev);
+  const c10::cuda::CUDAGuard guard(dev);
+  const auto stream = at::cuda::getCurrentCUDAStream(dev.index());
+  const int32_t rows = (int32_t)q.size(0), n = (int32_t)q.size(1), heads = (int32_t)q.size(2), dim = (int32_t)q.size(3);
+  const int32_t kv = (int32_t)keys.size(1), capacity = (int32_t)keys.size(2), code = logit_code(q);
+  const int32_t prefix = (int32_t)prefix_keys.size(1);
+  at::Tensor o = attention_out(out, q, dev);
+  const size_t bytes = sv_prefix_attention_workspace_bytes(code, rows, n, heads, kv, dim, prefix, capacity);
+  at::Tensor ws = workspace_for(dev, stream, bytes, 4 * (size_t)rows * kv);
+  const int rc = sv_prefix_attention(
+      q.data_ptr(), code, rows, n, heads, kv, dim, stride_of(q, 0), stride_of(q, 1), stride_of(q, 2),
+      prefix_keys.data_ptr(), prefix_values.data_ptr(), prefix, stride_of(prefix_keys, 0), stride_of(prefix_keys, 1),
+      keys.data_ptr(), values.data_ptr(), capacity, stride_of(keys, 0), stride_of(keys, 1), stride_of(keys, 2),
+      optptr<int32_t>(lengths, dev, "lengths", at::kInt, rows), scale, o.data_ptr(),
+      ws.defined() ? ws.data_ptr() : nullptr, ws.defined() ? (size_t)ws.numel() : 0,
+      optptr<int32_t>(out_status, dev, "status", at::kInt, rows), stream.stream());
+  return {rc, o};
+}
+
+// sv_kv_evict.  keys / values [layers, rows, heads, capacity, head_dim], weights /
+// positions [layers, rows, heads, capacity] contiguous.
+std::tuple<int, at::Tensor, at::Tensor, at::Tensor> kv_evict(const at::Tensor& keys, const OptT& values,
+                                                             const at::Tensor& weights, const at::Tensor& positions,
+                                                             const OptT& lengths, int64_t budget, int64_t sinks,
+                                                             int64_t recent, const OptT& weights_out,
+                                                             const OptT& positions_out, const OptT& lengths_out,
+                                                             const OptT& out_status) {
+  const at::Device dev = keys.device();
+  on_device(keys, dev, "keys");
+  const c10::cuda::CUDAGuard guard(dev);
+  const int64_t layers = keys.size(0), rows = keys.size(1), heads = keys.size(2), capacity = keys.size(3);
+  const int64_t all = layers * rows * heads * capacity;
+  at::Tensor wo = weights_out.has_value() ? *weights_out : at::empty_like(weights);
+  at::Tensor po = positions_out.has_value() ? *positions_out : at::empty_like(positions);
+  at::Tensor lo = lengths_out.has_value() ? *lengths_out
+                                          : at::empty({rows}, at::TensorOptions().dtype(at::kInt).device(dev));
+  TORCH_CHECK(weights.is_contiguous() && positions.is_contiguous() && wo.is_contiguous() && po.is_contiguous() &&
+                  lo.is_contiguous(),
+              "weights and positions must be contiguous");
+  const int rc = sv_kv_evict(
+      keys.data_ptr(), raw(values, dev, "values"), (int32_t)keys.element_size(), (int32_t)layers, (int32_t)rows,
+      (int32_t)heads, (int32_t)capacity, (int32_t)keys.size(4), stride_of(keys, 0), stride_of(keys, 1),
+      stride_of(keys, 2), stride_of(keys, 3), ptr<float>(weights, dev, "weights", at::kFloat, all),
+      ptr<int32_t>(positions, dev, "positions", at::kInt, all),
+      optptr<int32_t>(lengths, dev, "lengths", at::kInt, rows), (int32_t)budget, (int32_t)sinks, (int32_t)recent,
+      ptr<float>(wo, dev, "weights_out", at::kFloat, all), ptr<int32_t>(po, dev, "positions_out", at::kInt, all),
+      ptr<int32_t>(lo, dev, "lengths_out", at::kInt, rows), optptr<int32_t>(out_status, dev, "status", at::kInt, rows),
+      stream_of(keys));
+  return {rc, lo, wo, po};
+}
+
 }  // namespace
 
 PYBIND11_MODULE(sv_torch, m) {
@@ -199,4 +330,7 @@ PYBIND11_MODULE(sv_torch, m) {
   m.def("kv_reorder", &kv_reorder);
   m.def("loop_guard", &loop_guard);
   m.def("loop_guard_incremental", &loop_guard_incremental);
+  m.def("window_attention", &window_attention);
+  m.def("prefix_attention", &prefix_attention);
+  m.def("kv_evict", &kv_evict);
 }

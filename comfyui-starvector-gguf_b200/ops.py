@@ -3,8 +3,8 @@
 Every function enqueues on the current CUDA stream of the tensors' device and does
 not synchronise; results are device tensors.  Inputs must be CUDA tensors: there is
 no CPU path.  The hot entry points (sample_step, beam_step, beam_advance,
-kv_reorder, loop_guard, loop_guard_incremental) go through the thin PyTorch
-extension sv_torch (ext/sv_torch.cpp), the others through ctypes (_lib.py); both
+kv_reorder, loop_guard, loop_guard_incremental, window_attention, prefix_attention,
+kv_evict) go through the thin PyTorch extension sv_torch (ext/sv_torch.cpp), the others through ctypes (_lib.py); both
 call the same C library.
 """
 from __future__ import annotations
@@ -555,3 +555,163 @@ def kv_reorder(keys, values, parents, length, out_status=None):
         raise ValueError("parents must be a contiguous int64 tensor [beams]")
     rc = _ext().kv_reorder(keys, values, Lr, B, H, int(length), D, sl, sb, sh, ss, p, out_status)
     L.check(rc, "sv_kv_reorder")
+
+
+def _queries(q):
+    """q as [rows, tokens, heads, head_dim] with 16-byte aligned rows; [rows, heads,
+    head_dim] stands for one token."""
+    _need_cuda(q, "q")
+    x = q.unsqueeze(1) if q.dim() == 3 else q
+    if x.dim() != 4:
+        raise ValueError("q must be [rows, tokens, heads, head_dim] or [rows, heads, head_dim]")
+    if x.dtype not in _DTYPES:
+        raise ValueError(f"unsupported dtype {x.dtype}")
+    size, e = x.shape, x.element_size()
+    if x.stride(3) != 1 or x.data_ptr() % 16 or any(size[d] > 1 and x.stride(d) * e % 16 for d in (0, 1, 2)):
+        x = x.clone(memory_format=torch.contiguous_format)
+    return x
+
+
+def _layer_cache(keys, values, q, length, names=("keys", "values")):
+    """One layer's keys and values as [rows, kv_heads, capacity, head_dim], cut to
+    `length` slots when it is a number; checked against q."""
+    _need_cuda(keys, names[0])
+    _need_cuda(values, names[1])
+    if keys.dim() == 3:
+        keys, values = keys.unsqueeze(1), values.unsqueeze(1)
+    if keys.dim() != 4 or values.shape != keys.shape or values.stride() != keys.stride():
+        raise ValueError(f"{names[0]} must be [rows, capacity, head_dim] or [rows, kv_heads, capacity, head_dim], "
+                         f"and {names[1]} have their shape and strides")
+    R, K, cap, D = keys.shape
+    if keys.dtype != q.dtype or values.dtype != q.dtype:
+        raise ValueError(f"{names[0]} and {names[1]} must have q's dtype")
+    if R != q.shape[0] or D != q.shape[3] or K < 1 or q.shape[2] % K:
+        raise ValueError(f"{names[0]} must have q's rows and head_dim, and kv_heads must divide heads")
+    if D > 1 and keys.stride(3) != 1:
+        raise ValueError("head_dim must be contiguous")
+    if isinstance(length, int):
+        if not 1 <= length <= cap:
+            raise ValueError("length must be in [1, capacity]")
+        keys, values = keys.narrow(2, 0, length), values.narrow(2, 0, length)
+    return keys, values
+
+
+def _row_ints(t, rows, device, name):
+    """A per-row int32 tensor from a tensor of whole numbers (None stays None)."""
+    if t is None or isinstance(t, int):
+        return None
+    if not isinstance(t, torch.Tensor) or t.dtype not in (torch.int32, torch.int64) or t.numel() != rows:
+        raise ValueError(f"{name} must be an int32 or int64 tensor with one value per row")
+    if t.dtype == torch.int32 and t.device == device and t.is_contiguous():
+        return t
+    return t.reshape(-1).to(device=device, dtype=torch.int32).contiguous()
+
+
+def window_attention(q, keys, values, lengths=None, *, starts=None, window=0, sinks=0, scale=None, weights=None,
+                     out=None, status=None):
+    """Attention over one layer of the decoder's cache with a sliding window and a few
+    first tokens that stay visible (sv_window_attention).
+
+    q: [rows, tokens, heads, head_dim], or [rows, heads, head_dim] for one token;
+    keys / values: [rows, kv_heads, capacity, head_dim], or [rows, capacity,
+    head_dim] (MQA), same strides, q's dtype (float32, float16, bfloat16).  The
+    queries are the last `tokens` of each row's `lengths` slots (int32 [rows] on the
+    device, one number, or None for all).  A query at position p sees slot j iff
+    j <= p, j >= the row's `starts` (padding in front; None: 0), and, with a window,
+    j > p - window or j < start + sinks; a query that sees nothing gives zeros.
+    `scale` defaults to head_dim ** -0.5.  `weights` (float32 [rows, kv_heads,
+    capacity], or [rows, capacity]) has each slot's softmax weight added, summed over
+    the head group and the queries: kv_evict's input.  status: int32 [rows], filled
+    with 0 or SV_ST_LENGTH.  Returns the output, q's shape and dtype."""
+    x = _queries(q)
+    k, v = _layer_cache(keys, values, x, lengths)
+    R, dev = x.shape[0], x.device
+    w = weights
+    if w is not None:
+        _need_cuda(w, "weights")
+        w = w.unsqueeze(1) if w.dim() == 2 else w
+        if w.dtype != torch.float32 or w.dim() != 3 or w.shape[:2] != k.shape[:2] or w.shape[2] < k.shape[2] or \
+                w.stride(2) != 1:
+            raise ValueError("weights must be float32 [rows, kv_heads, capacity], contiguous along the slots")
+    if window < 0 or sinks < 0:
+        raise ValueError("window and sinks must not be negative")
+    rc, o = _ext().window_attention(x, k, v, _row_ints(lengths, R, dev, "lengths"),
+                                    _row_ints(starts, R, dev, "starts"), window, sinks,
+                                    x.shape[3] ** -0.5 if scale is None else float(scale), w, out, status)
+    L.check(rc, "sv_window_attention")
+    return o.view(q.shape) if out is None else out
+
+
+def prefix_attention(q, prefix_keys, prefix_values, keys, values, lengths=None, *, prefix_length=None, scale=None,
+                     out=None, status=None):
+    """Attention of rows that share a long prefix (sv_prefix_attention): every query
+    sees the whole prefix and, of its own row's cache, the slots up to its own.  The
+    prefix is read once for all rows.
+
+    prefix_keys / prefix_values: [kv_heads, prefix, head_dim], or [prefix, head_dim]
+    (MQA), of which the first `prefix_length` slots count (None: all); the rest as
+    window_attention, `lengths` counting the rows' own slots."""
+    x = _queries(q)
+    k, v = _layer_cache(keys, values, x, lengths)
+    _need_cuda(prefix_keys, "prefix_keys")
+    pk, pv = prefix_keys, prefix_values
+    if pk.dim() == 2:
+        pk, pv = pk.unsqueeze(0), pv.unsqueeze(0)
+    if pk.dim() != 3 or pv.shape != pk.shape or pv.stride() != pk.stride() or pk.dtype != x.dtype or \
+            pv.dtype != x.dtype or pk.shape[0] != k.shape[1] or pk.shape[2] != x.shape[3] or \
+            (pk.shape[2] > 1 and pk.stride(2) != 1):
+        raise ValueError("prefix_keys and prefix_values must be [kv_heads, prefix, head_dim] of q's dtype with the "
+                         "same strides")
+    if prefix_length is not None:
+        if not 0 <= prefix_length <= pk.shape[1]:
+            raise ValueError("prefix_length must be in [0, the prefix's slots]")
+        pk, pv = pk.narrow(1, 0, prefix_length), pv.narrow(1, 0, prefix_length)
+    rc, o = _ext().prefix_attention(x, pk, pv, k, v, _row_ints(lengths, x.shape[0], x.device, "lengths"),
+                                    x.shape[3] ** -0.5 if scale is None else float(scale), out, status)
+    L.check(rc, "sv_prefix_attention")
+    return o.view(q.shape) if out is None else out
+
+
+def kv_evict(keys, values, weights, positions, lengths=None, budget=None, *, sinks=0, recent=0, out=None,
+             status=None):
+    """Evicts slots of the KV cache by accumulated attention weight, in place
+    (sv_kv_evict): every (layer, row, head) with more than `budget` slots keeps the
+    tokens at positions < sinks, the `recent` newest and then the heaviest (ties to
+    the lowest slot); kept slots at budget and past it move into the freed ones.
+
+    keys / values: [layers, rows, capacity, head_dim] (MQA) or [layers, rows, heads,
+    capacity, head_dim]; weights float32 and positions int32 of that shape without
+    head_dim, contiguous; lengths: int32 [rows] on the device, one number or None
+    (all slots).  Returns a dict of new tensors (or fills `out`): lengths, weights
+    and positions after the eviction; the slots' order is not the tokens' order any
+    more, so attend to such a cache without a window."""
+    _need_cuda(keys, "keys")
+    k, v = keys, values
+    if k.dim() == 4:
+        k = k.unsqueeze(2)
+        v = None if v is None else v.unsqueeze(2)
+    if k.dim() != 5:
+        raise ValueError("keys must be [layers, rows, capacity, head_dim] or [layers, rows, heads, capacity, "
+                         "head_dim]")
+    if k.shape[4] > 1 and k.stride(4) != 1:
+        raise ValueError("head_dim must be contiguous")
+    if v is not None and (v.shape != k.shape or v.stride() != k.stride() or v.dtype != k.dtype):
+        raise ValueError("values must have the keys' shape, strides and dtype")
+    if weights.dtype != torch.float32 or positions.dtype != torch.int32 or weights.shape != keys.shape[:-1] or \
+            positions.shape != keys.shape[:-1]:
+        raise ValueError("weights (float32) and positions (int32) must have the keys' shape without head_dim")
+    R, cap = k.shape[1], k.shape[3]
+    if budget is None or not 1 <= budget <= cap:
+        raise ValueError("budget must be in [1, capacity]")
+    if sinks < 0 or recent < 0 or sinks + recent > budget:
+        raise ValueError("sinks and recent must not be negative and must fit in the budget")
+    if isinstance(lengths, int):
+        if not 0 <= lengths <= cap:
+            raise ValueError("lengths must be in [0, capacity]")
+        lengths = torch.full((R,), lengths, dtype=torch.int32, device=k.device)
+    o = out if out is not None else {}
+    rc, o["lengths"], o["weights"], o["positions"] = _ext().kv_evict(
+        k, v, weights, positions, _row_ints(lengths, R, k.device, "lengths"), budget, sinks, recent, o.get("weights"),
+        o.get("positions"), o.get("lengths"), status)
+    L.check(rc, "sv_kv_evict")
+    return o

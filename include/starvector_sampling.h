@@ -44,6 +44,7 @@ extern "C" {
 #define SV_ST_TIMEOUT 5    /* a bounded wait on an asynchronous copy ran out */
 #define SV_ST_SHARD_OVERFLOW 6 /* sv_merge_shards: a slice's kept list exceeded its capacity */
 #define SV_ST_GUARD_FULL 7     /* sv_loop_guard_incremental: a window did not fit in the table */
+#define SV_ST_LENGTH 8         /* a row's length or start lies outside its cache (it was clamped) */
 
 /* Logit dtypes. */
 #define SV_F32 0
@@ -372,6 +373,102 @@ int sv_beam_advance(const int64_t* picks, const float* pick_scores, const int32_
                     const uint32_t* seen_in, uint32_t* seen_out, int64_t seen_stride_words, const int32_t* hist_in,
                     int32_t* hist_out, int64_t hist_stride, const uint32_t* whash_in, uint32_t* whash_out,
                     unsigned long long* guard_table, int64_t guard_entries, int32_t window, void* stream);
+
+/*
+ * Attention over one layer of the decoder's cache, with a sliding window and a few
+ * first tokens that stay visible (sinks).  No counterpart in the reference (its
+ * decoders call torch).  Row r holds slots [starts[r], lengths[r]); its `tokens`
+ * queries are the last tokens of the row: query i stands at p = lengths[r] - tokens
+ * + i and sees slot j iff
+ *   starts[r] <= j <= p  and  (window == 0  or  j > p - window  or
+ *                              j < starts[r] + sinks),
+ * out = sum_j softmax_j(scale q.k_j) v_j over the slots it sees, 0 if it sees none
+ * (queries before their row's start).  The slots' order carries no meaning with
+ * window 0.  What lies in slots that no query of the row sees is never used, NaN
+ * and infinities included.
+ *   q      [rows, tokens, heads, head_dim] of dtype (SV_F32 / SV_F16 / SV_BF16),
+ *          strides in elements, head_dim contiguous; head h reads key/value head
+ *          h / (heads / kv_heads)
+ *   keys, values  element (row, head, slot, d) at row * kv_stride_row + head *
+ *          kv_stride_head + slot * kv_stride_slot + d, both alike (one layer of the
+ *          layouts of sv_kv_reorder; MQA: kv_heads = 1)
+ *   lengths, starts  int32 [rows] or NULL (= capacity, = 0); values outside
+ *          [0, capacity] / [0, length] are clamped and reported as SV_ST_LENGTH
+ *   weights  optional float [rows, kv_heads, capacity] at the given strides: each
+ *          slot's softmax weight, summed over the head's group and the queries, is
+ *          added (sv_kv_evict's input)
+ *   out    [rows, tokens, heads, head_dim] contiguous, of dtype
+ *   workspace  sv_window_attention_workspace_bytes(...) bytes, 16-byte aligned,
+ *          zero-filled before its first use; calls that overlap on the GPU need
+ *          different ones
+ * Scores, softmax and sums are f32; the 16-bit kernels round the weights to the
+ * inputs' type before they multiply the values.  head_dim a multiple of 8, 8..128;
+ * heads a multiple of kv_heads; rows * kv_heads <= 65535; rows * tokens * heads <=
+ * 2^30; pointers and every stride in bytes multiples of 16.
+ *   out_status  int32 [rows] or NULL
+ */
+size_t sv_window_attention_workspace_bytes(int32_t dtype, int32_t rows, int32_t tokens, int32_t heads,
+                                           int32_t kv_heads, int32_t head_dim, int32_t capacity, int32_t window,
+                                           int32_t sinks, int32_t with_weights);
+int sv_window_attention(const void* q, int32_t dtype, int32_t rows, int32_t tokens, int32_t heads, int32_t kv_heads,
+                        int32_t head_dim, int64_t q_stride_row, int64_t q_stride_token, int64_t q_stride_head,
+                        const void* keys, const void* values, int32_t capacity, int64_t kv_stride_row,
+                        int64_t kv_stride_head, int64_t kv_stride_slot, const int32_t* lengths, const int32_t* starts,
+                        int32_t window, int32_t sinks, double scale, float* weights, int64_t weights_stride_row,
+                        int64_t weights_stride_head, void* out, void* workspace, size_t workspace_bytes,
+                        int32_t* out_status, void* stream);
+
+/*
+ * Attention of rows that share a prefix (the beams of one prompt, a batch behind one
+ * system prompt): every query sees the prefix's prefix_length slots and, of its own
+ * row's cache, slot j iff j <= p (p = lengths[r] - tokens + i, lengths counting the
+ * row's own slots, the queries' included).  One softmax over both.  The prefix is
+ * read once per key/value head for all rows, not once per row.  No counterpart in
+ * the reference.
+ *   prefix_keys, prefix_values  element (head, slot, d) at head * prefix_stride_head
+ *          + slot * prefix_stride_slot + d; prefix_length 0: none (pointers unused)
+ * The rest as sv_window_attention.
+ */
+size_t sv_prefix_attention_workspace_bytes(int32_t dtype, int32_t rows, int32_t tokens, int32_t heads,
+                                           int32_t kv_heads, int32_t head_dim, int32_t prefix_length,
+                                           int32_t capacity);
+int sv_prefix_attention(const void* q, int32_t dtype, int32_t rows, int32_t tokens, int32_t heads, int32_t kv_heads,
+                        int32_t head_dim, int64_t q_stride_row, int64_t q_stride_token, int64_t q_stride_head,
+                        const void* prefix_keys, const void* prefix_values, int32_t prefix_length,
+                        int64_t prefix_stride_head, int64_t prefix_stride_slot, const void* keys, const void* values,
+                        int32_t capacity, int64_t kv_stride_row, int64_t kv_stride_head, int64_t kv_stride_slot,
+                        const int32_t* lengths, double scale, void* out, void* workspace, size_t workspace_bytes,
+                        int32_t* out_status, void* stream);
+
+/*
+ * Eviction from the cache by accumulated attention weight, in place.  No counterpart
+ * in the reference.  Each (layer, row, head) with n = lengths[row] valid slots and
+ * n > budget keeps `budget` of them: the slots of position < sinks and those of
+ * position > newest - recent (newest: the unit's largest position), then the
+ * heaviest; equal weights keep the lowest slots, NaN counts as the least, and should
+ * positions repeat so that too many are protected, protected slots count as weight
+ * +inf.  The survivors at slots >= budget, in slot order, move into the evicted
+ * slots below budget, in slot order; nothing else moves, so slots are not in token
+ * order afterwards (positions say which token a slot holds).  Slots >= budget keep
+ * what they held.  A unit of n <= budget slots stays as it is.
+ *   keys, values  as in sv_kv_reorder (values may be NULL), element (layer, row, head,
+ *          slot, d); elem_bytes 1, 2 or 4
+ *   weights, positions  float / int32 [layers, rows, heads, capacity], contiguous;
+ *          not changed
+ *   lengths  int32 [rows] or NULL (= capacity)
+ *   weights_out, positions_out  the same shape, other buffers: the kept slots' values
+ *          in their new places, 0 / -1 in every slot past them
+ *   lengths_out  int32 [rows] or NULL: min(length, budget)
+ *   out_status   int32 [rows] or NULL: SV_ST_LENGTH for a length outside [0, capacity]
+ * 1 <= budget <= capacity <= 2^20; sinks + recent <= budget; layers * rows * heads <=
+ * 65535; head_dim * elem_bytes, the strides in bytes and the cache pointers multiples
+ * of 16.
+ */
+int sv_kv_evict(void* keys, void* values, int32_t elem_bytes, int32_t layers, int32_t rows, int32_t heads,
+                int32_t capacity, int32_t head_dim, int64_t stride_layer, int64_t stride_row, int64_t stride_head,
+                int64_t stride_slot, const float* weights, const int32_t* positions, const int32_t* lengths,
+                int32_t budget, int32_t sinks, int32_t recent, float* weights_out, int32_t* positions_out,
+                int32_t* lengths_out, int32_t* out_status, void* stream);
 
 /* Text of a return or status code. */
 const char* sv_error_string(int32_t code);
