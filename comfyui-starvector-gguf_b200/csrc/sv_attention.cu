@@ -30,27 +30,44 @@ int choose_splits(int64_t blocks, int64_t slots) {
   return (int)(s < 1 ? 1 : s);
 }
 
+// The token kernel (16-bit types, at most 16 query rows per key/value head) or the
+// tile kernels.
+bool by_token(const AttnArgs& a) { return a.dtype != SV_F32 && (int64_t)a.n * a.group <= kTokenRows; }
+
 struct Plan {
+  bool token;
   int p_splits, o_splits;
-  size_t o_bytes, ml_bytes, lse_bytes;
-  size_t total() const { return o_bytes + ml_bytes + lse_bytes; }
+  size_t counters, o_bytes, ml_bytes, po_bytes, pml_bytes, lse_bytes, score_bytes;
+  size_t total() const { return counters + o_bytes + ml_bytes + po_bytes + pml_bytes + lse_bytes + score_bytes; }
 };
 
 Plan make_plan(const AttnArgs& a) {
   Plan p = {};
   const int64_t nG = (int64_t)a.n * a.group, all = a.rows * a.kv_heads * nG;
   const int64_t bm = nG <= 16 ? 16 : 64;
-  const int64_t blocks = a.rows * a.kv_heads * div_up(nG, bm);
-  p.o_splits = choose_splits(blocks, most_slots(a.capacity, a.window, a.sinks, div_up(bm, a.group)));
+  const int64_t units = (int64_t)a.rows * a.kv_heads;
+  // One size whatever the shape: a workspace may serve calls of other shapes in turn,
+  // and their partial results must not reach what this call counts in.
+  p.counters = SV_ATTENTION_ZERO_BYTES;
+  p.token = by_token(a);
   if (a.prefix) {
     const int64_t m = a.rows * nG, pb = a.kv_heads * div_up(m, m <= 16 ? 16 : 64);
     p.p_splits = choose_splits(pb, a.prefix);
-  } else if (p.o_splits == 1) {
-    p.o_splits = 0;
+    if (p.token && p.p_splits > 16) p.p_splits = 16;
+    p.po_bytes = up256(p.p_splits * all * a.dim * 4);
+    p.pml_bytes = up256(p.p_splits * all * 8);
   }
-  const int64_t slots = p.p_splits + p.o_splits;
-  p.o_bytes = up256(slots * all * a.dim * 4);
-  p.ml_bytes = up256(slots * all * 8);
+  if (p.token) {
+    p.o_bytes = up256((size_t)2 * kTokenBlocks * 16 * a.dim * 4);
+    p.ml_bytes = up256((size_t)2 * kTokenBlocks * 16 * 8);
+    p.score_bytes = a.weights ? up256(all * a.capacity * 4) : 0;
+  } else {
+    p.o_splits = choose_splits(units * div_up(nG, bm),
+                               most_slots(a.capacity, a.window, a.sinks, div_up(bm, a.group)));
+    if (!a.prefix && p.o_splits == 1) p.o_splits = 0;
+    p.o_bytes = up256(p.o_splits * all * a.dim * 4);
+    p.ml_bytes = up256(p.o_splits * all * 8);
+  }
   p.lse_bytes = a.weights ? up256(all * 4) : 0;
   return p;
 }
@@ -86,12 +103,26 @@ int run(AttnArgs& a, void* workspace, size_t workspace_bytes, cudaStream_t strea
   if (p.total() && (!workspace || workspace_bytes < p.total())) return SV_E_WORKSPACE;
   if (reinterpret_cast<uintptr_t>(workspace) % 16) return SV_E_ALIGN;
   unsigned char* w = static_cast<unsigned char*>(workspace);
+  auto take = [&](size_t bytes) {
+    unsigned char* at = w;
+    w += bytes;
+    return bytes ? at : nullptr;
+  };
   a.p_splits = p.p_splits;
   a.o_splits = p.o_splits;
-  a.part_o = reinterpret_cast<float*>(w);
-  a.part_ml = reinterpret_cast<float2*>(w + p.o_bytes);
-  a.lse = a.weights ? reinterpret_cast<float*>(w + p.o_bytes + p.ml_bytes) : nullptr;
+  a.counters = reinterpret_cast<unsigned*>(take(p.counters));
+  a.part_o = reinterpret_cast<float*>(take(p.o_bytes));
+  a.part_ml = reinterpret_cast<float2*>(take(p.ml_bytes));
+  a.prefix_o = reinterpret_cast<float*>(take(p.po_bytes));
+  a.prefix_ml = reinterpret_cast<float2*>(take(p.pml_bytes));
+  a.lse = reinterpret_cast<float*>(take(p.lse_bytes));
+  a.scores = reinterpret_cast<float*>(take(p.score_bytes));
   if (a.prefix && launch_attn_simt(a, true, stream) != cudaSuccess) return SV_E_CUDA;
+  if (p.token) {
+    if (launch_attn_token(a, kTokenBlocks, stream) != cudaSuccess) return SV_E_CUDA;
+    if (a.weights && launch_scores_weights(a, stream) != cudaSuccess) return SV_E_CUDA;
+    return SV_OK;
+  }
   if (launch_attn_simt(a, false, stream) != cudaSuccess) return SV_E_CUDA;
   if (p.o_splits && launch_attn_combine(a, stream) != cudaSuccess) return SV_E_CUDA;
   if (a.weights && launch_attn_weights(a, stream) != cudaSuccess) return SV_E_CUDA;

@@ -17,6 +17,8 @@
 namespace sv {
 
 constexpr int kAttnMaxDim = 128;
+constexpr int kTokenRows = 16;     // query rows per key/value head of the token kernel
+constexpr int kTokenBlocks = 148;  // its blocks: one per SM
 
 struct AttnArgs {
   const void* q;
@@ -35,10 +37,14 @@ struct AttnArgs {
   void* out;  // [rows, n, heads, dim]
   int32_t* status;
   // workspace
-  float* part_o;   // [slots][idx][dim]
-  float2* part_ml; // [slots][idx]
-  float* lse;      // [idx], with weights only: log2 of the softmax denominator, maximum included
-  int32_t p_splits, o_splits;  // workspace slots of the prefix and of the own part (0 own: written directly)
+  unsigned* counters;  // zero between calls: [rows * kv_heads], then two per block of the token kernel
+  float* part_o;       // own part: [o_splits][idx][dim], or of the token kernel [2 * blocks][16][dim]
+  float2* part_ml;     // the same without dim
+  float* prefix_o;     // prefix part: [p_splits][idx][dim]
+  float2* prefix_ml;
+  float* lse;          // [idx], with weights only: log2 of the softmax denominator, maximum included
+  float* scores;       // [idx][capacity], with weights in the token kernel only
+  int32_t p_splits, o_splits;  // o_splits 0: the own part is written directly
 };
 
 // The slots that row r's queries can see: queries stand at p = end - n + i, slots
@@ -101,6 +107,8 @@ __device__ __forceinline__ void load8(const __nv_bfloat16* p, float* x) {
 }
 
 cudaError_t launch_attn_simt(const AttnArgs& a, bool prefix, cudaStream_t stream);
+cudaError_t launch_attn_token(const AttnArgs& a, int blocks, cudaStream_t stream);
+cudaError_t launch_scores_weights(const AttnArgs& a, cudaStream_t stream);
 cudaError_t launch_attn_combine(const AttnArgs& a, cudaStream_t stream);
 cudaError_t launch_attn_weights(const AttnArgs& a, cudaStream_t stream);
 

@@ -197,14 +197,14 @@ __global__ void __launch_bounds__(NT) attn_simt_kernel(const AttnArgs a, const b
       }
       if (a.lse && tx == 0) a.lse[idx] = l[r] == 0.f ? INFINITY : m[r] + log2f(l[r]);
     } else {
-      const int64_t at = (int64_t)(prefix ? split : a.p_splits + split) * all + idx;
-      float* out = a.part_o + at * a.dim;
+      const int64_t at = (int64_t)split * all + idx;
+      float* out = (prefix ? a.prefix_o : a.part_o) + at * a.dim;
 #pragma unroll
       for (int c = 0; c < 8; ++c) {
         const int d = (c >> 2) * 64 + tx * 4 + (c & 3);
         if (d < a.dim) out[d] = o[r][c];
       }
-      if (tx == 0) a.part_ml[at] = make_float2(m[r], l[r]);
+      if (tx == 0) (prefix ? a.prefix_ml : a.part_ml)[at] = make_float2(m[r], l[r]);
     }
   }
   if (a.status && !prefix && threadIdx.x == 0 && blockIdx.x == 0 && h == 0) {
@@ -278,19 +278,24 @@ __global__ void __launch_bounds__(NT) attn_combine_kernel(const AttnArgs a) {
   if (idx >= all) return;
   const int lane = threadIdx.x & 31, d = lane * 4;
   float mx = -INFINITY;
-  for (int s = lane; s < S; s += 32) mx = fmaxf(mx, a.part_ml[s * all + idx].x);
+  auto ml_of = [&](int s) {
+    return s < a.p_splits ? a.prefix_ml[s * all + idx] : a.part_ml[(s - a.p_splits) * all + idx];
+  };
+  for (int s = lane; s < S; s += 32) mx = fmaxf(mx, ml_of(s).x);
 #pragma unroll
   for (int k = 1; k < 32; k <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, k));
   const float ref = mx == -INFINITY ? 0.f : mx;
   float l = 0.f;
   float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
   for (int s = 0; s < S; ++s) {
-    const float2 ml = a.part_ml[s * all + idx];
+    const float2 ml = ml_of(s);
     if (ml.y == 0.f) continue;  // the split saw nothing
     const float f = exp2f(ml.x - ref);
     l = fmaf(ml.y, f, l);
     if (d < a.dim) {
-      const float4 x = *reinterpret_cast<const float4*>(a.part_o + (s * all + idx) * a.dim + d);
+      const float* part = s < a.p_splits ? a.prefix_o + (s * all + idx) * a.dim
+                                         : a.part_o + ((s - a.p_splits) * all + idx) * a.dim;
+      const float4 x = *reinterpret_cast<const float4*>(part + d);
       o.x = fmaf(x.x, f, o.x);
       o.y = fmaf(x.y, f, o.y);
       o.z = fmaf(x.z, f, o.z);

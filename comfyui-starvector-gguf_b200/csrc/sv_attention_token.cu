@@ -1,0 +1,617 @@
+// sv_attention_token.cu -- attention of few query rows per key/value head over the
+// cache (single tokens, short drafts): at most 16 rows (query, head of the group),
+// float16 / bfloat16, one pass over the slots at memory speed.
+//
+// Mathematics.  Row m of a unit (cache row r, key/value head h): s_j = (q_m . k_j) *
+// scale * log2 e, o = sum_j 2^(s_j - ref) v_j, l = sum_j 2^(s_j - ref), joined over
+// slices of the slots by their references.  ref follows the running maximum only when
+// a score exceeds it by more than 2^8: the weights stay below 2^8 (exact in f32, in
+// range of float16), and most tiles need no maximum exchange and no rescaling.
+//
+// What bounds it: the bytes of the keys and values.  A warp takes 16 slots at a time
+// straight from global memory into the fragments of mma.m16n8k16, without shared
+// memory:
+//   * scores = Q K^T: the sum over dimensions may run in any order, so a thread's
+//     16-byte vector of a key (8 consecutive dimensions) serves as the B operand of
+//     two products whose A operand takes the queries' vectors in the same order;
+//   * output = P V: the thread that holds slots 2t, 2t+1, 2t+8, 2t+9 of the score
+//     fragment loads those four slots' vectors of 8 dimensions and interleaves them in
+//     pairs (byte permutes); which output column a dimension takes is free, so a
+//     thread ends with 16 consecutive dimensions of its two rows.
+// The next tile's keys are fetched as soon as the scores are formed, the next values
+// after the product, so a warp keeps 4 to 8 KB in flight.
+//
+// Work split: the tiles of all units form one list, in unit order, cut into equal
+// parts, one per block; ragged lengths balance by themselves.  A unit that spans
+// several blocks leaves partial results, which the last block to arrive joins, in
+// block order (so results repeat bit for bit); past 32 parts in two levels, so that no
+// block joins more than a few dozen.  The sums' counters return to zero.
+#include "sv_attention.h"
+
+namespace sv {
+namespace {
+
+constexpr int NW = 8, NT = NW * 32;
+constexpr int TK = 16;         // slots per tile
+constexpr int kJoin = 16;      // parts per first-level group
+constexpr int kMaxFlat = 32;   // parts joined in one level
+constexpr float kSlack = 8.f;  // log2 by which a score may exceed its reference
+
+template <typename T> struct Mma;
+template <> struct Mma<__half> {
+  __device__ static void run(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                             uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+                 "{%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  }
+  __device__ static uint32_t pack(float lo, float hi) {
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+  __device__ static uint32_t not_finite(uint32_t w) {
+    return (w & 0x7c00u) == 0x7c00u || (w & 0x7c000000u) == 0x7c000000u;
+  }
+  // The two values of a word, zeros for those that are not finite.
+  __device__ static uint32_t finite(uint32_t w) {
+    return ((w & 0x7c00u) == 0x7c00u ? 0u : w & 0xffffu) | ((w & 0x7c000000u) == 0x7c000000u ? 0u : w & 0xffff0000u);
+  }
+};
+template <> struct Mma<__nv_bfloat16> {
+  __device__ static void run(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                             uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+                 "{%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  }
+  __device__ static uint32_t pack(float lo, float hi) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+  __device__ static uint32_t not_finite(uint32_t w) {
+    return (w & 0x7f80u) == 0x7f80u || (w & 0x7f800000u) == 0x7f800000u;
+  }
+  // The two values of a word, zeros for those that are not finite.
+  __device__ static uint32_t finite(uint32_t w) {
+    return ((w & 0x7f80u) == 0x7f80u ? 0u : w & 0xffffu) | ((w & 0x7f800000u) == 0x7f800000u ? 0u : w & 0xffff0000u);
+  }
+};
+
+__device__ __forceinline__ uint4 load_stream(const void* p, bool ok) {
+  uint4 v = make_uint4(0u, 0u, 0u, 0u);
+  if (ok)
+    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                 : "l"(p));
+  return v;
+}
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// What one row's tiles are: [a0, a1) the sinks before the window, [b0, b1) the rest.
+struct RowTiles {
+  int start, end, a0, a1, b0, b1, ta, tiles;
+};
+
+__device__ __forceinline__ RowTiles row_tiles(const AttnArgs& a, int r) {
+  RowTiles t;
+  const RowSpan sp = row_span(a, r);
+  t.start = sp.start;
+  t.end = sp.end;
+  t.b0 = window_low(a, sp.start, sp.end - a.n);
+  t.b1 = max(sp.end, t.b0);
+  t.a0 = sp.start;
+  t.a1 = max(t.a0, min(sp.start + a.sinks, min(t.b0, t.b1)));
+  t.ta = (t.a1 - t.a0 + TK - 1) / TK;
+  t.tiles = max(1, t.ta + (t.b1 - t.b0 + TK - 1) / TK);  // an empty row is a tile of nothing
+  return t;
+}
+
+// MULTI: more than one query per row (then a tile may be visible to some of them only).
+template <typename T, int DC, bool FULL, bool MULTI>
+__global__ void __launch_bounds__(NT, 1) attn_token_kernel(const __grid_constant__ AttnArgs a, const int blocks_max) {
+  constexpr int OS = DC * 64 + 4;  // row stride of the warps' outputs in shared memory
+  extern __shared__ float dyn[];   // [NW][16][OS]
+  __shared__ float2 warp_ml[NW][16];
+  __shared__ float factor[kMaxFlat * 2][16];
+  __shared__ float2 joined[16];
+  __shared__ int64_t scan[NW + 1];
+  __shared__ int sh_row, sh_last;
+  __shared__ int64_t sh_before;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
+  const int nG = a.n * a.group, K = a.kv_heads, D = a.dim, vecs = D >> 3;
+
+  // Tiles of all rows (every head of a row has as many).
+  const bool uniform = !a.lengths && !a.starts;
+  int64_t total;
+  if (uniform) {
+    total = (int64_t)row_tiles(a, 0).tiles * a.rows;
+  } else {
+    int64_t mine = 0;
+    for (int r = tid; r < a.rows; r += NT) mine += row_tiles(a, r).tiles;
+#pragma unroll
+    for (int k = 16; k; k >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, k);
+    if (lane == 0) scan[warp] = mine;
+    __syncthreads();
+    total = 0;
+#pragma unroll
+    for (int k = 0; k < NW; ++k) total += scan[k];
+    __syncthreads();
+  }
+  const int64_t W = total * K;
+  // Blocks in use: at least one tile per warp each.
+  const int64_t N = min((int64_t)blocks_max, (W + NW - 1) / NW);
+  const int c = blockIdx.x;
+  if (c >= N) return;
+  auto first_tile = [&](int64_t b) { return b * W / N; };
+  auto block_of = [&](int64_t tile) {
+    int64_t b = tile * N / W;
+    while (b + 1 < N && first_tile(b + 1) <= tile) ++b;
+    while (first_tile(b) > tile) --b;
+    return (int)b;
+  };
+  const int64_t t0 = first_tile(c), t1 = first_tile(c + 1);
+  // The row that holds tile t0, and the tiles (of one head) before it.
+  int r;
+  int64_t before;
+  if (uniform) {
+    const int64_t per = row_tiles(a, 0).tiles;
+    r = (int)(t0 / (per * K));
+    before = per * r;
+  } else {
+    int64_t base = 0;
+    for (int r0 = 0;; r0 += NT) {
+      const int rr = r0 + tid;
+      const int64_t n = rr < a.rows ? row_tiles(a, rr).tiles : 0;
+      int64_t s = n;
+#pragma unroll
+      for (int k = 1; k < 32; k <<= 1) {
+        const int64_t x = __shfl_up_sync(0xffffffffu, s, k);
+        if (lane >= k) s += x;
+      }
+      if (lane == 31) scan[warp] = s;
+      if (tid == 0) sh_row = -1;
+      __syncthreads();
+      int64_t off = base, all = 0;
+      for (int k = 0; k < NW; ++k) {
+        if (k < warp) off += scan[k];
+        all += scan[k];
+      }
+      const int64_t lo = off + s - n;
+      if (lo * K <= t0 && t0 < (lo + n) * K) {
+        sh_row = rr;
+        sh_before = lo;
+      }
+      __syncthreads();
+      if (sh_row >= 0) break;
+      base += all;
+    }
+    r = sh_row;
+    before = sh_before;
+  }
+
+  RowTiles rt = row_tiles(a, r);
+  int h = (int)((t0 - before * K) / rt.tiles);
+  int64_t cur = t0;
+  const int64_t all_rows = (int64_t)a.rows * K * nG;
+  while (cur < t1) {
+    const int64_t unit_first = before * K + (int64_t)h * rt.tiles;
+    const int seg0 = (int)(cur - unit_first), seg1 = (int)min((int64_t)rt.tiles, t1 - unit_first);
+    const int unit = r * K + h;
+
+    // Queries of rows g and g + 8, vectors t, t + 4, ...
+    uint4 qf[2][2 * DC];
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      const int m = g + 8 * x, i = m / a.group, hd = h * a.group + m - i * a.group;
+      const T* p = static_cast<const T*>(a.q) + r * a.q_row + i * a.q_tok + hd * a.q_head;
+#pragma unroll
+      for (int u = 0; u < 2 * DC; ++u) {
+        const int vec = 4 * u + t;
+        qf[x][u] = m < nG && (FULL || vec < vecs) ? __ldg(reinterpret_cast<const uint4*>(p) + vec)
+                                                  : make_uint4(0u, 0u, 0u, 0u);
+      }
+    }
+    int pos[2], low[2];
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      pos[x] = rt.end - a.n + (g + 8 * x) / a.group;
+      low[x] = window_low(a, rt.start, pos[x]);
+    }
+    const int pos_first = rt.end - a.n, low_last = window_low(a, rt.start, rt.end - 1);
+
+    const T* kb = static_cast<const T*>(a.k) + r * a.kv_row + h * a.kv_head;
+    const T* vb = static_cast<const T*>(a.v) + r * a.kv_row + h * a.kv_head;
+    float o[8 * DC][4];
+#pragma unroll
+    for (int j = 0; j < 8 * DC; ++j)
+#pragma unroll
+      for (int x = 0; x < 4; ++x) o[j][x] = 0.f;
+    float ref[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+    uint4 kf[2][2 * DC], vf[4][DC];
+
+    auto tile_at = [&](int tile, int& j0, int& jend) {
+      const bool in_a = tile < rt.ta;
+      j0 = in_a ? rt.a0 + tile * TK : rt.b0 + (tile - rt.ta) * TK;
+      jend = in_a ? rt.a1 : rt.b1;
+    };
+    auto load_k = [&](int tile) {
+      int j0, jend;
+      tile_at(tile, j0, jend);
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        const int j = j0 + 8 * x + g;
+        const T* p = kb + j * a.kv_slot;
+#pragma unroll
+        for (int u = 0; u < 2 * DC; ++u)
+          kf[x][u] = load_stream(p + (4 * u + t) * 8, tile < seg1 && j < jend && (FULL || 4 * u + t < vecs));
+      }
+    };
+    auto load_v = [&](int tile) {
+      int j0, jend;
+      tile_at(tile, j0, jend);
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        const int j = j0 + 2 * t + (x & 1) + (x >> 1) * 8;
+        const T* p = vb + j * a.kv_slot;
+#pragma unroll
+        for (int u = 0; u < DC; ++u)
+          vf[x][u] = load_stream(p + (8 * u + g) * 8, tile < seg1 && j < jend && (FULL || 8 * u + g < vecs));
+      }
+    };
+    load_k(seg0 + warp);
+    load_v(seg0 + warp);
+    for (int tile = seg0 + warp; tile < seg1; tile += NW) {
+      int j0, jend;
+      tile_at(tile, j0, jend);
+      float s[2][4];
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) s[x][k] = 0.f;
+#pragma unroll
+        for (int u = 0; u < 2 * DC; ++u) {
+          Mma<T>::run(s[x], qf[0][u].x, qf[1][u].x, qf[0][u].y, qf[1][u].y, kf[x][u].x, kf[x][u].y);
+          Mma<T>::run(s[x], qf[0][u].z, qf[1][u].z, qf[0][u].w, qf[1][u].w, kf[x][u].z, kf[x][u].w);
+        }
+      }
+      load_k(tile + NW);
+      const bool whole = j0 + TK <= jend &&
+                         (tile < rt.ta || !MULTI || (j0 >= low_last && j0 + TK - 1 <= pos_first));
+#pragma unroll
+      for (int x = 0; x < 2; ++x)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) s[x][k] *= a.scale;
+      if (!whole) {
+#pragma unroll
+        for (int x = 0; x < 2; ++x)
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const int j = j0 + 8 * x + 2 * t + (k & 1), y = k >> 1;
+            if (j >= jend || !slot_seen(a, rt.start, pos[y], low[y], j)) s[x][k] = -INFINITY;
+          }
+      }
+      if (a.scores) {
+#pragma unroll
+        for (int x = 0; x < 2; ++x)
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const int j = j0 + 8 * x + 2 * t + (k & 1), m = g + 8 * (k >> 1);
+            if (j < jend && m < nG) a.scores[((int64_t)unit * nG + m) * a.capacity + j] = s[x][k];
+          }
+      }
+      float mx[2];
+#pragma unroll
+      for (int y = 0; y < 2; ++y)
+        mx[y] = fmaxf(fmaxf(s[0][2 * y], s[0][2 * y + 1]), fmaxf(s[1][2 * y], s[1][2 * y + 1]));
+      if (__any_sync(0xffffffffu, mx[0] > ref[0] + kSlack || mx[1] > ref[1] + kSlack)) {
+#pragma unroll
+        for (int y = 0; y < 2; ++y) {
+          mx[y] = fmaxf(mx[y], __shfl_xor_sync(0xffffffffu, mx[y], 1));
+          mx[y] = fmaxf(mx[y], __shfl_xor_sync(0xffffffffu, mx[y], 2));
+          const float now = fmaxf(mx[y], ref[y]);
+          const float f = now == ref[y] ? 1.f : ex2(ref[y] - now);
+          ref[y] = now;
+          l[y] *= f;
+#pragma unroll
+          for (int j = 0; j < 8 * DC; ++j) {
+            o[j][2 * y] *= f;
+            o[j][2 * y + 1] *= f;
+          }
+        }
+      }
+      uint32_t p[4];
+#pragma unroll
+      for (int y = 0; y < 2; ++y) {
+        const float at = ref[y] == -INFINITY ? 0.f : ref[y];
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          const float p0 = ex2(s[x][2 * y] - at), p1 = ex2(s[x][2 * y + 1] - at);
+          l[y] += p0 + p1;
+          p[2 * x + y] = Mma<T>::pack(p0, p1);
+          if (MULTI) s[x][2 * y] = p0, s[x][2 * y + 1] = p1;
+        }
+      }
+      if (MULTI && !whole) {
+        // A value that is not finite must not reach the queries that do not see its slot
+        // (0 * NaN): the product takes zeros in such places, and what the queries that see
+        // them get is added here.
+        uint32_t bad = 0;
+#pragma unroll
+        for (int x = 0; x < 4; ++x)
+#pragma unroll
+          for (int u = 0; u < DC; ++u)
+            bad |= Mma<T>::not_finite(vf[x][u].x) | Mma<T>::not_finite(vf[x][u].y) |
+                   Mma<T>::not_finite(vf[x][u].z) | Mma<T>::not_finite(vf[x][u].w);
+        if (__any_sync(0xffffffffu, bad != 0)) {
+          for (int e = 0; e < TK; ++e) {
+            const int from = (lane & 28) | (e >> 1 & 3), j = j0 + e;
+            float w[2];
+#pragma unroll
+            for (int y = 0; y < 2; ++y) {
+              const float lo = e & 1 ? s[0][2 * y + 1] : s[0][2 * y], hi = e & 1 ? s[1][2 * y + 1] : s[1][2 * y];
+              w[y] = __shfl_sync(0xffffffffu, e < 8 ? lo : hi, from);
+            }
+            if (j >= jend) break;
+#pragma unroll
+            for (int u = 0; u < DC; ++u)
+#pragma unroll
+              for (int x = 0; x < 2; ++x) {
+                const int d = 64 * u + 16 * t + 8 * x;
+                float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+                if (FULL || d < D) load8(vb + j * a.kv_slot + d, v);
+#pragma unroll
+                for (int k = 0; k < 8; ++k)
+#pragma unroll
+                  for (int y = 0; y < 2; ++y)
+                    if (w[y] != 0.f && !isfinite(v[k]))
+                      o[8 * u + k][2 * y + x] = fmaf(w[y], v[k], o[8 * u + k][2 * y + x]);
+              }
+          }
+#pragma unroll
+          for (int x = 0; x < 4; ++x)
+#pragma unroll
+            for (int u = 0; u < DC; ++u) {
+              vf[x][u].x = Mma<T>::finite(vf[x][u].x);
+              vf[x][u].y = Mma<T>::finite(vf[x][u].y);
+              vf[x][u].z = Mma<T>::finite(vf[x][u].z);
+              vf[x][u].w = Mma<T>::finite(vf[x][u].w);
+            }
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < DC; ++u) {
+        const uint32_t* v0 = reinterpret_cast<const uint32_t*>(&vf[0][u]);
+        const uint32_t* v1 = reinterpret_cast<const uint32_t*>(&vf[1][u]);
+        const uint32_t* v2 = reinterpret_cast<const uint32_t*>(&vf[2][u]);
+        const uint32_t* v3 = reinterpret_cast<const uint32_t*>(&vf[3][u]);
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          Mma<T>::run(o[8 * u + 2 * w], p[0], p[1], p[2], p[3], __byte_perm(v0[w], v1[w], 0x5410),
+                      __byte_perm(v2[w], v3[w], 0x5410));
+          Mma<T>::run(o[8 * u + 2 * w + 1], p[0], p[1], p[2], p[3], __byte_perm(v0[w], v1[w], 0x7632),
+                      __byte_perm(v2[w], v3[w], 0x7632));
+        }
+      }
+      load_v(tile + NW);
+    }
+
+    // The warps' results into shared memory.
+#pragma unroll
+    for (int y = 0; y < 2; ++y) {
+      l[y] += __shfl_xor_sync(0xffffffffu, l[y], 1);
+      l[y] += __shfl_xor_sync(0xffffffffu, l[y], 2);
+      const int m = g + 8 * y;
+      if (t == 0) warp_ml[warp][m] = make_float2(ref[y], l[y]);
+      float* row = dyn + (warp * 16 + m) * OS;
+#pragma unroll
+      for (int u = 0; u < DC; ++u)
+#pragma unroll
+        for (int x = 0; x < 2; ++x)
+#pragma unroll
+          for (int w = 0; w < 2; ++w) {
+            const int j = 8 * u + 4 * w;
+            *reinterpret_cast<float4*>(row + 64 * u + 16 * t + 8 * x + 4 * w) =
+                make_float4(o[j][2 * y + x], o[j + 1][2 * y + x], o[j + 2][2 * y + x], o[j + 3][2 * y + x]);
+          }
+    }
+    __syncthreads();
+    if (tid < 16) {
+      float M = -INFINITY;
+#pragma unroll
+      for (int k = 0; k < NW; ++k) M = fmaxf(M, warp_ml[k][tid].x);
+      const float at = M == -INFINITY ? 0.f : M;
+      float L = 0.f;
+#pragma unroll
+      for (int k = 0; k < NW; ++k) {
+        const float f = ex2(warp_ml[k][tid].x - at);
+        factor[k][tid] = f;
+        L = fmaf(warp_ml[k][tid].y, f, L);
+      }
+      joined[tid] = make_float2(M, L);
+    }
+    __syncthreads();
+
+    const int c_first = block_of(unit_first), parts = block_of(unit_first + rt.tiles - 1) - c_first + 1;
+    const bool direct = parts == 1 && !a.prefix;
+    const int row_vecs = D >> 2;
+    auto write_out = [&](int m, int d, float4 x, float L) {
+      const float inv = L == 0.f ? 0.f : 1.f / L;
+      const int i = m / a.group;
+      T* out = static_cast<T*>(a.out) + (((int64_t)r * a.n + i) * a.heads + h * a.group + m - i * a.group) * D + d;
+      *reinterpret_cast<uint2*>(out) =
+          make_uint2(Mma<T>::pack(x.x * inv, x.y * inv), Mma<T>::pack(x.z * inv, x.w * inv));
+    };
+    const int slot = 2 * c + (seg0 == 0);
+    for (int x = tid; x < nG * row_vecs; x += NT) {
+      const int m = x / row_vecs, d = (x - m * row_vecs) * 4;
+      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int k = 0; k < NW; ++k) {
+        const float4 y = *reinterpret_cast<const float4*>(dyn + (k * 16 + m) * OS + d);
+        const float f = factor[k][m];
+        v.x = fmaf(y.x, f, v.x);
+        v.y = fmaf(y.y, f, v.y);
+        v.z = fmaf(y.z, f, v.z);
+        v.w = fmaf(y.w, f, v.w);
+      }
+      if (direct)
+        write_out(m, d, v, joined[m].y);
+      else
+        *reinterpret_cast<float4*>(a.part_o + ((int64_t)slot * 16 + m) * D + d) = v;
+    }
+    if (direct) {
+      if (a.lse && tid < nG) a.lse[(int64_t)unit * nG + tid] = joined[tid].y == 0.f ? INFINITY : joined[tid].x + log2f(joined[tid].y);
+    } else if (tid < nG) {
+      a.part_ml[slot * 16 + tid] = joined[tid];
+    }
+    if (!direct) {
+      // Joins `count` parts of this unit (and, `last`, the prefix's): part k is block b0 + k * step's.
+      auto slot_of = [&](int b) { return 2 * b + (b == c_first); };
+      auto join = [&](int b0, int step, int count, bool last) {
+        const int more = last ? a.p_splits : 0;
+        auto ml_of = [&](int k, int m) -> float2 {
+          return k < count ? __ldcg(a.part_ml + slot_of(b0 + k * step) * 16 + m)
+                           : __ldcg(a.prefix_ml + (int64_t)(k - count) * all_rows + (int64_t)unit * nG + m);
+        };
+        __syncthreads();
+        if (tid < 16 && tid < nG) {
+          float M = -INFINITY;
+          for (int k = 0; k < count + more; ++k) M = fmaxf(M, ml_of(k, tid).x);
+          const float at = M == -INFINITY ? 0.f : M;
+          float L = 0.f;
+          for (int k = 0; k < count + more; ++k) {
+            const float2 ml = ml_of(k, tid);
+            const float f = ml.y == 0.f ? 0.f : ex2(ml.x - at);
+            factor[k][tid] = f;
+            L = fmaf(ml.y, f, L);
+          }
+          joined[tid] = make_float2(M, L);
+        }
+        __syncthreads();
+        for (int x = tid; x < nG * row_vecs; x += NT) {
+          const int m = x / row_vecs, d = (x - m * row_vecs) * 4;
+          float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+          for (int k = 0; k < count + more; ++k) {
+            const float* src = k < count
+                                   ? a.part_o + ((int64_t)slot_of(b0 + k * step) * 16 + m) * D + d
+                                   : a.prefix_o + ((int64_t)(k - count) * all_rows + (int64_t)unit * nG + m) * D + d;
+            const float4 y = __ldcg(reinterpret_cast<const float4*>(src));
+            const float f = factor[k][m];
+            v.x = fmaf(y.x, f, v.x);
+            v.y = fmaf(y.y, f, v.y);
+            v.z = fmaf(y.z, f, v.z);
+            v.w = fmaf(y.w, f, v.w);
+          }
+          if (last)
+            write_out(m, d, v, joined[m].y);
+          else
+            *reinterpret_cast<float4*>(a.part_o + ((int64_t)slot_of(b0) * 16 + m) * D + d) = v;
+        }
+        if (tid < nG) {
+          if (!last)
+            a.part_ml[slot_of(b0) * 16 + tid] = joined[tid];
+          else if (a.lse)
+            a.lse[(int64_t)unit * nG + tid] = joined[tid].y == 0.f ? INFINITY : joined[tid].x + log2f(joined[tid].y);
+        }
+      };
+      // True in the block that arrives last of `count` at a counter, which it clears.
+      auto arrive = [&](unsigned* counter, int count) {
+        __syncthreads();
+        if (tid == 0) {
+          __threadfence();
+          const bool is_last = atomicAdd(counter, 1u) == (unsigned)count - 1u;
+          if (is_last) *counter = 0u;
+          __threadfence();
+          sh_last = is_last;
+        }
+        __syncthreads();
+        return sh_last != 0;
+      };
+      bool go = true;
+      int step = 1, count = parts;
+      if (parts > kMaxFlat) {
+        const int first = (c - c_first) / kJoin * kJoin, n = min(kJoin, parts - first);
+        go = arrive(a.counters + (int64_t)a.rows * K + slot_of(c_first + first), n);
+        if (go) join(c_first + first, 1, n, false);
+        step = kJoin;
+        count = (parts + kJoin - 1) / kJoin;
+      }
+      if (go && parts > 1) go = arrive(a.counters + unit, count);
+      if (go) join(c_first, step, count, true);
+    }
+    __syncthreads();
+    cur = unit_first + seg1;
+    if (seg1 == rt.tiles && ++h == K) {
+      h = 0;
+      if (a.status && tid == 0) {
+        const int e = a.lengths ? a.lengths[r] : a.capacity, s = a.starts ? a.starts[r] : 0;
+        a.status[r] = (e < 0 || e > a.capacity || s < 0 || s > max(e, 0)) ? 8 : 0;
+      }
+      before += rt.tiles;
+      if (++r < a.rows) rt = row_tiles(a, r);
+    }
+  }
+}
+
+// Accumulated weights from the scores that the token kernel left: one thread per slot.
+__global__ void __launch_bounds__(256) scores_weights_kernel(const __grid_constant__ AttnArgs a) {
+  const int unit = blockIdx.y, h = unit % a.kv_heads, r = unit / a.kv_heads;
+  const RowSpan sp = row_span(a, r);
+  const int j = blockIdx.x * 256 + threadIdx.x;
+  if (j >= sp.end || j < sp.start) return;
+  const int nG = a.n * a.group;
+  const float* s = a.scores + (int64_t)unit * nG * a.capacity + j;
+  const float* lse = a.lse + (int64_t)unit * nG;
+  float sum = 0.f;
+  for (int i = 0; i < a.n; ++i) {
+    const int p = sp.end - a.n + i;
+    if (!slot_seen(a, sp.start, p, window_low(a, sp.start, p), j)) continue;
+    for (int g = 0; g < a.group; ++g) {
+      const int m = i * a.group + g;
+      sum += ex2(s[(int64_t)m * a.capacity] - lse[m]);
+    }
+  }
+  a.weights[r * a.w_row + h * a.w_head + j] += sum;
+}
+
+template <typename T, int DC, bool FULL, bool MULTI>
+cudaError_t token(const AttnArgs& a, int blocks, cudaStream_t stream) {
+  constexpr size_t smem = sizeof(float) * NW * 16 * (DC * 64 + 4);
+  const cudaError_t e = cudaFuncSetAttribute(attn_token_kernel<T, DC, FULL, MULTI>,
+                                             cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  if (e != cudaSuccess) return e;
+  attn_token_kernel<T, DC, FULL, MULTI><<<blocks, NT, smem, stream>>>(a, blocks);
+  return cudaGetLastError();
+}
+
+template <typename T, bool MULTI> cudaError_t token_dim(const AttnArgs& a, int blocks, cudaStream_t stream) {
+  if (a.dim == 128) return token<T, 2, true, MULTI>(a, blocks, stream);
+  if (a.dim == 64) return token<T, 1, true, MULTI>(a, blocks, stream);
+  return a.dim < 64 ? token<T, 1, false, MULTI>(a, blocks, stream) : token<T, 2, false, MULTI>(a, blocks, stream);
+}
+
+template <typename T> cudaError_t token_any(const AttnArgs& a, int blocks, cudaStream_t stream) {
+  return a.n > 1 ? token_dim<T, true>(a, blocks, stream) : token_dim<T, false>(a, blocks, stream);
+}
+
+}  // namespace
+
+cudaError_t launch_attn_token(const AttnArgs& a, int blocks, cudaStream_t stream) {
+  return a.dtype == 1 ? token_any<__half>(a, blocks, stream) : token_any<__nv_bfloat16>(a, blocks, stream);
+}
+
+cudaError_t launch_scores_weights(const AttnArgs& a, cudaStream_t stream) {
+  scores_weights_kernel<<<dim3((unsigned)((a.capacity + 255) / 256), (unsigned)(a.rows * a.kv_heads)), 256, 0,
+                          stream>>>(a);
+  return cudaGetLastError();
+}
+
+}  // namespace sv

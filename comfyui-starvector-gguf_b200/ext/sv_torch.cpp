@@ -248,7 +248,7 @@ std::tuple<int, at::Tensor> window_attention(const at::Tensor& q, const at::Tens
   at::Tensor o = attention_out(out, q, dev);
   const size_t bytes = sv_window_attention_workspace_bytes(code, rows, n, heads, kv, dim, capacity, (int32_t)window,
                                                            (int32_t)sinks, weights.has_value());
-  at::Tensor ws = workspace_for(dev, stream, bytes, 4 * (size_t)rows * kv);
+  at::Tensor ws = workspace_for(dev, stream, bytes, 4 * ((size_t)rows * kv + 1024));
   const int rc = sv_window_attention(
       q.data_ptr(), code, rows, n, heads, kv, dim, stride_of(q, 0), stride_of(q, 1), stride_of(q, 2), keys.data_ptr(),
       values.data_ptr(), capacity, stride_of(keys, 0), stride_of(keys, 1), stride_of(keys, 2),
@@ -276,7 +276,7 @@ std::tuple<int, at::Tensor> prefix_attention(const at::Tensor& q, const at::Tens
   const int32_t prefix = (int32_t)prefix_keys.size(1);
   at::Tensor o = attention_out(out, q, dev);
   const size_t bytes = sv_prefix_attention_workspace_bytes(code, rows, n, heads, kv, dim, prefix, capacity);
-  at::Tensor ws = workspace_for(dev, stream, bytes, 4 * (size_t)rows * kv);
+  at::Tensor ws = workspace_for(dev, stream, bytes, 4 * ((size_t)rows * kv + 1024));
   const int rc = sv_prefix_attention(
       q.data_ptr(), code, rows, n, heads, kv, dim, stride_of(q, 0), stride_of(q, 1), stride_of(q, 2),
       prefix_keys.data_ptr(), prefix_values.data_ptr(), prefix, stride_of(prefix_keys, 0), stride_of(prefix_keys, 1),

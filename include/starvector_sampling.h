@@ -374,6 +374,8 @@ int sv_beam_advance(const int64_t* picks, const float* pick_scores, const int32_
                     int32_t* hist_out, int64_t hist_stride, const uint32_t* whash_in, uint32_t* whash_out,
                     unsigned long long* guard_table, int64_t guard_entries, int32_t window, void* stream);
 
+#define SV_ATTENTION_ZERO_BYTES (4 * (65536 + 1024)) /* of an attention workspace: zero before its first use */
+
 /*
  * Attention over one layer of the decoder's cache, with a sliding window and a few
  * first tokens that stay visible (sinks).  No counterpart in the reference (its
@@ -398,9 +400,10 @@ int sv_beam_advance(const int64_t* picks, const float* pick_scores, const int32_
  *          slot's softmax weight, summed over the head's group and the queries, is
  *          added (sv_kv_evict's input)
  *   out    [rows, tokens, heads, head_dim] contiguous, of dtype
- *   workspace  sv_window_attention_workspace_bytes(...) bytes, 16-byte aligned,
- *          zero-filled before its first use; calls that overlap on the GPU need
- *          different ones
+ *   workspace  sv_window_attention_workspace_bytes(...) bytes, 16-byte aligned, of
+ *          which the first SV_ATTENTION_ZERO_BYTES are zero before its first use (each
+ *          call leaves them so; a call itself needs 4 * (rows * kv_heads + 1024) of
+ *          them); calls that overlap on the GPU need different ones
  * Scores, softmax and sums are f32; the 16-bit kernels round the weights to the
  * inputs' type before they multiply the values.  head_dim a multiple of 8, 8..128;
  * heads a multiple of kv_heads; rows * kv_heads <= 65535; rows * tokens * heads <=

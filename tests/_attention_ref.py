@@ -5,15 +5,16 @@ sums in f32, products of the inputs exact or f32):
   * a score is off by at most (D + 8) 2^-24 sum_d |q_d k_d| |scale|, so a softmax
     weight by twice the largest such error, relatively (numerator and denominator);
     exp2 and the sums over the slots add a few 2^-24 each, 2^-20 covers them;
-  * the 16-bit kernels round each weight once to the inputs' type (relative u = 2^-9
-    for bfloat16, 2^-12 for float16; float16 weights below 2^-14 of the largest
-    absolutely, 2^-25) and every kernel rounds the output once (u |o|).
+  * the 16-bit kernels round each weight once to the inputs' type (relative error at
+    most the unit roundoff u = 2^-p for p significant bits: 2^-8 for bfloat16, 2^-11
+    for float16; float16 weights below 2^-14 of the largest absolutely, 2^-25) and every
+    kernel rounds the output once (u |o|).
 With A = sum_j p_j |v_j| the output's error is at most
   u |o| + (u_weight + e) A + a sum_j |v_j|,  e = 2 (D + 8) 2^-24 S + 2^-20.
 """
 import torch
 
-U = {torch.float32: 2.0 ** -24, torch.float16: 2.0 ** -12, torch.bfloat16: 2.0 ** -9}
+U = {torch.float32: 2.0 ** -24, torch.float16: 2.0 ** -11, torch.bfloat16: 2.0 ** -8}
 
 
 def visible(n, lo_slot, end, start, window, sinks, device):
