@@ -9,6 +9,7 @@ namespace sv {
 namespace {
 
 constexpr int kSMs = 148;
+constexpr int kMostPrefixSplits = 16;  // that the token kernel joins
 
 size_t up256(size_t x) { return (x + 255) / 256 * 256; }
 
@@ -21,8 +22,8 @@ int64_t most_slots(int32_t capacity, int32_t window, int32_t sinks, int64_t tile
   return x < capacity ? x : capacity;
 }
 
-// Splits of the slots: enough blocks for every SM twice, at least two 64-slot tiles
-// each.
+// Splits of the slots among blocks of the f32 kernel: enough blocks for every SM
+// twice, at least two 64-slot tiles each.
 int choose_splits(int64_t blocks, int64_t slots) {
   if (blocks >= 2 * kSMs) return 1;
   const int64_t want = (2 * kSMs + blocks - 1) / blocks, most = (slots + 127) / 128;
@@ -30,13 +31,25 @@ int choose_splits(int64_t blocks, int64_t slots) {
   return (int)(s < 1 ? 1 : s);
 }
 
+// Of the tile kernel (one block per SM): one round of blocks at most, at least two
+// 128-slot tiles each.
+int tile_splits(int64_t blocks, int64_t slots) {
+  const int64_t want = kSMs / blocks, most = (slots + 255) / 256;
+  const int64_t s = want < most ? want : most;
+  return (int)(s < 1 ? 1 : s);
+}
+
+// Query tiles per block of the tile kernel: two (their softmax and products overlap)
+// unless blocks of one still fit the SMs.
+int tiles_per_block(int64_t units, int64_t rows_m) { return units * div_up(rows_m, 128) <= kSMs ? 1 : 2; }
+
 // The token kernel (16-bit types, at most 16 query rows per key/value head) or the
 // tile kernels.
 bool by_token(const AttnArgs& a) { return a.dtype != SV_F32 && (int64_t)a.n * a.group <= kTokenRows; }
 
 struct Plan {
   bool token;
-  int p_splits, o_splits;
+  int p_splits, o_splits, p_tiles, o_tiles;
   size_t counters, o_bytes, ml_bytes, po_bytes, pml_bytes, lse_bytes, score_bytes;
   size_t total() const { return counters + o_bytes + ml_bytes + po_bytes + pml_bytes + lse_bytes + score_bytes; }
 };
@@ -44,16 +57,21 @@ struct Plan {
 Plan make_plan(const AttnArgs& a) {
   Plan p = {};
   const int64_t nG = (int64_t)a.n * a.group, all = a.rows * a.kv_heads * nG;
-  const int64_t bm = nG <= 16 ? 16 : 64;
   const int64_t units = (int64_t)a.rows * a.kv_heads;
   // One size whatever the shape: a workspace may serve calls of other shapes in turn,
   // and their partial results must not reach what this call counts in.
   p.counters = SV_ATTENTION_ZERO_BYTES;
   p.token = by_token(a);
+  const bool f32 = a.dtype == SV_F32;
   if (a.prefix) {
-    const int64_t m = a.rows * nG, pb = a.kv_heads * div_up(m, m <= 16 ? 16 : 64);
-    p.p_splits = choose_splits(pb, a.prefix);
-    if (p.token && p.p_splits > 16) p.p_splits = 16;
+    const int64_t m = a.rows * nG;
+    if (f32) {
+      p.p_splits = choose_splits(a.kv_heads * div_up(m, m <= 16 ? 16 : 64), a.prefix);
+    } else {
+      p.p_tiles = tiles_per_block(a.kv_heads, m);
+      p.p_splits = tile_splits(a.kv_heads * div_up(m, 128 * p.p_tiles), a.prefix);
+      if (p.token && p.p_splits > kMostPrefixSplits) p.p_splits = kMostPrefixSplits;
+    }
     p.po_bytes = up256(p.p_splits * all * a.dim * 4);
     p.pml_bytes = up256(p.p_splits * all * 8);
   }
@@ -62,8 +80,10 @@ Plan make_plan(const AttnArgs& a) {
     p.ml_bytes = up256((size_t)2 * kTokenBlocks * 16 * 8);
     p.score_bytes = a.weights ? up256(all * a.capacity * 4) : 0;
   } else {
-    p.o_splits = choose_splits(units * div_up(nG, bm),
-                               most_slots(a.capacity, a.window, a.sinks, div_up(bm, a.group)));
+    p.o_tiles = tiles_per_block(units, nG);
+    const int64_t bm = !f32 ? 128 * p.o_tiles : (nG <= 16 ? 16 : 64), blocks = units * div_up(nG, bm);
+    const int64_t slots = most_slots(a.capacity, a.window, a.sinks, div_up(bm, a.group));
+    p.o_splits = f32 ? choose_splits(blocks, slots) : tile_splits(blocks, slots);
     if (!a.prefix && p.o_splits == 1) p.o_splits = 0;
     p.o_bytes = up256(p.o_splits * all * a.dim * 4);
     p.ml_bytes = up256(p.o_splits * all * 8);
@@ -117,13 +137,17 @@ int run(AttnArgs& a, void* workspace, size_t workspace_bytes, cudaStream_t strea
   a.prefix_ml = reinterpret_cast<float2*>(take(p.pml_bytes));
   a.lse = reinterpret_cast<float*>(take(p.lse_bytes));
   a.scores = reinterpret_cast<float*>(take(p.score_bytes));
-  if (a.prefix && launch_attn_simt(a, true, stream) != cudaSuccess) return SV_E_CUDA;
+  const bool f32 = a.dtype == SV_F32;
+  if (a.prefix &&
+      (f32 ? launch_attn_simt(a, true, stream) : launch_attn_tile(a, true, p.p_tiles, stream)) != cudaSuccess)
+    return SV_E_CUDA;
   if (p.token) {
     if (launch_attn_token(a, kTokenBlocks, stream) != cudaSuccess) return SV_E_CUDA;
     if (a.weights && launch_scores_weights(a, stream) != cudaSuccess) return SV_E_CUDA;
     return SV_OK;
   }
-  if (launch_attn_simt(a, false, stream) != cudaSuccess) return SV_E_CUDA;
+  if ((f32 ? launch_attn_simt(a, false, stream) : launch_attn_tile(a, false, p.o_tiles, stream)) != cudaSuccess)
+    return SV_E_CUDA;
   if (p.o_splits && launch_attn_combine(a, stream) != cudaSuccess) return SV_E_CUDA;
   if (a.weights && launch_attn_weights(a, stream) != cudaSuccess) return SV_E_CUDA;
   return SV_OK;

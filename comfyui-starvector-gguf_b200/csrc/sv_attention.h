@@ -107,6 +107,7 @@ __device__ __forceinline__ void load8(const __nv_bfloat16* p, float* x) {
 }
 
 cudaError_t launch_attn_simt(const AttnArgs& a, bool prefix, cudaStream_t stream);
+cudaError_t launch_attn_tile(const AttnArgs& a, bool prefix, int tiles_m, cudaStream_t stream);
 cudaError_t launch_attn_token(const AttnArgs& a, int blocks, cudaStream_t stream);
 cudaError_t launch_scores_weights(const AttnArgs& a, cudaStream_t stream);
 cudaError_t launch_attn_combine(const AttnArgs& a, cudaStream_t stream);

@@ -345,11 +345,7 @@ template <typename T> cudaError_t weights_any(const AttnArgs& a, cudaStream_t st
 }  // namespace
 
 cudaError_t launch_attn_simt(const AttnArgs& a, bool prefix, cudaStream_t stream) {
-  switch (a.dtype) {
-    case 0: return simt_any<float>(a, prefix, stream);
-    case 1: return simt_any<__half>(a, prefix, stream);
-    default: return simt_any<__nv_bfloat16>(a, prefix, stream);
-  }
+  return simt_any<float>(a, prefix, stream);
 }
 
 cudaError_t launch_attn_combine(const AttnArgs& a, cudaStream_t stream) {
