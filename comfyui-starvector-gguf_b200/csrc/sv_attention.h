@@ -9,6 +9,7 @@
 // output and its (maximum, sum) in the workspace; the maximum is in units of
 // log2 (score * scale * log2 e), so weights are exp2(s - m).
 #pragma once
+#include <atomic>
 #include <cstdint>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -104,6 +105,19 @@ __device__ __forceinline__ void load8(const __nv_bfloat16* p, float* x) {
     x[2 * i] = f.x;
     x[2 * i + 1] = f.y;
   }
+}
+
+// Raises a kernel's shared-memory limit, once per device and process.
+template <auto Kernel> cudaError_t allow_smem(size_t bytes) {
+  static std::atomic<uint64_t> done{0};
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  const uint64_t bit = dev < 64 ? (uint64_t)1 << dev : 0;
+  if (done.load(std::memory_order_relaxed) & bit) return cudaSuccess;
+  e = cudaFuncSetAttribute(Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+  if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_relaxed);
+  return e;
 }
 
 cudaError_t launch_attn_simt(const AttnArgs& a, bool prefix, cudaStream_t stream);

@@ -321,8 +321,7 @@ template <typename T, int BM> cudaError_t simt(const AttnArgs& a, bool prefix, c
   const int64_t S = prefix ? a.p_splits : (a.o_splits ? a.o_splits : 1);
   const dim3 grid((unsigned)((rows_m + BM - 1) / BM * S), (unsigned)(prefix ? a.kv_heads : a.rows * a.kv_heads));
   constexpr size_t smem = simt_smem<BM>();
-  cudaError_t e = cudaFuncSetAttribute(attn_simt_kernel<T, BM>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                       (int)smem);
+  cudaError_t e = allow_smem<attn_simt_kernel<T, BM>>(smem);
   if (e != cudaSuccess) return e;
   attn_simt_kernel<T, BM><<<grid, NT, smem, stream>>>(a, prefix);
   return cudaGetLastError();
@@ -335,7 +334,7 @@ template <typename T> cudaError_t simt_any(const AttnArgs& a, bool prefix, cudaS
 
 template <typename T> cudaError_t weights_any(const AttnArgs& a, cudaStream_t stream) {
   constexpr size_t smem = sizeof(float) * (64 * KS + BN * KS + 16 * BN);
-  cudaError_t e = cudaFuncSetAttribute(attn_weights_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  cudaError_t e = allow_smem<attn_weights_kernel<T>>(smem);
   if (e != cudaSuccess) return e;
   const dim3 grid((unsigned)((a.capacity + BN - 1) / BN), (unsigned)(a.rows * a.kv_heads));
   attn_weights_kernel<T><<<grid, NT, smem, stream>>>(a);

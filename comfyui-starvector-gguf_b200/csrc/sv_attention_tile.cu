@@ -508,8 +508,7 @@ cudaError_t tile(const AttnArgs& a, const Maps& maps, bool prefix, int tiles_m, 
   const int64_t S = prefix ? a.p_splits : (a.o_splits ? a.o_splits : 1);
   const dim3 grid((unsigned)((rows_m + tiles_m * BM - 1) / (tiles_m * BM) * S),
                   (unsigned)(prefix ? a.kv_heads : a.rows * a.kv_heads));
-  const cudaError_t e = cudaFuncSetAttribute(attn_tile_kernel<T, DC>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                             (int)Layout<DC>::kBytes);
+  const cudaError_t e = allow_smem<attn_tile_kernel<T, DC>>(Layout<DC>::kBytes);
   if (e != cudaSuccess) return e;
   attn_tile_kernel<T, DC><<<grid, NT, Layout<DC>::kBytes, stream>>>(a, maps, prefix, tiles_m);
   return cudaGetLastError();

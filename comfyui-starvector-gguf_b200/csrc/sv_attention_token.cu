@@ -99,7 +99,7 @@ struct RowTiles {
   int start, end, a0, a1, b0, b1, ta, tiles;
 };
 
-__device__ __forceinline__ RowTiles row_tiles(const AttnArgs& a, int r) {
+__device__ __noinline__ RowTiles row_tiles(const AttnArgs& a, int r) {
   RowTiles t;
   const RowSpan sp = row_span(a, r);
   t.start = sp.start;
@@ -121,95 +121,68 @@ __global__ void __launch_bounds__(NT, 1) attn_token_kernel(const __grid_constant
   __shared__ float2 warp_ml[NW][16];
   __shared__ float factor[kMaxFlat * 2][16];
   __shared__ float2 joined[16];
-  __shared__ int64_t scan[NW + 1];
-  __shared__ int sh_row, sh_last;
-  __shared__ int64_t sh_before;
+  __shared__ int scan[NW];
+  __shared__ int sh_row, sh_before, sh_last;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
-  const int nG = a.n * a.group, K = a.kv_heads, D = a.dim, vecs = D >> 3;
+  const int group = a.group, nG = MULTI ? a.n * group : group, K = a.kv_heads, D = FULL ? 64 * DC : a.dim;
+  const int vecs = D >> 3;
 
-  // Tiles of all rows (every head of a row has as many).
-  const bool uniform = !a.lengths && !a.starts;
-  int64_t total;
-  if (uniform) {
-    total = (int64_t)row_tiles(a, 0).tiles * a.rows;
-  } else {
-    int64_t mine = 0;
-    for (int r = tid; r < a.rows; r += NT) mine += row_tiles(a, r).tiles;
+  // Tiles of all rows (every head of a row has as many): thread x counts rows
+  // [x per, (x + 1) per), a scan gives the total and what lies before each thread.
+  const int per = (a.rows + NT - 1) / NT, row0 = tid * per;
+  int mine = 0;
+  for (int x = row0; x < min(row0 + per, a.rows); ++x) mine += row_tiles(a, x).tiles;
+  int upto = mine;
 #pragma unroll
-    for (int k = 16; k; k >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, k);
-    if (lane == 0) scan[warp] = mine;
-    __syncthreads();
-    total = 0;
-#pragma unroll
-    for (int k = 0; k < NW; ++k) total += scan[k];
-    __syncthreads();
+  for (int k = 1; k < 32; k <<= 1) {
+    const int x = __shfl_up_sync(0xffffffffu, upto, k);
+    if (lane >= k) upto += x;
   }
-  const int64_t W = total * K;
-  // Blocks in use: at least one tile per warp each.
-  const int64_t N = min((int64_t)blocks_max, (W + NW - 1) / NW);
+  if (lane == 31) scan[warp] = upto;
+  __syncthreads();
+  int total = 0;
+#pragma unroll
+  for (int k = 0; k < NW; ++k) {
+    if (k == warp) upto += total;
+    total += scan[k];
+  }
+  const int W = total * K;  // fits 31 bits (checked by the host)
+  // Blocks in use, at least one tile per warp each; the first `extra` take one more.
+  const int N = min(blocks_max, (W + NW - 1) / NW), share = W / N, extra = W - share * N;
   const int c = blockIdx.x;
   if (c >= N) return;
-  auto first_tile = [&](int64_t b) { return b * W / N; };
-  auto block_of = [&](int64_t tile) {
-    int64_t b = tile * N / W;
-    while (b + 1 < N && first_tile(b + 1) <= tile) ++b;
-    while (first_tile(b) > tile) --b;
-    return (int)b;
+  auto first_tile = [&](int b) { return b * share + min(b, extra); };
+  auto block_of = [&](int tile) {
+    const int b = tile / (share + 1);
+    return b < extra ? b : extra + (tile - extra * (share + 1)) / share;
   };
-  const int64_t t0 = first_tile(c), t1 = first_tile(c + 1);
+  const int t0 = first_tile(c), t1 = first_tile(c + 1);
   // The row that holds tile t0, and the tiles (of one head) before it.
-  int r;
-  int64_t before;
-  if (uniform) {
-    const int64_t per = row_tiles(a, 0).tiles;
-    r = (int)(t0 / (per * K));
-    before = per * r;
-  } else {
-    int64_t base = 0;
-    for (int r0 = 0;; r0 += NT) {
-      const int rr = r0 + tid;
-      const int64_t n = rr < a.rows ? row_tiles(a, rr).tiles : 0;
-      int64_t s = n;
-#pragma unroll
-      for (int k = 1; k < 32; k <<= 1) {
-        const int64_t x = __shfl_up_sync(0xffffffffu, s, k);
-        if (lane >= k) s += x;
-      }
-      if (lane == 31) scan[warp] = s;
-      if (tid == 0) sh_row = -1;
-      __syncthreads();
-      int64_t off = base, all = 0;
-      for (int k = 0; k < NW; ++k) {
-        if (k < warp) off += scan[k];
-        all += scan[k];
-      }
-      const int64_t lo = off + s - n;
-      if (lo * K <= t0 && t0 < (lo + n) * K) {
-        sh_row = rr;
-        sh_before = lo;
-      }
-      __syncthreads();
-      if (sh_row >= 0) break;
-      base += all;
+  if ((upto - mine) * K <= t0 && t0 < upto * K) {
+    int x = row0, at = upto - mine;
+    for (;; ++x) {
+      const int tiles = row_tiles(a, x).tiles;
+      if (t0 < (at + tiles) * K) break;
+      at += tiles;
     }
-    r = sh_row;
-    before = sh_before;
+    sh_row = x;
+    sh_before = at;
   }
-
+  __syncthreads();
+  int r = sh_row, before = sh_before;
   RowTiles rt = row_tiles(a, r);
-  int h = (int)((t0 - before * K) / rt.tiles);
-  int64_t cur = t0;
+  int h = (t0 - before * K) / rt.tiles, cur = t0;
   const int64_t all_rows = (int64_t)a.rows * K * nG;
   while (cur < t1) {
-    const int64_t unit_first = before * K + (int64_t)h * rt.tiles;
-    const int seg0 = (int)(cur - unit_first), seg1 = (int)min((int64_t)rt.tiles, t1 - unit_first);
+    const int unit_first = before * K + h * rt.tiles;
+    const int seg0 = cur - unit_first, seg1 = min(rt.tiles, t1 - unit_first);
     const int unit = r * K + h;
 
     // Queries of rows g and g + 8, vectors t, t + 4, ...
     uint4 qf[2][2 * DC];
 #pragma unroll
     for (int x = 0; x < 2; ++x) {
-      const int m = g + 8 * x, i = m / a.group, hd = h * a.group + m - i * a.group;
+      const int m = g + 8 * x, i = MULTI ? m / group : 0, hd = h * group + m - i * group;
       const T* p = static_cast<const T*>(a.q) + r * a.q_row + i * a.q_tok + hd * a.q_head;
 #pragma unroll
       for (int u = 0; u < 2 * DC; ++u) {
@@ -221,7 +194,7 @@ __global__ void __launch_bounds__(NT, 1) attn_token_kernel(const __grid_constant
     int pos[2], low[2];
 #pragma unroll
     for (int x = 0; x < 2; ++x) {
-      pos[x] = rt.end - a.n + (g + 8 * x) / a.group;
+      pos[x] = MULTI ? rt.end - a.n + (g + 8 * x) / group : rt.end - 1;
       low[x] = window_low(a, rt.start, pos[x]);
     }
     const int pos_first = rt.end - a.n, low_last = window_low(a, rt.start, rt.end - 1);
@@ -265,12 +238,14 @@ __global__ void __launch_bounds__(NT, 1) attn_token_kernel(const __grid_constant
           vf[x][u] = load_stream(p + (8 * u + g) * 8, tile < seg1 && j < jend && (FULL || 8 * u + g < vecs));
       }
     };
-    load_k(seg0 + warp);
-    load_v(seg0 + warp);
-    for (int tile = seg0 + warp; tile < seg1; tile += NW) {
+    // The round before the first only loads (one copy of the loads keeps the code
+    // small: for short calls, fetching instructions is what takes time).
+    for (int tile = seg0 + warp - NW; tile < seg1; tile += NW) {
+      const bool work = tile >= seg0;
       int j0, jend;
       tile_at(tile, j0, jend);
       float s[2][4];
+      if (work) {
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
 #pragma unroll
@@ -281,7 +256,9 @@ __global__ void __launch_bounds__(NT, 1) attn_token_kernel(const __grid_constant
           Mma<T>::run(s[x], qf[0][u].z, qf[1][u].z, qf[0][u].w, qf[1][u].w, kf[x][u].z, kf[x][u].w);
         }
       }
+      }
       load_k(tile + NW);
+      if (work) {
       const bool whole = j0 + TK <= jend &&
                          (tile < rt.ta || !MULTI || (j0 >= low_last && j0 + TK - 1 <= pos_first));
 #pragma unroll
@@ -399,6 +376,7 @@ __global__ void __launch_bounds__(NT, 1) attn_token_kernel(const __grid_constant
                       __byte_perm(v2[w], v3[w], 0x7632));
         }
       }
+      }
       load_v(tile + NW);
     }
 
@@ -443,8 +421,8 @@ __global__ void __launch_bounds__(NT, 1) attn_token_kernel(const __grid_constant
     const int row_vecs = D >> 2;
     auto write_out = [&](int m, int d, float4 x, float L) {
       const float inv = L == 0.f ? 0.f : 1.f / L;
-      const int i = m / a.group;
-      T* out = static_cast<T*>(a.out) + (((int64_t)r * a.n + i) * a.heads + h * a.group + m - i * a.group) * D + d;
+      const int i = MULTI ? m / group : 0;
+      T* out = static_cast<T*>(a.out) + (((int64_t)r * a.n + i) * a.heads + h * group + m - i * group) * D + d;
       *reinterpret_cast<uint2*>(out) =
           make_uint2(Mma<T>::pack(x.x * inv, x.y * inv), Mma<T>::pack(x.z * inv, x.w * inv));
     };
@@ -498,7 +476,7 @@ __global__ void __launch_bounds__(NT, 1) attn_token_kernel(const __grid_constant
         for (int x = tid; x < nG * row_vecs; x += NT) {
           const int m = x / row_vecs, d = (x - m * row_vecs) * 4;
           float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 8
+#pragma unroll 4
           for (int k = 0; k < count + more; ++k) {
             const float* src = k < count
                                    ? a.part_o + ((int64_t)slot_of(b0 + k * step) * 16 + m) * D + d
@@ -585,8 +563,7 @@ __global__ void __launch_bounds__(256) scores_weights_kernel(const __grid_consta
 template <typename T, int DC, bool FULL, bool MULTI>
 cudaError_t token(const AttnArgs& a, int blocks, cudaStream_t stream) {
   constexpr size_t smem = sizeof(float) * NW * 16 * (DC * 64 + 4);
-  const cudaError_t e = cudaFuncSetAttribute(attn_token_kernel<T, DC, FULL, MULTI>,
-                                             cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  const cudaError_t e = allow_smem<attn_token_kernel<T, DC, FULL, MULTI>>(smem);
   if (e != cudaSuccess) return e;
   attn_token_kernel<T, DC, FULL, MULTI><<<blocks, NT, smem, stream>>>(a, blocks);
   return cudaGetLastError();

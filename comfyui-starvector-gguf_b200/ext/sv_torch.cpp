@@ -6,9 +6,10 @@
 // returns its code (0 or a negative SV_E_*; ops.py turns codes into the same
 // exceptions as before).  Shapes and the history form are decided by the Python
 // wrappers (ops.py), which pass the same sizes and strides as the C signatures;
-// nothing here synchronises, and only the cache operators (window_attention,
-// prefix_attention, kv_evict) allocate: their outputs and a workspace kept per
-// device, stream and size.
+// nothing here synchronises or allocates.  The attention functions are called once per
+// layer and token, where each tensor attribute read from Python counts: they look at
+// the shapes here (ValueError where ops.py would raise one) and allocate their outputs
+// and a workspace kept per device, stream and size; so does kv_evict its outputs.
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
@@ -217,71 +218,138 @@ at::Tensor workspace_for(const at::Device& dev, c10::cuda::CUDAStream stream, si
 // Strides of a dimension of one entry mean nothing: 0 stands for them.
 int64_t stride_of(const at::Tensor& t, int64_t d) { return t.size(d) > 1 ? t.stride(d) : 0; }
 
-at::Tensor attention_out(const OptT& out, const at::Tensor& q, const at::Device& dev) {
+bool aligned(const at::Tensor& t, int64_t dims) {
+  if (reinterpret_cast<uintptr_t>(t.data_ptr()) % 16) return false;
+  const int64_t e = t.element_size();
+  for (int64_t d = 0; d < dims; ++d)
+    if (stride_of(t, d) * e % 16) return false;
+  return true;
+}
+
+// q as [rows, tokens, heads, head_dim] with 16-byte aligned rows; [rows, heads,
+// head_dim] stands for one token.
+at::Tensor queries(const at::Tensor& q) {
+  TORCH_CHECK(q.is_cuda(), "q must be a CUDA tensor (the B200 sampling kernels have no CPU path)");
+  TORCH_CHECK_VALUE(q.dim() == 3 || q.dim() == 4,
+                    "q must be [rows, tokens, heads, head_dim] or [rows, heads, head_dim]");
+  const auto st = q.scalar_type();
+  TORCH_CHECK_VALUE(st == at::kFloat || st == at::kHalf || st == at::kBFloat16, "unsupported dtype ", st);
+  at::Tensor x = q.dim() == 3 ? q.unsqueeze(1) : q;
+  if (stride_of(x, 3) > 1 || !aligned(x, 3)) x = x.clone(at::MemoryFormat::Contiguous);
+  return x;
+}
+
+// One layer's keys or values as [rows, kv_heads, capacity, head_dim].
+at::Tensor layer_cache(const at::Tensor& t) { return t.dim() == 3 ? t.unsqueeze(1) : t; }
+
+void check_cache(const at::Tensor& k, const at::Tensor& v, const at::Tensor& q) {
+  const at::Device dev = q.device();
+  on_device(k, dev, "keys");
+  on_device(v, dev, "values");
+  TORCH_CHECK_VALUE(k.dim() == 4 && v.sizes() == k.sizes() && v.strides() == k.strides(),
+                    "keys must be [rows, capacity, head_dim] or [rows, kv_heads, capacity, head_dim], and values "
+                    "have their shape and strides");
+  TORCH_CHECK_VALUE(k.scalar_type() == q.scalar_type() && v.scalar_type() == q.scalar_type(),
+                    "keys and values must have q's dtype");
+  TORCH_CHECK_VALUE(k.size(0) == q.size(0) && k.size(3) == q.size(3) && k.size(1) > 0 && q.size(2) % k.size(1) == 0,
+                    "keys must have q's rows and head_dim, and kv_heads must divide heads");
+  TORCH_CHECK_VALUE(stride_of(k, 3) <= 1, "head_dim must be contiguous");
+}
+
+// A per-row int32 tensor from a tensor of whole numbers (none stays none).
+OptT row_ints(const OptT& t, int64_t rows, const at::Device& dev, const char* name) {
+  if (!t.has_value()) return t;
+  const auto st = t->scalar_type();
+  TORCH_CHECK_VALUE((st == at::kInt || st == at::kLong) && t->numel() == rows, name,
+                    " must be an int32 or int64 tensor with one value per row");
+  if (st == at::kInt && t->device() == dev && t->is_contiguous()) return t;
+  return t->reshape({-1}).to(dev, at::kInt).contiguous();
+}
+
+at::Tensor attention_out(const OptT& out, const at::Tensor& q) {
   if (!out.has_value()) return at::empty(q.sizes(), q.options());
-  on_device(*out, dev, "out");
-  TORCH_CHECK(out->scalar_type() == q.scalar_type() && out->numel() == q.numel() && out->is_contiguous(),
+  on_device(*out, q.device(), "out");
+  TORCH_CHECK(out->scalar_type() == q.scalar_type() && out->sizes() == q.sizes() && out->is_contiguous(),
               "out must be a contiguous tensor of the queries' shape and dtype");
   return *out;
 }
 
-void same_cache(const at::Tensor& k, const at::Tensor& v, const at::Tensor& q, const at::Device& dev) {
-  on_device(k, dev, "keys");
-  on_device(v, dev, "values");
-  TORCH_CHECK(k.scalar_type() == q.scalar_type() && v.scalar_type() == q.scalar_type(),
-              "queries, keys and values must have one dtype");
-}
-
-// sv_window_attention.  q [rows, tokens, heads, head_dim], keys / values [rows,
-// kv_heads, capacity, head_dim], weights [rows, kv_heads, capacity].
-std::tuple<int, at::Tensor> window_attention(const at::Tensor& q, const at::Tensor& keys, const at::Tensor& values,
-                                             const OptT& lengths, const OptT& starts, int64_t window, int64_t sinks,
-                                             double scale, const OptT& weights, const OptT& out,
+// sv_window_attention.
+std::tuple<int, at::Tensor> window_attention(const at::Tensor& q_in, const at::Tensor& keys_in,
+                                             const at::Tensor& values_in, const OptT& lengths_in,
+                                             const OptT& starts_in, int64_t window, int64_t sinks,
+                                             std::optional<double> scale, const OptT& weights_in, const OptT& out,
                                              const OptT& out_status) {
+  const at::Tensor q = queries(q_in), keys = layer_cache(keys_in), values = layer_cache(values_in);
+  check_cache(keys, values, q);
   const at::Device dev = q.device();
-  on_device(q, dev, "q");
-  same_cache(keys, values, q, dev);
   const c10::cuda::CUDAGuard guard(dev);
   const auto stream = at::cuda::getCurrentCUDAStream(dev.index());
   const int32_t rows = (int32_t)q.size(0), n = (int32_t)q.size(1), heads = (int32_t)q.size(2), dim = (int32_t)q.size(3);
   const int32_t kv = (int32_t)keys.size(1), capacity = (int32_t)keys.size(2), code = logit_code(q);
-  at::Tensor o = attention_out(out, q, dev);
-  const size_t bytes = sv_window_attention_workspace_bytes(code, rows, n, heads, kv, dim, capacity, (int32_t)window,
-                                                           (int32_t)sinks, weights.has_value());
+  TORCH_CHECK_VALUE(window >= 0 && sinks >= 0, "window and sinks must not be negative");
+  TORCH_CHECK_VALUE(!scale.has_value() || std::isfinite(*scale), "scale must be finite");
+  OptT weights = weights_in;
+  if (weights.has_value()) {
+    if (weights->dim() == 2) weights = weights->unsqueeze(1);
+    TORCH_CHECK_VALUE(weights->scalar_type() == at::kFloat && weights->dim() == 3 && weights->size(0) == rows &&
+                          weights->size(1) == kv && weights->size(2) >= capacity && stride_of(*weights, 2) <= 1,
+                      "weights must be float32 [rows, kv_heads, capacity], contiguous along the slots");
+  }
+  const OptT lengths = row_ints(lengths_in, rows, dev, "lengths"), starts = row_ints(starts_in, rows, dev, "starts");
+  const int32_t w = (int32_t)std::min<int64_t>(window, 1 << 30), s = (int32_t)std::min<int64_t>(sinks, 1 << 30);
+  at::Tensor o = attention_out(out, q_in);
+  const size_t bytes =
+      sv_window_attention_workspace_bytes(code, rows, n, heads, kv, dim, capacity, w, s, weights.has_value());
   at::Tensor ws = workspace_for(dev, stream, bytes, 4 * ((size_t)rows * kv + 1024));
   const int rc = sv_window_attention(
       q.data_ptr(), code, rows, n, heads, kv, dim, stride_of(q, 0), stride_of(q, 1), stride_of(q, 2), keys.data_ptr(),
       values.data_ptr(), capacity, stride_of(keys, 0), stride_of(keys, 1), stride_of(keys, 2),
       optptr<int32_t>(lengths, dev, "lengths", at::kInt, rows), optptr<int32_t>(starts, dev, "starts", at::kInt, rows),
-      (int32_t)window, (int32_t)sinks, scale, optptr<float>(weights, dev, "weights", at::kFloat),
-      weights.has_value() ? stride_of(*weights, 0) : 0, weights.has_value() ? stride_of(*weights, 1) : 0,
-      o.data_ptr(), ws.defined() ? ws.data_ptr() : nullptr, ws.defined() ? (size_t)ws.numel() : 0,
-      optptr<int32_t>(out_status, dev, "status", at::kInt, rows), stream.stream());
+      w, s, scale.has_value() ? *scale : 1.0 / std::sqrt((double)dim),
+      optptr<float>(weights, dev, "weights", at::kFloat), weights.has_value() ? stride_of(*weights, 0) : 0,
+      weights.has_value() ? stride_of(*weights, 1) : 0, o.data_ptr(), ws.defined() ? ws.data_ptr() : nullptr,
+      ws.defined() ? (size_t)ws.numel() : 0, optptr<int32_t>(out_status, dev, "status", at::kInt, rows),
+      stream.stream());
   return {rc, o};
 }
 
-// sv_prefix_attention.  prefix_keys / prefix_values [kv_heads, prefix_length, head_dim].
-std::tuple<int, at::Tensor> prefix_attention(const at::Tensor& q, const at::Tensor& prefix_keys,
-                                             const at::Tensor& prefix_values, const at::Tensor& keys,
-                                             const at::Tensor& values, const OptT& lengths, double scale,
+// sv_prefix_attention.
+std::tuple<int, at::Tensor> prefix_attention(const at::Tensor& q_in, const at::Tensor& prefix_keys_in,
+                                             const at::Tensor& prefix_values_in, const at::Tensor& keys_in,
+                                             const at::Tensor& values_in, const OptT& lengths_in,
+                                             std::optional<int64_t> prefix_length, std::optional<double> scale,
                                              const OptT& out, const OptT& out_status) {
+  const at::Tensor q = queries(q_in), keys = layer_cache(keys_in), values = layer_cache(values_in);
+  check_cache(keys, values, q);
+  const at::Tensor pk = prefix_keys_in.dim() == 2 ? prefix_keys_in.unsqueeze(0) : prefix_keys_in;
+  const at::Tensor pv = prefix_values_in.dim() == 2 ? prefix_values_in.unsqueeze(0) : prefix_values_in;
   const at::Device dev = q.device();
-  on_device(q, dev, "q");
-  same_cache(keys, values, q, dev);
-  same_cache(prefix_keys, prefix_values, q, dev);
+  on_device(pk, dev, "prefix_keys");
+  on_device(pv, dev, "prefix_values");
+  TORCH_CHECK_VALUE(pk.dim() == 3 && pv.sizes() == pk.sizes() && pv.strides() == pk.strides() &&
+                        pk.scalar_type() == q.scalar_type() && pv.scalar_type() == q.scalar_type() &&
+                        pk.size(0) == keys.size(1) && pk.size(2) == q.size(3) && stride_of(pk, 2) <= 1,
+                    "prefix_keys and prefix_values must be [kv_heads, prefix, head_dim] of q's dtype with the same "
+                    "strides");
+  TORCH_CHECK_VALUE(!prefix_length.has_value() || (*prefix_length >= 0 && *prefix_length <= pk.size(1)),
+                    "prefix_length must be in [0, the prefix's slots]");
+  TORCH_CHECK_VALUE(!scale.has_value() || std::isfinite(*scale), "scale must be finite");
   const c10::cuda::CUDAGuard guard(dev);
   const auto stream = at::cuda::getCurrentCUDAStream(dev.index());
   const int32_t rows = (int32_t)q.size(0), n = (int32_t)q.size(1), heads = (int32_t)q.size(2), dim = (int32_t)q.size(3);
   const int32_t kv = (int32_t)keys.size(1), capacity = (int32_t)keys.size(2), code = logit_code(q);
-  const int32_t prefix = (int32_t)prefix_keys.size(1);
-  at::Tensor o = attention_out(out, q, dev);
+  const int32_t prefix = (int32_t)prefix_length.value_or(pk.size(1));
+  const OptT lengths = row_ints(lengths_in, rows, dev, "lengths");
+  at::Tensor o = attention_out(out, q_in);
   const size_t bytes = sv_prefix_attention_workspace_bytes(code, rows, n, heads, kv, dim, prefix, capacity);
   at::Tensor ws = workspace_for(dev, stream, bytes, 4 * ((size_t)rows * kv + 1024));
   const int rc = sv_prefix_attention(
-      q.data_ptr(), code, rows, n, heads, kv, dim, stride_of(q, 0), stride_of(q, 1), stride_of(q, 2),
-      prefix_keys.data_ptr(), prefix_values.data_ptr(), prefix, stride_of(prefix_keys, 0), stride_of(prefix_keys, 1),
-      keys.data_ptr(), values.data_ptr(), capacity, stride_of(keys, 0), stride_of(keys, 1), stride_of(keys, 2),
-      optptr<int32_t>(lengths, dev, "lengths", at::kInt, rows), scale, o.data_ptr(),
+      q.data_ptr(), code, rows, n, heads, kv, dim, stride_of(q, 0), stride_of(q, 1), stride_of(q, 2), pk.data_ptr(),
+      pv.data_ptr(), prefix, stride_of(pk, 0), stride_of(pk, 1), keys.data_ptr(), values.data_ptr(), capacity,
+      stride_of(keys, 0), stride_of(keys, 1), stride_of(keys, 2),
+      optptr<int32_t>(lengths, dev, "lengths", at::kInt, rows),
+      scale.has_value() ? *scale : 1.0 / std::sqrt((double)dim), o.data_ptr(),
       ws.defined() ? ws.data_ptr() : nullptr, ws.defined() ? (size_t)ws.numel() : 0,
       optptr<int32_t>(out_status, dev, "status", at::kInt, rows), stream.stream());
   return {rc, o};

@@ -557,43 +557,11 @@ def kv_reorder(keys, values, parents, length, out_status=None):
     L.check(rc, "sv_kv_reorder")
 
 
-def _queries(q):
-    """q as [rows, tokens, heads, head_dim] with 16-byte aligned rows; [rows, heads,
-    head_dim] stands for one token."""
-    _need_cuda(q, "q")
-    x = q.unsqueeze(1) if q.dim() == 3 else q
-    if x.dim() != 4:
-        raise ValueError("q must be [rows, tokens, heads, head_dim] or [rows, heads, head_dim]")
-    if x.dtype not in _DTYPES:
-        raise ValueError(f"unsupported dtype {x.dtype}")
-    size, e = x.shape, x.element_size()
-    if x.stride(3) != 1 or x.data_ptr() % 16 or any(size[d] > 1 and x.stride(d) * e % 16 for d in (0, 1, 2)):
-        x = x.clone(memory_format=torch.contiguous_format)
-    return x
-
-
-def _layer_cache(keys, values, q, length, names=("keys", "values")):
-    """One layer's keys and values as [rows, kv_heads, capacity, head_dim], cut to
-    `length` slots when it is a number; checked against q."""
-    _need_cuda(keys, names[0])
-    _need_cuda(values, names[1])
-    if keys.dim() == 3:
-        keys, values = keys.unsqueeze(1), values.unsqueeze(1)
-    if keys.dim() != 4 or values.shape != keys.shape or values.stride() != keys.stride():
-        raise ValueError(f"{names[0]} must be [rows, capacity, head_dim] or [rows, kv_heads, capacity, head_dim], "
-                         f"and {names[1]} have their shape and strides")
-    R, K, cap, D = keys.shape
-    if keys.dtype != q.dtype or values.dtype != q.dtype:
-        raise ValueError(f"{names[0]} and {names[1]} must have q's dtype")
-    if R != q.shape[0] or D != q.shape[3] or K < 1 or q.shape[2] % K:
-        raise ValueError(f"{names[0]} must have q's rows and head_dim, and kv_heads must divide heads")
-    if D > 1 and keys.stride(3) != 1:
-        raise ValueError("head_dim must be contiguous")
-    if isinstance(length, int):
-        if not 1 <= length <= cap:
-            raise ValueError("length must be in [1, capacity]")
-        keys, values = keys.narrow(2, 0, length), values.narrow(2, 0, length)
-    return keys, values
+def _first_slots(keys, values, length):
+    """The first `length` slots of one layer's keys and values."""
+    if not 1 <= length <= keys.shape[-2]:
+        raise ValueError("length must be in [1, capacity]")
+    return keys.narrow(-2, 0, length), values.narrow(-2, 0, length)
 
 
 def _row_ints(t, rows, device, name):
@@ -623,23 +591,11 @@ def window_attention(q, keys, values, lengths=None, *, starts=None, window=0, si
     capacity], or [rows, capacity]) has each slot's softmax weight added, summed over
     the head group and the queries: kv_evict's input.  status: int32 [rows], filled
     with 0 or SV_ST_LENGTH.  Returns the output, q's shape and dtype."""
-    x = _queries(q)
-    k, v = _layer_cache(keys, values, x, lengths)
-    R, dev = x.shape[0], x.device
-    w = weights
-    if w is not None:
-        _need_cuda(w, "weights")
-        w = w.unsqueeze(1) if w.dim() == 2 else w
-        if w.dtype != torch.float32 or w.dim() != 3 or w.shape[:2] != k.shape[:2] or w.shape[2] < k.shape[2] or \
-                w.stride(2) != 1:
-            raise ValueError("weights must be float32 [rows, kv_heads, capacity], contiguous along the slots")
-    if window < 0 or sinks < 0:
-        raise ValueError("window and sinks must not be negative")
-    rc, o = _ext().window_attention(x, k, v, _row_ints(lengths, R, dev, "lengths"),
-                                    _row_ints(starts, R, dev, "starts"), window, sinks,
-                                    x.shape[3] ** -0.5 if scale is None else float(scale), w, out, status)
+    if isinstance(lengths, int):
+        (keys, values), lengths = _first_slots(keys, values, lengths), None
+    rc, o = _ext().window_attention(q, keys, values, lengths, starts, window, sinks, scale, weights, out, status)
     L.check(rc, "sv_window_attention")
-    return o.view(q.shape) if out is None else out
+    return o
 
 
 def prefix_attention(q, prefix_keys, prefix_values, keys, values, lengths=None, *, prefix_length=None, scale=None,
@@ -651,25 +607,12 @@ def prefix_attention(q, prefix_keys, prefix_values, keys, values, lengths=None, 
     prefix_keys / prefix_values: [kv_heads, prefix, head_dim], or [prefix, head_dim]
     (MQA), of which the first `prefix_length` slots count (None: all); the rest as
     window_attention, `lengths` counting the rows' own slots."""
-    x = _queries(q)
-    k, v = _layer_cache(keys, values, x, lengths)
-    _need_cuda(prefix_keys, "prefix_keys")
-    pk, pv = prefix_keys, prefix_values
-    if pk.dim() == 2:
-        pk, pv = pk.unsqueeze(0), pv.unsqueeze(0)
-    if pk.dim() != 3 or pv.shape != pk.shape or pv.stride() != pk.stride() or pk.dtype != x.dtype or \
-            pv.dtype != x.dtype or pk.shape[0] != k.shape[1] or pk.shape[2] != x.shape[3] or \
-            (pk.shape[2] > 1 and pk.stride(2) != 1):
-        raise ValueError("prefix_keys and prefix_values must be [kv_heads, prefix, head_dim] of q's dtype with the "
-                         "same strides")
-    if prefix_length is not None:
-        if not 0 <= prefix_length <= pk.shape[1]:
-            raise ValueError("prefix_length must be in [0, the prefix's slots]")
-        pk, pv = pk.narrow(1, 0, prefix_length), pv.narrow(1, 0, prefix_length)
-    rc, o = _ext().prefix_attention(x, pk, pv, k, v, _row_ints(lengths, x.shape[0], x.device, "lengths"),
-                                    x.shape[3] ** -0.5 if scale is None else float(scale), out, status)
+    if isinstance(lengths, int):
+        (keys, values), lengths = _first_slots(keys, values, lengths), None
+    rc, o = _ext().prefix_attention(q, prefix_keys, prefix_values, keys, values, lengths, prefix_length, scale, out,
+                                    status)
     L.check(rc, "sv_prefix_attention")
-    return o.view(q.shape) if out is None else out
+    return o
 
 
 def kv_evict(keys, values, weights, positions, lengths=None, budget=None, *, sinks=0, recent=0, out=None,
