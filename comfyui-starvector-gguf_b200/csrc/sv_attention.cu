@@ -101,8 +101,8 @@ int check_shapes(const AttnArgs& a) {
   if (a.window < 0 || a.sinks < 0 || a.window > 1 << 30 || a.sinks > 1 << 30 || a.capacity > 1 << 30 ||
       a.prefix > 1 << 30)
     return SV_E_SHAPE;
-  // The token kernel counts 16-slot tiles in 31 bits (a cache row of broadcast strides could exceed them).
-  if ((int64_t)a.rows * a.kv_heads * (a.capacity / 16 + 3) >= (int64_t)1 << 31) return SV_E_SHAPE;
+  // The token kernel counts chunks of 64 slots in 31 bits (a cache of broadcast rows could exceed them).
+  if ((int64_t)a.rows * a.kv_heads * (a.capacity / 64 + 3) >= (int64_t)1 << 31) return SV_E_SHAPE;
   return SV_OK;
 }
 

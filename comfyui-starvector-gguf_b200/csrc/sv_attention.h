@@ -19,7 +19,9 @@ namespace sv {
 
 constexpr int kAttnMaxDim = 128;
 constexpr int kTokenRows = 16;     // query rows per key/value head of the token kernel
-constexpr int kTokenBlocks = 148;  // its blocks: one per SM
+constexpr int kTokenWarps = 8;     // its warps per block, blocks per SM, blocks
+constexpr int kTokenPerSM = 1;
+constexpr int kTokenBlocks = 148 * kTokenPerSM;
 
 struct AttnArgs {
   const void* q;

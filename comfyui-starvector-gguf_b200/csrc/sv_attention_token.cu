@@ -21,8 +21,8 @@
 // The next tile's keys are fetched as soon as the scores are formed, the next values
 // after the product, so a warp keeps 4 to 8 KB in flight.
 //
-// Work split: the tiles of all units form one list, in unit order, cut into equal
-// parts, one per block; ragged lengths balance by themselves.  A unit that spans
+// Work split: the chunks (eight tiles, one per warp) of all units form one list, in unit
+// order, cut into equal parts, one per block; ragged lengths balance by themselves.  A unit that spans
 // several blocks leaves partial results, which the last block to arrive joins, in
 // block order (so results repeat bit for bit); past 32 parts in two levels, so that no
 // block joins more than a few dozen.  The sums' counters return to zero.
@@ -31,7 +31,7 @@
 namespace sv {
 namespace {
 
-constexpr int NW = 8, NT = NW * 32;
+constexpr int NW = kTokenWarps, NT = NW * 32;
 constexpr int TK = 16;         // slots per tile
 constexpr int kJoin = 16;      // parts per first-level group
 constexpr int kMaxFlat = 32;   // parts joined in one level
@@ -94,9 +94,18 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
+// Counts an arrival: what the block wrote before (ordered by a barrier) is visible to
+// who arrives later, and this thread sees what earlier ones wrote.
+__device__ __forceinline__ unsigned arrive(unsigned* counter) {
+  unsigned old;
+  asm volatile("atom.acq_rel.gpu.global.add.u32 %0, [%1], 1;" : "=r"(old) : "l"(counter) : "memory");
+  return old;
+}
+
 // What one row's tiles are: [a0, a1) the sinks before the window, [b0, b1) the rest.
 struct RowTiles {
   int start, end, a0, a1, b0, b1, ta, tiles;
+  __device__ int chunks() const { return (tiles + NW - 1) / NW; }
 };
 
 __device__ __noinline__ RowTiles row_tiles(const AttnArgs& a, int r) {
@@ -113,25 +122,38 @@ __device__ __noinline__ RowTiles row_tiles(const AttnArgs& a, int r) {
   return t;
 }
 
+// One block's part of a unit (row r, head h): tiles [t0, t1) of the row.
+struct Part {
+  int r, h, before, first, end, t0, t1;  // before, first, end: chunks before the row (one head), of the unit
+  RowTiles rt;
+  __device__ __forceinline__ void open(int K, int c0, int c1) {
+    first = before * K + h * rt.chunks();
+    end = first + rt.chunks();
+    t0 = (max(c0, first) - first) * NW;
+    t1 = min(rt.tiles, (c1 - first) * NW);
+  }
+};
+
 // MULTI: more than one query per row (then a tile may be visible to some of them only).
 template <typename T, int DC, bool FULL, bool MULTI>
-__global__ void __launch_bounds__(NT, 1) attn_token_kernel(const __grid_constant__ AttnArgs a, const int blocks_max) {
+__global__ void __launch_bounds__(NT, kTokenPerSM) attn_token_kernel(const __grid_constant__ AttnArgs a, const int blocks_max) {
   constexpr int OS = DC * 64 + 4;  // row stride of the warps' outputs in shared memory
   extern __shared__ float dyn[];   // [NW][16][OS]
   __shared__ float2 warp_ml[NW][16];
   __shared__ float factor[kMaxFlat * 2][16];
+  __shared__ float2 part_ml[kMaxFlat * 2][16];
   __shared__ float2 joined[16];
   __shared__ int scan[NW];
-  __shared__ int sh_row, sh_before, sh_last;
+  __shared__ int sh_row, sh_before, sh_last[2];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
   const int group = a.group, nG = MULTI ? a.n * group : group, K = a.kv_heads, D = FULL ? 64 * DC : a.dim;
   const int vecs = D >> 3;
 
-  // Tiles of all rows (every head of a row has as many): thread x counts rows
+  // Chunks (a tile per warp) of all rows, every head of a row having as many: thread x counts rows
   // [x per, (x + 1) per), a scan gives the total and what lies before each thread.
   const int per = (a.rows + NT - 1) / NT, row0 = tid * per;
   int mine = 0;
-  for (int x = row0; x < min(row0 + per, a.rows); ++x) mine += row_tiles(a, x).tiles;
+  for (int x = row0; x < min(row0 + per, a.rows); ++x) mine += row_tiles(a, x).chunks();
   int upto = mine;
 #pragma unroll
   for (int k = 1; k < 32; k <<= 1) {
@@ -147,103 +169,200 @@ __global__ void __launch_bounds__(NT, 1) attn_token_kernel(const __grid_constant
     total += scan[k];
   }
   const int W = total * K;  // fits 31 bits (checked by the host)
-  // Blocks in use, at least one tile per warp each; the first `extra` take one more.
-  const int N = min(blocks_max, (W + NW - 1) / NW), share = W / N, extra = W - share * N;
+  // Blocks in use (a short call takes one per chunk); the first `extra` take one chunk more.
+  const int N = min(blocks_max, W), share = W / N, extra = W - share * N;
   const int c = blockIdx.x;
   if (c >= N) return;
-  auto first_tile = [&](int b) { return b * share + min(b, extra); };
-  auto block_of = [&](int tile) {
-    const int b = tile / (share + 1);
-    return b < extra ? b : extra + (tile - extra * (share + 1)) / share;
+  auto first_chunk = [&](int b) { return b * share + min(b, extra); };
+  auto block_of = [&](int chunk) {
+    const int b = chunk / (share + 1);
+    return b < extra ? b : extra + (chunk - extra * (share + 1)) / share;
   };
-  const int t0 = first_tile(c), t1 = first_tile(c + 1);
-  // The row that holds tile t0, and the tiles (of one head) before it.
-  if ((upto - mine) * K <= t0 && t0 < upto * K) {
+  const int c0 = first_chunk(c), c1 = first_chunk(c + 1);
+  // The row that holds chunk c0, and the chunks (of one head) before it.
+  if ((upto - mine) * K <= c0 && c0 < upto * K) {
     int x = row0, at = upto - mine;
     for (;; ++x) {
-      const int tiles = row_tiles(a, x).tiles;
-      if (t0 < (at + tiles) * K) break;
-      at += tiles;
+      const int chunks = row_tiles(a, x).chunks();
+      if (c0 < (at + chunks) * K) break;
+      at += chunks;
     }
     sh_row = x;
     sh_before = at;
   }
   __syncthreads();
-  int r = sh_row, before = sh_before;
-  RowTiles rt = row_tiles(a, r);
-  int h = (t0 - before * K) / rt.tiles, cur = t0;
+  Part p;
+  p.r = sh_row;
+  p.before = sh_before;
+  p.rt = row_tiles(a, p.r);
+  p.h = (c0 - p.before * K) / p.rt.chunks();
+  p.open(K, c0, c1);
   const int64_t all_rows = (int64_t)a.rows * K * nG;
-  while (cur < t1) {
-    const int unit_first = before * K + h * rt.tiles;
-    const int seg0 = cur - unit_first, seg1 = min(rt.tiles, t1 - unit_first);
-    const int unit = r * K + h;
+  const int row_vecs = D >> 2;
 
-    // Queries of rows g and g + 8, vectors t, t + 4, ...
-    uint4 qf[2][2 * DC];
+  // Queries of rows g and g + 8, vectors t, t + 4, ...
+  uint4 qf[2][2 * DC], kf[2][2 * DC], vf[4][DC];
+  auto load_q = [&](const Part& p) {
 #pragma unroll
     for (int x = 0; x < 2; ++x) {
-      const int m = g + 8 * x, i = MULTI ? m / group : 0, hd = h * group + m - i * group;
-      const T* p = static_cast<const T*>(a.q) + r * a.q_row + i * a.q_tok + hd * a.q_head;
+      const int m = g + 8 * x, i = MULTI ? m / group : 0, hd = p.h * group + m - i * group;
+      const T* src = static_cast<const T*>(a.q) + p.r * a.q_row + i * a.q_tok + hd * a.q_head;
 #pragma unroll
       for (int u = 0; u < 2 * DC; ++u) {
         const int vec = 4 * u + t;
-        qf[x][u] = m < nG && (FULL || vec < vecs) ? __ldg(reinterpret_cast<const uint4*>(p) + vec)
+        qf[x][u] = m < nG && (FULL || vec < vecs) ? __ldg(reinterpret_cast<const uint4*>(src) + vec)
                                                   : make_uint4(0u, 0u, 0u, 0u);
       }
     }
+  };
+  // The next tile to fetch: its slots [fetch_j0, fetch_end) and its unit's offset.
+  int fetch_j0, fetch_end;
+  int64_t fetch_base;
+  auto tile_at = [&](const RowTiles& rt, int tile, int& j0, int& jend) {
+    const bool in_a = tile < rt.ta;
+    j0 = in_a ? rt.a0 + tile * TK : rt.b0 + (tile - rt.ta) * TK;
+    jend = in_a ? rt.a1 : rt.b1;
+  };
+  auto fetch_at = [&](const Part& p, int tile) {
+    tile_at(p.rt, tile, fetch_j0, fetch_end);
+    if (tile >= p.t1) fetch_end = 0;
+    fetch_base = p.r * a.kv_row + p.h * a.kv_head;
+  };
+  auto load_k = [&]() {
+    const T* base = static_cast<const T*>(a.k) + fetch_base + t * 8;
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      const int j = fetch_j0 + 8 * x + g;
+      const T* src = base + j * a.kv_slot;
+#pragma unroll
+      for (int u = 0; u < 2 * DC; ++u)
+        kf[x][u] = load_stream(src + 32 * u, j < fetch_end && (FULL || 4 * u + t < vecs));
+    }
+  };
+  auto load_v = [&]() {
+    const T* base = static_cast<const T*>(a.v) + fetch_base + g * 8;
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      const int j = fetch_j0 + 2 * t + (x & 1) + (x >> 1) * 8;
+      const T* src = base + j * a.kv_slot;
+#pragma unroll
+      for (int u = 0; u < DC; ++u)
+        vf[x][u] = load_stream(src + 64 * u, j < fetch_end && (FULL || 8 * u + g < vecs));
+    }
+  };
+  auto write_out = [&](const Part& p, int m, int d, float4 x, float L) {
+    const float inv = L == 0.f ? 0.f : 1.f / L;
+    const int i = MULTI ? m / group : 0;
+    T* out = static_cast<T*>(a.out) + (((int64_t)p.r * a.n + i) * a.heads + p.h * group + m - i * group) * D + d;
+    *reinterpret_cast<uint2*>(out) =
+        make_uint2(Mma<T>::pack(x.x * inv, x.y * inv), Mma<T>::pack(x.z * inv, x.w * inv));
+  };
+  auto write_lse = [&](const Part& p, int m) {
+    if (a.lse)
+      a.lse[(int64_t)(p.r * K + p.h) * nG + m] =
+          joined[m].y == 0.f ? INFINITY : joined[m].x + log2f(joined[m].y);
+  };
+  // Joins `count` parts of a unit (and, `last`, the prefix's), the k-th that of block
+  // b0 + k * step; c_first is the unit's first block.
+  auto join = [&](const Part& p, int c_first, int b0, int step, int count, bool last) {
+    const int more = last ? a.p_splits : 0;
+    const int64_t row0 = (int64_t)(p.r * K + p.h) * nG;
+    auto slot_of = [&](int k) { return 2 * (b0 + k * step) + (b0 + k * step == c_first); };
+    __syncthreads();
+    for (int x = tid; x < (count + more) * 16; x += NT) {
+      const int k = x >> 4, m = x & 15;
+      if (m < nG)
+        part_ml[k][m] = __ldcg(k < count ? a.part_ml + slot_of(k) * 16 + m
+                                         : a.prefix_ml + (int64_t)(k - count) * all_rows + row0 + m);
+    }
+    __syncthreads();
+    if (tid < nG) {
+      float M = -INFINITY;
+      for (int k = 0; k < count + more; ++k) M = fmaxf(M, part_ml[k][tid].x);
+      const float at = M == -INFINITY ? 0.f : M;
+      float L = 0.f;
+      for (int k = 0; k < count + more; ++k) {
+        const float2 ml = part_ml[k][tid];
+        const float f = ml.y == 0.f ? 0.f : ex2(ml.x - at);
+        factor[k][tid] = f;
+        L = fmaf(ml.y, f, L);
+      }
+      joined[tid] = make_float2(M, L);
+    }
+    __syncthreads();
+    for (int x = tid; x < nG * row_vecs; x += NT) {
+      const int m = x / row_vecs, d = (x - m * row_vecs) * 4;
+      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+      for (int k = 0; k < count + more; ++k) {
+        const float* src = k < count ? a.part_o + ((int64_t)slot_of(k) * 16 + m) * D + d
+                                     : a.prefix_o + ((int64_t)(k - count) * all_rows + row0 + m) * D + d;
+        const float4 y = __ldcg(reinterpret_cast<const float4*>(src));
+        const float f = factor[k][m];
+        v.x = fmaf(y.x, f, v.x);
+        v.y = fmaf(y.y, f, v.y);
+        v.z = fmaf(y.z, f, v.z);
+        v.w = fmaf(y.w, f, v.w);
+      }
+      if (last)
+        write_out(p, m, d, v, joined[m].y);
+      else
+        *reinterpret_cast<float4*>(a.part_o + ((int64_t)slot_of(0) * 16 + m) * D + d) = v;
+    }
+    if (tid < nG) {
+      if (last)
+        write_lse(p, tid);
+      else
+        a.part_ml[slot_of(0) * 16 + tid] = joined[tid];
+    }
+  };
+
+  // The units this block shares with others: the one it starts in and the one it ends
+  // in at most.  They are joined at the end, when nothing is left to fetch.
+  Part shared_part[2];
+  int shared_parts = 0;
+  load_q(p);
+  fetch_at(p, p.t0 + warp);
+  load_k();
+  load_v();
+  for (;;) {
+    Part next = p;
+    const bool more_units = p.end < c1;
+    if (more_units) {
+      if (++next.h == K) {
+        next.h = 0;
+        next.before += next.rt.chunks();
+        next.rt = row_tiles(a, ++next.r);
+      }
+      next.open(K, c0, c1);
+    }
+    const int unit = p.r * K + p.h;
     int pos[2], low[2];
 #pragma unroll
     for (int x = 0; x < 2; ++x) {
-      pos[x] = MULTI ? rt.end - a.n + (g + 8 * x) / group : rt.end - 1;
-      low[x] = window_low(a, rt.start, pos[x]);
+      pos[x] = MULTI ? p.rt.end - a.n + (g + 8 * x) / group : p.rt.end - 1;
+      low[x] = window_low(a, p.rt.start, pos[x]);
     }
-    const int pos_first = rt.end - a.n, low_last = window_low(a, rt.start, rt.end - 1);
-
-    const T* kb = static_cast<const T*>(a.k) + r * a.kv_row + h * a.kv_head;
-    const T* vb = static_cast<const T*>(a.v) + r * a.kv_row + h * a.kv_head;
+    const int pos_first = p.rt.end - a.n, low_last = window_low(a, p.rt.start, p.rt.end - 1);
+    const T* vb = static_cast<const T*>(a.v) + p.r * a.kv_row + p.h * a.kv_head;
     float o[8 * DC][4];
 #pragma unroll
     for (int j = 0; j < 8 * DC; ++j)
 #pragma unroll
       for (int x = 0; x < 4; ++x) o[j][x] = 0.f;
     float ref[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
-    uint4 kf[2][2 * DC], vf[4][DC];
 
-    auto tile_at = [&](int tile, int& j0, int& jend) {
-      const bool in_a = tile < rt.ta;
-      j0 = in_a ? rt.a0 + tile * TK : rt.b0 + (tile - rt.ta) * TK;
-      jend = in_a ? rt.a1 : rt.b1;
-    };
-    auto load_k = [&](int tile) {
-      int j0, jend;
-      tile_at(tile, j0, jend);
-#pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        const int j = j0 + 8 * x + g;
-        const T* p = kb + j * a.kv_slot;
-#pragma unroll
-        for (int u = 0; u < 2 * DC; ++u)
-          kf[x][u] = load_stream(p + (4 * u + t) * 8, tile < seg1 && j < jend && (FULL || 4 * u + t < vecs));
+    // A warp's last round fetches its first tile of the next unit.
+    for (int tile = p.t0 + warp;; tile += NW) {
+      const bool work = tile < p.t1, again = tile + NW < p.t1;
+      if (again) {
+        fetch_at(p, tile + NW);
+      } else {
+        fetch_at(next, next.t0 + warp);
+        if (!more_units) fetch_end = 0;
       }
-    };
-    auto load_v = [&](int tile) {
       int j0, jend;
-      tile_at(tile, j0, jend);
-#pragma unroll
-      for (int x = 0; x < 4; ++x) {
-        const int j = j0 + 2 * t + (x & 1) + (x >> 1) * 8;
-        const T* p = vb + j * a.kv_slot;
-#pragma unroll
-        for (int u = 0; u < DC; ++u)
-          vf[x][u] = load_stream(p + (8 * u + g) * 8, tile < seg1 && j < jend && (FULL || 8 * u + g < vecs));
-      }
-    };
-    // The round before the first only loads (one copy of the loads keeps the code
-    // small: for short calls, fetching instructions is what takes time).
-    for (int tile = seg0 + warp - NW; tile < seg1; tile += NW) {
-      const bool work = tile >= seg0;
-      int j0, jend;
-      tile_at(tile, j0, jend);
+      tile_at(p.rt, tile, j0, jend);
       float s[2][4];
       if (work) {
 #pragma unroll
@@ -257,10 +376,10 @@ __global__ void __launch_bounds__(NT, 1) attn_token_kernel(const __grid_constant
         }
       }
       }
-      load_k(tile + NW);
+      load_k();
       if (work) {
       const bool whole = j0 + TK <= jend &&
-                         (tile < rt.ta || !MULTI || (j0 >= low_last && j0 + TK - 1 <= pos_first));
+                         (tile < p.rt.ta || !MULTI || (j0 >= low_last && j0 + TK - 1 <= pos_first));
 #pragma unroll
       for (int x = 0; x < 2; ++x)
 #pragma unroll
@@ -271,7 +390,7 @@ __global__ void __launch_bounds__(NT, 1) attn_token_kernel(const __grid_constant
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
             const int j = j0 + 8 * x + 2 * t + (k & 1), y = k >> 1;
-            if (j >= jend || !slot_seen(a, rt.start, pos[y], low[y], j)) s[x][k] = -INFINITY;
+            if (j >= jend || !slot_seen(a, p.rt.start, pos[y], low[y], j)) s[x][k] = -INFINITY;
           }
       }
       if (a.scores) {
@@ -303,7 +422,7 @@ __global__ void __launch_bounds__(NT, 1) attn_token_kernel(const __grid_constant
           }
         }
       }
-      uint32_t p[4];
+      uint32_t w16[4];
 #pragma unroll
       for (int y = 0; y < 2; ++y) {
         const float at = ref[y] == -INFINITY ? 0.f : ref[y];
@@ -311,7 +430,7 @@ __global__ void __launch_bounds__(NT, 1) attn_token_kernel(const __grid_constant
         for (int x = 0; x < 2; ++x) {
           const float p0 = ex2(s[x][2 * y] - at), p1 = ex2(s[x][2 * y + 1] - at);
           l[y] += p0 + p1;
-          p[2 * x + y] = Mma<T>::pack(p0, p1);
+          w16[2 * x + y] = Mma<T>::pack(p0, p1);
           if (MULTI) s[x][2 * y] = p0, s[x][2 * y + 1] = p1;
         }
       }
@@ -370,14 +489,15 @@ __global__ void __launch_bounds__(NT, 1) attn_token_kernel(const __grid_constant
         const uint32_t* v3 = reinterpret_cast<const uint32_t*>(&vf[3][u]);
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
-          Mma<T>::run(o[8 * u + 2 * w], p[0], p[1], p[2], p[3], __byte_perm(v0[w], v1[w], 0x5410),
+          Mma<T>::run(o[8 * u + 2 * w], w16[0], w16[1], w16[2], w16[3], __byte_perm(v0[w], v1[w], 0x5410),
                       __byte_perm(v2[w], v3[w], 0x5410));
-          Mma<T>::run(o[8 * u + 2 * w + 1], p[0], p[1], p[2], p[3], __byte_perm(v0[w], v1[w], 0x7632),
+          Mma<T>::run(o[8 * u + 2 * w + 1], w16[0], w16[1], w16[2], w16[3], __byte_perm(v0[w], v1[w], 0x7632),
                       __byte_perm(v2[w], v3[w], 0x7632));
         }
       }
       }
-      load_v(tile + NW);
+      load_v();
+      if (!again) break;
     }
 
     // The warps' results into shared memory.
@@ -386,6 +506,7 @@ __global__ void __launch_bounds__(NT, 1) attn_token_kernel(const __grid_constant
       l[y] += __shfl_xor_sync(0xffffffffu, l[y], 1);
       l[y] += __shfl_xor_sync(0xffffffffu, l[y], 2);
       const int m = g + 8 * y;
+      if (m >= nG) continue;
       if (t == 0) warp_ml[warp][m] = make_float2(ref[y], l[y]);
       float* row = dyn + (warp * 16 + m) * OS;
 #pragma unroll
@@ -399,8 +520,9 @@ __global__ void __launch_bounds__(NT, 1) attn_token_kernel(const __grid_constant
                 make_float4(o[j][2 * y + x], o[j + 1][2 * y + x], o[j + 2][2 * y + x], o[j + 3][2 * y + x]);
           }
     }
+    if (more_units) load_q(next);
     __syncthreads();
-    if (tid < 16) {
+    if (tid < nG) {
       float M = -INFINITY;
 #pragma unroll
       for (int k = 0; k < NW; ++k) M = fmaxf(M, warp_ml[k][tid].x);
@@ -415,18 +537,8 @@ __global__ void __launch_bounds__(NT, 1) attn_token_kernel(const __grid_constant
       joined[tid] = make_float2(M, L);
     }
     __syncthreads();
-
-    const int c_first = block_of(unit_first), parts = block_of(unit_first + rt.tiles - 1) - c_first + 1;
-    const bool direct = parts == 1 && !a.prefix;
-    const int row_vecs = D >> 2;
-    auto write_out = [&](int m, int d, float4 x, float L) {
-      const float inv = L == 0.f ? 0.f : 1.f / L;
-      const int i = MULTI ? m / group : 0;
-      T* out = static_cast<T*>(a.out) + (((int64_t)r * a.n + i) * a.heads + h * group + m - i * group) * D + d;
-      *reinterpret_cast<uint2*>(out) =
-          make_uint2(Mma<T>::pack(x.x * inv, x.y * inv), Mma<T>::pack(x.z * inv, x.w * inv));
-    };
-    const int slot = 2 * c + (seg0 == 0);
+    const bool alone = p.first >= c0 && p.end <= c1, direct = alone && !a.prefix;
+    const int slot = 2 * c + (p.first >= c0);
     for (int x = tid; x < nG * row_vecs; x += NT) {
       const int m = x / row_vecs, d = (x - m * row_vecs) * 4;
       float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -440,102 +552,60 @@ __global__ void __launch_bounds__(NT, 1) attn_token_kernel(const __grid_constant
         v.w = fmaf(y.w, f, v.w);
       }
       if (direct)
-        write_out(m, d, v, joined[m].y);
+        write_out(p, m, d, v, joined[m].y);
       else
         *reinterpret_cast<float4*>(a.part_o + ((int64_t)slot * 16 + m) * D + d) = v;
     }
-    if (direct) {
-      if (a.lse && tid < nG) a.lse[(int64_t)unit * nG + tid] = joined[tid].y == 0.f ? INFINITY : joined[tid].x + log2f(joined[tid].y);
-    } else if (tid < nG) {
-      a.part_ml[slot * 16 + tid] = joined[tid];
+    if (tid < nG) {
+      if (direct)
+        write_lse(p, tid);
+      else
+        a.part_ml[slot * 16 + tid] = joined[tid];
     }
-    if (!direct) {
-      // Joins `count` parts of this unit (and, `last`, the prefix's): part k is block b0 + k * step's.
-      auto slot_of = [&](int b) { return 2 * b + (b == c_first); };
-      auto join = [&](int b0, int step, int count, bool last) {
-        const int more = last ? a.p_splits : 0;
-        auto ml_of = [&](int k, int m) -> float2 {
-          return k < count ? __ldcg(a.part_ml + slot_of(b0 + k * step) * 16 + m)
-                           : __ldcg(a.prefix_ml + (int64_t)(k - count) * all_rows + (int64_t)unit * nG + m);
-        };
-        __syncthreads();
-        if (tid < 16 && tid < nG) {
-          float M = -INFINITY;
-          for (int k = 0; k < count + more; ++k) M = fmaxf(M, ml_of(k, tid).x);
-          const float at = M == -INFINITY ? 0.f : M;
-          float L = 0.f;
-          for (int k = 0; k < count + more; ++k) {
-            const float2 ml = ml_of(k, tid);
-            const float f = ml.y == 0.f ? 0.f : ex2(ml.x - at);
-            factor[k][tid] = f;
-            L = fmaf(ml.y, f, L);
-          }
-          joined[tid] = make_float2(M, L);
-        }
-        __syncthreads();
-        for (int x = tid; x < nG * row_vecs; x += NT) {
-          const int m = x / row_vecs, d = (x - m * row_vecs) * 4;
-          float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-          for (int k = 0; k < count + more; ++k) {
-            const float* src = k < count
-                                   ? a.part_o + ((int64_t)slot_of(b0 + k * step) * 16 + m) * D + d
-                                   : a.prefix_o + ((int64_t)(k - count) * all_rows + (int64_t)unit * nG + m) * D + d;
-            const float4 y = __ldcg(reinterpret_cast<const float4*>(src));
-            const float f = factor[k][m];
-            v.x = fmaf(y.x, f, v.x);
-            v.y = fmaf(y.y, f, v.y);
-            v.z = fmaf(y.z, f, v.z);
-            v.w = fmaf(y.w, f, v.w);
-          }
-          if (last)
-            write_out(m, d, v, joined[m].y);
-          else
-            *reinterpret_cast<float4*>(a.part_o + ((int64_t)slot_of(b0) * 16 + m) * D + d) = v;
-        }
-        if (tid < nG) {
-          if (!last)
-            a.part_ml[slot_of(b0) * 16 + tid] = joined[tid];
-          else if (a.lse)
-            a.lse[(int64_t)unit * nG + tid] = joined[tid].y == 0.f ? INFINITY : joined[tid].x + log2f(joined[tid].y);
-        }
-      };
-      // True in the block that arrives last of `count` at a counter, which it clears.
-      auto arrive = [&](unsigned* counter, int count) {
-        __syncthreads();
-        if (tid == 0) {
-          __threadfence();
-          const bool is_last = atomicAdd(counter, 1u) == (unsigned)count - 1u;
-          if (is_last) *counter = 0u;
-          __threadfence();
-          sh_last = is_last;
-        }
-        __syncthreads();
-        return sh_last != 0;
-      };
-      bool go = true;
-      int step = 1, count = parts;
-      if (parts > kMaxFlat) {
-        const int first = (c - c_first) / kJoin * kJoin, n = min(kJoin, parts - first);
-        go = arrive(a.counters + (int64_t)a.rows * K + slot_of(c_first + first), n);
-        if (go) join(c_first + first, 1, n, false);
-        step = kJoin;
-        count = (parts + kJoin - 1) / kJoin;
-      }
-      if (go && parts > 1) go = arrive(a.counters + unit, count);
-      if (go) join(c_first, step, count, true);
+    if (alone && a.prefix) join(p, c, c, 1, 1, true);
+    if (!alone) shared_part[shared_parts++] = p;
+    if (a.status && tid == 0 && p.h == K - 1 && p.end <= c1) {
+      const int e = a.lengths ? a.lengths[p.r] : a.capacity, s = a.starts ? a.starts[p.r] : 0;
+      a.status[p.r] = (e < 0 || e > a.capacity || s < 0 || s > max(e, 0)) ? 8 : 0;
     }
     __syncthreads();
-    cur = unit_first + seg1;
-    if (seg1 == rt.tiles && ++h == K) {
-      h = 0;
-      if (a.status && tid == 0) {
-        const int e = a.lengths ? a.lengths[r] : a.capacity, s = a.starts ? a.starts[r] : 0;
-        a.status[r] = (e < 0 || e > a.capacity || s < 0 || s > max(e, 0)) ? 8 : 0;
-      }
-      before += rt.tiles;
-      if (++r < a.rows) rt = row_tiles(a, r);
+    if (!more_units) break;
+    p = next;
+  }
+
+  // The block that arrives last at a unit (past kMaxFlat parts: at its group of parts,
+  // then at the unit) joins; both units' arrivals go out together.
+  auto arrives_last = [&](unsigned* counter, int count) {
+    const bool is_last = arrive(counter) == (unsigned)count - 1u;
+    if (is_last) *counter = 0u;
+    return is_last;
+  };
+  __syncthreads();
+  if (tid < shared_parts) {
+    const Part& p = shared_part[tid];
+    const int c_first = block_of(p.first), parts = block_of(p.end - 1) - c_first + 1;
+    const int first = c_first + (c - c_first) / kJoin * kJoin;
+    sh_last[tid] = parts > kMaxFlat ? arrives_last(a.counters + (int64_t)a.rows * K + 2 * first + (first == c_first),
+                                                   min(kJoin, c_first + parts - first))
+                                    : arrives_last(a.counters + p.r * K + p.h, parts);
+  }
+  __syncthreads();
+  for (int x = 0; x < shared_parts; ++x) {
+    if (!sh_last[x]) continue;
+    const Part p = shared_part[x];
+    const int c_first = block_of(p.first), parts = block_of(p.end - 1) - c_first + 1;
+    int step = 1, count = parts;
+    if (parts > kMaxFlat) {
+      const int first = c_first + (c - c_first) / kJoin * kJoin;
+      join(p, c_first, first, 1, min(kJoin, c_first + parts - first), false);
+      step = kJoin;
+      count = (parts + kJoin - 1) / kJoin;
+      __syncthreads();
+      if (tid == 0) sh_last[x] = arrives_last(a.counters + p.r * K + p.h, count);
+      __syncthreads();
+      if (!sh_last[x]) continue;
     }
+    join(p, c_first, c_first, step, count, true);
   }
 }
 
