@@ -9,12 +9,19 @@
 // are read and written: 2 x 2 x moved x head_dim x element bytes per unit, plus 8
 // bytes read and 8 written per slot of weights and positions.
 //
-// Selection is an exact radix select of the B-th largest 32-bit ordered key (four
-// passes of 8 bits over keys kept in shared memory), then one bit per slot and prefix
-// counts per 32-slot word: the k-th survivor and the k-th hole are found by a binary
-// search over the counts, so no list is built.  Several blocks share a unit: each
-// selects for itself (the weights are read from L2) and copies its part of the moves,
-// which needs no exchange between blocks.
+// Selection is exact: the weights become ordered 32-bit keys, kept in shared memory,
+// and the cut (the B-th largest key) is found by narrowing the interval between the
+// smallest and the largest key of the unprotected slots, 1024 equal bins at a time: a
+// count per bin, a scan from the top, the bin that holds the cut is the next interval.
+// It ends when exactly B keys lie at or above a bin's edge (mostly in the second round)
+// or the interval is one key (ties).  Fixed radix digits count worse: most weights share
+// their leading digit, and additions to one bin wait for one another.  Halving the
+// interval took twelve more rounds, each a barrier.  One bit per slot and prefix counts
+// per 32-slot word then number the survivors and the holes, whose lists take the keys'
+// place.  Several blocks share a unit when units are few: each selects for itself (the
+// weights come from L2) and copies its part of the moves, which needs no exchange.
+//
+// Bound by the moved bytes when many slots move, by the selection's latency otherwise.
 #include <cuda_runtime.h>
 
 #include <cstdint>
@@ -23,14 +30,15 @@
 
 namespace {
 
-constexpr int NT = 512;
-constexpr int NW = NT / 32;
-constexpr int kSmemKeys = 32768;  // slots whose keys are kept in shared memory
+constexpr int kBins = 1024;
+constexpr int kSmemKeys = 49152;  // slots whose keys are kept in shared memory
+constexpr uint32_t kTop = 0xff800000u;  // the key of +inf, and of protected slots
 
 struct EvictArgs {
   unsigned char* cache[2];
   int64_t s_layer, s_row, s_head, s_slot;  // bytes
-  int dv;                                  // 16-byte vectors per slot
+  int dv;                                  // 16-byte vectors per slot and tensor
+  int lanes_log2;                          // lanes that copy one slot (keys and values): at most 32
   int rows, heads, capacity, parts;
   const float* weights;  // [layers, rows, heads, capacity]
   const int32_t* positions;
@@ -47,9 +55,9 @@ __device__ __forceinline__ uint32_t ordered(float f) {
 }
 
 __device__ __forceinline__ uint32_t rank_key(float w, int pos, int sinks, int64_t recent_from) {
-  if (pos < sinks || pos >= recent_from) return 0xff800000u;  // +inf
-  if (w != w) return 0x007fffffu;                             // -inf
-  return ordered(w + 0.0f);                                   // -0 ties with +0
+  if (pos < sinks || pos >= recent_from) return kTop;
+  if (w != w) return 0x007fffffu;  // -inf
+  return ordered(w + 0.0f);        // -0 ties with +0
 }
 
 // The position of the k-th (from 0) set bit of the words whose exclusive prefix counts
@@ -64,13 +72,20 @@ __device__ __forceinline__ int select_bit(const int* before, int nw, int k, F wo
   return lo * 32 + (int)__fns(word(lo), 0, k - before[lo] + 1);
 }
 
-template <bool SMEM_KEYS>
-__global__ void __launch_bounds__(NT) kv_evict_kernel(const EvictArgs a) {
+// Bits of word i below / at and past slot B.
+__device__ __forceinline__ uint32_t below_bits(int i, int B) {
+  const int left = B - i * 32;
+  return left >= 32 ? 0xffffffffu : (left <= 0 ? 0u : (1u << left) - 1u);
+}
+
+template <int NT, int PER_SM, bool SMEM_KEYS>
+__global__ void __launch_bounds__(NT, PER_SM) kv_evict_kernel(const EvictArgs a) {
+  constexpr int NW = NT / 32, PER = kBins / NT;  // bins per thread
   extern __shared__ uint32_t dyn[];
-  __shared__ uint32_t hist[256];
-  __shared__ int warp_sum[2][NW];
-  __shared__ int sh_newest, sh_need, carry[2];
-  __shared__ uint32_t sh_prefix;
+  __shared__ int bins[kBins];
+  __shared__ int warp_count[NW], sh_bin, sh_over, sh_need;
+  __shared__ int sh_newest;
+  __shared__ uint32_t sh_low, sh_high;
   const int unit = blockIdx.y, part = blockIdx.x;
   const int h = unit % a.heads, r = (unit / a.heads) % a.rows, layer = unit / (a.heads * a.rows);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -98,147 +113,219 @@ __global__ void __launch_bounds__(NT) kv_evict_kernel(const EvictArgs a) {
   int* comes = holes + nw + 1;
   uint32_t* keys = reinterpret_cast<uint32_t*>(comes + nw + 1);
 
-  // Newest position, then the ranks.
+  // Newest position, then the keys and their range (protected ones left out).
+  if (tid == 0) {
+    sh_newest = INT32_MIN;
+    sh_low = 0xffffffffu;
+    sh_high = 0u;
+  }
   int newest = INT32_MIN;
+#pragma unroll 4
   for (int j = tid; j < n; j += NT) newest = max(newest, pos[j]);
   newest = __reduce_max_sync(0xffffffffu, newest);
-  if (tid == 0) sh_newest = INT32_MIN;
   __syncthreads();
   if (lane == 0) atomicMax(&sh_newest, newest);
   __syncthreads();
   const int64_t from = (int64_t)sh_newest - a.recent + 1;
-  if (SMEM_KEYS)
-    for (int j = tid; j < n; j += NT) keys[j] = rank_key(w[j], pos[j], a.sinks, from);
   auto key = [&](int j) { return SMEM_KEYS ? keys[j] : rank_key(w[j], pos[j], a.sinks, from); };
-
-  // Radix select of the B-th largest key.
-  if (tid == 0) {
-    sh_prefix = 0;
-    sh_need = B;
-  }
-  for (int shift = 24; shift >= 0; shift -= 8) {
-    for (int i = tid; i < 256; i += NT) hist[i] = 0;
-    __syncthreads();
-    const uint32_t prefix = sh_prefix;
-    const uint32_t high = shift == 24 ? 0u : 0xffffffffu << (shift + 8);
-    for (int j = tid; j < n; j += NT) {
-      const uint32_t k = key(j);
-      if ((k & high) == prefix) atomicAdd(&hist[(k >> shift) & 255u], 1u);
+  uint32_t low = 0xffffffffu, high = 0u;
+#pragma unroll 4
+  for (int j = tid; j < n; j += NT) {
+    const uint32_t k = rank_key(w[j], pos[j], a.sinks, from);
+    if (SMEM_KEYS) keys[j] = k;
+    if (k < kTop) {
+      low = min(low, k);
+      high = max(high, k);
     }
-    __syncthreads();
-    if (warp == 0) {
-      // Lane l holds bins 255 - 8 l down to 248 - 8 l.
-      int c[8], sum = 0;
+  }
+  low = __reduce_min_sync(0xffffffffu, low);
+  high = __reduce_max_sync(0xffffffffu, high);
+  if (lane == 0) {
+    atomicMin(&sh_low, low);
+    atomicMax(&sh_high, high);
+  }
+  __syncthreads();
+  // cut, next: what lies at next and above stays (`above` slots), and of the slots in
+  // [cut, next) all (exact) or, all being equal, the first `ties`.
+  uint32_t cut = kTop, next = kTop + 1u;
+  int above = 0;
+  bool exact = false;
+  if (sh_low <= sh_high) {  // some slot is not protected
+    // Keys in [lo, hi]; above that, `over` ones (at first the protected, which bin kBins - 1 takes up).
+    uint32_t lo = sh_low, hi = sh_high;
+    int over = 0;
+    for (bool first = true;; first = false) {
+      // Bin width: the smallest power of two that covers the interval.
+      const uint32_t span = hi - lo;
+      const int shift = span < kBins ? 0 : 32 - __clz(span) - 10;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) sum += c[i] = (int)hist[255 - 8 * lane - i];
-      int incl = sum;
+      for (int i = 0; i < PER; ++i) bins[tid + i * NT] = 0;
+      int top = 0;
+      __syncthreads();
+      for (int j = tid; j < n; j += NT) {
+        const uint32_t k = key(j);
+        if (first && k > hi) ++top;
+        if (k >= lo && k <= hi) atomicAdd(&bins[(k - lo) >> shift], 1);
+      }
+      if (first) {
+        top = __reduce_add_sync(0xffffffffu, top);
+        if (lane == 0) warp_count[warp] = top;
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < NW; ++i) over += warp_count[i];
+      }
+      __syncthreads();
+      if (over >= B) break;  // the protected alone fill the budget: only in the first round
+      // Scan from the top: thread x holds bins kBins - 1 - PER x and below.
+      int c[PER], sum = 0;
+#pragma unroll
+      for (int i = 0; i < PER; ++i) sum += c[i] = bins[kBins - 1 - PER * tid - i];
+      int upto = sum;
 #pragma unroll
       for (int k = 1; k < 32; k <<= 1) {
-        const int x = __shfl_up_sync(0xffffffffu, incl, k);
-        if (lane >= k) incl += x;
+        const int x = __shfl_up_sync(0xffffffffu, upto, k);
+        if (lane >= k) upto += x;
       }
-      const int need = sh_need;
-      int above = incl - sum;
-      if (above < need && need <= incl) {
+      if (lane == 31) warp_count[warp] = upto;
+      __syncthreads();
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          if (above < need && need <= above + c[i]) {
-            sh_prefix = prefix | ((uint32_t)(255 - 8 * lane - i) << shift);
-            sh_need = need - above;
-            above = need;  // found
-          } else {
-            above += c[i];
+      for (int i = 0; i < NW; ++i)
+        if (i < warp) upto += warp_count[i];
+      int at = over + upto - sum;
+      if (at < B && B <= at + sum) {
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+          if (at < B && B <= at + c[i]) {
+            sh_bin = kBins - 1 - PER * tid - i;
+            sh_over = at;
+            sh_need = c[i];
           }
+          at += c[i];
         }
       }
+      __syncthreads();
+      const uint32_t edge = lo + ((uint32_t)sh_bin << shift);
+      const int in_bin = sh_need;
+      over = sh_over;
+      if (over + in_bin == B || shift == 0) {
+        exact = over + in_bin == B;
+        cut = edge;
+        next = exact ? hi : edge + 1u;
+        above = over;
+        break;
+      }
+      hi = min(hi, edge + (1u << shift) - 1u);
+      lo = edge;
+      __syncthreads();
     }
-    __syncthreads();
   }
-  const uint32_t cut = sh_prefix;
-  const int ties = sh_need;  // of the slots at the cut, the first `ties` stay
+  const int ties = B - above;
 
-  // One bit per slot and the prefix counts, 32 x NW slots at a time.
-  if (tid == 0) carry[0] = carry[1] = 0;
-  int tie_base = 0;
-  for (int w0 = 0; w0 < nw; w0 += NW) {
-    const int word = w0 + warp, j = word * 32 + lane;
+  // One bit per slot.
+  for (int i = warp; i < nw; i += NW) {
+    const int j = i * 32 + lane;
     const uint32_t k = j < n ? key(j) : 0u;
-    const unsigned eq = __ballot_sync(0xffffffffu, j < n && k == cut);
-    const unsigned gt = __ballot_sync(0xffffffffu, j < n && k > cut);
-    if (lane == 0) warp_sum[0][warp] = __popc(eq);
-    __syncthreads();
-    int before = tie_base, all = 0;
-#pragma unroll
-    for (int i = 0; i < NW; ++i) {
-      const int c = warp_sum[0][i];
-      if (i < warp) before += c;
-      all += c;
+    const unsigned at = __ballot_sync(0xffffffffu, j < n && k >= cut);
+    const unsigned over = __ballot_sync(0xffffffffu, j < n && k >= next);
+    if (lane == 0) {
+      kept[i] = exact ? at : over;
+      if (!exact) holes[i] = (int)(at & ~over);  // the ties, resolved next
     }
-    tie_base += all;
-    const bool stays = (gt >> lane & 1u) ||
-                       ((eq >> lane & 1u) && before + __popc(eq & ((1u << lane) - 1u)) < ties);
-    const unsigned bits = __ballot_sync(0xffffffffu, stays);
-    if (lane == 0 && word < nw) kept[word] = bits;
-    __syncthreads();
   }
-  auto hole_bits = [&](int i) {
-    const int left = B - i * 32;
-    const uint32_t below = left >= 32 ? 0xffffffffu : (left <= 0 ? 0u : (1u << left) - 1u);
-    return ~kept[i] & below;
-  };
-  auto come_bits = [&](int i) {
-    const int left = B - i * 32;
-    const uint32_t below = left >= 32 ? 0xffffffffu : (left <= 0 ? 0u : (1u << left) - 1u);
-    return kept[i] & ~below;
-  };
-  for (int w0 = 0; w0 < nw; w0 += NT) {
-    const int i = w0 + tid;
-    const int c0 = i < nw ? __popc(hole_bits(i)) : 0, c1 = i < nw ? __popc(come_bits(i)) : 0;
-    int s0 = c0, s1 = c1;
+  __syncthreads();
+  if (warp == 0) {
+    int tied = 0, nh = 0, nc = 0;
+    for (int i0 = 0; i0 < nw; i0 += 32) {
+      const int i = i0 + lane;
+      uint32_t bits = i < nw ? kept[i] : 0u;
+      if (!exact) {
+        uint32_t eq = i < nw ? (uint32_t)holes[i] : 0u;
+        const int c = __popc(eq);
+        int s = c;
 #pragma unroll
-    for (int k = 1; k < 32; k <<= 1) {
-      const int x = __shfl_up_sync(0xffffffffu, s0, k), y = __shfl_up_sync(0xffffffffu, s1, k);
-      if (lane >= k) s0 += x, s1 += y;
+        for (int k = 1; k < 32; k <<= 1) {
+          const int x = __shfl_up_sync(0xffffffffu, s, k);
+          if (lane >= k) s += x;
+        }
+        int room = ties - (tied + s - c);
+        tied += __shfl_sync(0xffffffffu, s, 31);
+        if (room >= c) {
+          bits |= eq;
+        } else {
+          for (; room > 0; --room) {
+            bits |= eq & (0u - eq);
+            eq &= eq - 1u;
+          }
+        }
+        if (i < nw) kept[i] = bits;
+      }
+      const uint32_t below = below_bits(i, B);
+      const int c0 = i < nw ? __popc(~bits & below) : 0, c1 = i < nw ? __popc(bits & ~below) : 0;
+      int s = c0 | c1 << 16;  // 32 words hold 1024 slots at most
+#pragma unroll
+      for (int k = 1; k < 32; k <<= 1) {
+        const int x = __shfl_up_sync(0xffffffffu, s, k);
+        if (lane >= k) s += x;
+      }
+      if (i < nw) {
+        holes[i] = nh + (s & 0xffff) - c0;
+        comes[i] = nc + (s >> 16) - c1;
+      }
+      s = __shfl_sync(0xffffffffu, s, 31);
+      nh += s & 0xffff;
+      nc += s >> 16;
     }
-    if (lane == 31) warp_sum[0][warp] = s0, warp_sum[1][warp] = s1;
-    __syncthreads();
-    int b0 = carry[0], b1 = carry[1];
-    for (int k = 0; k < warp; ++k) b0 += warp_sum[0][k], b1 += warp_sum[1][k];
-    if (i < nw) holes[i] = b0 + s0 - c0, comes[i] = b1 + s1 - c1;
-    __syncthreads();
-    if (tid == NT - 1) carry[0] = b0 + s0, carry[1] = b1 + s1;
-    __syncthreads();
+    if (lane == 0) holes[nw] = nh, comes[nw] = nc;
   }
-  if (tid == 0) holes[nw] = carry[0], comes[nw] = carry[1];
   __syncthreads();
   const int moved = comes[nw];
-
-  // Weights and positions.
-  for (int j = part * NT + tid; j < a.capacity; j += a.parts * NT) {
-    float x = 0.f;
-    int p = -1;
-    if (j < B) {
-      int from_slot = j;
-      const uint32_t hb = hole_bits(j >> 5);
-      if (hb >> (j & 31) & 1u)
-        from_slot = select_bit(comes, nw, holes[j >> 5] + __popc(hb & ((1u << (j & 31)) - 1u)), come_bits);
-      x = w[from_slot];
-      p = pos[from_slot];
+  auto hole_bits = [&](int i) { return ~kept[i] & below_bits(i, B); };
+  auto come_bits = [&](int i) { return kept[i] & ~below_bits(i, B); };
+  // The lists of survivors past the budget and of holes below it, over the keys (at most
+  // n / 2 entries each).
+  int *src_list = reinterpret_cast<int*>(keys), *dst_list = src_list + moved;
+  if (SMEM_KEYS) {
+    for (int i = warp; i < nw; i += NW) {
+      const uint32_t hb = hole_bits(i), cb = come_bits(i), under = (1u << lane) - 1u;
+      if (hb >> lane & 1u) dst_list[holes[i] + __popc(hb & under)] = i * 32 + lane;
+      if (cb >> lane & 1u) src_list[comes[i] + __popc(cb & under)] = i * 32 + lane;
     }
-    wo[j] = x;
-    po[j] = p;
+    __syncthreads();
   }
-  // Keys and values: one warp per moved slot.
+  auto src_of = [&](int k) { return SMEM_KEYS ? src_list[k] : select_bit(comes, nw, k, come_bits); };
+  auto dst_of = [&](int k) { return SMEM_KEYS ? dst_list[k] : select_bit(holes, nw, k, hole_bits); };
+
+  // Keys and values: a group of lanes per moved slot, four slots in flight.
   const int64_t base = layer * a.s_layer + r * a.s_row + h * a.s_head;
-  for (int k = part * NW + warp; k < moved; k += a.parts * NW) {
-    const int64_t src = base + select_bit(comes, nw, k, come_bits) * a.s_slot;
-    const int64_t dst = base + select_bit(holes, nw, k, hole_bits) * a.s_slot;
-    for (int x = lane; x < 2 * a.dv; x += 32) {
-      const int c = x >= a.dv, v = c ? x - a.dv : x;
-      if (a.cache[c])
-        *reinterpret_cast<uint4*>(a.cache[c] + dst + v * 16) =
-            *reinterpret_cast<const uint4*>(a.cache[c] + src + v * 16);
+  const int vecs = a.cache[1] ? 2 * a.dv : a.dv, group = 1 << a.lanes_log2;
+  const int groups = (a.parts * NT) >> a.lanes_log2, me = (part * NT + tid) >> a.lanes_log2;
+  for (int e = tid & (group - 1); e < vecs; e += group) {
+    unsigned char* cache = (e >= a.dv ? a.cache[1] + (e - a.dv) * 16 : a.cache[0] + e * 16) + base;
+    for (int k0 = me; k0 < moved; k0 += 4 * groups) {
+      uint4 v[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        if (k0 + u * groups < moved)
+          v[u] = *reinterpret_cast<const uint4*>(cache + src_of(k0 + u * groups) * a.s_slot);
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        if (k0 + u * groups < moved) *reinterpret_cast<uint4*>(cache + dst_of(k0 + u * groups) * a.s_slot) = v[u];
     }
+  }
+  // Weights and positions: the slots that stay and the empty ones, then the moved.
+  for (int j = part * NT + tid; j < a.capacity; j += a.parts * NT) {
+    if (j >= B) {
+      wo[j] = 0.f;
+      po[j] = -1;
+    } else if (kept[j >> 5] >> (j & 31) & 1u) {
+      wo[j] = w[j];
+      po[j] = pos[j];
+    }
+  }
+  for (int k = part * NT + tid; k < moved; k += a.parts * NT) {
+    const int src = src_of(k), dst = dst_of(k);
+    wo[dst] = w[src];
+    po[dst] = pos[src];
   }
 }
 
@@ -260,6 +347,7 @@ extern "C" int sv_kv_evict(void* keys, void* values, int32_t elem_bytes, int32_t
   const int64_t row = (int64_t)head_dim * elem_bytes;
   const int64_t sb[4] = {stride_layer * elem_bytes, stride_row * elem_bytes, stride_head * elem_bytes,
                          stride_slot * elem_bytes};
+  if (row > 16384) return SV_E_SHAPE;
   if (row % 16) return SV_E_ALIGN;
   for (int k = 0; k < 4; ++k)
     if (sb[k] % 16 || sb[k] < 0) return SV_E_ALIGN;
@@ -286,15 +374,22 @@ extern "C" int sv_kv_evict(void* keys, void* values, int32_t elem_bytes, int32_t
   a.lengths_out = lengths_out;
   a.status = out_status;
   const int units = layers * rows * heads;
-  a.parts = units >= 592 ? 1 : (592 + units - 1) / units;
+  a.lanes_log2 = 0;
+  while (a.lanes_log2 < 5 && (1 << a.lanes_log2) < (values ? 2 : 1) * a.dv) ++a.lanes_log2;
+  // Many units: small blocks, seven per SM, overlap one another's phases (256 threads 66 us, 512 72 us,
+  // 1024 110 us at 1024 units of about 2200 slots, before the bins).  Few: large blocks, about two per SM
+  // in all, since each selects anew.
+  const bool many = units >= 296;
+  a.parts = many ? 1 : 296 / units;
   if (a.parts > 16) a.parts = 16;
   const bool in_smem = capacity <= kSmemKeys;
   const size_t nw = (capacity + 31) / 32;
   const size_t smem = 4 * (3 * nw + 2 + (in_smem ? capacity : 0));
-  auto kernel = in_smem ? kv_evict_kernel<true> : kv_evict_kernel<false>;
-  if (smem > 48 * 1024 &&
+  auto kernel = many ? (in_smem ? kv_evict_kernel<256, 7, true> : kv_evict_kernel<256, 7, false>)
+                     : (in_smem ? kv_evict_kernel<1024, 1, true> : kv_evict_kernel<1024, 1, false>);
+  if (smem > 40 * 1024 &&
       cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
     return SV_E_CUDA;
-  kernel<<<dim3(a.parts, units), NT, smem, static_cast<cudaStream_t>(stream)>>>(a);
+  kernel<<<dim3(a.parts, units), many ? 256 : 1024, smem, static_cast<cudaStream_t>(stream)>>>(a);
   return cudaGetLastError() == cudaSuccess ? SV_OK : SV_E_CUDA;
 }

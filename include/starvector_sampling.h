@@ -464,8 +464,8 @@ int sv_prefix_attention(const void* q, int32_t dtype, int32_t rows, int32_t toke
  *   lengths_out  int32 [rows] or NULL: min(length, budget)
  *   out_status   int32 [rows] or NULL: SV_ST_LENGTH for a length outside [0, capacity]
  * 1 <= budget <= capacity <= 2^20; sinks + recent <= budget; layers * rows * heads <=
- * 65535; head_dim * elem_bytes, the strides in bytes and the cache pointers multiples
- * of 16.
+ * 65535; head_dim * elem_bytes at most 16384 and, like the strides in bytes and the
+ * cache pointers, a multiple of 16.
  */
 int sv_kv_evict(void* keys, void* values, int32_t elem_bytes, int32_t layers, int32_t rows, int32_t heads,
                 int32_t capacity, int32_t head_dim, int64_t stride_layer, int64_t stride_row, int64_t stride_head,
