@@ -31,7 +31,7 @@
 namespace {
 
 constexpr int kBins = 1024;
-constexpr int kSmemKeys = 49152;  // slots whose keys are kept in shared memory
+constexpr int kSmemKeys = 24576;  // slots whose keys and positions are kept in shared memory
 constexpr uint32_t kTop = 0xff800000u;  // the key of +inf, and of protected slots
 
 struct EvictArgs {
@@ -54,8 +54,8 @@ __device__ __forceinline__ uint32_t ordered(float f) {
   return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
 }
 
-__device__ __forceinline__ uint32_t rank_key(float w, int pos, int sinks, int64_t recent_from) {
-  if (pos < sinks || pos >= recent_from) return kTop;
+__device__ __forceinline__ uint32_t rank_key(float w, int pos, int sinks, int recent_from) {
+  if (pos < sinks || pos > recent_from) return kTop;
   if (w != w) return 0x007fffffu;  // -inf
   return ordered(w + 0.0f);        // -0 ties with +0
 }
@@ -70,6 +70,19 @@ __device__ __forceinline__ int select_bit(const int* before, int nw, int k, F wo
     if (before[mid] <= k) lo = mid; else hi = mid;
   }
   return lo * 32 + (int)__fns(word(lo), 0, k - before[lo] + 1);
+}
+
+// Four consecutive values from j on (fill past n); vec: the four can be read at once.
+template <typename V, typename E> __device__ __forceinline__ void load4(const E* p, int j, int n, bool vec, E fill, E (&x)[4]) {
+  if (vec) {
+    const V v = *reinterpret_cast<const V*>(p + j);
+    x[0] = v.x, x[1] = v.y, x[2] = v.z, x[3] = v.w;
+  }
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    if (!vec) x[k] = j + k < n ? p[j + k] : fill;
+    if (j + k >= n) x[k] = fill;
+  }
 }
 
 // Bits of word i below / at and past slot B.
@@ -100,18 +113,43 @@ __global__ void __launch_bounds__(NT, PER_SM) kv_evict_kernel(const EvictArgs a)
     if (a.lengths_out) a.lengths_out[r] = keep;
     if (a.status) a.status[r] = raw == n ? 0 : SV_ST_LENGTH;
   }
-  if (n <= B) {
-    for (int j = part * NT + tid; j < a.capacity; j += a.parts * NT) {
-      wo[j] = j < n ? w[j] : 0.f;
-      po[j] = j < n ? pos[j] : -1;
+  // Weights and positions are read and written four slots at a time where units start
+  // 16-byte aligned; each block writes the slots [slot0, slot1).
+  const bool vec = !(a.capacity & 3) && !(((uintptr_t)a.weights | (uintptr_t)a.positions | (uintptr_t)a.weights_out |
+                                           (uintptr_t)a.positions_out) & 15);
+  const int per_part = ((a.capacity + a.parts - 1) / a.parts + 3) & ~3;
+  const int slot0 = min(part * per_part, a.capacity), slot1 = min(slot0 + per_part, a.capacity);
+  // Each slot's own weight and position go out as they are read; the moved follow at the end.
+  auto write4 = [&](int j, const float (&x)[4], const int (&y)[4]) {
+    if (vec) {
+      *reinterpret_cast<float4*>(wo + j) = make_float4(x[0], x[1], x[2], x[3]);
+      *reinterpret_cast<int4*>(po + j) = make_int4(y[0], y[1], y[2], y[3]);
+    } else {
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (j + k < slot1) wo[j + k] = x[k], po[j + k] = y[k];
     }
+  };
+  auto copy_meta = [&](int from) {
+#pragma unroll 2
+    for (int j = max(slot0, from) + 4 * tid; j < slot1; j += 4 * NT) {
+      float x[4];
+      int y[4];
+      load4<float4>(w, j, keep, vec, 0.f, x);
+      load4<int4>(pos, j, keep, vec, -1, y);
+      write4(j, x, y);
+    }
+  };
+  if (n <= B) {
+    copy_meta(0);
     return;
   }
-  const int nw = (n + 31) >> 5;
-  uint32_t* kept = dyn;                                    // one bit per slot
+  const int nw = (n + 31) >> 5, n4 = (n + 3) & ~3;
+  uint32_t* keys = dyn;                                    // [n4], later the lists of moves
+  int* held = reinterpret_cast<int*>(keys + (SMEM_KEYS ? n4 : 0));  // [n4] positions
+  uint32_t* kept = reinterpret_cast<uint32_t*>(held + (SMEM_KEYS ? n4 : 0));  // one bit per slot
   int* holes = reinterpret_cast<int*>(kept + nw);          // exclusive counts per word, nw + 1
   int* comes = holes + nw + 1;
-  uint32_t* keys = reinterpret_cast<uint32_t*>(comes + nw + 1);
 
   // Newest position, then the keys and their range (protected ones left out).
   if (tid == 0) {
@@ -120,23 +158,62 @@ __global__ void __launch_bounds__(NT, PER_SM) kv_evict_kernel(const EvictArgs a)
     sh_high = 0u;
   }
   int newest = INT32_MIN;
-#pragma unroll 4
-  for (int j = tid; j < n; j += NT) newest = max(newest, pos[j]);
+  if (SMEM_KEYS) {
+#pragma unroll 2
+    for (int j = 4 * tid; j < n; j += 4 * NT) {
+      float x[4];
+      int y[4];
+      load4<float4>(w, j, n, vec, 0.f, x);
+      load4<int4>(pos, j, n, vec, INT32_MIN, y);
+      newest = max(max(max(newest, y[0]), max(y[1], y[2])), y[3]);
+      *reinterpret_cast<float4*>(keys + j) = make_float4(x[0], x[1], x[2], x[3]);
+      *reinterpret_cast<int4*>(held + j) = make_int4(y[0], y[1], y[2], y[3]);
+      if (j >= slot0 && j < slot1) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          if (j + k >= B) x[k] = 0.f, y[k] = -1;
+        write4(j, x, y);
+      }
+    }
+    copy_meta(n4);
+  } else {
+    for (int j = tid; j < n; j += NT) newest = max(newest, pos[j]);
+    copy_meta(0);
+  }
   newest = __reduce_max_sync(0xffffffffu, newest);
   __syncthreads();
   if (lane == 0) atomicMax(&sh_newest, newest);
   __syncthreads();
-  const int64_t from = (int64_t)sh_newest - a.recent + 1;
-  auto key = [&](int j) { return SMEM_KEYS ? keys[j] : rank_key(w[j], pos[j], a.sinks, from); };
+  // Positions above `from` are recent (none when recent is 0; all when that would lie below the type's range).
+  const int64_t from64 = (int64_t)sh_newest - a.recent;
+  const int from = (int)max(from64, (int64_t)INT32_MIN);
+  const bool all_recent = from64 < INT32_MIN;
+  auto make_key = [&](float x, int p) { return all_recent ? kTop : rank_key(x, p, a.sinks, from); };
+  auto key = [&](int j) { return SMEM_KEYS ? keys[j] : make_key(w[j], pos[j]); };
   uint32_t low = 0xffffffffu, high = 0u;
-#pragma unroll 4
-  for (int j = tid; j < n; j += NT) {
-    const uint32_t k = rank_key(w[j], pos[j], a.sinks, from);
-    if (SMEM_KEYS) keys[j] = k;
+  auto widen = [&](uint32_t k) {
     if (k < kTop) {
       low = min(low, k);
       high = max(high, k);
     }
+  };
+  if (SMEM_KEYS) {
+    for (int j = 4 * tid; j < n; j += 4 * NT) {  // each thread's own four
+      const float4 x = *reinterpret_cast<const float4*>(keys + j);
+      const int4 y = *reinterpret_cast<const int4*>(held + j);
+      uint4 k;
+      k.x = make_key(x.x, y.x);
+      widen(k.x);
+      k.y = j + 1 < n ? make_key(x.y, y.y) : 0u;  // 0: below every slot's key
+      if (j + 1 < n) widen(k.y);
+      k.z = j + 2 < n ? make_key(x.z, y.z) : 0u;
+      if (j + 2 < n) widen(k.z);
+      k.w = j + 3 < n ? make_key(x.w, y.w) : 0u;
+      if (j + 3 < n) widen(k.w);
+      *reinterpret_cast<uint4*>(keys + j) = k;
+    }
+  } else {
+    for (int j = tid; j < n; j += NT) widen(make_key(w[j], pos[j]));
   }
   low = __reduce_min_sync(0xffffffffu, low);
   high = __reduce_max_sync(0xffffffffu, high);
@@ -162,10 +239,17 @@ __global__ void __launch_bounds__(NT, PER_SM) kv_evict_kernel(const EvictArgs a)
       for (int i = 0; i < PER; ++i) bins[tid + i * NT] = 0;
       int top = 0;
       __syncthreads();
-      for (int j = tid; j < n; j += NT) {
-        const uint32_t k = key(j);
-        if (first && k > hi) ++top;
+      auto put = [&](uint32_t k) {
+        top += k > hi;
         if (k >= lo && k <= hi) atomicAdd(&bins[(k - lo) >> shift], 1);
+      };
+      if (SMEM_KEYS) {
+        for (int j = 4 * tid; j < n; j += 4 * NT) {
+          const uint4 k = *reinterpret_cast<const uint4*>(keys + j);
+          put(k.x), put(k.y), put(k.z), put(k.w);
+        }
+      } else {
+        for (int j = tid; j < n; j += NT) put(key(j));
       }
       if (first) {
         top = __reduce_add_sync(0xffffffffu, top);
@@ -221,25 +305,35 @@ __global__ void __launch_bounds__(NT, PER_SM) kv_evict_kernel(const EvictArgs a)
   }
   const int ties = B - above;
 
-  // One bit per slot.
-  for (int i = warp; i < nw; i += NW) {
-    const int j = i * 32 + lane;
-    const uint32_t k = j < n ? key(j) : 0u;
-    const unsigned at = __ballot_sync(0xffffffffu, j < n && k >= cut);
-    const unsigned over = __ballot_sync(0xffffffffu, j < n && k >= next);
-    if (lane == 0) {
+  // One bit per slot: a thread compares four, eight threads make a word.
+  for (int i0 = 0; i0 < nw; i0 += NT / 8) {
+    const int i = i0 + (tid >> 3), j = i * 32 + (tid & 7) * 4;
+    uint32_t at = 0, over = 0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const uint32_t k = j + e < n ? key(j + e) : 0u;
+      at |= (uint32_t)(k >= cut) << e;
+      over |= (uint32_t)(k >= next) << e;
+    }
+    at <<= (tid & 7) * 4;
+    over <<= (tid & 7) * 4;
+#pragma unroll
+    for (int k = 1; k < 8; k <<= 1) {
+      at |= __shfl_xor_sync(0xffffffffu, at, k);
+      over |= __shfl_xor_sync(0xffffffffu, over, k);
+    }
+    if (!(tid & 7) && i < nw) {
       kept[i] = exact ? at : over;
       if (!exact) holes[i] = (int)(at & ~over);  // the ties, resolved next
     }
   }
   __syncthreads();
-  if (warp == 0) {
-    int tied = 0, nh = 0, nc = 0;
-    for (int i0 = 0; i0 < nw; i0 += 32) {
-      const int i = i0 + lane;
-      uint32_t bits = i < nw ? kept[i] : 0u;
-      if (!exact) {
-        uint32_t eq = i < nw ? (uint32_t)holes[i] : 0u;
+  if (!exact) {
+    if (warp == 0) {
+      int tied = 0;
+      for (int i0 = 0; i0 < nw && tied < ties; i0 += 32) {
+        const int i = i0 + lane;
+        uint32_t eq = i < nw ? (uint32_t)holes[i] : 0u, bits = 0u;
         const int c = __popc(eq);
         int s = c;
 #pragma unroll
@@ -250,45 +344,64 @@ __global__ void __launch_bounds__(NT, PER_SM) kv_evict_kernel(const EvictArgs a)
         int room = ties - (tied + s - c);
         tied += __shfl_sync(0xffffffffu, s, 31);
         if (room >= c) {
-          bits |= eq;
+          bits = eq;
         } else {
           for (; room > 0; --room) {
             bits |= eq & (0u - eq);
             eq &= eq - 1u;
           }
         }
-        if (i < nw) kept[i] = bits;
+        if (i < nw) kept[i] |= bits;
       }
-      const uint32_t below = below_bits(i, B);
-      const int c0 = i < nw ? __popc(~bits & below) : 0, c1 = i < nw ? __popc(bits & ~below) : 0;
-      int s = c0 | c1 << 16;  // 32 words hold 1024 slots at most
-#pragma unroll
-      for (int k = 1; k < 32; k <<= 1) {
-        const int x = __shfl_up_sync(0xffffffffu, s, k);
-        if (lane >= k) s += x;
-      }
-      if (i < nw) {
-        holes[i] = nh + (s & 0xffff) - c0;
-        comes[i] = nc + (s >> 16) - c1;
-      }
-      s = __shfl_sync(0xffffffffu, s, 31);
-      nh += s & 0xffff;
-      nc += s >> 16;
     }
-    if (lane == 0) holes[nw] = nh, comes[nw] = nc;
+    __syncthreads();
   }
+  // Exclusive counts per word, a word per thread (both counts in one value: NT words hold
+  // at most 32 NT = 2^15 slots).
+  int nh = 0, nc = 0;
+  for (int i0 = 0; i0 < nw; i0 += NT) {
+    const int i = i0 + tid;
+    const uint32_t bits = i < nw ? kept[i] : 0u, below = below_bits(i, B);
+    const uint32_t c = i < nw ? (uint32_t)__popc(~bits & below) | (uint32_t)__popc(bits & ~below) << 16 : 0u;
+    uint32_t s = c;
+#pragma unroll
+    for (int k = 1; k < 32; k <<= 1) {
+      const uint32_t x = __shfl_up_sync(0xffffffffu, s, k);
+      if (lane >= k) s += x;
+    }
+    if (lane == 31) warp_count[warp] = (int)s;
+    __syncthreads();
+    uint32_t all = 0;
+#pragma unroll
+    for (int k = 0; k < NW; ++k) {
+      if (k == warp) s += all;
+      all += (uint32_t)warp_count[k];
+    }
+    s -= c;
+    if (i < nw) {
+      holes[i] = nh + (int)(s & 0xffffu);
+      comes[i] = nc + (int)(s >> 16);
+    }
+    nh += (int)(all & 0xffffu);
+    nc += (int)(all >> 16);
+    __syncthreads();
+  }
+  if (tid == 0) holes[nw] = nh, comes[nw] = nc;
   __syncthreads();
   const int moved = comes[nw];
   auto hole_bits = [&](int i) { return ~kept[i] & below_bits(i, B); };
   auto come_bits = [&](int i) { return kept[i] & ~below_bits(i, B); };
   // The lists of survivors past the budget and of holes below it, over the keys (at most
-  // n / 2 entries each).
+  // n / 2 entries each).  Holes are few per word: a thread lists a word's.
   int *src_list = reinterpret_cast<int*>(keys), *dst_list = src_list + moved;
   if (SMEM_KEYS) {
-    for (int i = warp; i < nw; i += NW) {
-      const uint32_t hb = hole_bits(i), cb = come_bits(i), under = (1u << lane) - 1u;
-      if (hb >> lane & 1u) dst_list[holes[i] + __popc(hb & under)] = i * 32 + lane;
-      if (cb >> lane & 1u) src_list[comes[i] + __popc(cb & under)] = i * 32 + lane;
+    for (int i = tid; i < nw && i * 32 < B; i += NT) {
+      int at = holes[i];
+      for (uint32_t hb = hole_bits(i); hb; hb &= hb - 1u) dst_list[at++] = i * 32 + __ffs(hb) - 1;
+    }
+    for (int i = (B >> 5) + warp; i < nw; i += NW) {
+      const uint32_t cb = come_bits(i);
+      if (cb >> lane & 1u) src_list[comes[i] + __popc(cb & ((1u << lane) - 1u))] = i * 32 + lane;
     }
     __syncthreads();
   }
@@ -312,20 +425,13 @@ __global__ void __launch_bounds__(NT, PER_SM) kv_evict_kernel(const EvictArgs a)
         if (k0 + u * groups < moved) *reinterpret_cast<uint4*>(cache + dst_of(k0 + u * groups) * a.s_slot) = v[u];
     }
   }
-  // Weights and positions: the slots that stay and the empty ones, then the moved.
-  for (int j = part * NT + tid; j < a.capacity; j += a.parts * NT) {
-    if (j >= B) {
-      wo[j] = 0.f;
-      po[j] = -1;
-    } else if (kept[j >> 5] >> (j & 31) & 1u) {
-      wo[j] = w[j];
-      po[j] = pos[j];
-    }
-  }
-  for (int k = part * NT + tid; k < moved; k += a.parts * NT) {
-    const int src = src_of(k), dst = dst_of(k);
+  // Weights and positions of the moved (their places were written long ago by this block, barriers before).
+  for (int k = tid; k < moved; k += NT) {
+    const int dst = dst_of(k);
+    if (dst < slot0 || dst >= slot1) continue;
+    const int src = src_of(k);
     wo[dst] = w[src];
-    po[dst] = pos[src];
+    po[dst] = SMEM_KEYS ? held[src] : pos[src];
   }
 }
 
@@ -376,15 +482,15 @@ extern "C" int sv_kv_evict(void* keys, void* values, int32_t elem_bytes, int32_t
   const int units = layers * rows * heads;
   a.lanes_log2 = 0;
   while (a.lanes_log2 < 5 && (1 << a.lanes_log2) < (values ? 2 : 1) * a.dv) ++a.lanes_log2;
-  // Many units: small blocks, seven per SM, overlap one another's phases (256 threads 66 us, 512 72 us,
-  // 1024 110 us at 1024 units of about 2200 slots, before the bins).  Few: large blocks, about two per SM
-  // in all, since each selects anew.
+  // Many units: blocks of 256 threads, up to seven per SM (three to seven take the same time: 44.6-45.5 us
+  // at 1024 units of about 2200 slots).  Few: one block of 1024 threads per SM in all, since each selects
+  // anew (48 units of up to 8192 slots: 26 us, and 41 us with two rounds of such blocks).
   const bool many = units >= 296;
-  a.parts = many ? 1 : 296 / units;
+  a.parts = many || units > 148 ? 1 : 148 / units;
   if (a.parts > 16) a.parts = 16;
   const bool in_smem = capacity <= kSmemKeys;
   const size_t nw = (capacity + 31) / 32;
-  const size_t smem = 4 * (3 * nw + 2 + (in_smem ? capacity : 0));
+  const size_t smem = 4 * (3 * nw + 2 + (in_smem ? 2 * ((capacity + 3) & ~3) : 0));
   auto kernel = many ? (in_smem ? kv_evict_kernel<256, 7, true> : kv_evict_kernel<256, 7, false>)
                      : (in_smem ? kv_evict_kernel<1024, 1, true> : kv_evict_kernel<1024, 1, false>);
   if (smem > 40 * 1024 &&
