@@ -207,14 +207,18 @@ __global__ void __launch_bounds__(NT, 1) attn_tile_kernel(const __grid_constant_
   } else if (warp == 9) {
     // ------------------------------------------------------------- products
     constexpr uint32_t wqk = mma_word(Half16<T>::bf16, BN, false), wpv = mma_word(Half16<T>::bf16, 64 * DC, true);
-    const uint32_t qs = smem_u32(dyn), ring = qs + L::kRing;
-    auto qk = [&](int t, int item) {
-      if (lane == 0) {
-        const uint32_t kb = ring + (item % STAGES) * L::kTile, qb = qs + t * L::kTile;
+    // Descriptors are sums of a base and constants, so that they stay in uniform registers.
+    const uint64_t q_desc = smem_desc(smem_u32(dyn), 16), k_desc = smem_desc(smem_u32(dyn) + L::kRing, 16),
+                   v_desc = smem_desc(smem_u32(dyn) + L::kRing, L::kHalf);
+    constexpr uint32_t kStep = L::kTile >> 4;
+    const bool leader = elect_one();
+    auto qk = [&](int t, int stage) {
+      if (leader) {
+        const uint64_t qd = q_desc + t * kStep, kd = k_desc + stage * kStep;
 #pragma unroll
         for (int k = 0; k < 4 * DC; ++k) {
-          const uint32_t at = (k >> 2) * L::kHalf + (k & 3) * 32;
-          mma_ss(tmem + t * BN, smem_desc(qb + at, 16), smem_desc(kb + at, 16), wqk, k != 0);
+          const uint32_t at = ((k >> 2) * L::kHalf + (k & 3) * 32) >> 4;
+          mma_ss(tmem + t * BN, qd + at, kd + at, wqk, k != 0);
         }
         mma_commit(&sh.s_full[t]);
       }
@@ -226,7 +230,7 @@ __global__ void __launch_bounds__(NT, 1) attn_tile_kernel(const __grid_constant_
       if (ok) {
         tcgen05_after_sync();
         for (int t = 0; t < mt; ++t) qk(t, 0);
-        if (lane == 0) mma_commit(&sh.empty[0]);
+        if (leader) mma_commit(&sh.empty[0]);
       }
     }
     for (int j = 0; ok && j < nt; ++j) {
@@ -237,12 +241,11 @@ __global__ void __launch_bounds__(NT, 1) attn_tile_kernel(const __grid_constant_
         ok = ok && wait(sh, &sh.p_full[t], j & 1);
         if (!ok) break;
         tcgen05_after_sync();
-        if (lane == 0) {
-          const uint32_t vb = ring + (vi % STAGES) * L::kTile;
+        if (leader) {
+          const uint64_t vd = v_desc + (vi % STAGES) * kStep;
 #pragma unroll
           for (int k = 0; k < BN / 16; ++k)
-            mma_ts(tmem + 256 + t * 128, tmem + t * BN + k * 8, smem_desc(vb + k * 2048, L::kHalf), wpv,
-                   j != 0 || k != 0);
+            mma_ts(tmem + 256 + t * 128, tmem + t * BN + k * 8, vd + k * (2048 >> 4), wpv, j != 0 || k != 0);
           if (t == mt - 1) mma_commit(&sh.empty[vi % STAGES]);
           if (j + 1 == nt) mma_commit(&sh.o_full[t]);
         }
@@ -250,13 +253,13 @@ __global__ void __launch_bounds__(NT, 1) attn_tile_kernel(const __grid_constant_
           if (t == 0) ok = wait(sh, &sh.full[ki % STAGES], (ki / STAGES) & 1);
           if (!ok) break;
           tcgen05_after_sync();
-          qk(t, ki);
-          if (t == mt - 1 && lane == 0) mma_commit(&sh.empty[ki % STAGES]);
+          qk(t, ki % STAGES);
+          if (t == mt - 1 && leader) mma_commit(&sh.empty[ki % STAGES]);
         }
       }
     }
     if (__any_sync(0xffffffffu, sh.abort)) {  // the products in flight
-      if (lane == 0) {
+      if (leader) {
         mma_commit(&sh.drained);
         mbar_wait(&sh.drained, 0);
       }

@@ -9,6 +9,13 @@
 
 namespace sv {
 
+// One lane of a converged warp (the same one every time).
+__device__ __forceinline__ bool elect_one() {
+  uint32_t on;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(on));
+  return on != 0;
+}
+
 // ---------------------------------------------------------------- tensor memory
 
 // One warp allocates all 512 columns (128 lanes x 512 x 32 bits) and frees them.
