@@ -31,8 +31,8 @@ int choose_splits(int64_t blocks, int64_t slots) {
   return (int)(s < 1 ? 1 : s);
 }
 
-// Of the tile kernel (one block per SM): one round of blocks at most, at least two
-// 128-slot tiles each.
+// Of the tile kernel (one block per SM): one round of blocks at most, at least four
+// 64-slot tiles each.
 int tile_splits(int64_t blocks, int64_t slots) {
   const int64_t want = kSMs / blocks, most = (slots + 255) / 256;
   const int64_t s = want < most ? want : most;

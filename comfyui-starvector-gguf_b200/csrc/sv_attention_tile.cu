@@ -3,7 +3,7 @@
 // cores, float16 / bfloat16.
 //
 // A block holds up to two tiles of 128 query rows (row m = query i * G + head g of one
-// key/value head's group, so that a group's heads share every load) and walks 128-slot
+// key/value head's group, so that a group's heads share every load) and walks 64-slot
 // tiles of the keys and values.  Per row, in one pass: s_j = (q . k_j) scale log2 e,
 // o += 2^(s_j - ref) v_j, l += 2^(s_j - ref).  ref is the running maximum, except that
 // it moves only when a score exceeds it by more than 2^8 (the weights stay in range of
@@ -14,21 +14,25 @@
 //                   TMEM into registers, mask, exponentials, sums; the weights go back
 //                   to TMEM in 16 bits over the scores they came from; at the end the
 //                   division and the output
-//   warp 8          TMA: keys and values in turn through a ring of four 128-slot
+//   warp 8          TMA: keys and values in turn through a ring of eight 64-slot
 //                   stages, 128-byte swizzle
 //   warp 9          the products: S = Q K^T (both operands in shared memory) and
-//                   O += P V (P in TMEM, V as it lies: MN-major).  The order PV0 QK0 PV1
-//                   QK1 leaves a softmax group the other tile's two products to work in
+//                   O += P V (P in TMEM, V as it lies: MN-major).  Each query tile has
+//                   two score buffers: while its softmax works on one, the other tile's
+//                   products and this tile's next scores run
 //   warps 10-11     values of tiles that not every row sees whole: zeros in slots past
 //                   the end, and in place of what is not finite, which would reach
 //                   rows that do not see it (0 * NaN); such slots are noted, and the
 //                   rows that do see them get their values at the end
-// TMEM: S0 | S1 | O0 | O1, 128 columns each; P overlays S.
+// TMEM: S0 (two buffers of 64 columns) | S1 | O0 | O1, 128 columns each; P overlays its
+// S.  With one 128-slot score buffer per tile the chain softmax -> P V -> Q K^T -> softmax
+// left the tensor cores idle half of the time (545 us for the 8192-token prompt).
 //
 // Every wait is bounded: a role that waits in vain sets the block's abort flag, all
 // roles leave their loops, copies and products in flight are waited for (bounded), the
 // TMEM is freed and the rows' outputs become NaN (status SV_ST_TIMEOUT).
 #include <cstring>
+#include <type_traits>
 
 #include "../../include/starvector_sampling.h"
 #include "sv_attention.h"
@@ -38,20 +42,25 @@ namespace sv {
 namespace {
 
 constexpr int NT = 384;
-constexpr int BM = 128, BN = 128;
-constexpr int STAGES = 4;
+constexpr int BM = 128, BN = 64;
+constexpr int RING = 4;            // steps (64 slots) whose keys and values are held
+constexpr int STAGES = 2 * RING;
 constexpr float kSlack = 8.f;
-constexpr int kEdges = 8;  // tiles that not every row of a block sees whole: at most six, see whole()
+constexpr uint32_t kPoly = 0x00;  // which of eight pairs of weights take the polynomial
+constexpr int kEdges = 16;  // tiles that not every row of a block sees whole: at most twelve, see whole()
 
 template <int DC> struct Layout {
-  static constexpr uint32_t kHalf = BM * 128;             // 64 dimensions of 128 rows
-  static constexpr uint32_t kTile = DC * kHalf;           // a query tile or a stage
-  static constexpr uint32_t kRing = 2 * kTile;            // after two query tiles
+  static constexpr uint32_t kQHalf = BM * 128, kHalf = BN * 128;  // 64 dimensions of a tile's rows
+  static constexpr uint32_t kQTile = DC * kQHalf, kTile = DC * kHalf;
+  static constexpr uint32_t kRing = 2 * kQTile;                      // after two query tiles
   static constexpr uint32_t kBytes = kRing + STAGES * kTile + 1024;  // alignment slack
 };
 
 struct Shared {
-  uint64_t q_full[2], full[STAGES], empty[STAGES], ready[STAGES], s_full[2], p_full[2], o_full[2], drained;
+  // full, ready: a stage's copy, and its edge-tile pass.  s_full, pv_done: a query tile's scores of step j and
+  // its product of step j (they also free the step's keys and values); one barrier for each of the four steps
+  // that the ring holds, so that none gets two phases ahead of who waits for it.
+  uint64_t q_full[2], full[STAGES], ready[STAGES], s_full[2][RING], p_full[2][2], pv_done[2][RING], drained;
   uint32_t tmem;
   uint32_t bad[kEdges][BN / 32];  // per edge tile: its slots with values that are not finite
   int bad_from[kEdges], any_bad;
@@ -67,6 +76,47 @@ __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+
+// Two f32 values as one operand of the packed FP32 instructions.
+__device__ __forceinline__ uint64_t pack2(float x, float y) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+  return r;
+}
+__device__ __forceinline__ void unpack2(uint64_t v, float& x, float& y) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(v));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
+// 2^x for two x at once on the FP32 pipes: x = n + f with n = round(x) (the addition of
+// 1.5 2^23 leaves n in the low bits), 2^f by a polynomial of degree 4 (weighted least
+// squares towards equal relative error on [-1/2, 1/2]: below 2.7e-6, under a 16-bit
+// weight's rounding), n added to the exponent.  Below -126 it stays at 2^-126.
+__device__ __forceinline__ void exp2_poly(uint64_t x2, float& u, float& v) {
+  float x, y;
+  unpack2(x2, x, y);
+  x2 = pack2(fmaxf(x, -126.f), fmaxf(y, -126.f));
+  const uint64_t big = pack2(12582912.f, 12582912.f), minus_big = pack2(-12582912.f, -12582912.f);
+  const uint64_t t = add2(x2, big), n = add2(t, minus_big), f = fma2(n, pack2(-1.f, -1.f), x2);
+  uint64_t p = fma2(pack2(0.00957010221f, 0.00957010221f), f, pack2(0.0559178628f, 0.0559178628f));
+  p = fma2(p, f, pack2(0.240247443f, 0.240247443f));
+  p = fma2(p, f, pack2(0.693121791f, 0.693121791f));
+  p = fma2(p, f, pack2(0.999999285f, 0.999999285f));
+  float tx, ty;
+  unpack2(t, tx, ty);
+  unpack2(p, x, y);
+  u = __int_as_float(__float_as_int(x) + (__float_as_int(tx) << 23));
+  v = __int_as_float(__float_as_int(y) + (__float_as_int(ty) << 23));
 }
 
 template <typename T> struct Half16;
@@ -146,26 +196,29 @@ __global__ void __launch_bounds__(NT, 1) attn_tile_kernel(const __grid_constant_
     j0 = t < ta ? a0 + t * BN : b0 + (t - ta) * BN;
     jend = t < ta ? a1 : b1;
   };
-  // Whether rows [first, last] all see the whole tile.
-  auto whole = [&](int j, int first, int last) {
+  // Whether rows that all see the slots [from, to] of the window see the whole tile.
+  auto whole = [&](int j, int from, int to) {
     int j0, jend;
     tile_at(j, j0, jend);
     if (j0 + BN > jend) return false;
-    if (prefix || t0 + j < ta) return true;
-    const int pf = sp.end - a.n + first / a.group, pl = sp.end - a.n + last / a.group;
-    return j0 >= window_low(a, sp.start, pl) && j0 + BN - 1 <= pf;
+    return prefix || t0 + j < ta || (j0 >= from && j0 + BN - 1 <= to);
+  };
+  auto seen_by_all = [&](int first, int last, int& from, int& to) {  // rows [first, last]
+    from = window_low(a, sp.start, sp.end - a.n + last / a.group);
+    to = sp.end - a.n + first / a.group;
   };
 
   if (tid == 0) {
     for (int i = 0; i < 2; ++i) {
       mbar_init(&sh.q_full[i], 128);
-      mbar_init(&sh.s_full[i], 1);
-      mbar_init(&sh.p_full[i], 128);
-      mbar_init(&sh.o_full[i], 1);
+      for (int k = 0; k < 2; ++k) mbar_init(&sh.p_full[i][k], 128);
+      for (int k = 0; k < RING; ++k) {
+        mbar_init(&sh.s_full[i][k], 1);
+        mbar_init(&sh.pv_done[i][k], 1);
+      }
     }
     for (int i = 0; i < STAGES; ++i) {
       mbar_init(&sh.full[i], 1);
-      mbar_init(&sh.empty[i], 1);
       mbar_init(&sh.ready[i], 2);
     }
     mbar_init(&sh.drained, 1);
@@ -188,8 +241,10 @@ __global__ void __launch_bounds__(NT, 1) attn_tile_kernel(const __grid_constant_
       tma_prefetch_map(&maps.v);
       int issued = 0;
       for (; issued < 2 * nt; ++issued) {
-        const int st = issued % STAGES;
-        if (issued >= STAGES && !wait_one(sh, &sh.empty[st], (issued / STAGES - 1) & 1)) break;
+        const int st = issued % STAGES, step = (issued >> 1) % RING;
+        if (issued >= STAGES &&
+            !wait_one(sh, issued & 1 ? &sh.pv_done[mt - 1][step] : &sh.s_full[mt - 1][step], (issued / STAGES - 1) & 1))
+          break;
         int j0, jend;
         tile_at(issued >> 1, j0, jend);
         mbar_expect_tx(&sh.full[st], L::kTile);
@@ -212,50 +267,50 @@ __global__ void __launch_bounds__(NT, 1) attn_tile_kernel(const __grid_constant_
                    v_desc = smem_desc(smem_u32(dyn) + L::kRing, L::kHalf);
     constexpr uint32_t kStep = L::kTile >> 4;
     const bool leader = elect_one();
-    auto qk = [&](int t, int stage) {
-      if (leader) {
-        const uint64_t qd = q_desc + t * kStep, kd = k_desc + stage * kStep;
+    constexpr uint32_t kQStep = L::kQTile >> 4;
+    // Loop bounds and addresses that the compiler can tell are the same in all lanes (a
+    // reduction's result is), or every product would first move its operands to uniform
+    // registers: about 50 cycles each.
+    const int steps = __reduce_max_sync(0xffffffffu, nt);
+    const uint32_t tm = __reduce_max_sync(0xffffffffu, tmem);
+    // One lane waits and issues.  After an abort its waits fail at once and the rest of the
+    // loop computes on what is there, which nobody uses.
+    auto qk = [&](int t, int j) {
+      const uint64_t qd = q_desc + t * kQStep, kd = k_desc + (2 * j) % STAGES * kStep;
 #pragma unroll
-        for (int k = 0; k < 4 * DC; ++k) {
-          const uint32_t at = ((k >> 2) * L::kHalf + (k & 3) * 32) >> 4;
-          mma_ss(tmem + t * BN, qd + at, kd + at, wqk, k != 0);
-        }
-        mma_commit(&sh.s_full[t]);
-      }
+      for (int k = 0; k < 4 * DC; ++k)
+        mma_ss(tm + t * 128 + (j & 1) * BN, qd + (((k >> 2) * L::kQHalf + (k & 3) * 32) >> 4),
+               kd + (((k >> 2) * L::kHalf + (k & 3) * 32) >> 4), wqk, k != 0);
+      mma_commit(&sh.s_full[t][j % RING]);
     };
-    bool ok = nt > 0;
-    if (ok) {
-      for (int t = 0; t < mt && ok; ++t) ok = wait(sh, &sh.q_full[t], 0);
-      ok = ok && wait(sh, &sh.full[0], 0);
-      if (ok) {
-        tcgen05_after_sync();
-        for (int t = 0; t < mt; ++t) qk(t, 0);
-        if (leader) mma_commit(&sh.empty[0]);
+    if (leader && steps > 0) {
+      for (int t = 0; t < mt; ++t) wait_one(sh, &sh.q_full[t], 0);
+      for (int j = 0; j < min(steps, 2); ++j) {
+        wait_one(sh, &sh.full[2 * j], 0);
+        for (int t = 0; t < mt; ++t) qk(t, j);
       }
     }
-    for (int j = 0; ok && j < nt; ++j) {
-      const int vi = 2 * j + 1, ki = 2 * j + 2;
+    __syncwarp();
+#pragma unroll 1
+    for (int j = 0; j < steps; ++j) {
+      const int vi = 2 * j + 1, ki = 2 * j + 4;
+#pragma unroll 1
       for (int t = 0; t < mt; ++t) {
-        if (t == 0)
-          ok = wait(sh, &sh.full[vi % STAGES], (vi / STAGES) & 1) && wait(sh, &sh.ready[vi % STAGES], (vi / STAGES) & 1);
-        ok = ok && wait(sh, &sh.p_full[t], j & 1);
-        if (!ok) break;
-        tcgen05_after_sync();
         if (leader) {
+          if (t == 0) wait_one(sh, &sh.ready[vi % STAGES], (vi / STAGES) & 1);
+          wait_one(sh, &sh.p_full[t][j & 1], (j >> 1) & 1);
+          tcgen05_after_sync();
           const uint64_t vd = v_desc + (vi % STAGES) * kStep;
 #pragma unroll
           for (int k = 0; k < BN / 16; ++k)
-            mma_ts(tmem + 256 + t * 128, tmem + t * BN + k * 8, vd + k * (2048 >> 4), wpv, j != 0 || k != 0);
-          if (t == mt - 1) mma_commit(&sh.empty[vi % STAGES]);
-          if (j + 1 == nt) mma_commit(&sh.o_full[t]);
+            mma_ts(tm + 256 + t * 128, tm + t * 128 + (j & 1) * BN + k * 8, vd + k * (2048 >> 4), wpv, j != 0 || k != 0);
+          mma_commit(&sh.pv_done[t][j % RING]);
+          if (j + 2 < steps) {
+            if (t == 0) wait_one(sh, &sh.full[ki % STAGES], (ki / STAGES) & 1);
+            qk(t, j + 2);
+          }
         }
-        if (j + 1 < nt) {
-          if (t == 0) ok = wait(sh, &sh.full[ki % STAGES], (ki / STAGES) & 1);
-          if (!ok) break;
-          tcgen05_after_sync();
-          qk(t, ki % STAGES);
-          if (t == mt - 1 && leader) mma_commit(&sh.empty[ki % STAGES]);
-        }
+        __syncwarp();
       }
     }
     if (__any_sync(0xffffffffu, sh.abort)) {  // the products in flight
@@ -267,11 +322,12 @@ __global__ void __launch_bounds__(NT, 1) attn_tile_kernel(const __grid_constant_
     }
   } else if (warp >= 10) {
     // ------------------------------------------------------------- values of edge tiles
-    int edge = 0;
+    int edge = 0, from, to;
+    seen_by_all(m0, m_last, from, to);
     for (int j = 0; j < nt; ++j) {
       const int vi = 2 * j + 1, st = vi % STAGES;
       if (!wait(sh, &sh.full[st], (vi / STAGES) & 1)) break;
-      if (!whole(j, m0, m_last)) {
+      if (!whole(j, from, to)) {
         int j0, jend;
         tile_at(j, j0, jend);
         unsigned char* vb = dyn + L::kRing + st * L::kTile;
@@ -312,7 +368,7 @@ __global__ void __launch_bounds__(NT, 1) attn_tile_kernel(const __grid_constant_
       const uint32_t flip = a.scale < 0.f ? 0x80008000u : 0u;  // a negative scale turns the queries' signs
       const float scale = fabsf(a.scale);
       const int mfirst = m0 + t * BM, mlast = min(mfirst + BM, rows_m) - 1;
-      unsigned char* qb = dyn + t * L::kTile;
+      unsigned char* qb = dyn + t * L::kQTile;
       for (int x = row; x < BM * DC * 8; x += 128) {
         const int rr = x / (DC * 8), vec = x % (DC * 8), m = mfirst + rr;
         uint4 v = make_uint4(0u, 0u, 0u, 0u);
@@ -323,7 +379,7 @@ __global__ void __launch_bounds__(NT, 1) attn_tile_kernel(const __grid_constant_
                                                    (int64_t)(h * a.group + g) * a.q_head) + vec);
           v.x ^= flip, v.y ^= flip, v.z ^= flip, v.w ^= flip;
         }
-        *reinterpret_cast<uint4*>(qb + (vec >> 3) * L::kHalf + rr * 128 + (((vec & 7) ^ (rr & 7)) << 4)) = v;
+        *reinterpret_cast<uint4*>(qb + (vec >> 3) * L::kQHalf + rr * 128 + (((vec & 7) ^ (rr & 7)) << 4)) = v;
       }
       fence_proxy_async_smem();
       mbar_arrive(&sh.q_full[t]);
@@ -333,16 +389,21 @@ __global__ void __launch_bounds__(NT, 1) attn_tile_kernel(const __grid_constant_
       const int pos = prefix ? a.prefix : sp.end - a.n + mr / a.group;
       const int low = prefix ? 0 : window_low(a, sp.start, pos);
       const uint32_t lanes = tmem + ((uint32_t)(warp & 3) << 21);
-      const uint32_t s_at = lanes + t * BN, o_at = lanes + 256 + t * 128;
+      const uint32_t o_at = lanes + 256 + t * 128;
+      int from, to;
+      seen_by_all(mfirst, mlast, from, to);
+      auto products_done = [&](int j) { return wait(sh, &sh.pv_done[t][j % RING], (j / RING) & 1); };
       float ref = -INFINITY, l = 0.f;
       bool ok = true;
       for (int j = 0; j < nt; ++j) {
-        ok = wait(sh, &sh.s_full[t], j & 1);
+        ok = wait(sh, &sh.s_full[t][j % RING], (j / RING) & 1);
         if (!ok) break;
         tcgen05_after_sync();
+        const uint32_t s_at = lanes + t * 128 + (j & 1) * BN;
         float s[BN];
-        tmem_load128(s_at, s);
-        if (!whole(j, mfirst, mlast)) {
+        tmem_load64(s_at, s);
+        const bool all_seen = whole(j, from, to);
+        if (!all_seen) {
           int j0, jend;
           tile_at(j, j0, jend);
           const int r1 = min(pos + 1, jend) - j0, r0 = low - j0, s1 = min(sp.start + a.sinks, min(pos + 1, jend)) - j0;
@@ -352,14 +413,22 @@ __global__ void __launch_bounds__(NT, 1) attn_tile_kernel(const __grid_constant_
         }
         float mx[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
-        for (int c = 4; c < BN; ++c) mx[c & 3] = fmaxf(mx[c & 3], s[c]);
-        const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * scale;
-        const bool need = top > ref + kSlack;
+        for (int c = 4; c < BN; c += 8) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            mx[k] = max_nan(max_nan(mx[k], s[c + k]), c + 4 + k < BN ? s[(c + 4 + k) % BN] : mx[k]);
+        }
+        // A NaN stays in the maximum, so that it makes the whole row NaN.
+        const float top = max_nan(max_nan(mx[0], mx[1]), max_nan(mx[2], mx[3])) * scale;
+        const bool need = !(top <= ref + kSlack) && top != -INFINITY;
         if (__any_sync(0xffffffffu, need)) {
           const float f = need ? ex2(ref - top) : 1.f;
           if (need) ref = top;
           l *= f;
-          if (j > 0) {
+          if (j > 0) {  // the product before must be in, and this tile's waits for these weights
+            ok = products_done(j - 1);
+            if (!ok) break;
+            tcgen05_after_sync();
 #pragma unroll 1
             for (int c = 0; c < 64 * DC; c += 32) {
               float o[32];
@@ -370,27 +439,45 @@ __global__ void __launch_bounds__(NT, 1) attn_tile_kernel(const __grid_constant_
             }
           }
         }
-        const float at = ref == -INFINITY ? 0.f : ref;
-        float sum[2] = {0.f, 0.f};
+        // Nothing seen yet: weights of zero; a maximum of +inf: NaN, as inf - inf.
+        const float at = ref == -INFINITY ? 0.f : (ref == INFINITY ? __int_as_float(0x7fc00000) : ref);
+        const uint64_t scale2 = pack2(scale, scale), at2 = pack2(-at, -at);
+        uint64_t sum[2] = {0, 0};
+        // The special function unit takes 8 cycles for a warp's 32 exponentials: in tiles
+        // without hidden slots some go to the FP32 pipes instead.
+        auto weights = [&](auto mixed) {
+          {
+            uint32_t p[32];
 #pragma unroll
-        for (int c = 0; c < BN; c += 64) {
-          uint32_t p[32];
-#pragma unroll
-          for (int k = 0; k < 32; ++k) {
-            const float x = ex2(fmaf(s[c + 2 * k], scale, -at)), y = ex2(fmaf(s[c + 2 * k + 1], scale, -at));
-            sum[0] += x;
-            sum[1] += y;
-            p[k] = Half16<T>::pack(x, y);
+            for (int k = 0; k < 32; ++k) {
+              float x, y;
+              const uint64_t z = fma2(pack2(s[2 * k], s[2 * k + 1]), scale2, at2);
+              if (decltype(mixed)::value && kPoly >> (k & 7) & 1) {
+                exp2_poly(z, x, y);
+              } else {
+                unpack2(z, x, y);
+                x = ex2(x);
+                y = ex2(y);
+              }
+              sum[k & 1] = add2(sum[k & 1], pack2(x, y));
+              p[k] = Half16<T>::pack(x, y);
+            }
+            tmem_store32(s_at, p);
           }
-          tmem_store32(s_at + (c >> 1), p);
-        }
-        l += sum[0] + sum[1];
+        };
+        if (all_seen)
+          weights(std::true_type());
+        else
+          weights(std::false_type());
+        float sx, sy;
+        unpack2(add2(sum[0], sum[1]), sx, sy);
+        l += sx + sy;
         tmem_wait_store();
         tcgen05_before_sync();
-        mbar_arrive(&sh.p_full[t]);
+        mbar_arrive(&sh.p_full[t][j & 1]);
       }
       if (ok && nt > 0) {
-        ok = wait(sh, &sh.o_full[t], 0);
+        ok = products_done(nt - 1);
         tcgen05_after_sync();
       }
       ok = __all_sync(0xffffffffu, ok && !sh.abort);
@@ -489,7 +576,7 @@ EncodeFn encode_fn() {
 }
 
 // [rows][heads][slots][dim] with the given strides in elements; a box is 64 dimensions
-// x 128 slots, zeros outside.  Dimensions of one entry, or whose entries coincide
+// x 64 slots, zeros outside.  Dimensions of one entry, or whose entries coincide
 // (stride 0), become dimensions of size one.
 bool encode(CUtensorMap* map, const AttnArgs& a, const void* base, int64_t slots, int64_t heads, int64_t rows,
             int64_t s_slot, int64_t s_head, int64_t s_row) {
