@@ -16,11 +16,12 @@
 //                   division and the output
 //   warp 8          TMA: keys and values in turn through a ring of eight 64-slot
 //                   stages, 128-byte swizzle
-//   warp 9          the products: S = Q K^T (both operands in shared memory) and
-//                   O += P V (P in TMEM, V as it lies: MN-major).  Each query tile has
-//                   two score buffers: while its softmax works on one, the other tile's
-//                   products and this tile's next scores run
-//   warps 10-11     values of tiles that not every row sees whole: zeros in slots past
+//   warps 9, 10     the products of one query tile each, issued by one lane:
+//                   S = Q K^T (both operands in shared memory) and O += P V (P in TMEM,
+//                   V as it lies: MN-major).  Each tile has two score buffers: while its
+//                   softmax works on one, its next scores form in the other.  One warp for
+//                   both tiles took longer to issue than the products take
+//   warp 11         values of tiles that not every row sees whole: zeros in slots past
 //                   the end, and in place of what is not finite, which would reach
 //                   rows that do not see it (0 * NaN); such slots are noted, and the
 //                   rows that do see them get their values at the end
@@ -219,9 +220,9 @@ __global__ void __launch_bounds__(NT, 1) attn_tile_kernel(const __grid_constant_
     }
     for (int i = 0; i < STAGES; ++i) {
       mbar_init(&sh.full[i], 1);
-      mbar_init(&sh.ready[i], 2);
+      mbar_init(&sh.ready[i], 1);
     }
-    mbar_init(&sh.drained, 1);
+    mbar_init(&sh.drained, 2);
     sh.any_bad = 0;
     for (int i = 0; i < kEdges; ++i)
       for (int k = 0; k < BN / 32; ++k) sh.bad[i][k] = 0;
@@ -242,9 +243,10 @@ __global__ void __launch_bounds__(NT, 1) attn_tile_kernel(const __grid_constant_
       int issued = 0;
       for (; issued < 2 * nt; ++issued) {
         const int st = issued % STAGES, step = (issued >> 1) % RING;
-        if (issued >= STAGES &&
-            !wait_one(sh, issued & 1 ? &sh.pv_done[mt - 1][step] : &sh.s_full[mt - 1][step], (issued / STAGES - 1) & 1))
-          break;
+        bool free = true;  // once both tiles' products of four steps ago are done
+        for (int t = 0; t < mt && issued >= STAGES; ++t)
+          free = free && wait_one(sh, issued & 1 ? &sh.pv_done[t][step] : &sh.s_full[t][step], (issued / STAGES - 1) & 1);
+        if (!free) break;
         int j0, jend;
         tile_at(issued >> 1, j0, jend);
         mbar_expect_tx(&sh.full[st], L::kTile);
@@ -259,7 +261,7 @@ __global__ void __launch_bounds__(NT, 1) attn_tile_kernel(const __grid_constant_
         for (int i = max(0, issued - STAGES); i < issued; ++i)
           mbar_wait(&sh.full[i % STAGES], (i / STAGES) & 1);
     }
-  } else if (warp == 9) {
+  } else if (warp == 9 || warp == 10) {
     // ------------------------------------------------------------- products
     constexpr uint32_t wqk = mma_word(Half16<T>::bf16, BN, false), wpv = mma_word(Half16<T>::bf16, 64 * DC, true);
     // Descriptors are sums of a base and constants, so that they stay in uniform registers.
@@ -275,39 +277,41 @@ __global__ void __launch_bounds__(NT, 1) attn_tile_kernel(const __grid_constant_
     const uint32_t tm = __reduce_max_sync(0xffffffffu, tmem);
     // One lane waits and issues.  After an abort its waits fail at once and the rest of the
     // loop computes on what is there, which nobody uses.
-    auto qk = [&](int t, int j) {
-      const uint64_t qd = q_desc + t * kQStep, kd = k_desc + (2 * j) % STAGES * kStep;
+    const int t = warp - 9;
+    const uint32_t s_at = tm + t * 128, o_at = tm + 256 + t * 128;
+    const uint64_t qd = q_desc + t * kQStep;
+    auto qk = [&](int j) {
+      const uint64_t kd = k_desc + (2 * j) % STAGES * kStep;
 #pragma unroll
       for (int k = 0; k < 4 * DC; ++k)
-        mma_ss(tm + t * 128 + (j & 1) * BN, qd + (((k >> 2) * L::kQHalf + (k & 3) * 32) >> 4),
+        mma_ss(s_at + (j & 1) * BN, qd + (((k >> 2) * L::kQHalf + (k & 3) * 32) >> 4),
                kd + (((k >> 2) * L::kHalf + (k & 3) * 32) >> 4), wqk, k != 0);
       mma_commit(&sh.s_full[t][j % RING]);
     };
-    if (leader && steps > 0) {
-      for (int t = 0; t < mt; ++t) wait_one(sh, &sh.q_full[t], 0);
+    if (leader && t < mt && steps > 0) {
+      wait_one(sh, &sh.q_full[t], 0);
       for (int j = 0; j < min(steps, 2); ++j) {
         wait_one(sh, &sh.full[2 * j], 0);
-        for (int t = 0; t < mt; ++t) qk(t, j);
+        qk(j);
       }
     }
     __syncwarp();
+    if (t < mt) {
 #pragma unroll 1
-    for (int j = 0; j < steps; ++j) {
-      const int vi = 2 * j + 1, ki = 2 * j + 4;
-#pragma unroll 1
-      for (int t = 0; t < mt; ++t) {
+      for (int j = 0; j < steps; ++j) {
+        const int vi = 2 * j + 1, ki = 2 * j + 4;
         if (leader) {
-          if (t == 0) wait_one(sh, &sh.ready[vi % STAGES], (vi / STAGES) & 1);
+          wait_one(sh, &sh.ready[vi % STAGES], (vi / STAGES) & 1);
           wait_one(sh, &sh.p_full[t][j & 1], (j >> 1) & 1);
           tcgen05_after_sync();
           const uint64_t vd = v_desc + (vi % STAGES) * kStep;
 #pragma unroll
           for (int k = 0; k < BN / 16; ++k)
-            mma_ts(tm + 256 + t * 128, tm + t * 128 + (j & 1) * BN + k * 8, vd + k * (2048 >> 4), wpv, j != 0 || k != 0);
+            mma_ts(o_at, s_at + (j & 1) * BN + k * 8, vd + k * (2048 >> 4), wpv, j != 0 || k != 0);
           mma_commit(&sh.pv_done[t][j % RING]);
           if (j + 2 < steps) {
-            if (t == 0) wait_one(sh, &sh.full[ki % STAGES], (ki / STAGES) & 1);
-            qk(t, j + 2);
+            wait_one(sh, &sh.full[ki % STAGES], (ki / STAGES) & 1);
+            qk(j + 2);
           }
         }
         __syncwarp();
@@ -320,7 +324,7 @@ __global__ void __launch_bounds__(NT, 1) attn_tile_kernel(const __grid_constant_
       }
       __syncwarp();
     }
-  } else if (warp >= 10) {
+  } else if (warp == 11) {
     // ------------------------------------------------------------- values of edge tiles
     int edge = 0, from, to;
     seen_by_all(m0, m_last, from, to);
@@ -332,7 +336,7 @@ __global__ void __launch_bounds__(NT, 1) attn_tile_kernel(const __grid_constant_
         tile_at(j, j0, jend);
         unsigned char* vb = dyn + L::kRing + st * L::kTile;
         // A vector of 16 bytes at a time; the swizzle permutes vectors within a row only.
-        for (int x = (warp - 10) * 32 + lane; x < BN * DC * 8; x += 64) {
+        for (int x = lane; x < BN * DC * 8; x += 32) {
           const int half = x / (BN * 8), row = (x >> 3) & (BN - 1), vec = x & 7;
           uint4* p = reinterpret_cast<uint4*>(vb + half * L::kHalf + row * 128 + vec * 16);
           if (j0 + row >= jend) {
