@@ -47,7 +47,7 @@ constexpr int BM = 128, BN = 64;
 constexpr int RING = 4;            // steps (64 slots) whose keys and values are held
 constexpr int STAGES = 2 * RING;
 constexpr float kSlack = 8.f;
-constexpr uint32_t kPoly = 0x00;  // which of eight pairs of weights take the polynomial
+constexpr uint32_t kPoly = 0x22;  // which of eight pairs of weights take the polynomial
 constexpr int kEdges = 16;  // tiles that not every row of a block sees whole: at most twelve, see whole()
 
 template <int DC> struct Layout {
@@ -372,25 +372,26 @@ __global__ void __launch_bounds__(NT, 1) attn_tile_kernel(const __grid_constant_
       const uint32_t flip = a.scale < 0.f ? 0x80008000u : 0u;  // a negative scale turns the queries' signs
       const float scale = fabsf(a.scale);
       const int mfirst = m0 + t * BM, mlast = min(mfirst + BM, rows_m) - 1;
-      unsigned char* qb = dyn + t * L::kQTile;
-      for (int x = row; x < BM * DC * 8; x += 128) {
-        const int rr = x / (DC * 8), vec = x % (DC * 8), m = mfirst + rr;
-        uint4 v = make_uint4(0u, 0u, 0u, 0u);
-        if (m < rows_m && vec * 8 < a.dim) {
-          const int r = prefix ? m / nG : r_own, mr = prefix ? m - r * nG : m;
-          const int i = mr / a.group, g = mr - i * a.group;
-          v = __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + r * a.q_row + i * a.q_tok +
-                                                   (int64_t)(h * a.group + g) * a.q_head) + vec);
-          v.x ^= flip, v.y ^= flip, v.z ^= flip, v.w ^= flip;
+      const int m = mfirst + row;
+      const int r = prefix ? m / nG : r_own, mr = prefix ? m - r * nG : m;
+      const int i = mr / a.group, g = mr - i * a.group;
+      {  // a thread brings its own row: all its vectors in flight at once
+        uint4 v[DC * 8];
+        const T* src = static_cast<const T*>(a.q) + r * a.q_row + i * a.q_tok + (int64_t)(h * a.group + g) * a.q_head;
+#pragma unroll
+        for (int c = 0; c < DC * 8; ++c)
+          v[c] = m < rows_m && c * 8 < a.dim ? __ldg(reinterpret_cast<const uint4*>(src) + c) : make_uint4(0u, 0u, 0u, 0u);
+        unsigned char* qb = dyn + t * L::kQTile + row * 128;
+#pragma unroll
+        for (int c = 0; c < DC * 8; ++c) {
+          v[c].x ^= flip, v[c].y ^= flip, v[c].z ^= flip, v[c].w ^= flip;
+          *reinterpret_cast<uint4*>(qb + (c >> 3) * L::kQHalf + (((c & 7) ^ (row & 7)) << 4)) = v[c];
         }
-        *reinterpret_cast<uint4*>(qb + (vec >> 3) * L::kQHalf + rr * 128 + (((vec & 7) ^ (rr & 7)) << 4)) = v;
       }
       fence_proxy_async_smem();
       mbar_arrive(&sh.q_full[t]);
 
-      const int m = mfirst + row;
-      const int r = prefix ? m / nG : r_own, mr = prefix ? m - r * nG : m;
-      const int pos = prefix ? a.prefix : sp.end - a.n + mr / a.group;
+      const int pos = prefix ? a.prefix : sp.end - a.n + i;
       const int low = prefix ? 0 : window_low(a, sp.start, pos);
       const uint32_t lanes = tmem + ((uint32_t)(warp & 3) << 21);
       const uint32_t o_at = lanes + 256 + t * 128;
@@ -488,7 +489,6 @@ __global__ void __launch_bounds__(NT, 1) attn_tile_kernel(const __grid_constant_
       const bool any_bad = *static_cast<volatile int*>(&sh.any_bad) != 0;
       const bool direct = !prefix && a.o_splits == 0;
       const int64_t idx = ((int64_t)r * a.kv_heads + h) * nG + mr;
-      const int i = mr / a.group, g = mr - i * a.group;
       const float inv = !ok ? __int_as_float(0x7fc00000) : (l == 0.f ? 0.f : (direct ? 1.f / l : 1.f));
       const int64_t all = (int64_t)a.rows * a.kv_heads * nG;
 #pragma unroll 1
