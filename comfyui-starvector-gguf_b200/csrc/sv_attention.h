@@ -43,12 +43,17 @@ struct AttnArgs {
   unsigned* counters;  // zero between calls: [rows * kv_heads], then two per block of the token kernel
   float* part_o;       // own part: [o_splits][idx][dim], or of the token kernel [2 * blocks][16][dim]
   float2* part_ml;     // the same without dim
-  float* prefix_o;     // prefix part: [p_splits][idx][dim]
+  float* prefix_o;     // prefix part: [p_splits][prefix_index][dim]
   float2* prefix_ml;
   float* lse;          // [idx], with weights only: log2 of the softmax denominator, maximum included
   float* scores;       // [idx][capacity], with weights in the token kernel only
   int32_t p_splits, o_splits;  // o_splits 0: the own part is written directly
 };
+
+// A prefix part's rows are numbered by head first: (h * rows + r) * n * G + m.
+__device__ __forceinline__ int64_t prefix_index(const AttnArgs& a, int r, int h, int m) {
+  return ((int64_t)h * a.rows + r) * a.n * a.group + m;
+}
 
 // The slots that row r's queries can see: queries stand at p = end - n + i, slots
 // before `start` (padding in front) are never seen.
@@ -120,6 +125,29 @@ template <auto Kernel> cudaError_t allow_smem(size_t bytes) {
   e = cudaFuncSetAttribute(Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
   if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_relaxed);
   return e;
+}
+
+// Programmatic dependent launch: a kernel launched by launch_after may start once every
+// block of the kernel before it in the stream has called launch_dependents (or ended); it
+// calls wait_before before it uses that kernel's results, and before it ends, so that
+// what comes after it in the stream finds both done.
+__device__ __forceinline__ void launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void wait_before() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
+template <typename... P, typename... A>
+cudaError_t launch_after(bool early, void (*kernel)(P...), dim3 grid, unsigned threads, size_t smem,
+                         cudaStream_t stream, A... args) {
+  cudaLaunchConfig_t c = {};
+  c.gridDim = grid;
+  c.blockDim = dim3(threads);
+  c.dynamicSmemBytes = smem;
+  c.stream = stream;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  c.attrs = &attr;
+  c.numAttrs = early ? 1 : 0;
+  return cudaLaunchKernelEx(&c, kernel, args...);
 }
 
 cudaError_t launch_attn_simt(const AttnArgs& a, bool prefix, cudaStream_t stream);

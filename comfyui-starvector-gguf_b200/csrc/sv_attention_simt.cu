@@ -197,7 +197,7 @@ __global__ void __launch_bounds__(NT) attn_simt_kernel(const AttnArgs a, const b
       }
       if (a.lse && tx == 0) a.lse[idx] = l[r] == 0.f ? INFINITY : m[r] + log2f(l[r]);
     } else {
-      const int64_t at = (int64_t)split * all + idx;
+      const int64_t at = (int64_t)split * all + (prefix ? prefix_index(a, row, h, mr) : idx);
       float* out = (prefix ? a.prefix_o : a.part_o) + at * a.dim;
 #pragma unroll
       for (int c = 0; c < 8; ++c) {
@@ -278,8 +278,12 @@ __global__ void __launch_bounds__(NT) attn_combine_kernel(const AttnArgs a) {
   if (idx >= all) return;
   const int lane = threadIdx.x & 31, d = lane * 4;
   float mx = -INFINITY;
+  const int64_t unit = idx / nG;
+  const int m = (int)(idx - unit * nG), i = m / a.group, g = m - i * a.group;
+  const int h = (int)(unit % a.kv_heads), r = (int)(unit / a.kv_heads);
+  const int64_t pidx = prefix_index(a, r, h, m);
   auto ml_of = [&](int s) {
-    return s < a.p_splits ? a.prefix_ml[s * all + idx] : a.part_ml[(s - a.p_splits) * all + idx];
+    return s < a.p_splits ? a.prefix_ml[s * all + pidx] : a.part_ml[(s - a.p_splits) * all + idx];
   };
   for (int s = lane; s < S; s += 32) mx = fmaxf(mx, ml_of(s).x);
 #pragma unroll
@@ -293,7 +297,7 @@ __global__ void __launch_bounds__(NT) attn_combine_kernel(const AttnArgs a) {
     const float f = exp2f(ml.x - ref);
     l = fmaf(ml.y, f, l);
     if (d < a.dim) {
-      const float* part = s < a.p_splits ? a.prefix_o + (s * all + idx) * a.dim
+      const float* part = s < a.p_splits ? a.prefix_o + (s * all + pidx) * a.dim
                                          : a.part_o + ((s - a.p_splits) * all + idx) * a.dim;
       const float4 x = *reinterpret_cast<const float4*>(part + d);
       o.x = fmaf(x.x, f, o.x);
@@ -303,9 +307,6 @@ __global__ void __launch_bounds__(NT) attn_combine_kernel(const AttnArgs a) {
     }
   }
   const float inv = l == 0.f ? 0.f : 1.f / l;
-  const int64_t unit = idx / nG;
-  const int m = (int)(idx - unit * nG), i = m / a.group, g = m - i * a.group;
-  const int h = (int)(unit % a.kv_heads), r = (int)(unit / a.kv_heads);
   if (d < a.dim) {
     T* out = static_cast<T*>(a.out) + (((int64_t)r * a.n + i) * a.heads + h * a.group + g) * a.dim + d;
     out[0] = from_float<T>(o.x * inv);

@@ -2,7 +2,7 @@
 // chunks of prompts, a batch over a shared prefix) on the fifth-generation tensor
 // cores, float16 / bfloat16.
 //
-// A block holds up to two tiles of 128 query rows (row m = query i * G + head g of one
+// A block (one per SM, taking pieces of work in turn) holds up to two tiles of 128 query rows (row m = query i * G + head g of one
 // key/value head's group, so that a group's heads share every load) and walks 64-slot
 // tiles of the keys and values.  Per row, in one pass: s_j = (q . k_j) scale log2 e,
 // o += 2^(s_j - ref) v_j, l += 2^(s_j - ref).  ref is the running maximum, except that
@@ -33,7 +33,6 @@
 // roles leave their loops, copies and products in flight are waited for (bounded), the
 // TMEM is freed and the rows' outputs become NaN (status SV_ST_TIMEOUT).
 #include <cstring>
-#include <type_traits>
 
 #include "../../include/starvector_sampling.h"
 #include "sv_attention.h"
@@ -43,11 +42,11 @@ namespace sv {
 namespace {
 
 constexpr int NT = 384;
+constexpr int kSMs = 148;
 constexpr int BM = 128, BN = 64;
 constexpr int RING = 4;            // steps (64 slots) whose keys and values are held
 constexpr int STAGES = 2 * RING;
 constexpr float kSlack = 8.f;
-constexpr uint32_t kPoly = 0x22;  // which of eight pairs of weights take the polynomial
 constexpr int kEdges = 16;  // tiles that not every row of a block sees whole: at most twelve, see whole()
 
 template <int DC> struct Layout {
@@ -61,7 +60,7 @@ struct Shared {
   // full, ready: a stage's copy, and its edge-tile pass.  s_full, pv_done: a query tile's scores of step j and
   // its product of step j (they also free the step's keys and values); one barrier for each of the four steps
   // that the ring holds, so that none gets two phases ahead of who waits for it.
-  uint64_t q_full[2], full[STAGES], ready[STAGES], s_full[2][RING], p_full[2][2], pv_done[2][RING], drained;
+  uint64_t q_full[2], full[STAGES], ready[STAGES], s_full[2][RING], p_full[2][2], pv_done[2][RING], written, drained;
   uint32_t tmem;
   uint32_t bad[kEdges][BN / 32];  // per edge tile: its slots with values that are not finite
   int bad_from[kEdges], any_bad;
@@ -76,6 +75,13 @@ struct Maps {
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// 2^x kept in its place among volatile instructions (within a group's turn).
+__device__ __forceinline__ float ex2_here(float x) {
+  float y;
+  asm volatile("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
 
@@ -99,26 +105,9 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
   return r;
 }
 
-// 2^x for two x at once on the FP32 pipes: x = n + f with n = round(x) (the addition of
-// 1.5 2^23 leaves n in the low bits), 2^f by a polynomial of degree 4 (weighted least
-// squares towards equal relative error on [-1/2, 1/2]: below 2.7e-6, under a 16-bit
-// weight's rounding), n added to the exponent.  Below -126 it stays at 2^-126.
-__device__ __forceinline__ void exp2_poly(uint64_t x2, float& u, float& v) {
-  float x, y;
-  unpack2(x2, x, y);
-  x2 = pack2(fmaxf(x, -126.f), fmaxf(y, -126.f));
-  const uint64_t big = pack2(12582912.f, 12582912.f), minus_big = pack2(-12582912.f, -12582912.f);
-  const uint64_t t = add2(x2, big), n = add2(t, minus_big), f = fma2(n, pack2(-1.f, -1.f), x2);
-  uint64_t p = fma2(pack2(0.00957010221f, 0.00957010221f), f, pack2(0.0559178628f, 0.0559178628f));
-  p = fma2(p, f, pack2(0.240247443f, 0.240247443f));
-  p = fma2(p, f, pack2(0.693121791f, 0.693121791f));
-  p = fma2(p, f, pack2(0.999999285f, 0.999999285f));
-  float tx, ty;
-  unpack2(t, tx, ty);
-  unpack2(p, x, y);
-  u = __int_as_float(__float_as_int(x) + (__float_as_int(tx) << 23));
-  v = __int_as_float(__float_as_int(y) + (__float_as_int(ty) << 23));
-}
+// Named barriers 1 and 2: softmax group t waits for its turn, or passes it to the other.
+__device__ __forceinline__ void turn_wait(int t) { asm volatile("bar.sync %0, 256;" ::"r"(1 + t) : "memory"); }
+__device__ __forceinline__ void turn_pass(int t) { asm volatile("bar.arrive %0, 256;" ::"r"(2 - t) : "memory"); }
 
 template <typename T> struct Half16;
 template <> struct Half16<__half> {
@@ -159,54 +148,113 @@ __device__ __forceinline__ bool wait(Shared& sh, void* bar, uint32_t phase) {
   return __all_sync(0xffffffffu, wait_one(sh, bar, phase));
 }
 
+// One piece of work: up to two query tiles of a unit over a share of its slots.
+struct Item {
+  int m0, mt, m_last;      // first query row, tiles that hold rows, last row
+  int h, r, split;         // key/value head, cache row (own part), share of the slots
+  int start, end;          // the row's slots
+  int a0, a1, b0, b1, ta;  // [a0, a1) sinks before the window, [b0, b1) the rest; steps of the former
+  int t0, nt;              // steps
+};
+
 template <typename T, int DC>
 __global__ void __launch_bounds__(NT, 1) attn_tile_kernel(const __grid_constant__ AttnArgs a,
                                                           const __grid_constant__ Maps maps, const bool prefix,
-                                                          const int tiles_m) {
+                                                          const int tiles_m, const int units, const int items) {
   using L = Layout<DC>;
+  constexpr int LPR = DC * 8, RPI = 32 / LPR;  // lanes of a row's 16-byte vectors, rows per warp instruction
   extern __shared__ unsigned char dyn_raw[];
   __shared__ Shared sh;
   unsigned char* dyn = dyn_raw + ((1024u - (smem_u32(dyn_raw) & 1023u)) & 1023u);
+  launch_dependents();
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int nG = a.n * a.group;
   const int rows_m = prefix ? a.rows * nG : nG;
   const int S = prefix ? a.p_splits : max(a.o_splits, 1);
-  // The last rows see the most slots under a causal mask: they start first.
-  const int blocks_m = gridDim.x / S;
-  const int split = blockIdx.x % S, m0 = (blocks_m - 1 - blockIdx.x / S) * tiles_m * BM;
-  const int unit = blockIdx.y;
-  const int h = prefix ? unit : unit % a.kv_heads, r_own = prefix ? 0 : unit / a.kv_heads;
-  const int mt = min(tiles_m, (rows_m - m0 + BM - 1) / BM);  // query tiles that hold rows
+  const int blocks_m = items / (S * units);
 
-  // Slots: [a0, a1) sinks before the window, [b0, b1) the rest.
-  RowSpan sp = {0, a.prefix};
-  int a0 = 0, a1 = 0, b0 = 0, b1 = a.prefix;
-  const int m_last = min(m0 + tiles_m * BM, rows_m) - 1;
-  if (!prefix) {
-    sp = row_span(a, r_own);
-    const int pf = sp.end - a.n + m0 / a.group, pl = sp.end - a.n + m_last / a.group;
-    b0 = window_low(a, sp.start, pf);
-    b1 = pl < sp.start ? b0 : max(pl + 1, b0);
-    a0 = sp.start;
-    a1 = pl >= sp.start ? max(a0, min(sp.start + a.sinks, b0)) : a0;
-  }
-  const int ta = (a1 - a0 + BN - 1) / BN, tiles = ta + (b1 - b0 + BN - 1) / BN;
-  const int t0 = (int)((int64_t)tiles * split / S), nt = (int)((int64_t)tiles * (split + 1) / S) - t0;
-  auto tile_at = [&](int j, int& j0, int& jend) {
-    const int t = t0 + j;
-    j0 = t < ta ? a0 + t * BN : b0 + (t - ta) * BN;
-    jend = t < ta ? a1 : b1;
+  // The last rows see the most slots under a causal mask: they come first.
+  auto item_at = [&](int w) {
+    Item it;
+    const int unit = w % units, x = w / units;
+    it.split = x % S;
+    it.m0 = (blocks_m - 1 - x / S) * tiles_m * BM;
+    it.mt = min(tiles_m, (rows_m - it.m0 + BM - 1) / BM);
+    it.m_last = min(it.m0 + tiles_m * BM, rows_m) - 1;
+    it.h = prefix ? unit : unit % a.kv_heads;
+    it.r = prefix ? 0 : unit / a.kv_heads;
+    it.start = it.a0 = it.a1 = it.b0 = 0;
+    it.end = it.b1 = a.prefix;
+    if (!prefix) {
+      const RowSpan sp = row_span(a, it.r);
+      it.start = sp.start;
+      it.end = sp.end;
+      const int pf = sp.end - a.n + it.m0 / a.group, pl = sp.end - a.n + it.m_last / a.group;
+      it.b0 = window_low(a, sp.start, pf);
+      it.b1 = pl < sp.start ? it.b0 : max(pl + 1, it.b0);
+      it.a0 = sp.start;
+      it.a1 = pl >= sp.start ? max(it.a0, min(sp.start + a.sinks, it.b0)) : it.a0;
+    }
+    it.ta = (it.a1 - it.a0 + BN - 1) / BN;
+    const int steps = it.ta + (it.b1 - it.b0 + BN - 1) / BN;
+    it.t0 = (int)((int64_t)steps * it.split / S);
+    it.nt = (int)((int64_t)steps * (it.split + 1) / S) - it.t0;
+    return it;
   };
-  // Whether rows that all see the slots [from, to] of the window see the whole tile.
-  auto whole = [&](int j, int from, int to) {
-    int j0, jend;
-    tile_at(j, j0, jend);
-    if (j0 + BN > jend) return false;
-    return prefix || t0 + j < ta || (j0 >= from && j0 + BN - 1 <= to);
+  auto tile_at = [](const Item& it, int j, int& j0, int& jend) {
+    const int t = it.t0 + j;
+    j0 = t < it.ta ? it.a0 + t * BN : it.b0 + (t - it.ta) * BN;
+    jend = t < it.ta ? it.a1 : it.b1;
   };
-  auto seen_by_all = [&](int first, int last, int& from, int& to) {  // rows [first, last]
-    from = window_low(a, sp.start, sp.end - a.n + last / a.group);
-    to = sp.end - a.n + first / a.group;
+  // The steps whose slots rows [first, last] all see: j < a_whole (sinks) or w0 <= j < w1.
+  struct Whole {
+    int a_whole, w0, w1;
+    __device__ __forceinline__ bool operator()(int j) const { return j < a_whole || (j >= w0 && j < w1); }
+  };
+  auto whole_steps = [&](const Item& it, int first, int last) {
+    const int from = prefix ? it.b0 : window_low(a, it.start, it.end - a.n + last / a.group);
+    const int to = prefix ? it.b1 : min(it.b1, it.end - a.n + first / a.group + 1);
+    const int b = it.ta - it.t0;  // the window's first step
+    Whole x;
+    x.a_whole = (it.a1 - it.a0) / BN - it.t0;
+    x.w0 = b + (max(from - it.b0, 0) + BN - 1) / BN;
+    x.w1 = b + max(to - it.b0, 0) / BN;
+    return x;
+  };
+
+  // A softmax warp reads and writes its 32 rows of queries and output RPI rows at a time,
+  // LPR lanes to a row: row my_row + k RPI for this lane, its vector my_vec.
+  const int my_row = (warp & 3) * 32 + lane / LPR, my_vec = lane % LPR;
+  const int wg = warp >> 2;                   // a softmax warp's query tile
+  unsigned char* qb = dyn + wg * L::kQTile;  // its queries, and at the end its output on the way out
+  auto q_vec = [&](int row, int vec) {
+    return reinterpret_cast<uint4*>(qb + (vec >> 3) * L::kQHalf + row * 128 + (((vec & 7) ^ (row & 7)) << 4));
+  };
+  const uint32_t flip = a.scale < 0.f ? 0x80008000u : 0u;  // a negative scale turns the queries' signs
+  auto load_queries = [&](const Item& it) {
+    uint4 v[LPR];
+    int m = it.m0 + wg * BM + my_row;
+    int r = prefix ? m / nG : it.r, i = prefix ? m - r * nG : m, g = i;
+    i /= a.group;
+    g -= i * a.group;
+    const T* src = static_cast<const T*>(a.q) + r * a.q_row + i * a.q_tok + (int64_t)(it.h * a.group + g) * a.q_head +
+                   my_vec * 8;
+    const int64_t step = RPI * a.q_head, next_query = a.q_tok - a.group * a.q_head, next_row = a.q_row - a.n * a.q_tok;
+#pragma unroll
+    for (int k = 0; k < LPR; ++k, m += RPI) {
+      v[k] = m < rows_m && my_vec * 8 < a.dim ? __ldg(reinterpret_cast<const uint4*>(src)) : make_uint4(0u, 0u, 0u, 0u);
+      src += step;
+      for (g += RPI; g >= a.group; g -= a.group) {
+        src += next_query;
+        if (++i == a.n) i = 0, src += next_row;  // (without a prefix: past the last row, not read)
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < LPR; ++k) {
+      v[k].x ^= flip, v[k].y ^= flip, v[k].z ^= flip, v[k].w ^= flip;
+      *q_vec(my_row + k * RPI, my_vec) = v[k];
+    }
+    fence_proxy_async_smem();
   };
 
   if (tid == 0) {
@@ -222,6 +270,7 @@ __global__ void __launch_bounds__(NT, 1) attn_tile_kernel(const __grid_constant_
       mbar_init(&sh.full[i], 1);
       mbar_init(&sh.ready[i], 1);
     }
+    mbar_init(&sh.written, 256);
     mbar_init(&sh.drained, 2);
     sh.any_bad = 0;
     for (int i = 0; i < kEdges; ++i)
@@ -230,92 +279,117 @@ __global__ void __launch_bounds__(NT, 1) attn_tile_kernel(const __grid_constant_
     mbar_init_fence();
   }
   if (warp == 9) tmem_alloc512(&sh.tmem);
+  Item it = item_at(blockIdx.x);  // the grid has at most one block per item
+  if (wg < it.mt && it.nt > 0) load_queries(it);
   tcgen05_before_sync();
   __syncthreads();
   tcgen05_after_sync();
   const uint32_t tmem = sh.tmem;
 
+  // Steps are numbered through all the block's items: J = base + j.  Step J's keys and
+  // values are in stages 2 J and 2 J + 1 (mod STAGES).  A query tile's scores alternate
+  // between its two buffers by its own count P of steps (items may lack the second tile).
   if (warp == 8) {
     // ------------------------------------------------------------- copies
-    if (lane == 0 && nt > 0) {
+    if (lane == 0) {
       tma_prefetch_map(&maps.k);
       tma_prefetch_map(&maps.v);
       int issued = 0;
-      for (; issued < 2 * nt; ++issued) {
-        const int st = issued % STAGES, step = (issued >> 1) % RING;
-        bool free = true;  // once both tiles' products of four steps ago are done
-        for (int t = 0; t < mt && issued >= STAGES; ++t)
-          free = free && wait_one(sh, issued & 1 ? &sh.pv_done[t][step] : &sh.s_full[t][step], (issued / STAGES - 1) & 1);
-        if (!free) break;
-        int j0, jend;
-        tile_at(issued >> 1, j0, jend);
-        mbar_expect_tx(&sh.full[st], L::kTile);
-        const CUtensorMap* map = issued & 1 ? &maps.v : &maps.k;
+      bool ok = true;
+      for (int w = blockIdx.x; ok && w < items; w += gridDim.x) {
+        if (w != (int)blockIdx.x) it = item_at(w);
+        for (int x = 0; x < 2 * it.nt; ++x, ++issued) {
+          const int st = issued % STAGES, step = (issued >> 1) % RING;
+          // Free once all tiles' products of four steps ago are done.
+          for (int t = 0; t < tiles_m && issued >= STAGES; ++t)
+            ok = ok && wait_one(sh, x & 1 ? &sh.pv_done[t][step] : &sh.s_full[t][step], (issued / STAGES - 1) & 1);
+          if (!ok) break;
+          int j0, jend;
+          tile_at(it, x >> 1, j0, jend);
+          mbar_expect_tx(&sh.full[st], L::kTile);
+          const CUtensorMap* map = x & 1 ? &maps.v : &maps.k;
 #pragma unroll
-        for (int d = 0; d < DC; ++d)
-          tma_load4(dyn + L::kRing + st * L::kTile + d * L::kHalf, map, d * 64, j0, h * maps.head_mul,
-                    r_own * maps.row_mul, &sh.full[st]);
+          for (int d = 0; d < DC; ++d)
+            tma_load4(dyn + L::kRing + st * L::kTile + d * L::kHalf, map, d * 64, j0, it.h * maps.head_mul,
+                      it.r * maps.row_mul, &sh.full[st]);
+        }
       }
       // After an abort nothing may still be landing when the block ends.
       if (sh.abort)
-        for (int i = max(0, issued - STAGES); i < issued; ++i)
-          mbar_wait(&sh.full[i % STAGES], (i / STAGES) & 1);
+        for (int i = max(0, issued - STAGES); i < issued; ++i) mbar_wait(&sh.full[i % STAGES], (i / STAGES) & 1);
     }
   } else if (warp == 9 || warp == 10) {
     // ------------------------------------------------------------- products
     constexpr uint32_t wqk = mma_word(Half16<T>::bf16, BN, false), wpv = mma_word(Half16<T>::bf16, 64 * DC, true);
-    // Descriptors are sums of a base and constants, so that they stay in uniform registers.
-    const uint64_t q_desc = smem_desc(smem_u32(dyn), 16), k_desc = smem_desc(smem_u32(dyn) + L::kRing, 16),
-                   v_desc = smem_desc(smem_u32(dyn) + L::kRing, L::kHalf);
-    constexpr uint32_t kStep = L::kTile >> 4;
+    constexpr uint32_t kStep = L::kTile >> 4, kQStep = L::kQTile >> 4;
+    const int t = warp - 9;
     const bool leader = elect_one();
-    constexpr uint32_t kQStep = L::kQTile >> 4;
-    // Loop bounds and addresses that the compiler can tell are the same in all lanes (a
-    // reduction's result is), or every product would first move its operands to uniform
-    // registers: about 50 cycles each.
-    const int steps = __reduce_max_sync(0xffffffffu, nt);
+    // Descriptors are sums of a base and constants, and what the loops depend on comes from
+    // reductions, whose results the compiler knows to be the same in all lanes: otherwise
+    // every product would first move its operands to uniform registers.
     const uint32_t tm = __reduce_max_sync(0xffffffffu, tmem);
+    const uint32_t s_at = tm + t * 128, o_at = tm + 256 + t * 128;
+    const uint64_t qd = smem_desc(smem_u32(dyn), 16) + t * kQStep;
+    const uint64_t k_desc = smem_desc(smem_u32(dyn) + L::kRing, 16),
+                   v_desc = smem_desc(smem_u32(dyn) + L::kRing, L::kHalf);
     // One lane waits and issues.  After an abort its waits fail at once and the rest of the
     // loop computes on what is there, which nobody uses.
-    const int t = warp - 9;
-    const uint32_t s_at = tm + t * 128, o_at = tm + 256 + t * 128;
-    const uint64_t qd = q_desc + t * kQStep;
-    auto qk = [&](int j) {
-      const uint64_t kd = k_desc + (2 * j) % STAGES * kStep;
+    auto qk = [&](int J, int P) {
+      const uint64_t kd = k_desc + (2 * J) % STAGES * kStep;
 #pragma unroll
       for (int k = 0; k < 4 * DC; ++k)
-        mma_ss(s_at + (j & 1) * BN, qd + (((k >> 2) * L::kQHalf + (k & 3) * 32) >> 4),
+        mma_ss(s_at + (P & 1) * BN, qd + (((k >> 2) * L::kQHalf + (k & 3) * 32) >> 4),
                kd + (((k >> 2) * L::kHalf + (k & 3) * 32) >> 4), wqk, k != 0);
-      mma_commit(&sh.s_full[t][j % RING]);
+      mma_commit(&sh.s_full[t][J % RING]);
     };
-    if (leader && t < mt && steps > 0) {
-      wait_one(sh, &sh.q_full[t], 0);
-      for (int j = 0; j < min(steps, 2); ++j) {
-        wait_one(sh, &sh.full[2 * j], 0);
-        qk(j);
+    int base_ = 0, mine_ = 0, queries = 0;
+    for (int w = blockIdx.x; w < items && t < tiles_m; w += gridDim.x) {
+      if (w != (int)blockIdx.x) it = item_at(w);
+      const int steps = __reduce_max_sync(0xffffffffu, it.nt);
+      const int base = __reduce_max_sync(0xffffffffu, base_), mine = __reduce_max_sync(0xffffffffu, mine_);
+      if (t >= it.mt) {  // no rows: the stages are passed on as they come
+        if (leader)
+          for (int J = base; J < base + steps; ++J) {
+            wait_one(sh, &sh.full[(2 * J) % STAGES], (2 * J / STAGES) & 1);
+            mma_commit(&sh.s_full[t][J % RING]);
+            wait_one(sh, &sh.ready[(2 * J + 1) % STAGES], ((2 * J + 1) / STAGES) & 1);
+            mma_commit(&sh.pv_done[t][J % RING]);
+          }
+        __syncwarp();
+        base_ += steps;
+        continue;
       }
-    }
-    __syncwarp();
-    if (t < mt) {
+      if (leader && steps > 0) {
+        wait_one(sh, &sh.q_full[t], queries & 1);
+        for (int j = 0; j < min(steps, 2); ++j) {
+          wait_one(sh, &sh.full[(2 * (base + j)) % STAGES], (2 * (base + j) / STAGES) & 1);
+          qk(base + j, mine + j);
+        }
+      }
+      queries += steps > 0;
+      __syncwarp();
 #pragma unroll 1
       for (int j = 0; j < steps; ++j) {
-        const int vi = 2 * j + 1, ki = 2 * j + 4;
+        const int J = base + j, P = mine + j, vi = 2 * J + 1, ki = 2 * J + 4;
         if (leader) {
           wait_one(sh, &sh.ready[vi % STAGES], (vi / STAGES) & 1);
-          wait_one(sh, &sh.p_full[t][j & 1], (j >> 1) & 1);
+          wait_one(sh, &sh.p_full[t][P & 1], (P >> 1) & 1);
           tcgen05_after_sync();
           const uint64_t vd = v_desc + (vi % STAGES) * kStep;
 #pragma unroll
           for (int k = 0; k < BN / 16; ++k)
-            mma_ts(o_at, s_at + (j & 1) * BN + k * 8, vd + k * (2048 >> 4), wpv, j != 0 || k != 0);
-          mma_commit(&sh.pv_done[t][j % RING]);
+            mma_ts(o_at, s_at + (P & 1) * BN + k * 8, vd + k * (2048 >> 4), wpv, j != 0 || k != 0);
+          mma_commit(&sh.pv_done[t][J % RING]);
           if (j + 2 < steps) {
             wait_one(sh, &sh.full[ki % STAGES], (ki / STAGES) & 1);
-            qk(j + 2);
+            qk(J + 2, P + 2);
           }
         }
         __syncwarp();
       }
+      base_ += steps;
+      mine_ += steps;
+      if (__any_sync(0xffffffffu, sh.abort)) break;
     }
     if (__any_sync(0xffffffffu, sh.abort)) {  // the products in flight
       if (leader) {
@@ -326,240 +400,270 @@ __global__ void __launch_bounds__(NT, 1) attn_tile_kernel(const __grid_constant_
     }
   } else if (warp == 11) {
     // ------------------------------------------------------------- values of edge tiles
-    int edge = 0, from, to;
-    seen_by_all(m0, m_last, from, to);
-    for (int j = 0; j < nt; ++j) {
-      const int vi = 2 * j + 1, st = vi % STAGES;
-      if (!wait(sh, &sh.full[st], (vi / STAGES) & 1)) break;
-      if (!whole(j, from, to)) {
-        int j0, jend;
-        tile_at(j, j0, jend);
-        unsigned char* vb = dyn + L::kRing + st * L::kTile;
-        // A vector of 16 bytes at a time; the swizzle permutes vectors within a row only.
-        for (int x = lane; x < BN * DC * 8; x += 32) {
-          const int half = x / (BN * 8), row = (x >> 3) & (BN - 1), vec = x & 7;
-          uint4* p = reinterpret_cast<uint4*>(vb + half * L::kHalf + row * 128 + vec * 16);
-          if (j0 + row >= jend) {
-            *p = make_uint4(0u, 0u, 0u, 0u);
-            continue;
-          }
-          uint4 v = *p;
-          uint32_t* w = reinterpret_cast<uint32_t*>(&v);
-          bool bad = false;
-          constexpr uint32_t E = Half16<T>::expo;
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            if ((w[k] & E) == E) w[k] &= 0xffff0000u, bad = true;
-            if ((w[k] & (E << 16)) == E << 16) w[k] &= 0xffffu, bad = true;
-          }
-          if (bad) {
-            *p = v;
-            atomicOr(&sh.bad[edge][row >> 5], 1u << (row & 31));
-            sh.bad_from[edge] = j0;
-            sh.any_bad = 1;
-          }
+    int base = 0, count = 0;
+    bool ok = true;
+    for (int w = blockIdx.x; ok && w < items; w += gridDim.x, ++count) {
+      if (w != (int)blockIdx.x) it = item_at(w);
+      if (count > 0) {  // the notes of the item before have been read
+        ok = wait(sh, &sh.written, (count - 1) & 1);
+        if (!ok) break;
+        if (sh.any_bad) {
+          __syncwarp();
+          for (int i = lane; i < kEdges * (BN / 32); i += 32) sh.bad[i / (BN / 32)][i % (BN / 32)] = 0;
+          sh.any_bad = 0;
+          __syncwarp();
         }
-        fence_proxy_async_smem();
-        edge = min(edge + 1, kEdges - 1);
       }
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&sh.ready[st]);
+      int edge = 0;
+      const Whole whole = whole_steps(it, it.m0, it.m_last);
+      for (int j = 0; j < it.nt; ++j) {
+        const int vi = 2 * (base + j) + 1, st = vi % STAGES;
+        ok = wait(sh, &sh.full[st], (vi / STAGES) & 1);
+        if (!ok) break;
+        if (!whole(j)) {
+          int j0, jend;
+          tile_at(it, j, j0, jend);
+          unsigned char* vb = dyn + L::kRing + st * L::kTile;
+          // A vector of 16 bytes at a time; the swizzle permutes vectors within a row only.
+          for (int x = lane; x < BN * DC * 8; x += 32) {
+            const int half = x / (BN * 8), row = (x >> 3) & (BN - 1), vec = x & 7;
+            uint4* p = reinterpret_cast<uint4*>(vb + half * L::kHalf + row * 128 + vec * 16);
+            if (j0 + row >= jend) {
+              *p = make_uint4(0u, 0u, 0u, 0u);
+              continue;
+            }
+            uint4 v = *p;
+            uint32_t* q = reinterpret_cast<uint32_t*>(&v);
+            bool bad = false;
+            constexpr uint32_t E = Half16<T>::expo;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              if ((q[k] & E) == E) q[k] &= 0xffff0000u, bad = true;
+              if ((q[k] & (E << 16)) == E << 16) q[k] &= 0xffffu, bad = true;
+            }
+            if (bad) {
+              *p = v;
+              atomicOr(&sh.bad[edge][row >> 5], 1u << (row & 31));
+              sh.bad_from[edge] = j0;
+              sh.any_bad = 1;
+            }
+          }
+          fence_proxy_async_smem();
+          edge = min(edge + 1, kEdges - 1);
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sh.ready[st]);
+      }
+      base += it.nt;
     }
   } else {
     // ------------------------------------------------------------- softmax and output
-    const int t = warp >> 2, row = tid & 127;
-    if (t < mt) {
-      const uint32_t flip = a.scale < 0.f ? 0x80008000u : 0u;  // a negative scale turns the queries' signs
-      const float scale = fabsf(a.scale);
-      const int mfirst = m0 + t * BM, mlast = min(mfirst + BM, rows_m) - 1;
-      const int m = mfirst + row;
-      const int r = prefix ? m / nG : r_own, mr = prefix ? m - r * nG : m;
-      const int i = mr / a.group, g = mr - i * a.group;
-      {  // a thread brings its own row: all its vectors in flight at once
-        uint4 v[DC * 8];
-        const T* src = static_cast<const T*>(a.q) + r * a.q_row + i * a.q_tok + (int64_t)(h * a.group + g) * a.q_head;
-#pragma unroll
-        for (int c = 0; c < DC * 8; ++c)
-          v[c] = m < rows_m && c * 8 < a.dim ? __ldg(reinterpret_cast<const uint4*>(src) + c) : make_uint4(0u, 0u, 0u, 0u);
-        unsigned char* qb = dyn + t * L::kQTile + row * 128;
-#pragma unroll
-        for (int c = 0; c < DC * 8; ++c) {
-          v[c].x ^= flip, v[c].y ^= flip, v[c].z ^= flip, v[c].w ^= flip;
-          *reinterpret_cast<uint4*>(qb + (c >> 3) * L::kQHalf + (((c & 7) ^ (row & 7)) << 4)) = v[c];
-        }
+    const int t = wg, row = tid & 127;
+    const float scale = fabsf(a.scale);
+    const uint32_t lanes = tmem + ((uint32_t)(warp & 3) << 21);
+    const uint32_t o_at = lanes + 256 + t * 128;
+    const bool direct = !prefix && a.o_splits == 0;
+    const int64_t all = (int64_t)a.rows * a.kv_heads * nG;
+    // After an abort the groups go through their steps all the same (on scores that nobody
+    // uses), so that neither waits for a turn that does not come.
+    if (t == 1 && tiles_m == 2) turn_pass(1);
+    int base = 0, mine = 0;
+    for (int w = blockIdx.x; w < items; w += gridDim.x) {
+      if (w != (int)blockIdx.x) {
+        it = item_at(w);
+        if (t < it.mt && it.nt > 0) load_queries(it);
       }
-      fence_proxy_async_smem();
-      mbar_arrive(&sh.q_full[t]);
-
-      const int pos = prefix ? a.prefix : sp.end - a.n + i;
-      const int low = prefix ? 0 : window_low(a, sp.start, pos);
-      const uint32_t lanes = tmem + ((uint32_t)(warp & 3) << 21);
-      const uint32_t o_at = lanes + 256 + t * 128;
-      int from, to;
-      seen_by_all(mfirst, mlast, from, to);
-      auto products_done = [&](int j) { return wait(sh, &sh.pv_done[t][j % RING], (j / RING) & 1); };
       float ref = -INFINITY, l = 0.f;
       bool ok = true;
-      for (int j = 0; j < nt; ++j) {
-        ok = wait(sh, &sh.s_full[t][j % RING], (j / RING) & 1);
-        if (!ok) break;
-        tcgen05_after_sync();
-        const uint32_t s_at = lanes + t * 128 + (j & 1) * BN;
-        float s[BN];
-        tmem_load64(s_at, s);
-        const bool all_seen = whole(j, from, to);
-        if (!all_seen) {
-          int j0, jend;
-          tile_at(j, j0, jend);
-          const int r1 = min(pos + 1, jend) - j0, r0 = low - j0, s1 = min(sp.start + a.sinks, min(pos + 1, jend)) - j0;
+      const int mfirst = it.m0 + t * BM, mlast = min(mfirst + BM, rows_m) - 1, m = mfirst + row;
+      const int pos = prefix ? a.prefix : it.end - a.n + m / a.group, low = prefix ? 0 : window_low(a, it.start, pos);
+      // The item's rows are neighbours in the partial results (per head, for the prefix: all
+      // cache rows' queries).
+      const int64_t part_row = it.split * all + (int64_t)(prefix ? it.h : it.r * a.kv_heads + it.h) * rows_m;
+      if (t < it.mt && it.nt > 0) {
+        mbar_arrive(&sh.q_full[t]);
+        const Whole whole = whole_steps(it, mfirst, mlast);
+        for (int j = 0; j < it.nt; ++j) {
+          const int J = base + j, P = mine + j;
+          ok = ok && wait(sh, &sh.s_full[t][J % RING], (J / RING) & 1);
+          tcgen05_after_sync();
+          const uint32_t s_at = lanes + t * 128 + (P & 1) * BN;
+          float s[BN];
+          tmem_load64(s_at, s);
+          const bool all_seen = whole(j);
+          if (!all_seen) {
+            int j0, jend;
+            tile_at(it, j, j0, jend);
+            const int r1 = min(pos + 1, jend) - j0, r0 = low - j0,
+                      s1 = min(it.start + a.sinks, min(pos + 1, jend)) - j0;
 #pragma unroll
-          for (int c = 0; c < BN; ++c)
-            if (!(c < r1 && (c >= r0 || c < s1))) s[c] = -INFINITY;
-        }
-        float mx[4] = {s[0], s[1], s[2], s[3]};
-#pragma unroll
-        for (int c = 4; c < BN; c += 8) {
-#pragma unroll
-          for (int k = 0; k < 4; ++k)
-            mx[k] = max_nan(max_nan(mx[k], s[c + k]), c + 4 + k < BN ? s[(c + 4 + k) % BN] : mx[k]);
-        }
-        // A NaN stays in the maximum, so that it makes the whole row NaN.
-        const float top = max_nan(max_nan(mx[0], mx[1]), max_nan(mx[2], mx[3])) * scale;
-        const bool need = !(top <= ref + kSlack) && top != -INFINITY;
-        if (__any_sync(0xffffffffu, need)) {
-          const float f = need ? ex2(ref - top) : 1.f;
-          if (need) ref = top;
-          l *= f;
-          if (j > 0) {  // the product before must be in, and this tile's waits for these weights
-            ok = products_done(j - 1);
-            if (!ok) break;
-            tcgen05_after_sync();
-#pragma unroll 1
-            for (int c = 0; c < 64 * DC; c += 32) {
-              float o[32];
-              tmem_load32(o_at + c, o);
-#pragma unroll
-              for (int k = 0; k < 32; ++k) o[k] *= f;
-              tmem_store32(o_at + c, o);
-            }
+            for (int c = 0; c < BN; ++c)
+              if (!(c < r1 && (c >= r0 || c < s1))) s[c] = -INFINITY;
           }
-        }
-        // Nothing seen yet: weights of zero; a maximum of +inf: NaN, as inf - inf.
-        const float at = ref == -INFINITY ? 0.f : (ref == INFINITY ? __int_as_float(0x7fc00000) : ref);
-        const uint64_t scale2 = pack2(scale, scale), at2 = pack2(-at, -at);
-        uint64_t sum[2] = {0, 0};
-        // The special function unit takes 8 cycles for a warp's 32 exponentials: in tiles
-        // without hidden slots some go to the FP32 pipes instead.
-        auto weights = [&](auto mixed) {
-          {
-            uint32_t p[32];
+          float mx[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
-            for (int k = 0; k < 32; ++k) {
-              float x, y;
-              const uint64_t z = fma2(pack2(s[2 * k], s[2 * k + 1]), scale2, at2);
-              if (decltype(mixed)::value && kPoly >> (k & 7) & 1) {
-                exp2_poly(z, x, y);
-              } else {
-                unpack2(z, x, y);
-                x = ex2(x);
-                y = ex2(y);
+          for (int c = 4; c < BN; c += 8) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              mx[k] = max_nan(max_nan(mx[k], s[c + k]), c + 4 + k < BN ? s[(c + 4 + k) % BN] : mx[k]);
+          }
+          // A NaN stays in the maximum, so that it makes the whole row NaN.
+          const float top = max_nan(max_nan(mx[0], mx[1]), max_nan(mx[2], mx[3])) * scale;
+          const bool need = !(top <= ref + kSlack) && top != -INFINITY;
+          if (__any_sync(0xffffffffu, need)) {
+            const float f = need ? ex2(ref - top) : 1.f;
+            if (need) ref = top;
+            l *= f;
+            if (j > 0) {  // the product before must be in, and this step's waits for these weights
+              ok = ok && wait(sh, &sh.pv_done[t][(J - 1) % RING], ((J - 1) / RING) & 1);
+              tcgen05_after_sync();
+#pragma unroll 1
+              for (int c = 0; c < 64 * DC; c += 32) {
+                float o[32];
+                tmem_load32(o_at + c, o);
+#pragma unroll
+                for (int k = 0; k < 32; ++k) o[k] *= f;
+                tmem_store32(o_at + c, o);
               }
-              sum[k & 1] = add2(sum[k & 1], pack2(x, y));
-              p[k] = Half16<T>::pack(x, y);
             }
-            tmem_store32(s_at, p);
           }
-        };
-        if (all_seen)
-          weights(std::true_type());
-        else
-          weights(std::false_type());
-        float sx, sy;
-        unpack2(add2(sum[0], sum[1]), sx, sy);
-        l += sx + sy;
-        tmem_wait_store();
-        tcgen05_before_sync();
-        mbar_arrive(&sh.p_full[t][j & 1]);
-      }
-      if (ok && nt > 0) {
-        ok = products_done(nt - 1);
-        tcgen05_after_sync();
-      }
-      ok = __all_sync(0xffffffffu, ok && !sh.abort);
-      const bool any_bad = *static_cast<volatile int*>(&sh.any_bad) != 0;
-      const bool direct = !prefix && a.o_splits == 0;
-      const int64_t idx = ((int64_t)r * a.kv_heads + h) * nG + mr;
-      const float inv = !ok ? __int_as_float(0x7fc00000) : (l == 0.f ? 0.f : (direct ? 1.f / l : 1.f));
-      const int64_t all = (int64_t)a.rows * a.kv_heads * nG;
-#pragma unroll 1
-      for (int c = 0; c < 64 * DC; c += 32) {
-        float o[32];
-        if (ok && nt > 0) {
-          tmem_load32(o_at + c, o);
-        } else {
+          // Nothing seen yet: weights of zero; a maximum of +inf: NaN, as inf - inf.
+          const float at = ref == -INFINITY ? 0.f : (ref == INFINITY ? __int_as_float(0x7fc00000) : ref);
+          const uint64_t scale2 = pack2(scale, scale), at2 = pack2(-at, -at);
+          uint64_t sum[2] = {0, 0}, z[BN / 2];
 #pragma unroll
-          for (int k = 0; k < 32; ++k) o[k] = 0.f;
+          for (int k = 0; k < BN / 2; ++k) z[k] = fma2(pack2(s[2 * k], s[2 * k + 1]), scale2, at2);
+          // The special function unit takes 8 cycles for a warp's 32 exponentials, which is what
+          // bounds a step: the two groups take turns at it, so that one is always busy with
+          // its other work (445 us for the 8192-token prompt, 470 us without turns).  Moving
+          // exponentials to the FP32 pipes by a polynomial (one pair in eight, or in four) took
+          // 2 to 4 % longer: those pipes do the scaling and the sums already.
+          uint32_t p[32];
+          if (it.mt == 2) turn_wait(t);
+#pragma unroll
+          for (int k = 0; k < 32; ++k) {
+            float x, y;
+            unpack2(z[k], x, y);
+            x = ex2_here(x);
+            y = ex2_here(y);
+            sum[k & 1] = add2(sum[k & 1], pack2(x, y));
+            p[k] = Half16<T>::pack(x, y);
+          }
+          tmem_store32(s_at, p);
+          if (it.mt == 2) turn_pass(t);
+          float sx, sy;
+          unpack2(add2(sum[0], sum[1]), sx, sy);
+          l += sx + sy;
+          tmem_wait_store();
+          tcgen05_before_sync();
+          mbar_arrive(&sh.p_full[t][P & 1]);
+        }
+      }
+      base += it.nt;
+      if (t < it.mt) mine += it.nt;
+      if (t < it.mt) {
+        if (ok && it.nt > 0) {
+          ok = wait(sh, &sh.pv_done[t][(base - 1) % RING], ((base - 1) / RING) & 1);
+          tcgen05_after_sync();
+        }
+        ok = __all_sync(0xffffffffu, ok && !sh.abort);
+        const bool any_bad = *static_cast<volatile int*>(&sh.any_bad) != 0;
+        const float inv = !ok ? __int_as_float(0x7fc00000) : (l == 0.f ? 0.f : (direct ? 1.f / l : 1.f));
+#pragma unroll 1
+        for (int c = 0; c < 64 * DC; c += 32) {
+          float o[32];
+          if (ok && it.nt > 0) {
+            tmem_load32(o_at + c, o);
+          } else {
+#pragma unroll
+            for (int k = 0; k < 32; ++k) o[k] = 0.f;
+          }
+          if (any_bad && m < rows_m) {  // values that are not finite, for the rows that see them
+            for (int e = 0; e < kEdges * BN; ++e) {
+              if (!(sh.bad[e / BN][(e % BN) >> 5] >> (e & 31) & 1u)) continue;
+              const int slot = sh.bad_from[e / BN] + e % BN;
+              if (!prefix && !slot_seen(a, it.start, pos, low, slot)) continue;
+              const T* vp = static_cast<const T*>(prefix ? a.pv : a.v) +
+                            (prefix ? it.h * a.p_head + slot * a.p_slot
+                                    : it.r * a.kv_row + it.h * a.kv_head + slot * a.kv_slot);
+#pragma unroll
+              for (int k = 0; k < 32; k += 8) {
+                float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+                if (c + k < a.dim) load8(vp + c + k, v);
+#pragma unroll
+                for (int x = 0; x < 8; ++x)
+                  if (!isfinite(v[x])) o[k + x] += v[x];
+              }
+            }
+          }
+          __syncwarp();
+#pragma unroll
+          for (int k = 0; k < 32; ++k) o[k] *= inv;
+          // Through the queries' place (the products that read it are done): a thread writes
+          // its row, then the lanes of a row write it out together.  16-bit rows go out whole,
+          // f32 ones 32 DC dimensions at a time.
+          bool flush;
+          if (direct) {
+#pragma unroll
+            for (int k = 0; k < 32; k += 8)
+              *q_vec(row, (c + k) >> 3) = make_uint4(Half16<T>::pack(o[k], o[k + 1]), Half16<T>::pack(o[k + 2], o[k + 3]),
+                                                     Half16<T>::pack(o[k + 4], o[k + 5]), Half16<T>::pack(o[k + 6], o[k + 7]));
+            flush = c + 32 == 64 * DC;
+          } else {
+#pragma unroll
+            for (int k = 0; k < 32; k += 4)
+              *q_vec(row, ((c % (32 * DC)) + k) >> 2) =
+                  make_uint4(__float_as_uint(o[k]), __float_as_uint(o[k + 1]), __float_as_uint(o[k + 2]),
+                             __float_as_uint(o[k + 3]));
+            flush = (c + 32) % (32 * DC) == 0;
+          }
+          __syncwarp();
+          if (flush) {
+            const int d = direct ? my_vec * 8 : c + 32 - 32 * DC + my_vec * 4;
+            int mm = mfirst + my_row, g = mm % a.group;
+            T* out = static_cast<T*>(a.out) +
+                     (((int64_t)it.r * a.n + mm / a.group) * a.heads + it.h * a.group + g) * a.dim + d;
+            float* part = (prefix ? a.prefix_o : a.part_o) + (part_row + mm) * a.dim + d;
+            const int64_t next_query = (int64_t)(a.heads - a.group) * a.dim;
+#pragma unroll 4
+            for (int k = 0; k < LPR; ++k, mm += RPI) {
+              const uint4 v = *q_vec(my_row + k * RPI, my_vec);
+              const bool in = mm < rows_m && d < a.dim;
+              if (direct) {
+                if (in) *reinterpret_cast<uint4*>(out) = v;
+                out += RPI * a.dim;
+                for (g += RPI; g >= a.group; g -= a.group) out += next_query;
+              } else {
+                if (in) *reinterpret_cast<uint4*>(part) = v;
+                part += RPI * a.dim;
+              }
+            }
+            __syncwarp();
+          }
         }
         if (m < rows_m) {
-        if (any_bad) {  // values that are not finite, for the rows that see them
-          for (int e = 0; e < kEdges * BN; ++e) {
-            if (!(sh.bad[e / BN][(e % BN) >> 5] >> (e & 31) & 1u)) continue;
-            const int slot = sh.bad_from[e / BN] + e % BN;
-            if (!prefix && !slot_seen(a, sp.start, pos, low, slot)) continue;
-            const T* vp = static_cast<const T*>(prefix ? a.pv : a.v) +
-                          (prefix ? h * a.p_head + slot * a.p_slot
-                                  : r_own * a.kv_row + h * a.kv_head + slot * a.kv_slot);
-#pragma unroll
-            for (int k = 0; k < 32; k += 8) {
-              float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-              if (c + k < a.dim) load8(vp + c + k, v);
-#pragma unroll
-              for (int x = 0; x < 8; ++x)
-                if (!isfinite(v[x])) o[k + x] += v[x];
-            }
-          }
+          if (!ok) l = inv;
+          if (!direct)
+            (prefix ? a.prefix_ml : a.part_ml)[part_row + m] = make_float2(ref, l);
+          else if (a.lse)
+            a.lse[part_row + m] = l == 0.f ? INFINITY : ref + log2f(l);
         }
-#pragma unroll
-        for (int k = 0; k < 32; ++k) o[k] *= inv;
-        if (direct) {
-          T* out = static_cast<T*>(a.out) + (((int64_t)r * a.n + i) * a.heads + h * a.group + g) * a.dim;
-#pragma unroll
-          for (int k = 0; k < 32; k += 8)
-            if (c + k < a.dim)
-              *reinterpret_cast<uint4*>(out + c + k) =
-                  make_uint4(Half16<T>::pack(o[k], o[k + 1]), Half16<T>::pack(o[k + 2], o[k + 3]),
-                             Half16<T>::pack(o[k + 4], o[k + 5]), Half16<T>::pack(o[k + 6], o[k + 7]));
-        } else {
-          float* out = (prefix ? a.prefix_o : a.part_o) + ((int64_t)split * all + idx) * a.dim;
-#pragma unroll
-          for (int k = 0; k < 32; k += 4)
-            if (c + k < a.dim)
-              *reinterpret_cast<float4*>(out + c + k) = make_float4(o[k], o[k + 1], o[k + 2], o[k + 3]);
-        }
-        }
-        __syncwarp();
+        tcgen05_before_sync();
       }
-      if (m < rows_m) {
-        if (!ok) l = inv;
-        if (!direct)
-          (prefix ? a.prefix_ml : a.part_ml)[(int64_t)split * all + idx] = make_float2(ref, l);
-        else if (a.lse)
-          a.lse[idx] = l == 0.f ? INFINITY : ref + log2f(l);
+      if (a.status && !prefix && tid == 0 && it.h == 0) {
+        const int e = a.lengths ? a.lengths[it.r] : a.capacity, s = a.starts ? a.starts[it.r] : 0;
+        if (!ok)
+          a.status[it.r] = SV_ST_TIMEOUT;
+        else if (it.m0 == 0 && it.split == 0)
+          a.status[it.r] = (e < 0 || e > a.capacity || s < 0 || s > max(e, 0)) ? SV_ST_LENGTH : 0;
       }
-      tcgen05_before_sync();
+      mbar_arrive(&sh.written);
     }
   }
   __syncthreads();
   if (warp == 9) {
     tcgen05_after_sync();
     tmem_free512(tmem);
-  }
-  if (a.status && !prefix && tid == 0 && h == 0) {
-    const int e = a.lengths ? a.lengths[r_own] : a.capacity, s = a.starts ? a.starts[r_own] : 0;
-    if (sh.abort)
-      a.status[r_own] = SV_ST_TIMEOUT;
-    else if (blockIdx.x == 0)
-      a.status[r_own] = (e < 0 || e > a.capacity || s < 0 || s > max(e, 0)) ? SV_ST_LENGTH : 0;
   }
 }
 
@@ -600,11 +704,13 @@ template <typename T, int DC>
 cudaError_t tile(const AttnArgs& a, const Maps& maps, bool prefix, int tiles_m, cudaStream_t stream) {
   const int64_t rows_m = (int64_t)(prefix ? a.rows : 1) * a.n * a.group;
   const int64_t S = prefix ? a.p_splits : (a.o_splits ? a.o_splits : 1);
-  const dim3 grid((unsigned)((rows_m + tiles_m * BM - 1) / (tiles_m * BM) * S),
-                  (unsigned)(prefix ? a.kv_heads : a.rows * a.kv_heads));
+  const int64_t units = prefix ? a.kv_heads : (int64_t)a.rows * a.kv_heads;
+  const int64_t items = (rows_m + tiles_m * BM - 1) / (tiles_m * BM) * S * units;
+  if (items >= (int64_t)1 << 31) return cudaErrorInvalidValue;
   const cudaError_t e = allow_smem<attn_tile_kernel<T, DC>>(Layout<DC>::kBytes);
   if (e != cudaSuccess) return e;
-  attn_tile_kernel<T, DC><<<grid, NT, Layout<DC>::kBytes, stream>>>(a, maps, prefix, tiles_m);
+  attn_tile_kernel<T, DC><<<(unsigned)(items < kSMs ? items : kSMs), NT, Layout<DC>::kBytes, stream>>>(
+      a, maps, prefix, tiles_m, (int)units, (int)items);
   return cudaGetLastError();
 }
 

@@ -135,10 +135,15 @@ struct Part {
 };
 
 // MULTI: more than one query per row (then a tile may be visible to some of them only).
+extern __shared__ float dyn[];  // [NW][16][64 DC]
 template <typename T, int DC, bool FULL, bool MULTI>
 __global__ void __launch_bounds__(NT, kTokenPerSM) attn_token_kernel(const __grid_constant__ AttnArgs a, const int blocks_max) {
-  constexpr int OS = DC * 64 + 4;  // row stride of the warps' outputs in shared memory
-  extern __shared__ float dyn[];   // [NW][16][OS]
+  // The warps' outputs in shared memory: 16-byte vector c of row m, placed so that neither
+  // the fragments' writes nor the rows' reads meet in a bank.
+  constexpr int OS = DC * 64;
+  auto vec_at = [](int w, int m, int c) {
+    return reinterpret_cast<float4*>(dyn) + (w * 16 + m) * (OS / 4) + (c ^ (m & 1) ^ ((c >> 2) & 2));
+  };
   __shared__ float2 warp_ml[NW][16];
   __shared__ float factor[kMaxFlat * 2][16];
   __shared__ float2 part_ml[kMaxFlat * 2][16];
@@ -172,7 +177,11 @@ __global__ void __launch_bounds__(NT, kTokenPerSM) attn_token_kernel(const __gri
   // Blocks in use (a short call takes one per chunk); the first `extra` take one chunk more.
   const int N = min(blocks_max, W), share = W / N, extra = W - share * N;
   const int c = blockIdx.x;
-  if (c >= N) return;
+  launch_dependents();
+  if (c >= N) {
+    wait_before();
+    return;
+  }
   auto first_chunk = [&](int b) { return b * share + min(b, extra); };
   auto block_of = [&](int chunk) {
     const int b = chunk / (share + 1);
@@ -266,8 +275,14 @@ __global__ void __launch_bounds__(NT, kTokenPerSM) attn_token_kernel(const __gri
   // b0 + k * step; c_first is the unit's first block.
   auto join = [&](const Part& p, int c_first, int b0, int step, int count, bool last) {
     const int more = last ? a.p_splits : 0;
-    const int64_t row0 = (int64_t)(p.r * K + p.h) * nG;
+    if (more) wait_before();  // the prefix's kernel may have run beside this one
+    const int64_t row0 = prefix_index(a, p.r, p.h, 0);
     auto slot_of = [&](int k) { return 2 * (b0 + k * step) + (b0 + k * step == c_first); };
+    auto part_at = [&](int k, int m, int d) {
+      return __ldcg(reinterpret_cast<const float4*>(
+          k < count ? a.part_o + ((int64_t)slot_of(k) * 16 + m) * D + d
+                    : a.prefix_o + ((int64_t)(k - count) * all_rows + row0 + m) * D + d));
+    };
     __syncthreads();
     for (int x = tid; x < (count + more) * 16; x += NT) {
       const int k = x >> 4, m = x & 15;
@@ -293,17 +308,14 @@ __global__ void __launch_bounds__(NT, kTokenPerSM) attn_token_kernel(const __gri
     for (int x = tid; x < nG * row_vecs; x += NT) {
       const int m = x / row_vecs, d = (x - m * row_vecs) * 4;
       float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-      for (int k = 0; k < count + more; ++k) {
-        const float* src = k < count ? a.part_o + ((int64_t)slot_of(k) * 16 + m) * D + d
-                                     : a.prefix_o + ((int64_t)(k - count) * all_rows + row0 + m) * D + d;
-        const float4 y = __ldcg(reinterpret_cast<const float4*>(src));
-        const float f = factor[k][m];
+      auto add = [&](float4 y, float f) {
         v.x = fmaf(y.x, f, v.x);
         v.y = fmaf(y.y, f, v.y);
         v.z = fmaf(y.z, f, v.z);
         v.w = fmaf(y.w, f, v.w);
-      }
+      };
+#pragma unroll 4
+      for (int k = 0; k < count + more; ++k) add(part_at(k, m, d), factor[k][m]);
       if (last)
         write_out(p, m, d, v, joined[m].y);
       else
@@ -508,7 +520,6 @@ __global__ void __launch_bounds__(NT, kTokenPerSM) attn_token_kernel(const __gri
       const int m = g + 8 * y;
       if (m >= nG) continue;
       if (t == 0) warp_ml[warp][m] = make_float2(ref[y], l[y]);
-      float* row = dyn + (warp * 16 + m) * OS;
 #pragma unroll
       for (int u = 0; u < DC; ++u)
 #pragma unroll
@@ -516,7 +527,7 @@ __global__ void __launch_bounds__(NT, kTokenPerSM) attn_token_kernel(const __gri
 #pragma unroll
           for (int w = 0; w < 2; ++w) {
             const int j = 8 * u + 4 * w;
-            *reinterpret_cast<float4*>(row + 64 * u + 16 * t + 8 * x + 4 * w) =
+            *vec_at(warp, m, 16 * u + 4 * t + 2 * x + w) =
                 make_float4(o[j][2 * y + x], o[j + 1][2 * y + x], o[j + 2][2 * y + x], o[j + 3][2 * y + x]);
           }
     }
@@ -544,7 +555,7 @@ __global__ void __launch_bounds__(NT, kTokenPerSM) attn_token_kernel(const __gri
       float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
       for (int k = 0; k < NW; ++k) {
-        const float4 y = *reinterpret_cast<const float4*>(dyn + (k * 16 + m) * OS + d);
+        const float4 y = *vec_at(k, m, d >> 2);
         const float f = factor[k][m];
         v.x = fmaf(y.x, f, v.x);
         v.y = fmaf(y.y, f, v.y);
@@ -607,6 +618,7 @@ __global__ void __launch_bounds__(NT, kTokenPerSM) attn_token_kernel(const __gri
     }
     join(p, c_first, c_first, step, count, true);
   }
+  wait_before();
 }
 
 // Accumulated weights from the scores that the token kernel left: one thread per slot.
@@ -614,6 +626,7 @@ __global__ void __launch_bounds__(256) scores_weights_kernel(const __grid_consta
   const int unit = blockIdx.y, h = unit % a.kv_heads, r = unit / a.kv_heads;
   const RowSpan sp = row_span(a, r);
   const int j = blockIdx.x * 256 + threadIdx.x;
+  wait_before();
   if (j >= sp.end || j < sp.start) return;
   const int nG = a.n * a.group;
   const float* s = a.scores + (int64_t)unit * nG * a.capacity + j;
@@ -632,11 +645,11 @@ __global__ void __launch_bounds__(256) scores_weights_kernel(const __grid_consta
 
 template <typename T, int DC, bool FULL, bool MULTI>
 cudaError_t token(const AttnArgs& a, int blocks, cudaStream_t stream) {
-  constexpr size_t smem = sizeof(float) * NW * 16 * (DC * 64 + 4);
+  constexpr size_t smem = sizeof(float) * NW * 16 * DC * 64;
   const cudaError_t e = allow_smem<attn_token_kernel<T, DC, FULL, MULTI>>(smem);
   if (e != cudaSuccess) return e;
-  attn_token_kernel<T, DC, FULL, MULTI><<<blocks, NT, smem, stream>>>(a, blocks);
-  return cudaGetLastError();
+  // Beside the prefix's kernel where that leaves SMs: its results are needed at the joins only.
+  return launch_after(a.prefix != 0, attn_token_kernel<T, DC, FULL, MULTI>, dim3(blocks), NT, smem, stream, a, blocks);
 }
 
 template <typename T, bool MULTI> cudaError_t token_dim(const AttnArgs& a, int blocks, cudaStream_t stream) {
@@ -656,9 +669,8 @@ cudaError_t launch_attn_token(const AttnArgs& a, int blocks, cudaStream_t stream
 }
 
 cudaError_t launch_scores_weights(const AttnArgs& a, cudaStream_t stream) {
-  scores_weights_kernel<<<dim3((unsigned)((a.capacity + 255) / 256), (unsigned)(a.rows * a.kv_heads)), 256, 0,
-                          stream>>>(a);
-  return cudaGetLastError();
+  return launch_after(true, scores_weights_kernel,
+                      dim3((unsigned)((a.capacity + 255) / 256), (unsigned)(a.rows * a.kv_heads)), 256, 0, stream, a);
 }
 
 }  // namespace sv
