@@ -22,11 +22,10 @@ int64_t most_slots(int32_t capacity, int32_t window, int32_t sinks, int64_t tile
   return x < capacity ? x : capacity;
 }
 
-// Splits of the slots among blocks of the f32 kernel: enough blocks for every SM
-// twice, at least two 64-slot tiles each.
-int choose_splits(int64_t blocks, int64_t slots) {
-  if (blocks >= 2 * kSMs) return 1;
-  const int64_t want = (2 * kSMs + blocks - 1) / blocks, most = (slots + 127) / 128;
+// Splits of the slots among blocks of the f32 kernel (one per SM): one round of blocks
+// at most, at least 128 slots each.
+int f32_splits(int64_t blocks, int64_t slots) {
+  const int64_t want = kSMs / blocks, most = (slots + 127) / 128;
   const int64_t s = want < most ? want : most;
   return (int)(s < 1 ? 1 : s);
 }
@@ -66,7 +65,7 @@ Plan make_plan(const AttnArgs& a) {
   if (a.prefix) {
     const int64_t m = a.rows * nG;
     if (f32) {
-      p.p_splits = choose_splits(a.kv_heads * div_up(m, m <= 16 ? 16 : 64), a.prefix);
+      p.p_splits = f32_splits(a.kv_heads * div_up(m, 16), a.prefix);
     } else {
       p.p_tiles = tiles_per_block(a.kv_heads, m);
       p.p_splits = tile_splits(a.kv_heads * div_up(m, 128 * p.p_tiles), a.prefix);
@@ -81,9 +80,9 @@ Plan make_plan(const AttnArgs& a) {
     p.score_bytes = a.weights ? up256(all * a.capacity * 4) : 0;
   } else {
     p.o_tiles = tiles_per_block(units, nG);
-    const int64_t bm = !f32 ? 128 * p.o_tiles : (nG <= 16 ? 16 : 64), blocks = units * div_up(nG, bm);
+    const int64_t bm = f32 ? 16 : 128 * p.o_tiles, blocks = units * div_up(nG, bm);
     const int64_t slots = most_slots(a.capacity, a.window, a.sinks, div_up(bm, a.group));
-    p.o_splits = f32 ? choose_splits(blocks, slots) : tile_splits(blocks, slots);
+    p.o_splits = f32 ? f32_splits(blocks, slots) : tile_splits(blocks, slots);
     if (!a.prefix && p.o_splits == 1) p.o_splits = 0;
     p.o_bytes = up256(p.o_splits * all * a.dim * 4);
     p.ml_bytes = up256(p.o_splits * all * 8);
@@ -141,14 +140,14 @@ int run(AttnArgs& a, void* workspace, size_t workspace_bytes, cudaStream_t strea
   a.scores = reinterpret_cast<float*>(take(p.score_bytes));
   const bool f32 = a.dtype == SV_F32;
   if (a.prefix &&
-      (f32 ? launch_attn_simt(a, true, stream) : launch_attn_tile(a, true, p.p_tiles, stream)) != cudaSuccess)
+      (f32 ? launch_attn_f32(a, true, stream) : launch_attn_tile(a, true, p.p_tiles, stream)) != cudaSuccess)
     return SV_E_CUDA;
   if (p.token) {
     if (launch_attn_token(a, kTokenBlocks, stream) != cudaSuccess) return SV_E_CUDA;
     if (a.weights && launch_scores_weights(a, stream) != cudaSuccess) return SV_E_CUDA;
     return SV_OK;
   }
-  if ((f32 ? launch_attn_simt(a, false, stream) : launch_attn_tile(a, false, p.o_tiles, stream)) != cudaSuccess)
+  if ((f32 ? launch_attn_f32(a, false, stream) : launch_attn_tile(a, false, p.o_tiles, stream)) != cudaSuccess)
     return SV_E_CUDA;
   if (p.o_splits && launch_attn_combine(a, stream) != cudaSuccess) return SV_E_CUDA;
   if (a.weights && launch_attn_weights(a, stream) != cudaSuccess) return SV_E_CUDA;

@@ -150,7 +150,7 @@ cudaError_t launch_after(bool early, void (*kernel)(P...), dim3 grid, unsigned t
   return cudaLaunchKernelEx(&c, kernel, args...);
 }
 
-cudaError_t launch_attn_simt(const AttnArgs& a, bool prefix, cudaStream_t stream);
+cudaError_t launch_attn_f32(const AttnArgs& a, bool prefix, cudaStream_t stream);
 cudaError_t launch_attn_tile(const AttnArgs& a, bool prefix, int tiles_m, cudaStream_t stream);
 cudaError_t launch_attn_token(const AttnArgs& a, int blocks, cudaStream_t stream);
 cudaError_t launch_scores_weights(const AttnArgs& a, cudaStream_t stream);
