@@ -38,6 +38,7 @@ __device__ __forceinline__ void mma(float (&c)[4], float a0, float a1, float a2,
                  "r"(__float_as_uint(a3)), "r"(__float_as_uint(b0)), "r"(__float_as_uint(b1)));
 }
 
+// Truncated, not rounded: the type's largest values must not become infinite.
 __device__ __forceinline__ float upper(float x) { return __uint_as_float(__float_as_uint(x) & 0xffffe000u); }
 __device__ __forceinline__ float4 upper(float4 x) { return make_float4(upper(x.x), upper(x.y), upper(x.z), upper(x.w)); }
 __device__ __forceinline__ float4 minus(float4 a, float4 b) {
@@ -279,10 +280,16 @@ __global__ void __launch_bounds__(NT, 1) attn_f32_kernel(const __grid_constant__
 #pragma unroll
     for (int u = 0; u < VU; ++u) {
       const float4 h0 = upper(vf[0][u]), h1 = upper(vf[1][u]), l0 = minus(vf[0][u], h0), l1 = minus(vf[1][u], h1);
-#define SV_PV(e, f)                                          \
-  mma(o[4 * u + e], ph[0], ph[2], ph[1], ph[3], h0.f, h1.f); \
-  mma(o[4 * u + e], ph[0], ph[2], ph[1], ph[3], l0.f, l1.f); \
-  mma(o[4 * u + e], pl[0], pl[2], pl[1], pl[3], h0.f, h1.f);
+      // A tile's products in a sum of their own, added in f32 with rounding: the tensor core
+      // truncates as it adds, which over many slots would pull the output towards zero.
+#define SV_PV(e, f)                                     \
+  {                                                     \
+    float c[4] = {0.f, 0.f, 0.f, 0.f};                  \
+    mma(c, pl[0], pl[2], pl[1], pl[3], h0.f, h1.f);     \
+    mma(c, ph[0], ph[2], ph[1], ph[3], l0.f, l1.f);     \
+    mma(c, ph[0], ph[2], ph[1], ph[3], h0.f, h1.f);     \
+    for (int k = 0; k < 4; ++k) o[4 * u + e][k] += c[k]; \
+  }
       SV_PV(0, x) SV_PV(1, y) SV_PV(2, z) SV_PV(3, w)
 #undef SV_PV
     }
