@@ -30,17 +30,19 @@ int f32_splits(int64_t blocks, int64_t slots) {
   return (int)(s < 1 ? 1 : s);
 }
 
-// Of the tile kernel (one block per SM): one round of blocks at most, at least four
-// 64-slot tiles each.
-int tile_splits(int64_t blocks, int64_t slots) {
-  const int64_t want = kSMs / blocks, most = (slots + 255) / 256;
+// The tile kernel's (one block per SM): with blocks of one tile, one round of blocks at
+// most, at least four 64-slot steps each.  A block's two halves pay over many steps: 100
+// queries over 2048 slots (36 steps) 30.4 us, 35.3 us without; a prefix of 8192 slots in
+// seven splits (19 steps) 63.9 us, 62.5 us without.
+TileSplit tile_split(int64_t units, int64_t rows_m, int64_t slots, int most_splits) {
+  TileSplit x;
+  x.tiles = units * div_up(rows_m, 128) <= kSMs ? 1 : 2;
+  const int64_t want = kSMs / (units * div_up(rows_m, 128 * x.tiles)), most = (slots + 255) / 256;
   const int64_t s = want < most ? want : most;
-  return (int)(s < 1 ? 1 : s);
+  x.splits = (int)(s < 1 ? 1 : (s > most_splits ? most_splits : s));
+  x.paired = x.tiles == 1 && slots / x.splits >= 1536;
+  return x;
 }
-
-// Query tiles per block of the tile kernel: two (their softmax and products overlap)
-// unless blocks of one still fit the SMs.
-int tiles_per_block(int64_t units, int64_t rows_m) { return units * div_up(rows_m, 128) <= kSMs ? 1 : 2; }
 
 // The token kernel (16-bit types, at most 16 query rows per key/value head) or the
 // tile kernels.
@@ -48,9 +50,10 @@ bool by_token(const AttnArgs& a) { return a.dtype != SV_F32 && (int64_t)a.n * a.
 
 struct Plan {
   bool token;
-  int p_splits, o_splits, p_tiles, o_tiles;
-  size_t counters, o_bytes, ml_bytes, po_bytes, pml_bytes, lse_bytes, score_bytes;
-  size_t total() const { return counters + o_bytes + ml_bytes + po_bytes + pml_bytes + lse_bytes + score_bytes; }
+  int p_splits, o_splits, w_splits;
+  TileSplit prefix, own;
+  size_t counters, o_bytes, ml_bytes, po_bytes, pml_bytes, lse_bytes, score_bytes, weight_bytes;
+  size_t total() const { return counters + o_bytes + ml_bytes + po_bytes + pml_bytes + lse_bytes + score_bytes + weight_bytes; }
 };
 
 Plan make_plan(const AttnArgs& a) {
@@ -67,9 +70,8 @@ Plan make_plan(const AttnArgs& a) {
     if (f32) {
       p.p_splits = f32_splits(a.kv_heads * div_up(m, 16), a.prefix);
     } else {
-      p.p_tiles = tiles_per_block(a.kv_heads, m);
-      p.p_splits = tile_splits(a.kv_heads * div_up(m, 128 * p.p_tiles), a.prefix);
-      if (p.token && p.p_splits > kMostPrefixSplits) p.p_splits = kMostPrefixSplits;
+      p.prefix = tile_split(a.kv_heads, m, a.prefix, p.token ? kMostPrefixSplits : kSMs);
+      p.p_splits = p.prefix.splits;
     }
     p.po_bytes = up256(p.p_splits * all * a.dim * 4);
     p.pml_bytes = up256(p.p_splits * all * 8);
@@ -79,15 +81,25 @@ Plan make_plan(const AttnArgs& a) {
     p.ml_bytes = up256((size_t)2 * kTokenBlocks * 16 * 8);
     p.score_bytes = a.weights ? up256(all * a.capacity * 4) : 0;
   } else {
-    p.o_tiles = tiles_per_block(units, nG);
-    const int64_t bm = f32 ? 16 : 128 * p.o_tiles, blocks = units * div_up(nG, bm);
-    const int64_t slots = most_slots(a.capacity, a.window, a.sinks, div_up(bm, a.group));
-    p.o_splits = f32 ? f32_splits(blocks, slots) : tile_splits(blocks, slots);
+    if (f32) {
+      const int64_t slots = most_slots(a.capacity, a.window, a.sinks, div_up(16, a.group));
+      p.o_splits = f32_splits(units * div_up(nG, 16), slots);
+    } else {
+      p.own = tile_split(units, nG, most_slots(a.capacity, a.window, a.sinks, div_up(128, a.group)), kSMs);
+      p.o_splits = p.own.splits;
+    }
     if (!a.prefix && p.o_splits == 1) p.o_splits = 0;
     p.o_bytes = up256(p.o_splits * all * a.dim * 4);
     p.ml_bytes = up256(p.o_splits * all * 8);
   }
   p.lse_bytes = a.weights ? up256(all * 4) : 0;
+  p.w_splits = 1;
+  if (a.weights && !p.token) {  // about four blocks per SM, at least 64 query rows each
+    const int64_t want = 4 * kSMs / (units * div_up(a.capacity, f32 ? 64 : 128)), most = div_up(nG, 64);
+    const int64_t s = want < most ? want : most;
+    p.w_splits = (int)(s < 1 ? 1 : s);
+    p.weight_bytes = p.w_splits > 1 ? up256(p.w_splits * units * a.capacity * 4) : 0;
+  }
   return p;
 }
 
@@ -131,6 +143,7 @@ int run(AttnArgs& a, void* workspace, size_t workspace_bytes, cudaStream_t strea
   };
   a.p_splits = p.p_splits;
   a.o_splits = p.o_splits;
+  a.w_splits = p.w_splits;
   a.counters = reinterpret_cast<unsigned*>(take(p.counters));
   a.part_o = reinterpret_cast<float*>(take(p.o_bytes));
   a.part_ml = reinterpret_cast<float2*>(take(p.ml_bytes));
@@ -138,19 +151,22 @@ int run(AttnArgs& a, void* workspace, size_t workspace_bytes, cudaStream_t strea
   a.prefix_ml = reinterpret_cast<float2*>(take(p.pml_bytes));
   a.lse = reinterpret_cast<float*>(take(p.lse_bytes));
   a.scores = reinterpret_cast<float*>(take(p.score_bytes));
+  a.weight_parts = reinterpret_cast<float*>(take(p.weight_bytes));
   const bool f32 = a.dtype == SV_F32;
   if (a.prefix &&
-      (f32 ? launch_attn_f32(a, true, stream) : launch_attn_tile(a, true, p.p_tiles, stream)) != cudaSuccess)
+      (f32 ? launch_attn_f32(a, true, stream) : launch_attn_tile(a, true, p.prefix, stream)) != cudaSuccess)
     return SV_E_CUDA;
   if (p.token) {
     if (launch_attn_token(a, kTokenBlocks, stream) != cudaSuccess) return SV_E_CUDA;
     if (a.weights && launch_scores_weights(a, stream) != cudaSuccess) return SV_E_CUDA;
     return SV_OK;
   }
-  if ((f32 ? launch_attn_f32(a, false, stream) : launch_attn_tile(a, false, p.o_tiles, stream)) != cudaSuccess)
+  if ((f32 ? launch_attn_f32(a, false, stream) : launch_attn_tile(a, false, p.own, stream)) != cudaSuccess)
     return SV_E_CUDA;
   if (p.o_splits && launch_attn_combine(a, stream) != cudaSuccess) return SV_E_CUDA;
-  if (a.weights && launch_attn_weights(a, stream) != cudaSuccess) return SV_E_CUDA;
+  if (a.weights && (f32 ? launch_attn_weights(a, stream) : launch_weights16(a, stream)) != cudaSuccess)
+    return SV_E_CUDA;
+  if (p.w_splits > 1 && launch_weights_sum(a, stream) != cudaSuccess) return SV_E_CUDA;
   return SV_OK;
 }
 

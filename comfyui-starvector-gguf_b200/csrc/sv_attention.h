@@ -47,7 +47,9 @@ struct AttnArgs {
   float2* prefix_ml;
   float* lse;          // [idx], with weights only: log2 of the softmax denominator, maximum included
   float* scores;       // [idx][capacity], with weights in the token kernel only
+  float* weight_parts; // [w_splits][rows * kv_heads][capacity], with weights and w_splits > 1
   int32_t p_splits, o_splits;  // o_splits 0: the own part is written directly
+  int32_t w_splits;            // of the query rows, for the accumulated weights of calls with many
 };
 
 // A prefix part's rows are numbered by head first: (h * rows + r) * n * G + m.
@@ -150,9 +152,40 @@ cudaError_t launch_after(bool early, void (*kernel)(P...), dim3 grid, unsigned t
   return cudaLaunchKernelEx(&c, kernel, args...);
 }
 
+// The query rows [first, last) that share `split` of the sum over those that may see
+// slots [j0, j0 + count): under the causal mask none before the first whose position
+// reaches j0, under a window none past the last that still has the last of them.
+__device__ __forceinline__ void weight_rows(const AttnArgs& a, const RowSpan& sp, int j0, int count, int split,
+                                            int& first, int& last) {
+  const int nG = a.n * a.group, at = sp.end - a.n;
+  const int64_t lo = max(0, j0 - at) * (int64_t)a.group;
+  int64_t hi = nG;
+  if (a.window && j0 >= sp.start + a.sinks) hi = ((int64_t)j0 + count - 1 + a.window - at) * a.group;
+  hi = min((int64_t)nG, max(hi, lo));
+  first = (int)(lo + (hi - lo) * split / a.w_splits);
+  last = (int)(lo + (hi - lo) * (split + 1) / a.w_splits);
+}
+
+// A slot's sum: added to the weights, or left for launch_weights_sum.
+__device__ __forceinline__ void add_weight(const AttnArgs& a, int unit, int r, int h, int j, int split, float x) {
+  if (a.w_splits > 1)
+    a.weight_parts[((int64_t)split * a.rows * a.kv_heads + unit) * a.capacity + j] = x;
+  else
+    a.weights[r * a.w_row + h * a.w_head + j] += x;
+}
+
+cudaError_t launch_weights_sum(const AttnArgs& a, cudaStream_t stream);
 cudaError_t launch_attn_f32(const AttnArgs& a, bool prefix, cudaStream_t stream);
-cudaError_t launch_attn_tile(const AttnArgs& a, bool prefix, int tiles_m, cudaStream_t stream);
+// How the tile kernel divides its work: query tiles per block (two, unless blocks of one
+// still fit the SMs), splits of the slots, and whether a block of one tile takes its
+// steps in two interleaved halves.
+struct TileSplit {
+  int tiles, splits;
+  bool paired;
+};
+cudaError_t launch_attn_tile(const AttnArgs& a, bool prefix, const TileSplit& split, cudaStream_t stream);
 cudaError_t launch_attn_token(const AttnArgs& a, int blocks, cudaStream_t stream);
+cudaError_t launch_weights16(const AttnArgs& a, cudaStream_t stream);
 cudaError_t launch_scores_weights(const AttnArgs& a, cudaStream_t stream);
 cudaError_t launch_attn_combine(const AttnArgs& a, cudaStream_t stream);
 cudaError_t launch_attn_weights(const AttnArgs& a, cudaStream_t stream);

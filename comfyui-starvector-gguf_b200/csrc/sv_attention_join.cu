@@ -10,8 +10,7 @@ constexpr int BN = 64;                  // slots per tile
 constexpr int KS = kAttnMaxDim + 4;     // row stride of the staged queries and keys (floats)
 
 // Stages `count` rows of `dim` elements as float, zeros past `valid` rows.
-template <typename T>
-__device__ __forceinline__ void stage(float* dst, int stride, const T* src, int64_t src_stride, int count, int valid,
+__device__ __forceinline__ void stage(float* dst, int stride, const float* src, int64_t src_stride, int count, int valid,
                                       int dim) {
   const int vec = dim >> 3;
   for (int x = threadIdx.x; x < count * vec; x += NT) {
@@ -24,10 +23,9 @@ __device__ __forceinline__ void stage(float* dst, int stride, const T* src, int6
   }
 }
 
-template <typename T>
-__device__ __forceinline__ const T* query_row(const AttnArgs& a, int r, int h, int m) {
+__device__ __forceinline__ const float* query_row(const AttnArgs& a, int r, int h, int m) {
   const int i = m / a.group, g = m - i * a.group;
-  return static_cast<const T*>(a.q) + r * a.q_row + i * a.q_tok + (int64_t)(h * a.group + g) * a.q_head;
+  return static_cast<const float*>(a.q) + r * a.q_row + i * a.q_tok + (int64_t)(h * a.group + g) * a.q_head;
 }
 
 // Scores of RPT rows x 4 slots (slots tx, tx + 16, ...) of the staged tiles.
@@ -51,10 +49,9 @@ __device__ __forceinline__ void scores(const float* qs, const float* ks, int ty,
   }
 }
 
-// Accumulated weights: w[slot] += sum over the group's rows of 2^(s - lse).  One block
-// owns 64 slots of one row and head and walks the query rows, so the sum's order is
-// fixed and no atomics are needed.
-template <typename T>
+// Accumulated weights of float calls, on the FP32 pipes: w[slot] += sum over the group's
+// rows of 2^(s - lse).  One block owns 64 slots of one row and head and walks (a split
+// of) the query rows, so the sum's order is fixed and no atomics are needed.
 __global__ void __launch_bounds__(NT) attn_weights_kernel(const AttnArgs a) {
   constexpr int BM = 64, RPT = BM / 16;
   extern __shared__ float4 smem4[];
@@ -68,16 +65,18 @@ __global__ void __launch_bounds__(NT) attn_weights_kernel(const AttnArgs a) {
   const int j0 = blockIdx.x * BN;
   const int valid = min(BN, sp.end - j0);
   if (valid <= 0) return;
+  int m_first, m_end;
+  weight_rows(a, sp, j0, valid, blockIdx.z, m_first, m_end);
   const int64_t base = r * a.kv_row + h * a.kv_head + j0 * a.kv_slot;
-  stage(ks, KS, static_cast<const T*>(a.k) + base, a.kv_slot, BN, valid, a.dim);
+  stage(ks, KS, static_cast<const float*>(a.k) + base, a.kv_slot, BN, valid, a.dim);
   float sum[4] = {0.f, 0.f, 0.f, 0.f};
-  for (int m0 = 0; m0 < nG; m0 += BM) {
+  for (int m0 = m_first; m0 < m_end; m0 += BM) {
     __syncthreads();
     const int vec = a.dim >> 3;
     for (int x = threadIdx.x; x < BM * vec; x += NT) {
       const int row = x / vec, c = (x - row * vec) * 8;
       float f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-      if (m0 + row < nG) load8(query_row<T>(a, r, h, m0 + row) + c, f);
+      if (m0 + row < m_end) load8(query_row(a, r, h, m0 + row) + c, f);
       float4* d = reinterpret_cast<float4*>(qs + row * KS + c);
       d[0] = make_float4(f[0], f[1], f[2], f[3]);
       d[1] = make_float4(f[4], f[5], f[6], f[7]);
@@ -88,7 +87,7 @@ __global__ void __launch_bounds__(NT) attn_weights_kernel(const AttnArgs a) {
 #pragma unroll
     for (int k = 0; k < RPT; ++k) {
       const int m = m0 + ty * RPT + k;
-      if (m >= nG) continue;
+      if (m >= m_end) continue;
       const int p = sp.end - a.n + m / a.group, lo = window_low(a, sp.start, p);
       const float lse = a.lse[(int64_t)unit * nG + m];
 #pragma unroll
@@ -103,8 +102,21 @@ __global__ void __launch_bounds__(NT) attn_weights_kernel(const AttnArgs a) {
     float t = 0.f;
 #pragma unroll
     for (int k = 0; k < 16; ++k) t += sums[k * BN + threadIdx.x];
-    a.weights[r * a.w_row + h * a.w_head + j0 + threadIdx.x] += t;
+    if (j0 + (int)threadIdx.x >= sp.start) add_weight(a, unit, r, h, j0 + threadIdx.x, blockIdx.z, t);
   }
+}
+
+// The splits of the weights' sums, in order: one thread per slot.
+__global__ void __launch_bounds__(NT) weights_sum_kernel(const AttnArgs a) {
+  const int unit = blockIdx.y, h = unit % a.kv_heads, r = unit / a.kv_heads;
+  const RowSpan sp = row_span(a, r);
+  const int j = blockIdx.x * NT + threadIdx.x;
+  if (j < sp.start || j >= sp.end) return;
+  float t = 0.f;
+#pragma unroll 8
+  for (int s = 0; s < a.w_splits; ++s)
+    t += a.weight_parts[((int64_t)s * a.rows * a.kv_heads + unit) * a.capacity + j];
+  a.weights[r * a.w_row + h * a.w_head + j] += t;
 }
 
 // Joins the splits of one query row per warp: a lane holds four dimensions.
@@ -155,15 +167,6 @@ __global__ void __launch_bounds__(NT) attn_combine_kernel(const AttnArgs a) {
   if (a.lse && lane == 0) a.lse[idx] = l == 0.f ? INFINITY : mx + log2f(l);
 }
 
-template <typename T> cudaError_t weights_any(const AttnArgs& a, cudaStream_t stream) {
-  constexpr size_t smem = sizeof(float) * (64 * KS + BN * KS + 16 * BN);
-  cudaError_t e = allow_smem<attn_weights_kernel<T>>(smem);
-  if (e != cudaSuccess) return e;
-  const dim3 grid((unsigned)((a.capacity + BN - 1) / BN), (unsigned)(a.rows * a.kv_heads));
-  attn_weights_kernel<T><<<grid, NT, smem, stream>>>(a);
-  return cudaGetLastError();
-}
-
 }  // namespace
 
 cudaError_t launch_attn_combine(const AttnArgs& a, cudaStream_t stream) {
@@ -177,12 +180,18 @@ cudaError_t launch_attn_combine(const AttnArgs& a, cudaStream_t stream) {
   return cudaGetLastError();
 }
 
+cudaError_t launch_weights_sum(const AttnArgs& a, cudaStream_t stream) {
+  weights_sum_kernel<<<dim3((unsigned)((a.capacity + NT - 1) / NT), (unsigned)(a.rows * a.kv_heads)), NT, 0, stream>>>(a);
+  return cudaGetLastError();
+}
+
 cudaError_t launch_attn_weights(const AttnArgs& a, cudaStream_t stream) {
-  switch (a.dtype) {
-    case 0: return weights_any<float>(a, stream);
-    case 1: return weights_any<__half>(a, stream);
-    default: return weights_any<__nv_bfloat16>(a, stream);
-  }
+  constexpr size_t smem = sizeof(float) * (64 * KS + BN * KS + 16 * BN);
+  const cudaError_t e = allow_smem<attn_weights_kernel>(smem);
+  if (e != cudaSuccess) return e;
+  const dim3 grid((unsigned)((a.capacity + BN - 1) / BN), (unsigned)(a.rows * a.kv_heads), (unsigned)a.w_splits);
+  attn_weights_kernel<<<grid, NT, smem, stream>>>(a);
+  return cudaGetLastError();
 }
 
 }  // namespace sv

@@ -61,6 +61,7 @@ struct Shared {
   // its product of step j (they also free the step's keys and values); one barrier for each of the four steps
   // that the ring holds, so that none gets two phases ahead of who waits for it.
   uint64_t q_full[2], full[STAGES], ready[STAGES], s_full[2][RING], p_full[2][2], pv_done[2][RING], written, drained;
+  float2 pair[BM];  // PAIRED: the second group's references and sums
   uint32_t tmem;
   uint32_t bad[kEdges][BN / 32];  // per edge tile: its slots with values that are not finite
   int bad_from[kEdges], any_bad;
@@ -157,7 +158,9 @@ struct Item {
   int t0, nt;              // steps
 };
 
-template <typename T, int DC>
+// PAIRED: blocks of one query tile (and one item each), whose steps the two softmax groups
+// and product warps take in turn, each with an output of its own, joined at the end.
+template <typename T, int DC, bool PAIRED>
 __global__ void __launch_bounds__(NT, 1) attn_tile_kernel(const __grid_constant__ AttnArgs a,
                                                           const __grid_constant__ Maps maps, const bool prefix,
                                                           const int tiles_m, const int units, const int items) {
@@ -301,7 +304,7 @@ __global__ void __launch_bounds__(NT, 1) attn_tile_kernel(const __grid_constant_
         for (int x = 0; x < 2 * it.nt; ++x, ++issued) {
           const int st = issued % STAGES, step = (issued >> 1) % RING;
           // Free once all tiles' products of four steps ago are done.
-          for (int t = 0; t < tiles_m && issued >= STAGES; ++t)
+          for (int t = PAIRED ? (x >> 1) & 1 : 0; t < (PAIRED ? ((x >> 1) & 1) + 1 : tiles_m) && issued >= STAGES; ++t)
             ok = ok && wait_one(sh, x & 1 ? &sh.pv_done[t][step] : &sh.s_full[t][step], (issued / STAGES - 1) & 1);
           if (!ok) break;
           int j0, jend;
@@ -329,7 +332,7 @@ __global__ void __launch_bounds__(NT, 1) attn_tile_kernel(const __grid_constant_
     // every product would first move its operands to uniform registers.
     const uint32_t tm = __reduce_max_sync(0xffffffffu, tmem);
     const uint32_t s_at = tm + t * 128, o_at = tm + 256 + t * 128;
-    const uint64_t qd = smem_desc(smem_u32(dyn), 16) + t * kQStep;
+    const uint64_t qd = smem_desc(smem_u32(dyn), 16) + (PAIRED ? 0 : t * kQStep);
     const uint64_t k_desc = smem_desc(smem_u32(dyn) + L::kRing, 16),
                    v_desc = smem_desc(smem_u32(dyn) + L::kRing, L::kHalf);
     // One lane waits and issues.  After an abort its waits fail at once and the rest of the
@@ -343,7 +346,37 @@ __global__ void __launch_bounds__(NT, 1) attn_tile_kernel(const __grid_constant_
       mma_commit(&sh.s_full[t][J % RING]);
     };
     int base_ = 0, mine_ = 0, queries = 0;
-    for (int w = blockIdx.x; w < items && t < tiles_m; w += gridDim.x) {
+    if (PAIRED) {
+      const int steps = __reduce_max_sync(0xffffffffu, it.nt);
+      if (leader && t < steps) {
+        wait_one(sh, &sh.q_full[0], 0);
+        for (int j = t; j < min(steps, t + 4); j += 2) {
+          wait_one(sh, &sh.full[2 * j], 0);
+          qk(j, j >> 1);
+        }
+      }
+      __syncwarp();
+#pragma unroll 1
+      for (int c = 0; 2 * c + t < steps; ++c) {
+        const int j = 2 * c + t, vi = 2 * j + 1, ki = 2 * j + 8;
+        if (leader) {
+          wait_one(sh, &sh.ready[vi % STAGES], (vi / STAGES) & 1);
+          wait_one(sh, &sh.p_full[t][c & 1], (c >> 1) & 1);
+          tcgen05_after_sync();
+          const uint64_t vd = v_desc + (vi % STAGES) * kStep;
+#pragma unroll
+          for (int k = 0; k < BN / 16; ++k)
+            mma_ts(o_at, s_at + (c & 1) * BN + k * 8, vd + k * (2048 >> 4), wpv, c != 0 || k != 0);
+          mma_commit(&sh.pv_done[t][j % RING]);
+          if (j + 4 < steps) {
+            wait_one(sh, &sh.full[ki % STAGES], (ki / STAGES) & 1);
+            qk(j + 4, c + 2);
+          }
+        }
+        __syncwarp();
+      }
+    }
+    for (int w = blockIdx.x; !PAIRED && w < items && t < tiles_m; w += gridDim.x) {
       if (w != (int)blockIdx.x) it = item_at(w);
       const int steps = __reduce_max_sync(0xffffffffu, it.nt);
       const int base = __reduce_max_sync(0xffffffffu, base_), mine = __reduce_max_sync(0xffffffffu, mine_);
@@ -466,7 +499,7 @@ __global__ void __launch_bounds__(NT, 1) attn_tile_kernel(const __grid_constant_
     const int64_t all = (int64_t)a.rows * a.kv_heads * nG;
     // After an abort the groups go through their steps all the same (on scores that nobody
     // uses), so that neither waits for a turn that does not come.
-    if (t == 1 && tiles_m == 2) turn_pass(1);
+    if (t == 1 && (PAIRED || tiles_m == 2)) turn_pass(1);
     int base = 0, mine = 0;
     for (int w = blockIdx.x; w < items; w += gridDim.x) {
       if (w != (int)blockIdx.x) {
@@ -475,16 +508,23 @@ __global__ void __launch_bounds__(NT, 1) attn_tile_kernel(const __grid_constant_
       }
       float ref = -INFINITY, l = 0.f;
       bool ok = true;
-      const int mfirst = it.m0 + t * BM, mlast = min(mfirst + BM, rows_m) - 1, m = mfirst + row;
+      const int mfirst = it.m0 + (PAIRED ? 0 : t * BM), mlast = min(mfirst + BM, rows_m) - 1, m = mfirst + row;
       const int pos = prefix ? a.prefix : it.end - a.n + m / a.group, low = prefix ? 0 : window_low(a, it.start, pos);
       // The item's rows are neighbours in the partial results (per head, for the prefix: all
       // cache rows' queries).
       const int64_t part_row = it.split * all + (int64_t)(prefix ? it.h : it.r * a.kv_heads + it.h) * rows_m;
-      if (t < it.mt && it.nt > 0) {
-        mbar_arrive(&sh.q_full[t]);
+      const bool both = PAIRED || it.mt == 2;
+      if ((PAIRED || t < it.mt) && it.nt > 0) {
+        if (t < it.mt) mbar_arrive(&sh.q_full[t]);
         const Whole whole = whole_steps(it, mfirst, mlast);
-        for (int j = 0; j < it.nt; ++j) {
-          const int J = base + j, P = mine + j;
+        const int rounds = PAIRED ? (it.nt + 1) >> 1 : it.nt;
+        for (int own = 0; own < rounds; ++own) {
+          const int j = PAIRED ? 2 * own + t : own, J = base + j, P = mine + own;
+          if (PAIRED && j >= it.nt) {  // an odd step out: the other group's
+            turn_wait(t);
+            turn_pass(t);
+            continue;
+          }
           ok = ok && wait(sh, &sh.s_full[t][J % RING], (J / RING) & 1);
           tcgen05_after_sync();
           const uint32_t s_at = lanes + t * 128 + (P & 1) * BN;
@@ -514,16 +554,17 @@ __global__ void __launch_bounds__(NT, 1) attn_tile_kernel(const __grid_constant_
             const float f = need ? ex2(ref - top) : 1.f;
             if (need) ref = top;
             l *= f;
-            if (j > 0) {  // the product before must be in, and this step's waits for these weights
-              ok = ok && wait(sh, &sh.pv_done[t][(J - 1) % RING], ((J - 1) / RING) & 1);
+            if (own > 0) {  // the product before must be in, and this step's waits for these weights
+              constexpr int back = PAIRED ? 2 : 1;
+              ok = ok && wait(sh, &sh.pv_done[t][(J - back) % RING], ((J - back) / RING) & 1);
               tcgen05_after_sync();
 #pragma unroll 1
-              for (int c = 0; c < 64 * DC; c += 32) {
+              for (int d = 0; d < 64 * DC; d += 32) {
                 float o[32];
-                tmem_load32(o_at + c, o);
+                tmem_load32(o_at + d, o);
 #pragma unroll
                 for (int k = 0; k < 32; ++k) o[k] *= f;
-                tmem_store32(o_at + c, o);
+                tmem_store32(o_at + d, o);
               }
             }
           }
@@ -539,7 +580,7 @@ __global__ void __launch_bounds__(NT, 1) attn_tile_kernel(const __grid_constant_
           // exponentials to the FP32 pipes by a polynomial (one pair in eight, or in four) took
           // 2 to 4 % longer: those pipes do the scaling and the sums already.
           uint32_t p[32];
-          if (it.mt == 2) turn_wait(t);
+          if (both) turn_wait(t);
 #pragma unroll
           for (int k = 0; k < 32; ++k) {
             float x, y;
@@ -550,7 +591,7 @@ __global__ void __launch_bounds__(NT, 1) attn_tile_kernel(const __grid_constant_
             p[k] = Half16<T>::pack(x, y);
           }
           tmem_store32(s_at, p);
-          if (it.mt == 2) turn_pass(t);
+          if (both) turn_pass(t);
           float sx, sy;
           unpack2(add2(sum[0], sum[1]), sx, sy);
           l += sx + sy;
@@ -561,11 +602,29 @@ __global__ void __launch_bounds__(NT, 1) attn_tile_kernel(const __grid_constant_
       }
       base += it.nt;
       if (t < it.mt) mine += it.nt;
-      if (t < it.mt) {
-        if (ok && it.nt > 0) {
-          ok = wait(sh, &sh.pv_done[t][(base - 1) % RING], ((base - 1) / RING) & 1);
-          tcgen05_after_sync();
+      const int last = PAIRED ? ((it.nt - 1 - t) & ~1) + t : base - 1;  // this group's last step
+      float f0 = 1.f, f1 = 0.f;                                         // PAIRED: the two outputs' factors
+      bool second = false;
+      if ((PAIRED ? last >= 0 && it.nt > t : t < it.mt && it.nt > 0) && ok) {
+        ok = wait(sh, &sh.pv_done[t][last % RING], (last / RING) & 1);
+        tcgen05_after_sync();
+      }
+      if (PAIRED) {
+        if (t == 1) sh.pair[row] = make_float2(ref, ok ? l : __int_as_float(0x7fc00000));
+        tcgen05_before_sync();
+        asm volatile("bar.sync 3, 256;" ::: "memory");
+        tcgen05_after_sync();
+        if (t == 0) {
+          const float2 other = sh.pair[row];
+          const float top = fmaxf(ref, other.x), at = top == -INFINITY ? 0.f : top;
+          second = it.nt > 1;
+          f0 = ex2(ref - at);
+          f1 = ex2(other.x - at);
+          l = second ? l * f0 + other.y * f1 : l * f0;
+          ref = top;
         }
+      }
+      if (t < it.mt) {
         ok = __all_sync(0xffffffffu, ok && !sh.abort);
         const bool any_bad = *static_cast<volatile int*>(&sh.any_bad) != 0;
         const float inv = !ok ? __int_as_float(0x7fc00000) : (l == 0.f ? 0.f : (direct ? 1.f / l : 1.f));
@@ -574,6 +633,17 @@ __global__ void __launch_bounds__(NT, 1) attn_tile_kernel(const __grid_constant_
           float o[32];
           if (ok && it.nt > 0) {
             tmem_load32(o_at + c, o);
+            if (PAIRED) {
+              if (second) {
+                float o1[32];
+                tmem_load32(o_at + 128 + c, o1);
+#pragma unroll
+                for (int k = 0; k < 32; ++k) o[k] = o[k] * f0 + o1[k] * f1;
+              } else {
+#pragma unroll
+                for (int k = 0; k < 32; ++k) o[k] *= f0;
+              }
+            }
           } else {
 #pragma unroll
             for (int k = 0; k < 32; ++k) o[k] = 0.f;
@@ -700,23 +770,30 @@ bool encode(CUtensorMap* map, const AttnArgs& a, const void* base, int64_t slots
                      CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <typename T, int DC>
+template <typename T, int DC, bool PAIRED>
 cudaError_t tile(const AttnArgs& a, const Maps& maps, bool prefix, int tiles_m, cudaStream_t stream) {
   const int64_t rows_m = (int64_t)(prefix ? a.rows : 1) * a.n * a.group;
   const int64_t S = prefix ? a.p_splits : (a.o_splits ? a.o_splits : 1);
   const int64_t units = prefix ? a.kv_heads : (int64_t)a.rows * a.kv_heads;
   const int64_t items = (rows_m + tiles_m * BM - 1) / (tiles_m * BM) * S * units;
-  if (items >= (int64_t)1 << 31) return cudaErrorInvalidValue;
-  const cudaError_t e = allow_smem<attn_tile_kernel<T, DC>>(Layout<DC>::kBytes);
+  if (items >= (int64_t)1 << 31 || (PAIRED && items > kSMs)) return cudaErrorInvalidValue;
+  const cudaError_t e = allow_smem<attn_tile_kernel<T, DC, PAIRED>>(Layout<DC>::kBytes);
   if (e != cudaSuccess) return e;
-  attn_tile_kernel<T, DC><<<(unsigned)(items < kSMs ? items : kSMs), NT, Layout<DC>::kBytes, stream>>>(
+  attn_tile_kernel<T, DC, PAIRED><<<(unsigned)(items < kSMs ? items : kSMs), NT, Layout<DC>::kBytes, stream>>>(
       a, maps, prefix, tiles_m, (int)units, (int)items);
   return cudaGetLastError();
 }
 
+template <typename T>
+cudaError_t tile_any(const AttnArgs& a, const Maps& maps, bool prefix, const TileSplit& x, cudaStream_t stream) {
+  if (a.dim <= 64)
+    return x.paired ? tile<T, 1, true>(a, maps, prefix, 1, stream) : tile<T, 1, false>(a, maps, prefix, x.tiles, stream);
+  return x.paired ? tile<T, 2, true>(a, maps, prefix, 1, stream) : tile<T, 2, false>(a, maps, prefix, x.tiles, stream);
+}
+
 }  // namespace
 
-cudaError_t launch_attn_tile(const AttnArgs& args, bool prefix, int tiles_m, cudaStream_t stream) {
+cudaError_t launch_attn_tile(const AttnArgs& args, bool prefix, const TileSplit& split, cudaStream_t stream) {
   AttnArgs a = args;
   // A scale of zero weighs all slots alike; a tiny one does so without 0 * inf at the mask.
   if (fabsf(a.scale) < 1e-30f) a.scale = 1e-30f;
@@ -735,11 +812,8 @@ cudaError_t launch_attn_tile(const AttnArgs& args, bool prefix, int tiles_m, cud
     maps.row_mul = a.kv_row != 0;
   }
   if (!ok) return cudaErrorInvalidValue;
-  if (a.dtype == 1)
-    return a.dim <= 64 ? tile<__half, 1>(a, maps, prefix, tiles_m, stream)
-                       : tile<__half, 2>(a, maps, prefix, tiles_m, stream);
-  return a.dim <= 64 ? tile<__nv_bfloat16, 1>(a, maps, prefix, tiles_m, stream)
-                     : tile<__nv_bfloat16, 2>(a, maps, prefix, tiles_m, stream);
+  return a.dtype == 1 ? tile_any<__half>(a, maps, prefix, split, stream)
+                      : tile_any<__nv_bfloat16>(a, maps, prefix, split, stream);
 }
 
 }  // namespace sv

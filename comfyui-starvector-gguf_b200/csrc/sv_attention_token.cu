@@ -643,6 +643,76 @@ __global__ void __launch_bounds__(256) scores_weights_kernel(const __grid_consta
   a.weights[r * a.w_row + h * a.w_head + j] += sum;
 }
 
+// Accumulated weights of calls with many query rows: w[slot] += sum of 2^(s - lse) over
+// the group's rows.  A warp holds 16 slots' keys as the A operand and walks the query
+// rows 8 at a time as the B operand, both straight from global memory as above; the
+// queries come from L1 for seven of a block's eight warps.  One warp owns its slots, so
+// the sum's order is fixed and no atomics are needed.  Bound by the products.
+template <typename T, int DC, bool FULL>
+__global__ void __launch_bounds__(NT) attn_weights16_kernel(const __grid_constant__ AttnArgs a) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+  const int unit = blockIdx.y, h = unit % a.kv_heads, r = unit / a.kv_heads, nG = a.n * a.group, vecs = a.dim >> 3;
+  const RowSpan sp = row_span(a, r);
+  const int j0 = (blockIdx.x * NW + warp) * 16;
+  if (j0 >= sp.end || j0 + 16 <= sp.start) return;
+  const T* kb = static_cast<const T*>(a.k) + r * a.kv_row + h * a.kv_head;
+  uint4 kf[2][2 * DC], qf[2 * DC], qn[2 * DC];
+#pragma unroll
+  for (int x = 0; x < 2; ++x)
+#pragma unroll
+    for (int u = 0; u < 2 * DC; ++u)
+      kf[x][u] = load_stream(kb + (j0 + g + 8 * x) * a.kv_slot + (4 * u + t) * 8,
+                             j0 + g + 8 * x < sp.end && (FULL || 4 * u + t < vecs));
+  const int first_pos = sp.end - a.n;
+  int m_first, m_end;
+  weight_rows(a, sp, j0, 16, blockIdx.z, m_first, m_end);
+  auto load_q = [&](int m0) {
+    const int m = m0 + g, i = m / a.group;
+    const T* src = static_cast<const T*>(a.q) + r * a.q_row + i * a.q_tok +
+                   (int64_t)(h * a.group + m - i * a.group) * a.q_head;
+#pragma unroll
+    for (int u = 0; u < 2 * DC; ++u)
+      qn[u] = m < nG && (FULL || 4 * u + t < vecs) ? __ldg(reinterpret_cast<const uint4*>(src) + 4 * u + t)
+                                                   : make_uint4(0u, 0u, 0u, 0u);
+  };
+  float sum[2] = {0.f, 0.f};
+  const float* lse = a.lse + (int64_t)unit * nG;
+  load_q(m_first);
+  for (int m0 = m_first; m0 < m_end; m0 += 8) {
+#pragma unroll
+    for (int u = 0; u < 2 * DC; ++u) qf[u] = qn[u];
+    load_q(m0 + 8);
+    float l[2], c[2][4];
+    int pos[2], low[2];
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int m = m0 + 2 * t + e;
+      l[e] = m < m_end ? lse[m] : INFINITY;
+      pos[e] = first_pos + m / a.group;
+      low[e] = window_low(a, sp.start, pos[e]);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) c[e][k] = 0.f;
+    }
+#pragma unroll
+    for (int u = 0; u < 2 * DC; ++u) {
+      Mma<T>::run(c[0], kf[0][u].x, kf[1][u].x, kf[0][u].y, kf[1][u].y, qf[u].x, qf[u].y);
+      Mma<T>::run(c[1], kf[0][u].z, kf[1][u].z, kf[0][u].w, kf[1][u].w, qf[u].z, qf[u].w);
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int j = j0 + g + 8 * (k >> 1), e = k & 1;
+      if (slot_seen(a, sp.start, pos[e], low[e], j)) sum[k >> 1] += ex2((c[0][k] + c[1][k]) * a.scale - l[e]);
+    }
+  }
+#pragma unroll
+  for (int x = 0; x < 2; ++x) {
+    sum[x] += __shfl_xor_sync(0xffffffffu, sum[x], 1);
+    sum[x] += __shfl_xor_sync(0xffffffffu, sum[x], 2);
+    const int j = j0 + g + 8 * x;
+    if (t == 0 && j >= sp.start && j < sp.end) add_weight(a, unit, r, h, j, blockIdx.z, sum[x]);
+  }
+}
+
 template <typename T, int DC, bool FULL, bool MULTI>
 cudaError_t token(const AttnArgs& a, int blocks, cudaStream_t stream) {
   constexpr size_t smem = sizeof(float) * NW * 16 * DC * 64;
@@ -666,6 +736,22 @@ template <typename T> cudaError_t token_any(const AttnArgs& a, int blocks, cudaS
 
 cudaError_t launch_attn_token(const AttnArgs& a, int blocks, cudaStream_t stream) {
   return a.dtype == 1 ? token_any<__half>(a, blocks, stream) : token_any<__nv_bfloat16>(a, blocks, stream);
+}
+
+template <typename T> cudaError_t weights16(const AttnArgs& a, cudaStream_t stream) {
+  const dim3 grid((unsigned)((a.capacity + NW * 16 - 1) / (NW * 16)), (unsigned)(a.rows * a.kv_heads),
+                  (unsigned)a.w_splits);
+  if (a.dim == 128)
+    attn_weights16_kernel<T, 2, true><<<grid, NT, 0, stream>>>(a);
+  else if (a.dim > 64)
+    attn_weights16_kernel<T, 2, false><<<grid, NT, 0, stream>>>(a);
+  else
+    attn_weights16_kernel<T, 1, false><<<grid, NT, 0, stream>>>(a);
+  return cudaGetLastError();
+}
+
+cudaError_t launch_weights16(const AttnArgs& a, cudaStream_t stream) {
+  return a.dtype == 1 ? weights16<__half>(a, stream) : weights16<__nv_bfloat16>(a, stream);
 }
 
 cudaError_t launch_scores_weights(const AttnArgs& a, cudaStream_t stream) {
