@@ -26,6 +26,8 @@
 // several blocks leaves partial results, which the last block to arrive joins, in
 // block order (so results repeat bit for bit); past 32 parts in two levels, so that no
 // block joins more than a few dozen.  The sums' counters return to zero.
+#include <type_traits>
+
 #include "sv_attention.h"
 
 namespace sv {
@@ -272,31 +274,47 @@ __global__ void __launch_bounds__(NT, kTokenPerSM) attn_token_kernel(const __gri
           joined[m].y == 0.f ? INFINITY : joined[m].x + log2f(joined[m].y);
   };
   // Joins `count` parts of a unit (and, `last`, the prefix's), the k-th that of block
-  // b0 + k * step; c_first is the unit's first block.
-  auto join = [&](const Part& p, int c_first, int b0, int step, int count, bool last) {
-    const int more = last ? a.p_splits : 0;
+  // b0 + k * step; c_first is the unit's first block.  ahead: the first parts' values are
+  // fetched while the factors are made (where registers are free).
+  auto join = [&](const Part& p, int c_first, int b0, int step, int count, bool last, auto ahead) {
+    constexpr int ITEMS = (16 * DC * 16 + NT - 1) / NT, AHEAD = decltype(ahead)::value ? 6 : 0;
+    const int more = last ? a.p_splits : 0, all_parts = count + more;
     if (more) wait_before();  // the prefix's kernel may have run beside this one
     const int64_t row0 = prefix_index(a, p.r, p.h, 0);
     auto slot_of = [&](int k) { return 2 * (b0 + k * step) + (b0 + k * step == c_first); };
-    auto part_at = [&](int k, int m, int d) {
+    // Row m (of nG) and first dimension of this thread's x-th vector of four.
+    int m[ITEMS], d[ITEMS];
+#pragma unroll
+    for (int x = 0; x < ITEMS; ++x) {
+      m[x] = (tid + x * NT) / row_vecs;
+      d[x] = (tid + x * NT - m[x] * row_vecs) * 4;
+    }
+    auto part_at = [&](int k, int x) {
       return __ldcg(reinterpret_cast<const float4*>(
-          k < count ? a.part_o + ((int64_t)slot_of(k) * 16 + m) * D + d
-                    : a.prefix_o + ((int64_t)(k - count) * all_rows + row0 + m) * D + d));
+          k < count ? a.part_o + ((int64_t)slot_of(k) * 16 + m[x]) * D + d[x]
+                    : a.prefix_o + ((int64_t)(k - count) * all_rows + row0 + m[x]) * D + d[x]));
     };
     __syncthreads();
-    for (int x = tid; x < (count + more) * 16; x += NT) {
-      const int k = x >> 4, m = x & 15;
-      if (m < nG)
-        part_ml[k][m] = __ldcg(k < count ? a.part_ml + slot_of(k) * 16 + m
-                                         : a.prefix_ml + (int64_t)(k - count) * all_rows + row0 + m);
+    float4 early[AHEAD ? AHEAD : 1][ITEMS];
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k)
+#pragma unroll
+      for (int x = 0; x < ITEMS; ++x)
+        if (k < all_parts && m[x] < nG) early[k][x] = part_at(k, x);
+    for (int x = tid; x < all_parts * 16; x += NT) {
+      const int k = x >> 4, mm = x & 15;
+      if (mm < nG)
+        part_ml[k][mm] = __ldcg(k < count ? a.part_ml + slot_of(k) * 16 + mm
+                                          : a.prefix_ml + (int64_t)(k - count) * all_rows + row0 + mm);
     }
     __syncthreads();
     if (tid < nG) {
       float M = -INFINITY;
-      for (int k = 0; k < count + more; ++k) M = fmaxf(M, part_ml[k][tid].x);
+      for (int k = 0; k < all_parts; ++k) M = fmaxf(M, part_ml[k][tid].x);
       const float at = M == -INFINITY ? 0.f : M;
       float L = 0.f;
-      for (int k = 0; k < count + more; ++k) {
+#pragma unroll 4
+      for (int k = 0; k < all_parts; ++k) {
         const float2 ml = part_ml[k][tid];
         const float f = ml.y == 0.f ? 0.f : ex2(ml.x - at);
         factor[k][tid] = f;
@@ -305,21 +323,33 @@ __global__ void __launch_bounds__(NT, kTokenPerSM) attn_token_kernel(const __gri
       joined[tid] = make_float2(M, L);
     }
     __syncthreads();
-    for (int x = tid; x < nG * row_vecs; x += NT) {
-      const int m = x / row_vecs, d = (x - m * row_vecs) * 4;
-      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-      auto add = [&](float4 y, float f) {
-        v.x = fmaf(y.x, f, v.x);
-        v.y = fmaf(y.y, f, v.y);
-        v.z = fmaf(y.z, f, v.z);
-        v.w = fmaf(y.w, f, v.w);
-      };
+    float4 v[ITEMS];
+#pragma unroll
+    for (int x = 0; x < ITEMS; ++x) v[x] = make_float4(0.f, 0.f, 0.f, 0.f);
+    auto add = [&](int x, float4 y, float f) {
+      v[x].x = fmaf(y.x, f, v[x].x);
+      v[x].y = fmaf(y.y, f, v[x].y);
+      v[x].z = fmaf(y.z, f, v[x].z);
+      v[x].w = fmaf(y.w, f, v[x].w);
+    };
+#pragma unroll
+    for (int x = 0; x < ITEMS; ++x) {
+#pragma unroll
+      for (int k = 0; k < AHEAD; ++k)
+        if (k < all_parts && m[x] < nG) add(x, early[k][x], factor[k][m[x]]);
+    }
 #pragma unroll 4
-      for (int k = 0; k < count + more; ++k) add(part_at(k, m, d), factor[k][m]);
+    for (int k = AHEAD; k < all_parts; ++k)
+#pragma unroll
+      for (int x = 0; x < ITEMS; ++x)
+        if (m[x] < nG) add(x, part_at(k, x), factor[k][m[x]]);
+#pragma unroll
+    for (int x = 0; x < ITEMS; ++x) {
+      if (m[x] >= nG) continue;
       if (last)
-        write_out(p, m, d, v, joined[m].y);
+        write_out(p, m[x], d[x], v[x], joined[m[x]].y);
       else
-        *reinterpret_cast<float4*>(a.part_o + ((int64_t)slot_of(0) * 16 + m) * D + d) = v;
+        *reinterpret_cast<float4*>(a.part_o + ((int64_t)slot_of(0) * 16 + m[x]) * D + d[x]) = v[x];
     }
     if (tid < nG) {
       if (last)
@@ -573,7 +603,7 @@ __global__ void __launch_bounds__(NT, kTokenPerSM) attn_token_kernel(const __gri
       else
         a.part_ml[slot * 16 + tid] = joined[tid];
     }
-    if (alone && a.prefix) join(p, c, c, 1, 1, true);
+    if (alone && a.prefix) join(p, c, c, 1, 1, true, std::false_type());
     if (!alone) shared_part[shared_parts++] = p;
     if (a.status && tid == 0 && p.h == K - 1 && p.end <= c1) {
       const int e = a.lengths ? a.lengths[p.r] : a.capacity, s = a.starts ? a.starts[p.r] : 0;
@@ -608,7 +638,7 @@ __global__ void __launch_bounds__(NT, kTokenPerSM) attn_token_kernel(const __gri
     int step = 1, count = parts;
     if (parts > kMaxFlat) {
       const int first = c_first + (c - c_first) / kJoin * kJoin;
-      join(p, c_first, first, 1, min(kJoin, c_first + parts - first), false);
+      join(p, c_first, first, 1, min(kJoin, c_first + parts - first), false, std::false_type());
       step = kJoin;
       count = (parts + kJoin - 1) / kJoin;
       __syncthreads();
@@ -616,7 +646,7 @@ __global__ void __launch_bounds__(NT, kTokenPerSM) attn_token_kernel(const __gri
       __syncthreads();
       if (!sh_last[x]) continue;
     }
-    join(p, c_first, c_first, step, count, true);
+    join(p, c_first, c_first, step, count, true, std::true_type());
   }
   wait_before();
 }
