@@ -27,6 +27,7 @@
 #include <cstdint>
 
 #include "../../include/starvector_sampling.h"
+#include "sv_attention.h"
 
 namespace {
 
@@ -435,6 +436,10 @@ __global__ void __launch_bounds__(NT, PER_SM) kv_evict_kernel(const EvictArgs a)
   }
 }
 
+template <auto K> struct Kernel {
+  static constexpr auto value = K;
+};
+
 }  // namespace
 
 // See include/starvector_sampling.h.
@@ -491,11 +496,18 @@ extern "C" int sv_kv_evict(void* keys, void* values, int32_t elem_bytes, int32_t
   const bool in_smem = capacity <= kSmemKeys;
   const size_t nw = (capacity + 31) / 32;
   const size_t smem = 4 * (3 * nw + 2 + (in_smem ? 2 * ((capacity + 3) & ~3) : 0));
-  auto kernel = many ? (in_smem ? kv_evict_kernel<256, 7, true> : kv_evict_kernel<256, 7, false>)
-                     : (in_smem ? kv_evict_kernel<1024, 1, true> : kv_evict_kernel<1024, 1, false>);
-  if (smem > 40 * 1024 &&
-      cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
-    return SV_E_CUDA;
-  kernel<<<dim3(a.parts, units), many ? 256 : 1024, smem, static_cast<cudaStream_t>(stream)>>>(a);
-  return cudaGetLastError() == cudaSuccess ? SV_OK : SV_E_CUDA;
+  static_assert(4 * (3 * (kSmemKeys / 32) + 2 + 2 * kSmemKeys) <= 220 * 1024, "the keys fit a block's shared memory");
+  cudaError_t e;
+  auto run = [&](auto which) {
+    constexpr auto kernel = decltype(which)::value;
+    e = smem > 40 * 1024 ? sv::allow_smem<kernel>(220 * 1024) : cudaSuccess;
+    if (e != cudaSuccess) return;
+    kernel<<<dim3(a.parts, units), many ? 256 : 1024, smem, static_cast<cudaStream_t>(stream)>>>(a);
+    e = cudaGetLastError();
+  };
+  if (many)
+    in_smem ? run(Kernel<kv_evict_kernel<256, 7, true>>()) : run(Kernel<kv_evict_kernel<256, 7, false>>());
+  else
+    in_smem ? run(Kernel<kv_evict_kernel<1024, 1, true>>()) : run(Kernel<kv_evict_kernel<1024, 1, false>>());
+  return e == cudaSuccess ? SV_OK : SV_E_CUDA;
 }

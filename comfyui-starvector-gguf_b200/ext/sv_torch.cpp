@@ -6,10 +6,11 @@
 // returns its code (0 or a negative SV_E_*; ops.py turns codes into the same
 // exceptions as before).  Shapes and the history form are decided by the Python
 // wrappers (ops.py), which pass the same sizes and strides as the C signatures;
-// nothing here synchronises or allocates.  The attention functions are called once per
-// layer and token, where each tensor attribute read from Python counts: they look at
-// the shapes here (ValueError where ops.py would raise one) and allocate their outputs
-// and a workspace kept per device, stream and size; so does kv_evict its outputs.
+// nothing here synchronises or allocates.  The cache operators (window_attention,
+// prefix_attention, kv_evict) are called once per layer or token, where each tensor
+// attribute read from Python counts: they look at the shapes here (ValueError where
+// ops.py would raise one) and allocate their outputs, the attention functions also a
+// workspace kept per device, stream and size.
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
@@ -355,31 +356,46 @@ std::tuple<int, at::Tensor> prefix_attention(const at::Tensor& q_in, const at::T
   return {rc, o};
 }
 
-// sv_kv_evict.  keys / values [layers, rows, heads, capacity, head_dim], weights /
-// positions [layers, rows, heads, capacity] contiguous.
-std::tuple<int, at::Tensor, at::Tensor, at::Tensor> kv_evict(const at::Tensor& keys, const OptT& values,
-                                                             const at::Tensor& weights, const at::Tensor& positions,
-                                                             const OptT& lengths, int64_t budget, int64_t sinks,
-                                                             int64_t recent, const OptT& weights_out,
-                                                             const OptT& positions_out, const OptT& lengths_out,
-                                                             const OptT& out_status) {
+// sv_kv_evict.  keys / values [layers, rows, (heads,) capacity, head_dim], weights /
+// positions the same without head_dim.  lengths_in: a tensor, a number or none.
+std::tuple<int, at::Tensor, at::Tensor, at::Tensor> kv_evict(
+    const at::Tensor& keys, const OptT& values, const at::Tensor& weights, const at::Tensor& positions,
+    const OptT& lengths_in, std::optional<int64_t> length, int64_t budget, int64_t sinks, int64_t recent,
+    const OptT& weights_out, const OptT& positions_out, const OptT& lengths_out, const OptT& out_status) {
   const at::Device dev = keys.device();
   on_device(keys, dev, "keys");
+  TORCH_CHECK_VALUE(keys.dim() == 4 || keys.dim() == 5,
+                    "keys must be [layers, rows, capacity, head_dim] or [layers, rows, heads, capacity, head_dim]");
+  const int64_t last = keys.dim() - 1;
+  const bool heads_dim = keys.dim() == 5;
+  TORCH_CHECK_VALUE(stride_of(keys, last) <= 1, "head_dim must be contiguous");
+  TORCH_CHECK_VALUE(!values.has_value() || (values->sizes() == keys.sizes() && values->strides() == keys.strides() &&
+                                            values->scalar_type() == keys.scalar_type()),
+                    "values must have the keys' shape, strides and dtype");
+  TORCH_CHECK_VALUE(weights.scalar_type() == at::kFloat && positions.scalar_type() == at::kInt &&
+                        weights.sizes() == keys.sizes().slice(0, last) && positions.sizes() == weights.sizes(),
+                    "weights (float32) and positions (int32) must have the keys' shape without head_dim");
+  const int64_t layers = keys.size(0), rows = keys.size(1), heads = heads_dim ? keys.size(2) : 1;
+  const int64_t capacity = keys.size(last - 1), all = layers * rows * heads * capacity;
+  TORCH_CHECK_VALUE(budget >= 1 && budget <= capacity, "budget must be in [1, capacity]");
+  TORCH_CHECK_VALUE(sinks >= 0 && recent >= 0 && sinks + recent <= budget,
+                    "sinks and recent must not be negative and must fit in the budget");
+  TORCH_CHECK_VALUE(!length.has_value() || (*length >= 0 && *length <= capacity), "lengths must be in [0, capacity]");
   const c10::cuda::CUDAGuard guard(dev);
-  const int64_t layers = keys.size(0), rows = keys.size(1), heads = keys.size(2), capacity = keys.size(3);
-  const int64_t all = layers * rows * heads * capacity;
-  at::Tensor wo = weights_out.has_value() ? *weights_out : at::empty_like(weights);
-  at::Tensor po = positions_out.has_value() ? *positions_out : at::empty_like(positions);
-  at::Tensor lo = lengths_out.has_value() ? *lengths_out
-                                          : at::empty({rows}, at::TensorOptions().dtype(at::kInt).device(dev));
+  const auto ints = at::TensorOptions().dtype(at::kInt).device(dev);
+  OptT lengths = row_ints(lengths_in, rows, dev, "lengths");
+  if (length.has_value()) lengths = at::full({rows}, *length, ints);
+  at::Tensor wo = weights_out.has_value() ? *weights_out : at::empty(weights.sizes(), weights.options());
+  at::Tensor po = positions_out.has_value() ? *positions_out : at::empty(positions.sizes(), positions.options());
+  at::Tensor lo = lengths_out.has_value() ? *lengths_out : at::empty({rows}, ints);
   TORCH_CHECK(weights.is_contiguous() && positions.is_contiguous() && wo.is_contiguous() && po.is_contiguous() &&
                   lo.is_contiguous(),
               "weights and positions must be contiguous");
   const int rc = sv_kv_evict(
       keys.data_ptr(), raw(values, dev, "values"), (int32_t)keys.element_size(), (int32_t)layers, (int32_t)rows,
-      (int32_t)heads, (int32_t)capacity, (int32_t)keys.size(4), stride_of(keys, 0), stride_of(keys, 1),
-      stride_of(keys, 2), stride_of(keys, 3), ptr<float>(weights, dev, "weights", at::kFloat, all),
-      ptr<int32_t>(positions, dev, "positions", at::kInt, all),
+      (int32_t)heads, (int32_t)capacity, (int32_t)keys.size(last), stride_of(keys, 0), stride_of(keys, 1),
+      heads_dim ? stride_of(keys, 2) : 0, stride_of(keys, last - 1),
+      ptr<float>(weights, dev, "weights", at::kFloat, all), ptr<int32_t>(positions, dev, "positions", at::kInt, all),
       optptr<int32_t>(lengths, dev, "lengths", at::kInt, rows), (int32_t)budget, (int32_t)sinks, (int32_t)recent,
       ptr<float>(wo, dev, "weights_out", at::kFloat, all), ptr<int32_t>(po, dev, "positions_out", at::kInt, all),
       ptr<int32_t>(lo, dev, "lengths_out", at::kInt, rows), optptr<int32_t>(out_status, dev, "status", at::kInt, rows),

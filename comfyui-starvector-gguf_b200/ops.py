@@ -564,17 +564,6 @@ def _first_slots(keys, values, length):
     return keys.narrow(-2, 0, length), values.narrow(-2, 0, length)
 
 
-def _row_ints(t, rows, device, name):
-    """A per-row int32 tensor from a tensor of whole numbers (None stays None)."""
-    if t is None or isinstance(t, int):
-        return None
-    if not isinstance(t, torch.Tensor) or t.dtype not in (torch.int32, torch.int64) or t.numel() != rows:
-        raise ValueError(f"{name} must be an int32 or int64 tensor with one value per row")
-    if t.dtype == torch.int32 and t.device == device and t.is_contiguous():
-        return t
-    return t.reshape(-1).to(device=device, dtype=torch.int32).contiguous()
-
-
 def window_attention(q, keys, values, lengths=None, *, starts=None, window=0, sinks=0, scale=None, weights=None,
                      out=None, status=None):
     """Attention over one layer of the decoder's cache with a sliding window and a few
@@ -628,33 +617,12 @@ def kv_evict(keys, values, weights, positions, lengths=None, budget=None, *, sin
     (all slots).  Returns a dict of new tensors (or fills `out`): lengths, weights
     and positions after the eviction; the slots' order is not the tokens' order any
     more, so attend to such a cache without a window."""
-    _need_cuda(keys, "keys")
-    k, v = keys, values
-    if k.dim() == 4:
-        k = k.unsqueeze(2)
-        v = None if v is None else v.unsqueeze(2)
-    if k.dim() != 5:
-        raise ValueError("keys must be [layers, rows, capacity, head_dim] or [layers, rows, heads, capacity, "
-                         "head_dim]")
-    if k.shape[4] > 1 and k.stride(4) != 1:
-        raise ValueError("head_dim must be contiguous")
-    if v is not None and (v.shape != k.shape or v.stride() != k.stride() or v.dtype != k.dtype):
-        raise ValueError("values must have the keys' shape, strides and dtype")
-    if weights.dtype != torch.float32 or positions.dtype != torch.int32 or weights.shape != keys.shape[:-1] or \
-            positions.shape != keys.shape[:-1]:
-        raise ValueError("weights (float32) and positions (int32) must have the keys' shape without head_dim")
-    R, cap = k.shape[1], k.shape[3]
-    if budget is None or not 1 <= budget <= cap:
-        raise ValueError("budget must be in [1, capacity]")
-    if sinks < 0 or recent < 0 or sinks + recent > budget:
-        raise ValueError("sinks and recent must not be negative and must fit in the budget")
-    if isinstance(lengths, int):
-        if not 0 <= lengths <= cap:
-            raise ValueError("lengths must be in [0, capacity]")
-        lengths = torch.full((R,), lengths, dtype=torch.int32, device=k.device)
+    if budget is None:
+        raise ValueError("budget must be given")
+    number = isinstance(lengths, int)
     o = out if out is not None else {}
     rc, o["lengths"], o["weights"], o["positions"] = _ext().kv_evict(
-        k, v, weights, positions, _row_ints(lengths, R, k.device, "lengths"), budget, sinks, recent, o.get("weights"),
-        o.get("positions"), o.get("lengths"), status)
+        keys, values, weights, positions, None if number else lengths, lengths if number else None, budget, sinks,
+        recent, o.get("weights"), o.get("positions"), o.get("lengths"), status)
     L.check(rc, "sv_kv_evict")
     return o
