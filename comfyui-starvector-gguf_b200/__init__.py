@@ -1,4 +1,5 @@
-"""B200-native (sm_100a) decode-sampling step of ComfyUI-StarVector-GGUF.
+"""B200-native (sm_100a) decode-sampling step of ComfyUI-StarVector-GGUF, and the
+operators that read and trim the decoder's KV cache.
 
 Layout:
   csrc/               CUDA kernels and the extern "C" layer (include/starvector_sampling.h)
