@@ -10,6 +10,8 @@ namespace {
 
 constexpr int kSMs = 148;
 constexpr int kMostPrefixSplits = 16;  // that the token kernel joins
+constexpr int kMostSlots = 1 << 29;    // sums of two slot numbers stay in 31 bits
+constexpr size_t kMostScores = (size_t)256 << 20;  // bytes of scores kept for the accumulated weights
 
 size_t up256(size_t x) { return (x + 255) / 256 * 256; }
 
@@ -80,6 +82,7 @@ Plan make_plan(const AttnArgs& a) {
     p.o_bytes = up256((size_t)2 * kTokenBlocks * 16 * a.dim * 4);
     p.ml_bytes = up256((size_t)2 * kTokenBlocks * 16 * 8);
     p.score_bytes = a.weights ? up256(all * a.capacity * 4) : 0;
+    if (p.score_bytes > kMostScores) p.score_bytes = 0;  // the weights take a second product instead
   } else {
     if (f32) {
       const int64_t slots = most_slots(a.capacity, a.window, a.sinks, div_up(16, a.group));
@@ -94,7 +97,7 @@ Plan make_plan(const AttnArgs& a) {
   }
   p.lse_bytes = a.weights ? up256(all * 4) : 0;
   p.w_splits = 1;
-  if (a.weights && !p.token) {  // about four blocks per SM, at least 64 query rows each
+  if (a.weights && !p.score_bytes) {  // about four blocks per SM, at least 64 query rows each
     const int64_t want = 4 * kSMs / (units * div_up(a.capacity, f32 ? 64 : 128)), most = div_up(nG, 64);
     const int64_t s = want < most ? want : most;
     p.w_splits = (int)(s < 1 ? 1 : s);
@@ -109,9 +112,7 @@ int check_shapes(const AttnArgs& a) {
     return SV_E_SHAPE;
   if (a.dim < 8 || a.dim > kAttnMaxDim || a.dim % 8) return SV_E_SHAPE;
   if ((int64_t)a.rows * a.kv_heads > 65535 || (int64_t)a.rows * a.n * a.heads > (int64_t)1 << 30) return SV_E_SHAPE;
-  if (a.window < 0 || a.sinks < 0 || a.window > 1 << 30 || a.sinks > 1 << 30 || a.capacity > 1 << 30 ||
-      a.prefix > 1 << 30)
-    return SV_E_SHAPE;
+  if (a.window < 0 || a.sinks < 0 || a.capacity > kMostSlots || a.prefix > kMostSlots) return SV_E_SHAPE;
   // The token kernel counts chunks of 64 slots in 31 bits (a cache of broadcast rows could exceed them).
   if ((int64_t)a.rows * a.kv_heads * (a.capacity / 64 + 3) >= (int64_t)1 << 31) return SV_E_SHAPE;
   return SV_OK;
@@ -128,7 +129,16 @@ int check_pointers(const AttnArgs& a, double scale) {
   for (const void* p : ptrs)
     if (reinterpret_cast<uintptr_t>(p) % 16) return SV_E_ALIGN;
   if (a.weights && (a.w_row < 0 || a.w_head < 0)) return SV_E_SHAPE;
+  // One slot for all positions is no cache (and no dimension of a copy).
+  if ((a.capacity > 1 && a.kv_slot == 0) || (a.prefix > 1 && a.p_slot == 0)) return SV_E_SHAPE;
   return SV_OK;
+}
+
+// The accumulated weights by a second product, from the rows' sums.
+int run_weights(const AttnArgs& a, cudaStream_t stream) {
+  if ((a.dtype == SV_F32 ? launch_attn_weights(a, stream) : launch_weights16(a, stream)) != cudaSuccess)
+    return SV_E_CUDA;
+  return a.w_splits > 1 && launch_weights_sum(a, stream) != cudaSuccess ? SV_E_CUDA : SV_OK;
 }
 
 int run(AttnArgs& a, void* workspace, size_t workspace_bytes, cudaStream_t stream) {
@@ -158,16 +168,20 @@ int run(AttnArgs& a, void* workspace, size_t workspace_bytes, cudaStream_t strea
     return SV_E_CUDA;
   if (p.token) {
     if (launch_attn_token(a, kTokenBlocks, stream) != cudaSuccess) return SV_E_CUDA;
-    if (a.weights && launch_scores_weights(a, stream) != cudaSuccess) return SV_E_CUDA;
-    return SV_OK;
+    if (a.scores) return launch_scores_weights(a, stream) == cudaSuccess ? SV_OK : SV_E_CUDA;
+    return a.weights ? run_weights(a, stream) : SV_OK;
   }
   if ((f32 ? launch_attn_f32(a, false, stream) : launch_attn_tile(a, false, p.own, stream)) != cudaSuccess)
     return SV_E_CUDA;
   if (p.o_splits && launch_attn_combine(a, stream) != cudaSuccess) return SV_E_CUDA;
-  if (a.weights && (f32 ? launch_attn_weights(a, stream) : launch_weights16(a, stream)) != cudaSuccess)
-    return SV_E_CUDA;
-  if (p.w_splits > 1 && launch_weights_sum(a, stream) != cudaSuccess) return SV_E_CUDA;
-  return SV_OK;
+  return a.weights ? run_weights(a, stream) : SV_OK;
+}
+
+// Sinks that cover the cache, or a window as wide, leave no limit.
+void set_window(AttnArgs& a, int32_t window, int32_t sinks) {
+  const bool limit = window < a.capacity && sinks < a.capacity;
+  a.window = window < 0 || limit ? window : 0;
+  a.sinks = sinks < 0 || (limit && window > 0) ? sinks : 0;
 }
 
 AttnArgs base_args(int32_t dtype, int32_t rows, int32_t tokens, int32_t heads, int32_t kv_heads, int32_t head_dim,
@@ -195,8 +209,7 @@ size_t sv_window_attention_workspace_bytes(int32_t dtype, int32_t rows, int32_t 
                                            int32_t kv_heads, int32_t head_dim, int32_t capacity, int32_t window,
                                            int32_t sinks, int32_t with_weights) {
   AttnArgs a = base_args(dtype, rows, tokens, heads, kv_heads, head_dim, capacity);
-  a.window = window;
-  a.sinks = sinks;
+  set_window(a, window, sinks);
   if (check_shapes(a)) return 0;
   float dummy;
   a.weights = with_weights ? &dummy : nullptr;
@@ -222,8 +235,7 @@ int sv_window_attention(const void* q, int32_t dtype, int32_t rows, int32_t toke
   a.kv_slot = kv_stride_slot;
   a.lengths = lengths;
   a.starts = starts;
-  a.window = window;
-  a.sinks = sinks;
+  set_window(a, window, sinks);
   a.scale = (float)(scale * 1.4426950408889634);
   a.weights = weights;
   a.w_row = weights_stride_row;

@@ -300,6 +300,8 @@ std::tuple<int, at::Tensor> window_attention(const at::Tensor& q_in, const at::T
   const OptT lengths = row_ints(lengths_in, rows, dev, "lengths"), starts = row_ints(starts_in, rows, dev, "starts");
   const int32_t w = (int32_t)std::min<int64_t>(window, 1 << 30), s = (int32_t)std::min<int64_t>(sinks, 1 << 30);
   at::Tensor o = attention_out(out, q_in);
+  if (o.numel() == 0) return {0, o};
+  if (capacity == 0) return {0, o.zero_()};  // no slots: every query sees nothing
   const size_t bytes =
       sv_window_attention_workspace_bytes(code, rows, n, heads, kv, dim, capacity, w, s, weights.has_value());
   at::Tensor ws = workspace_for(dev, stream, bytes, 4 * ((size_t)rows * kv + 1024));
@@ -343,6 +345,12 @@ std::tuple<int, at::Tensor> prefix_attention(const at::Tensor& q_in, const at::T
   const int32_t prefix = (int32_t)prefix_length.value_or(pk.size(1));
   const OptT lengths = row_ints(lengths_in, rows, dev, "lengths");
   at::Tensor o = attention_out(out, q_in);
+  if (o.numel() == 0) return {0, o};
+  if (capacity == 0) {  // no own slots: as a cache of one that no row has filled
+    const at::Tensor none = at::zeros({rows, kv, 1, dim}, q.options());
+    return prefix_attention(q, pk, pv, none, none, at::zeros({rows}, at::TensorOptions().dtype(at::kInt).device(dev)),
+                            prefix, scale, o.view(q.sizes()), out_status);
+  }
   const size_t bytes = sv_prefix_attention_workspace_bytes(code, rows, n, heads, kv, dim, prefix, capacity);
   at::Tensor ws = workspace_for(dev, stream, bytes, 4 * ((size_t)rows * kv + 1024));
   const int rc = sv_prefix_attention(

@@ -407,7 +407,10 @@ int sv_beam_advance(const int64_t* picks, const float* pick_scores, const int32_
  * Scores, softmax and sums are f32; the 16-bit kernels round the weights to the
  * inputs' type before they multiply the values.  head_dim a multiple of 8, 8..128;
  * heads a multiple of kv_heads; rows * kv_heads <= 65535; rows * tokens * heads <=
- * 2^30; pointers and every stride in bytes multiples of 16.
+ * 2^30; capacity (and prefix_length) <= 2^29, with a slot stride other than 0 (rows and
+ * heads may be broadcast); pointers and every stride in bytes multiples of 16.  A wait
+ * inside a kernel that runs out (~2 s) gives NaN outputs and SV_ST_TIMEOUT (the latter
+ * not where it is the prefix's).
  *   out_status  int32 [rows] or NULL
  */
 size_t sv_window_attention_workspace_bytes(int32_t dtype, int32_t rows, int32_t tokens, int32_t heads,

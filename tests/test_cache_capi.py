@@ -21,6 +21,7 @@ WINDOW = dict(q=16, dtype=1, rows=2, tokens=1, heads=16, kv_heads=1, head_dim=12
     (dict(sinks=-1), -3), (dict(scale=float("nan")), -4), (dict(scale=float("inf")), -4), (dict(q=8), -5),
     (dict(kv_slot=100), -5), (dict(q_head=-128), -5), (dict(out=24), -5), (dict(weights=16, w_row=-1), -3),
     (dict(ws=None), -6), (dict(ws=16, ws_bytes=8), -6),
+    (dict(kv_slot=0), -3), (dict(capacity=2 ** 29 + 1), -3),
 ])
 def test_window_attention_rejects(sv, kw, code):
     assert call(sv._lib.lib().sv_window_attention, WINDOW, kw) == code

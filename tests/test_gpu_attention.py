@@ -260,6 +260,57 @@ def test_streams_and_graphs(sv):
     check(got_p, *attention(q, k, v, lengths, prefix=(pk, pv))[:2])
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n", [1, 3, 130])
+def test_negative_and_zero_scale(sv, dtype, n):
+    q, k, v = rand((2, n, 6, 80), 50, dtype), rand((2, 2, 210, 80), 51, dtype), rand((2, 2, 210, 80), 52, dtype)
+    for scale in (-0.2, 0.0, 1e-4):
+        check(sv.window_attention(q, k, v, scale=scale, window=100, sinks=3),
+              *attention(q, k, v, None, None, 100, 3, scale)[:2], f"scale {scale}")
+        check(sv.prefix_attention(q, k[0], v[0], k, v, scale=scale),
+              *attention(q, k, v, scale=scale, prefix=(k[0], v[0]))[:2], f"prefix, scale {scale}")
+
+
+def test_empty_sizes(sv):
+    """No rows, no queries, no slots."""
+    dtype = torch.bfloat16
+    k = rand((2, 2, 9, 64), 53, dtype)
+    assert sv.window_attention(k.new_empty((0, 1, 4, 64)), k[:0], k[:0]).shape == (0, 1, 4, 64)
+    assert sv.window_attention(k.new_empty((2, 0, 4, 64)), k, k).shape == (2, 0, 4, 64)
+    q = rand((2, 3, 4, 64), 54, dtype)
+    assert (sv.window_attention(q, k[:, :, :0], k[:, :, :0]) == 0).all()
+    pk, pv = rand((2, 77, 64), 55, dtype), rand((2, 77, 64), 56, dtype)
+    got = sv.prefix_attention(q, pk, pv, k[:, :, :0], k[:, :, :0])
+    check(got, *attention(q, k[:, :, :1], k[:, :, :1], [0, 0], prefix=(pk, pv))[:2])
+
+
+def test_large_window_and_sinks(sv):
+    """Numbers past the cache and past 31 bits mean no limit."""
+    dtype = torch.float16
+    for n in (1, 60):
+        q, k, v = rand((2, n, 4, 64), 57, dtype), rand((2, 1, 300, 64), 58, dtype), rand((2, 1, 300, 64), 59, dtype)
+        want = sv.window_attention(q, k, v)
+        starts = i32([0, 100])
+        for window, sinks in ((2 ** 40, 0), (300, 0), (2 ** 31 - 1, 2 ** 31 - 1), (10, 2 ** 35), (7, 300)):
+            assert torch.equal(sv.window_attention(q, k, v, window=window, sinks=sinks), want)
+            check(sv.window_attention(q, k, v, starts=starts, window=window, sinks=sinks),
+                  *attention(q, k, v, None, starts)[:2], f"{window} {sinks}")
+
+
+def test_weights_past_the_kept_scores(sv):
+    """Scores beyond 256 MiB are not kept: the weights come from a second product."""
+    R, H, K, D, C = 8, 64, 4, 64, 140000
+    q, k, v = rand((R, 1, H, D), 60, torch.bfloat16), rand((1, 1, C, D), 61, torch.bfloat16), \
+        rand((1, 1, C, D), 62, torch.bfloat16)
+    lengths = i32([C - 100 * r for r in range(R)])
+    w = torch.zeros((R, K, C), device=DEV)
+    got = sv.window_attention(q, k.expand(R, K, -1, -1), v.expand(R, K, -1, -1), lengths, weights=w)
+    r = 3
+    want, tol, wts, wtol = attention(q[r:r + 1, :, :16], k, v, lengths[r:r + 1])
+    check(got[r:r + 1, :, :16], want, tol)
+    check(w[r:r + 1, :1], wts, wtol + 2.0 ** -22 * wts + 1e-30)
+
+
 def test_statuses_and_clamped_lengths(sv):
     dtype = torch.float16
     q, k, v = rand((3, 1, 4, 64), 42, dtype), rand((3, 4, 50, 64), 43, dtype), rand((3, 4, 50, 64), 44, dtype)
@@ -296,7 +347,8 @@ def test_refusals(sv):
                dict(out=torch.empty((2, 1, 4, 32), dtype=dtype, device=DEV)), dict(status=torch.zeros(2, device=DEV)),
                dict(q=rand((2, 1, 4, 136), 1, dtype), keys=wide, values=wide),
                dict(q=q[..., :60], keys=k[..., :60], values=k[..., :60]),
-               dict(keys=wide[..., 1:65], values=wide[..., 1:65])):
+               dict(keys=wide[..., 1:65], values=wide[..., 1:65]),
+               dict(keys=k[:, :, :1].expand(-1, -1, 50, -1), values=k[:, :, :1].expand(-1, -1, 50, -1))):
         with pytest.raises(RuntimeError):
             call(**kw)
     for kw in (dict(prefix_keys=k[0, :1], prefix_values=k[0, :1]), dict(prefix_length=51), dict(prefix_length=-1)):
