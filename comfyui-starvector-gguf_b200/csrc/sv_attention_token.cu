@@ -562,11 +562,21 @@ __global__ void __launch_bounds__(NT, kTokenPerSM) attn_token_kernel(const __gri
           }
     }
     if (more_units) load_q(next);
+    // A unit of this block alone is finished here, the prefix's parts joined with the warps'.
+    const bool alone = p.first >= c0 && p.end <= c1;
+    const int extra = alone ? a.p_splits : 0, slot = 2 * c + (p.first >= c0);
+    const int64_t row0 = prefix_index(a, p.r, p.h, 0);
+    if (extra) {
+      wait_before();  // the prefix's kernel may have run beside this one
+      for (int x = tid; x < extra * 16; x += NT)
+        if ((x & 15) < nG) part_ml[x >> 4][x & 15] = __ldcg(a.prefix_ml + (int64_t)(x >> 4) * all_rows + row0 + (x & 15));
+    }
     __syncthreads();
     if (tid < nG) {
       float M = -INFINITY;
 #pragma unroll
       for (int k = 0; k < NW; ++k) M = fmaxf(M, warp_ml[k][tid].x);
+      for (int k = 0; k < extra; ++k) M = fmaxf(M, part_ml[k][tid].x);
       const float at = M == -INFINITY ? 0.f : M;
       float L = 0.f;
 #pragma unroll
@@ -575,35 +585,40 @@ __global__ void __launch_bounds__(NT, kTokenPerSM) attn_token_kernel(const __gri
         factor[k][tid] = f;
         L = fmaf(warp_ml[k][tid].y, f, L);
       }
+      for (int k = 0; k < extra; ++k) {
+        const float f = part_ml[k][tid].y == 0.f ? 0.f : ex2(part_ml[k][tid].x - at);
+        factor[NW + k][tid] = f;
+        L = fmaf(part_ml[k][tid].y, f, L);
+      }
       joined[tid] = make_float2(M, L);
     }
     __syncthreads();
-    const bool alone = p.first >= c0 && p.end <= c1, direct = alone && !a.prefix;
-    const int slot = 2 * c + (p.first >= c0);
     for (int x = tid; x < nG * row_vecs; x += NT) {
       const int m = x / row_vecs, d = (x - m * row_vecs) * 4;
       float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-      for (int k = 0; k < NW; ++k) {
-        const float4 y = *vec_at(k, m, d >> 2);
-        const float f = factor[k][m];
+      auto add = [&](float4 y, float f) {
         v.x = fmaf(y.x, f, v.x);
         v.y = fmaf(y.y, f, v.y);
         v.z = fmaf(y.z, f, v.z);
         v.w = fmaf(y.w, f, v.w);
-      }
-      if (direct)
+      };
+#pragma unroll
+      for (int k = 0; k < NW; ++k) add(*vec_at(k, m, d >> 2), factor[k][m]);
+#pragma unroll 4
+      for (int k = 0; k < extra; ++k)
+        add(__ldcg(reinterpret_cast<const float4*>(a.prefix_o + ((int64_t)k * all_rows + row0 + m) * D + d)),
+            factor[NW + k][m]);
+      if (alone)
         write_out(p, m, d, v, joined[m].y);
       else
         *reinterpret_cast<float4*>(a.part_o + ((int64_t)slot * 16 + m) * D + d) = v;
     }
     if (tid < nG) {
-      if (direct)
+      if (alone)
         write_lse(p, tid);
       else
         a.part_ml[slot * 16 + tid] = joined[tid];
     }
-    if (alone && a.prefix) join(p, c, c, 1, 1, true, std::false_type());
     if (!alone) shared_part[shared_parts++] = p;
     if (a.status && tid == 0 && p.h == K - 1 && p.end <= c1) {
       const int e = a.lengths ? a.lengths[p.r] : a.capacity, s = a.starts ? a.starts[p.r] : 0;
