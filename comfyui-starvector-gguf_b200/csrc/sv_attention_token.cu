@@ -593,25 +593,43 @@ __global__ void __launch_bounds__(NT, kTokenPerSM) attn_token_kernel(const __gri
       joined[tid] = make_float2(M, L);
     }
     __syncthreads();
-    for (int x = tid; x < nG * row_vecs; x += NT) {
-      const int m = x / row_vecs, d = (x - m * row_vecs) * 4;
-      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-      auto add = [&](float4 y, float f) {
-        v.x = fmaf(y.x, f, v.x);
-        v.y = fmaf(y.y, f, v.y);
-        v.z = fmaf(y.z, f, v.z);
-        v.w = fmaf(y.w, f, v.w);
+    {
+      // This thread's vectors of four side by side: their loads are in flight together.
+      constexpr int ITEMS = (16 * DC * 16 + NT - 1) / NT;
+      int m[ITEMS], d[ITEMS];
+      float4 v[ITEMS];
+#pragma unroll
+      for (int x = 0; x < ITEMS; ++x) v[x] = make_float4(0.f, 0.f, 0.f, 0.f);
+      auto add = [&](int x, float4 y, float f) {
+        v[x].x = fmaf(y.x, f, v[x].x);
+        v[x].y = fmaf(y.y, f, v[x].y);
+        v[x].z = fmaf(y.z, f, v[x].z);
+        v[x].w = fmaf(y.w, f, v[x].w);
       };
 #pragma unroll
-      for (int k = 0; k < NW; ++k) add(*vec_at(k, m, d >> 2), factor[k][m]);
+      for (int x = 0; x < ITEMS; ++x) {
+        m[x] = (tid + x * NT) / row_vecs;
+        d[x] = (tid + x * NT - m[x] * row_vecs) * 4;
+        if (m[x] < nG) {
+#pragma unroll
+          for (int k = 0; k < NW; ++k) add(x, *vec_at(k, m[x], d[x] >> 2), factor[k][m[x]]);
+        }
+      }
 #pragma unroll 4
       for (int k = 0; k < extra; ++k)
-        add(__ldcg(reinterpret_cast<const float4*>(a.prefix_o + ((int64_t)k * all_rows + row0 + m) * D + d)),
-            factor[NW + k][m]);
-      if (alone)
-        write_out(p, m, d, v, joined[m].y);
-      else
-        *reinterpret_cast<float4*>(a.part_o + ((int64_t)slot * 16 + m) * D + d) = v;
+#pragma unroll
+        for (int x = 0; x < ITEMS; ++x)
+          if (m[x] < nG)
+            add(x, __ldcg(reinterpret_cast<const float4*>(a.prefix_o + ((int64_t)k * all_rows + row0 + m[x]) * D + d[x])),
+                factor[NW + k][m[x]]);
+#pragma unroll
+      for (int x = 0; x < ITEMS; ++x) {
+        if (m[x] >= nG) continue;
+        if (alone)
+          write_out(p, m[x], d[x], v[x], joined[m[x]].y);
+        else
+          *reinterpret_cast<float4*>(a.part_o + ((int64_t)slot * 16 + m[x]) * D + d[x]) = v[x];
+      }
     }
     if (tid < nG) {
       if (alone)
