@@ -209,6 +209,8 @@ __global__ void __launch_bounds__(NT, 1) attn_tile_kernel(const __grid_constant_
     j0 = t < it.ta ? it.a0 + t * BN : it.b0 + (t - it.ta) * BN;
     jend = t < it.ta ? it.a1 : it.b1;
   };
+  // How many 16-slot products a step's values need: the rest of its tile is not read.
+  auto value_blocks = [](int j0, int jend) { return min(BN / 16, (jend - j0 + 15) / 16); };
   // The steps whose slots rows [first, last] all see: j < a_whole (sinks) or w0 <= j < w1.
   struct Whole {
     int a_whole, w0, w1;
@@ -362,6 +364,9 @@ __global__ void __launch_bounds__(NT, 1) attn_tile_kernel(const __grid_constant_
 #pragma unroll 1
       for (int c = 0; 2 * c + t < steps; ++c) {
         const int j = 2 * c + t, vi = 2 * j + 1, ki = 2 * j + 8;
+        int j0, jend;
+        tile_at(it, j, j0, jend);
+        const int blocks = value_blocks(j0, jend);
         if (leader) {
           wait_one(sh, &sh.ready[vi % STAGES], (vi / STAGES) & 1);
           wait_one(sh, &sh.p_full[t][c & 1], (c >> 1) & 1);
@@ -369,7 +374,7 @@ __global__ void __launch_bounds__(NT, 1) attn_tile_kernel(const __grid_constant_
           const uint64_t vd = v_desc + (vi % STAGES) * kStep;
 #pragma unroll
           for (int k = 0; k < BN / 16; ++k)
-            mma_ts(o_at, s_at + (c & 1) * BN + k * 8, vd + k * (2048 >> 4), wpv, c != 0 || k != 0);
+            if (k < blocks) mma_ts(o_at, s_at + (c & 1) * BN + k * 8, vd + k * (2048 >> 4), wpv, c != 0 || k != 0);
           mma_commit(&sh.pv_done[t][j % RING]);
           if (j + 4 < steps) {
             wait_one(sh, &sh.full[ki % STAGES], (ki / STAGES) & 1);
@@ -407,6 +412,9 @@ __global__ void __launch_bounds__(NT, 1) attn_tile_kernel(const __grid_constant_
 #pragma unroll 1
       for (int j = 0; j < steps; ++j) {
         const int J = base + j, P = mine + j, vi = 2 * J + 1, ki = 2 * J + 4;
+        int j0, jend;
+        tile_at(it, j, j0, jend);
+        const int blocks = value_blocks(j0, jend);
         if (leader) {
           wait_one(sh, &sh.ready[vi % STAGES], (vi / STAGES) & 1);
           wait_one(sh, &sh.p_full[t][P & 1], (P >> 1) & 1);
@@ -414,7 +422,7 @@ __global__ void __launch_bounds__(NT, 1) attn_tile_kernel(const __grid_constant_
           const uint64_t vd = v_desc + (vi % STAGES) * kStep;
 #pragma unroll
           for (int k = 0; k < BN / 16; ++k)
-            mma_ts(o_at, s_at + (P & 1) * BN + k * 8, vd + k * (2048 >> 4), wpv, j != 0 || k != 0);
+            if (k < blocks) mma_ts(o_at, s_at + (P & 1) * BN + k * 8, vd + k * (2048 >> 4), wpv, j != 0 || k != 0);
           mma_commit(&sh.pv_done[t][J % RING]);
           if (j + 2 < steps) {
             wait_one(sh, &sh.full[ki % STAGES], (ki / STAGES) & 1);
@@ -461,46 +469,58 @@ __global__ void __launch_bounds__(NT, 1) attn_tile_kernel(const __grid_constant_
           tile_at(it, j, j0, jend);
           unsigned char* vb = dyn + L::kRing + st * L::kTile;
           // Only slots that some row does not see are looked at (sinks before the window are seen
-          // by all): where a block has few queries that is a small part of the tile, and the
-          // steps wait for this warp (looking at all of it, one vector at a time: 4 x 100
-          // queries of 64 dimensions 31.9 us, now 27.5; 3 x 577 of 128 20.2 and 18.5).  16
-          // bytes at a time, four of them in flight; the swizzle permutes vectors within a slot only.
+          // by all), and behind the last slot those of its product are zeroed: where a block has
+          // few queries that is a small part of the tile, and the steps wait for this warp
+          // (looking at the whole tile, 4 x 100 queries of 64 dimensions took 31.9 us, now
+          // 27.5; 3 x 577 of 128 20.2 and 18.5).  The swizzle permutes 16-byte vectors within
+          // a slot only.
           const bool sink = it.t0 + j < it.ta;
-          const int s0 = sink ? j0 : whole.from, s1 = sink ? jend : whole.to;
-          constexpr int kAhead = 4;
+          const int n = min(jend - j0, BN), last = 16 * value_blocks(j0, jend);
+          const int seen0 = sink ? 0 : min(max(whole.from - j0, 0), n), seen1 = sink ? n : min(max(whole.to - j0, seen0), n);
+          auto look = [&](int r0, int r1) {
+            constexpr uint32_t E = Half16<T>::expo * 0x10001u;
+            constexpr int kAhead = 4;  // vectors of a lane in flight
 #pragma unroll 1
-          for (int x0 = lane; x0 < BN * DC * 8; x0 += 32 * kAhead) {
-            uint4 v[kAhead];
-            uint4* p[kAhead];
-            bool look[kAhead];
+            for (int d = 0; d < DC; ++d) {
+              uint4* vd = reinterpret_cast<uint4*>(vb + d * L::kHalf);
+#pragma unroll 1
+              for (int x0 = r0 * 8 + lane; x0 < r1 * 8; x0 += 32 * kAhead) {
+                uint4 v[kAhead];
+                uint32_t any = 0;
 #pragma unroll
-            for (int k = 0; k < kAhead; ++k) {
-              const int x = x0 + 32 * k, row = (x >> 3) & (BN - 1), slot = j0 + row;
-              p[k] = reinterpret_cast<uint4*>(vb + x / (BN * 8) * L::kHalf + row * 128 + (x & 7) * 16);
-              look[k] = slot < jend && (slot < s0 || slot >= s1);
-              if (look[k]) v[k] = *p[k];
-              if (slot >= jend) *p[k] = make_uint4(0u, 0u, 0u, 0u);
-            }
+                for (int k = 0; k < kAhead; ++k) v[k] = vd[min(x0 + 32 * k, r1 * 8 - 1)];
+                // A half with all exponent bits set leaves zero, and the subtraction its sign.
 #pragma unroll
-            for (int k = 0; k < kAhead; ++k) {
-              if (!look[k]) continue;
-              const int row = ((x0 + 32 * k) >> 3) & (BN - 1);
-              uint32_t* q = reinterpret_cast<uint32_t*>(&v[k]);
-              bool bad = false;
-              constexpr uint32_t E = Half16<T>::expo;
+                for (int k = 0; k < kAhead; ++k)
+                  any |= (((v[k].x & E) ^ E) - 0x10001u) | (((v[k].y & E) ^ E) - 0x10001u) |
+                         (((v[k].z & E) ^ E) - 0x10001u) | (((v[k].w & E) ^ E) - 0x10001u);
+                if (!(any & 0x80008000u)) continue;
+                for (int k = 0; k < kAhead && x0 + 32 * k < r1 * 8; ++k) {
+                  const int x = x0 + 32 * k;
+                  uint32_t* w = reinterpret_cast<uint32_t*>(vd + x);
+                  bool bad = false;
 #pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                if ((q[i] & E) == E) q[i] &= 0xffff0000u, bad = true;
-                if ((q[i] & (E << 16)) == E << 16) q[i] &= 0xffffu, bad = true;
+                  for (int i = 0; i < 4; ++i) {
+                    const uint32_t e = w[i] & E, lo = (e & 0xffffu) == (E & 0xffffu) ? 0xffffu : 0u,
+                                   hi = (e & 0xffff0000u) == (E & 0xffff0000u) ? 0xffff0000u : 0u;
+                    if (lo | hi) w[i] &= ~(lo | hi), bad = true;
+                  }
+                  if (bad) {
+                    atomicOr(&sh.bad[edge][x >> 8], 1u << ((x >> 3) & 31));
+                    sh.bad_from[edge] = j0;
+                    sh.any_bad = 1;
+                  }
+                }
               }
-              if (bad) {
-                *p[k] = v[k];
-                atomicOr(&sh.bad[edge][row >> 5], 1u << (row & 31));
-                sh.bad_from[edge] = j0;
-                sh.any_bad = 1;
-              }
             }
-          }
+          };
+          look(0, seen0);
+          look(seen1, n);
+          for (int x = n * 8 + lane; x < last * 8; x += 32)
+#pragma unroll
+            for (int d = 0; d < DC; ++d)
+              *reinterpret_cast<uint4*>(vb + d * L::kHalf + x * 16) = make_uint4(0u, 0u, 0u, 0u);
+          __syncwarp();
           fence_proxy_async_smem();
           edge = min(edge + 1, kEdges - 1);
         }
