@@ -3,12 +3,14 @@
 //
 // Mathematics: one pass with a running reference, as the 16-bit kernels (o = sum_j
 // 2^(s_j - ref) v_j, l = sum_j 2^(s_j - ref); ref follows the maximum once a score
-// exceeds it by 2^8).  Every f32 operand x is taken as hi + lo, hi its upper 11
+// exceeds it by 2^8).  Every f32 operand x is taken as hi + lo, hi x rounded to 11
 // significant bits and lo = x - hi (exact; the tensor core reads its upper 11 bits):
-// x y = hi hi + hi lo + lo hi with a relative error of about 2^-21 per product, sums in
-// f32; three products m16n8k8 (TF32) per step.  On the FP32 pipes the same work took 2.5
-// times as long.  An operand that is not finite has no such split: it is computed value by
-// value instead.  (A query that is not finite makes its row NaN, as an infinite score does.)
+// x y = hi hi + hi lo + lo hi with a relative error of about 2^-22 per product, sums in
+// f32; three products m16n8k8 (TF32) per step.  Rounded halves and scores summed outside the
+// tensor core take 98 us for 2 x 333 queries over 512 slots, truncated ones 94 us with up to
+// twice the error (1.6e-6 and 8e-7 of the output for 24 rows over 1460 shared slots).  On the
+// FP32 pipes the same work took 140 us.  An operand that is not finite (or, a key, that
+// rounds to infinity) has no such split: it is computed value by value instead.  (A query that is not finite makes its row NaN, as an infinite score does.)
 //
 // A block of 8 warps holds 16 query rows of one key/value head's group and takes the
 // slots 8 per warp and round, straight from global memory into the fragments (as in the
@@ -40,6 +42,14 @@ __device__ __forceinline__ void mma(float (&c)[4], float a0, float a1, float a2,
 
 // Truncated, not rounded: the type's largest values must not become infinite.
 __device__ __forceinline__ float upper(float x) { return __uint_as_float(__float_as_uint(x) & 0xffffe000u); }
+// Rounded (ties away), for queries, keys and weights: their lower halves then have either
+// sign, where truncated ones have their number's, and the dropped lo lo and the lower halves'
+// own truncation would make every score too small by some 2^-22 of itself.  Below kRoundable only.
+constexpr float kRoundable = 0x1.ffep127f;
+__device__ __forceinline__ float nearest(float x) { return __uint_as_float((__float_as_uint(x) + 0x1000u) & 0xffffe000u); }
+__device__ __forceinline__ float4 nearest(float4 x) {
+  return make_float4(nearest(x.x), nearest(x.y), nearest(x.z), nearest(x.w));
+}
 __device__ __forceinline__ float4 upper(float4 x) { return make_float4(upper(x.x), upper(x.y), upper(x.z), upper(x.w)); }
 __device__ __forceinline__ float4 minus(float4 a, float4 b) {
   return make_float4(a.x - b.x, a.y - b.y, a.z - b.z, a.w - b.w);
@@ -53,6 +63,10 @@ __device__ __forceinline__ float4 load_stream(const float* p, bool ok) {
   return v;
 }
 __device__ __forceinline__ float finite(float x) { return fabsf(x) < INFINITY ? x : 0.f; }
+__device__ __forceinline__ float roundable(float x) { return fabsf(x) < kRoundable ? x : 0.f; }
+__device__ __forceinline__ float4 roundable(float4 x) {
+  return make_float4(roundable(x.x), roundable(x.y), roundable(x.z), roundable(x.w));
+}
 __device__ __forceinline__ float4 finite(float4 x) { return make_float4(finite(x.x), finite(x.y), finite(x.z), finite(x.w)); }
 // The largest magnitude of four values and m, NaN if one is NaN.
 __device__ __forceinline__ float widest(float4 v, float m) {
@@ -88,7 +102,8 @@ __global__ void __launch_bounds__(NT, 1) attn_f32_kernel(const __grid_constant__
     const int ln = x & 31, y = (x >> 5) & 1, u = x >> 6, m = m0 + (ln >> 2) + 8 * y, d = 16 * u + 4 * (ln & 3);
     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
     if (m < rows_m && (FULL || d < D)) v = __ldg(reinterpret_cast<const float4*>(query(m) + d));
-    const float4 hi = upper(v);
+    auto half = [](float x) { return fabsf(x) < kRoundable ? nearest(x) : upper(x); };
+    const float4 hi = make_float4(half(v.x), half(v.y), half(v.z), half(v.w));
     dyn[(u * 2 + y) * 32 + ln] = hi;
     dyn[((KU + u) * 2 + y) * 32 + ln] = minus(v, hi);
   }
@@ -160,34 +175,41 @@ __global__ void __launch_bounds__(NT, 1) attn_f32_kernel(const __grid_constant__
     float wide = 0.f;
 #pragma unroll
     for (int u = 0; u < KU; ++u) wide = widest(kf[u], wide);
-    const unsigned bad_k = __ballot_sync(0xffffffffu, !(wide < INFINITY));
+    const unsigned bad_k = __ballot_sync(0xffffffffu, !(wide < kRoundable));
     if (bad_k) {
 #pragma unroll
-      for (int u = 0; u < KU; ++u) kf[u] = finite(kf[u]);
+      for (int u = 0; u < KU; ++u) kf[u] = roundable(kf[u]);
     }
     float s[4];
     {
-      // Sums of their own for the halves' products and for two dimensions of each vector:
-      // a product waits for the one before it in the same sum.
-      float c[4][4];
+      // Sums of their own for the halves' products (a product waits for the one before it in
+      // the same sum); those of the upper halves are added in f32 with rounding, as the
+      // tensor core truncates as it adds.
+      float c[2][4], e[2][4];
 #pragma unroll
-      for (int x = 0; x < 4; ++x)
+      for (int x = 0; x < 2; ++x)
 #pragma unroll
-        for (int k = 0; k < 4; ++k) c[x][k] = 0.f;
+        for (int k = 0; k < 4; ++k) c[x][k] = e[x][k] = 0.f;
 #pragma unroll
       for (int u = 0; u < KU; ++u) {
         const float4 qh0 = dyn[u * 64 + lane], qh1 = dyn[u * 64 + 32 + lane];
         const float4 ql0 = dyn[(KU + u) * 64 + lane], ql1 = dyn[(KU + u) * 64 + 32 + lane];
-        const float4 kh = upper(kf[u]), kl = minus(kf[u], kh);
-        mma(c[0], qh0.x, qh1.x, qh0.y, qh1.y, kh.x, kh.y);
-        mma(c[1], qh0.z, qh1.z, qh0.w, qh1.w, kh.z, kh.w);
-        mma(c[2], qh0.x, qh1.x, qh0.y, qh1.y, kl.x, kl.y);
-        mma(c[3], ql0.x, ql1.x, ql0.y, ql1.y, kh.x, kh.y);
-        mma(c[2], qh0.z, qh1.z, qh0.w, qh1.w, kl.z, kl.w);
-        mma(c[3], ql0.z, ql1.z, ql0.w, ql1.w, kh.z, kh.w);
+        const float4 kh = nearest(kf[u]), kl = minus(kf[u], kh);
+        float d[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+        mma(d[0], qh0.x, qh1.x, qh0.y, qh1.y, kh.x, kh.y);
+        mma(d[1], qh0.z, qh1.z, qh0.w, qh1.w, kh.z, kh.w);
+        mma(c[0], qh0.x, qh1.x, qh0.y, qh1.y, kl.x, kl.y);
+        mma(c[1], ql0.x, ql1.x, ql0.y, ql1.y, kh.x, kh.y);
+        mma(c[0], qh0.z, qh1.z, qh0.w, qh1.w, kl.z, kl.w);
+        mma(c[1], ql0.z, ql1.z, ql0.w, ql1.w, kh.z, kh.w);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          e[0][k] += d[0][k];
+          e[1][k] += d[1][k];
+        }
       }
 #pragma unroll
-      for (int k = 0; k < 4; ++k) s[k] = (c[0][k] + c[1][k]) + (c[2][k] + c[3][k]);
+      for (int k = 0; k < 4; ++k) s[k] = (e[0][k] + e[1][k]) + (c[0][k] + c[1][k]);
     }
     if (bad_k) {  // the slots whose keys are not finite, value by value
 #pragma unroll
@@ -274,7 +296,7 @@ __global__ void __launch_bounds__(NT, 1) attn_f32_kernel(const __grid_constant__
     float ph[4], pl[4];
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
-      ph[k] = upper(s[k]);
+      ph[k] = nearest(s[k]);
       pl[k] = s[k] - ph[k];
     }
 #pragma unroll

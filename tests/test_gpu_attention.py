@@ -354,3 +354,24 @@ def test_refusals(sv):
     for kw in (dict(prefix_keys=k[0, :1], prefix_values=k[0, :1]), dict(prefix_length=51), dict(prefix_length=-1)):
         with pytest.raises(ValueError):
             sv.prefix_attention(**{**dict(q=q, prefix_keys=k[0], prefix_values=k[0], keys=k, values=k), **kw})
+
+
+@pytest.mark.parametrize("n", [1, 40])
+def test_float_keys_at_the_end_of_the_range(sv, n):
+    """Keys that rounding to fewer bits would make infinite, under a scale that keeps the scores ordinary."""
+    g = torch.Generator(device="cuda").manual_seed(11)
+    q = torch.randn((2, n, 4, 128), generator=g, device="cuda") * 2.0 ** -8
+    k = torch.randn((2, 2, 200, 128), generator=g, device="cuda").clamp(-1, 1)
+    k[:, :, 5::7] = k[:, :, 5::7].sign()
+    k = k * torch.finfo(torch.float32).max
+    v = torch.randn((2, 2, 200, 128), generator=g, device="cuda")
+    out = sv.window_attention(q, k, v, scale=2.0 ** -124)
+    x = q.double().reshape(2, n, 2, 2, 128).permute(0, 2, 3, 1, 4)
+    s = torch.einsum("rkgnd,rkcd->rkgnc", x, k.double()) * 2.0 ** -124
+    at = torch.arange(200 - n, 200, device="cuda")[:, None]
+    s = s.masked_fill(torch.arange(200, device="cuda") > at, float("-inf"))
+    want = torch.einsum("rkgnc,rkcd->rkgnd", s.softmax(-1), v.double()).permute(0, 3, 1, 2, 4).reshape(2, n, 4, 128)
+    # Products of 128 dimensions with |q k| scale below 1 (2^4 in sum), each within 2^-20 of itself: scores
+    # within 2^-16, weights and their sum within 2^-15 of themselves together, outputs as much of the largest value.
+    assert torch.isfinite(out).all()
+    assert (out.double() - want).abs().max() <= v.abs().max() * 2.0 ** -15
