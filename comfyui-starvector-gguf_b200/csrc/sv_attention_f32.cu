@@ -7,8 +7,8 @@
 // significant bits and lo = x - hi (exact; the tensor core reads its upper 11 bits):
 // x y = hi hi + hi lo + lo hi with a relative error of about 2^-22 per product, sums in
 // f32; three products m16n8k8 (TF32) per step.  Rounded halves and scores summed outside the
-// tensor core take 98 us for 2 x 333 queries over 512 slots, truncated ones 94 us with up to
-// twice the error (1.6e-6 and 8e-7 of the output for 24 rows over 1460 shared slots).  On the
+// tensor core take 98 us for 2 x 333 queries over 512 slots, truncated ones 94 us with more
+// error (1.6e-6 of the output for 24 rows over 1460 shared slots, and 3.2e-7 rounded).  On the
 // FP32 pipes the same work took 140 us.  An operand that is not finite (or, a key, that
 // rounds to infinity) has no such split: it is computed value by value instead.  (A query that is not finite makes its row NaN, as an infinite score does.)
 //

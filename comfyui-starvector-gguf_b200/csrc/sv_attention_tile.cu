@@ -472,7 +472,7 @@ __global__ void __launch_bounds__(NT, 1) attn_tile_kernel(const __grid_constant_
           // by all), and behind the last slot those of its product are zeroed: where a block has
           // few queries that is a small part of the tile, and the steps wait for this warp
           // (looking at the whole tile, 4 x 100 queries of 64 dimensions took 31.9 us, now
-          // 27.5; 3 x 577 of 128 20.2 and 18.5).  The swizzle permutes 16-byte vectors within
+          // 26.8; 3 x 577 of 128 20.2 and 16.9, the 8192-token prompt 443 and 413).  The swizzle permutes 16-byte vectors within
           // a slot only.
           const bool sink = it.t0 + j < it.ta;
           const int n = min(jend - j0, BN), last = 16 * value_blocks(j0, jend);
