@@ -129,6 +129,8 @@ int check_pointers(const AttnArgs& a, double scale) {
   for (const void* p : ptrs)
     if (reinterpret_cast<uintptr_t>(p) % 16) return SV_E_ALIGN;
   if (a.weights && (a.w_row < 0 || a.w_head < 0)) return SV_E_SHAPE;
+  // Rows and heads add to their own words without atomics.
+  if (a.weights && !entries_apart<2>(a.capacity, {a.rows, a.kv_heads}, {a.w_row, a.w_head})) return SV_E_SHAPE;
   // One slot for all positions is no cache (and no dimension of a copy).
   if ((a.capacity > 1 && a.kv_slot == 0) || (a.prefix > 1 && a.p_slot == 0)) return SV_E_SHAPE;
   return SV_OK;

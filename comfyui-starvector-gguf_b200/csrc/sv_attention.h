@@ -116,6 +116,24 @@ __device__ __forceinline__ void load8(const __nv_bfloat16* p, float* x) {
   }
 }
 
+// Whether the entries of a strided array that is written are apart from one another:
+// runs of `extent` contiguous elements, D dimensions of `sizes` entries at `strides`.
+// From the smallest stride up, each has to step over all that lies within it (layouts
+// that interleave dimensions otherwise are refused, apart or not).
+template <int D> bool entries_apart(int64_t extent, const int64_t (&sizes)[D], const int64_t (&strides)[D]) {
+  bool done[D] = {};
+  for (int k = 0; k < D; ++k) {
+    int at = -1;
+    for (int d = 0; d < D; ++d)
+      if (!done[d] && (at < 0 || strides[d] < strides[at])) at = d;
+    done[at] = true;
+    if (sizes[at] <= 1) continue;  // the stride of one entry means nothing
+    if (strides[at] < extent) return false;
+    extent += (sizes[at] - 1) * strides[at];
+  }
+  return true;
+}
+
 // Raises a kernel's shared-memory limit, once per device and process.
 template <auto Kernel> cudaError_t allow_smem(size_t bytes) {
   static std::atomic<uint64_t> done{0};

@@ -219,6 +219,9 @@ at::Tensor workspace_for(const at::Device& dev, c10::cuda::CUDAStream stream, si
 // Strides of a dimension of one entry mean nothing: 0 stands for them.
 int64_t stride_of(const at::Tensor& t, int64_t d) { return t.size(d) > 1 ? t.stride(d) : 0; }
 
+// Whether dimension d lies contiguously (a broadcast one, of stride 0, does not).
+bool contiguous_along(const at::Tensor& t, int64_t d) { return t.size(d) <= 1 || t.stride(d) == 1; }
+
 bool aligned(const at::Tensor& t, int64_t dims) {
   if (reinterpret_cast<uintptr_t>(t.data_ptr()) % 16) return false;
   const int64_t e = t.element_size();
@@ -294,8 +297,10 @@ std::tuple<int, at::Tensor> window_attention(const at::Tensor& q_in, const at::T
   if (weights.has_value()) {
     if (weights->dim() == 2) weights = weights->unsqueeze(1);
     TORCH_CHECK_VALUE(weights->scalar_type() == at::kFloat && weights->dim() == 3 && weights->size(0) == rows &&
-                          weights->size(1) == kv && weights->size(2) >= capacity && stride_of(*weights, 2) <= 1,
+                          weights->size(1) == kv && weights->size(2) >= capacity && contiguous_along(*weights, 2),
                       "weights must be float32 [rows, kv_heads, capacity], contiguous along the slots");
+    TORCH_CHECK_VALUE((rows <= 1 || weights->stride(0) > 0) && (kv <= 1 || weights->stride(1) > 0),
+                      "weights are added to in place: rows and heads must not be broadcast");
   }
   const OptT lengths = row_ints(lengths_in, rows, dev, "lengths"), starts = row_ints(starts_in, rows, dev, "starts");
   const int32_t w = (int32_t)std::min<int64_t>(window, 1 << 30), s = (int32_t)std::min<int64_t>(sinks, 1 << 30);

@@ -1,0 +1,25 @@
+"""Layouts that the cache operators' entry points refuse, without a GPU: every refusal
+below returns its code before any CUDA call."""
+import pytest
+
+from test_cache_capi import WINDOW, call
+
+
+@pytest.mark.parametrize("kw", [
+    dict(w_row=0, w_head=0), dict(w_row=0, w_head=1000), dict(kv_heads=2, w_row=1000, w_head=0),
+    dict(w_row=999), dict(kv_heads=4, w_row=1000, w_head=1000), dict(kv_heads=4, w_row=1, w_head=2000),
+    dict(kv_heads=2, w_row=1999, w_head=1000),
+])
+def test_accumulated_weights_that_overlap(sv, kw):
+    """Rows or heads that would add to the same words."""
+    assert call(sv._lib.lib().sv_window_attention, {**WINDOW, "weights": 16, "w_row": 1000}, kw) == -3
+
+
+@pytest.mark.parametrize("kw", [
+    dict(), dict(kv_heads=2, w_row=2000, w_head=1000), dict(kv_heads=2, w_row=1000, w_head=2000),
+    dict(rows=1, w_row=0), dict(kv_heads=1, w_row=1003, w_head=0), dict(rows=1, kv_heads=4, w_row=0, w_head=1003),
+    dict(rows=1, capacity=1, w_row=0, w_head=0),
+])
+def test_accumulated_weights_that_lie_apart(sv, kw):
+    """Past the layout's check: the next thing that is missing is the workspace."""
+    assert call(sv._lib.lib().sv_window_attention, {**WINDOW, "weights": 16, "w_row": 1000}, kw) == -6

@@ -1,0 +1,32 @@
+"""Views that the cache operators refuse or copy: broadcast and overlapping dimensions.
+What is refused is refused on the host, before anything runs."""
+import pytest
+import torch
+
+from test_gpu_attention import rand
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+
+
+@pytest.mark.parametrize("n", [1, 40])
+def test_broadcast_accumulated_weights_are_refused(sv, n):
+    """An accumulator expanded along its slots, rows or heads: torch refuses both for its own additions."""
+    R, K, C = 2, 2, 50
+    q, k = rand((R, n, 4, 64), 1, torch.float16), rand((R, K, C, 64), 2, torch.float16)
+    one = torch.zeros((R, K, 1), device=DEV)
+    for w in (one.expand(R, K, C), torch.zeros((1, K, C), device=DEV).expand(R, K, C),
+              torch.zeros((R, 1, C), device=DEV).expand(R, K, C), torch.zeros(1, device=DEV).expand(R, K, C)):
+        before = w.clone()
+        with pytest.raises(ValueError):
+            sv.window_attention(q, k, k, weights=w)
+        assert torch.equal(w, before)
+    with pytest.raises(RuntimeError):  # the second row starts within the first
+        sv.window_attention(q, k, k, weights=torch.zeros(300, device=DEV).as_strided((R, K, C), (C, C, 1)))
+    # Size-one dimensions have no stride, and a wider accumulator's rows lie apart.
+    w = torch.zeros((1, 1, C + 3), device=DEV).expand(1, 1, C + 3)
+    sv.window_attention(q[:1], k[:1, :1], k[:1, :1], weights=w)
+    assert abs(w[..., :C].sum().item() - 4 * n) < 1e-2 and (w[..., C:] == 0).all()
+    w = torch.zeros((K, R, C + 3), device=DEV).transpose(0, 1)
+    sv.window_attention(q, k, k, weights=w)
+    assert abs(w[..., :C].sum().item() - R * 4 * n) < 1e-2 and (w[..., C:] == 0).all()
