@@ -239,7 +239,7 @@ at::Tensor queries(const at::Tensor& q) {
   const auto st = q.scalar_type();
   TORCH_CHECK_VALUE(st == at::kFloat || st == at::kHalf || st == at::kBFloat16, "unsupported dtype ", st);
   at::Tensor x = q.dim() == 3 ? q.unsqueeze(1) : q;
-  if (stride_of(x, 3) > 1 || !aligned(x, 3)) x = x.clone(at::MemoryFormat::Contiguous);
+  if (!contiguous_along(x, 3) || !aligned(x, 3)) x = x.clone(at::MemoryFormat::Contiguous);
   return x;
 }
 
@@ -257,7 +257,7 @@ void check_cache(const at::Tensor& k, const at::Tensor& v, const at::Tensor& q) 
                     "keys and values must have q's dtype");
   TORCH_CHECK_VALUE(k.size(0) == q.size(0) && k.size(3) == q.size(3) && k.size(1) > 0 && q.size(2) % k.size(1) == 0,
                     "keys must have q's rows and head_dim, and kv_heads must divide heads");
-  TORCH_CHECK_VALUE(stride_of(k, 3) <= 1, "head_dim must be contiguous");
+  TORCH_CHECK_VALUE(contiguous_along(k, 3), "head_dim must be contiguous");
 }
 
 // A per-row int32 tensor from a tensor of whole numbers (none stays none).
@@ -337,7 +337,7 @@ std::tuple<int, at::Tensor> prefix_attention(const at::Tensor& q_in, const at::T
   on_device(pv, dev, "prefix_values");
   TORCH_CHECK_VALUE(pk.dim() == 3 && pv.sizes() == pk.sizes() && pv.strides() == pk.strides() &&
                         pk.scalar_type() == q.scalar_type() && pv.scalar_type() == q.scalar_type() &&
-                        pk.size(0) == keys.size(1) && pk.size(2) == q.size(3) && stride_of(pk, 2) <= 1,
+                        pk.size(0) == keys.size(1) && pk.size(2) == q.size(3) && contiguous_along(pk, 2),
                     "prefix_keys and prefix_values must be [kv_heads, prefix, head_dim] of q's dtype with the same "
                     "strides");
   TORCH_CHECK_VALUE(!prefix_length.has_value() || (*prefix_length >= 0 && *prefix_length <= pk.size(1)),
@@ -381,7 +381,7 @@ std::tuple<int, at::Tensor, at::Tensor, at::Tensor> kv_evict(
                     "keys must be [layers, rows, capacity, head_dim] or [layers, rows, heads, capacity, head_dim]");
   const int64_t last = keys.dim() - 1;
   const bool heads_dim = keys.dim() == 5;
-  TORCH_CHECK_VALUE(stride_of(keys, last) <= 1, "head_dim must be contiguous");
+  TORCH_CHECK_VALUE(contiguous_along(keys, last), "head_dim must be contiguous");
   TORCH_CHECK_VALUE(!values.has_value() || (values->sizes() == keys.sizes() && values->strides() == keys.strides() &&
                                             values->scalar_type() == keys.scalar_type()),
                     "values must have the keys' shape, strides and dtype");

@@ -30,3 +30,23 @@ def test_broadcast_accumulated_weights_are_refused(sv, n):
     w = torch.zeros((K, R, C + 3), device=DEV).transpose(0, 1)
     sv.window_attention(q, k, k, weights=w)
     assert abs(w[..., :C].sum().item() - R * 4 * n) < 1e-2 and (w[..., C:] == 0).all()
+
+
+@pytest.mark.parametrize("n", [1, 40])
+def test_values_broadcast_along_head_dim(sv, n):
+    """One stored value for a whole head_dim: queries are copied out, caches refused."""
+    dtype = torch.float16
+    q, k, v = rand((2, n, 4, 64), 3, dtype), rand((2, 2, 50, 64), 4, dtype), rand((2, 2, 50, 64), 5, dtype)
+    for thin in (q[..., :1], q[:1, :1, :1, :1]):
+        wide = thin.expand(2, n, 4, 64)
+        assert torch.equal(sv.window_attention(wide, k, v), sv.window_attention(wide.contiguous(), k, v))
+        assert torch.equal(sv.prefix_attention(wide, k[0], v[0], k, v),
+                           sv.prefix_attention(wide.contiguous(), k[0], v[0], k, v))
+    flat = k[..., :1].expand(-1, -1, -1, 64)
+    with pytest.raises(ValueError):
+        sv.window_attention(q, flat, flat)
+    with pytest.raises(ValueError):
+        sv.prefix_attention(q, flat[0], flat[0], k, v)
+    weights, positions = torch.zeros((1, 2, 2, 50), device=DEV), torch.zeros((1, 2, 2, 50), dtype=torch.int32, device=DEV)
+    with pytest.raises(ValueError):
+        sv.kv_evict(flat[None], None, weights, positions, budget=20)
