@@ -463,6 +463,8 @@ extern "C" int sv_kv_evict(void* keys, void* values, int32_t elem_bytes, int32_t
   for (int k = 0; k < 4; ++k)
     if (sb[k] % 16 || sb[k] < 0) return SV_E_ALIGN;
   if (reinterpret_cast<uintptr_t>(keys) % 16 || reinterpret_cast<uintptr_t>(values) % 16) return SV_E_ALIGN;
+  // Every unit moves its own slots, in place.
+  if (!sv::entries_apart<4>(row, {layers, rows, heads, capacity}, sb)) return SV_E_SHAPE;
   EvictArgs a;
   a.cache[0] = static_cast<unsigned char*>(keys);
   a.cache[1] = static_cast<unsigned char*>(values);

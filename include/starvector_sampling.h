@@ -458,7 +458,7 @@ int sv_prefix_attention(const void* q, int32_t dtype, int32_t rows, int32_t toke
  * order afterwards (positions say which token a slot holds).  Slots >= budget keep
  * what they held.  A unit of n <= budget slots stays as it is.
  *   keys, values  as in sv_kv_reorder (values may be NULL), element (layer, row, head,
- *          slot, d); elem_bytes 1, 2 or 4
+ *          slot, d); elem_bytes 1, 2 or 4; no two of their elements may coincide
  *   weights, positions  float / int32 [layers, rows, heads, capacity], contiguous;
  *          not changed
  *   lengths  int32 [rows] or NULL (= capacity)

@@ -2,7 +2,7 @@
 below returns its code before any CUDA call."""
 import pytest
 
-from test_cache_capi import WINDOW, call
+from test_cache_capi import EVICT, WINDOW, call
 
 
 @pytest.mark.parametrize("kw", [
@@ -23,3 +23,12 @@ def test_accumulated_weights_that_overlap(sv, kw):
 def test_accumulated_weights_that_lie_apart(sv, kw):
     """Past the layout's check: the next thing that is missing is the workspace."""
     assert call(sv._lib.lib().sv_window_attention, {**WINDOW, "weights": 16, "w_row": 1000}, kw) == -6
+
+
+@pytest.mark.parametrize("kw", [
+    dict(s_layer=0), dict(s_row=0), dict(heads=2, s_head=0), dict(s_slot=0), dict(s_slot=64), dict(s_row=12672),
+    dict(s_layer=12800), dict(heads=2, s_head=12800, s_row=12800), dict(layers=1, rows=3, s_layer=0, s_row=6400),
+])
+def test_evicted_caches_that_overlap(sv, kw):
+    """Layers, rows, heads or slots that share memory would be moved by several units at once."""
+    assert call(sv._lib.lib().sv_kv_evict, EVICT, kw) == -3

@@ -50,3 +50,23 @@ def test_values_broadcast_along_head_dim(sv, n):
     weights, positions = torch.zeros((1, 2, 2, 50), device=DEV), torch.zeros((1, 2, 2, 50), dtype=torch.int32, device=DEV)
     with pytest.raises(ValueError):
         sv.kv_evict(flat[None], None, weights, positions, budget=20)
+
+
+def test_evicting_from_a_broadcast_cache_is_refused(sv):
+    base = rand((2, 2, 2, 50, 64), 6, torch.float16)
+    weights = torch.zeros((2, 2, 2, 50), device=DEV)
+    positions = torch.zeros((2, 2, 2, 50), dtype=torch.int32, device=DEV)
+    for d in range(4):
+        keys = base.narrow(d, 0, 1).expand(2, 2, 2, 50, 64)
+        before = keys.clone()
+        for values in (None, keys):
+            with pytest.raises(RuntimeError):
+                sv.kv_evict(keys, values, weights, positions, budget=20)
+        assert torch.equal(keys, before)
+    # Other orders of the dimensions are layouts like any other.
+    keys = rand((50, 2, 2, 2, 64), 7, torch.float16)
+    view, want = keys.permute(1, 2, 3, 0, 4), keys.clone().permute(1, 2, 3, 0, 4).contiguous()
+    weights.copy_(torch.rand(weights.shape, generator=torch.Generator(device=DEV).manual_seed(8), device=DEV))
+    a = sv.kv_evict(view, None, weights, positions, budget=20)
+    b = sv.kv_evict(want, None, weights, positions, budget=20)
+    assert torch.equal(view, want) and torch.equal(a["weights"], b["weights"])
