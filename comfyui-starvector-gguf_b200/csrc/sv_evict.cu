@@ -436,6 +436,17 @@ __global__ void __launch_bounds__(NT, PER_SM) kv_evict_kernel(const EvictArgs a)
   }
 }
 
+// Lengths updated in place: after the eviction, whose blocks all read them.
+__global__ void __launch_bounds__(256) lengths_kernel(int32_t* lengths, int rows, int capacity, int budget) {
+  const int r = blockIdx.x * 256 + threadIdx.x;
+  if (r < rows) lengths[r] = min(min(max(lengths[r], 0), capacity), budget);
+}
+
+bool overlap(const void* a, int64_t a_bytes, const void* b, int64_t b_bytes) {
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+  return a && b && x < y + (uintptr_t)b_bytes && y < x + (uintptr_t)a_bytes;
+}
+
 template <auto K> struct Kernel {
   static constexpr auto value = K;
 };
@@ -465,6 +476,19 @@ extern "C" int sv_kv_evict(void* keys, void* values, int32_t elem_bytes, int32_t
   if (reinterpret_cast<uintptr_t>(keys) % 16 || reinterpret_cast<uintptr_t>(values) % 16) return SV_E_ALIGN;
   // Every unit moves its own slots, in place.
   if (!sv::entries_apart<4>(row, {layers, rows, heads, capacity}, sb)) return SV_E_SHAPE;
+  // Blocks read a row's length, weights and positions while others write: outputs lie apart
+  // from the inputs and from one another (the new lengths may take the old ones' place).
+  const bool in_place = lengths_out && lengths_out == lengths;
+  const int64_t slots = 4ll * layers * rows * heads * capacity;
+  const void* outs[4] = {weights_out, positions_out, out_status, lengths_out};
+  const void* ins[3] = {weights, positions, lengths};
+  for (int i = 0; i < 4; ++i) {
+    const int64_t bytes = i < 2 ? slots : 4ll * rows;
+    for (int k = 0; k < 3; ++k)
+      if (!(in_place && i == 3 && k == 2) && overlap(outs[i], bytes, ins[k], k < 2 ? slots : 4ll * rows)) return SV_E_ARG;
+    for (int k = 0; k < i; ++k)
+      if (overlap(outs[i], bytes, outs[k], k < 2 ? slots : 4ll * rows)) return SV_E_ARG;
+  }
   EvictArgs a;
   a.cache[0] = static_cast<unsigned char*>(keys);
   a.cache[1] = static_cast<unsigned char*>(values);
@@ -484,7 +508,7 @@ extern "C" int sv_kv_evict(void* keys, void* values, int32_t elem_bytes, int32_t
   a.recent = recent;
   a.weights_out = weights_out;
   a.positions_out = positions_out;
-  a.lengths_out = lengths_out;
+  a.lengths_out = in_place ? nullptr : lengths_out;
   a.status = out_status;
   const int units = layers * rows * heads;
   a.lanes_log2 = 0;
@@ -511,5 +535,9 @@ extern "C" int sv_kv_evict(void* keys, void* values, int32_t elem_bytes, int32_t
     in_smem ? run(Kernel<kv_evict_kernel<256, 7, true>>()) : run(Kernel<kv_evict_kernel<256, 7, false>>());
   else
     in_smem ? run(Kernel<kv_evict_kernel<1024, 1, true>>()) : run(Kernel<kv_evict_kernel<1024, 1, false>>());
+  if (in_place && e == cudaSuccess) {
+    lengths_kernel<<<(rows + 255) / 256, 256, 0, static_cast<cudaStream_t>(stream)>>>(lengths_out, rows, capacity, budget);
+    e = cudaGetLastError();
+  }
   return e == cudaSuccess ? SV_OK : SV_E_CUDA;
 }

@@ -616,7 +616,8 @@ def kv_evict(keys, values, weights, positions, lengths=None, budget=None, *, sin
     head_dim, contiguous; lengths: int32 [rows] on the device, one number or None
     (all slots).  Returns a dict of new tensors (or fills `out`): lengths, weights
     and positions after the eviction; the slots' order is not the tokens' order any
-    more, so attend to such a cache without a window."""
+    more, so attend to such a cache without a window.  out["lengths"] may be `lengths`
+    itself, updated in place; the other outputs need memory of their own."""
     if budget is None:
         raise ValueError("budget must be given")
     number = isinstance(lengths, int)

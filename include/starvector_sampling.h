@@ -464,7 +464,9 @@ int sv_prefix_attention(const void* q, int32_t dtype, int32_t rows, int32_t toke
  *   lengths  int32 [rows] or NULL (= capacity)
  *   weights_out, positions_out  the same shape, other buffers: the kept slots' values
  *          in their new places, 0 / -1 in every slot past them
- *   lengths_out  int32 [rows] or NULL: min(length, budget)
+ *   lengths_out  int32 [rows] or NULL: min(length, budget); may be `lengths` itself
+ *          (then written by a second launch).  Outputs otherwise overlap neither inputs
+ *          nor one another (SV_E_ARG)
  *   out_status   int32 [rows] or NULL: SV_ST_LENGTH for a length outside [0, capacity]
  * 1 <= budget <= capacity <= 2^20; sinks + recent <= budget; layers * rows * heads <=
  * 65535; head_dim * elem_bytes at most 16384 and, like the strides in bytes and the

@@ -32,3 +32,24 @@ def test_accumulated_weights_that_lie_apart(sv, kw):
 def test_evicted_caches_that_overlap(sv, kw):
     """Layers, rows, heads or slots that share memory would be moved by several units at once."""
     assert call(sv._lib.lib().sv_kv_evict, EVICT, kw) == -3
+
+
+SIZE = 4 * 2 * 2 * 100  # bytes of EVICT's weights, of its positions
+APART = {**EVICT, "weights": 1 << 20, "positions": 2 << 20, "lengths": 3 << 20, "w_out": 4 << 20, "p_out": 5 << 20,
+         "l_out": 6 << 20, "status": 7 << 20}
+
+
+@pytest.mark.parametrize("out,into", [(o, i) for o in ("w_out", "p_out", "l_out", "status")
+                                      for i in ("weights", "positions", "lengths")])
+def test_eviction_outputs_over_inputs(sv, out, into):
+    """Every output over every input, from its start, its last word or from a word before it."""
+    last = {"weights": SIZE, "positions": SIZE, "lengths": 8}[into] - 4
+    size = {"w_out": SIZE, "p_out": SIZE, "l_out": 8, "status": 8}[out]
+    for at in (0, last, 4 - size):
+        if not (out == "l_out" and into == "lengths" and at == 0):
+            assert call(sv._lib.lib().sv_kv_evict, APART, {out: APART[into] + at}) == -1
+
+
+@pytest.mark.parametrize("a,b", [("w_out", "p_out"), ("l_out", "w_out"), ("status", "p_out"), ("l_out", "status")])
+def test_eviction_outputs_over_one_another(sv, a, b):
+    assert call(sv._lib.lib().sv_kv_evict, APART, {a: APART[b] + 4}) == -1

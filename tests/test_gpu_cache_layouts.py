@@ -70,3 +70,28 @@ def test_evicting_from_a_broadcast_cache_is_refused(sv):
     a = sv.kv_evict(view, None, weights, positions, budget=20)
     b = sv.kv_evict(want, None, weights, positions, budget=20)
     assert torch.equal(view, want) and torch.equal(a["weights"], b["weights"])
+
+
+@pytest.mark.parametrize("shape,lengths,budget", [
+    ((32, 8, 4, 130, 16), [130, 129, 65, 64, 0, 200, -1, 100], 64),  # many waves of blocks
+    ((2, 3, 1, 5000, 64), [5000, 1001, 900], 1000)])                 # several blocks share a unit
+def test_lengths_updated_in_place(sv, shape, lengths, budget):
+    """out["lengths"] is `lengths`: every layer, head and part still evicts by the old ones."""
+    g = torch.Generator(device=DEV).manual_seed(9)
+    keys = torch.randn(shape, generator=g, device=DEV).half()
+    weights = torch.rand(shape[:-1], generator=g, device=DEV)
+    positions = torch.argsort(torch.rand(shape[:-1], generator=g, device=DEV), -1).int()
+    old = torch.tensor(lengths, dtype=torch.int32, device=DEV)
+    want_keys, want_values = keys.clone(), -keys
+    want = sv.kv_evict(want_keys, want_values, weights, positions, old, budget, sinks=4, recent=16)
+    for _ in range(5):
+        k, v, n = keys.clone(), -keys, old.clone()
+        status = torch.full_like(n, -1)
+        got = sv.kv_evict(k, v, weights, positions, n, budget, sinks=4, recent=16, out={"lengths": n}, status=status)
+        assert got["lengths"] is n and torch.equal(n, want["lengths"])
+        assert n.tolist() == [min(max(0, min(x, shape[3])), budget) for x in lengths]
+        assert status.tolist() == [0 if 0 <= x <= shape[3] else 8 for x in lengths]
+        assert torch.equal(k, want_keys) and torch.equal(v, want_values)
+        assert torch.equal(got["weights"], want["weights"]) and torch.equal(got["positions"], want["positions"])
+    with pytest.raises(RuntimeError):
+        sv.kv_evict(k, v, weights, positions, n, budget, status=n)
