@@ -60,7 +60,7 @@ struct Shared {
   // full, ready: a stage's copy, and its edge-tile pass.  s_full, pv_done: a query tile's scores of step j and
   // its product of step j (they also free the step's keys and values); one barrier for each of the four steps
   // that the ring holds, so that none gets two phases ahead of who waits for it.
-  uint64_t q_full[2], full[STAGES], ready[STAGES], s_full[2][RING], p_full[2][2], pv_done[2][RING], written, drained;
+  uint64_t q_full[2], full[STAGES], ready[STAGES], s_full[2][RING], p_full[2][2], pv_done[2][RING], written[2], drained;
   float2 pair[BM];  // PAIRED: the second group's references and sums
   uint32_t tmem;
   uint32_t bad[kEdges][BN / 32];  // per edge tile: its slots with values that are not finite
@@ -268,6 +268,7 @@ __global__ void __launch_bounds__(NT, 1) attn_tile_kernel(const __grid_constant_
   if (tid == 0) {
     for (int i = 0; i < 2; ++i) {
       mbar_init(&sh.q_full[i], 128);
+      mbar_init(&sh.written[i], 128);
       for (int k = 0; k < 2; ++k) mbar_init(&sh.p_full[i][k], 128);
       for (int k = 0; k < RING; ++k) {
         mbar_init(&sh.s_full[i][k], 1);
@@ -278,7 +279,6 @@ __global__ void __launch_bounds__(NT, 1) attn_tile_kernel(const __grid_constant_
       mbar_init(&sh.full[i], 1);
       mbar_init(&sh.ready[i], 1);
     }
-    mbar_init(&sh.written, 256);
     mbar_init(&sh.drained, 2);
     sh.any_bad = 0;
     for (int i = 0; i < kEdges; ++i)
@@ -444,12 +444,18 @@ __global__ void __launch_bounds__(NT, 1) attn_tile_kernel(const __grid_constant_
     }
   } else if (warp == 11) {
     // ------------------------------------------------------------- values of edge tiles
-    int base = 0, count = 0;
+    // Before an item's notes are made those of the item before have to be read: by the groups
+    // that had rows and steps in it, no others.  Such a group cannot end its next item before
+    // this warp has let that item's steps go, so it is never two phases ahead of a wait here.
+    int base = 0, read_by = 0, phases[2] = {0, 0};  // the groups that read the item before's notes
     bool ok = true;
-    for (int w = blockIdx.x; ok && w < items; w += gridDim.x, ++count) {
+    for (int w = blockIdx.x; ok && w < items; w += gridDim.x) {
       if (w != (int)blockIdx.x) it = item_at(w);
-      if (count > 0) {  // the notes of the item before have been read
-        ok = wait(sh, &sh.written, (count - 1) & 1);
+      if (it.nt <= 0) continue;  // no steps, no notes
+      if (read_by > 0) {
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+          if (t < read_by) ok = ok && wait(sh, &sh.written[t], phases[t]++ & 1);
         if (!ok) break;
         if (sh.any_bad) {
           __syncwarp();
@@ -458,6 +464,7 @@ __global__ void __launch_bounds__(NT, 1) attn_tile_kernel(const __grid_constant_
           __syncwarp();
         }
       }
+      read_by = it.mt;
       int edge = 0;
       const Whole whole = whole_steps(it, it.m0, it.m_last);
       for (int j = 0; j < it.nt; ++j) {
@@ -666,7 +673,7 @@ __global__ void __launch_bounds__(NT, 1) attn_tile_kernel(const __grid_constant_
       }
       if (t < it.mt) {
         ok = __all_sync(0xffffffffu, ok && !sh.abort);
-        const bool any_bad = *static_cast<volatile int*>(&sh.any_bad) != 0;
+        const bool any_bad = it.nt > 0 && *static_cast<volatile int*>(&sh.any_bad) != 0;
         const float inv = !ok ? __int_as_float(0x7fc00000) : (l == 0.f ? 0.f : (direct ? 1.f / l : 1.f));
 #pragma unroll 1
         for (int c = 0; c < 64 * DC; c += 32) {
@@ -767,7 +774,7 @@ __global__ void __launch_bounds__(NT, 1) attn_tile_kernel(const __grid_constant_
         else if (it.m0 == 0 && it.split == 0)
           a.status[it.r] = (e < 0 || e > a.capacity || s < 0 || s > max(e, 0)) ? SV_ST_LENGTH : 0;
       }
-      mbar_arrive(&sh.written);
+      if (t < it.mt && it.nt > 0) mbar_arrive(&sh.written[t]);
     }
   }
   __syncthreads();
