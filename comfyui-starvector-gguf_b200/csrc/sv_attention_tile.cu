@@ -322,9 +322,9 @@ __global__ void __launch_bounds__(NT, 1) attn_tile_kernel(const __grid_constant_
                       it.r * maps.row_mul, &sh.full[st]);
         }
       }
-      // After an abort nothing may still be landing when the block ends.
-      if (sh.abort)
-        for (int i = max(0, issued - STAGES); i < issued; ++i) mbar_wait(&sh.full[i % STAGES], (i / STAGES) & 1);
+      // Nothing may still be landing when the block ends.  (Without an abort its steps wait for it
+      // anyway; one may still come after this point.)
+      for (int i = max(0, issued - STAGES); i < issued; ++i) mbar_wait(&sh.full[i % STAGES], (i / STAGES) & 1);
     }
   } else if (warp == 9 || warp == 10) {
     // ------------------------------------------------------------- products
