@@ -22,9 +22,12 @@
 // weights come from L2) and copies its part of the moves, which needs no exchange.
 //
 // Bound by the moved bytes when many slots move, by the selection's latency otherwise.
+// Past kSmemKeys slots keys and positions are read again from global memory where they are
+// needed, lists of moves are searched bit by bit, and only every eighth word has its counts.
 #include <cuda_runtime.h>
 
 #include <cstdint>
+#include <type_traits>
 
 #include "../../include/starvector_sampling.h"
 #include "sv_attention.h"
@@ -33,6 +36,8 @@ namespace {
 
 constexpr int kBins = 1024;
 constexpr int kSmemKeys = 24576;  // slots whose keys and positions are kept in shared memory
+constexpr int kMostSlots = 1 << 20;
+constexpr int kSparse = 8;  // past kSmemKeys: words per count, so that the bits of kMostSlots fit beside their counts
 constexpr uint32_t kTop = 0xff800000u;  // the key of +inf, and of protected slots
 
 struct EvictArgs {
@@ -61,16 +66,19 @@ __device__ __forceinline__ uint32_t rank_key(float w, int pos, int sinks, int re
   return ordered(w + 0.0f);        // -0 ties with +0
 }
 
-// The position of the k-th (from 0) set bit of the words whose exclusive prefix counts
-// are `before` (nw + 1 entries); word(i) gives the words.
-template <typename F>
-__device__ __forceinline__ int select_bit(const int* before, int nw, int k, F word) {
-  int lo = 0, hi = nw;  // before[lo] <= k < before[hi]
+// The position of the k-th (from 0) set bit of words whose exclusive prefix counts, one
+// for every WPC words, are `before` (n + 1 entries); word(i) gives the words.
+template <int WPC, typename F>
+__device__ __forceinline__ int select_bit(const int* before, int n, int k, F word) {
+  int lo = 0, hi = n;  // before[lo] <= k < before[hi]
   while (hi - lo > 1) {
     const int mid = (lo + hi) >> 1;
     if (before[mid] <= k) lo = mid; else hi = mid;
   }
-  return lo * 32 + (int)__fns(word(lo), 0, k - before[lo] + 1);
+  int i = lo * WPC, left = k - before[lo];
+  if (WPC > 1)
+    for (int c; left >= (c = __popc(word(i))); ++i) left -= c;
+  return i * 32 + (int)__fns(word(i), 0, left + 1);
 }
 
 // Four consecutive values from j on (fill past n); vec: the four can be read at once.
@@ -95,10 +103,15 @@ __device__ __forceinline__ uint32_t below_bits(int i, int B) {
 template <int NT, int PER_SM, bool SMEM_KEYS>
 __global__ void __launch_bounds__(NT, PER_SM) kv_evict_kernel(const EvictArgs a) {
   constexpr int NW = NT / 32, PER = kBins / NT;  // bins per thread
+  constexpr int WPC = SMEM_KEYS ? 1 : kSparse;   // words per count
+  using Both = std::conditional_t<SMEM_KEYS, uint32_t, unsigned long long>;  // two counts of a round in one value
+  constexpr int kHalf = sizeof(Both) * 4;
   extern __shared__ uint32_t dyn[];
   __shared__ int bins[kBins];
   __shared__ int warp_count[NW], sh_bin, sh_over, sh_need;
   __shared__ int sh_newest;
+  __shared__ Both warp_both[NW];
+  __shared__ uint32_t round_ties[SMEM_KEYS ? 1 : NT / 8];
   __shared__ uint32_t sh_low, sh_high;
   const int unit = blockIdx.y, part = blockIdx.x;
   const int h = unit % a.heads, r = (unit / a.heads) % a.rows, layer = unit / (a.heads * a.rows);
@@ -145,12 +158,12 @@ __global__ void __launch_bounds__(NT, PER_SM) kv_evict_kernel(const EvictArgs a)
     copy_meta(0);
     return;
   }
-  const int nw = (n + 31) >> 5, n4 = (n + 3) & ~3;
+  const int nw = (n + 31) >> 5, counts = (nw + WPC - 1) / WPC, n4 = (n + 3) & ~3;
   uint32_t* keys = dyn;                                    // [n4], later the lists of moves
   int* held = reinterpret_cast<int*>(keys + (SMEM_KEYS ? n4 : 0));  // [n4] positions
   uint32_t* kept = reinterpret_cast<uint32_t*>(held + (SMEM_KEYS ? n4 : 0));  // one bit per slot
-  int* holes = reinterpret_cast<int*>(kept + nw);          // exclusive counts per word, nw + 1
-  int* comes = holes + nw + 1;
+  int* holes = reinterpret_cast<int*>(kept + nw);          // exclusive counts per WPC words, counts + 1
+  int* comes = holes + counts + 1;
 
   // Newest position, then the keys and their range (protected ones left out).
   if (tid == 0) {
@@ -306,6 +319,34 @@ __global__ void __launch_bounds__(NT, PER_SM) kv_evict_kernel(const EvictArgs a)
   }
   const int ties = B - above;
 
+  // The first `ties` of the tied slots stay: warp 0 goes through the words of ties (of words
+  // `first` on) in order.
+  uint32_t* tie_words = SMEM_KEYS ? reinterpret_cast<uint32_t*>(holes) : round_ties;
+  int tied = 0;
+  auto take_ties = [&](int first, int words) {
+    for (int i0 = 0; i0 < words && tied < ties; i0 += 32) {
+      const int i = i0 + lane;
+      uint32_t eq = i < words ? tie_words[i] : 0u, bits = 0u;
+      const int c = __popc(eq);
+      int s = c;
+#pragma unroll
+      for (int k = 1; k < 32; k <<= 1) {
+        const int x = __shfl_up_sync(0xffffffffu, s, k);
+        if (lane >= k) s += x;
+      }
+      int room = ties - (tied + s - c);
+      tied += __shfl_sync(0xffffffffu, s, 31);
+      if (room >= c) {
+        bits = eq;
+      } else {
+        for (; room > 0; --room) {
+          bits |= eq & (0u - eq);
+          eq &= eq - 1u;
+        }
+      }
+      if (i < words) kept[first + i] |= bits;
+    }
+  };
   // One bit per slot: a thread compares four, eight threads make a word.
   for (int i0 = 0; i0 < nw; i0 += NT / 8) {
     const int i = i0 + (tid >> 3), j = i * 32 + (tid & 7) * 4;
@@ -325,71 +366,58 @@ __global__ void __launch_bounds__(NT, PER_SM) kv_evict_kernel(const EvictArgs a)
     }
     if (!(tid & 7) && i < nw) {
       kept[i] = exact ? at : over;
-      if (!exact) holes[i] = (int)(at & ~over);  // the ties, resolved next
+      if (!exact) tie_words[SMEM_KEYS ? i : tid >> 3] = at & ~over;
+    }
+    if (!SMEM_KEYS && !exact) {  // there is room for one round's ties only
+      __syncthreads();
+      if (warp == 0) take_ties(i0, min(NT / 8, nw - i0));
+      __syncthreads();
     }
   }
   __syncthreads();
-  if (!exact) {
-    if (warp == 0) {
-      int tied = 0;
-      for (int i0 = 0; i0 < nw && tied < ties; i0 += 32) {
-        const int i = i0 + lane;
-        uint32_t eq = i < nw ? (uint32_t)holes[i] : 0u, bits = 0u;
-        const int c = __popc(eq);
-        int s = c;
-#pragma unroll
-        for (int k = 1; k < 32; k <<= 1) {
-          const int x = __shfl_up_sync(0xffffffffu, s, k);
-          if (lane >= k) s += x;
-        }
-        int room = ties - (tied + s - c);
-        tied += __shfl_sync(0xffffffffu, s, 31);
-        if (room >= c) {
-          bits = eq;
-        } else {
-          for (; room > 0; --room) {
-            bits |= eq & (0u - eq);
-            eq &= eq - 1u;
-          }
-        }
-        if (i < nw) kept[i] |= bits;
-      }
-    }
+  if (SMEM_KEYS && !exact) {
+    if (warp == 0) take_ties(0, nw);
     __syncthreads();
   }
-  // Exclusive counts per word, a word per thread (both counts in one value: NT words hold
-  // at most 32 NT = 2^15 slots).
+  // Exclusive counts, those of WPC words per thread (both in one value: NT words hold at most
+  // 32 NT = 2^15 slots, for the sparse counts' eight times as many the value is wider).
   int nh = 0, nc = 0;
-  for (int i0 = 0; i0 < nw; i0 += NT) {
+  for (int i0 = 0; i0 < counts; i0 += NT) {
     const int i = i0 + tid;
-    const uint32_t bits = i < nw ? kept[i] : 0u, below = below_bits(i, B);
-    const uint32_t c = i < nw ? (uint32_t)__popc(~bits & below) | (uint32_t)__popc(bits & ~below) << 16 : 0u;
-    uint32_t s = c;
+    Both c = 0;
+#pragma unroll 1
+    for (int k = 0; k < WPC; ++k) {
+      const int x = i * WPC + k;
+      const uint32_t bits = x < nw ? kept[x] : 0u, below = below_bits(x, B);
+      if (x < nw) c += (Both)__popc(~bits & below) | (Both)__popc(bits & ~below) << kHalf;
+    }
+    Both s = c;
 #pragma unroll
     for (int k = 1; k < 32; k <<= 1) {
-      const uint32_t x = __shfl_up_sync(0xffffffffu, s, k);
+      const Both x = __shfl_up_sync(0xffffffffu, s, k);
       if (lane >= k) s += x;
     }
-    if (lane == 31) warp_count[warp] = (int)s;
+    if (lane == 31) warp_both[warp] = s;
     __syncthreads();
-    uint32_t all = 0;
+    Both all = 0;
 #pragma unroll
     for (int k = 0; k < NW; ++k) {
       if (k == warp) s += all;
-      all += (uint32_t)warp_count[k];
+      all += warp_both[k];
     }
     s -= c;
-    if (i < nw) {
-      holes[i] = nh + (int)(s & 0xffffu);
-      comes[i] = nc + (int)(s >> 16);
+    constexpr Both low = ((Both)1 << kHalf) - 1;
+    if (i < counts) {
+      holes[i] = nh + (int)(s & low);
+      comes[i] = nc + (int)(s >> kHalf);
     }
-    nh += (int)(all & 0xffffu);
-    nc += (int)(all >> 16);
+    nh += (int)(all & low);
+    nc += (int)(all >> kHalf);
     __syncthreads();
   }
-  if (tid == 0) holes[nw] = nh, comes[nw] = nc;
+  if (tid == 0) holes[counts] = nh, comes[counts] = nc;
   __syncthreads();
-  const int moved = comes[nw];
+  const int moved = comes[counts];
   auto hole_bits = [&](int i) { return ~kept[i] & below_bits(i, B); };
   auto come_bits = [&](int i) { return kept[i] & ~below_bits(i, B); };
   // The lists of survivors past the budget and of holes below it, over the keys (at most
@@ -406,8 +434,8 @@ __global__ void __launch_bounds__(NT, PER_SM) kv_evict_kernel(const EvictArgs a)
     }
     __syncthreads();
   }
-  auto src_of = [&](int k) { return SMEM_KEYS ? src_list[k] : select_bit(comes, nw, k, come_bits); };
-  auto dst_of = [&](int k) { return SMEM_KEYS ? dst_list[k] : select_bit(holes, nw, k, hole_bits); };
+  auto src_of = [&](int k) { return SMEM_KEYS ? src_list[k] : select_bit<WPC>(comes, counts, k, come_bits); };
+  auto dst_of = [&](int k) { return SMEM_KEYS ? dst_list[k] : select_bit<WPC>(holes, counts, k, hole_bits); };
 
   // Keys and values: a group of lanes per moved slot, four slots in flight.
   const int64_t base = layer * a.s_layer + r * a.s_row + h * a.s_head;
@@ -462,7 +490,7 @@ extern "C" int sv_kv_evict(void* keys, void* values, int32_t elem_bytes, int32_t
   if (!keys || !weights || !positions || !weights_out || !positions_out) return SV_E_ARG;
   if (weights == weights_out || positions == positions_out) return SV_E_ARG;
   if (elem_bytes != 1 && elem_bytes != 2 && elem_bytes != 4) return SV_E_DTYPE;
-  if (layers < 1 || rows < 1 || heads < 1 || capacity < 1 || head_dim < 1 || capacity > (1 << 20)) return SV_E_SHAPE;
+  if (layers < 1 || rows < 1 || heads < 1 || capacity < 1 || head_dim < 1 || capacity > kMostSlots) return SV_E_SHAPE;
   if ((int64_t)layers * rows * heads > 65535) return SV_E_SHAPE;
   if (budget < 1 || budget > capacity || sinks < 0 || recent < 0 || (int64_t)sinks + recent > budget)
     return SV_E_RANGE;
@@ -521,7 +549,8 @@ extern "C" int sv_kv_evict(void* keys, void* values, int32_t elem_bytes, int32_t
   if (a.parts > 16) a.parts = 16;
   const bool in_smem = capacity <= kSmemKeys;
   const size_t nw = (capacity + 31) / 32;
-  const size_t smem = 4 * (3 * nw + 2 + (in_smem ? 2 * ((capacity + 3) & ~3) : 0));
+  const size_t smem = 4 * (in_smem ? 3 * nw + 2 + 2 * ((capacity + 3) & ~3) : nw + 2 * ((nw + kSparse - 1) / kSparse + 1));
+  static_assert(4 * (kMostSlots / 32 + 2 * (kMostSlots / 32 / kSparse + 1)) <= 220 * 1024, "the bits and counts fit");
   static_assert(4 * (3 * (kSmemKeys / 32) + 2 + 2 * kSmemKeys) <= 220 * 1024, "the keys fit a block's shared memory");
   cudaError_t e;
   auto run = [&](auto which) {
