@@ -23,7 +23,7 @@
 //
 // Bound by the moved bytes when many slots move, by the selection's latency otherwise.
 // Past kSmemKeys slots keys and positions are read again from global memory where they are
-// needed, lists of moves are searched bit by bit, and only every eighth word has its counts.
+// needed and lists of moves are searched bit by bit.
 #include <cuda_runtime.h>
 
 #include <cstdint>
@@ -37,7 +37,11 @@ namespace {
 constexpr int kBins = 1024;
 constexpr int kSmemKeys = 24576;  // slots whose keys and positions are kept in shared memory
 constexpr int kMostSlots = 1 << 20;
-constexpr int kSparse = 8;  // past kSmemKeys: words per count, so that the bits of kMostSlots fit beside their counts
+constexpr size_t kMostSmem = 220 * 1024;  // of a block's shared memory, for what depends on the capacity
+// Words per count where counts for every word would not fit, from 600705 slots on.  (With counts
+// for every eighth word 2 units of 40000 slots took 117 us, 105 with all, and 300 units of 30000
+// slots 556 and 511; one of 600000 slots 905 and 1000.)
+constexpr int kSparse = 4;
 constexpr uint32_t kTop = 0xff800000u;  // the key of +inf, and of protected slots
 
 struct EvictArgs {
@@ -100,18 +104,17 @@ __device__ __forceinline__ uint32_t below_bits(int i, int B) {
   return left >= 32 ? 0xffffffffu : (left <= 0 ? 0u : (1u << left) - 1u);
 }
 
-template <int NT, int PER_SM, bool SMEM_KEYS>
+template <int NT, int PER_SM, bool SMEM_KEYS, int WPC>  // WPC: words per count
 __global__ void __launch_bounds__(NT, PER_SM) kv_evict_kernel(const EvictArgs a) {
   constexpr int NW = NT / 32, PER = kBins / NT;  // bins per thread
-  constexpr int WPC = SMEM_KEYS ? 1 : kSparse;   // words per count
-  using Both = std::conditional_t<SMEM_KEYS, uint32_t, unsigned long long>;  // two counts of a round in one value
+  using Both = std::conditional_t<WPC == 1, uint32_t, unsigned long long>;  // two counts of a round in one value
   constexpr int kHalf = sizeof(Both) * 4;
   extern __shared__ uint32_t dyn[];
   __shared__ int bins[kBins];
   __shared__ int warp_count[NW], sh_bin, sh_over, sh_need;
   __shared__ int sh_newest;
   __shared__ Both warp_both[NW];
-  __shared__ uint32_t round_ties[SMEM_KEYS ? 1 : NT / 8];
+  __shared__ uint32_t round_ties[WPC == 1 ? 1 : NT / 8];
   __shared__ uint32_t sh_low, sh_high;
   const int unit = blockIdx.y, part = blockIdx.x;
   const int h = unit % a.heads, r = (unit / a.heads) % a.rows, layer = unit / (a.heads * a.rows);
@@ -321,7 +324,7 @@ __global__ void __launch_bounds__(NT, PER_SM) kv_evict_kernel(const EvictArgs a)
 
   // The first `ties` of the tied slots stay: warp 0 goes through the words of ties (of words
   // `first` on) in order.
-  uint32_t* tie_words = SMEM_KEYS ? reinterpret_cast<uint32_t*>(holes) : round_ties;
+  uint32_t* tie_words = WPC == 1 ? reinterpret_cast<uint32_t*>(holes) : round_ties;
   int tied = 0;
   auto take_ties = [&](int first, int words) {
     for (int i0 = 0; i0 < words && tied < ties; i0 += 32) {
@@ -366,21 +369,21 @@ __global__ void __launch_bounds__(NT, PER_SM) kv_evict_kernel(const EvictArgs a)
     }
     if (!(tid & 7) && i < nw) {
       kept[i] = exact ? at : over;
-      if (!exact) tie_words[SMEM_KEYS ? i : tid >> 3] = at & ~over;
+      if (!exact) tie_words[WPC == 1 ? i : tid >> 3] = at & ~over;
     }
-    if (!SMEM_KEYS && !exact) {  // there is room for one round's ties only
+    if (WPC > 1 && !exact) {  // there is room for one round's ties only
       __syncthreads();
       if (warp == 0) take_ties(i0, min(NT / 8, nw - i0));
       __syncthreads();
     }
   }
   __syncthreads();
-  if (SMEM_KEYS && !exact) {
+  if (WPC == 1 && !exact) {
     if (warp == 0) take_ties(0, nw);
     __syncthreads();
   }
   // Exclusive counts, those of WPC words per thread (both in one value: NT words hold at most
-  // 32 NT = 2^15 slots, for the sparse counts' eight times as many the value is wider).
+  // 32 NT = 2^15 slots, for sparse counts the value is wider).
   int nh = 0, nc = 0;
   for (int i0 = 0; i0 < counts; i0 += NT) {
     const int i = i0 + tid;
@@ -549,21 +552,25 @@ extern "C" int sv_kv_evict(void* keys, void* values, int32_t elem_bytes, int32_t
   if (a.parts > 16) a.parts = 16;
   const bool in_smem = capacity <= kSmemKeys;
   const size_t nw = (capacity + 31) / 32;
-  const size_t smem = 4 * (in_smem ? 3 * nw + 2 + 2 * ((capacity + 3) & ~3) : nw + 2 * ((nw + kSparse - 1) / kSparse + 1));
-  static_assert(4 * (kMostSlots / 32 + 2 * (kMostSlots / 32 / kSparse + 1)) <= 220 * 1024, "the bits and counts fit");
-  static_assert(4 * (3 * (kSmemKeys / 32) + 2 + 2 * kSmemKeys) <= 220 * 1024, "the keys fit a block's shared memory");
+  const size_t dense = 4 * (3 * nw + 2 + (in_smem ? 2 * ((capacity + 3) & ~3) : 0));
+  const bool sparse = dense > kMostSmem;
+  const size_t smem = sparse ? 4 * (nw + 2 * ((nw + kSparse - 1) / kSparse + 1)) : dense;
+  static_assert(4 * (3 * (kSmemKeys / 32) + 2 + 2 * kSmemKeys) <= kMostSmem, "the keys fit a block's shared memory");
+  static_assert(4 * (kMostSlots / 32 + 2 * (kMostSlots / 32 / kSparse + 1)) <= kMostSmem, "bits and sparse counts fit");
   cudaError_t e;
   auto run = [&](auto which) {
     constexpr auto kernel = decltype(which)::value;
-    e = smem > 40 * 1024 ? sv::allow_smem<kernel>(220 * 1024) : cudaSuccess;
+    e = smem > 40 * 1024 ? sv::allow_smem<kernel>(kMostSmem) : cudaSuccess;
     if (e != cudaSuccess) return;
-    kernel<<<dim3(a.parts, units), many ? 256 : 1024, smem, static_cast<cudaStream_t>(stream)>>>(a);
+    kernel<<<dim3(a.parts, units), many && !sparse ? 256 : 1024, smem, static_cast<cudaStream_t>(stream)>>>(a);
     e = cudaGetLastError();
   };
-  if (many)
-    in_smem ? run(Kernel<kv_evict_kernel<256, 7, true>>()) : run(Kernel<kv_evict_kernel<256, 7, false>>());
+  if (sparse)
+    run(Kernel<kv_evict_kernel<1024, 1, false, kSparse>>());
+  else if (many)
+    in_smem ? run(Kernel<kv_evict_kernel<256, 7, true, 1>>()) : run(Kernel<kv_evict_kernel<256, 7, false, 1>>());
   else
-    in_smem ? run(Kernel<kv_evict_kernel<1024, 1, true>>()) : run(Kernel<kv_evict_kernel<1024, 1, false>>());
+    in_smem ? run(Kernel<kv_evict_kernel<1024, 1, true, 1>>()) : run(Kernel<kv_evict_kernel<1024, 1, false, 1>>());
   if (in_place && e == cudaSuccess) {
     lengths_kernel<<<(rows + 255) / 256, 256, 0, static_cast<cudaStream_t>(stream)>>>(lengths_out, rows, capacity, budget);
     e = cudaGetLastError();
