@@ -173,6 +173,7 @@ int run(AttnArgs& a, void* workspace, size_t workspace_bytes, cudaStream_t strea
     if (a.scores) return launch_scores_weights(a, stream) == cudaSuccess ? SV_OK : SV_E_CUDA;
     return a.weights ? run_weights(a, stream) : SV_OK;
   }
+  if (a.status && !f32 && launch_attn_status(a, stream) != cudaSuccess) return SV_E_CUDA;
   if ((f32 ? launch_attn_f32(a, false, stream) : launch_attn_tile(a, false, p.own, stream)) != cudaSuccess)
     return SV_E_CUDA;
   if (p.o_splits && launch_attn_combine(a, stream) != cudaSuccess) return SV_E_CUDA;

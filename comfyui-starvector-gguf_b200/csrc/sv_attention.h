@@ -50,6 +50,7 @@ struct AttnArgs {
   float* weight_parts; // [w_splits][rows * kv_heads][capacity], with weights and w_splits > 1
   int32_t p_splits, o_splits;  // o_splits 0: the own part is written directly
   int32_t w_splits;            // of the query rows, for the accumulated weights of calls with many
+  int32_t test_head;           // test hook: one plus the key/value head whose waits run out
 };
 
 // A prefix part's rows are numbered by head first: (h * rows + r) * n * G + m.
@@ -201,6 +202,7 @@ struct TileSplit {
   int tiles, splits;
   bool paired;
 };
+cudaError_t launch_attn_status(const AttnArgs& a, cudaStream_t stream);
 cudaError_t launch_attn_tile(const AttnArgs& a, bool prefix, const TileSplit& split, cudaStream_t stream);
 cudaError_t launch_attn_token(const AttnArgs& a, int blocks, cudaStream_t stream);
 cudaError_t launch_weights16(const AttnArgs& a, cudaStream_t stream);

@@ -1,5 +1,6 @@
 // sv_attention_join.cu -- what follows the attention kernels: the join of parts that
 // were split over the slots, and the accumulated weights of calls with many queries.
+#include "../../include/starvector_sampling.h"
 #include "sv_attention.h"
 
 namespace sv {
@@ -119,6 +120,14 @@ __global__ void __launch_bounds__(NT) weights_sum_kernel(const AttnArgs a) {
   a.weights[r * a.w_row + h * a.w_head + j] += t;
 }
 
+// The rows' statuses ahead of the tile kernel, any of whose blocks may then report that it gave up.
+__global__ void __launch_bounds__(NT) attn_status_kernel(const AttnArgs a) {
+  const int r = blockIdx.x * NT + threadIdx.x;
+  if (r >= a.rows) return;
+  const int e = a.lengths ? a.lengths[r] : a.capacity, s = a.starts ? a.starts[r] : 0;
+  a.status[r] = (e < 0 || e > a.capacity || s < 0 || s > max(e, 0)) ? SV_ST_LENGTH : 0;
+}
+
 // Joins the splits of one query row per warp: a lane holds four dimensions.
 template <typename T>
 __global__ void __launch_bounds__(NT) attn_combine_kernel(const AttnArgs a) {
@@ -168,6 +177,11 @@ __global__ void __launch_bounds__(NT) attn_combine_kernel(const AttnArgs a) {
 }
 
 }  // namespace
+
+cudaError_t launch_attn_status(const AttnArgs& a, cudaStream_t stream) {
+  attn_status_kernel<<<(unsigned)((a.rows + NT - 1) / NT), NT, 0, stream>>>(a);
+  return cudaGetLastError();
+}
 
 cudaError_t launch_attn_combine(const AttnArgs& a, cudaStream_t stream) {
   const int64_t all = (int64_t)a.rows * a.n * a.heads;

@@ -409,8 +409,8 @@ int sv_beam_advance(const int64_t* picks, const float* pick_scores, const int32_
  * heads a multiple of kv_heads; rows * kv_heads <= 65535; rows * tokens * heads <=
  * 2^30; capacity (and prefix_length) <= 2^29, with a slot stride other than 0 (rows and
  * heads may be broadcast); pointers and every stride in bytes multiples of 16.  A wait
- * inside a kernel that runs out (~2 s) gives NaN outputs and SV_ST_TIMEOUT (the latter
- * not where it is the prefix's).
+ * inside a kernel that runs out (~2 s) gives NaN outputs and, for every row that has
+ * some, SV_ST_TIMEOUT (the latter not where it is the prefix's).
  *   out_status  int32 [rows] or NULL
  */
 size_t sv_window_attention_workspace_bytes(int32_t dtype, int32_t rows, int32_t tokens, int32_t heads,
@@ -423,6 +423,12 @@ int sv_window_attention(const void* q, int32_t dtype, int32_t rows, int32_t toke
                         int32_t window, int32_t sinks, double scale, float* weights, int64_t weights_stride_row,
                         int64_t weights_stride_head, void* out, void* workspace, size_t workspace_bytes,
                         int32_t* out_status, void* stream);
+
+/* Test hook: in the next launch of the tile kernel (f16 / bf16, more than 16 query rows per
+ * key/value head) by any call of the process, blocks at work on this key/value head hold back
+ * arrivals, so that their waits run out after ~2 ms: what they compute is NaN, with
+ * SV_ST_TIMEOUT. */
+void sv_test_attention_timeout(int32_t head);
 
 /*
  * Attention of rows that share a prefix (the beams of one prompt, a batch behind one
