@@ -61,7 +61,7 @@ struct Shared {
   // full, ready: a stage's copy, and its edge-tile pass.  s_full, pv_done: a query tile's scores of step j and
   // its product of step j (they also free the step's keys and values); one barrier for each of the four steps
   // that the ring holds, so that none gets two phases ahead of who waits for it.
-  uint64_t q_full[2], full[STAGES], ready[STAGES], s_full[2][RING], p_full[2][2], pv_done[2][RING], written[2], drained;
+  uint64_t q_full[2], full[STAGES], ready[STAGES], s_full[2][RING], p_full[2][2], pv_done[2][RING], written[2], drained[2];
   float2 pair[BM];  // PAIRED: the second group's references and sums
   uint32_t tmem;
   uint32_t bad[kEdges][BN / 32];  // per edge tile: its slots with values that are not finite
@@ -271,6 +271,7 @@ __global__ void __launch_bounds__(NT, 1) attn_tile_kernel(const __grid_constant_
     for (int i = 0; i < 2; ++i) {
       mbar_init(&sh.q_full[i], 128);
       mbar_init(&sh.written[i], 128);
+      mbar_init(&sh.drained[i], 1);
       for (int k = 0; k < 2; ++k) mbar_init(&sh.p_full[i][k], 128);
       for (int k = 0; k < RING; ++k) {
         mbar_init(&sh.s_full[i][k], 1);
@@ -281,7 +282,6 @@ __global__ void __launch_bounds__(NT, 1) attn_tile_kernel(const __grid_constant_
       mbar_init(&sh.full[i], 1);
       mbar_init(&sh.ready[i], 1);
     }
-    mbar_init(&sh.drained, 2);
     sh.any_bad = 0;
     sh.limit_ns = a.test_head ? 2000000u : 2000000000u;
     for (int i = 0; i < kEdges; ++i)
@@ -440,8 +440,8 @@ __global__ void __launch_bounds__(NT, 1) attn_tile_kernel(const __grid_constant_
     }
     if (__any_sync(0xffffffffu, sh.abort)) {  // the products in flight
       if (leader) {
-        mma_commit(&sh.drained);
-        mbar_wait(&sh.drained, 0);
+        mma_commit(&sh.drained[t]);
+        mbar_wait(&sh.drained[t], 0);
       }
       __syncwarp();
     }

@@ -32,3 +32,19 @@ def test_a_wait_that_runs_out(sv, shape, head):
     got = sv.window_attention(q, k, v, lengths, status=status)
     assert status.tolist() == [0] * (R - 1) + [sv._lib.ST_LENGTH]
     check(got, want, tol, "the next call")
+
+
+def test_nothing_else_is_waited_for(sv):
+    """A block of one tile: its other product warp has no products to drain and is not waited for."""
+    R, n, H, K, D, C = SHAPES[0]
+    q, k = rand((R, n, H, D), 1, torch.float16), rand((R, K, C, D), 2, torch.float16)
+    sv.window_attention(q, k, k)
+    start, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+    torch.cuda.synchronize()
+    sv._lib.lib().sv_test_attention_timeout(1)
+    start.record()
+    got = sv.window_attention(q, k, k)
+    end.record()
+    end.synchronize()
+    assert torch.isnan(got[:, :, 2:4]).all()
+    assert start.elapsed_time(end) < 500  # ms: waits of 2 ms each, none of the 1 s of a barrier that nobody reaches
