@@ -270,6 +270,12 @@ OptT row_ints(const OptT& t, int64_t rows, const at::Device& dev, const char* na
   return t->reshape({-1}).to(dev, at::kInt).contiguous();
 }
 
+// A status per row, or none.
+int32_t* status_ptr(const OptT& t, int64_t rows, const at::Device& dev) {
+  TORCH_CHECK(!t.has_value() || t->is_contiguous(), "status must be contiguous");
+  return optptr<int32_t>(t, dev, "status", at::kInt, rows);
+}
+
 at::Tensor attention_out(const OptT& out, const at::Tensor& q) {
   if (!out.has_value()) return at::empty(q.sizes(), q.options());
   on_device(*out, q.device(), "out");
@@ -317,7 +323,7 @@ std::tuple<int, at::Tensor> window_attention(const at::Tensor& q_in, const at::T
       w, s, scale.has_value() ? *scale : 1.0 / std::sqrt((double)dim),
       optptr<float>(weights, dev, "weights", at::kFloat), weights.has_value() ? stride_of(*weights, 0) : 0,
       weights.has_value() ? stride_of(*weights, 1) : 0, o.data_ptr(), ws.defined() ? ws.data_ptr() : nullptr,
-      ws.defined() ? (size_t)ws.numel() : 0, optptr<int32_t>(out_status, dev, "status", at::kInt, rows),
+      ws.defined() ? (size_t)ws.numel() : 0, status_ptr(out_status, rows, dev),
       stream.stream());
   return {rc, o};
 }
@@ -365,7 +371,7 @@ std::tuple<int, at::Tensor> prefix_attention(const at::Tensor& q_in, const at::T
       optptr<int32_t>(lengths, dev, "lengths", at::kInt, rows),
       scale.has_value() ? *scale : 1.0 / std::sqrt((double)dim), o.data_ptr(),
       ws.defined() ? ws.data_ptr() : nullptr, ws.defined() ? (size_t)ws.numel() : 0,
-      optptr<int32_t>(out_status, dev, "status", at::kInt, rows), stream.stream());
+      status_ptr(out_status, rows, dev), stream.stream());
   return {rc, o};
 }
 
@@ -411,7 +417,7 @@ std::tuple<int, at::Tensor, at::Tensor, at::Tensor> kv_evict(
       ptr<float>(weights, dev, "weights", at::kFloat, all), ptr<int32_t>(positions, dev, "positions", at::kInt, all),
       optptr<int32_t>(lengths, dev, "lengths", at::kInt, rows), (int32_t)budget, (int32_t)sinks, (int32_t)recent,
       ptr<float>(wo, dev, "weights_out", at::kFloat, all), ptr<int32_t>(po, dev, "positions_out", at::kInt, all),
-      ptr<int32_t>(lo, dev, "lengths_out", at::kInt, rows), optptr<int32_t>(out_status, dev, "status", at::kInt, rows),
+      ptr<int32_t>(lo, dev, "lengths_out", at::kInt, rows), status_ptr(out_status, rows, dev),
       stream_of(keys));
   return {rc, lo, wo, po};
 }

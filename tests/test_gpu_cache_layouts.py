@@ -95,3 +95,18 @@ def test_lengths_updated_in_place(sv, shape, lengths, budget):
         assert torch.equal(got["weights"], want["weights"]) and torch.equal(got["positions"], want["positions"])
     with pytest.raises(RuntimeError):
         sv.kv_evict(k, v, weights, positions, n, budget, status=n)
+
+
+@pytest.mark.parametrize("n", [1, 40])
+def test_statuses_need_a_word_per_row(sv, n):
+    """One word broadcast over the rows, or rows apart from one another."""
+    q, k = rand((3, n, 4, 64), 10, torch.float16), rand((3, 2, 50, 64), 11, torch.float16)
+    weights, positions = torch.zeros((1, 3, 2, 50), device=DEV), torch.zeros((1, 3, 2, 50), dtype=torch.int32, device=DEV)
+    words = torch.full((3, 2), -1, dtype=torch.int32, device=DEV)
+    for status in (words[:1, 0].expand(3), words[:, 0]):
+        for call in (lambda: sv.window_attention(q, k, k, status=status),
+                     lambda: sv.prefix_attention(q, k[0], k[0], k, k, status=status),
+                     lambda: sv.kv_evict(k[None], None, weights, positions, budget=9, status=status)):
+            with pytest.raises(RuntimeError):
+                call()
+    assert (words == -1).all()
