@@ -276,6 +276,20 @@ int32_t* status_ptr(const OptT& t, int64_t rows, const at::Device& dev) {
   return optptr<int32_t>(t, dev, "status", at::kInt, rows);
 }
 
+// The statuses of a call that has no queries or no slots, and launches nothing.
+void fill_status(const OptT& status, const OptT& lengths, const OptT& starts, int64_t rows, int64_t capacity,
+                 const at::Device& dev) {
+  if (status_ptr(status, rows, dev) == nullptr || rows == 0) return;
+  const auto ints = at::TensorOptions().dtype(at::kInt).device(dev);
+  const at::Tensor end = lengths.has_value() ? lengths->reshape({-1}) : at::full({rows}, capacity, ints);
+  at::Tensor bad = end.lt(0).logical_or(end.gt(capacity));
+  if (starts.has_value()) {
+    const at::Tensor start = starts->reshape({-1});
+    bad = bad.logical_or(start.lt(0)).logical_or(start.gt(end.clamp_min(0)));
+  }
+  status->view({-1}).narrow(0, 0, rows).copy_(bad.to(at::kInt).mul(SV_ST_LENGTH));
+}
+
 at::Tensor attention_out(const OptT& out, const at::Tensor& q) {
   if (!out.has_value()) return at::empty(q.sizes(), q.options());
   on_device(*out, q.device(), "out");
@@ -311,8 +325,10 @@ std::tuple<int, at::Tensor> window_attention(const at::Tensor& q_in, const at::T
   const OptT lengths = row_ints(lengths_in, rows, dev, "lengths"), starts = row_ints(starts_in, rows, dev, "starts");
   const int32_t w = (int32_t)std::min<int64_t>(window, 1 << 30), s = (int32_t)std::min<int64_t>(sinks, 1 << 30);
   at::Tensor o = attention_out(out, q_in);
-  if (o.numel() == 0) return {0, o};
-  if (capacity == 0) return {0, o.zero_()};  // no slots: every query sees nothing
+  if (o.numel() == 0 || capacity == 0) {  // no slots: every query sees nothing
+    fill_status(out_status, lengths, starts, rows, capacity, dev);
+    return {0, o.zero_()};
+  }
   const size_t bytes =
       sv_window_attention_workspace_bytes(code, rows, n, heads, kv, dim, capacity, w, s, weights.has_value());
   at::Tensor ws = workspace_for(dev, stream, bytes, 4 * ((size_t)rows * kv + 1024));
@@ -356,11 +372,15 @@ std::tuple<int, at::Tensor> prefix_attention(const at::Tensor& q_in, const at::T
   const int32_t prefix = (int32_t)prefix_length.value_or(pk.size(1));
   const OptT lengths = row_ints(lengths_in, rows, dev, "lengths");
   at::Tensor o = attention_out(out, q_in);
-  if (o.numel() == 0) return {0, o};
-  if (capacity == 0) {  // no own slots: as a cache of one that no row has filled
+  if (o.numel() == 0 || capacity == 0) {
+    fill_status(out_status, lengths, std::nullopt, rows, capacity, dev);
+    if (o.numel() == 0) return {0, o};
+    // No own slots: as a cache of one that no row has filled.
     const at::Tensor none = at::zeros({rows, kv, 1, dim}, q.options());
-    return prefix_attention(q, pk, pv, none, none, at::zeros({rows}, at::TensorOptions().dtype(at::kInt).device(dev)),
-                            prefix, scale, o.view(q.sizes()), out_status);
+    const at::Tensor zero = at::zeros({rows}, at::TensorOptions().dtype(at::kInt).device(dev));
+    const int rc = std::get<0>(
+        prefix_attention(q, pk, pv, none, none, zero, prefix, scale, o.view(q.sizes()), std::nullopt));
+    return {rc, o};
   }
   const size_t bytes = sv_prefix_attention_workspace_bytes(code, rows, n, heads, kv, dim, prefix, capacity);
   at::Tensor ws = workspace_for(dev, stream, bytes, 4 * ((size_t)rows * kv + 1024));
