@@ -133,6 +133,18 @@ int check_pointers(const AttnArgs& a, double scale) {
   if (a.weights && !entries_apart<2>(a.capacity, {a.rows, a.kv_heads}, {a.w_row, a.w_head})) return SV_E_SHAPE;
   // One slot for all positions is no cache (and no dimension of a copy).
   if ((a.capacity > 1 && a.kv_slot == 0) || (a.prefix > 1 && a.p_slot == 0)) return SV_E_SHAPE;
+  // Outputs take their own queries' place after those have been read, which blocks do apart from
+  // one another; other places hold queries still to be read, as all do for the weights' second product.
+  const int64_t sizes[3] = {a.rows, a.n, a.heads}, steps[3] = {a.q_row, a.q_tok, a.q_head};
+  bool same = a.q == a.out && !a.weights;
+  int64_t span = a.dim, packed = a.dim;
+  for (int d = 2; d >= 0; --d) {
+    same = same && (sizes[d] == 1 || steps[d] == packed);
+    packed *= sizes[d];
+    span += (sizes[d] - 1) * steps[d];
+  }
+  const uintptr_t q = reinterpret_cast<uintptr_t>(a.q), out = reinterpret_cast<uintptr_t>(a.out);
+  if (!same && out < q + (uintptr_t)(span * e) && q < out + (uintptr_t)(packed * e)) return SV_E_ARG;
   return SV_OK;
 }
 

@@ -399,7 +399,8 @@ int sv_beam_advance(const int64_t* picks, const float* pick_scores, const int32_
  *   weights  optional float [rows, kv_heads, capacity] at the given strides: each
  *          slot's softmax weight, summed over the head's group and the queries, is
  *          added (sv_kv_evict's input); the rows' and heads' slots must not overlap
- *   out    [rows, tokens, heads, head_dim] contiguous, of dtype
+ *   out    [rows, tokens, heads, head_dim] contiguous, of dtype; without weights it may be
+ *          q itself (contiguous, too), otherwise it does not overlap q (SV_E_ARG)
  *   workspace  sv_window_attention_workspace_bytes(...) bytes, 16-byte aligned, of
  *          which the first SV_ATTENTION_ZERO_BYTES are zero before its first use (each
  *          call leaves them so; a call itself needs 4 * (rows * kv_heads + 1024) of

@@ -2,7 +2,10 @@
 below returns its code before any CUDA call."""
 import pytest
 
-from test_cache_capi import EVICT, WINDOW, call
+from test_cache_capi import EVICT, PREFIX, WINDOW, call
+
+
+WEIGHED = {**WINDOW, "weights": 16, "w_row": 1000, "out": 1 << 20}
 
 
 @pytest.mark.parametrize("kw", [
@@ -12,7 +15,7 @@ from test_cache_capi import EVICT, WINDOW, call
 ])
 def test_accumulated_weights_that_overlap(sv, kw):
     """Rows or heads that would add to the same words."""
-    assert call(sv._lib.lib().sv_window_attention, {**WINDOW, "weights": 16, "w_row": 1000}, kw) == -3
+    assert call(sv._lib.lib().sv_window_attention, WEIGHED, kw) == -3
 
 
 @pytest.mark.parametrize("kw", [
@@ -22,7 +25,7 @@ def test_accumulated_weights_that_overlap(sv, kw):
 ])
 def test_accumulated_weights_that_lie_apart(sv, kw):
     """Past the layout's check: the next thing that is missing is the workspace."""
-    assert call(sv._lib.lib().sv_window_attention, {**WINDOW, "weights": 16, "w_row": 1000}, kw) == -6
+    assert call(sv._lib.lib().sv_window_attention, WEIGHED, kw) == -6
 
 
 @pytest.mark.parametrize("kw", [
@@ -53,3 +56,17 @@ def test_eviction_outputs_over_inputs(sv, out, into):
 @pytest.mark.parametrize("a,b", [("w_out", "p_out"), ("l_out", "w_out"), ("status", "p_out"), ("l_out", "status")])
 def test_eviction_outputs_over_one_another(sv, a, b):
     assert call(sv._lib.lib().sv_kv_evict, APART, {a: APART[b] + 4}) == -1
+
+
+@pytest.mark.parametrize("base,kw,code", [
+    (WINDOW, dict(), -6), (WINDOW, dict(weights=16, w_row=1000), -1), (WINDOW, dict(q_row=4096), -1),
+    (WINDOW, dict(q_row=2048 + 128), -1), (WINDOW, dict(rows=1, q_row=0), -6), (WINDOW, dict(out=32), -1),
+    (WINDOW, dict(out=16 + 2 * 2 * 2048 - 16), -1), (WINDOW, dict(out=16 + 2 * 2 * 2048), -6),
+    (WINDOW, dict(q=16 + 2 * 2 * 2048 - 16), -1), (WINDOW, dict(q=16 + 2 * 2 * 2048), -6),
+    (WINDOW, dict(q=16 + 2 * 2 * 2048, weights=16, w_row=1000), -6), (WINDOW, dict(q_head=0), -1),
+    (PREFIX, dict(), -6), (PREFIX, dict(out=32), -1), (PREFIX, dict(q_tok=16, tokens=2), -1),
+])
+def test_outputs_over_queries(sv, base, kw, code):
+    """The same memory throughout, without weights, passes (to the workspace that is missing)."""
+    fn = "sv_window_attention" if base is WINDOW else "sv_prefix_attention"
+    assert call(getattr(sv._lib.lib(), fn), base, kw) == code

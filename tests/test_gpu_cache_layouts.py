@@ -110,3 +110,22 @@ def test_statuses_need_a_word_per_row(sv, n):
             with pytest.raises(RuntimeError):
                 call()
     assert (words == -1).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
+@pytest.mark.parametrize("n", [1, 40, 300])
+def test_outputs_in_the_queries_place(sv, n, dtype):
+    """out is q: the same result, without weights; with them the queries are needed again."""
+    q, k, v = rand((3, n, 8, 64), 12, dtype), rand((3, 2, 900, 64), 13, dtype), rand((3, 2, 900, 64), 14, dtype)
+    for call in (lambda x, **kw: sv.window_attention(x, k, v, window=400, sinks=3, **kw),
+                 lambda x, **kw: sv.prefix_attention(x, k[0], v[0], k, v, **kw)):
+        want, x = call(q), q.clone()
+        assert call(x, out=x) is x and torch.equal(x, want)
+    w = torch.zeros((3, 2, 900), device=DEV)
+    x = q.clone()
+    with pytest.raises(RuntimeError):
+        sv.window_attention(x, k, v, weights=w, out=x)
+    both = rand((2, 3, n, 8, 64), 15, dtype)
+    with pytest.raises(RuntimeError):
+        sv.window_attention(both.view(6, n, 8, 64)[2:5], k, v, out=both.view(6, n, 8, 64)[3:6])
+    assert torch.equal(x, q) and (w == 0).all()
