@@ -222,6 +222,12 @@ int64_t stride_of(const at::Tensor& t, int64_t d) { return t.size(d) > 1 ? t.str
 // Whether dimension d lies contiguously (a broadcast one, of stride 0, does not).
 bool contiguous_along(const at::Tensor& t, int64_t d) { return t.size(d) <= 1 || t.stride(d) == 1; }
 
+// A size as the C interface takes it.
+int32_t size32(const at::Tensor& t, int64_t d) {
+  TORCH_CHECK_VALUE(t.size(d) <= INT32_MAX, "a dimension of ", t.size(d), " entries is too large");
+  return (int32_t)t.size(d);
+}
+
 bool aligned(const at::Tensor& t, int64_t dims) {
   if (reinterpret_cast<uintptr_t>(t.data_ptr()) % 16) return false;
   const int64_t e = t.element_size();
@@ -309,8 +315,8 @@ std::tuple<int, at::Tensor> window_attention(const at::Tensor& q_in, const at::T
   const at::Device dev = q.device();
   const c10::cuda::CUDAGuard guard(dev);
   const auto stream = at::cuda::getCurrentCUDAStream(dev.index());
-  const int32_t rows = (int32_t)q.size(0), n = (int32_t)q.size(1), heads = (int32_t)q.size(2), dim = (int32_t)q.size(3);
-  const int32_t kv = (int32_t)keys.size(1), capacity = (int32_t)keys.size(2), code = logit_code(q);
+  const int32_t rows = size32(q, 0), n = size32(q, 1), heads = size32(q, 2), dim = size32(q, 3);
+  const int32_t kv = size32(keys, 1), capacity = size32(keys, 2), code = logit_code(q);
   TORCH_CHECK_VALUE(window >= 0 && sinks >= 0, "window and sinks must not be negative");
   TORCH_CHECK_VALUE(!scale.has_value() || std::isfinite(*scale), "scale must be finite");
   OptT weights = weights_in;
@@ -367,9 +373,9 @@ std::tuple<int, at::Tensor> prefix_attention(const at::Tensor& q_in, const at::T
   TORCH_CHECK_VALUE(!scale.has_value() || std::isfinite(*scale), "scale must be finite");
   const c10::cuda::CUDAGuard guard(dev);
   const auto stream = at::cuda::getCurrentCUDAStream(dev.index());
-  const int32_t rows = (int32_t)q.size(0), n = (int32_t)q.size(1), heads = (int32_t)q.size(2), dim = (int32_t)q.size(3);
-  const int32_t kv = (int32_t)keys.size(1), capacity = (int32_t)keys.size(2), code = logit_code(q);
-  const int32_t prefix = (int32_t)prefix_length.value_or(pk.size(1));
+  const int32_t rows = size32(q, 0), n = size32(q, 1), heads = size32(q, 2), dim = size32(q, 3);
+  const int32_t kv = size32(keys, 1), capacity = size32(keys, 2), code = logit_code(q);
+  const int32_t prefix = prefix_length.has_value() ? (int32_t)std::min<int64_t>(*prefix_length, INT32_MAX) : size32(pk, 1);
   const OptT lengths = row_ints(lengths_in, rows, dev, "lengths");
   at::Tensor o = attention_out(out, q_in);
   if (o.numel() == 0 || capacity == 0) {
@@ -414,8 +420,8 @@ std::tuple<int, at::Tensor, at::Tensor, at::Tensor> kv_evict(
   TORCH_CHECK_VALUE(weights.scalar_type() == at::kFloat && positions.scalar_type() == at::kInt &&
                         weights.sizes() == keys.sizes().slice(0, last) && positions.sizes() == weights.sizes(),
                     "weights (float32) and positions (int32) must have the keys' shape without head_dim");
-  const int64_t layers = keys.size(0), rows = keys.size(1), heads = heads_dim ? keys.size(2) : 1;
-  const int64_t capacity = keys.size(last - 1), all = layers * rows * heads * capacity;
+  const int64_t layers = size32(keys, 0), rows = size32(keys, 1), heads = heads_dim ? size32(keys, 2) : 1;
+  const int64_t capacity = size32(keys, last - 1), all = layers * rows * heads * capacity;
   TORCH_CHECK_VALUE(budget >= 1 && budget <= capacity, "budget must be in [1, capacity]");
   TORCH_CHECK_VALUE(sinks >= 0 && recent >= 0 && sinks + recent <= budget,
                     "sinks and recent must not be negative and must fit in the budget");
@@ -432,7 +438,7 @@ std::tuple<int, at::Tensor, at::Tensor, at::Tensor> kv_evict(
               "weights and positions must be contiguous");
   const int rc = sv_kv_evict(
       keys.data_ptr(), raw(values, dev, "values"), (int32_t)keys.element_size(), (int32_t)layers, (int32_t)rows,
-      (int32_t)heads, (int32_t)capacity, (int32_t)keys.size(last), stride_of(keys, 0), stride_of(keys, 1),
+      (int32_t)heads, (int32_t)capacity, size32(keys, last), stride_of(keys, 0), stride_of(keys, 1),
       heads_dim ? stride_of(keys, 2) : 0, stride_of(keys, last - 1),
       ptr<float>(weights, dev, "weights", at::kFloat, all), ptr<int32_t>(positions, dev, "positions", at::kInt, all),
       optptr<int32_t>(lengths, dev, "lengths", at::kInt, rows), (int32_t)budget, (int32_t)sinks, (int32_t)recent,

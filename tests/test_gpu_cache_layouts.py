@@ -129,3 +129,18 @@ def test_outputs_in_the_queries_place(sv, n, dtype):
     with pytest.raises(RuntimeError):
         sv.window_attention(both.view(6, n, 8, 64)[2:5], k, v, out=both.view(6, n, 8, 64)[3:6])
     assert torch.equal(x, q) and (w == 0).all()
+
+
+def test_sizes_past_31_bits(sv):
+    """Sizes whose low 32 bits alone would be taken for a small cache."""
+    q, k = rand((1, 1, 2, 64), 16, torch.float16), rand((1, 1, 1, 64), 17, torch.float16)
+    many = 2 ** 32 + 1
+    wide = k.expand(1, 1, many, 64)
+    for call in (lambda: sv.window_attention(q, wide, wide), lambda: sv.prefix_attention(q, wide[0], wide[0], k, k),
+                 lambda: sv.prefix_attention(q, k[0], k[0], wide, wide),
+                 lambda: sv.kv_evict(wide[None], None, torch.zeros((), device=DEV).expand(1, 1, 1, many),
+                                     torch.zeros((), dtype=torch.int32, device=DEV).expand(1, 1, 1, many), budget=1)):
+        with pytest.raises(ValueError):
+            call()
+    assert torch.equal(sv.prefix_attention(q, wide[0], wide[0], k, k, prefix_length=1),
+                       sv.prefix_attention(q, k[0], k[0], k, k))
