@@ -219,6 +219,14 @@ at::Tensor workspace_for(const at::Device& dev, c10::cuda::CUDAStream stream, si
 // Strides of a dimension of one entry mean nothing: 0 stands for them.
 int64_t stride_of(const at::Tensor& t, int64_t d) { return t.size(d) > 1 ? t.stride(d) : 0; }
 
+// Whether b is laid out as a.
+bool same_layout(const at::Tensor& a, const at::Tensor& b) {
+  if (a.sizes() != b.sizes()) return false;
+  for (int64_t d = 0; d < a.dim(); ++d)
+    if (stride_of(a, d) != stride_of(b, d)) return false;
+  return true;
+}
+
 // Whether dimension d lies contiguously (a broadcast one, of stride 0, does not).
 bool contiguous_along(const at::Tensor& t, int64_t d) { return t.size(d) <= 1 || t.stride(d) == 1; }
 
@@ -256,7 +264,7 @@ void check_cache(const at::Tensor& k, const at::Tensor& v, const at::Tensor& q) 
   const at::Device dev = q.device();
   on_device(k, dev, "keys");
   on_device(v, dev, "values");
-  TORCH_CHECK_VALUE(k.dim() == 4 && v.sizes() == k.sizes() && v.strides() == k.strides(),
+  TORCH_CHECK_VALUE(k.dim() == 4 && same_layout(k, v),
                     "keys must be [rows, capacity, head_dim] or [rows, kv_heads, capacity, head_dim], and values "
                     "have their shape and strides");
   TORCH_CHECK_VALUE(k.scalar_type() == q.scalar_type() && v.scalar_type() == q.scalar_type(),
@@ -363,7 +371,7 @@ std::tuple<int, at::Tensor> prefix_attention(const at::Tensor& q_in, const at::T
   const at::Device dev = q.device();
   on_device(pk, dev, "prefix_keys");
   on_device(pv, dev, "prefix_values");
-  TORCH_CHECK_VALUE(pk.dim() == 3 && pv.sizes() == pk.sizes() && pv.strides() == pk.strides() &&
+  TORCH_CHECK_VALUE(pk.dim() == 3 && same_layout(pk, pv) &&
                         pk.scalar_type() == q.scalar_type() && pv.scalar_type() == q.scalar_type() &&
                         pk.size(0) == keys.size(1) && pk.size(2) == q.size(3) && contiguous_along(pk, 2),
                     "prefix_keys and prefix_values must be [kv_heads, prefix, head_dim] of q's dtype with the same "
@@ -414,8 +422,7 @@ std::tuple<int, at::Tensor, at::Tensor, at::Tensor> kv_evict(
   const int64_t last = keys.dim() - 1;
   const bool heads_dim = keys.dim() == 5;
   TORCH_CHECK_VALUE(contiguous_along(keys, last), "head_dim must be contiguous");
-  TORCH_CHECK_VALUE(!values.has_value() || (values->sizes() == keys.sizes() && values->strides() == keys.strides() &&
-                                            values->scalar_type() == keys.scalar_type()),
+  TORCH_CHECK_VALUE(!values.has_value() || (same_layout(keys, *values) && values->scalar_type() == keys.scalar_type()),
                     "values must have the keys' shape, strides and dtype");
   TORCH_CHECK_VALUE(weights.scalar_type() == at::kFloat && positions.scalar_type() == at::kInt &&
                         weights.sizes() == keys.sizes().slice(0, last) && positions.sizes() == weights.sizes(),

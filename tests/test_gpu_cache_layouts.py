@@ -144,3 +144,22 @@ def test_sizes_past_31_bits(sv):
             call()
     assert torch.equal(sv.prefix_attention(q, wide[0], wide[0], k, k, prefix_length=1),
                        sv.prefix_attention(q, k[0], k[0], k, k))
+
+
+def test_strides_of_single_entries_mean_nothing(sv):
+    """Keys and values of one row and head, cut from caches of different capacities."""
+    q, big, small = rand((1, 1, 4, 64), 18, torch.float16), rand((1, 1, 90, 64), 19, torch.float16), \
+        rand((1, 1, 70, 64), 20, torch.float16)
+    k, v = big[:, :, :60], small[:, :, :60]
+    want = sv.window_attention(q, k.contiguous(), v.contiguous())
+    assert torch.equal(sv.window_attention(q, k, v), want)
+    assert torch.equal(sv.prefix_attention(q, k[0], v[0], k, v),
+                       sv.prefix_attention(q, k[0].contiguous(), v[0].contiguous(), k, v.contiguous().clone()))
+    weights = torch.rand((1, 1, 1, 60), generator=torch.Generator(device=DEV).manual_seed(1), device=DEV)
+    positions = torch.arange(60, dtype=torch.int32, device=DEV).view(1, 1, 1, 60)
+    a, b = k.contiguous()[None], v.contiguous()[None]
+    sv.kv_evict(a, b, weights, positions, budget=20)
+    sv.kv_evict(k[None], v[None], weights, positions, budget=20)
+    assert torch.equal(k[None], a) and torch.equal(v[None], b)
+    with pytest.raises(ValueError):  # where there are two heads the strides count
+        sv.window_attention(q, big.expand(1, 2, -1, -1)[:, :, :60], small.repeat(1, 2, 1, 1)[:, :, :60])
