@@ -299,7 +299,7 @@ __global__ void __launch_bounds__(NT, 1) attn_tile_kernel(const __grid_constant_
 
   // Steps are numbered through all the block's items: J = base + j.  Step J's keys and
   // values are in stages 2 J and 2 J + 1 (mod STAGES).  A query tile's scores alternate
-  // between its two buffers by its own count P of steps (items may lack the second tile).
+  // between its two buffers (PAIRED: by its own count P of steps, every other one).
   if (warp == 8) {
     // ------------------------------------------------------------- copies
     if (lane == 0) {
@@ -353,7 +353,7 @@ __global__ void __launch_bounds__(NT, 1) attn_tile_kernel(const __grid_constant_
                kd + (((k >> 2) * L::kHalf + (k & 3) * 32) >> 4), wqk, k != 0);
       mma_commit(&sh.s_full[t][J % RING]);
     };
-    int base_ = 0, mine_ = 0, queries = 0;
+    int base_ = 0, queries = 0;
     if (PAIRED) {
       const int steps = __reduce_max_sync(0xffffffffu, it.nt);
       if (leader && t < steps) {
@@ -390,13 +390,14 @@ __global__ void __launch_bounds__(NT, 1) attn_tile_kernel(const __grid_constant_
     for (int w = blockIdx.x; !PAIRED && w < items && t < tiles_m; w += gridDim.x) {
       if (w != (int)blockIdx.x) it = item_at(w);
       const int steps = __reduce_max_sync(0xffffffffu, it.nt);
-      const int base = __reduce_max_sync(0xffffffffu, base_), mine = __reduce_max_sync(0xffffffffu, mine_);
-      if (t >= it.mt) {  // no rows: the stages are passed on as they come
+      const int base = __reduce_max_sync(0xffffffffu, base_);
+      if (t >= it.mt) {  // no rows: the stages are passed on as they come, through the softmax group
         if (leader)
           for (int J = base; J < base + steps; ++J) {
             wait_one(sh, &sh.full[(2 * J) % STAGES], (2 * J / STAGES) & 1);
             mma_commit(&sh.s_full[t][J % RING]);
             wait_one(sh, &sh.ready[(2 * J + 1) % STAGES], ((2 * J + 1) / STAGES) & 1);
+            wait_one(sh, &sh.p_full[t][J & 1], (J >> 1) & 1);
             mma_commit(&sh.pv_done[t][J % RING]);
           }
         __syncwarp();
@@ -407,35 +408,34 @@ __global__ void __launch_bounds__(NT, 1) attn_tile_kernel(const __grid_constant_
         wait_one(sh, &sh.q_full[t], queries & 1);
         for (int j = 0; j < min(steps, 2); ++j) {
           wait_one(sh, &sh.full[(2 * (base + j)) % STAGES], (2 * (base + j) / STAGES) & 1);
-          qk(base + j, mine + j);
+          qk(base + j, base + j);
         }
       }
       queries += steps > 0;
       __syncwarp();
 #pragma unroll 1
       for (int j = 0; j < steps; ++j) {
-        const int J = base + j, P = mine + j, vi = 2 * J + 1, ki = 2 * J + 4;
+        const int J = base + j, vi = 2 * J + 1, ki = 2 * J + 4;
         int j0, jend;
         tile_at(it, j, j0, jend);
         const int blocks = value_blocks(j0, jend);
         if (leader) {
           wait_one(sh, &sh.ready[vi % STAGES], (vi / STAGES) & 1);
-          wait_one(sh, &sh.p_full[t][P & 1], (P >> 1) & 1);
+          wait_one(sh, &sh.p_full[t][J & 1], (J >> 1) & 1);
           tcgen05_after_sync();
           const uint64_t vd = v_desc + (vi % STAGES) * kStep;
 #pragma unroll
           for (int k = 0; k < BN / 16; ++k)
-            if (k < blocks) mma_ts(o_at, s_at + (P & 1) * BN + k * 8, vd + k * (2048 >> 4), wpv, j != 0 || k != 0);
+            if (k < blocks) mma_ts(o_at, s_at + (J & 1) * BN + k * 8, vd + k * (2048 >> 4), wpv, j != 0 || k != 0);
           mma_commit(&sh.pv_done[t][J % RING]);
           if (j + 2 < steps) {
             wait_one(sh, &sh.full[ki % STAGES], (ki / STAGES) & 1);
-            qk(J + 2, P + 2);
+            qk(J + 2, J + 2);
           }
         }
         __syncwarp();
       }
       base_ += steps;
-      mine_ += steps;
       if (__any_sync(0xffffffffu, sh.abort)) break;
     }
     if (__any_sync(0xffffffffu, sh.abort)) {  // the products in flight
@@ -550,7 +550,7 @@ __global__ void __launch_bounds__(NT, 1) attn_tile_kernel(const __grid_constant_
     // After an abort the groups go through their steps all the same (on scores that nobody
     // uses), so that neither waits for a turn that does not come.
     if (t == 1 && (PAIRED || tiles_m == 2)) turn_pass(1);
-    int base = 0, mine = 0;
+    int base = 0;
     for (int w = blockIdx.x; w < items; w += gridDim.x) {
       if (w != (int)blockIdx.x) {
         it = item_at(w);
@@ -569,7 +569,7 @@ __global__ void __launch_bounds__(NT, 1) attn_tile_kernel(const __grid_constant_
         const Whole whole = whole_steps(it, mfirst, mlast);
         const int rounds = PAIRED ? (it.nt + 1) >> 1 : it.nt;
         for (int own = 0; own < rounds; ++own) {
-          const int j = PAIRED ? 2 * own + t : own, J = base + j, P = mine + own;
+          const int j = PAIRED ? 2 * own + t : own, J = base + j, P = PAIRED ? own : J;
           if (PAIRED && j >= it.nt) {  // an odd step out: the other group's
             turn_wait(t);
             turn_pass(t);
@@ -649,9 +649,16 @@ __global__ void __launch_bounds__(NT, 1) attn_tile_kernel(const __grid_constant_
           tcgen05_before_sync();
           mbar_arrive(&sh.p_full[t][P & 1]);
         }
+      } else if (!PAIRED && t < tiles_m) {
+        // No rows: step by step all the same.  A group that went ahead to its next item could
+        // take an older phase of that item's barriers for the one it waits for.
+        for (int j = 0; j < it.nt; ++j) {
+          const int J = base + j;
+          wait(sh, &sh.s_full[t][J % RING], (J / RING) & 1);
+          mbar_arrive(&sh.p_full[t][J & 1]);
+        }
       }
       base += it.nt;
-      if (t < it.mt) mine += it.nt;
       const int last = PAIRED ? ((it.nt - 1 - t) & ~1) + t : base - 1;  // this group's last step
       float f0 = 1.f, f1 = 0.f;                                         // PAIRED: the two outputs' factors
       bool second = false;

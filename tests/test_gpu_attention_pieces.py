@@ -21,6 +21,11 @@ CASES = {
     "rowless second tiles, window": (300, 13, 8, 2, 128, 200, 40, 3, "ragged", None),
     # 100 pieces of 44 rows, then 100 of 256.
     "last tile of a unit alone": (100, 150, 2, 1, 64, 160, 0, 0, "ragged", None),
+    # The same with many steps: a block's first piece has no second tile, its next one has.
+    "last tile of a unit alone, long": (100, 150, 2, 1, 64, 1500, 0, 0, "full", None),
+    "last tile of a unit alone, long, ragged": (120, 130, 2, 1, 128, 1000, 0, 0, "ragged", None),
+    "last tile of a unit alone, window": (60, 288, 3, 1, 128, 1479, 448, 1, "ragged", None),
+    "last tile of a unit alone, wide group": (18, 322, 16, 1, 40, 745, 0, 0, "ragged", "padded"),
     # Four in five rows are empty: blocks have empty pieces one after the other, before and after others.
     "empty rows": (900, 20, 2, 1, 64, 100, 0, 0, "holes", None),
     "empty rows, two tiles": (600, 130, 2, 1, 64, 140, 30, 2, "holes", None),
@@ -103,6 +108,8 @@ def test_pieces(sv, name, dtype):
 PREFIX = {
     "two tiles": (100, 12, 16, 1, 64, 300, 40),        # 150 tiles of prefix queries, own pieces with rowless tiles
     "two tiles, more than one piece": (200, 24, 8, 1, 128, 200, 30),
+    "last tile alone": (26, 131, 10, 5, 40, 14, 572),  # of every unit of the own part, with many steps
+    "last tile of the prefix alone": (15, 203, 100, 5, 72, 1000, 80),
     "halves": (64, 9, 16, 1, 128, 3300, 20),            # two splits of 1650 slots
     "halves, one split": (40, 40, 8, 1, 64, 1601, 50),  # 100 tiles
 }
