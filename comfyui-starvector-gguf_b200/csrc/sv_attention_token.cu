@@ -751,7 +751,7 @@ __global__ void __launch_bounds__(NT) attn_weights16_kernel(const __grid_constan
     for (int e = 0; e < 2; ++e) {
       const int m = m0 + 2 * t + e;
       l[e] = m < m_end ? lse[m] : INFINITY;
-      pos[e] = first_pos + m / a.group;
+      pos[e] = m < m_end ? first_pos + m / a.group : -1;  // past the end: sees nothing (its product may be 0 * inf)
       low[e] = window_low(a, sp.start, pos[e]);
 #pragma unroll
       for (int k = 0; k < 4; ++k) c[e][k] = 0.f;
