@@ -729,14 +729,17 @@ __global__ void __launch_bounds__(NT) attn_weights16_kernel(const __grid_constan
   const int first_pos = sp.end - a.n;
   int m_first, m_end;
   weight_rows(a, sp, j0, 16, blockIdx.z, m_first, m_end);
+  // Past the last row that row again, with a sum of infinity: its exponentials are zero, and NaN only
+  // where the row's own is (of a zero query and an infinite key they would be anyway).
+  const int m_last = max(m_end - 1, 0);
   auto load_q = [&](int m0) {
-    const int m = m0 + g, i = m / a.group;
+    const int m = min(m0 + g, m_last), i = m / a.group;
     const T* src = static_cast<const T*>(a.q) + r * a.q_row + i * a.q_tok +
                    (int64_t)(h * a.group + m - i * a.group) * a.q_head;
 #pragma unroll
     for (int u = 0; u < 2 * DC; ++u)
-      qn[u] = m < nG && (FULL || 4 * u + t < vecs) ? __ldg(reinterpret_cast<const uint4*>(src) + 4 * u + t)
-                                                   : make_uint4(0u, 0u, 0u, 0u);
+      qn[u] = FULL || 4 * u + t < vecs ? __ldg(reinterpret_cast<const uint4*>(src) + 4 * u + t)
+                                       : make_uint4(0u, 0u, 0u, 0u);
   };
   float sum[2] = {0.f, 0.f};
   const float* lse = a.lse + (int64_t)unit * nG;
@@ -751,7 +754,7 @@ __global__ void __launch_bounds__(NT) attn_weights16_kernel(const __grid_constan
     for (int e = 0; e < 2; ++e) {
       const int m = m0 + 2 * t + e;
       l[e] = m < m_end ? lse[m] : INFINITY;
-      pos[e] = m < m_end ? first_pos + m / a.group : -1;  // past the end: sees nothing (its product may be 0 * inf)
+      pos[e] = first_pos + min(m, m_last) / a.group;
       low[e] = window_low(a, sp.start, pos[e]);
 #pragma unroll
       for (int k = 0; k < 4; ++k) c[e][k] = 0.f;
