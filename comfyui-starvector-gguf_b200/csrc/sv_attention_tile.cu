@@ -683,7 +683,8 @@ __global__ void __launch_bounds__(NT, 1) attn_tile_kernel(const __grid_constant_
       }
       if (t < it.mt) {
         ok = __all_sync(0xffffffffu, ok && !sh.abort);
-        const bool any_bad = it.nt > 0 && *static_cast<volatile int*>(&sh.any_bad) != 0;
+        // (Rows of an item without steps may meet another item's notes, and see none of their slots.)
+        const bool any_bad = *static_cast<volatile int*>(&sh.any_bad) != 0;
         const float inv = !ok ? __int_as_float(0x7fc00000) : (l == 0.f ? 0.f : (direct ? 1.f / l : 1.f));
 #pragma unroll 1
         for (int c = 0; c < 64 * DC; c += 32) {
