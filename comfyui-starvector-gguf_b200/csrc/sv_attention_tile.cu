@@ -626,7 +626,7 @@ __global__ void __launch_bounds__(NT, 1) attn_tile_kernel(const __grid_constant_
           for (int k = 0; k < BN / 2; ++k) z[k] = fma2(pack2(s[2 * k], s[2 * k + 1]), scale2, at2);
           // The special function unit takes 8 cycles for a warp's 32 exponentials, which is what
           // bounds a step: the two groups take turns at it, so that one is always busy with
-          // its other work (445 us for the 8192-token prompt, 470 us without turns).  Moving
+          // its other work (when they came in, 445 us for the 8192-token prompt with and 470 us without them).  Moving
           // exponentials to the FP32 pipes by a polynomial (one pair in eight, or in four) took
           // 2 to 4 % longer: those pipes do the scaling and the sums already.
           uint32_t p[32];

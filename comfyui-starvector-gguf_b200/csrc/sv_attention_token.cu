@@ -1,6 +1,6 @@
 // sv_attention_token.cu -- attention of few query rows per key/value head over the
-// cache (single tokens, short drafts): at most 16 rows (query, head of the group),
-// float16 / bfloat16, one pass over the slots at memory speed.
+// cache: at most 16 rows (query, head of the group), so single tokens, and drafts of a few
+// where the groups are small; float16 / bfloat16, one pass over the slots at memory speed.
 //
 // Mathematics.  Row m of a unit (cache row r, key/value head h): s_j = (q_m . k_j) *
 // scale * log2 e, o = sum_j 2^(s_j - ref) v_j, l = sum_j 2^(s_j - ref), joined over

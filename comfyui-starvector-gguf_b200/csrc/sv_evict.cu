@@ -545,7 +545,7 @@ extern "C" int sv_kv_evict(void* keys, void* values, int32_t elem_bytes, int32_t
   a.lanes_log2 = 0;
   while (a.lanes_log2 < 5 && (1 << a.lanes_log2) < (values ? 2 : 1) * a.dv) ++a.lanes_log2;
   // Many units: blocks of 256 threads, up to seven per SM (three to seven take the same time: 44.6-45.5 us
-  // at 1024 units of about 2200 slots).  Few: one block of 1024 threads per SM in all, since each selects
+  // at 1024 units of about 2200 slots; at seven, 32 registers, a few words spill).  Few: one block of 1024 threads per SM in all, since each selects
   // anew (48 units of up to 8192 slots: 26 us, and 41 us with two rounds of such blocks).
   const bool many = units >= 296;
   a.parts = many || units > 148 ? 1 : 148 / units;

@@ -578,8 +578,9 @@ def window_attention(q, keys, values, lengths=None, *, starts=None, window=0, si
     j > p - window or j < start + sinks; a query that sees nothing gives zeros.
     `scale` defaults to head_dim ** -0.5.  `weights` (float32 [rows, kv_heads,
     capacity], or [rows, capacity]) has each slot's softmax weight added, summed over
-    the head group and the queries: kv_evict's input.  status: int32 [rows], filled
-    with 0 or SV_ST_LENGTH.  Returns the output, q's shape and dtype."""
+    the head group and the queries: kv_evict's input; its rows and heads must not be
+    broadcast.  `out` may be q itself, without weights.  status: int32 [rows], filled
+    with 0, SV_ST_LENGTH or SV_ST_TIMEOUT.  Returns the output, q's shape and dtype."""
     if isinstance(lengths, int):
         (keys, values), lengths = _first_slots(keys, values, lengths), None
     rc, o = _ext().window_attention(q, keys, values, lengths, starts, window, sinks, scale, weights, out, status)

@@ -405,7 +405,8 @@ int sv_beam_advance(const int64_t* picks, const float* pick_scores, const int32_
  *          which the first SV_ATTENTION_ZERO_BYTES are zero before its first use (each
  *          call leaves them so; a call itself needs 4 * (rows * kv_heads + 1024) of
  *          them); calls that overlap on the GPU need different ones
- * Scores, softmax and sums are f32; the 16-bit kernels round the weights to the
+ * Scores, softmax and sums are f32 (before the division sums of weights of up to 2^8:
+ * |values| times slots up to 2^119); the 16-bit kernels round the weights to the
  * inputs' type before they multiply the values.  head_dim a multiple of 8, 8..128;
  * heads a multiple of kv_heads; rows * kv_heads <= 65535; rows * tokens * heads <=
  * 2^30; capacity (and prefix_length) <= 2^29, with a slot stride other than 0 (rows and
