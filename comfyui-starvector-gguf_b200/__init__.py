@@ -14,10 +14,11 @@ load it by path, e.g. through __graft_entry__.load_package(), which registers it
 `starvector_b200`.
 """
 from . import _lib, sharded
-from .ops import (beam_advance, beam_step, beam_workspace, kv_evict, kv_reorder, loop_guard, merge_beam_shards,
-                  merge_shards, penalize, prefix_attention, sample_step, seen_bitmap, seen_reorder, seen_update,
-                  window_attention)
+from .ops import (beam_advance, beam_step, beam_workspace, kv_dequantize, kv_evict, kv_quantize, kv_record_bytes,
+                  kv_reorder, loop_guard, merge_beam_shards, merge_shards, penalize, prefix_attention,
+                  quantized_attention, sample_step, seen_bitmap, seen_reorder, seen_update, window_attention)
 
-__all__ = ["sample_step", "beam_step", "beam_workspace", "beam_advance", "kv_evict", "kv_reorder", "loop_guard",
-           "merge_beam_shards", "merge_shards", "penalize", "prefix_attention", "seen_bitmap", "seen_reorder",
-           "seen_update", "sharded", "window_attention"]
+__all__ = ["sample_step", "beam_step", "beam_workspace", "beam_advance", "kv_dequantize", "kv_evict", "kv_quantize",
+           "kv_record_bytes", "kv_reorder", "loop_guard", "merge_beam_shards", "merge_shards", "penalize",
+           "prefix_attention", "quantized_attention", "seen_bitmap", "seen_reorder", "seen_update", "sharded",
+           "window_attention"]

@@ -55,6 +55,13 @@ _SIGNATURES = {
                                    _P, _P, _I32, _I64, _I64, _I64, _P, _D, _P, _P, _SZ, _P, _P]),
     "sv_kv_evict": (_I32, [_P, _P, _I32, _I32, _I32, _I32, _I32, _I32, _I64, _I64, _I64, _I64, _P, _P, _P, _I32, _I32,
                            _I32, _P, _P, _P, _P, _P]),
+    "sv_kv_record_bytes": (_I32, [_I32]),
+    "sv_kv_quantize": (_I32, [_P, _P, _I32, _I32, _I32, _I32, _I32, _I64, _I64, _I64, _P, _P, _I32, _I64, _I64, _I64, _P,
+                              _P, _P]),
+    "sv_kv_dequantize": (_I32, [_P, _P, _I32, _I32, _I32, _I32, _I64, _I64, _I64, _P, _I32, _P, _P, _I32, _P, _P]),
+    "sv_quantized_attention_workspace_bytes": (_SZ, [_I32] * 10),
+    "sv_quantized_attention": (_I32, [_P, _I32, _I32, _I32, _I32, _I32, _I32, _I64, _I64, _I64, _P, _P, _I32, _I64,
+                                      _I64, _I64, _P, _P, _I32, _I32, _D, _P, _I64, _I64, _P, _P, _SZ, _P, _P]),
     "sv_test_attention_timeout": (None, [_I32]),
     "sv_error_string": (C.c_char_p, [_I32]),
     "sv_abi_version": (_I32, []),

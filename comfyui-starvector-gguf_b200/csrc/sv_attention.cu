@@ -4,6 +4,7 @@
 
 #include "../../include/starvector_sampling.h"
 #include "sv_attention.h"
+#include "sv_record.cuh"
 
 namespace sv {
 namespace {
@@ -199,6 +200,11 @@ void set_window(AttnArgs& a, int32_t window, int32_t sinks) {
   a.sinks = sinks < 0 || (limit && window > 0) ? sinks : 0;
 }
 
+// The plain keys and values of a whole cache.
+size_t read_bytes(const AttnArgs& a) {
+  return 2 * up256((size_t)a.rows * a.kv_heads * a.capacity * a.dim * (a.dtype == SV_F32 ? 4 : 2));
+}
+
 AttnArgs base_args(int32_t dtype, int32_t rows, int32_t tokens, int32_t heads, int32_t kv_heads, int32_t head_dim,
                    int32_t capacity) {
   AttnArgs a = {};
@@ -260,6 +266,77 @@ int sv_window_attention(const void* q, int32_t dtype, int32_t rows, int32_t toke
   int rc = check_shapes(a);
   if (!rc) rc = check_pointers(a, scale);
   return rc ? rc : run(a, workspace, workspace_bytes, static_cast<cudaStream_t>(stream));
+}
+
+size_t sv_quantized_attention_workspace_bytes(int32_t dtype, int32_t rows, int32_t tokens, int32_t heads,
+                                              int32_t kv_heads, int32_t head_dim, int32_t capacity, int32_t window,
+                                              int32_t sinks, int32_t with_weights) {
+  AttnArgs a = base_args(dtype, rows, tokens, heads, kv_heads, head_dim, capacity);
+  set_window(a, window, sinks);
+  if (check_shapes(a)) return 0;
+  float dummy;
+  a.weights = with_weights ? &dummy : nullptr;
+  return make_plan(a).total() + read_bytes(a);
+}
+
+int sv_quantized_attention(const void* q, int32_t dtype, int32_t rows, int32_t tokens, int32_t heads, int32_t kv_heads,
+                           int32_t head_dim, int64_t q_stride_row, int64_t q_stride_token, int64_t q_stride_head,
+                           const void* cache_keys, const void* cache_values, int32_t capacity, int64_t cache_stride_row,
+                           int64_t cache_stride_head, int64_t cache_stride_slot, const int32_t* lengths,
+                           const int32_t* starts, int32_t window, int32_t sinks, double scale, float* weights,
+                           int64_t weights_stride_row, int64_t weights_stride_head, void* out, void* workspace,
+                           size_t workspace_bytes, int32_t* out_status, void* stream) {
+  AttnArgs a = base_args(dtype, rows, tokens, heads, kv_heads, head_dim, capacity);
+  a.q = q;
+  a.q_row = q_stride_row;
+  a.q_tok = q_stride_token;
+  a.q_head = q_stride_head;
+  a.k = cache_keys;
+  a.v = cache_values;
+  a.lengths = lengths;
+  a.starts = starts;
+  set_window(a, window, sinks);
+  a.scale = (float)(scale * 1.4426950408889634);
+  a.weights = weights;
+  a.w_row = weights_stride_row;
+  a.w_head = weights_stride_head;
+  a.out = out;
+  a.status = out_status;
+  int rc = check_shapes(a);
+  if (rc) return rc;
+  if (cache_stride_row < 0 || cache_stride_head < 0 || cache_stride_slot < 0 || (capacity > 1 && cache_stride_slot == 0))
+    return SV_E_SHAPE;
+  if (cache_stride_row % 16 || cache_stride_head % 16 || cache_stride_slot % 16) return SV_E_ALIGN;
+  // The values that the records stand for, of the slots that some query sees.
+  a.kv_slot = head_dim;
+  a.kv_head = (int64_t)capacity * head_dim;
+  a.kv_row = kv_heads * a.kv_head;
+  rc = check_pointers(a, scale);
+  if (rc) return rc;
+  const size_t before = make_plan(a).total(), bytes = read_bytes(a);
+  if (!workspace || workspace_bytes < before + bytes) return SV_E_WORKSPACE;
+  unsigned char* values = static_cast<unsigned char*>(workspace) + before;
+  ReadArgs x = {};
+  x.cache[0] = static_cast<const unsigned char*>(cache_keys);
+  x.cache[1] = static_cast<const unsigned char*>(cache_values);
+  x.row = cache_stride_row;
+  x.head = cache_stride_head;
+  x.slot = cache_stride_slot;
+  a.k = x.out[0] = values;
+  a.v = x.out[1] = values + bytes / 2;
+  x.lengths = lengths;
+  x.starts = starts;
+  x.dtype = dtype;
+  x.rows = rows;
+  x.kv_heads = kv_heads;
+  x.dim = head_dim;
+  x.capacity = x.tokens = capacity;
+  x.seen = tokens;
+  x.window = a.window;
+  x.sinks = a.sinks;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (launch_read_records(x, s) != cudaSuccess) return SV_E_CUDA;
+  return run(a, workspace, before, s);
 }
 
 size_t sv_prefix_attention_workspace_bytes(int32_t dtype, int32_t rows, int32_t tokens, int32_t heads,

@@ -1,0 +1,368 @@
+// sv_record.cu -- the cache held in 4 bits (sv_record.cuh): writing and reading records.
+//
+// A group of threads takes one slot of one head: thread (i, y) of it block i's dimensions
+// 8 y .. 8 y + 7 and 16 + 8 y .. 16 + 8 y + 7, which are the words t = 2 y and 2 y + 1 of the
+// block.  Both kernels move each byte once; a warp's loads and stores cover whole
+// sectors.
+//
+// Writing.  Of a group's finite values x, clamped to +-32768, with extremes lo, hi:
+//   scale = f16((hi - lo) / 15),  mid = f16(lo + 8 scale),
+//   c = 8 + the whole number next to (x - mid) / scale (ties to the even one), within 0..15,
+// each rounded once from the exact number.  In f32 that is the same except next to a
+// border between two results, where it is decided in 64 bits, so that the codes do not
+// depend on how a quotient rounds.  A group with a NaN or an infinity stands for NaN.
+#include "../../include/starvector_sampling.h"
+#include "sv_attention.h"
+#include "sv_record.cuh"
+
+namespace sv {
+namespace {
+
+constexpr int NT = 256;
+
+struct WriteArgs {
+  const void* in[2];
+  int64_t i_row, i_head, i_tok;  // strides in elements
+  unsigned char* cache[2];
+  int64_t row, head, slot;  // strides in bytes
+  const int32_t* lengths;
+  int32_t* status;
+  int32_t rows, kv_heads, dim, capacity, tokens;
+};
+
+__device__ __forceinline__ float min_nan(float a, float b) {
+  float r;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
+// x + e rounded to float16, where e in +-|x| 2^-21 is not known in f32: false where it decides.
+__device__ __forceinline__ bool half_sure(float x, __half& h) {
+  h = __float2half_rn(x);
+  const __half below = __float2half_rn(fmaf(x, -0x1p-21f, x)), above = __float2half_rn(fmaf(x, 0x1p-21f, x));
+  return __half_as_ushort(below) == __half_as_ushort(above);
+}
+
+// The code next to q, which was computed as (x - mid) / scale to within 2^-17.
+__device__ __noinline__ float code_exactly(float x, float mid, float scale, float q) {
+  const float k = floorf(q);
+  const double border = (double)mid + ((double)k + 0.5) * (double)scale;  // exact: 11 bits and 16, 30 binades
+  const double v = x;
+  if (v > border) return k + 1.f;
+  if (v < border) return k;
+  return (int)k & 1 ? k + 1.f : k;
+}
+
+// Where an item (one slot of one head, of keys or values) lies: blocks take slots of one
+// unit, or units whole where these have few slots.
+struct Item {
+  int r, h, i;
+  bool in;
+};
+__device__ __forceinline__ Item item_at(int item, int units_log2, int slots_log2, int kv_heads, int rows, int tokens) {
+  // A block: 2^units_log2 units of 2^slots_log2 slots each.
+  const int unit = ((int)blockIdx.y << units_log2) + (item >> slots_log2);
+  Item x;
+  x.r = unit / kv_heads;
+  x.h = unit - x.r * kv_heads;
+  x.i = ((int)blockIdx.x << slots_log2) + (item & ((1 << slots_log2) - 1));
+  x.in = x.r < rows && x.i < tokens;
+  return x;
+}
+
+template <typename T, int LPS_LOG2>  // 2^LPS_LOG2 threads per slot
+__global__ void __launch_bounds__(NT) kv_quantize_kernel(const __grid_constant__ WriteArgs a, const int units_log2,
+                                                         const int slots_log2) {
+  const int lane = threadIdx.x & ((1 << LPS_LOG2) - 1), y = lane & 1, i = lane >> 1;
+  const Item it = item_at(threadIdx.x >> LPS_LOG2, units_log2, slots_log2, a.kv_heads, a.rows, a.tokens);
+  int end = a.capacity, given = 0;
+  if (it.in && a.lengths) {
+    given = a.lengths[it.r];
+    end = min(max(given, 0), a.capacity);
+  }
+  if (it.in && a.status && it.h == 0 && it.i == 0 && lane == 0 && blockIdx.z == 0)
+    a.status[it.r] = a.lengths && given != end ? SV_ST_LENGTH : 0;
+  const int slot = end - a.tokens + it.i, blocks = (a.dim + 31) >> 5;
+  const bool in = it.in && slot >= 0 && i < blocks;  // (the shuffles need all lanes)
+  const T* src = static_cast<const T*>(blockIdx.z ? a.in[1] : a.in[0]) + it.r * a.i_row + it.h * a.i_head + it.i * a.i_tok;
+  float x[2][8];
+  bool has[2];
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    const int d = 32 * i + 16 * e + 8 * y;
+    has[e] = in && d < a.dim;
+    if (has[e]) load8(src + d, x[e]);
+  }
+  float lo[2], hi[2];
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    lo[e] = INFINITY;
+    hi[e] = -INFINITY;
+    if (has[e]) {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        lo[e] = min_nan(lo[e], x[e][k]);
+        hi[e] = max_nan(hi[e], x[e][k]);
+      }
+    }
+  }
+  const bool wide = a.dim > 64;  // groups of 32
+  if (wide) {
+    lo[0] = min_nan(lo[0], lo[1]);
+    hi[0] = max_nan(hi[0], hi[1]);
+  }
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    if (e && wide) break;
+    lo[e] = min_nan(lo[e], __shfl_xor_sync(0xffffffffu, lo[e], 1));
+    hi[e] = max_nan(hi[e], __shfl_xor_sync(0xffffffffu, hi[e], 1));
+  }
+  uint32_t word[2] = {0u, 0u};
+  uint32_t pair[2] = {0u, 0u};
+  float scale = 0.f, mid = 0.f, inv = 0.f;
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    if (!e || !wide) {
+      // Without a value (dimensions past head_dim): zeros.
+      const bool none = lo[e] > hi[e], bad = !none && !(lo[e] > -INFINITY && hi[e] < INFINITY);
+      const float l = fminf(fmaxf(lo[e], -kRecordMost), kRecordMost), h = fminf(fmaxf(hi[e], -kRecordMost), kRecordMost);
+      __half s16, m16;
+      if (!half_sure((h - l) * (1.f / 15.f), s16)) s16 = __double2half(((double)h - (double)l) / 15.0);
+      scale = __half2float(s16);
+      if (!half_sure(fmaf(8.f, scale, l), m16)) m16 = __double2half((double)l + 8.0 * (double)scale);
+      mid = __half2float(m16);
+      inv = scale > 0.f ? 1.f / scale : 0.f;
+      pair[e] = none ? 0u : bad ? 0x7e007e00u : (uint32_t)__half_as_ushort(s16) | (uint32_t)__half_as_ushort(m16) << 16;
+      if (none || bad) has[e] = false, has[1] = has[1] && (!wide || e);
+    }
+    if (has[e]) {
+      float q[8], edge = 0.f;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const float v = fminf(fmaxf(x[e][k], -kRecordMost), kRecordMost);
+        q[k] = fminf(fmaxf((v - mid) * inv, -8.f), 7.f);
+        const float r = rintf(q[k]);
+        edge = fmaxf(edge, fabsf(q[k] - r));
+      }
+      if (edge > 0.5f - 0x1p-16f) {
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+          if (fabsf(q[k] - rintf(q[k])) > 0.5f - 0x1p-16f)
+            q[k] = code_exactly(fminf(fmaxf(x[e][k], -kRecordMost), kRecordMost), mid, scale, q[k]);
+      }
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const int c = __float2int_rn(q[k]) + 8;  // dimension 4 t + 2 a + b, t = 2 y + (k >> 2)
+        word[k >> 2] |= (uint32_t)c << 4 * (4 * (k & 1) + 2 * e + (k >> 1 & 1));
+      }
+    }
+  }
+  if (!in) return;
+  unsigned char* rec = (blockIdx.z ? a.cache[1] : a.cache[0]) + it.r * a.row + it.h * a.head + (int64_t)slot * a.slot;
+  uint32_t* codes = reinterpret_cast<uint32_t*>(rec);
+  codes[2 * y * blocks + i] = word[0];
+  codes[(2 * y + 1) * blocks + i] = word[1];
+  uint32_t* pairs = codes + 4 * blocks;
+  if (wide) {
+    if (y == 0) pairs[i] = pair[0];
+    if (i == 0 && y == 1 && blocks == 3) pairs[3] = 0u;
+  } else {
+    pairs[2 * i + y] = pair[y];
+    if (blocks == 1) pairs[2 + y] = 0u;
+  }
+}
+
+template <typename T> __device__ __forceinline__ void store8(T* p, const float (&x)[8]);
+template <> __device__ __forceinline__ void store8<float>(float* p, const float (&x)[8]) {
+  reinterpret_cast<float4*>(p)[0] = make_float4(x[0], x[1], x[2], x[3]);
+  reinterpret_cast<float4*>(p)[1] = make_float4(x[4], x[5], x[6], x[7]);
+}
+template <> __device__ __forceinline__ void store8<__half>(__half* p, const float (&x)[8]) {
+  __half2 h[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) h[k] = __floats2half2_rn(x[2 * k], x[2 * k + 1]);
+  *reinterpret_cast<uint4*>(p) = *reinterpret_cast<const uint4*>(h);
+}
+template <> __device__ __forceinline__ void store8<__nv_bfloat16>(__nv_bfloat16* p, const float (&x)[8]) {
+  __nv_bfloat162 h[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) h[k] = __floats2bfloat162_rn(x[2 * k], x[2 * k + 1]);
+  *reinterpret_cast<uint4*>(p) = *reinterpret_cast<const uint4*>(h);
+}
+
+template <typename T, int LPS_LOG2>
+__global__ void __launch_bounds__(NT) kv_dequantize_kernel(const __grid_constant__ ReadArgs a, const int units_log2,
+                                                           const int slots_log2) {
+  const int lane = threadIdx.x & ((1 << LPS_LOG2) - 1), y = lane & 1, i = lane >> 1;
+  const Item it = item_at(threadIdx.x >> LPS_LOG2, units_log2, slots_log2, a.kv_heads, a.rows, a.tokens);
+  const int blocks = (a.dim + 31) >> 5;
+  if (!it.in || i >= blocks) return;
+  int end = a.capacity, given = 0;
+  if (a.lengths) {
+    given = a.lengths[it.r];
+    end = min(max(given, 0), a.capacity);
+  }
+  if (a.status && it.h == 0 && it.i == 0 && lane == 0 && blockIdx.z == 0)
+    a.status[it.r] = a.lengths && given != end ? SV_ST_LENGTH : 0;
+  const int slot = a.newest ? end - a.tokens + it.i : it.i;
+  if (a.seen) {
+    const int start = a.starts ? min(max(a.starts[it.r], 0), end) : 0;
+    const int low = a.window ? max(start, end - a.seen - a.window + 1) : start;
+    if (slot < start || slot >= end || (slot < low && slot >= start + a.sinks)) return;
+  }
+  uint32_t word[2] = {0u, 0u}, pair[2] = {0u, 0u};
+  if (slot >= 0 && slot < end) {
+    const unsigned char* rec = (blockIdx.z ? a.cache[1] : a.cache[0]) + it.r * a.row + it.h * a.head + (int64_t)slot * a.slot;
+    const uint32_t* codes = reinterpret_cast<const uint32_t*>(rec);
+    word[0] = __ldg(codes + 2 * y * blocks + i);
+    word[1] = __ldg(codes + (2 * y + 1) * blocks + i);
+    const bool wide = a.dim > 64;
+    pair[0] = __ldg(codes + 4 * blocks + (wide ? i : 2 * i));
+    pair[1] = wide ? pair[0] : __ldg(codes + 4 * blocks + 2 * i + 1);
+  }
+  T* out = static_cast<T*>(blockIdx.z ? a.out[1] : a.out[0]) +
+           (((int64_t)it.r * a.kv_heads + it.h) * a.tokens + it.i) * a.dim;
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    const int d = 32 * i + 16 * e + 8 * y;
+    if (d >= a.dim) break;
+    const float scale = __half2float(__ushort_as_half((unsigned short)(pair[e] & 0xffffu)));
+    const float mid = __half2float(__ushort_as_half((unsigned short)(pair[e] >> 16)));
+    float x[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const int c = (int)(word[k >> 2] >> 4 * (4 * (k & 1) + 2 * e + (k >> 1 & 1)) & 15u) - 8;
+      x[k] = fmaf(scale, (float)c, mid);
+    }
+    store8(out + d, x);
+  }
+}
+
+// The grid of a kernel whose blocks take 2^(8 - lps_log2) slots: of one unit, or of several whole ones.
+dim3 grid_of(int lps_log2, int64_t units, int tokens, bool both, int& units_log2, int& slots_log2) {
+  slots_log2 = 0;
+  while ((1 << slots_log2) < tokens && slots_log2 < 8 - lps_log2) ++slots_log2;
+  units_log2 = 8 - lps_log2 - slots_log2;
+  return dim3((unsigned)((tokens + (1 << slots_log2) - 1) >> slots_log2), (unsigned)((units + (1 << units_log2) - 1) >> units_log2),
+              both ? 2u : 1u);
+}
+
+template <typename T> cudaError_t write_records(const WriteArgs& a, cudaStream_t stream) {
+  int u, s;
+  const int64_t units = (int64_t)a.rows * a.kv_heads;
+  auto go = [&](auto kernel, int lps_log2) {
+    const dim3 grid = grid_of(lps_log2, units, a.tokens, a.in[1] != nullptr, u, s);
+    kernel<<<grid, NT, 0, stream>>>(a, u, s);
+    return cudaGetLastError();
+  };
+  if (a.dim > 64) return go(kv_quantize_kernel<T, 3>, 3);
+  return a.dim > 32 ? go(kv_quantize_kernel<T, 2>, 2) : go(kv_quantize_kernel<T, 1>, 1);
+}
+
+template <typename T> cudaError_t read_records(const ReadArgs& a, cudaStream_t stream) {
+  int u, s;
+  const int64_t units = (int64_t)a.rows * a.kv_heads;
+  auto go = [&](auto kernel, int lps_log2) {
+    const dim3 grid = grid_of(lps_log2, units, a.tokens, a.out[1] != nullptr, u, s);
+    kernel<<<grid, NT, 0, stream>>>(a, u, s);
+    return cudaGetLastError();
+  };
+  if (a.dim > 64) return go(kv_dequantize_kernel<T, 3>, 3);
+  return a.dim > 32 ? go(kv_dequantize_kernel<T, 2>, 2) : go(kv_dequantize_kernel<T, 1>, 1);
+}
+
+// What both calls take of a cache.
+int check_records(const void* k, const void* v, int32_t rows, int32_t kv_heads, int32_t dim, int32_t capacity,
+                  int32_t tokens, int64_t row, int64_t head, int64_t slot) {
+  if (!k) return SV_E_ARG;
+  if (rows < 1 || kv_heads < 1 || capacity < 1 || tokens < 0 || capacity > 1 << 29 || tokens > 1 << 29) return SV_E_SHAPE;
+  if (dim < 8 || dim > kAttnMaxDim || dim % 8 || (int64_t)rows * kv_heads > 65535) return SV_E_SHAPE;
+  if (row < 0 || head < 0 || slot < 0 || (capacity > 1 && slot == 0)) return SV_E_SHAPE;
+  if (row % 16 || head % 16 || slot % 16) return SV_E_ALIGN;
+  if (reinterpret_cast<uintptr_t>(k) % 16 || reinterpret_cast<uintptr_t>(v) % 16) return SV_E_ALIGN;
+  return SV_OK;
+}
+
+}  // namespace
+
+cudaError_t launch_read_records(const ReadArgs& a, cudaStream_t stream) {
+  if (a.dtype == SV_F32) return read_records<float>(a, stream);
+  return a.dtype == SV_F16 ? read_records<__half>(a, stream) : read_records<__nv_bfloat16>(a, stream);
+}
+
+}  // namespace sv
+
+using namespace sv;
+
+// See include/starvector_sampling.h.
+extern "C" {
+
+int32_t sv_kv_record_bytes(int32_t head_dim) {
+  return head_dim < 8 || head_dim > kAttnMaxDim || head_dim % 8 ? 0 : record_bytes(head_dim);
+}
+
+int sv_kv_quantize(const void* keys, const void* values, int32_t dtype, int32_t rows, int32_t kv_heads, int32_t tokens,
+                   int32_t head_dim, int64_t stride_row, int64_t stride_head, int64_t stride_token, void* cache_keys,
+                   void* cache_values, int32_t capacity, int64_t cache_stride_row, int64_t cache_stride_head,
+                   int64_t cache_stride_slot, const int32_t* lengths, int32_t* out_status, void* stream) {
+  if (dtype != SV_F32 && dtype != SV_F16 && dtype != SV_BF16) return SV_E_DTYPE;
+  if (!keys || (values != nullptr) != (cache_values != nullptr) || cache_keys == cache_values) return SV_E_ARG;
+  const int rc = check_records(cache_keys, cache_values, rows, kv_heads, head_dim, capacity, tokens, cache_stride_row,
+                               cache_stride_head, cache_stride_slot);
+  if (rc) return rc;
+  const int64_t e = dtype == SV_F32 ? 4 : 2;
+  for (int64_t s : {stride_row, stride_head, stride_token})
+    if (s < 0 || s * e % 16) return SV_E_ALIGN;
+  if (reinterpret_cast<uintptr_t>(keys) % 16 || reinterpret_cast<uintptr_t>(values) % 16) return SV_E_ALIGN;
+  // Every slot's record is written by its own threads.
+  if (!entries_apart<3>(record_bytes(head_dim), {rows, kv_heads, capacity},
+                        {cache_stride_row, cache_stride_head, cache_stride_slot}))
+    return SV_E_SHAPE;
+  if (tokens == 0) return SV_OK;
+  WriteArgs a = {{keys, values}, stride_row, stride_head, stride_token,
+                 {static_cast<unsigned char*>(cache_keys), static_cast<unsigned char*>(cache_values)},
+                 cache_stride_row, cache_stride_head, cache_stride_slot, lengths, out_status,
+                 rows, kv_heads, head_dim, capacity, tokens};
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const cudaError_t err = dtype == SV_F32   ? write_records<float>(a, s)
+                          : dtype == SV_F16 ? write_records<__half>(a, s)
+                                            : write_records<__nv_bfloat16>(a, s);
+  return err == cudaSuccess ? SV_OK : SV_E_CUDA;
+}
+
+int sv_kv_dequantize(const void* cache_keys, const void* cache_values, int32_t rows, int32_t kv_heads, int32_t head_dim,
+                     int32_t capacity, int64_t cache_stride_row, int64_t cache_stride_head, int64_t cache_stride_slot,
+                     const int32_t* lengths, int32_t tokens, void* keys, void* values, int32_t dtype,
+                     int32_t* out_status, void* stream) {
+  if (dtype != SV_F32 && dtype != SV_F16 && dtype != SV_BF16) return SV_E_DTYPE;
+  if (!keys || (values != nullptr) != (cache_values != nullptr) || keys == values) return SV_E_ARG;
+  const int rc = check_records(cache_keys, cache_values, rows, kv_heads, head_dim, capacity, tokens, cache_stride_row,
+                               cache_stride_head, cache_stride_slot);
+  if (rc) return rc;
+  if (reinterpret_cast<uintptr_t>(keys) % 16 || reinterpret_cast<uintptr_t>(values) % 16) return SV_E_ALIGN;
+  ReadArgs a = {};
+  a.cache[0] = static_cast<const unsigned char*>(cache_keys);
+  a.cache[1] = static_cast<const unsigned char*>(cache_values);
+  a.row = cache_stride_row;
+  a.head = cache_stride_head;
+  a.slot = cache_stride_slot;
+  a.out[0] = keys;
+  a.out[1] = values;
+  a.lengths = lengths;
+  a.status = out_status;
+  a.dtype = dtype;
+  a.rows = rows;
+  a.kv_heads = kv_heads;
+  a.dim = head_dim;
+  a.capacity = capacity;
+  a.tokens = tokens ? tokens : capacity;
+  a.newest = tokens != 0;
+  return launch_read_records(a, static_cast<cudaStream_t>(stream)) == cudaSuccess ? SV_OK : SV_E_CUDA;
+}
+
+}  // extern "C"

@@ -7,7 +7,7 @@
 // exceptions as before).  Shapes and the history form are decided by the Python
 // wrappers (ops.py), which pass the same sizes and strides as the C signatures;
 // nothing here synchronises or allocates.  The cache operators (window_attention,
-// prefix_attention, kv_evict) are called once per layer or token, where each tensor
+// prefix_attention, quantized_attention, kv_quantize, kv_dequantize, kv_evict) are called once per layer or token, where each tensor
 // attribute read from Python counts: they look at the shapes here (ValueError where
 // ops.py would raise one) and allocate their outputs, the attention functions also a
 // workspace kept per device, stream and size.
@@ -312,6 +312,24 @@ at::Tensor attention_out(const OptT& out, const at::Tensor& q) {
   return *out;
 }
 
+void check_window(int64_t window, int64_t sinks, std::optional<double> scale) {
+  TORCH_CHECK_VALUE(window >= 0 && sinks >= 0, "window and sinks must not be negative");
+  TORCH_CHECK_VALUE(!scale.has_value() || std::isfinite(*scale), "scale must be finite");
+}
+
+// The accumulator of an attention's weights as [rows, kv_heads, slots], or none.
+OptT check_weights(const OptT& given, int64_t rows, int64_t kv, int64_t capacity) {
+  OptT weights = given;
+  if (!weights.has_value()) return weights;
+  if (weights->dim() == 2) weights = weights->unsqueeze(1);
+  TORCH_CHECK_VALUE(weights->scalar_type() == at::kFloat && weights->dim() == 3 && weights->size(0) == rows &&
+                        weights->size(1) == kv && weights->size(2) >= capacity && contiguous_along(*weights, 2),
+                    "weights must be float32 [rows, kv_heads, capacity], contiguous along the slots");
+  TORCH_CHECK_VALUE((rows <= 1 || weights->stride(0) > 0) && (kv <= 1 || weights->stride(1) > 0),
+                    "weights are added to in place: rows and heads must not be broadcast");
+  return weights;
+}
+
 // sv_window_attention.
 std::tuple<int, at::Tensor> window_attention(const at::Tensor& q_in, const at::Tensor& keys_in,
                                              const at::Tensor& values_in, const OptT& lengths_in,
@@ -325,17 +343,8 @@ std::tuple<int, at::Tensor> window_attention(const at::Tensor& q_in, const at::T
   const auto stream = at::cuda::getCurrentCUDAStream(dev.index());
   const int32_t rows = size32(q, 0), n = size32(q, 1), heads = size32(q, 2), dim = size32(q, 3);
   const int32_t kv = size32(keys, 1), capacity = size32(keys, 2), code = logit_code(q);
-  TORCH_CHECK_VALUE(window >= 0 && sinks >= 0, "window and sinks must not be negative");
-  TORCH_CHECK_VALUE(!scale.has_value() || std::isfinite(*scale), "scale must be finite");
-  OptT weights = weights_in;
-  if (weights.has_value()) {
-    if (weights->dim() == 2) weights = weights->unsqueeze(1);
-    TORCH_CHECK_VALUE(weights->scalar_type() == at::kFloat && weights->dim() == 3 && weights->size(0) == rows &&
-                          weights->size(1) == kv && weights->size(2) >= capacity && contiguous_along(*weights, 2),
-                      "weights must be float32 [rows, kv_heads, capacity], contiguous along the slots");
-    TORCH_CHECK_VALUE((rows <= 1 || weights->stride(0) > 0) && (kv <= 1 || weights->stride(1) > 0),
-                      "weights are added to in place: rows and heads must not be broadcast");
-  }
+  check_window(window, sinks, scale);
+  const OptT weights = check_weights(weights_in, rows, kv, capacity);
   const OptT lengths = row_ints(lengths_in, rows, dev, "lengths"), starts = row_ints(starts_in, rows, dev, "starts");
   const int32_t w = (int32_t)std::min<int64_t>(window, 1 << 30), s = (int32_t)std::min<int64_t>(sinks, 1 << 30);
   at::Tensor o = attention_out(out, q_in);
@@ -355,6 +364,142 @@ std::tuple<int, at::Tensor> window_attention(const at::Tensor& q_in, const at::T
       weights.has_value() ? stride_of(*weights, 1) : 0, o.data_ptr(), ws.defined() ? ws.data_ptr() : nullptr,
       ws.defined() ? (size_t)ws.numel() : 0, status_ptr(out_status, rows, dev),
       stream.stream());
+  return {rc, o};
+}
+
+// One layer of a cache held in 4 bits as [rows, kv_heads, capacity, record].
+void check_records(const at::Tensor& k, const OptT& v, int64_t rows, int64_t dim, const at::Device& dev) {
+  on_device(k, dev, "cache_keys");
+  if (v.has_value()) on_device(*v, dev, "cache_values");
+  const int64_t bytes = dim >= 0 && dim <= INT32_MAX ? sv_kv_record_bytes((int32_t)dim) : 0;
+  TORCH_CHECK_VALUE(bytes > 0, "head_dim must be a multiple of 8 in [8, 128]");
+  TORCH_CHECK_VALUE(k.scalar_type() == at::kByte && (!v.has_value() || v->scalar_type() == at::kByte),
+                    "caches held in 4 bits must be uint8");
+  TORCH_CHECK_VALUE(k.dim() == 4 && k.size(3) == bytes && k.size(0) == rows && k.size(1) > 0,
+                    "cache_keys must be [rows, capacity, record] or [rows, kv_heads, capacity, record], of ", bytes,
+                    " bytes a record for this head_dim");
+  TORCH_CHECK_VALUE(!v.has_value() || same_layout(k, *v), "cache_values must have the shape and strides of cache_keys");
+  TORCH_CHECK_VALUE(contiguous_along(k, 3), "records must be contiguous");
+}
+
+OptT layer_cache(const OptT& t) { return t.has_value() ? OptT(layer_cache(*t)) : t; }
+
+// sv_kv_quantize.
+int kv_quantize(const at::Tensor& keys_in, const OptT& values_in, const at::Tensor& cache_keys_in,
+                const OptT& cache_values_in, const OptT& lengths_in, const OptT& out_status) {
+  at::Tensor keys = layer_cache(keys_in);
+  OptT values = layer_cache(values_in);
+  const at::Tensor ck = layer_cache(cache_keys_in);
+  const OptT cv = layer_cache(cache_values_in);
+  const at::Device dev = keys.device();
+  on_device(keys, dev, "keys");
+  const auto st = keys.scalar_type();
+  TORCH_CHECK_VALUE(st == at::kFloat || st == at::kHalf || st == at::kBFloat16, "unsupported dtype ", st);
+  TORCH_CHECK_VALUE(keys.dim() == 4, "keys must be [rows, tokens, head_dim] or [rows, kv_heads, tokens, head_dim]");
+  TORCH_CHECK_VALUE(values.has_value() == cv.has_value(), "values and cache_values go together");
+  if (values.has_value()) {
+    on_device(*values, dev, "values");
+    TORCH_CHECK_VALUE(values->scalar_type() == st && values->sizes() == keys.sizes(),
+                      "values must have the keys' shape and dtype");
+  }
+  check_records(ck, cv, keys.size(0), keys.size(3), dev);
+  TORCH_CHECK_VALUE(ck.size(1) == keys.size(1), "the cache must have the keys' heads");
+  const c10::cuda::CUDAGuard guard(dev);
+  const OptT lengths = row_ints(lengths_in, keys.size(0), dev, "lengths");
+  if (keys.numel() == 0 || ck.numel() == 0) {
+    fill_status(out_status, lengths, std::nullopt, keys.size(0), ck.size(2), dev);
+    return 0;
+  }
+  // Other layouts are copied first (values at strides of their own among them).
+  if (!contiguous_along(keys, 3) || !aligned(keys, 3) ||
+      (values.has_value() && (!same_layout(keys, *values) || !aligned(*values, 3)))) {
+    keys = keys.clone(at::MemoryFormat::Contiguous);
+    if (values.has_value()) values = values->clone(at::MemoryFormat::Contiguous);
+  }
+  return sv_kv_quantize(keys.data_ptr(), raw(values, dev, "values"), logit_code(keys), size32(keys, 0), size32(keys, 1),
+                        size32(keys, 2), size32(keys, 3), stride_of(keys, 0), stride_of(keys, 1), stride_of(keys, 2),
+                        ck.data_ptr(), raw(cv, dev, "cache_values"), size32(ck, 2), stride_of(ck, 0), stride_of(ck, 1),
+                        stride_of(ck, 2), optptr<int32_t>(lengths, dev, "lengths", at::kInt, keys.size(0)),
+                        status_ptr(out_status, keys.size(0), dev), stream_of(keys));
+}
+
+// sv_kv_dequantize.
+std::tuple<int, at::Tensor, OptT> kv_dequantize(const at::Tensor& cache_keys_in, const OptT& cache_values_in,
+                                                int64_t head_dim, const OptT& lengths_in, std::optional<int64_t> tokens,
+                                                at::ScalarType dtype, const OptT& keys_out, const OptT& values_out,
+                                                const OptT& out_status) {
+  const at::Tensor ck = layer_cache(cache_keys_in);
+  const OptT cv = layer_cache(cache_values_in);
+  const at::Device dev = ck.device();
+  TORCH_CHECK_VALUE(ck.dim() == 4, "cache_keys must be [rows, capacity, record] or [rows, kv_heads, capacity, record]");
+  check_records(ck, cv, ck.size(0), head_dim, dev);
+  TORCH_CHECK_VALUE(dtype == at::kFloat || dtype == at::kHalf || dtype == at::kBFloat16, "unsupported dtype ", dtype);
+  TORCH_CHECK_VALUE(!tokens.has_value() || (*tokens >= 0 && *tokens <= 1 << 29), "tokens must be in [0, 2^29]");
+  const int64_t places = tokens.has_value() ? *tokens : ck.size(2);
+  auto shape = cache_keys_in.sizes().vec();
+  shape[shape.size() - 2] = places;
+  shape[shape.size() - 1] = head_dim;
+  const c10::cuda::CUDAGuard guard(dev);
+  const auto make = [&](const OptT& given, const char* name) {
+    if (!given.has_value()) return at::empty(shape, ck.options().dtype(dtype));
+    on_device(*given, dev, name);
+    TORCH_CHECK(given->scalar_type() == dtype && given->sizes() == at::IntArrayRef(shape) && given->is_contiguous(),
+                "out must be contiguous tensors of the outputs' shape and dtype");
+    return *given;
+  };
+  at::Tensor keys = make(keys_out, "out");
+  OptT values;
+  if (cv.has_value()) values = make(values_out, "out");
+  const OptT lengths = row_ints(lengths_in, ck.size(0), dev, "lengths");
+  if (keys.numel() == 0 || ck.numel() == 0) {
+    fill_status(out_status, lengths, std::nullopt, ck.size(0), ck.size(2), dev);
+    keys.zero_();
+    if (values.has_value()) values->zero_();
+    return {0, keys, values};
+  }
+  const int rc = sv_kv_dequantize(
+      ck.data_ptr(), raw(cv, dev, "cache_values"), size32(ck, 0), size32(ck, 1), (int32_t)head_dim, size32(ck, 2),
+      stride_of(ck, 0), stride_of(ck, 1), stride_of(ck, 2),
+      optptr<int32_t>(lengths, dev, "lengths", at::kInt, ck.size(0)), tokens.has_value() ? (int32_t)places : 0,
+      keys.data_ptr(), values.has_value() ? values->data_ptr() : nullptr, logit_code(keys),
+      status_ptr(out_status, ck.size(0), dev), stream_of(ck));
+  return {rc, keys, values};
+}
+
+// sv_quantized_attention.
+std::tuple<int, at::Tensor> quantized_attention(const at::Tensor& q_in, const at::Tensor& cache_keys_in,
+                                                const at::Tensor& cache_values_in, const OptT& lengths_in,
+                                                const OptT& starts_in, int64_t window, int64_t sinks,
+                                                std::optional<double> scale, const OptT& weights_in, const OptT& out,
+                                                const OptT& out_status) {
+  const at::Tensor q = queries(q_in), ck = layer_cache(cache_keys_in), cv = layer_cache(cache_values_in);
+  const at::Device dev = q.device();
+  check_records(ck, cv, q.size(0), q.size(3), dev);
+  TORCH_CHECK_VALUE(q.size(2) % ck.size(1) == 0, "kv_heads must divide heads");
+  const c10::cuda::CUDAGuard guard(dev);
+  const auto stream = at::cuda::getCurrentCUDAStream(dev.index());
+  const int32_t rows = size32(q, 0), n = size32(q, 1), heads = size32(q, 2), dim = size32(q, 3);
+  const int32_t kv = size32(ck, 1), capacity = size32(ck, 2), code = logit_code(q);
+  check_window(window, sinks, scale);
+  const OptT weights = check_weights(weights_in, rows, kv, capacity);
+  const OptT lengths = row_ints(lengths_in, rows, dev, "lengths"), starts = row_ints(starts_in, rows, dev, "starts");
+  const int32_t w = (int32_t)std::min<int64_t>(window, 1 << 30), s = (int32_t)std::min<int64_t>(sinks, 1 << 30);
+  at::Tensor o = attention_out(out, q_in);
+  if (o.numel() == 0 || capacity == 0) {  // no slots: every query sees nothing
+    fill_status(out_status, lengths, starts, rows, capacity, dev);
+    return {0, o.zero_()};
+  }
+  const size_t bytes =
+      sv_quantized_attention_workspace_bytes(code, rows, n, heads, kv, dim, capacity, w, s, weights.has_value());
+  at::Tensor ws = workspace_for(dev, stream, bytes, 4 * ((size_t)rows * kv + 1024));
+  const int rc = sv_quantized_attention(
+      q.data_ptr(), code, rows, n, heads, kv, dim, stride_of(q, 0), stride_of(q, 1), stride_of(q, 2), ck.data_ptr(),
+      cv.data_ptr(), capacity, stride_of(ck, 0), stride_of(ck, 1), stride_of(ck, 2),
+      optptr<int32_t>(lengths, dev, "lengths", at::kInt, rows), optptr<int32_t>(starts, dev, "starts", at::kInt, rows),
+      w, s, scale.has_value() ? *scale : 1.0 / std::sqrt((double)dim),
+      optptr<float>(weights, dev, "weights", at::kFloat), weights.has_value() ? stride_of(*weights, 0) : 0,
+      weights.has_value() ? stride_of(*weights, 1) : 0, o.data_ptr(), ws.defined() ? ws.data_ptr() : nullptr,
+      ws.defined() ? (size_t)ws.numel() : 0, status_ptr(out_status, rows, dev), stream.stream());
   return {rc, o};
 }
 
@@ -469,4 +614,7 @@ PYBIND11_MODULE(sv_torch, m) {
   m.def("window_attention", &window_attention);
   m.def("prefix_attention", &prefix_attention);
   m.def("kv_evict", &kv_evict);
+  m.def("kv_quantize", &kv_quantize);
+  m.def("kv_dequantize", &kv_dequantize);
+  m.def("quantized_attention", &quantized_attention);
 }

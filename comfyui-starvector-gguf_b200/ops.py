@@ -628,3 +628,73 @@ def kv_evict(keys, values, weights, positions, lengths=None, budget=None, *, sin
         recent, o.get("weights"), o.get("positions"), o.get("lengths"), status)
     L.check(rc, "sv_kv_evict")
     return o
+
+
+def kv_record_bytes(head_dim):
+    """Bytes of a record of the cache held in 4 bits (sv_kv_record_bytes): one slot of one
+    head.  head_dim a multiple of 8, 8..128."""
+    n = L.lib().sv_kv_record_bytes(int(head_dim))
+    if n == 0:
+        raise ValueError("head_dim must be a multiple of 8 in [8, 128]")
+    return n
+
+
+def kv_quantize(keys, values, cache_keys, cache_values, lengths=None, *, status=None):
+    """Writes tokens into a cache held in 4 bits (sv_kv_quantize): they are the newest
+    `tokens` of each row's `lengths` slots, the other slots stay as they are.
+
+    keys / values: [rows, kv_heads, tokens, head_dim], or [rows, tokens, head_dim] (MQA),
+    float32, float16 or bfloat16 (values may be None, with cache_values); cache_keys /
+    cache_values: one layer of the cache, uint8 [rows, kv_heads, capacity,
+    kv_record_bytes(head_dim)], or [rows, capacity, ...] (MQA), written in place; a new
+    cache is torch.zeros of that.  Groups of 32 dimensions (16 where head_dim <= 64) share a
+    float16 scale and middle; finite values beyond 32768 in magnitude count as that, and a
+    group with a NaN or infinity reads back as NaN.  lengths: int32 [rows] on the device, the
+    new tokens included, one number or None (all slots); a row of fewer leaves out the first
+    tokens (padding in front).  status: int32 [rows], filled with 0 or SV_ST_LENGTH.
+
+    kv_reorder and kv_evict take such caches (with their layers in front) as they are."""
+    if isinstance(lengths, int):
+        (cache_keys, cache_values), lengths = _first_records(cache_keys, cache_values, lengths), None
+    L.check(_ext().kv_quantize(keys, values, cache_keys, cache_values, lengths, status), "sv_kv_quantize")
+
+
+def kv_dequantize(cache_keys, cache_values, head_dim, lengths=None, *, tokens=None, dtype=torch.float16, out=None,
+                  status=None):
+    """Reads a cache held in 4 bits back (sv_kv_dequantize): keys and values [rows,
+    kv_heads, places, head_dim], or [rows, places, head_dim] (MQA), of `dtype`.
+
+    Place i holds slot i (tokens None: as many places as slots), or of the newest `tokens`
+    of each row's `lengths` slots the i-th; places without a slot are zero.  The caches and
+    lengths as in kv_quantize (cache_values may be None, then values are None).  out: a pair of
+    contiguous tensors to fill."""
+    if isinstance(lengths, int):
+        (cache_keys, cache_values), lengths = _first_records(cache_keys, cache_values, lengths), None
+    keys, values = out if out is not None else (None, None)
+    rc, keys, values = _ext().kv_dequantize(cache_keys, cache_values, head_dim, lengths, tokens, dtype, keys, values,
+                                            status)
+    L.check(rc, "sv_kv_dequantize")
+    return keys, values
+
+
+def _first_records(cache_keys, cache_values, length):
+    """The first `length` slots of a layer's records (values may be None)."""
+    if not 1 <= length <= cache_keys.shape[-2]:
+        raise ValueError("length must be in [1, capacity]")
+    return cache_keys.narrow(-2, 0, length), None if cache_values is None else cache_values.narrow(-2, 0, length)
+
+
+def quantized_attention(q, cache_keys, cache_values, lengths=None, *, starts=None, window=0, sinks=0, scale=None,
+                        weights=None, out=None, status=None):
+    """window_attention over one layer of a cache held in 4 bits (sv_quantized_attention):
+    the same of the values that the records stand for.
+
+    cache_keys / cache_values: uint8 [rows, kv_heads, capacity, kv_record_bytes(head_dim)],
+    or [rows, capacity, ...] (MQA), as kv_quantize leaves them, same strides; q (float32,
+    float16, bfloat16) and the rest as window_attention."""
+    if isinstance(lengths, int):
+        (cache_keys, cache_values), lengths = _first_records(cache_keys, cache_values, lengths), None
+    rc, o = _ext().quantized_attention(q, cache_keys, cache_values, lengths, starts, window, sinks, scale, weights, out,
+                                       status)
+    L.check(rc, "sv_quantized_attention")
+    return o

@@ -486,6 +486,74 @@ int sv_kv_evict(void* keys, void* values, int32_t elem_bytes, int32_t layers, in
                 int32_t budget, int32_t sinks, int32_t recent, float* weights_out, int32_t* positions_out,
                 int32_t* lengths_out, int32_t* out_status, void* stream);
 
+/*
+ * A cache held in 4 bits: a record of sv_kv_record_bytes(head_dim) bytes per slot and
+ * key/value head, 80 bytes for 128 dimensions.  Values are taken in groups of neighbouring
+ * dimensions, 32 of them where head_dim > 64, 16 otherwise; a value is held as a code c of
+ * 4 bits and stands for mid + scale (c - 8), the group's scale and mid being float16:
+ *   scale = f16((hi - lo) / 15), mid = f16(lo + 8 scale), c = 8 + the whole number next to
+ *   (x - mid) / scale (ties to the even one; 8 where scale is 0), within 0..15,
+ * lo and hi the group's extremes; each is rounded once from the exact number.  Finite
+ * values beyond +-32768 count as that; a group with a NaN or an infinity stands for NaN.
+ * A record: P / 2 bytes of codes (P: head_dim rounded up to a multiple of 32), then four
+ * pairs (scale, mid), one per group.  The codes are 32-bit words; nibble 4 b + 2 e + a of
+ * word t P / 32 + i holds dimension 32 i + 16 e + 4 t + 2 a + b (t, a, b, e, i from 0).
+ * Codes past head_dim and pairs without a group are 0.  Records may be moved as they
+ * are (sv_kv_reorder and sv_kv_evict with elem_bytes 1 and the record's bytes as head_dim).
+ * head_dim a multiple of 8, 8..128 (otherwise sv_kv_record_bytes returns 0).
+ */
+int32_t sv_kv_record_bytes(int32_t head_dim);
+
+/*
+ * Writes tokens into a cache held in 4 bits: token i of row r goes to slot lengths[r] -
+ * tokens + i (the newest slots, as the queries of the attention stand); tokens that
+ * would lie before slot 0 (rows with fewer) are left out, other slots as they were.  No counterpart in
+ * the reference.
+ *   keys, values  [rows, kv_heads, tokens, head_dim] of dtype (SV_F32 / SV_F16 / SV_BF16)
+ *          at the given strides in elements, head_dim contiguous; both alike
+ *   cache_keys, cache_values  records (row, head, slot) at row * cache_stride_row + head *
+ *          cache_stride_head + slot * cache_stride_slot bytes, both alike; no two may
+ *          coincide, the two caches included
+ *   lengths  int32 [rows] or NULL (= capacity), the new tokens included; values outside [0,
+ *          capacity] are clamped and reported as SV_ST_LENGTH
+ *   out_status  int32 [rows] or NULL
+ * values and cache_values may both be NULL.  rows * kv_heads <= 65535; capacity and tokens <=
+ * 2^29; pointers and all strides in bytes multiples of 16.
+ */
+int sv_kv_quantize(const void* keys, const void* values, int32_t dtype, int32_t rows, int32_t kv_heads, int32_t tokens,
+                   int32_t head_dim, int64_t stride_row, int64_t stride_head, int64_t stride_token, void* cache_keys,
+                   void* cache_values, int32_t capacity, int64_t cache_stride_row, int64_t cache_stride_head,
+                   int64_t cache_stride_slot, const int32_t* lengths, int32_t* out_status, void* stream);
+
+/*
+ * Reads such a cache back: place i of keys / values [rows, kv_heads, places, head_dim]
+ * (contiguous, of dtype) gets what slot i stands for (tokens 0: places = capacity), or with tokens > 0 that of
+ * slot lengths[r] - tokens + i (places = tokens), rounded once to dtype; places without a slot of the row
+ * (before 0, from lengths[r] on) become 0.  The rest as sv_kv_quantize.  The outputs must
+ * not overlap the caches.
+ */
+int sv_kv_dequantize(const void* cache_keys, const void* cache_values, int32_t rows, int32_t kv_heads, int32_t head_dim,
+                     int32_t capacity, int64_t cache_stride_row, int64_t cache_stride_head, int64_t cache_stride_slot,
+                     const int32_t* lengths, int32_t tokens, void* keys, void* values, int32_t dtype,
+                     int32_t* out_status, void* stream);
+
+/*
+ * sv_window_attention over a cache held in 4 bits: the same of the values that the records
+ * stand for.  cache_keys, cache_values as in sv_kv_dequantize; they hold records that
+ * sv_kv_quantize made.  The workspace has
+ * sv_quantized_attention_workspace_bytes(...) bytes; the rest as sv_window_attention.
+ */
+size_t sv_quantized_attention_workspace_bytes(int32_t dtype, int32_t rows, int32_t tokens, int32_t heads,
+                                              int32_t kv_heads, int32_t head_dim, int32_t capacity, int32_t window,
+                                              int32_t sinks, int32_t with_weights);
+int sv_quantized_attention(const void* q, int32_t dtype, int32_t rows, int32_t tokens, int32_t heads, int32_t kv_heads,
+                           int32_t head_dim, int64_t q_stride_row, int64_t q_stride_token, int64_t q_stride_head,
+                           const void* cache_keys, const void* cache_values, int32_t capacity, int64_t cache_stride_row,
+                           int64_t cache_stride_head, int64_t cache_stride_slot, const int32_t* lengths,
+                           const int32_t* starts, int32_t window, int32_t sinks, double scale, float* weights,
+                           int64_t weights_stride_row, int64_t weights_stride_head, void* out, void* workspace,
+                           size_t workspace_bytes, int32_t* out_status, void* stream);
+
 /* Text of a return or status code. */
 const char* sv_error_string(int32_t code);
 
