@@ -12,6 +12,7 @@ namespace {
 constexpr int kSMs = 148;
 constexpr int kMostPrefixSplits = 16;  // that the token kernel joins
 constexpr int kMostSlots = 1 << 29;    // sums of two slot numbers stay in 31 bits
+constexpr int kMostRecordGroups = 4;   // groups of query rows that the kernel over 4-bit records takes one by one
 constexpr size_t kMostScores = (size_t)256 << 20;  // bytes of scores kept for the accumulated weights
 
 size_t up256(size_t x) { return (x + 255) / 256 * 256; }
@@ -200,9 +201,34 @@ void set_window(AttnArgs& a, int32_t window, int32_t sinks) {
   a.sinks = sinks < 0 || (limit && window > 0) ? sinks : 0;
 }
 
-// The plain keys and values of a whole cache.
-size_t read_bytes(const AttnArgs& a) {
-  return 2 * up256((size_t)a.rows * a.kv_heads * a.capacity * a.dim * (a.dtype == SV_F32 ? 4 : 2));
+// How a call over 4-bit records is done: by the kernel that takes them as they are (few query rows),
+// or from the plain values of the slots that some query sees.
+struct RecordPlan {
+  bool direct;
+  RecordRows rows;
+  size_t counters, o_bytes, ml_bytes, lse_bytes, score_bytes;  // direct
+  size_t before, values;                                       // the other way: the attention's own, the plain values
+  size_t total() const { return direct ? counters + o_bytes + ml_bytes + lse_bytes + score_bytes : before + values; }
+};
+
+RecordPlan record_plan(const AttnArgs& a) {
+  RecordPlan p = {};
+  const int64_t nG = (int64_t)a.n * a.group, units = (int64_t)a.rows * a.kv_heads, all = units * nG;
+  p.rows.tiles = nG <= 8 ? 1 : 2;
+  p.rows.groups = div_up(nG, 8 * p.rows.tiles);
+  p.counters = SV_ATTENTION_ZERO_BYTES;
+  p.o_bytes = up256((size_t)2 * kTokenBlocks * 8 * p.rows.tiles * record_dims(a.dim) * 4);
+  p.ml_bytes = up256((size_t)2 * kTokenBlocks * 8 * p.rows.tiles * 8);
+  p.lse_bytes = a.weights ? up256(all * 4) : 0;
+  p.score_bytes = a.weights ? up256(all * a.capacity * 4) : 0;
+  // A unit's counter each, and chunks (of at least 128 slots) counted in 31 bits.
+  p.direct = a.dtype != SV_F32 && p.rows.groups <= kMostRecordGroups && units * p.rows.groups <= 65536 &&
+             units * p.rows.groups * (a.capacity / 128 + 3) < (int64_t)1 << 31 && p.score_bytes <= kMostScores;
+  if (!p.direct) {
+    p.before = make_plan(a).total();
+    p.values = 2 * up256((size_t)units * a.capacity * a.dim * (a.dtype == SV_F32 ? 4 : 2));
+  }
+  return p;
 }
 
 AttnArgs base_args(int32_t dtype, int32_t rows, int32_t tokens, int32_t heads, int32_t kv_heads, int32_t head_dim,
@@ -276,7 +302,7 @@ size_t sv_quantized_attention_workspace_bytes(int32_t dtype, int32_t rows, int32
   if (check_shapes(a)) return 0;
   float dummy;
   a.weights = with_weights ? &dummy : nullptr;
-  return make_plan(a).total() + read_bytes(a);
+  return record_plan(a).total();
 }
 
 int sv_quantized_attention(const void* q, int32_t dtype, int32_t rows, int32_t tokens, int32_t heads, int32_t kv_heads,
@@ -307,23 +333,45 @@ int sv_quantized_attention(const void* q, int32_t dtype, int32_t rows, int32_t t
   if (cache_stride_row < 0 || cache_stride_head < 0 || cache_stride_slot < 0 || (capacity > 1 && cache_stride_slot == 0))
     return SV_E_SHAPE;
   if (cache_stride_row % 16 || cache_stride_head % 16 || cache_stride_slot % 16) return SV_E_ALIGN;
-  // The values that the records stand for, of the slots that some query sees.
-  a.kv_slot = head_dim;
-  a.kv_head = (int64_t)capacity * head_dim;
-  a.kv_row = kv_heads * a.kv_head;
+  const RecordPlan p = record_plan(a);
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  unsigned char* w = static_cast<unsigned char*>(workspace);
+  if (p.direct) {
+    // The queries' and the output's checks; the records' strides are bytes.
+    a.kv_row = cache_stride_row;
+    a.kv_head = cache_stride_head;
+    a.kv_slot = cache_stride_slot;
+  } else {
+    a.kv_slot = head_dim;
+    a.kv_head = (int64_t)capacity * head_dim;
+    a.kv_row = kv_heads * a.kv_head;
+  }
   rc = check_pointers(a, scale);
   if (rc) return rc;
-  const size_t before = make_plan(a).total(), bytes = read_bytes(a);
-  if (!workspace || workspace_bytes < before + bytes) return SV_E_WORKSPACE;
-  unsigned char* values = static_cast<unsigned char*>(workspace) + before;
+  if (!workspace || workspace_bytes < p.total()) return SV_E_WORKSPACE;
+  if (reinterpret_cast<uintptr_t>(workspace) % 16) return SV_E_ALIGN;
+  if (p.direct) {
+    auto take = [&](size_t bytes) {
+      unsigned char* at = w;
+      w += bytes;
+      return bytes ? at : nullptr;
+    };
+    a.counters = reinterpret_cast<unsigned*>(take(p.counters));
+    a.part_o = reinterpret_cast<float*>(take(p.o_bytes));
+    a.part_ml = reinterpret_cast<float2*>(take(p.ml_bytes));
+    a.lse = reinterpret_cast<float*>(take(p.lse_bytes));
+    a.scores = reinterpret_cast<float*>(take(p.score_bytes));
+    if (launch_attn_record(a, p.rows, s) != cudaSuccess) return SV_E_CUDA;
+    return a.weights && launch_scores_weights(a, s) != cudaSuccess ? SV_E_CUDA : SV_OK;
+  }
   ReadArgs x = {};
   x.cache[0] = static_cast<const unsigned char*>(cache_keys);
   x.cache[1] = static_cast<const unsigned char*>(cache_values);
   x.row = cache_stride_row;
   x.head = cache_stride_head;
   x.slot = cache_stride_slot;
-  a.k = x.out[0] = values;
-  a.v = x.out[1] = values + bytes / 2;
+  a.k = x.out[0] = w + p.before;
+  a.v = x.out[1] = w + p.before + p.values / 2;
   x.lengths = lengths;
   x.starts = starts;
   x.dtype = dtype;
@@ -334,9 +382,8 @@ int sv_quantized_attention(const void* q, int32_t dtype, int32_t rows, int32_t t
   x.seen = tokens;
   x.window = a.window;
   x.sinks = a.sinks;
-  cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (launch_read_records(x, s) != cudaSuccess) return SV_E_CUDA;
-  return run(a, workspace, before, s);
+  return run(a, workspace, p.before, s);
 }
 
 size_t sv_prefix_attention_workspace_bytes(int32_t dtype, int32_t rows, int32_t tokens, int32_t heads,

@@ -491,7 +491,7 @@ std::tuple<int, at::Tensor> quantized_attention(const at::Tensor& q_in, const at
   }
   const size_t bytes =
       sv_quantized_attention_workspace_bytes(code, rows, n, heads, kv, dim, capacity, w, s, weights.has_value());
-  at::Tensor ws = workspace_for(dev, stream, bytes, 4 * ((size_t)rows * kv + 1024));
+  at::Tensor ws = workspace_for(dev, stream, bytes, 4 * ((size_t)rows * kv * 4 + 1024));
   const int rc = sv_quantized_attention(
       q.data_ptr(), code, rows, n, heads, kv, dim, stride_of(q, 0), stride_of(q, 1), stride_of(q, 2), ck.data_ptr(),
       cv.data_ptr(), capacity, stride_of(ck, 0), stride_of(ck, 1), stride_of(ck, 2),
