@@ -9,11 +9,12 @@
 // of a word is, read as float16, its subnormal c 2^-24 (or, four bits further up, c 2^-20:
 // those dimensions' queries are divided by 16), so a key needs no arithmetic before the
 // tensor core takes it.  The queries are brought into float16's upper range by a power of two
-// per row, which loses nothing of a bfloat16.  The -8 is the products' initial value, the scales
-// multiply the groups' sums in f32, the mids are a last product with the queries' group sums
-// (in two halves).  So scores are as exact as those of f32 keys.  Values are formed in
-// float16, v = scale (c - 8) + mid rounded once, and weights rounded once to float16; both are
-// below the rounding of a bfloat16 output, and next to a float16 one's.
+// per row, which loses nothing of a bfloat16.  The scales multiply the groups' sums in f32; the rest,
+// sum_g (mid_g - 8 scale_g) times the queries' group sums, is one product more, whose A operand is the
+// record's pairs as they lie (the group sums in two halves).  So scores are as exact as those of f32 keys.
+// Values are formed in float16, v = scale (c - 8) + mid rounded once, and the weights rounded to
+// float16, for float16 outputs in two halves: one such rounding is about what the output's own adds (error of
+// one token's output 0.0003 against 64 bits, 0.0002 that of the output's rounding alone; with both 0.00032).
 // The softmax as in sv_attention_token.cu: the reference moves only when a score exceeds it by
 // 2^8.
 //
@@ -54,20 +55,21 @@ __device__ __forceinline__ uint32_t pack16(float lo, float hi) {
   const __half2 h = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&h);
 }
-__device__ __forceinline__ void mma16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
-                                      uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+// d = a b + c; d = a b.
+__device__ __forceinline__ void mma16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                      uint32_t b1, const float (&c)[4]) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
 }
-__device__ __forceinline__ void mma8(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t b0) {
-  asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5}, {%6}, {%0,%1,%2,%3};"
-               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-               : "r"(a0), "r"(a1), "r"(b0));
+__device__ __forceinline__ void mma16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                      uint32_t b1) {
+  const float zero[4] = {0.f, 0.f, 0.f, 0.f};
+  mma16(d, a0, a1, a2, a3, b0, b1, zero);
 }
 __device__ __forceinline__ uint32_t transposed(uint32_t x) {
   uint32_t y;
-  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
   return y;
 }
 __device__ __forceinline__ uint32_t fma16(uint32_t a, uint32_t b, uint32_t c) {
@@ -80,7 +82,10 @@ __device__ __forceinline__ uint32_t add16(uint32_t a, uint32_t b) {
   asm("add.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
   return d;
 }
-__device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool ok) {
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void copy16_or_zeros(uint32_t dst, const void* src, bool ok) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(ok ? 16 : 0) : "memory");
 }
 __device__ __forceinline__ unsigned arrive(unsigned* counter) {
@@ -134,12 +139,15 @@ template <int NW> struct Place {
     rt = row_tiles(a, r_);
     chunks = (rt.tiles + NW - 1) / NW;
   }
-  __device__ __forceinline__ void next(const AttnArgs& a, int heads) {
-    if (++k < chunks) return;
+  // Whether the next place is another unit's.
+  __device__ __forceinline__ bool next(const AttnArgs& a, int heads) {
+    if (++k < chunks) return false;
     k = 0;
-    if (++h < heads) return;
-    h = 0;
-    if (r + 1 < a.rows) row(a, r + 1);  // (past the last chunk of all nothing is looked at)
+    if (++h == heads) {
+      h = 0;
+      if (r + 1 < a.rows) row(a, r + 1);  // (past the last chunk of all nothing is looked at)
+    }
+    return true;
   }
 };
 
@@ -151,6 +159,8 @@ __global__ void __launch_bounds__(NW * 32, 1)
   using F = Form<NI>;
   constexpr int REC = F::REC, NG = F::NG, NB = F::NB, MT = 4 * NB, ROWS = 8 * NT, THREADS = NW * 32;
   constexpr int OS = 32 * NI;  // dimensions of the warps' outputs
+  constexpr bool HALVES = std::is_same<T, __half>::value;
+  constexpr uint32_t kOnes = 0x3c003c00u;
   extern __shared__ __align__(16) unsigned char ring_bytes[];  // [NW][RING][keys, values], then [NW][ROWS][OS] floats
   float* const outs = reinterpret_cast<float*>(ring_bytes + NW * RING * 2 * F::TILE);
   __shared__ float2 warp_ml[NW][ROWS];
@@ -218,7 +228,15 @@ __global__ void __launch_bounds__(NW * 32, 1)
   // ---- copies: this warp's tile of chunk f, the f-th place ahead
   Place<NW> f = p;
   int fetched = c0;
+  const unsigned char *fk, *fv;  // its unit's records
+  auto open = [&]() {
+    const int64_t base = f.r * a.kv_row + (f.h / row_groups) * a.kv_head;
+    fk = static_cast<const unsigned char*>(a.k) + base;
+    fv = static_cast<const unsigned char*>(a.v) + base;
+  };
+  open();
   const uint32_t ring = (uint32_t)__cvta_generic_to_shared(ring_bytes) + warp * RING * 2 * F::TILE;
+  uint32_t put = ring + lane * 16;
   const bool dense = a.kv_slot == REC;
   auto fetch = [&]() {
     if (fetched < c1) {
@@ -226,31 +244,33 @@ __global__ void __launch_bounds__(NW * 32, 1)
       const bool in_a = tile < f.rt.ta;
       const int j0 = in_a ? f.rt.a0 + tile * TK : f.rt.b0 + (tile - f.rt.ta) * TK;
       const int count = tile < f.rt.tiles ? min(TK, (in_a ? f.rt.a1 : f.rt.b1) - j0) : 0;
-      if (count > 0) {
-        const int64_t base = f.r * a.kv_row + (f.h / row_groups) * a.kv_head + j0 * a.kv_slot;
-        const unsigned char* kb = static_cast<const unsigned char*>(a.k) + base;
-        const unsigned char* vb = static_cast<const unsigned char*>(a.v) + base;
-        const uint32_t dst = ring + (fetched - c0) % RING * 2 * F::TILE;
+      const int64_t off = j0 * a.kv_slot;
+      if (dense && count == TK) {  // a run of bytes each
+        const unsigned char *kb = fk + off + lane * 16, *vb = fv + off + lane * 16 - F::TILE;
 #pragma unroll
         for (int x = 0; x < F::COPIES; ++x) {
-          const int at = lane + 32 * x;
-          const bool is_v = at >= F::TILE / 16;
-          const int in = is_v ? at - F::TILE / 16 : at, slot = in / (REC / 16);
-          const int64_t off = dense ? (int64_t)in * 16 : slot * a.kv_slot + (in - slot * (REC / 16)) * 16;
-          const bool ok = slot < count;
-          copy16(dst + at * 16, (is_v ? vb : kb) + (ok ? off : 0), ok);
+          constexpr int K = F::TILE / 16;  // copies of keys
+          const unsigned char* src = 32 * x + 32 <= K ? kb : 32 * x >= K ? vb : lane + 32 * x < K ? kb : vb;
+          copy16(put + x * 512, src + x * 512);
+        }
+      } else if (count > 0) {
+#pragma unroll 1
+        for (int x = lane; x < 2 * F::TILE / 16; x += 32) {
+          const int in = x >= F::TILE / 16 ? x - F::TILE / 16 : x, slot = in / (REC / 16);
+          const int64_t at = off + slot * a.kv_slot + (in - slot * (REC / 16)) * 16;
+          copy16_or_zeros(put + (x - lane) * 16, (x == in ? fk : fv) + (slot < count ? at : 0), slot < count);
         }
       }
+      put = put + 2 * F::TILE == ring + lane * 16 + RING * 2 * F::TILE ? ring + lane * 16 : put + 2 * F::TILE;
       ++fetched;
-      f.next(a, K);
+      if (f.next(a, K)) open();
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
 
-  // ---- queries: the B operand of each step over 16 dimensions, the groups' initial values and
-  // their sums' halves, the rows' factors
-  uint32_t qb[NT][NI][2][2], qm[NT];
-  float qi[NT][NG][2], fr[NT][2];
+  // ---- queries: the B operand of each step over 16 dimensions, the groups' sums in halves, the rows' factors
+  uint32_t qb[NT][NI][2][2], qm[NT][2];
+  float fr[NT][2];
   auto load_q = [&](int r, int h) {
     const int head = h / row_groups, m0 = (h - head * row_groups) * ROWS;
 #pragma unroll
@@ -276,7 +296,7 @@ __global__ void __launch_bounds__(NW * 32, 1)
       most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
       // The row's largest value to [2^14, 2^15).
       const int ex = max(15, (int)(__float_as_uint(most) >> 23));
-      const float up = __uint_as_float((uint32_t)(268 - min(ex, 254)) << 23);
+      const float up = copysignf(__uint_as_float((uint32_t)(268 - min(ex, 254)) << 23), a.scale);
       float sum[NG];
 #pragma unroll
       for (int k = 0; k < NG; ++k) sum[k] = 0.f;
@@ -292,22 +312,20 @@ __global__ void __launch_bounds__(NW * 32, 1)
           qb[u][b][e][0] = pack16(x[b][e][0], x[b][e][1]);
           qb[u][b][e][1] = pack16(x[b][e][2] * 0.0625f, x[b][e][3] * 0.0625f);
         }
-      float part[4] = {0.f, 0.f, 0.f, 0.f};
+      // Group t's sum, in the keys' units; in halves, for scale (times -8) and mid.
+      float own = 0.f;
 #pragma unroll
       for (int k = 0; k < NG; ++k) {
         sum[k] += __shfl_xor_sync(0xffffffffu, sum[k], 1);
         sum[k] += __shfl_xor_sync(0xffffffffu, sum[k], 2);
-        // Of rows 2 t and 2 t + 1, from the lanes that have them as g.
-#pragma unroll
-        for (int y = 0; y < 2; ++y)
-          qi[u][k][y] = -0x1p-21f * __shfl_sync(0xffffffffu, sum[k], 8 * t + 4 * y);
-        part[k] = sum[k] * 0x1p-6f;
+        if (k == t) own = sum[k] * 0x1p-24f;
       }
-      const float pa = t & 1 ? part[2] : part[0], pb = t & 1 ? part[3] : part[1];
-      const float ha = __half2float(__float2half_rn(pa)), hb = __half2float(__float2half_rn(pb));
-      qm[u] = t < 2 ? pack16(ha, hb) : pack16(pa - ha, pb - hb);
-      // (Scores past f32's range stay within it by a smaller factor: any of them is the whole softmax.)
-      const float mine = a.scale * __uint_as_float((uint32_t)(min(ex, 230) + 10) << 23);  // 2^(ex - 141 + 24)
+      const float high = __half2float(__float2half_rn(own));
+      qm[u][0] = pack16(-8.f * high, high);
+      qm[u][1] = pack16(-8.f * (own - high), own - high);
+      // (Scores past f32's range stay within it by a smaller factor: any of them is the whole softmax.  A
+      // factor of zero would make NaN of hidden slots' -infinity.)
+      const float mine = fmaxf(fabsf(a.scale) * __uint_as_float((uint32_t)(min(ex, 230) + 10) << 23), 0x1p-126f);  // 2^(ex - 141 + 24)
 #pragma unroll
       for (int y = 0; y < 2; ++y) fr[u][y] = __shfl_sync(0xffffffffu, mine, 8 * t + 4 * y);
     }
@@ -334,17 +352,21 @@ __global__ void __launch_bounds__(NW * 32, 1)
 #pragma unroll
   for (int k = 0; k < RING - 1; ++k) fetch();
   int at = c0;
+  uint32_t get = ring;
   for (;;) {  // units
     load_q(p.r, p.h);
     const int head = p.h / row_groups, m0 = (p.h - head * row_groups) * ROWS, rows_here = min(ROWS, nG - m0);
     const int first = before * K + p.h * p.chunks, end = first + p.chunks, stop = min(end, c1);
     const RowTiles rt = p.rt;
     const int pos_first = rt.end - a.n, low_last = window_low(a, rt.start, rt.end - 1);
-    float o[NT][MT][4], ref[NT][2], l[NT][2];
+    // ref: a row's reference; edge: the raw score past which it moves.
+    float o[NT][MT][4], ref[NT][2], edge[NT][2], l[NT][4];
 #pragma unroll
     for (int u = 0; u < NT; ++u) {
 #pragma unroll
-      for (int y = 0; y < 2; ++y) ref[u][y] = -INFINITY, l[u][y] = 0.f;
+      for (int y = 0; y < 2; ++y) ref[u][y] = edge[u][y] = -INFINITY;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) l[u][k] = 0.f;
 #pragma unroll
       for (int j = 0; j < MT; ++j)
 #pragma unroll
@@ -352,7 +374,8 @@ __global__ void __launch_bounds__(NW * 32, 1)
     }
     for (; at < stop; ++at) {
       const int tile = (at - first) * NW + warp;
-      const uint32_t kt = ring + (at - c0) % RING * 2 * F::TILE, vt = kt + F::TILE;
+      const uint32_t kt = get, vt = kt + F::TILE;
+      get = get + 2 * F::TILE == ring + RING * 2 * F::TILE ? ring : get + 2 * F::TILE;
       asm volatile("cp.async.wait_group %0;" ::"n"(RING - 2) : "memory");
       __syncwarp();
       fetch();  // into the place that the last round has left
@@ -361,9 +384,9 @@ __global__ void __launch_bounds__(NW * 32, 1)
       if (tile >= rt.tiles || j0 >= jend) continue;
       // ---- scores
       const int s0 = slot_at(g), s1 = slot_at(g + 8);
-      float s[NT][2][2];  // slots s0 and s1, rows 2 t and 2 t + 1
+      float s[NT][4];  // slots s0 and s1 of rows 2 t and 2 t + 1, in units of 1 / fr
       {
-        uint32_t kw[2][NI], pr[2][4];
+        uint32_t kw[2][NI], pr[2][4], own[2];
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
           const uint32_t rec = kt + (x ? s1 : s0) * REC;
@@ -376,50 +399,36 @@ __global__ void __launch_bounds__(NW * 32, 1)
             for (int b = 0; b < NI; ++b) asm volatile("ld.shared.u32 %0, [%1];" : "=r"(kw[x][b]) : "r"(rec + (t * NI + b) * 4));
           }
           asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(pr[x][0]), "=r"(pr[x][1]), "=r"(pr[x][2]), "=r"(pr[x][3]) : "r"(rec + 16 * NI));
+          asm volatile("ld.shared.u32 %0, [%1];" : "=r"(own[x]) : "r"(rec + 16 * NI + 4 * t));
         }
-        float acc[NT][4];
 #pragma unroll
-        for (int u = 0; u < NT; ++u) {
-#pragma unroll
-          for (int k = 0; k < 4; ++k) acc[u][k] = 0.f;
-          mma8(acc[u], __byte_perm(t & 1 ? pr[0][2] : pr[0][0], t & 1 ? pr[0][3] : pr[0][1], 0x7632),
-               __byte_perm(t & 1 ? pr[1][2] : pr[1][0], t & 1 ? pr[1][3] : pr[1][1], 0x7632), qm[u]);
-#pragma unroll
-          for (int x = 0; x < 2; ++x)
-#pragma unroll
-            for (int y = 0; y < 2; ++y) s[u][x][y] = acc[u][2 * x + y] * 0x1p-18f;
-        }
+        for (int u = 0; u < NT; ++u) mma16(s[u], own[0], own[1], own[0], own[1], qm[u][0], qm[u][1]);
 #pragma unroll
         for (int grp = 0; grp < NG; ++grp) {
-#pragma unroll
-          for (int u = 0; u < NT; ++u)
-#pragma unroll
-            for (int k = 0; k < 4; ++k) acc[u][k] = qi[u][grp][k & 1];
+          float acc[NT][4];
 #pragma unroll
           for (int e = NI > 2 ? 0 : grp & 1; e < (NI > 2 ? 2 : (grp & 1) + 1); ++e) {
             const int b = NI > 2 ? grp : grp >> 1;
             const uint32_t w0 = e ? kw[0][b] >> 8 : kw[0][b], w1 = e ? kw[1][b] >> 8 : kw[1][b];
 #pragma unroll
-            for (int u = 0; u < NT; ++u)
-              mma16(acc[u], w0 & 0x000f000fu, w1 & 0x000f000fu, w0 & 0x00f000f0u, w1 & 0x00f000f0u, qb[u][b][e][0], qb[u][b][e][1]);
+            for (int u = 0; u < NT; ++u) {
+              if (NI > 2 && e)
+                mma16(acc[u], w0 & 0x000f000fu, w1 & 0x000f000fu, w0 & 0x00f000f0u, w1 & 0x00f000f0u, qb[u][b][e][0], qb[u][b][e][1], acc[u]);
+              else
+                mma16(acc[u], w0 & 0x000f000fu, w1 & 0x000f000fu, w0 & 0x00f000f0u, w1 & 0x00f000f0u, qb[u][b][e][0], qb[u][b][e][1]);
+            }
           }
 #pragma unroll
           for (int x = 0; x < 2; ++x) {
-            const float sc = __half2float(__ushort_as_half((unsigned short)(pr[x][grp] & 0xffffu)));
+            const float sc = __low2float(*reinterpret_cast<const __half2*>(&pr[x][grp]));
 #pragma unroll
             for (int u = 0; u < NT; ++u)
 #pragma unroll
-              for (int y = 0; y < 2; ++y) s[u][x][y] = fmaf(sc, acc[u][2 * x + y], s[u][x][y]);
+              for (int y = 0; y < 2; ++y) s[u][2 * x + y] = fmaf(sc, acc[u][2 * x + y], s[u][2 * x + y]);
           }
         }
       }
       const bool whole = j0 + TK <= jend && (in_a || !MULTI || (j0 >= low_last && j0 + TK - 1 <= pos_first));
-#pragma unroll
-      for (int u = 0; u < NT; ++u)
-#pragma unroll
-        for (int x = 0; x < 2; ++x)
-#pragma unroll
-          for (int y = 0; y < 2; ++y) s[u][x][y] *= fr[u][y];
       if (!whole) {
 #pragma unroll
         for (int u = 0; u < NT; ++u)
@@ -430,7 +439,7 @@ __global__ void __launch_bounds__(NW * 32, 1)
 #pragma unroll
             for (int x = 0; x < 2; ++x) {
               const int j = j0 + (x ? s1 : s0);
-              if (j >= jend || !slot_seen(a, rt.start, pos, low, j)) s[u][x][y] = -INFINITY;
+              if (j >= jend || !slot_seen(a, rt.start, pos, low, j)) s[u][2 * x + y] = -INFINITY;
             }
           }
       }
@@ -443,7 +452,7 @@ __global__ void __launch_bounds__(NW * 32, 1)
             for (int y = 0; y < 2; ++y) {
               const int j = j0 + (x ? s1 : s0), m = 8 * u + 2 * t + y;
               if (j < jend && m < rows_here)
-                a.scores[((int64_t)(p.r * a.kv_heads + head) * nG + m0 + m) * a.capacity + j] = s[u][x][y];
+                a.scores[((int64_t)(p.r * a.kv_heads + head) * nG + m0 + m) * a.capacity + j] = s[u][2 * x + y] * fr[u][y];
             }
       }
       // ---- weights
@@ -451,19 +460,21 @@ __global__ void __launch_bounds__(NW * 32, 1)
 #pragma unroll
       for (int u = 0; u < NT; ++u)
 #pragma unroll
-        for (int y = 0; y < 2; ++y) over |= fmaxf(s[u][0][y], s[u][1][y]) > ref[u][y] + kSlack;
+        for (int y = 0; y < 2; ++y) over |= fmaxf(s[u][y], s[u][2 + y]) > edge[u][y];
       if (__any_sync(0xffffffffu, over)) {
 #pragma unroll
         for (int u = 0; u < NT; ++u)
 #pragma unroll
           for (int y = 0; y < 2; ++y) {
-            float mx = fmaxf(s[u][0][y], s[u][1][y]);
+            float mx = fmaxf(s[u][y], s[u][2 + y]);
 #pragma unroll
             for (int k = 4; k < 32; k <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, k));
-            const float now = fmaxf(mx, ref[u][y]);
+            const float now = fmaxf(mx * fr[u][y], ref[u][y]);
             const float by = now == ref[u][y] ? 1.f : ex2(ref[u][y] - now);
             ref[u][y] = now;
+            edge[u][y] = now == -INFINITY ? -INFINITY : (now + kSlack) / fr[u][y];
             l[u][y] *= by;
+            l[u][2 + y] *= by;
 #pragma unroll
             for (int j = 0; j < MT; ++j) {
               o[u][j][y] *= by;
@@ -471,19 +482,26 @@ __global__ void __launch_bounds__(NW * 32, 1)
             }
           }
       }
-      uint32_t pb[NT][2];  // weights as B operand: slots rows 0..7 and 8..15 of the tile's order
+      // Weights as B operand: slots of rows 0..7 and 8..15 of the tile's order; their sums are a product with ones.
+      uint32_t pb[NT][2];
+      [[maybe_unused]] uint32_t pl[NT][2];  // float16 outputs: what the rounding left
 #pragma unroll
-      for (int u = 0; u < NT; ++u)
+      for (int u = 0; u < NT; ++u) {
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
           float w[2];
 #pragma unroll
-          for (int y = 0; y < 2; ++y) {
-            w[y] = ex2(s[u][x][y] - (ref[u][y] == -INFINITY ? 0.f : ref[u][y]));
-            l[u][y] += w[y];
+          for (int y = 0; y < 2; ++y) w[y] = ex2(fmaf(s[u][2 * x + y], fr[u][y], -(ref[u][y] == -INFINITY ? 0.f : ref[u][y])));
+          const uint32_t both = pack16(w[0], w[1]);
+          pb[u][x] = transposed(both);
+          if constexpr (HALVES) {
+            const float2 high = __half22float2(*reinterpret_cast<const __half2*>(&both));
+            pl[u][x] = transposed(pack16(w[0] - high.x, w[1] - high.y));
           }
-          pb[u][x] = transposed(pack16(w[0], w[1]));
         }
+        mma16(l[u], kOnes, kOnes, kOnes, kOnes, pb[u][0], pb[u][1], l[u]);
+        if constexpr (HALVES) mma16(l[u], kOnes, kOnes, kOnes, kOnes, pl[u][0], pl[u][1], l[u]);
+      }
       // ---- values
       {
         const int va = slot_at(2 * t), vb = slot_at(2 * t + 1);  // and each + 1 in rows 8..15
@@ -553,7 +571,10 @@ __global__ void __launch_bounds__(NW * 32, 1)
             const uint32_t a0 = value(l0, j, sc[0][k], mi[0][k]), a1 = value(h0, j, sc[0][k], mi[0][k]);
             const uint32_t a2 = value(l1, j, sc[1][k], mi[1][k]), a3 = value(h1, j, sc[1][k], mi[1][k]);
 #pragma unroll
-            for (int u = 0; u < NT; ++u) mma16(o[u][4 * b + j], a0, a1, a2, a3, pb[u][0], pb[u][1]);
+            for (int u = 0; u < NT; ++u) {
+              mma16(o[u][4 * b + j], a0, a1, a2, a3, pb[u][0], pb[u][1], o[u][4 * b + j]);
+              if constexpr (HALVES) mma16(o[u][4 * b + j], a0, a1, a2, a3, pl[u][0], pl[u][1], o[u][4 * b + j]);
+            }
           }
         }
         if (MULTI && hide) {
@@ -565,7 +586,7 @@ __global__ void __launch_bounds__(NW * 32, 1)
               const uint32_t x = bad[0][k] & 0x3c003c00u, z = bad[1][k] & 0x3c003c00u;
 #pragma unroll
               for (int u = 0; u < NT; ++u) {
-                float seen[4] = {0.f, 0.f, 0.f, 0.f};
+                float seen[4];
                 mma16(seen, x, x, z, z, pb[u][0], pb[u][1]);
 #pragma unroll
                 for (int q = 0; q < 4; ++q)
@@ -581,8 +602,6 @@ __global__ void __launch_bounds__(NW * 32, 1)
     for (int u = 0; u < NT; ++u) {
 #pragma unroll
       for (int y = 0; y < 2; ++y) {
-#pragma unroll
-        for (int k = 4; k < 32; k <<= 1) l[u][y] += __shfl_xor_sync(0xffffffffu, l[u][y], k);
         const int m = 8 * u + 2 * t + y;
         if (g == 0) warp_ml[warp][m] = make_float2(ref[u][y], l[u][y]);
 #pragma unroll
