@@ -33,6 +33,7 @@
 // Work split and joins as in sv_attention_token.cu: one list of chunks (a tile per warp) over all
 // units, cut into equal parts, one per block; the last block to arrive joins a unit that
 // several share, in block order.
+#include <climits>
 #include <type_traits>
 
 #include "sv_attention.h"
@@ -45,6 +46,7 @@ constexpr int TK = 16;         // slots per tile
 constexpr int kJoin = 16;      // parts per first-level group
 constexpr int kMaxFlat = 32;   // parts joined in one level
 constexpr float kSlack = 8.f;  // log2 by which a score may exceed its reference
+constexpr float kNever = -1e30f;  // a reference before the first score
 
 __device__ __forceinline__ float ex2(float x) {
   float y;
@@ -55,17 +57,18 @@ __device__ __forceinline__ uint32_t pack16(float lo, float hi) {
   const __half2 h = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&h);
 }
-// d = a b + c; d = a b.
-__device__ __forceinline__ void mma16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
-                                      uint32_t b1, const float (&c)[4]) {
-  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
+// d = a b; d += a b.
+__device__ __forceinline__ void mma_new(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                        uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
       : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
-      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
 }
-__device__ __forceinline__ void mma16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
-                                      uint32_t b1) {
-  const float zero[4] = {0.f, 0.f, 0.f, 0.f};
-  mma16(d, a0, a1, a2, a3, b0, b1, zero);
+__device__ __forceinline__ void mma_add(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                        uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ uint32_t transposed(uint32_t x) {
   uint32_t y;
@@ -82,11 +85,34 @@ __device__ __forceinline__ uint32_t add16(uint32_t a, uint32_t b) {
   asm("add.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
   return d;
 }
+// (a & b) | c as one instruction: b and c in registers whose values the compiler does not see (as
+// immediates they would take an instruction each).
+__device__ __forceinline__ uint32_t and_or(uint32_t a, uint32_t b, uint32_t c) {
+  uint32_t d;
+  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
+  return d;
+}
+__device__ __forceinline__ uint32_t hidden(uint32_t x) {
+  uint32_t y;
+  asm volatile("mov.u32 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
 __device__ __forceinline__ void copy16(uint32_t dst, const void* src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
 __device__ __forceinline__ void copy16_or_zeros(uint32_t dst, const void* src, bool ok) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(ok ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ uint32_t load1(uint32_t at) {
+  uint32_t x;
+  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(x) : "r"(at));
+  return x;
+}
+template <int N> __device__ __forceinline__ void load2(uint32_t (&x)[N], uint32_t at) {
+  asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(x[0]), "=r"(x[1]) : "r"(at));
+}
+__device__ __forceinline__ void load4(uint32_t (&x)[4], uint32_t at) {
+  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3]) : "r"(at));
 }
 __device__ __forceinline__ unsigned arrive(unsigned* counter) {
   unsigned old;
@@ -108,8 +134,8 @@ template <int NI> struct Form {
   static constexpr int NG = NI > 2 ? NI : 2 * NI;             // groups
   static constexpr int NB = NI > 2 ? 2 : 1;                   // words of a value that one thread turns into operands
   static constexpr int TILE = TK * REC;                       // bytes of a tile's keys (or values)
-  static constexpr int COPIES = 2 * TILE / 512;               // 16-byte copies per thread and tile
 };
+
 
 // Like sv_attention_token.cu's: [a0, a1) the sinks before the window, [b0, b1) the rest.
 struct RowTiles {
@@ -139,19 +165,9 @@ template <int NW> struct Place {
     rt = row_tiles(a, r_);
     chunks = (rt.tiles + NW - 1) / NW;
   }
-  // Whether the next place is another unit's.
-  __device__ __forceinline__ bool next(const AttnArgs& a, int heads) {
-    if (++k < chunks) return false;
-    k = 0;
-    if (++h == heads) {
-      h = 0;
-      if (r + 1 < a.rows) row(a, r + 1);  // (past the last chunk of all nothing is looked at)
-    }
-    return true;
-  }
 };
 
-// NI blocks of 32 dimensions, NT column tiles of eight query rows, NW warps, a ring of RING tiles.
+// NI blocks of 32 dimensions, NT column tiles of eight query rows, NW warps, rings of RING tiles.
 // MULTI: more than one query per row.
 template <typename T, int NI, int NT, int NW, int RING, bool MULTI>
 __global__ void __launch_bounds__(NW * 32, 1)
@@ -160,13 +176,18 @@ __global__ void __launch_bounds__(NW * 32, 1)
   constexpr int REC = F::REC, NG = F::NG, NB = F::NB, MT = 4 * NB, ROWS = 8 * NT, THREADS = NW * 32;
   constexpr int OS = 32 * NI;  // dimensions of the warps' outputs
   constexpr bool HALVES = std::is_same<T, __half>::value;
+  constexpr bool KEEP_Q = NT * NW <= 16;  // the queries' operands in registers
   constexpr uint32_t kOnes = 0x3c003c00u;
-  extern __shared__ __align__(16) unsigned char ring_bytes[];  // [NW][RING][keys, values], then [NW][ROWS][OS] floats
+  // [NW][RING][keys, values of a tile], then [NW][ROWS][OS] floats.
+  extern __shared__ __align__(16) unsigned char ring_bytes[];
   float* const outs = reinterpret_cast<float*>(ring_bytes + NW * RING * 2 * F::TILE);
-  __shared__ float2 warp_ml[NW][ROWS];
+  __shared__ float warp_m[NW][ROWS], warp_l[NW][ROWS];
   __shared__ float factor[kMaxFlat > NW ? kMaxFlat : NW][ROWS];
   __shared__ float2 part_ml[kMaxFlat][ROWS];
   __shared__ float2 joined[ROWS];
+  __shared__ uint4 sh_q[NT][NI][32];
+  __shared__ uint2 sh_qm[NT][32];
+  __shared__ float sh_fr[ROWS];
   __shared__ int scan[NW];
   __shared__ int sh_row, sh_before, sh_last[2];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
@@ -225,110 +246,133 @@ __global__ void __launch_bounds__(NW * 32, 1)
   }
   int before = sh_before;  // chunks (of one head) before row p.r
 
-  // ---- copies: this warp's tile of chunk f, the f-th place ahead
+  // ---- copies: this warp's tile of chunk f, the f-th place ahead.  The next `runs` of them are whole
+  // tiles of one unit, each a run of bytes f_step behind the one before.
   Place<NW> f = p;
-  int fetched = c0;
-  const unsigned char *fk, *fv;  // its unit's records
-  auto open = [&]() {
-    const int64_t base = f.r * a.kv_row + (f.h / row_groups) * a.kv_head;
-    fk = static_cast<const unsigned char*>(a.k) + base;
-    fv = static_cast<const unsigned char*>(a.v) + base;
-  };
-  open();
+  int f_left = c1 - c0, runs = 0;
+  const unsigned char *f_k, *f_v;
+  const int64_t f_step = (int64_t)NW * TK * a.kv_slot;
   const uint32_t ring = (uint32_t)__cvta_generic_to_shared(ring_bytes) + warp * RING * 2 * F::TILE;
   uint32_t put = ring + lane * 16;
-  const bool dense = a.kv_slot == REC;
-  auto fetch = [&]() {
-    if (fetched < c1) {
-      const int tile = f.k * NW + warp;
+  // The place f by slots (the end of a unit, sinks, other strides), or none; then what comes after it.
+  auto fetch_slots = [&]() {
+    if (f_left <= 0) return;
+    const int tile = f.k * NW + warp, f_hi = f.rt.ta + (f.rt.b1 - f.rt.b0) / TK;
+    const int64_t base = f.r * a.kv_row + (f.h / row_groups) * a.kv_head;
+    if (tile < f.rt.tiles) {
       const bool in_a = tile < f.rt.ta;
       const int j0 = in_a ? f.rt.a0 + tile * TK : f.rt.b0 + (tile - f.rt.ta) * TK;
-      const int count = tile < f.rt.tiles ? min(TK, (in_a ? f.rt.a1 : f.rt.b1) - j0) : 0;
-      const int64_t off = j0 * a.kv_slot;
-      if (dense && count == TK) {  // a run of bytes each
-        const unsigned char *kb = fk + off + lane * 16, *vb = fv + off + lane * 16 - F::TILE;
-#pragma unroll
-        for (int x = 0; x < F::COPIES; ++x) {
-          constexpr int K = F::TILE / 16;  // copies of keys
-          const unsigned char* src = 32 * x + 32 <= K ? kb : 32 * x >= K ? vb : lane + 32 * x < K ? kb : vb;
-          copy16(put + x * 512, src + x * 512);
-        }
-      } else if (count > 0) {
+      const int count = min(TK, (in_a ? f.rt.a1 : f.rt.b1) - j0);
 #pragma unroll 1
-        for (int x = lane; x < 2 * F::TILE / 16; x += 32) {
-          const int in = x >= F::TILE / 16 ? x - F::TILE / 16 : x, slot = in / (REC / 16);
-          const int64_t at = off + slot * a.kv_slot + (in - slot * (REC / 16)) * 16;
-          copy16_or_zeros(put + (x - lane) * 16, (x == in ? fk : fv) + (slot < count ? at : 0), slot < count);
-        }
+      for (int x = lane; x < 2 * F::TILE / 16; x += 32) {
+        const int in = x >= F::TILE / 16 ? x - F::TILE / 16 : x, slot = in / (REC / 16);
+        const int64_t at = base + (j0 + slot) * a.kv_slot + (in - slot * (REC / 16)) * 16;
+        copy16_or_zeros(put + (x - lane) * 16, static_cast<const unsigned char*>(x == in ? a.k : a.v) + (slot < count ? at : 0),
+                        slot < count);
       }
-      put = put + 2 * F::TILE == ring + lane * 16 + RING * 2 * F::TILE ? ring + lane * 16 : put + 2 * F::TILE;
-      ++fetched;
-      if (f.next(a, K)) open();
     }
+    --f_left;
+    if (++f.k == f.chunks) {
+      f.k = 0;
+      if (++f.h == K) {
+        f.h = 0;
+        if (f.r + 1 < a.rows) f.row(a, f.r + 1);  // (past the last chunk of all nothing is looked at)
+      }
+    }
+  };
+  auto find_runs = [&]() {
+    runs = 0;
+    const int tile = f.k * NW + warp, f_hi = f.rt.ta + (f.rt.b1 - f.rt.b0) / TK;
+    if (f_left <= 0 || a.kv_slot != REC || tile < f.rt.ta || tile >= f_hi) return;
+    // Not a unit's last chunk, after which the place moves on.
+    runs = min(min((f_hi - tile + NW - 1) / NW, f.chunks - 1 - f.k), f_left);
+    const int64_t at = f.r * a.kv_row + (f.h / row_groups) * a.kv_head + (f.rt.b0 + (tile - f.rt.ta) * TK) * a.kv_slot;
+    f_k = static_cast<const unsigned char*>(a.k) + at + lane * 16;
+    f_v = static_cast<const unsigned char*>(a.v) + at + lane * 16 - F::TILE;
+    f.k += runs;
+    f_left -= runs;
+  };
+  find_runs();
+  auto fetch = [&]() {
+    if (runs > 0) {
+#pragma unroll
+      for (int x = 0; x < 2 * F::TILE / 512; ++x) {
+        constexpr int K = F::TILE / 16;  // copies of keys
+        copy16(put + x * 512, (32 * x + 32 <= K || (32 * x < K && lane + 32 * x < K) ? f_k : f_v) + x * 512);
+      }
+      --runs;
+      f_k += f_step;
+      f_v += f_step;
+    } else {
+      fetch_slots();
+      find_runs();
+    }
+    put = put + 2 * F::TILE == ring + lane * 16 + RING * 2 * F::TILE ? ring + lane * 16 : put + 2 * F::TILE;
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
 
-  // ---- queries: the B operand of each step over 16 dimensions, the groups' sums in halves, the rows' factors
-  uint32_t qb[NT][NI][2][2], qm[NT][2];
-  float fr[NT][2];
+  // ---- queries, for the whole block, row tile u by warp u: the B operand of each step over 16 dimensions, the
+  // groups' sums in halves, the rows' factors
+  uint2 raw[NI][2];
   auto load_q = [&](int r, int h) {
-    const int head = h / row_groups, m0 = (h - head * row_groups) * ROWS;
+    const int head = h / row_groups, m = (h - head * row_groups) * ROWS + 8 * warp + g, i = MULTI ? m / group : 0;
+    const T* src = static_cast<const T*>(a.q) + r * a.q_row + i * a.q_tok + (int64_t)(head * group + m - i * group) * a.q_head;
 #pragma unroll
-    for (int u = 0; u < NT; ++u) {
-      const int m = m0 + 8 * u + g, i = MULTI ? m / group : 0;
-      const T* src = static_cast<const T*>(a.q) + r * a.q_row + i * a.q_tok + (int64_t)(head * group + m - i * group) * a.q_head;
-      float x[NI][2][4], most = 0.f;
+    for (int b = 0; b < NI; ++b)
 #pragma unroll
-      for (int b = 0; b < NI; ++b)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int d = 32 * b + 16 * e + 4 * t;
-          uint2 w = make_uint2(0u, 0u);
-          if (m < nG && d < D) w = __ldg(reinterpret_cast<const uint2*>(src + d));
-          const T* y = reinterpret_cast<const T*>(&w);
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            x[b][e][k] = (float)y[k];
-            if (fabsf(x[b][e][k]) < INFINITY) most = fmaxf(most, fabsf(x[b][e][k]));
-          }
-        }
-      most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
-      most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
-      // The row's largest value to [2^14, 2^15).
-      const int ex = max(15, (int)(__float_as_uint(most) >> 23));
-      const float up = copysignf(__uint_as_float((uint32_t)(268 - min(ex, 254)) << 23), a.scale);
-      float sum[NG];
-#pragma unroll
-      for (int k = 0; k < NG; ++k) sum[k] = 0.f;
-#pragma unroll
-      for (int b = 0; b < NI; ++b)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            x[b][e][k] *= up;
-            sum[NI > 2 ? b : 2 * b + e] += x[b][e][k];
-          }
-          qb[u][b][e][0] = pack16(x[b][e][0], x[b][e][1]);
-          qb[u][b][e][1] = pack16(x[b][e][2] * 0.0625f, x[b][e][3] * 0.0625f);
-        }
-      // Group t's sum, in the keys' units; in halves, for scale (times -8) and mid.
-      float own = 0.f;
-#pragma unroll
-      for (int k = 0; k < NG; ++k) {
-        sum[k] += __shfl_xor_sync(0xffffffffu, sum[k], 1);
-        sum[k] += __shfl_xor_sync(0xffffffffu, sum[k], 2);
-        if (k == t) own = sum[k] * 0x1p-24f;
+      for (int e = 0; e < 2; ++e) {
+        const int d = 32 * b + 16 * e + 4 * t;
+        raw[b][e] = warp < NT && m < nG && d < D ? __ldg(reinterpret_cast<const uint2*>(src + d)) : make_uint2(0u, 0u);
       }
-      const float high = __half2float(__float2half_rn(own));
-      qm[u][0] = pack16(-8.f * high, high);
-      qm[u][1] = pack16(-8.f * (own - high), own - high);
-      // (Scores past f32's range stay within it by a smaller factor: any of them is the whole softmax.  A
-      // factor of zero would make NaN of hidden slots' -infinity.)
-      const float mine = fmaxf(fabsf(a.scale) * __uint_as_float((uint32_t)(min(ex, 230) + 10) << 23), 0x1p-126f);  // 2^(ex - 141 + 24)
+  };
+  auto make_q = [&]() {
+    if (warp >= NT) return;
+    float x[NI][2][4], most = 0.f;
 #pragma unroll
-      for (int y = 0; y < 2; ++y) fr[u][y] = __shfl_sync(0xffffffffu, mine, 8 * t + 4 * y);
+    for (int b = 0; b < NI; ++b)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const T* y = reinterpret_cast<const T*>(&raw[b][e]);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          x[b][e][k] = (float)y[k];
+          if (fabsf(x[b][e][k]) < INFINITY) most = fmaxf(most, fabsf(x[b][e][k]));
+        }
+      }
+    most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
+    most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
+    // The row's largest value to [2^14, 2^15).
+    const int ex = max(15, (int)(__float_as_uint(most) >> 23));
+    const float up = copysignf(__uint_as_float((uint32_t)(268 - min(ex, 254)) << 23), a.scale);
+    float sum[NG];
+#pragma unroll
+    for (int k = 0; k < NG; ++k) sum[k] = 0.f;
+#pragma unroll
+    for (int b = 0; b < NI; ++b) {
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          x[b][e][k] *= up;
+          sum[NI > 2 ? b : 2 * b + e] += x[b][e][k];
+        }
+      sh_q[warp][b][lane] = make_uint4(pack16(x[b][0][0], x[b][0][1]), pack16(x[b][0][2] * 0.0625f, x[b][0][3] * 0.0625f),
+                                       pack16(x[b][1][0], x[b][1][1]), pack16(x[b][1][2] * 0.0625f, x[b][1][3] * 0.0625f));
     }
+    // Group t's sum, in the keys' units; in halves, for scale (times -8) and mid.
+    float own = 0.f;
+#pragma unroll
+    for (int k = 0; k < NG; ++k) {
+      sum[k] += __shfl_xor_sync(0xffffffffu, sum[k], 1);
+      sum[k] += __shfl_xor_sync(0xffffffffu, sum[k], 2);
+      if (k == t) own = sum[k] * 0x1p-24f;
+    }
+    const float high = __half2float(__float2half_rn(own));
+    sh_qm[warp][lane] = make_uint2(pack16(-8.f * high, high), pack16(-8.f * (own - high), own - high));
+    // (Scores past f32's range stay within it by a smaller factor: any of them is the whole softmax.  A
+    // factor of zero would make NaN of hidden slots' -infinity.)
+    if (t == 0)
+      sh_fr[8 * warp + g] = fmaxf(fabsf(a.scale) * __uint_as_float((uint32_t)(min(ex, 230) + 10) << 23), 0x1p-126f);  // 2^(ex - 141 + 24)
   };
 
   auto write_out = [&](int r, int head, int m, int d, float4 x, float L) {  // m: row of the head's nG
@@ -349,41 +393,73 @@ __global__ void __launch_bounds__(NW * 32, 1)
   int shared_parts = 0;
   constexpr int VECS = ROWS * (OS / 4), ITEMS = (VECS + THREADS - 1) / THREADS;
 
-#pragma unroll
+  auto arrives_last = [&](unsigned* counter, int count) {
+    const bool is_last = arrive(counter) == (unsigned)count - 1u;
+    if (is_last) *counter = 0u;
+    return is_last;
+  };
+  // By one thread, once the part's results are written: whether the others' are all there (past kMaxFlat parts:
+  // of its group of parts).
+  auto arrive_at = [&](const Shared& q) {
+    const int c_first = block_of(q.first), parts = block_of(q.end - 1) - c_first + 1;
+    const int b0 = c_first + (c - c_first) / kJoin * kJoin;
+    return parts > kMaxFlat ? arrives_last(a.counters + (int64_t)a.rows * K + 2 * b0 + (b0 == c_first), min(kJoin, c_first + parts - b0))
+                            : arrives_last(a.counters + q.r * K + q.h, parts);
+  };
+#pragma unroll 1
   for (int k = 0; k < RING - 1; ++k) fetch();
-  int at = c0;
   uint32_t get = ring;
+  const uint32_t k_even = hidden(0x000f000fu), k_odd = hidden(0x00f000f0u), k_1024 = hidden(0x64006400u), k_64 = hidden(0x54005400u);
+  int at = c0;
+  bool last_shared = false;  // whether the part before was
+  load_q(p.r, p.h);
+  make_q();
+  __syncthreads();
   for (;;) {  // units
-    load_q(p.r, p.h);
     const int head = p.h / row_groups, m0 = (p.h - head * row_groups) * ROWS, rows_here = min(ROWS, nG - m0);
     const int first = before * K + p.h * p.chunks, end = first + p.chunks, stop = min(end, c1);
     const RowTiles rt = p.rt;
     const int pos_first = rt.end - a.n, low_last = window_low(a, rt.start, rt.end - 1);
-    // ref: a row's reference; edge: the raw score past which it moves.
-    float o[NT][MT][4], ref[NT][2], edge[NT][2], l[NT][4];
+    // This warp's tiles of the part; in [w_lo, w_hi) every row sees the whole tile.
+    const int chunks = stop - at, tile0 = (at - first) * NW + warp;
+    const int valid = min(chunks, max(0, (rt.tiles - tile0 + NW - 1) / NW));
+    const int w_lo = rt.ta + (MULTI ? (low_last - rt.b0 + TK - 1) / TK : 0);
+    const int w_hi = rt.ta + ((MULTI ? min(rt.b1, pos_first + 1) : rt.b1) - rt.b0) / TK;
+    // As numbers of the loop's rounds.
+    const int k_lo = (w_lo - tile0 + NW - 1) / NW, k_hi = w_hi > tile0 ? (w_hi - tile0 + NW - 1) / NW : 0;
+    at = stop;
+    const int s0 = slot_at(g), s1 = slot_at(g + 8);
+    const uint32_t va = slot_at(2 * t) * REC, vb = slot_at(2 * t + 1) * REC;  // rows 8..15: the slots behind them
+    float fr[NT][2], from[NT][2];  // from: a row's reference, negative (far below any score before the first)
+    float o[NT][MT][4], l[NT][2];
+    uint4 qb[KEEP_Q ? NT : 1][NI];
+    uint2 qm[NT];
 #pragma unroll
     for (int u = 0; u < NT; ++u) {
+      if constexpr (KEEP_Q) {
+        qm[u] = sh_qm[u][lane];
 #pragma unroll
-      for (int y = 0; y < 2; ++y) ref[u][y] = edge[u][y] = -INFINITY;
+        for (int b = 0; b < NI; ++b) qb[u][b] = sh_q[u][b][lane];
+      }
+      const float2 both = *reinterpret_cast<const float2*>(&sh_fr[8 * u + 2 * t]);
+      fr[u][0] = both.x;
+      fr[u][1] = both.y;
 #pragma unroll
-      for (int k = 0; k < 4; ++k) l[u][k] = 0.f;
+      for (int y = 0; y < 2; ++y) from[u][y] = -kNever, l[u][y] = 0.f;
 #pragma unroll
       for (int j = 0; j < MT; ++j)
 #pragma unroll
         for (int k = 0; k < 4; ++k) o[u][j][k] = 0.f;
     }
-    for (; at < stop; ++at) {
-      const int tile = (at - first) * NW + warp;
-      const uint32_t kt = get, vt = kt + F::TILE;
-      get = get + 2 * F::TILE == ring + RING * 2 * F::TILE ? ring : get + 2 * F::TILE;
+#pragma unroll 1
+    for (int k = 0; k < chunks; ++k) {
       asm volatile("cp.async.wait_group %0;" ::"n"(RING - 2) : "memory");
       __syncwarp();
-      fetch();  // into the place that the last round has left
-      const bool in_a = tile < rt.ta;
-      const int j0 = in_a ? rt.a0 + tile * TK : rt.b0 + (tile - rt.ta) * TK, jend = in_a ? rt.a1 : rt.b1;
-      if (tile >= rt.tiles || j0 >= jend) continue;
+      fetch();
+      const uint32_t kt = get, vt = get + F::TILE;
+      get = get + 2 * F::TILE == ring + RING * 2 * F::TILE ? ring : get + 2 * F::TILE;
+      if (k >= valid) break;  // (the last one at most)
       // ---- scores
-      const int s0 = slot_at(g), s1 = slot_at(g + 8);
       float s[NT][4];  // slots s0 and s1 of rows 2 t and 2 t + 1, in units of 1 / fr
       {
         uint32_t kw[2][NI], pr[2][4], own[2];
@@ -391,31 +467,36 @@ __global__ void __launch_bounds__(NW * 32, 1)
         for (int x = 0; x < 2; ++x) {
           const uint32_t rec = kt + (x ? s1 : s0) * REC;
           if constexpr (NI == 4) {
-            asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(kw[x][0]), "=r"(kw[x][1]), "=r"(kw[x][2]), "=r"(kw[x][3]) : "r"(rec + t * 16));
+            load4(kw[x], rec + t * 16);
           } else if constexpr (NI == 2) {
-            asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(kw[x][0]), "=r"(kw[x][1]) : "r"(rec + t * 8));
+            load2(kw[x], rec + t * 8);
           } else {
 #pragma unroll
-            for (int b = 0; b < NI; ++b) asm volatile("ld.shared.u32 %0, [%1];" : "=r"(kw[x][b]) : "r"(rec + (t * NI + b) * 4));
+            for (int b = 0; b < NI; ++b) kw[x][b] = load1(rec + (t * NI + b) * 4);
           }
-          asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(pr[x][0]), "=r"(pr[x][1]), "=r"(pr[x][2]), "=r"(pr[x][3]) : "r"(rec + 16 * NI));
-          asm volatile("ld.shared.u32 %0, [%1];" : "=r"(own[x]) : "r"(rec + 16 * NI + 4 * t));
+          load4(pr[x], rec + 16 * NI);
+          own[x] = load1(rec + 16 * NI + 4 * t);
         }
 #pragma unroll
-        for (int u = 0; u < NT; ++u) mma16(s[u], own[0], own[1], own[0], own[1], qm[u][0], qm[u][1]);
+        for (int u = 0; u < NT; ++u) {
+          const uint2 q = KEEP_Q ? qm[u] : sh_qm[u][lane];
+          mma_new(s[u], own[0], own[1], own[0], own[1], q.x, q.y);
+        }
 #pragma unroll
         for (int grp = 0; grp < NG; ++grp) {
+          const int b = NI > 2 ? grp : grp >> 1;
           float acc[NT][4];
 #pragma unroll
           for (int e = NI > 2 ? 0 : grp & 1; e < (NI > 2 ? 2 : (grp & 1) + 1); ++e) {
-            const int b = NI > 2 ? grp : grp >> 1;
             const uint32_t w0 = e ? kw[0][b] >> 8 : kw[0][b], w1 = e ? kw[1][b] >> 8 : kw[1][b];
 #pragma unroll
             for (int u = 0; u < NT; ++u) {
+              const uint4 q = KEEP_Q ? qb[KEEP_Q ? u : 0][b] : sh_q[u][b][lane];
+              const uint32_t b0 = e ? q.z : q.x, b1 = e ? q.w : q.y;
               if (NI > 2 && e)
-                mma16(acc[u], w0 & 0x000f000fu, w1 & 0x000f000fu, w0 & 0x00f000f0u, w1 & 0x00f000f0u, qb[u][b][e][0], qb[u][b][e][1], acc[u]);
+                mma_add(acc[u], w0 & 0x000f000fu, w1 & 0x000f000fu, w0 & 0x00f000f0u, w1 & 0x00f000f0u, b0, b1);
               else
-                mma16(acc[u], w0 & 0x000f000fu, w1 & 0x000f000fu, w0 & 0x00f000f0u, w1 & 0x00f000f0u, qb[u][b][e][0], qb[u][b][e][1]);
+                mma_new(acc[u], w0 & 0x000f000fu, w1 & 0x000f000fu, w0 & 0x00f000f0u, w1 & 0x00f000f0u, b0, b1);
             }
           }
 #pragma unroll
@@ -428,182 +509,175 @@ __global__ void __launch_bounds__(NW * 32, 1)
           }
         }
       }
-      const bool whole = j0 + TK <= jend && (in_a || !MULTI || (j0 >= low_last && j0 + TK - 1 <= pos_first));
-      if (!whole) {
+      const bool whole = k >= k_lo && k < k_hi;
+      if (!whole || a.scores) {
+        const int tile = tile0 + k * NW;
+        const bool in_a = tile < rt.ta;
+        const int j0 = in_a ? rt.a0 + tile * TK : rt.b0 + (tile - rt.ta) * TK, jend = in_a ? rt.a1 : rt.b1;
 #pragma unroll
         for (int u = 0; u < NT; ++u)
 #pragma unroll
           for (int y = 0; y < 2; ++y) {
-            const int pos = MULTI ? pos_first + (m0 + 8 * u + 2 * t + y) / group : pos_first;
+            const int m = 8 * u + 2 * t + y;
+            const int pos = MULTI ? pos_first + (m0 + m) / group : pos_first;
             const int low = window_low(a, rt.start, pos);
 #pragma unroll
             for (int x = 0; x < 2; ++x) {
               const int j = j0 + (x ? s1 : s0);
               if (j >= jend || !slot_seen(a, rt.start, pos, low, j)) s[u][2 * x + y] = -INFINITY;
+              if (a.scores && j < jend && m < rows_here)
+                a.scores[((int64_t)(p.r * a.kv_heads + head) * nG + m0 + m) * a.capacity + j] = s[u][2 * x + y] * fr[u][y];
             }
           }
       }
-      if (a.scores) {
+      // ---- weights, by what exceeds the reference; past the slack it moves
+      float z[NT][2][2], most = -INFINITY;
+      auto shift = [&]() {
 #pragma unroll
         for (int u = 0; u < NT; ++u)
 #pragma unroll
           for (int x = 0; x < 2; ++x)
 #pragma unroll
-            for (int y = 0; y < 2; ++y) {
-              const int j = j0 + (x ? s1 : s0), m = 8 * u + 2 * t + y;
-              if (j < jend && m < rows_here)
-                a.scores[((int64_t)(p.r * a.kv_heads + head) * nG + m0 + m) * a.capacity + j] = s[u][2 * x + y] * fr[u][y];
-            }
-      }
-      // ---- weights
-      bool over = false;
+            for (int y = 0; y < 2; ++y) z[u][x][y] = fmaf(s[u][2 * x + y], fr[u][y], from[u][y]);
+      };
+      shift();
 #pragma unroll
-      for (int u = 0; u < NT; ++u)
-#pragma unroll
-        for (int y = 0; y < 2; ++y) over |= fmaxf(s[u][y], s[u][2 + y]) > edge[u][y];
-      if (__any_sync(0xffffffffu, over)) {
+      for (int u = 0; u < NT; ++u) most = fmaxf(most, fmaxf(fmaxf(z[u][0][0], z[u][0][1]), fmaxf(z[u][1][0], z[u][1][1])));
+      if (__any_sync(0xffffffffu, most > kSlack)) {
 #pragma unroll
         for (int u = 0; u < NT; ++u)
 #pragma unroll
           for (int y = 0; y < 2; ++y) {
             float mx = fmaxf(s[u][y], s[u][2 + y]);
 #pragma unroll
-            for (int k = 4; k < 32; k <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, k));
-            const float now = fmaxf(mx * fr[u][y], ref[u][y]);
-            const float by = now == ref[u][y] ? 1.f : ex2(ref[u][y] - now);
-            ref[u][y] = now;
-            edge[u][y] = now == -INFINITY ? -INFINITY : (now + kSlack) / fr[u][y];
+            for (int x = 4; x < 32; x <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
+            const float now = fminf(-mx * fr[u][y], from[u][y]);
+            const float by = now == from[u][y] ? 1.f : ex2(now - from[u][y]);
+            from[u][y] = now;
             l[u][y] *= by;
-            l[u][2 + y] *= by;
 #pragma unroll
             for (int j = 0; j < MT; ++j) {
               o[u][j][y] *= by;
               o[u][j][2 + y] *= by;
             }
           }
+        shift();
       }
-      // Weights as B operand: slots of rows 0..7 and 8..15 of the tile's order; their sums are a product with ones.
-      uint32_t pb[NT][2];
-      [[maybe_unused]] uint32_t pl[NT][2];  // float16 outputs: what the rounding left
+      // As B operand of the values' product: slots of rows 0..7 and 8..15 of the tile's order (float16 outputs: and
+      // what their rounding left).
+      uint32_t pw[HALVES ? 2 : 1][NT][2];
 #pragma unroll
-      for (int u = 0; u < NT; ++u) {
+      for (int u = 0; u < NT; ++u)
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
-          float w[2];
-#pragma unroll
-          for (int y = 0; y < 2; ++y) w[y] = ex2(fmaf(s[u][2 * x + y], fr[u][y], -(ref[u][y] == -INFINITY ? 0.f : ref[u][y])));
-          const uint32_t both = pack16(w[0], w[1]);
-          pb[u][x] = transposed(both);
+          const float w0 = ex2(z[u][x][0]), w1 = ex2(z[u][x][1]);
+          l[u][0] += w0;
+          l[u][1] += w1;
+          const uint32_t both = pack16(w0, w1);
+          pw[0][u][x] = transposed(both);
           if constexpr (HALVES) {
-            const float2 high = __half22float2(*reinterpret_cast<const __half2*>(&both));
-            pl[u][x] = transposed(pack16(w[0] - high.x, w[1] - high.y));
+            const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&both));
+            pw[1][u][x] = transposed(pack16(w0 - h.x, w1 - h.y));
           }
         }
-        mma16(l[u], kOnes, kOnes, kOnes, kOnes, pb[u][0], pb[u][1], l[u]);
-        if constexpr (HALVES) mma16(l[u], kOnes, kOnes, kOnes, kOnes, pl[u][0], pl[u][1], l[u]);
-      }
       // ---- values
-      {
-        const int va = slot_at(2 * t), vb = slot_at(2 * t + 1);  // and each + 1 in rows 8..15
-        const uint32_t ra[4] = {vt + va * REC, vt + vb * REC, vt + (va + 1) * REC, vt + (vb + 1) * REC};
-        uint32_t vw[4][NB], pr[4][2];
+      const uint32_t ra[4] = {vt + va, vt + vb, vt + va + REC, vt + vb + REC};
+      uint32_t vw[4][NB], pr[4][2];
 #pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          if constexpr (NI == 4) {
-            asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(vw[x][0]), "=r"(vw[x][1]) : "r"(ra[x] + g * 8));
-            asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(pr[x][0]), "=r"(pr[x][1]) : "r"(ra[x] + 16 * NI + (g & 1) * 8));
-          } else if constexpr (NI == 3) {  // words 2 g, 2 g + 1 of twelve
-            const int w = min(2 * g, 10);
-            asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(vw[x][0]), "=r"(vw[x][1]) : "r"(ra[x] + w * 4));
-            asm volatile("ld.shared.u32 %0, [%1];" : "=r"(pr[x][0]) : "r"(ra[x] + 16 * NI + w % 3 * 4));
-            asm volatile("ld.shared.u32 %0, [%1];" : "=r"(pr[x][1]) : "r"(ra[x] + 16 * NI + (w + 1) % 3 * 4));
-          } else {
-            const int w = NI == 2 ? g : g & 3;
-            asm volatile("ld.shared.u32 %0, [%1];" : "=r"(vw[x][0]) : "r"(ra[x] + w * 4));
-            asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(pr[x][0]), "=r"(pr[x][1]) : "r"(ra[x] + 16 * NI + w % NI * 8));
-          }
+      for (int x = 0; x < 4; ++x) {
+        if constexpr (NI == 4) {
+          load2(vw[x], ra[x] + g * 8);
+          load2(pr[x], ra[x] + 16 * NI + (g & 1) * 8);
+        } else if constexpr (NI == 3) {  // words 2 g, 2 g + 1 of twelve
+          const int w = min(2 * g, 10);
+          load2(vw[x], ra[x] + w * 4);
+          pr[x][0] = load1(ra[x] + 16 * NI + w % 3 * 4);
+          pr[x][1] = load1(ra[x] + 16 * NI + (w + 1) % 3 * 4);
+        } else {
+          const int w = NI == 2 ? g : g & 3;
+          vw[x][0] = load1(ra[x] + w * 4);
+          load2(pr[x], ra[x] + 16 * NI + w % NI * 8);
         }
-        uint32_t sc[2][2], mi[2][2];  // [rows 0..7, 8..15][group]
+      }
+      uint32_t sc[2][2], mi[2][2];  // [rows 0..7, 8..15][group]
+#pragma unroll
+      for (int x = 0; x < 2; ++x)
+#pragma unroll
+        for (int y = 0; y < 2; ++y) {
+          sc[x][y] = __byte_perm(pr[2 * x][y], pr[2 * x + 1][y], 0x5410);
+          mi[x][y] = __byte_perm(pr[2 * x][y], pr[2 * x + 1][y], 0x7632);
+        }
+      // A group that stands for NaN must not reach the rows that do not see its slot (0 * NaN): the
+      // product takes zeros in its place, and the rows that see it become NaN below.
+      bool hide = false;
+      uint32_t bad[2][2] = {{0u, 0u}, {0u, 0u}};
+      if (MULTI && !whole) {
+        uint32_t any = 0u;
 #pragma unroll
         for (int x = 0; x < 2; ++x)
 #pragma unroll
-          for (int k = 0; k < 2; ++k) {
-            sc[x][k] = __byte_perm(pr[2 * x][k], pr[2 * x + 1][k], 0x5410);
-            mi[x][k] = __byte_perm(pr[2 * x][k], pr[2 * x + 1][k], 0x7632);
+          for (int y = 0; y < 2; ++y) {
+            const uint32_t lo = (sc[x][y] & 0x7c00u) == 0x7c00u || (mi[x][y] & 0x7c00u) == 0x7c00u ? 0xffffu : 0u;
+            const uint32_t hi = (sc[x][y] & 0x7c000000u) == 0x7c000000u || (mi[x][y] & 0x7c000000u) == 0x7c000000u ? 0xffff0000u : 0u;
+            bad[x][y] = lo | hi;
+            any |= bad[x][y];
+            sc[x][y] &= ~bad[x][y];
+            mi[x][y] &= ~bad[x][y];
           }
-        // A group that stands for NaN must not reach the rows that do not see its slot (0 * NaN): the
-        // product takes zeros in its place, and the rows that see it become NaN below.
-        bool hide = false;
-        uint32_t bad[2][2] = {{0u, 0u}, {0u, 0u}};
-        if (MULTI && !whole) {
-          uint32_t any = 0u;
+        hide = __any_sync(0xffffffffu, any != 0u);
+      }
+      // The value of nibble j (0..3) of a 16-bit half, of two slots side by side.
+      auto value = [&](uint32_t w, int j, uint32_t scale, uint32_t mid) {
+        const uint32_t x = j & 2 ? w >> 8 : w;
+        const uint32_t c8 = j & 1 ? add16(and_or(x, k_odd, k_64), 0xd480d480u)      // 64 + c - 72
+                                  : add16(and_or(x, k_even, k_1024), 0xe408e408u);  // 1024 + c - 1032
+        return fma16(c8, scale, mid);
+      };
 #pragma unroll
-          for (int x = 0; x < 2; ++x)
+      for (int b = 0; b < NB; ++b) {
+        const uint32_t l0 = __byte_perm(vw[0][b], vw[1][b], 0x5410), h0 = __byte_perm(vw[0][b], vw[1][b], 0x7632);
+        const uint32_t l1 = __byte_perm(vw[2][b], vw[3][b], 0x5410), h1 = __byte_perm(vw[2][b], vw[3][b], 0x7632);
 #pragma unroll
-            for (int k = 0; k < 2; ++k) {
-              const uint32_t lo = (sc[x][k] & 0x7c00u) == 0x7c00u || (mi[x][k] & 0x7c00u) == 0x7c00u ? 0xffffu : 0u;
-              const uint32_t hi = (sc[x][k] & 0x7c000000u) == 0x7c000000u || (mi[x][k] & 0x7c000000u) == 0x7c000000u ? 0xffff0000u : 0u;
-              bad[x][k] = lo | hi;
-              any |= bad[x][k];
-            }
-          hide = __any_sync(0xffffffffu, any != 0u);
-          if (hide) {
+        for (int j = 0; j < 4; ++j) {
+          const int y = NI > 2 ? b : j >> 1;
+          const uint32_t a0 = value(l0, j, sc[0][y], mi[0][y]), a1 = value(h0, j, sc[0][y], mi[0][y]);
+          const uint32_t a2 = value(l1, j, sc[1][y], mi[1][y]), a3 = value(h1, j, sc[1][y], mi[1][y]);
 #pragma unroll
-            for (int x = 0; x < 2; ++x)
+          for (int z = 0; z < (HALVES ? 2 : 1); ++z)
 #pragma unroll
-              for (int k = 0; k < 2; ++k) sc[x][k] &= ~bad[x][k], mi[x][k] &= ~bad[x][k];
-          }
-        }
-        // The value of nibble j (0..3) of a 16-bit half, of two slots side by side.
-        auto value = [&](uint32_t w, int j, uint32_t scale, uint32_t mid) {
-          const uint32_t x = j & 2 ? w >> 8 : w;
-          const uint32_t c8 = j & 1 ? fma16((x & 0x00f000f0u) | 0x64006400u, 0x2c002c00u, 0xd480d480u)   // (1024 + 16 c) / 16 - 72
-                                    : add16((x & 0x000f000fu) | 0x64006400u, 0xe408e408u);              // 1024 + c - 1032
-          return fma16(c8, scale, mid);
-        };
-#pragma unroll
-        for (int b = 0; b < NB; ++b) {
-          const uint32_t l0 = __byte_perm(vw[0][b], vw[1][b], 0x5410), h0 = __byte_perm(vw[0][b], vw[1][b], 0x7632);
-          const uint32_t l1 = __byte_perm(vw[2][b], vw[3][b], 0x5410), h1 = __byte_perm(vw[2][b], vw[3][b], 0x7632);
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const int k = NI > 2 ? b : j >> 1;
-            const uint32_t a0 = value(l0, j, sc[0][k], mi[0][k]), a1 = value(h0, j, sc[0][k], mi[0][k]);
-            const uint32_t a2 = value(l1, j, sc[1][k], mi[1][k]), a3 = value(h1, j, sc[1][k], mi[1][k]);
-#pragma unroll
-            for (int u = 0; u < NT; ++u) {
-              mma16(o[u][4 * b + j], a0, a1, a2, a3, pb[u][0], pb[u][1], o[u][4 * b + j]);
-              if constexpr (HALVES) mma16(o[u][4 * b + j], a0, a1, a2, a3, pl[u][0], pl[u][1], o[u][4 * b + j]);
-            }
-          }
-        }
-        if (MULTI && hide) {
-#pragma unroll
-          for (int b = 0; b < NB; ++b)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              const int k = NI > 2 ? b : j >> 1;
-              const uint32_t x = bad[0][k] & 0x3c003c00u, z = bad[1][k] & 0x3c003c00u;
-#pragma unroll
-              for (int u = 0; u < NT; ++u) {
-                float seen[4];
-                mma16(seen, x, x, z, z, pb[u][0], pb[u][1]);
-#pragma unroll
-                for (int q = 0; q < 4; ++q)
-                  if (seen[q] != 0.f) o[u][4 * b + j][q] = __int_as_float(0x7fc00000);
-              }
-            }
+            for (int u = 0; u < NT; ++u) mma_add(o[u][4 * b + j], a0, a1, a2, a3, pw[z][u][0], pw[z][u][1]);
         }
       }
+      if (MULTI && hide) {
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const int y = NI > 2 ? b : j >> 1;
+            const uint32_t x0 = bad[0][y] & kOnes, x1 = bad[1][y] & kOnes;
+#pragma unroll
+            for (int u = 0; u < NT; ++u) {
+              float seen[4];
+              mma_new(seen, x0, x0, x1, x1, pw[0][u][0], pw[0][u][1]);
+#pragma unroll
+              for (int q = 0; q < 4; ++q)
+                if (seen[q] != 0.f) o[u][4 * b + j][q] = __int_as_float(0x7fc00000);
+            }
+          }
+      }
     }
-
-    // ---- the warps' results into shared memory
+    // The warp's results into shared memory.
 #pragma unroll
     for (int u = 0; u < NT; ++u) {
 #pragma unroll
       for (int y = 0; y < 2; ++y) {
         const int m = 8 * u + 2 * t + y;
-        if (g == 0) warp_ml[warp][m] = make_float2(ref[u][y], l[u][y]);
+#pragma unroll
+        for (int x = 4; x < 32; x <<= 1) l[u][y] += __shfl_xor_sync(0xffffffffu, l[u][y], x);
+        if (g == 0) {
+          warp_m[warp][m] = -from[u][y];
+          warp_l[warp][m] = l[u][y];
+        }
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
           const int w = NI > 2 ? 2 * g + b : g, tw = w / NI, blk = w - tw * NI;
@@ -617,21 +691,24 @@ __global__ void __launch_bounds__(NW * 32, 1)
         }
       }
     }
+    if (end < c1) {
+      const bool row_ends = p.h + 1 == K;
+      load_q(row_ends ? p.r + 1 : p.r, row_ends ? 0 : p.h + 1);
+    }
     __syncthreads();
     const bool alone = first >= c0 && end <= c1;
     const int slot = 2 * c + (first >= c0);
     if (tid < ROWS) {
-      float M = -INFINITY, L = 0.f;
+      float top = -INFINITY, L = 0.f;
 #pragma unroll
-      for (int k = 0; k < NW; ++k) M = fmaxf(M, warp_ml[k][tid].x);
-      const float z = M == -INFINITY ? 0.f : M;
+      for (int k = 0; k < NW; ++k) top = fmaxf(top, warp_m[k][tid]);
 #pragma unroll
       for (int k = 0; k < NW; ++k) {
-        const float by = ex2(warp_ml[k][tid].x - z);
+        const float by = ex2(warp_m[k][tid] - top);
         factor[k][tid] = by;
-        L = fmaf(warp_ml[k][tid].y, by, L);
+        L = fmaf(warp_l[k][tid], by, L);
       }
-      joined[tid] = make_float2(M, L);
+      joined[tid] = make_float2(top, L);
       if (tid < rows_here) {
         if (alone)
           write_lse(p.r, head, m0 + tid, joined[tid]);
@@ -664,8 +741,12 @@ __global__ void __launch_bounds__(NW * 32, 1)
       const int e = a.lengths ? a.lengths[p.r] : a.capacity, s = a.starts ? a.starts[p.r] : 0;
       a.status[p.r] = (e < 0 || e > a.capacity || s < 0 || s > max(e, 0)) ? 8 : 0;
     }
+    if (end < c1) make_q();  // (nobody reads the queries past the barriers above)
     __syncthreads();
+    last_shared = !alone;
     if (end >= c1) break;
+    // A unit that an earlier block began arrives at once: that block, which ends with it, mostly finds all there.
+    if (!alone && tid == 0) sh_last[shared_parts - 1] = arrive_at(shared_part[shared_parts - 1]);
     p.k = 0;
     if (++p.h == K) {
       p.h = 0;
@@ -678,6 +759,18 @@ __global__ void __launch_bounds__(NW * 32, 1)
   auto join = [&](const Shared& q, int c_first, int b0, int step, int count, bool last) {
     const int head = q.h / row_groups, m0 = (q.h - head * row_groups) * ROWS, rows_here = min(ROWS, nG - m0);
     auto slot_of = [&](int k) { return (int64_t)2 * (b0 + k * step) + (b0 + k * step == c_first); };
+    // The first parts' values are on their way while their factors are made.
+    constexpr int AHEAD = 16 / ITEMS > 6 ? 6 : 16 / ITEMS;
+    float4 early[ITEMS][AHEAD];
+    auto part_at = [&](int k, int x) {
+      const int v = tid + x * THREADS, m = v / (OS / 4), d = (v - m * (OS / 4)) * 4;
+      return __ldcg(reinterpret_cast<const float4*>(a.part_o + (slot_of(k) * ROWS + min(m, ROWS - 1)) * OS + d));
+    };
+#pragma unroll
+    for (int x = 0; x < ITEMS; ++x)
+#pragma unroll
+      for (int k = 0; k < AHEAD; ++k)
+        if (k < count) early[x][k] = part_at(k, x);
     __syncthreads();
     for (int x = tid; x < count * ROWS; x += THREADS) {
       const int k = x / ROWS, m = x - k * ROWS;
@@ -706,34 +799,25 @@ __global__ void __launch_bounds__(NW * 32, 1)
       const int v = tid + x * THREADS, m = v / (OS / 4), d = (v - m * (OS / 4)) * 4;
       if (m >= rows_here) continue;
       float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 8
-      for (int k = 0; k < count; ++k) {
-        const float4 y = __ldcg(reinterpret_cast<const float4*>(a.part_o + (slot_of(k) * ROWS + m) * OS + d));
+      auto add = [&](int k, float4 y) {
         const float by = factor[k][m];
         sum.x = fmaf(y.x, by, sum.x);
         sum.y = fmaf(y.y, by, sum.y);
         sum.z = fmaf(y.z, by, sum.z);
         sum.w = fmaf(y.w, by, sum.w);
-      }
+      };
+#pragma unroll
+      for (int k = 0; k < AHEAD; ++k)
+        if (k < count) add(k, early[x][k]);
+#pragma unroll 4
+      for (int k = AHEAD; k < count; ++k) add(k, part_at(k, x));
       if (last)
         write_out(q.r, head, m0 + m, d, sum, joined[m].y);
       else
         *reinterpret_cast<float4*>(a.part_o + (slot_of(0) * ROWS + m) * OS + d) = sum;
     }
   };
-  auto arrives_last = [&](unsigned* counter, int count) {
-    const bool is_last = arrive(counter) == (unsigned)count - 1u;
-    if (is_last) *counter = 0u;
-    return is_last;
-  };
-  if (tid < shared_parts) {
-    const Shared& q = shared_part[tid];
-    const int c_first = block_of(q.first), parts = block_of(q.end - 1) - c_first + 1;
-    const int b0 = c_first + (c - c_first) / kJoin * kJoin;
-    sh_last[tid] = parts > kMaxFlat ? arrives_last(a.counters + (int64_t)a.rows * K + 2 * b0 + (b0 == c_first),
-                                                   min(kJoin, c_first + parts - b0))
-                                    : arrives_last(a.counters + q.r * K + q.h, parts);
-  }
+  if (tid == 0 && last_shared) sh_last[shared_parts - 1] = arrive_at(shared_part[shared_parts - 1]);
   __syncthreads();
   for (int x = 0; x < shared_parts; ++x) {
     if (!sh_last[x]) continue;
@@ -764,8 +848,8 @@ cudaError_t record(const AttnArgs& a, int row_groups, cudaStream_t stream) {
 }
 
 template <typename T, int NI, bool MULTI> cudaError_t record_rows(const AttnArgs& a, const RecordRows& x, cudaStream_t stream) {
-  if (x.tiles == 1) return record<T, NI, 1, 16, 3, MULTI>(a, x.groups, stream);
-  return record<T, NI, 2, 8, 4, MULTI>(a, x.groups, stream);
+  if (x.tiles == 1) return record<T, NI, 1, 12, 4, MULTI>(a, x.groups, stream);
+  return record<T, NI, 2, 8, 5, MULTI>(a, x.groups, stream);
 }
 
 template <typename T> cudaError_t record_any(const AttnArgs& a, const RecordRows& x, cudaStream_t stream) {
