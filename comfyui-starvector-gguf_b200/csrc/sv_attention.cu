@@ -1,5 +1,6 @@
 // sv_attention.cu -- entry points of the attention over the decoder's cache: argument
 // checks, the split of the slots over blocks, workspace layout and launches.
+#include <algorithm>
 #include <cmath>
 
 #include "../../include/starvector_sampling.h"
@@ -13,6 +14,7 @@ constexpr int kSMs = 148;
 constexpr int kMostPrefixSplits = 16;  // that the token kernel joins
 constexpr int kMostSlots = 1 << 29;    // sums of two slot numbers stay in 31 bits
 constexpr int kMostRecordGroups = 4;   // groups of query rows that the kernel over 4-bit records takes one by one
+constexpr size_t kMostValues = (size_t)96 << 20;  // bytes of plain values of 4-bit records at a time: they stay in L2
 constexpr size_t kMostScores = (size_t)256 << 20;  // bytes of scores kept for the accumulated weights
 
 size_t up256(size_t x) { return (x + 255) / 256 * 256; }
@@ -91,6 +93,7 @@ Plan make_plan(const AttnArgs& a) {
       p.o_splits = f32_splits(units * div_up(nG, 16), slots);
     } else {
       p.own = tile_split(units, nG, most_slots(a.capacity, a.window, a.sinks, div_up(128, a.group)), kSMs);
+      if (a.k_low && a.dim > 64) p.own.paired = false;  // its ring holds three steps
       p.o_splits = p.own.splits;
     }
     if (!a.prefix && p.o_splits == 1) p.o_splits = 0;
@@ -201,14 +204,21 @@ void set_window(AttnArgs& a, int32_t window, int32_t sinks) {
   a.sinks = sinks < 0 || (limit && window > 0) ? sinks : 0;
 }
 
-// How a call over 4-bit records is done: by the kernel that takes them as they are (few query rows),
-// or from the plain values of the slots that some query sees.
+// How a call over 4-bit records is done: by the kernel that takes them as they are (few query rows), or
+// from the plain values of the slots that some query sees, as many cache rows at a time as kMostValues holds (long
+// prompts read each value many times: turning it once, 8192 slots of four heads take 8 us, is cheaper than in every
+// block that reads it; four more warps in the tile kernel that did so took 926 us for 2048 queries over 16384
+// slots, 489 us this way).
 struct RecordPlan {
   bool direct;
   RecordRows rows;
   size_t counters, o_bytes, ml_bytes, lse_bytes, score_bytes;  // direct
-  size_t before, values;                                       // the other way: the attention's own, the plain values
-  size_t total() const { return direct ? counters + o_bytes + ml_bytes + lse_bytes + score_bytes : before + values; }
+  int32_t batch;                                               // otherwise: cache rows at a time,
+  int32_t halves, pairs;                                       // float16 values, the keys' in pairs;
+  size_t before, array;                                        // bytes of the attention's own, of the keys or values
+  size_t total() const {
+    return direct ? counters + o_bytes + ml_bytes + lse_bytes + score_bytes : before + (pairs ? 3 : 2) * array;
+  }
 };
 
 RecordPlan record_plan(const AttnArgs& a) {
@@ -225,8 +235,20 @@ RecordPlan record_plan(const AttnArgs& a) {
   p.direct = a.dtype != SV_F32 && p.rows.groups <= kMostRecordGroups && units * p.rows.groups <= 65536 &&
              units * p.rows.groups * (a.capacity / 128 + 3) < (int64_t)1 << 31 && p.score_bytes <= kMostScores;
   if (!p.direct) {
-    p.before = make_plan(a).total();
-    p.values = 2 * up256((size_t)units * a.capacity * a.dim * (a.dtype == SV_F32 ? 4 : 2));
+    p.halves = a.dtype != SV_F32 && !a.weights;  // (the accumulated weights' product takes keys of the queries' type)
+    p.pairs = p.halves && a.dtype == SV_F16;
+    const size_t row = (size_t)a.kv_heads * a.capacity * a.dim * (a.dtype == SV_F32 ? 4 : 2);
+    const size_t fit = kMostValues / ((p.pairs ? 3 : 2) * row);
+    p.batch = fit >= (size_t)a.rows ? a.rows : fit > 1 ? (int32_t)fit : 1;
+    p.array = up256(p.batch * row);
+    static const char some = 0;
+    AttnArgs b = a;
+    b.halves = p.halves;
+    b.k_low = p.pairs ? &some : nullptr;
+    for (int32_t rows : {p.batch, a.rows % p.batch}) {
+      b.rows = rows;
+      if (rows) p.before = std::max(p.before, make_plan(b).total());
+    }
   }
   return p;
 }
@@ -365,25 +387,37 @@ int sv_quantized_attention(const void* q, int32_t dtype, int32_t rows, int32_t t
     return a.weights && launch_scores_weights(a, s) != cudaSuccess ? SV_E_CUDA : SV_OK;
   }
   ReadArgs x = {};
-  x.cache[0] = static_cast<const unsigned char*>(cache_keys);
-  x.cache[1] = static_cast<const unsigned char*>(cache_values);
   x.row = cache_stride_row;
   x.head = cache_stride_head;
   x.slot = cache_stride_slot;
   a.k = x.out[0] = w + p.before;
-  a.v = x.out[1] = w + p.before + p.values / 2;
-  x.lengths = lengths;
-  x.starts = starts;
-  x.dtype = dtype;
-  x.rows = rows;
+  a.v = x.out[1] = w + p.before + p.array;
+  a.halves = p.halves;
+  a.k_low = x.low = p.pairs ? w + p.before + 2 * p.array : nullptr;
+  x.dtype = p.halves ? SV_F16 : dtype;
   x.kv_heads = kv_heads;
   x.dim = head_dim;
   x.capacity = x.tokens = capacity;
   x.seen = tokens;
   x.window = a.window;
   x.sinks = a.sinks;
-  if (launch_read_records(x, s) != cudaSuccess) return SV_E_CUDA;
-  return run(a, workspace, p.before, s);
+  const int64_t e = dtype == SV_F32 ? 4 : 2;
+  for (int32_t r = 0; r < rows; r += p.batch) {
+    AttnArgs b = a;
+    x.rows = b.rows = std::min(p.batch, rows - r);
+    x.cache[0] = static_cast<const unsigned char*>(cache_keys) + r * cache_stride_row;
+    x.cache[1] = static_cast<const unsigned char*>(cache_values) + r * cache_stride_row;
+    x.lengths = b.lengths = lengths ? lengths + r : nullptr;
+    x.starts = b.starts = starts ? starts + r : nullptr;
+    b.q = static_cast<const unsigned char*>(q) + r * q_stride_row * e;
+    b.out = static_cast<unsigned char*>(out) + (int64_t)r * tokens * heads * head_dim * e;
+    b.status = out_status ? out_status + r : nullptr;
+    b.weights = weights ? weights + r * weights_stride_row : nullptr;
+    if (launch_read_records(x, s) != cudaSuccess) return SV_E_CUDA;
+    rc = run(b, workspace, p.before, s);
+    if (rc) return rc;
+  }
+  return SV_OK;
 }
 
 size_t sv_prefix_attention_workspace_bytes(int32_t dtype, int32_t rows, int32_t tokens, int32_t heads,

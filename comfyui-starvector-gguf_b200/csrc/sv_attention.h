@@ -50,6 +50,8 @@ struct AttnArgs {
   float* weight_parts; // [w_splits][rows * kv_heads][capacity], with weights and w_splits > 1
   int32_t p_splits, o_splits;  // o_splits 0: the own part is written directly
   int32_t w_splits;            // of the query rows, for the accumulated weights of calls with many
+  const void* k_low;           // with halves and float16 queries: what the keys' rounding left, laid out as they are
+  int32_t halves;              // keys and values are float16 whatever the queries are (values of a 4-bit cache)
   int32_t test_head;           // test hook: one plus the key/value head whose waits run out
 };
 

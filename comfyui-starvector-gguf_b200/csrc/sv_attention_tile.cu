@@ -34,6 +34,7 @@
 // TMEM is freed and the rows' outputs become NaN (status SV_ST_TIMEOUT).
 #include <atomic>
 #include <cstring>
+#include <type_traits>
 
 #include "../../include/starvector_sampling.h"
 #include "sv_attention.h"
@@ -45,23 +46,33 @@ namespace {
 constexpr int NT = 384;
 constexpr int kSMs = 148;
 constexpr int BM = 128, BN = 64;
-constexpr int RING = 4;            // steps (64 slots) whose keys and values are held
-constexpr int STAGES = 2 * RING;
+constexpr int kMostRing = 4;       // steps (64 slots) whose keys and values are held
 constexpr float kSlack = 8.f;
+
+// kPlain: keys and values of the queries' type.  What a cache held in 4 bits stands for comes as float16:
+// kHalves: for bfloat16 queries, which become float16 too, each row times a power of two (they lose nothing, and the
+// keys an eighth of what bfloat16 would); kPairs: for float16 queries, each key and each weight as two float16, the
+// second what the first one's rounding left (error of 4 x 100 queries against 64 bits: 0.00058 without, 0.00036 with the
+// keys' alone; 0.00021 is the output's own rounding).
+enum Source { kPlain, kHalves, kPairs };
 constexpr int kEdges = 16;  // tiles that not every row of a block sees whole: at most twelve, see whole()
 
-template <int DC> struct Layout {
+template <int DC, Source SRC> struct Layout {
+  static constexpr int RING = SRC == kPairs && DC == 2 ? 3 : kMostRing, STAGES = 2 * RING;
   static constexpr uint32_t kQHalf = BM * 128, kHalf = BN * 128;  // 64 dimensions of a tile's rows
   static constexpr uint32_t kQTile = DC * kQHalf, kTile = DC * kHalf;
   static constexpr uint32_t kRing = 2 * kQTile;                      // after two query tiles
-  static constexpr uint32_t kBytes = kRing + STAGES * kTile + 1024;  // alignment slack
+  static constexpr uint32_t kLow = kRing + STAGES * kTile;           // kPairs: the keys' second halves, one tile a step
+  static constexpr uint32_t kBytes = kLow + (SRC == kPairs ? RING * kTile : 0) + 1024;  // alignment slack
 };
 
 struct Shared {
   // full, ready: a stage's copy, and its edge-tile pass.  s_full, pv_done: a query tile's scores of step j and
-  // its product of step j (they also free the step's keys and values); one barrier for each of the four steps
+  // its product of step j (they also free the step's keys and values); one barrier for each of the steps
   // that the ring holds, so that none gets two phases ahead of who waits for it.
-  uint64_t q_full[2], full[STAGES], ready[STAGES], s_full[2][RING], p_full[2][2], pv_done[2][RING], written[2], drained[2];
+  uint64_t q_full[2], full[2 * kMostRing], ready[2 * kMostRing], s_full[2][kMostRing], p_full[2][2], pv_done[2][kMostRing],
+      written[2], drained[2];
+  float row_scale[2][BM];  // kHalves: of a row's scores
   float2 pair[BM];  // PAIRED: the second group's references and sums
   uint32_t tmem;
   uint32_t bad[kEdges][BN / 32];  // per edge tile: its slots with values that are not finite
@@ -71,7 +82,7 @@ struct Shared {
 };
 
 struct Maps {
-  CUtensorMap k, v;
+  CUtensorMap k, v, low;
   int32_t row_mul, head_mul;  // 0: all rows (heads) share one entry
 };
 
@@ -130,6 +141,16 @@ template <> struct Half16<__nv_bfloat16> {
   }
 };
 
+__device__ __forceinline__ void unpack8(const uint4& v, float (&x)[8]) {  // of bfloat16
+  const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&v);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 f = __bfloat1622float2(h[i]);
+    x[2 * i] = f.x;
+    x[2 * i + 1] = f.y;
+  }
+}
+
 // A bounded wait that also ends when another role has given up.
 __device__ __noinline__ bool wait_slow(Shared& sh, uint32_t bar, uint32_t phase) {
   const uint64_t t0 = gtimer_ns();
@@ -162,11 +183,15 @@ struct Item {
 
 // PAIRED: blocks of one query tile (and one item each), whose steps the two softmax groups
 // and product warps take in turn, each with an output of its own, joined at the end.
-template <typename T, int DC, bool PAIRED>
+// T: the queries' and the output's type; H: that of the products' operands.
+template <typename T, int DC, bool PAIRED, Source SRC>
 __global__ void __launch_bounds__(NT, 1) attn_tile_kernel(const __grid_constant__ AttnArgs a,
                                                           const __grid_constant__ Maps maps, const bool prefix,
                                                           const int tiles_m, const int units, const int items) {
-  using L = Layout<DC>;
+  using L = Layout<DC, SRC>;
+  using H = std::conditional_t<SRC == kPlain, T, __half>;
+  constexpr int RING = L::RING, STAGES = L::STAGES;
+  static_assert(!PAIRED || RING % 2 == 0, "a group's every other step alternates a barrier's phase");
   constexpr int LPR = DC * 8, RPI = 32 / LPR;  // lanes of a row's 16-byte vectors, rows per warp instruction
   extern __shared__ unsigned char dyn_raw[];
   __shared__ Shared sh;
@@ -261,9 +286,28 @@ __global__ void __launch_bounds__(NT, 1) attn_tile_kernel(const __grid_constant_
     }
 #pragma unroll
     for (int k = 0; k < LPR; ++k) {
-      v[k].x ^= flip, v[k].y ^= flip, v[k].z ^= flip, v[k].w ^= flip;
+      if constexpr (SRC == kHalves) {
+        float x[8], most = 0.f;
+        unpack8(v[k], x);
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (fabsf(x[e]) < INFINITY) most = fmaxf(most, fabsf(x[e]));
+#pragma unroll
+        for (int e = 1; e < LPR; e <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, e));
+        // The row's largest value to [2^14, 2^15), with the scale's sign.
+        const int ex = max(15, (int)(__float_as_uint(most) >> 23));
+        const float up = copysignf(__uint_as_float((uint32_t)(268 - min(ex, 254)) << 23), a.scale);
+        v[k] = make_uint4(Half16<H>::pack(x[0] * up, x[1] * up), Half16<H>::pack(x[2] * up, x[3] * up),
+                          Half16<H>::pack(x[4] * up, x[5] * up), Half16<H>::pack(x[6] * up, x[7] * up));
+        // (Zero would make NaN of hidden slots' -infinity.)
+        if (my_vec == 0)
+          sh.row_scale[wg][my_row + k * RPI] = fmaxf(fabsf(a.scale) * __uint_as_float((uint32_t)(min(ex, 254) - 14) << 23), 0x1p-126f);
+      } else {
+        v[k].x ^= flip, v[k].y ^= flip, v[k].z ^= flip, v[k].w ^= flip;
+      }
       *q_vec(my_row + k * RPI, my_vec) = v[k];
     }
+    if (SRC == kHalves) __syncwarp();
     fence_proxy_async_smem();
   };
 
@@ -305,6 +349,7 @@ __global__ void __launch_bounds__(NT, 1) attn_tile_kernel(const __grid_constant_
     if (lane == 0) {
       tma_prefetch_map(&maps.k);
       tma_prefetch_map(&maps.v);
+      if (SRC == kPairs) tma_prefetch_map(&maps.low);
       int issued = 0;
       bool ok = true;
       for (int w = blockIdx.x; ok && w < items; w += gridDim.x) {
@@ -317,12 +362,18 @@ __global__ void __launch_bounds__(NT, 1) attn_tile_kernel(const __grid_constant_
           if (!ok) break;
           int j0, jend;
           tile_at(it, x >> 1, j0, jend);
-          mbar_expect_tx(&sh.full[st], L::kTile);
+          const bool low = SRC == kPairs && !(x & 1);
+          mbar_expect_tx(&sh.full[st], low ? 2 * L::kTile : L::kTile);
           const CUtensorMap* map = x & 1 ? &maps.v : &maps.k;
 #pragma unroll
           for (int d = 0; d < DC; ++d)
             tma_load4(dyn + L::kRing + st * L::kTile + d * L::kHalf, map, d * 64, j0, it.h * maps.head_mul,
                       it.r * maps.row_mul, &sh.full[st]);
+          if (low)
+#pragma unroll
+            for (int d = 0; d < DC; ++d)
+              tma_load4(dyn + L::kLow + step * L::kTile + d * L::kHalf, &maps.low, d * 64, j0, it.h * maps.head_mul,
+                        it.r * maps.row_mul, &sh.full[st]);
         }
       }
       // Nothing may still be landing when the block ends.  (Without an abort its steps wait for it
@@ -331,7 +382,7 @@ __global__ void __launch_bounds__(NT, 1) attn_tile_kernel(const __grid_constant_
     }
   } else if (warp == 9 || warp == 10) {
     // ------------------------------------------------------------- products
-    constexpr uint32_t wqk = mma_word(Half16<T>::bf16, BN, false), wpv = mma_word(Half16<T>::bf16, 64 * DC, true);
+    constexpr uint32_t wqk = mma_word(Half16<H>::bf16, BN, false), wpv = mma_word(Half16<H>::bf16, 64 * DC, true);
     constexpr uint32_t kStep = L::kTile >> 4, kQStep = L::kQTile >> 4;
     const int t = warp - 9;
     const bool leader = elect_one();
@@ -342,7 +393,8 @@ __global__ void __launch_bounds__(NT, 1) attn_tile_kernel(const __grid_constant_
     const uint32_t s_at = tm + t * 128, o_at = tm + 256 + t * 128;
     const uint64_t qd = smem_desc(smem_u32(dyn), 16) + (PAIRED ? 0 : t * kQStep);
     const uint64_t k_desc = smem_desc(smem_u32(dyn) + L::kRing, 16),
-                   v_desc = smem_desc(smem_u32(dyn) + L::kRing, L::kHalf);
+                   v_desc = smem_desc(smem_u32(dyn) + L::kRing, L::kHalf),
+                   low_desc = smem_desc(smem_u32(dyn) + L::kLow, 16);
     // One lane waits and issues.  After an abort its waits fail at once and the rest of the
     // loop computes on what is there, which nobody uses.
     auto qk = [&](int J, int P) {
@@ -351,6 +403,13 @@ __global__ void __launch_bounds__(NT, 1) attn_tile_kernel(const __grid_constant_
       for (int k = 0; k < 4 * DC; ++k)
         mma_ss(s_at + (P & 1) * BN, qd + (((k >> 2) * L::kQHalf + (k & 3) * 32) >> 4),
                kd + (((k >> 2) * L::kHalf + (k & 3) * 32) >> 4), wqk, k != 0);
+      if constexpr (SRC == kPairs) {
+        const uint64_t ld = low_desc + J % RING * kStep;
+#pragma unroll
+        for (int k = 0; k < 4 * DC; ++k)
+          mma_ss(s_at + (P & 1) * BN, qd + (((k >> 2) * L::kQHalf + (k & 3) * 32) >> 4),
+                 ld + (((k >> 2) * L::kHalf + (k & 3) * 32) >> 4), wqk, true);
+      }
       mma_commit(&sh.s_full[t][J % RING]);
     };
     int base_ = 0, queries = 0;
@@ -378,6 +437,10 @@ __global__ void __launch_bounds__(NT, 1) attn_tile_kernel(const __grid_constant_
 #pragma unroll
           for (int k = 0; k < BN / 16; ++k)
             if (k < blocks) mma_ts(o_at, s_at + (c & 1) * BN + k * 8, vd + k * (2048 >> 4), wpv, c != 0 || k != 0);
+          if (SRC == kPairs)
+#pragma unroll
+            for (int k = 0; k < BN / 16; ++k)
+              if (k < blocks) mma_ts(o_at, s_at + (c & 1) * BN + 32 + k * 8, vd + k * (2048 >> 4), wpv, true);
           mma_commit(&sh.pv_done[t][j % RING]);
           if (j + 4 < steps) {
             wait_one(sh, &sh.full[ki % STAGES], (ki / STAGES) & 1);
@@ -427,6 +490,10 @@ __global__ void __launch_bounds__(NT, 1) attn_tile_kernel(const __grid_constant_
 #pragma unroll
           for (int k = 0; k < BN / 16; ++k)
             if (k < blocks) mma_ts(o_at, s_at + (J & 1) * BN + k * 8, vd + k * (2048 >> 4), wpv, j != 0 || k != 0);
+          if (SRC == kPairs)
+#pragma unroll
+            for (int k = 0; k < BN / 16; ++k)
+              if (k < blocks) mma_ts(o_at, s_at + (J & 1) * BN + 32 + k * 8, vd + k * (2048 >> 4), wpv, true);
           mma_commit(&sh.pv_done[t][J % RING]);
           if (j + 2 < steps) {
             wait_one(sh, &sh.full[ki % STAGES], (ki / STAGES) & 1);
@@ -488,7 +555,7 @@ __global__ void __launch_bounds__(NT, 1) attn_tile_kernel(const __grid_constant_
           const int n = min(jend - j0, BN), last = 16 * value_blocks(j0, jend);
           const int seen0 = sink ? 0 : min(max(whole.from - j0, 0), n), seen1 = sink ? n : min(max(whole.to - j0, seen0), n);
           auto look = [&](int r0, int r1) {
-            constexpr uint32_t E = Half16<T>::expo * 0x10001u;
+            constexpr uint32_t E = Half16<H>::expo * 0x10001u;
             constexpr int kAhead = 4;  // vectors of a lane in flight
 #pragma unroll 1
             for (int d = 0; d < DC; ++d) {
@@ -542,7 +609,6 @@ __global__ void __launch_bounds__(NT, 1) attn_tile_kernel(const __grid_constant_
   } else {
     // ------------------------------------------------------------- softmax and output
     const int t = wg, row = tid & 127;
-    const float scale = fabsf(a.scale);
     const uint32_t lanes = tmem + ((uint32_t)(warp & 3) << 21);
     const uint32_t o_at = lanes + 256 + t * 128;
     const bool direct = !prefix && a.o_splits == 0;
@@ -558,6 +624,8 @@ __global__ void __launch_bounds__(NT, 1) attn_tile_kernel(const __grid_constant_
       }
       float ref = -INFINITY, l = 0.f;
       bool ok = true;
+      // (With two groups at one query tile there is one item, whose rows' scales all threads saw at the start.)
+      const float scale = SRC == kHalves ? sh.row_scale[PAIRED ? 0 : t][row] : fabsf(a.scale);
       const int mfirst = it.m0 + (PAIRED ? 0 : t * BM), mlast = min(mfirst + BM, rows_m) - 1, m = mfirst + row;
       const int pos = prefix ? a.prefix : it.end - a.n + m / a.group, low = prefix ? 0 : window_low(a, it.start, pos);
       // The item's rows are neighbours in the partial results (per head, for the prefix: all
@@ -638,9 +706,18 @@ __global__ void __launch_bounds__(NT, 1) attn_tile_kernel(const __grid_constant_
             x = ex2_here(x);
             y = ex2_here(y);
             sum[k & 1] = add2(sum[k & 1], pack2(x, y));
-            p[k] = Half16<T>::pack(x, y);
+            p[k] = Half16<H>::pack(x, y);
+            if constexpr (SRC == kPairs) {  // over the scores' place: what the rounding left, behind the weights
+              const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&p[k]));
+              s[k] = __uint_as_float(Half16<H>::pack(x - h.x, y - h.y));
+            }
           }
           tmem_store32(s_at, p);
+          if constexpr (SRC == kPairs) {
+#pragma unroll
+            for (int k = 0; k < 32; ++k) p[k] = __float_as_uint(s[k]);
+            tmem_store32(s_at + 32, p);
+          }
           if (both) turn_pass(t);
           float sx, sy;
           unpack2(add2(sum[0], sum[1]), sx, sy);
@@ -711,7 +788,7 @@ __global__ void __launch_bounds__(NT, 1) attn_tile_kernel(const __grid_constant_
               if (!(sh.bad[e / BN][(e % BN) >> 5] >> (e & 31) & 1u)) continue;
               const int slot = sh.bad_from[e / BN] + e % BN;
               if (!prefix && !slot_seen(a, it.start, pos, low, slot)) continue;
-              const T* vp = static_cast<const T*>(prefix ? a.pv : a.v) +
+              const H* vp = static_cast<const H*>(prefix ? a.pv : a.v) +
                             (prefix ? it.h * a.p_head + slot * a.p_slot
                                     : it.r * a.kv_row + it.h * a.kv_head + slot * a.kv_slot);
 #pragma unroll
@@ -817,31 +894,35 @@ bool encode(CUtensorMap* map, const AttnArgs& a, const void* base, int64_t slots
   const cuuint64_t strides[3] = {s_slot ? (cuuint64_t)s_slot * 2 : one, s_head ? (cuuint64_t)s_head * 2 : one,
                                  s_row ? (cuuint64_t)s_row * 2 : one};
   const cuuint32_t box[4] = {64, (cuuint32_t)BN, 1, 1}, steps[4] = {1, 1, 1, 1};
-  return encode_fn()(map, a.dtype == 1 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4,
+  return encode_fn()(map, a.dtype == 1 || a.halves ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4,
                      const_cast<void*>(base), dims, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE,
                      CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                      CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <typename T, int DC, bool PAIRED>
+template <typename T, int DC, bool PAIRED, Source SRC>
 cudaError_t tile(const AttnArgs& a, const Maps& maps, bool prefix, int tiles_m, cudaStream_t stream) {
   const int64_t rows_m = (int64_t)(prefix ? a.rows : 1) * a.n * a.group;
   const int64_t S = prefix ? a.p_splits : (a.o_splits ? a.o_splits : 1);
   const int64_t units = prefix ? a.kv_heads : (int64_t)a.rows * a.kv_heads;
   const int64_t items = (rows_m + tiles_m * BM - 1) / (tiles_m * BM) * S * units;
   if (items >= (int64_t)1 << 31 || (PAIRED && items > kSMs)) return cudaErrorInvalidValue;
-  const cudaError_t e = allow_smem<attn_tile_kernel<T, DC, PAIRED>>(Layout<DC>::kBytes);
+  constexpr uint32_t bytes = Layout<DC, SRC>::kBytes;
+  const cudaError_t e = allow_smem<attn_tile_kernel<T, DC, PAIRED, SRC>>(bytes);
   if (e != cudaSuccess) return e;
-  attn_tile_kernel<T, DC, PAIRED><<<(unsigned)(items < kSMs ? items : kSMs), NT, Layout<DC>::kBytes, stream>>>(
+  attn_tile_kernel<T, DC, PAIRED, SRC><<<(unsigned)(items < kSMs ? items : kSMs), NT, bytes, stream>>>(
       a, maps, prefix, tiles_m, (int)units, (int)items);
   return cudaGetLastError();
 }
 
-template <typename T>
+template <typename T, Source SRC>
 cudaError_t tile_any(const AttnArgs& a, const Maps& maps, bool prefix, const TileSplit& x, cudaStream_t stream) {
   if (a.dim <= 64)
-    return x.paired ? tile<T, 1, true>(a, maps, prefix, 1, stream) : tile<T, 1, false>(a, maps, prefix, x.tiles, stream);
-  return x.paired ? tile<T, 2, true>(a, maps, prefix, 1, stream) : tile<T, 2, false>(a, maps, prefix, x.tiles, stream);
+    return x.paired ? tile<T, 1, true, SRC>(a, maps, prefix, 1, stream) : tile<T, 1, false, SRC>(a, maps, prefix, x.tiles, stream);
+  if constexpr (SRC != kPairs) {
+    if (x.paired) return tile<T, 2, true, SRC>(a, maps, prefix, 1, stream);
+  }
+  return tile<T, 2, false, SRC>(a, maps, prefix, x.tiles, stream);
 }
 
 }  // namespace
@@ -864,12 +945,17 @@ cudaError_t launch_attn_tile(const AttnArgs& args, bool prefix, const TileSplit&
   } else {
     ok = encode(&maps.k, a, a.k, a.capacity, a.kv_heads, a.rows, a.kv_slot, a.kv_head, a.kv_row) &&
          encode(&maps.v, a, a.v, a.capacity, a.kv_heads, a.rows, a.kv_slot, a.kv_head, a.kv_row);
+    if (a.k_low)
+      ok = ok && encode(&maps.low, a, a.k_low, a.capacity, a.kv_heads, a.rows, a.kv_slot, a.kv_head, a.kv_row);
     maps.head_mul = a.kv_head != 0;
     maps.row_mul = a.kv_row != 0;
   }
   if (!ok) return cudaErrorInvalidValue;
-  return a.dtype == 1 ? tile_any<__half>(a, maps, prefix, split, stream)
-                      : tile_any<__nv_bfloat16>(a, maps, prefix, split, stream);
+  if (a.halves)
+    return a.dtype == 1 ? tile_any<__half, kPairs>(a, maps, prefix, split, stream)
+                        : tile_any<__nv_bfloat16, kHalves>(a, maps, prefix, split, stream);
+  return a.dtype == 1 ? tile_any<__half, kPlain>(a, maps, prefix, split, stream)
+                      : tile_any<__nv_bfloat16, kPlain>(a, maps, prefix, split, stream);
 }
 
 }  // namespace sv

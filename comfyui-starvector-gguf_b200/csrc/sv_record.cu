@@ -11,6 +11,8 @@
 // each rounded once from the exact number.  In f32 that is the same except next to a
 // border between two results, where it is decided in 64 bits, so that the codes do not
 // depend on how a quotient rounds.  A group with a NaN or an infinity stands for NaN.
+#include <type_traits>
+
 #include "../../include/starvector_sampling.h"
 #include "sv_attention.h"
 #include "sv_record.cuh"
@@ -48,7 +50,7 @@ __device__ __forceinline__ bool half_sure(float x, __half& h) {
   return __half_as_ushort(below) == __half_as_ushort(above);
 }
 
-// The code next to q, which was computed as (x - mid) / scale to within 2^-17.
+// The code next to q, which was computed as (x - mid) / scale to within 2^-17, less 8.
 __device__ __noinline__ float code_exactly(float x, float mid, float scale, float q) {
   const float k = floorf(q);
   const double border = (double)mid + ((double)k + 0.5) * (double)scale;  // exact: 11 bits and 16, 30 binades
@@ -57,6 +59,42 @@ __device__ __noinline__ float code_exactly(float x, float mid, float scale, floa
   if (v < border) return k;
   return (int)k & 1 ? k + 1.f : k;
 }
+
+// The smallest and the largest of eight values as they lie, NaN if one is.
+__device__ __forceinline__ void extremes(const float4 (&v)[2], float& lo, float& hi) {
+  lo = min_nan(min_nan(min_nan(v[0].x, v[0].y), min_nan(v[0].z, v[0].w)), min_nan(min_nan(v[1].x, v[1].y), min_nan(v[1].z, v[1].w)));
+  hi = max_nan(max_nan(max_nan(v[0].x, v[0].y), max_nan(v[0].z, v[0].w)), max_nan(max_nan(v[1].x, v[1].y), max_nan(v[1].z, v[1].w)));
+}
+__device__ __forceinline__ void extremes(const uint4& v, float& lo, float& hi, __half) {
+  auto f = [](uint32_t x) { return *reinterpret_cast<const __half2*>(&x); };
+  const __half2 l = __hmin2_nan(__hmin2_nan(f(v.x), f(v.y)), __hmin2_nan(f(v.z), f(v.w)));
+  const __half2 h = __hmax2_nan(__hmax2_nan(f(v.x), f(v.y)), __hmax2_nan(f(v.z), f(v.w)));
+  lo = min_nan(__low2float(l), __high2float(l));
+  hi = max_nan(__low2float(h), __high2float(h));
+}
+__device__ __forceinline__ void extremes(const uint4& v, float& lo, float& hi, __nv_bfloat16) {
+  auto f = [](uint32_t x) { return *reinterpret_cast<const __nv_bfloat162*>(&x); };
+  const __nv_bfloat162 l = __hmin2_nan(__hmin2_nan(f(v.x), f(v.y)), __hmin2_nan(f(v.z), f(v.w)));
+  const __nv_bfloat162 h = __hmax2_nan(__hmax2_nan(f(v.x), f(v.y)), __hmax2_nan(f(v.z), f(v.w)));
+  lo = min_nan(__low2float(l), __high2float(l));
+  hi = max_nan(__low2float(h), __high2float(h));
+}
+// Eight values in a thread: as loaded, their extremes, one by one.
+template <typename T> struct Eight {
+  uint4 v;
+  __device__ __forceinline__ void load(const T* p) { v = __ldg(reinterpret_cast<const uint4*>(p)); }
+  __device__ __forceinline__ void ends(float& lo, float& hi) const { extremes(v, lo, hi, T()); }
+  __device__ __forceinline__ float at(int k) const { return (float)reinterpret_cast<const T*>(&v)[k]; }
+};
+template <> struct Eight<float> {
+  float4 v[2];
+  __device__ __forceinline__ void load(const float* p) {
+    v[0] = __ldg(reinterpret_cast<const float4*>(p));
+    v[1] = __ldg(reinterpret_cast<const float4*>(p) + 1);
+  }
+  __device__ __forceinline__ void ends(float& lo, float& hi) const { extremes(v, lo, hi); }
+  __device__ __forceinline__ float at(int k) const { return reinterpret_cast<const float*>(v)[k]; }
+};
 
 // Where an item (one slot of one head, of keys or values) lies: blocks take slots of one
 // unit, or units whole where these have few slots.
@@ -90,76 +128,73 @@ __global__ void __launch_bounds__(NT) kv_quantize_kernel(const __grid_constant__
   const int slot = end - a.tokens + it.i, blocks = (a.dim + 31) >> 5;
   const bool in = it.in && slot >= 0 && i < blocks;  // (the shuffles need all lanes)
   const T* src = static_cast<const T*>(blockIdx.z ? a.in[1] : a.in[0]) + it.r * a.i_row + it.h * a.i_head + it.i * a.i_tok;
-  float x[2][8];
+  Eight<T> x[2];
   bool has[2];
 #pragma unroll
   for (int e = 0; e < 2; ++e) {
     const int d = 32 * i + 16 * e + 8 * y;
     has[e] = in && d < a.dim;
-    if (has[e]) load8(src + d, x[e]);
+    if (has[e]) x[e].load(src + d);
   }
   float lo[2], hi[2];
 #pragma unroll
   for (int e = 0; e < 2; ++e) {
     lo[e] = INFINITY;
     hi[e] = -INFINITY;
-    if (has[e]) {
-#pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        lo[e] = min_nan(lo[e], x[e][k]);
-        hi[e] = max_nan(hi[e], x[e][k]);
-      }
-    }
+    if (has[e]) x[e].ends(lo[e], hi[e]);
   }
-  const bool wide = a.dim > 64;  // groups of 32
+  constexpr bool wide = LPS_LOG2 == 3;  // groups of 32
   if (wide) {
     lo[0] = min_nan(lo[0], lo[1]);
     hi[0] = max_nan(hi[0], hi[1]);
   }
 #pragma unroll
-  for (int e = 0; e < 2; ++e) {
-    if (e && wide) break;
+  for (int e = 0; e < (wide ? 1 : 2); ++e) {
     lo[e] = min_nan(lo[e], __shfl_xor_sync(0xffffffffu, lo[e], 1));
     hi[e] = max_nan(hi[e], __shfl_xor_sync(0xffffffffu, hi[e], 1));
   }
   uint32_t word[2] = {0u, 0u};
   uint32_t pair[2] = {0u, 0u};
   float scale = 0.f, mid = 0.f, inv = 0.f;
+  bool clamps = false, none = true;
 #pragma unroll
   for (int e = 0; e < 2; ++e) {
     if (!e || !wide) {
-      // Without a value (dimensions past head_dim): zeros.
-      const bool none = lo[e] > hi[e], bad = !none && !(lo[e] > -INFINITY && hi[e] < INFINITY);
+      // Without a value (dimensions past head_dim): zeros.  With one that is not finite: NaN.
+      none = lo[e] > hi[e];
+      const bool bad = !none && !(lo[e] > -INFINITY && hi[e] < INFINITY);
+      clamps = lo[e] < -kRecordMost || hi[e] > kRecordMost;
       const float l = fminf(fmaxf(lo[e], -kRecordMost), kRecordMost), h = fminf(fmaxf(hi[e], -kRecordMost), kRecordMost);
       __half s16, m16;
       if (!half_sure((h - l) * (1.f / 15.f), s16)) s16 = __double2half(((double)h - (double)l) / 15.0);
       scale = __half2float(s16);
       if (!half_sure(fmaf(8.f, scale, l), m16)) m16 = __double2half((double)l + 8.0 * (double)scale);
       mid = __half2float(m16);
-      inv = scale > 0.f ? 1.f / scale : 0.f;
+      inv = scale > 0.f ? __fdividef(1.f, scale) : 0.f;  // (to within two units in the last place)
       pair[e] = none ? 0u : bad ? 0x7e007e00u : (uint32_t)__half_as_ushort(s16) | (uint32_t)__half_as_ushort(m16) << 16;
-      if (none || bad) has[e] = false, has[1] = has[1] && (!wide || e);
+      none = none || bad;
     }
-    if (has[e]) {
-      float q[8], edge = 0.f;
+    if (has[e] && !none) {
+      // The whole number next to q by adding 1.5 2^23, whose last bits it then is (with 8 more, the code).
+      constexpr float kAdd = 12582912.f + 8.f;
+      float q[8], r[8], edge = 0.f;
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
-        const float v = fminf(fmaxf(x[e][k], -kRecordMost), kRecordMost);
+        float v = x[e].at(k);
+        if (clamps) v = fminf(fmaxf(v, -kRecordMost), kRecordMost);
         q[k] = fminf(fmaxf((v - mid) * inv, -8.f), 7.f);
-        const float r = rintf(q[k]);
-        edge = fmaxf(edge, fabsf(q[k] - r));
+        r[k] = q[k] + kAdd;
+        edge = fmaxf(edge, fabsf(q[k] - (r[k] - kAdd)));
       }
       if (edge > 0.5f - 0x1p-16f) {
 #pragma unroll
         for (int k = 0; k < 8; ++k)
-          if (fabsf(q[k] - rintf(q[k])) > 0.5f - 0x1p-16f)
-            q[k] = code_exactly(fminf(fmaxf(x[e][k], -kRecordMost), kRecordMost), mid, scale, q[k]);
+          if (fabsf(q[k] - (r[k] - kAdd)) > 0.5f - 0x1p-16f)
+            r[k] = code_exactly(fminf(fmaxf(x[e].at(k), -kRecordMost), kRecordMost), mid, scale, q[k]) + kAdd;
       }
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        const int c = __float2int_rn(q[k]) + 8;  // dimension 4 t + 2 a + b, t = 2 y + (k >> 2)
-        word[k >> 2] |= (uint32_t)c << 4 * (4 * (k & 1) + 2 * e + (k >> 1 & 1));
-      }
+      for (int k = 0; k < 8; ++k)  // dimension 4 t + 2 a + b, t = 2 y + (k >> 2)
+        word[k >> 2] += (__float_as_uint(r[k]) - __float_as_uint(12582912.f)) << 4 * (4 * (k & 1) + 2 * e + (k >> 1 & 1));
     }
   }
   if (!in) return;
@@ -195,13 +230,15 @@ template <> __device__ __forceinline__ void store8<__nv_bfloat16>(__nv_bfloat16*
   *reinterpret_cast<uint4*>(p) = *reinterpret_cast<const uint4*>(h);
 }
 
-template <typename T, int LPS_LOG2>
+// A thread takes PER slots, 2^slots_log2 apart: their words are on their way together.
+template <typename T, int LPS_LOG2, int PER>
 __global__ void __launch_bounds__(NT) kv_dequantize_kernel(const __grid_constant__ ReadArgs a, const int units_log2,
                                                            const int slots_log2) {
   const int lane = threadIdx.x & ((1 << LPS_LOG2) - 1), y = lane & 1, i = lane >> 1;
-  const Item it = item_at(threadIdx.x >> LPS_LOG2, units_log2, slots_log2, a.kv_heads, a.rows, a.tokens);
+  Item it = item_at(threadIdx.x >> LPS_LOG2, units_log2, slots_log2, a.kv_heads, a.rows, a.tokens);
+  if (PER > 1) it.i += (int)blockIdx.x * (PER - 1) << slots_log2;
   const int blocks = (a.dim + 31) >> 5;
-  if (!it.in || i >= blocks) return;
+  if (it.r >= a.rows || it.i >= a.tokens || i >= blocks) return;
   int end = a.capacity, given = 0;
   if (a.lengths) {
     given = a.lengths[it.r];
@@ -209,37 +246,57 @@ __global__ void __launch_bounds__(NT) kv_dequantize_kernel(const __grid_constant
   }
   if (a.status && it.h == 0 && it.i == 0 && lane == 0 && blockIdx.z == 0)
     a.status[it.r] = a.lengths && given != end ? SV_ST_LENGTH : 0;
-  const int slot = a.newest ? end - a.tokens + it.i : it.i;
+  const int shift = a.newest ? end - a.tokens : 0;
+  int start = 0, low = 0;
   if (a.seen) {
-    const int start = a.starts ? min(max(a.starts[it.r], 0), end) : 0;
-    const int low = a.window ? max(start, end - a.seen - a.window + 1) : start;
-    if (slot < start || slot >= end || (slot < low && slot >= start + a.sinks)) return;
+    start = a.starts ? min(max(a.starts[it.r], 0), end) : 0;
+    low = a.window ? max(start, end - a.seen - a.window + 1) : start;
   }
-  uint32_t word[2] = {0u, 0u}, pair[2] = {0u, 0u};
-  if (slot >= 0 && slot < end) {
-    const unsigned char* rec = (blockIdx.z ? a.cache[1] : a.cache[0]) + it.r * a.row + it.h * a.head + (int64_t)slot * a.slot;
-    const uint32_t* codes = reinterpret_cast<const uint32_t*>(rec);
-    word[0] = __ldg(codes + 2 * y * blocks + i);
-    word[1] = __ldg(codes + (2 * y + 1) * blocks + i);
-    const bool wide = a.dim > 64;
-    pair[0] = __ldg(codes + 4 * blocks + (wide ? i : 2 * i));
-    pair[1] = wide ? pair[0] : __ldg(codes + 4 * blocks + 2 * i + 1);
-  }
+  constexpr bool wide = LPS_LOG2 == 3;
+  const unsigned char* unit = (blockIdx.z ? a.cache[1] : a.cache[0]) + it.r * a.row + it.h * a.head;
   T* out = static_cast<T*>(blockIdx.z ? a.out[1] : a.out[0]) +
            (((int64_t)it.r * a.kv_heads + it.h) * a.tokens + it.i) * a.dim;
+  uint32_t word[PER][2], pair[PER][wide ? 1 : 2];
+  bool writes[PER];
 #pragma unroll
-  for (int e = 0; e < 2; ++e) {
-    const int d = 32 * i + 16 * e + 8 * y;
-    if (d >= a.dim) break;
-    const float scale = __half2float(__ushort_as_half((unsigned short)(pair[e] & 0xffffu)));
-    const float mid = __half2float(__ushort_as_half((unsigned short)(pair[e] >> 16)));
-    float x[8];
-#pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      const int c = (int)(word[k >> 2] >> 4 * (4 * (k & 1) + 2 * e + (k >> 1 & 1)) & 15u) - 8;
-      x[k] = fmaf(scale, (float)c, mid);
+  for (int x = 0; x < PER; ++x) {
+    const int place = it.i + (x << slots_log2), slot = place + shift;
+    const bool in = slot >= 0 && slot < end;
+    writes[x] = place < a.tokens && (!a.seen || (in && slot >= start && (slot >= low || slot < start + a.sinks)));
+    word[x][0] = word[x][1] = pair[x][0] = pair[x][wide ? 0 : 1] = 0u;
+    if (writes[x] && in) {
+      const uint32_t* codes = reinterpret_cast<const uint32_t*>(unit + (int64_t)slot * a.slot);
+      word[x][0] = __ldg(codes + 2 * y * blocks + i);
+      word[x][1] = __ldg(codes + (2 * y + 1) * blocks + i);
+      pair[x][0] = __ldg(codes + 4 * blocks + (wide ? i : 2 * i));
+      if (!wide) pair[x][wide ? 0 : 1] = __ldg(codes + 4 * blocks + 2 * i + 1);
     }
-    store8(out + d, x);
+  }
+#pragma unroll
+  for (int x = 0; x < PER; ++x) {
+    if (!writes[x]) continue;
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int d = 32 * i + 16 * e + 8 * y;
+      if (d >= a.dim) break;
+      const float2 sm = __half22float2(*reinterpret_cast<const __half2*>(&pair[x][wide ? 0 : e]));
+      float v[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        // The nibble as the last bits of 2^23 + c.
+        const uint32_t c = word[x][k >> 2] >> 4 * (4 * (k & 1) + 2 * e + (k >> 1 & 1)) & 15u;
+        v[k] = fmaf(sm.x, __uint_as_float(0x4b000000u | c) - 8388616.f, sm.y);
+      }
+      T* to = out + ((int64_t)x << slots_log2) * a.dim + d;
+      store8(to, v);
+      if constexpr (std::is_same<T, __half>::value) {
+        if (a.low && blockIdx.z == 0) {
+#pragma unroll
+          for (int k = 0; k < 8; ++k) v[k] -= __half2float(__float2half_rn(v[k]));
+          store8(static_cast<T*>(a.low) + (to - static_cast<T*>(a.out[0])), v);
+        }
+      }
+    }
   }
 }
 
@@ -267,13 +324,20 @@ template <typename T> cudaError_t write_records(const WriteArgs& a, cudaStream_t
 template <typename T> cudaError_t read_records(const ReadArgs& a, cudaStream_t stream) {
   int u, s;
   const int64_t units = (int64_t)a.rows * a.kv_heads;
-  auto go = [&](auto kernel, int lps_log2) {
-    const dim3 grid = grid_of(lps_log2, units, a.tokens, a.out[1] != nullptr, u, s);
-    kernel<<<grid, NT, 0, stream>>>(a, u, s);
+  auto go = [&](auto one, auto four, int lps_log2) {
+    // Four slots a thread where that still leaves several blocks per SM.
+    dim3 grid = grid_of(lps_log2, units, a.tokens, a.out[1] != nullptr, u, s);
+    if ((int64_t)grid.x * grid.y * grid.z >= 8 * 4 * 148) {
+      grid.x = (grid.x + 3) / 4;
+      four<<<grid, NT, 0, stream>>>(a, u, s);
+    } else {
+      one<<<grid, NT, 0, stream>>>(a, u, s);
+    }
     return cudaGetLastError();
   };
-  if (a.dim > 64) return go(kv_dequantize_kernel<T, 3>, 3);
-  return a.dim > 32 ? go(kv_dequantize_kernel<T, 2>, 2) : go(kv_dequantize_kernel<T, 1>, 1);
+  if (a.dim > 64) return go(kv_dequantize_kernel<T, 3, 1>, kv_dequantize_kernel<T, 3, 4>, 3);
+  return a.dim > 32 ? go(kv_dequantize_kernel<T, 2, 1>, kv_dequantize_kernel<T, 2, 4>, 2)
+                    : go(kv_dequantize_kernel<T, 1, 1>, kv_dequantize_kernel<T, 1, 4>, 1);
 }
 
 // What both calls take of a cache.
