@@ -224,7 +224,7 @@ struct RecordPlan {
 RecordPlan record_plan(const AttnArgs& a) {
   RecordPlan p = {};
   const int64_t nG = (int64_t)a.n * a.group, units = (int64_t)a.rows * a.kv_heads, all = units * nG;
-  p.rows.tiles = nG <= 8 ? 1 : 2;
+  p.rows.tiles = nG <= 8 || a.dtype == SV_F32 ? 1 : 2;
   p.rows.groups = div_up(nG, 8 * p.rows.tiles);
   p.counters = SV_ATTENTION_ZERO_BYTES;
   p.o_bytes = up256((size_t)2 * kTokenBlocks * 8 * p.rows.tiles * record_dims(a.dim) * 4);
@@ -232,7 +232,7 @@ RecordPlan record_plan(const AttnArgs& a) {
   p.lse_bytes = a.weights ? up256(all * 4) : 0;
   p.score_bytes = a.weights ? up256(all * a.capacity * 4) : 0;
   // A unit's counter each, and chunks (of at least 128 slots) counted in 31 bits.
-  p.direct = a.dtype != SV_F32 && p.rows.groups <= kMostRecordGroups && units * p.rows.groups <= 65536 &&
+  p.direct = p.rows.groups <= kMostRecordGroups && units * p.rows.groups <= 65536 &&
              units * p.rows.groups * (a.capacity / 128 + 3) < (int64_t)1 << 31 && p.score_bytes <= kMostScores;
   if (!p.direct) {
     p.halves = a.dtype != SV_F32 && !a.weights;  // (the accumulated weights' product takes keys of the queries' type)

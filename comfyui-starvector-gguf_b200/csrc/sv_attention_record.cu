@@ -15,6 +15,8 @@
 // Values are formed in float16, v = scale (c - 8) + mid rounded once, and the weights rounded to
 // float16, for float16 outputs in two halves: one such rounding is about what the output's own adds (error of
 // one token's output 0.0003 against 64 bits, 0.0002 that of the output's rounding alone; with both 0.00032).
+// Float32: queries in two float16 pieces, weights and values in three bfloat16 pieces each and the six products
+// that count.
 // The softmax as in sv_attention_token.cu: the reference moves only when a score exceeds it by
 // 2^8.
 //
@@ -69,6 +71,30 @@ __device__ __forceinline__ void mma_add(float (&d)[4], uint32_t a0, uint32_t a1,
   asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_bf16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                         uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// Two values rounded to bfloat16, which are taken off them.
+__device__ __forceinline__ uint32_t next_piece(float2& x) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(x.x, x.y);
+  const float2 f = __bfloat1622float2(h);
+  x.x -= f.x;
+  x.y -= f.y;
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+// Float32: the values of nibble j of two slots' 16-bit halves, in three bfloat16 pieces each.
+__device__ __forceinline__ void pieces(uint32_t w, int j, uint32_t scale, uint32_t mid, uint32_t& a, uint32_t& b, uint32_t& c) {
+  const float2 s = __half22float2(*reinterpret_cast<const __half2*>(&scale)), m = __half22float2(*reinterpret_cast<const __half2*>(&mid));
+  const float c0 = __uint_as_float((w >> 4 * j & 15u) | 0x4b000000u) - 8388616.f;  // 2^23 + c - (2^23 + 8)
+  const float c1 = __uint_as_float((w >> (16 + 4 * j) & 15u) | 0x4b000000u) - 8388616.f;
+  float2 v = make_float2(fmaf(s.x, c0, m.x), fmaf(s.y, c1, m.y));
+  a = next_piece(v);
+  b = next_piece(v);
+  c = next_piece(v);
 }
 __device__ __forceinline__ uint32_t transposed(uint32_t x) {
   uint32_t y;
@@ -175,8 +201,9 @@ __global__ void __launch_bounds__(NW * 32, 1)
   using F = Form<NI>;
   constexpr int REC = F::REC, NG = F::NG, NB = F::NB, MT = 4 * NB, ROWS = 8 * NT, THREADS = NW * 32;
   constexpr int OS = 32 * NI;  // dimensions of the warps' outputs
-  constexpr bool HALVES = std::is_same<T, __half>::value;
-  constexpr bool KEEP_Q = NT * NW <= 16;  // the queries' operands in registers
+  constexpr bool HALVES = std::is_same<T, __half>::value, FULL = std::is_same<T, float>::value;
+  constexpr int QP = FULL ? 2 : 1, WP = FULL ? 3 : HALVES ? 2 : 1;  // pieces of a query, of a weight
+  constexpr bool KEEP_Q = NT * NW <= 16 && !FULL;                   // the queries' operands in registers
   constexpr uint32_t kOnes = 0x3c003c00u;
   // [NW][RING][keys, values of a tile], then [NW][ROWS][OS] floats.
   extern __shared__ __align__(16) unsigned char ring_bytes[];
@@ -185,7 +212,7 @@ __global__ void __launch_bounds__(NW * 32, 1)
   __shared__ float factor[kMaxFlat > NW ? kMaxFlat : NW][ROWS];
   __shared__ float2 part_ml[kMaxFlat][ROWS];
   __shared__ float2 joined[ROWS];
-  __shared__ uint4 sh_q[NT][NI][32];
+  __shared__ uint4 sh_q[QP][NT][NI][32];
   __shared__ uint2 sh_qm[NT][32];
   __shared__ float sh_fr[ROWS];
   __shared__ int scan[NW];
@@ -313,7 +340,8 @@ __global__ void __launch_bounds__(NW * 32, 1)
 
   // ---- queries, for the whole block, row tile u by warp u: the B operand of each step over 16 dimensions, the
   // groups' sums in halves, the rows' factors
-  uint2 raw[NI][2];
+  using Four = std::conditional_t<FULL, uint4, uint2>;  // four values as they lie
+  Four raw[NI][2];
   auto load_q = [&](int r, int h) {
     const int head = h / row_groups, m = (h - head * row_groups) * ROWS + 8 * warp + g, i = MULTI ? m / group : 0;
     const T* src = static_cast<const T*>(a.q) + r * a.q_row + i * a.q_tok + (int64_t)(head * group + m - i * group) * a.q_head;
@@ -322,7 +350,8 @@ __global__ void __launch_bounds__(NW * 32, 1)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const int d = 32 * b + 16 * e + 4 * t;
-        raw[b][e] = warp < NT && m < nG && d < D ? __ldg(reinterpret_cast<const uint2*>(src + d)) : make_uint2(0u, 0u);
+        raw[b][e] = Four();
+        if (warp < NT && m < nG && d < D) raw[b][e] = __ldg(reinterpret_cast<const Four*>(src + d));
       }
   };
   auto make_q = [&]() {
@@ -356,8 +385,21 @@ __global__ void __launch_bounds__(NW * 32, 1)
           x[b][e][k] *= up;
           sum[NI > 2 ? b : 2 * b + e] += x[b][e][k];
         }
-      sh_q[warp][b][lane] = make_uint4(pack16(x[b][0][0], x[b][0][1]), pack16(x[b][0][2] * 0.0625f, x[b][0][3] * 0.0625f),
-                                       pack16(x[b][1][0], x[b][1][1]), pack16(x[b][1][2] * 0.0625f, x[b][1][3] * 0.0625f));
+#pragma unroll
+      for (int y = 0; y < QP; ++y) {
+        const uint4 q = make_uint4(pack16(x[b][0][0], x[b][0][1]), pack16(x[b][0][2] * 0.0625f, x[b][0][3] * 0.0625f),
+                                   pack16(x[b][1][0], x[b][1][1]), pack16(x[b][1][2] * 0.0625f, x[b][1][3] * 0.0625f));
+        sh_q[y][warp][b][lane] = q;
+        if (y + 1 < QP) {  // what the rounding left
+          const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&w[k]));
+            x[b][k >> 1][2 * (k & 1)] -= k & 1 ? 16.f * h.x : h.x;
+            x[b][k >> 1][2 * (k & 1) + 1] -= k & 1 ? 16.f * h.y : h.y;
+          }
+        }
+      }
     }
     // Group t's sum, in the keys' units; in halves, for scale (times -8) and mid.
     float own = 0.f;
@@ -365,7 +407,7 @@ __global__ void __launch_bounds__(NW * 32, 1)
     for (int k = 0; k < NG; ++k) {
       sum[k] += __shfl_xor_sync(0xffffffffu, sum[k], 1);
       sum[k] += __shfl_xor_sync(0xffffffffu, sum[k], 2);
-      if (k == t) own = sum[k] * 0x1p-24f;
+      if (k == t) own = sum[k] * (FULL ? 0x1p-14f : 0x1p-24f);  // (float32: clear of float16's subnormals)
     }
     const float high = __half2float(__float2half_rn(own));
     sh_qm[warp][lane] = make_uint2(pack16(-8.f * high, high), pack16(-8.f * (own - high), own - high));
@@ -380,8 +422,8 @@ __global__ void __launch_bounds__(NW * 32, 1)
     const float inv = L == 0.f ? 0.f : 1.f / L;
     const int i = MULTI ? m / group : 0;
     T* out = static_cast<T*>(a.out) + (((int64_t)r * a.n + i) * a.heads + head * group + m - i * group) * D + d;
-    T y[4] = {from_float<T>(x.x * inv), from_float<T>(x.y * inv), from_float<T>(x.z * inv), from_float<T>(x.w * inv)};
-    *reinterpret_cast<uint2*>(out) = *reinterpret_cast<const uint2*>(y);
+    alignas(16) T y[4] = {from_float<T>(x.x * inv), from_float<T>(x.y * inv), from_float<T>(x.z * inv), from_float<T>(x.w * inv)};
+    *reinterpret_cast<Four*>(out) = *reinterpret_cast<const Four*>(y);
   };
   auto write_lse = [&](int r, int head, int m, float2 j) {
     if (a.lse) a.lse[(int64_t)(r * a.kv_heads + head) * nG + m] = j.y == 0.f ? INFINITY : j.x + log2f(j.y);
@@ -439,7 +481,7 @@ __global__ void __launch_bounds__(NW * 32, 1)
       if constexpr (KEEP_Q) {
         qm[u] = sh_qm[u][lane];
 #pragma unroll
-        for (int b = 0; b < NI; ++b) qb[u][b] = sh_q[u][b][lane];
+        for (int b = 0; b < NI; ++b) qb[u][b] = sh_q[0][u][b][lane];
       }
       const float2 both = *reinterpret_cast<const float2*>(&sh_fr[8 * u + 2 * t]);
       fr[u][0] = both.x;
@@ -481,6 +523,10 @@ __global__ void __launch_bounds__(NW * 32, 1)
         for (int u = 0; u < NT; ++u) {
           const uint2 q = KEEP_Q ? qm[u] : sh_qm[u][lane];
           mma_new(s[u], own[0], own[1], own[0], own[1], q.x, q.y);
+          if constexpr (FULL) {
+#pragma unroll
+            for (int y = 0; y < 4; ++y) s[u][y] *= 0x1p-10f;
+          }
         }
 #pragma unroll
         for (int grp = 0; grp < NG; ++grp) {
@@ -490,14 +536,16 @@ __global__ void __launch_bounds__(NW * 32, 1)
           for (int e = NI > 2 ? 0 : grp & 1; e < (NI > 2 ? 2 : (grp & 1) + 1); ++e) {
             const uint32_t w0 = e ? kw[0][b] >> 8 : kw[0][b], w1 = e ? kw[1][b] >> 8 : kw[1][b];
 #pragma unroll
-            for (int u = 0; u < NT; ++u) {
-              const uint4 q = KEEP_Q ? qb[KEEP_Q ? u : 0][b] : sh_q[u][b][lane];
-              const uint32_t b0 = e ? q.z : q.x, b1 = e ? q.w : q.y;
-              if (NI > 2 && e)
-                mma_add(acc[u], w0 & 0x000f000fu, w1 & 0x000f000fu, w0 & 0x00f000f0u, w1 & 0x00f000f0u, b0, b1);
-              else
-                mma_new(acc[u], w0 & 0x000f000fu, w1 & 0x000f000fu, w0 & 0x00f000f0u, w1 & 0x00f000f0u, b0, b1);
-            }
+            for (int y = 0; y < QP; ++y)
+#pragma unroll
+              for (int u = 0; u < NT; ++u) {
+                const uint4 q = KEEP_Q ? qb[KEEP_Q ? u : 0][b] : sh_q[y][u][b][lane];
+                const uint32_t b0 = e ? q.z : q.x, b1 = e ? q.w : q.y;
+                if ((NI > 2 && e) || y)
+                  mma_add(acc[u], w0 & 0x000f000fu, w1 & 0x000f000fu, w0 & 0x00f000f0u, w1 & 0x00f000f0u, b0, b1);
+                else
+                  mma_new(acc[u], w0 & 0x000f000fu, w1 & 0x000f000fu, w0 & 0x00f000f0u, w1 & 0x00f000f0u, b0, b1);
+              }
           }
 #pragma unroll
           for (int x = 0; x < 2; ++x) {
@@ -565,7 +613,7 @@ __global__ void __launch_bounds__(NW * 32, 1)
       }
       // As B operand of the values' product: slots of rows 0..7 and 8..15 of the tile's order (float16 outputs: and
       // what their rounding left).
-      uint32_t pw[HALVES ? 2 : 1][NT][2];
+      uint32_t pw[WP][NT][2];
 #pragma unroll
       for (int u = 0; u < NT; ++u)
 #pragma unroll
@@ -573,6 +621,12 @@ __global__ void __launch_bounds__(NW * 32, 1)
           const float w0 = ex2(z[u][x][0]), w1 = ex2(z[u][x][1]);
           l[u][0] += w0;
           l[u][1] += w1;
+          if constexpr (FULL) {
+            float2 rest = make_float2(w0, w1);
+#pragma unroll
+            for (int y = 0; y < 3; ++y) pw[y][u][x] = transposed(next_piece(rest));
+            continue;
+          }
           const uint32_t both = pack16(w0, w1);
           pw[0][u][x] = transposed(both);
           if constexpr (HALVES) {
@@ -640,12 +694,28 @@ __global__ void __launch_bounds__(NW * 32, 1)
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const int y = NI > 2 ? b : j >> 1;
-          const uint32_t a0 = value(l0, j, sc[0][y], mi[0][y]), a1 = value(h0, j, sc[0][y], mi[0][y]);
-          const uint32_t a2 = value(l1, j, sc[1][y], mi[1][y]), a3 = value(h1, j, sc[1][y], mi[1][y]);
+          if constexpr (FULL) {
+            uint32_t v[3][4];
+            pieces(l0, j, sc[0][y], mi[0][y], v[0][0], v[1][0], v[2][0]);
+            pieces(h0, j, sc[0][y], mi[0][y], v[0][1], v[1][1], v[2][1]);
+            pieces(l1, j, sc[1][y], mi[1][y], v[0][2], v[1][2], v[2][2]);
+            pieces(h1, j, sc[1][y], mi[1][y], v[0][3], v[1][3], v[2][3]);
+            // The smallest products first; those below 2^-24 of the whole are left out.
 #pragma unroll
-          for (int z = 0; z < (HALVES ? 2 : 1); ++z)
+            for (int z = 2; z >= 0; --z)
 #pragma unroll
-            for (int u = 0; u < NT; ++u) mma_add(o[u][4 * b + j], a0, a1, a2, a3, pw[z][u][0], pw[z][u][1]);
+              for (int x = z; x >= 0; --x)
+#pragma unroll
+                for (int u = 0; u < NT; ++u)
+                  mma_bf16(o[u][4 * b + j], v[x][0], v[x][1], v[x][2], v[x][3], pw[z - x][u][0], pw[z - x][u][1]);
+          } else {
+            const uint32_t a0 = value(l0, j, sc[0][y], mi[0][y]), a1 = value(h0, j, sc[0][y], mi[0][y]);
+            const uint32_t a2 = value(l1, j, sc[1][y], mi[1][y]), a3 = value(h1, j, sc[1][y], mi[1][y]);
+#pragma unroll
+            for (int z = 0; z < WP; ++z)
+#pragma unroll
+              for (int u = 0; u < NT; ++u) mma_add(o[u][4 * b + j], a0, a1, a2, a3, pw[z][u][0], pw[z][u][1]);
+          }
         }
       }
       if (MULTI && hide) {
@@ -654,11 +724,16 @@ __global__ void __launch_bounds__(NW * 32, 1)
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             const int y = NI > 2 ? b : j >> 1;
-            const uint32_t x0 = bad[0][y] & kOnes, x1 = bad[1][y] & kOnes;
+            const uint32_t one = FULL ? 0x3f803f80u : kOnes, x0 = bad[0][y] & one, x1 = bad[1][y] & one;
 #pragma unroll
             for (int u = 0; u < NT; ++u) {
               float seen[4];
-              mma_new(seen, x0, x0, x1, x1, pw[0][u][0], pw[0][u][1]);
+              if constexpr (FULL) {
+                seen[0] = seen[1] = seen[2] = seen[3] = 0.f;
+                mma_bf16(seen, x0, x0, x1, x1, pw[0][u][0], pw[0][u][1]);
+              } else {
+                mma_new(seen, x0, x0, x1, x1, pw[0][u][0], pw[0][u][1]);
+              }
 #pragma unroll
               for (int q = 0; q < 4; ++q)
                 if (seen[q] != 0.f) o[u][4 * b + j][q] = __int_as_float(0x7fc00000);
@@ -848,8 +923,10 @@ cudaError_t record(const AttnArgs& a, int row_groups, cudaStream_t stream) {
 }
 
 template <typename T, int NI, bool MULTI> cudaError_t record_rows(const AttnArgs& a, const RecordRows& x, cudaStream_t stream) {
-  if (x.tiles == 1) return record<T, NI, 1, 12, 4, MULTI>(a, x.groups, stream);
-  return record<T, NI, 2, 8, 5, MULTI>(a, x.groups, stream);
+  if constexpr (!std::is_same<T, float>::value) {
+    if (x.tiles == 2) return record<T, NI, 2, 8, 5, MULTI>(a, x.groups, stream);
+  }
+  return record<T, NI, 1, 12, 4, MULTI>(a, x.groups, stream);
 }
 
 template <typename T> cudaError_t record_any(const AttnArgs& a, const RecordRows& x, cudaStream_t stream) {
@@ -865,6 +942,7 @@ template <typename T> cudaError_t record_any(const AttnArgs& a, const RecordRows
 }  // namespace
 
 cudaError_t launch_attn_record(const AttnArgs& a, const RecordRows& x, cudaStream_t stream) {
+  if (a.dtype == 0) return record_any<float>(a, x, stream);
   return a.dtype == 1 ? record_any<__half>(a, x, stream) : record_any<__nv_bfloat16>(a, x, stream);
 }
 

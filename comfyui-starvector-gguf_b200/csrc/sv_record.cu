@@ -85,6 +85,10 @@ template <typename T> struct Eight {
   __device__ __forceinline__ void load(const T* p) { v = __ldg(reinterpret_cast<const uint4*>(p)); }
   __device__ __forceinline__ void ends(float& lo, float& hi) const { extremes(v, lo, hi, T()); }
   __device__ __forceinline__ float at(int k) const { return (float)reinterpret_cast<const T*>(&v)[k]; }
+  __device__ __forceinline__ void clamp() {  // (the bounds are exact in either type)
+#pragma unroll
+    for (int k = 0; k < 8; ++k) reinterpret_cast<T*>(&v)[k] = from_float<T>(fminf(fmaxf(at(k), -kRecordMost), kRecordMost));
+  }
 };
 template <> struct Eight<float> {
   float4 v[2];
@@ -94,6 +98,10 @@ template <> struct Eight<float> {
   }
   __device__ __forceinline__ void ends(float& lo, float& hi) const { extremes(v, lo, hi); }
   __device__ __forceinline__ float at(int k) const { return reinterpret_cast<const float*>(v)[k]; }
+  __device__ __forceinline__ void clamp() {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) reinterpret_cast<float*>(v)[k] = fminf(fmaxf(at(k), -kRecordMost), kRecordMost);
+  }
 };
 
 // Where an item (one slot of one head, of keys or values) lies: blocks take slots of one
@@ -125,7 +133,7 @@ __global__ void __launch_bounds__(NT) kv_quantize_kernel(const __grid_constant__
   }
   if (it.in && a.status && it.h == 0 && it.i == 0 && lane == 0 && blockIdx.z == 0)
     a.status[it.r] = a.lengths && given != end ? SV_ST_LENGTH : 0;
-  const int slot = end - a.tokens + it.i, blocks = (a.dim + 31) >> 5;
+  const int blocks = (a.dim + 31) >> 5, slot = end - a.tokens + it.i;
   const bool in = it.in && slot >= 0 && i < blocks;  // (the shuffles need all lanes)
   const T* src = static_cast<const T*>(blockIdx.z ? a.in[1] : a.in[0]) + it.r * a.i_row + it.h * a.i_head + it.i * a.i_tok;
   Eight<T> x[2];
@@ -148,22 +156,28 @@ __global__ void __launch_bounds__(NT) kv_quantize_kernel(const __grid_constant__
     lo[0] = min_nan(lo[0], lo[1]);
     hi[0] = max_nan(hi[0], hi[1]);
   }
+  bool clamps = false;
 #pragma unroll
   for (int e = 0; e < (wide ? 1 : 2); ++e) {
     lo[e] = min_nan(lo[e], __shfl_xor_sync(0xffffffffu, lo[e], 1));
     hi[e] = max_nan(hi[e], __shfl_xor_sync(0xffffffffu, hi[e], 1));
+    clamps |= lo[e] <= hi[e] && (lo[e] < -kRecordMost || hi[e] > kRecordMost);
+  }
+  if (__any_sync(0xffffffffu, clamps)) {
+#pragma unroll
+    for (int e = 0; e < 2; ++e)
+      if (has[e]) x[e].clamp();
   }
   uint32_t word[2] = {0u, 0u};
   uint32_t pair[2] = {0u, 0u};
   float scale = 0.f, mid = 0.f, inv = 0.f;
-  bool clamps = false, none = true;
+  bool none = true;
 #pragma unroll
   for (int e = 0; e < 2; ++e) {
     if (!e || !wide) {
       // Without a value (dimensions past head_dim): zeros.  With one that is not finite: NaN.
       none = lo[e] > hi[e];
       const bool bad = !none && !(lo[e] > -INFINITY && hi[e] < INFINITY);
-      clamps = lo[e] < -kRecordMost || hi[e] > kRecordMost;
       const float l = fminf(fmaxf(lo[e], -kRecordMost), kRecordMost), h = fminf(fmaxf(hi[e], -kRecordMost), kRecordMost);
       __half s16, m16;
       if (!half_sure((h - l) * (1.f / 15.f), s16)) s16 = __double2half(((double)h - (double)l) / 15.0);
@@ -175,26 +189,26 @@ __global__ void __launch_bounds__(NT) kv_quantize_kernel(const __grid_constant__
       none = none || bad;
     }
     if (has[e] && !none) {
-      // The whole number next to q by adding 1.5 2^23, whose last bits it then is (with 8 more, the code).
+      // The whole number next to q by adding 1.5 2^23 (and 8): its last bits are the code then.
       constexpr float kAdd = 12582912.f + 8.f;
+      constexpr uint32_t kBits = 0x4b400000u;
       float q[8], r[8], edge = 0.f;
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
-        float v = x[e].at(k);
-        if (clamps) v = fminf(fmaxf(v, -kRecordMost), kRecordMost);
-        q[k] = fminf(fmaxf((v - mid) * inv, -8.f), 7.f);
+        q[k] = fminf(fmaxf((x[e].at(k) - mid) * inv, -8.f), 7.f);
         r[k] = q[k] + kAdd;
         edge = fmaxf(edge, fabsf(q[k] - (r[k] - kAdd)));
       }
       if (edge > 0.5f - 0x1p-16f) {
 #pragma unroll
         for (int k = 0; k < 8; ++k)
-          if (fabsf(q[k] - (r[k] - kAdd)) > 0.5f - 0x1p-16f)
-            r[k] = code_exactly(fminf(fmaxf(x[e].at(k), -kRecordMost), kRecordMost), mid, scale, q[k]) + kAdd;
+          if (fabsf(q[k] - (r[k] - kAdd)) > 0.5f - 0x1p-16f) r[k] = code_exactly(x[e].at(k), mid, scale, q[k]) + kAdd;
       }
+      // Dimension 4 t + 2 a + b, t = 2 y + (k >> 2); the numbers' other bits are taken off the sum.
 #pragma unroll
-      for (int k = 0; k < 8; ++k)  // dimension 4 t + 2 a + b, t = 2 y + (k >> 2)
-        word[k >> 2] += (__float_as_uint(r[k]) - __float_as_uint(12582912.f)) << 4 * (4 * (k & 1) + 2 * e + (k >> 1 & 1));
+      for (int k = 0; k < 8; ++k) word[k >> 2] += __float_as_uint(r[k]) << 4 * (4 * (k & 1) + 2 * e + (k >> 1 & 1));
+      word[0] -= kBits * (0x00110011u << 8 * e);
+      word[1] -= kBits * (0x00110011u << 8 * e);
     }
   }
   if (!in) return;
@@ -325,9 +339,9 @@ template <typename T> cudaError_t read_records(const ReadArgs& a, cudaStream_t s
   int u, s;
   const int64_t units = (int64_t)a.rows * a.kv_heads;
   auto go = [&](auto one, auto four, int lps_log2) {
-    // Four slots a thread where that still leaves several blocks per SM.
+    // Four slots a thread where that leaves two blocks per SM.
     dim3 grid = grid_of(lps_log2, units, a.tokens, a.out[1] != nullptr, u, s);
-    if ((int64_t)grid.x * grid.y * grid.z >= 8 * 4 * 148) {
+    if ((int64_t)grid.x * grid.y * grid.z >= 8 * 148) {
       grid.x = (grid.x + 3) / 4;
       four<<<grid, NT, 0, stream>>>(a, u, s);
     } else {
