@@ -233,7 +233,7 @@ RecordPlan record_plan(const AttnArgs& a) {
   p.score_bytes = a.weights ? up256(all * a.capacity * 4) : 0;
   // A unit's counter each, and chunks (of at least 128 slots) counted in 31 bits.
   p.direct = p.rows.groups <= kMostRecordGroups && units * p.rows.groups <= 65536 &&
-             units * p.rows.groups * (a.capacity / 128 + 3) < (int64_t)1 << 31 && p.score_bytes <= kMostScores;
+             units * p.rows.groups * (a.capacity / 128 + 8) < (int64_t)1 << 31 && p.score_bytes <= kMostScores;
   if (!p.direct) {
     p.halves = a.dtype != SV_F32 && !a.weights;  // (the accumulated weights' product takes keys of the queries' type)
     p.pairs = p.halves && a.dtype == SV_F16;

@@ -44,7 +44,6 @@
 namespace sv {
 namespace {
 
-constexpr int TK = 16;         // slots per tile
 constexpr int kJoin = 16;      // parts per first-level group
 constexpr int kMaxFlat = 32;   // parts joined in one level
 constexpr float kSlack = 8.f;  // log2 by which a score may exceed its reference
@@ -155,7 +154,8 @@ __device__ __forceinline__ int slot_at(int k) {
 }
 
 // Numbers of a record's layout for NI blocks of 32 dimensions.
-template <int NI> struct Form {
+template <int NI, int SUB> struct Form {
+  static constexpr int TK = 16 * SUB;                         // slots of a tile
   static constexpr int REC = 16 * NI + 16;                    // bytes
   static constexpr int NG = NI > 2 ? NI : 2 * NI;             // groups
   static constexpr int NB = NI > 2 ? 2 : 1;                   // words of a value that one thread turns into operands
@@ -168,7 +168,7 @@ struct RowTiles {
   int start, end, a0, a1, b0, b1, ta, tiles;
 };
 
-__device__ __noinline__ RowTiles row_tiles(const AttnArgs& a, int r) {
+template <int TK> __device__ __noinline__ RowTiles row_tiles(const AttnArgs& a, int r) {
   RowTiles t;
   const RowSpan sp = row_span(a, r);
   t.start = sp.start;
@@ -182,24 +182,30 @@ __device__ __noinline__ RowTiles row_tiles(const AttnArgs& a, int r) {
   return t;
 }
 
+// Empty places of the list behind every unit's chunks, where blocks take eight and more: what beginning and ending a
+// unit costs, so that blocks of many units get fewer chunks (64 rows over 4096 slots 64 us, 66 without: some blocks
+// worked 8 us longer).
+constexpr int kBetween = 2;
+
 // A place in the list of chunks: chunk k of unit (r, h), h counting the heads' groups of rows.
-template <int NW> struct Place {
+template <int NW, int TK> struct Place {
   int r, h, k, chunks;
   RowTiles rt;
   __device__ __forceinline__ void row(const AttnArgs& a, int r_) {
     r = r_;
-    rt = row_tiles(a, r_);
+    rt = row_tiles<TK>(a, r_);
     chunks = (rt.tiles + NW - 1) / NW;
   }
 };
 
 // NI blocks of 32 dimensions, NT column tiles of eight query rows, NW warps, rings of RING tiles.
 // MULTI: more than one query per row.
-template <typename T, int NI, int NT, int NW, int RING, bool MULTI>
+// A tile is SUB times 16 slots, whose steps have nothing to wait for from one another.
+template <typename T, int NI, int NT, int SUB, int NW, int RING, bool MULTI>
 __global__ void __launch_bounds__(NW * 32, 1)
     attn_record_kernel(const __grid_constant__ AttnArgs a, const int blocks_max, const int row_groups) {
-  using F = Form<NI>;
-  constexpr int REC = F::REC, NG = F::NG, NB = F::NB, MT = 4 * NB, ROWS = 8 * NT, THREADS = NW * 32;
+  using F = Form<NI, SUB>;
+  constexpr int TK = F::TK, REC = F::REC, NG = F::NG, NB = F::NB, MT = 4 * NB, ROWS = 8 * NT, THREADS = NW * 32;
   constexpr int OS = 32 * NI;  // dimensions of the warps' outputs
   constexpr bool HALVES = std::is_same<T, __half>::value, FULL = std::is_same<T, float>::value;
   constexpr int QP = FULL ? 2 : 1, WP = FULL ? 3 : HALVES ? 2 : 1;  // pieces of a query, of a weight
@@ -228,7 +234,7 @@ __global__ void __launch_bounds__(NW * 32, 1)
   // Chunks of all rows, every head of a row having as many: see sv_attention_token.cu.
   const int per = (a.rows + THREADS - 1) / THREADS, row0 = tid * per;
   int mine = 0;
-  for (int x = row0; x < min(row0 + per, a.rows); ++x) mine += (row_tiles(a, x).tiles + NW - 1) / NW;
+  for (int x = row0; x < min(row0 + per, a.rows); ++x) mine += (row_tiles<TK>(a, x).tiles + NW - 1) / NW;
   int upto = mine;
 #pragma unroll
   for (int k = 1; k < 32; k <<= 1) {
@@ -243,6 +249,10 @@ __global__ void __launch_bounds__(NW * 32, 1)
     if (k == warp) upto += total;
     total += scan[k];
   }
+  const int between = total * K >= 8 * blocks_max ? kBetween : 0;
+  mine += between * max(min(per, a.rows - row0), 0);
+  upto += between * min(row0 + per, a.rows);
+  total += between * a.rows;
   const int W = total * K;  // fits 31 bits (checked by the host)
   const int N = min(blocks_max, W), share = W / N, extra = W - share * N;
   const int c = blockIdx.x;
@@ -256,7 +266,7 @@ __global__ void __launch_bounds__(NW * 32, 1)
   if ((upto - mine) * K <= c0 && c0 < upto * K) {
     int x = row0, at = upto - mine;
     for (;; ++x) {
-      const int chunks = (row_tiles(a, x).tiles + NW - 1) / NW;
+      const int chunks = (row_tiles<TK>(a, x).tiles + NW - 1) / NW + between;
       if (c0 < (at + chunks) * K) break;
       at += chunks;
     }
@@ -264,26 +274,37 @@ __global__ void __launch_bounds__(NW * 32, 1)
     sh_before = at;
   }
   __syncthreads();
-  Place<NW> p;
+  Place<NW, TK> p;
   p.row(a, sh_row);
   {
     const int off = c0 - sh_before * K;
-    p.h = off / p.chunks;
-    p.k = off - p.h * p.chunks;
+    p.h = off / (p.chunks + between);
+    p.k = off - p.h * (p.chunks + between);
   }
-  int before = sh_before;  // chunks (of one head) before row p.r
+  int before = sh_before;  // places (of one head) before row p.r
+  int f_place = c0;        // the next chunk to fetch
+  if (p.k >= p.chunks) {   // behind a unit's chunks: on to the next one, if it begins here
+    f_place += p.chunks + between - p.k;
+    if (f_place >= c1) return;
+    p.k = 0;
+    if (++p.h == K) {
+      p.h = 0;
+      before += p.chunks + between;
+      p.row(a, p.r + 1);
+    }
+  }
 
   // ---- copies: this warp's tile of chunk f, the f-th place ahead.  The next `runs` of them are whole
   // tiles of one unit, each a run of bytes f_step behind the one before.
-  Place<NW> f = p;
-  int f_left = c1 - c0, runs = 0;
+  Place<NW, TK> f = p;
+  int runs = 0;
   const unsigned char *f_k, *f_v;
   const int64_t f_step = (int64_t)NW * TK * a.kv_slot;
   const uint32_t ring = (uint32_t)__cvta_generic_to_shared(ring_bytes) + warp * RING * 2 * F::TILE;
   uint32_t put = ring + lane * 16;
   // The place f by slots (the end of a unit, sinks, other strides), or none; then what comes after it.
   auto fetch_slots = [&]() {
-    if (f_left <= 0) return;
+    if (f_place >= c1) return;
     const int tile = f.k * NW + warp, f_hi = f.rt.ta + (f.rt.b1 - f.rt.b0) / TK;
     const int64_t base = f.r * a.kv_row + (f.h / row_groups) * a.kv_head;
     if (tile < f.rt.tiles) {
@@ -298,9 +319,10 @@ __global__ void __launch_bounds__(NW * 32, 1)
                         slot < count);
       }
     }
-    --f_left;
+    ++f_place;
     if (++f.k == f.chunks) {
       f.k = 0;
+      f_place += between;
       if (++f.h == K) {
         f.h = 0;
         if (f.r + 1 < a.rows) f.row(a, f.r + 1);  // (past the last chunk of all nothing is looked at)
@@ -310,14 +332,14 @@ __global__ void __launch_bounds__(NW * 32, 1)
   auto find_runs = [&]() {
     runs = 0;
     const int tile = f.k * NW + warp, f_hi = f.rt.ta + (f.rt.b1 - f.rt.b0) / TK;
-    if (f_left <= 0 || a.kv_slot != REC || tile < f.rt.ta || tile >= f_hi) return;
+    if (f_place >= c1 || a.kv_slot != REC || tile < f.rt.ta || tile >= f_hi) return;
     // Not a unit's last chunk, after which the place moves on.
-    runs = min(min((f_hi - tile + NW - 1) / NW, f.chunks - 1 - f.k), f_left);
+    runs = min(min((f_hi - tile + NW - 1) / NW, f.chunks - 1 - f.k), c1 - f_place);
     const int64_t at = f.r * a.kv_row + (f.h / row_groups) * a.kv_head + (f.rt.b0 + (tile - f.rt.ta) * TK) * a.kv_slot;
     f_k = static_cast<const unsigned char*>(a.k) + at + lane * 16;
     f_v = static_cast<const unsigned char*>(a.v) + at + lane * 16 - F::TILE;
     f.k += runs;
-    f_left -= runs;
+    f_place += runs;
   };
   find_runs();
   auto fetch = [&]() {
@@ -448,18 +470,19 @@ __global__ void __launch_bounds__(NW * 32, 1)
     return parts > kMaxFlat ? arrives_last(a.counters + (int64_t)a.rows * K + 2 * b0 + (b0 == c_first), min(kJoin, c_first + parts - b0))
                             : arrives_last(a.counters + q.r * K + q.h, parts);
   };
+  load_q(p.r, p.h);  // (behind the tiles' loads they would wait for them)
 #pragma unroll 1
   for (int k = 0; k < RING - 1; ++k) fetch();
   uint32_t get = ring;
   const uint32_t k_even = hidden(0x000f000fu), k_odd = hidden(0x00f000f0u), k_1024 = hidden(0x64006400u), k_64 = hidden(0x54005400u);
-  int at = c0;
   bool last_shared = false;  // whether the part before was
-  load_q(p.r, p.h);
   make_q();
   __syncthreads();
   for (;;) {  // units
     const int head = p.h / row_groups, m0 = (p.h - head * row_groups) * ROWS, rows_here = min(ROWS, nG - m0);
-    const int first = before * K + p.h * p.chunks, end = first + p.chunks, stop = min(end, c1);
+    const int first = before * K + p.h * (p.chunks + between), end = first + p.chunks, stop = min(end, c1);
+    const bool more = end + between < c1;  // the next unit begins here, too
+    const int at = max(c0, first);
     const RowTiles rt = p.rt;
     const int pos_first = rt.end - a.n, low_last = window_low(a, rt.start, rt.end - 1);
     // This warp's tiles of the part; in [w_lo, w_hi) every row sees the whole tile.
@@ -469,7 +492,6 @@ __global__ void __launch_bounds__(NW * 32, 1)
     const int w_hi = rt.ta + ((MULTI ? min(rt.b1, pos_first + 1) : rt.b1) - rt.b0) / TK;
     // As numbers of the loop's rounds.
     const int k_lo = (w_lo - tile0 + NW - 1) / NW, k_hi = w_hi > tile0 ? (w_hi - tile0 + NW - 1) / NW : 0;
-    at = stop;
     const int s0 = slot_at(g), s1 = slot_at(g + 8);
     const uint32_t va = slot_at(2 * t) * REC, vb = slot_at(2 * t + 1) * REC;  // rows 8..15: the slots behind them
     float fr[NT][2], from[NT][2];  // from: a row's reference, negative (far below any score before the first)
@@ -502,12 +524,13 @@ __global__ void __launch_bounds__(NW * 32, 1)
       get = get + 2 * F::TILE == ring + RING * 2 * F::TILE ? ring : get + 2 * F::TILE;
       if (k >= valid) break;  // (the last one at most)
       // ---- scores
-      float s[NT][4];  // slots s0 and s1 of rows 2 t and 2 t + 1, in units of 1 / fr
-      {
+      float s[SUB][NT][4];  // slots 16 h + s0, 16 h + s1 of rows 2 t and 2 t + 1, in units of 1 / fr
+#pragma unroll
+      for (int h = 0; h < SUB; ++h) {
         uint32_t kw[2][NI], pr[2][4], own[2];
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
-          const uint32_t rec = kt + (x ? s1 : s0) * REC;
+          const uint32_t rec = kt + (16 * h + (x ? s1 : s0)) * REC;
           if constexpr (NI == 4) {
             load4(kw[x], rec + t * 16);
           } else if constexpr (NI == 2) {
@@ -522,10 +545,10 @@ __global__ void __launch_bounds__(NW * 32, 1)
 #pragma unroll
         for (int u = 0; u < NT; ++u) {
           const uint2 q = KEEP_Q ? qm[u] : sh_qm[u][lane];
-          mma_new(s[u], own[0], own[1], own[0], own[1], q.x, q.y);
+          mma_new(s[h][u], own[0], own[1], own[0], own[1], q.x, q.y);
           if constexpr (FULL) {
 #pragma unroll
-            for (int y = 0; y < 4; ++y) s[u][y] *= 0x1p-10f;
+            for (int y = 0; y < 4; ++y) s[h][u][y] *= 0x1p-10f;
           }
         }
 #pragma unroll
@@ -553,7 +576,7 @@ __global__ void __launch_bounds__(NW * 32, 1)
 #pragma unroll
             for (int u = 0; u < NT; ++u)
 #pragma unroll
-              for (int y = 0; y < 2; ++y) s[u][2 * x + y] = fmaf(sc, acc[u][2 * x + y], s[u][2 * x + y]);
+              for (int y = 0; y < 2; ++y) s[h][u][2 * x + y] = fmaf(sc, acc[u][2 * x + y], s[h][u][2 * x + y]);
           }
         }
       }
@@ -570,33 +593,39 @@ __global__ void __launch_bounds__(NW * 32, 1)
             const int pos = MULTI ? pos_first + (m0 + m) / group : pos_first;
             const int low = window_low(a, rt.start, pos);
 #pragma unroll
-            for (int x = 0; x < 2; ++x) {
-              const int j = j0 + (x ? s1 : s0);
-              if (j >= jend || !slot_seen(a, rt.start, pos, low, j)) s[u][2 * x + y] = -INFINITY;
+            for (int x = 0; x < 2 * SUB; ++x) {
+              const int h = x >> 1, j = j0 + 16 * h + (x & 1 ? s1 : s0);
+              if (j >= jend || !slot_seen(a, rt.start, pos, low, j)) s[h][u][2 * (x & 1) + y] = -INFINITY;
               if (a.scores && j < jend && m < rows_here)
-                a.scores[((int64_t)(p.r * a.kv_heads + head) * nG + m0 + m) * a.capacity + j] = s[u][2 * x + y] * fr[u][y];
+                a.scores[((int64_t)(p.r * a.kv_heads + head) * nG + m0 + m) * a.capacity + j] = s[h][u][2 * (x & 1) + y] * fr[u][y];
             }
           }
       }
       // ---- weights, by what exceeds the reference; past the slack it moves
-      float z[NT][2][2], most = -INFINITY;
+      float z[SUB][NT][2][2], most = -INFINITY;
       auto shift = [&]() {
 #pragma unroll
-        for (int u = 0; u < NT; ++u)
+        for (int h = 0; h < SUB; ++h)
 #pragma unroll
-          for (int x = 0; x < 2; ++x)
+          for (int u = 0; u < NT; ++u)
 #pragma unroll
-            for (int y = 0; y < 2; ++y) z[u][x][y] = fmaf(s[u][2 * x + y], fr[u][y], from[u][y]);
+            for (int x = 0; x < 2; ++x)
+#pragma unroll
+              for (int y = 0; y < 2; ++y) z[h][u][x][y] = fmaf(s[h][u][2 * x + y], fr[u][y], from[u][y]);
       };
       shift();
 #pragma unroll
-      for (int u = 0; u < NT; ++u) most = fmaxf(most, fmaxf(fmaxf(z[u][0][0], z[u][0][1]), fmaxf(z[u][1][0], z[u][1][1])));
+      for (int h = 0; h < SUB; ++h)
+#pragma unroll
+        for (int u = 0; u < NT; ++u) most = fmaxf(most, fmaxf(fmaxf(z[h][u][0][0], z[h][u][0][1]), fmaxf(z[h][u][1][0], z[h][u][1][1])));
       if (__any_sync(0xffffffffu, most > kSlack)) {
 #pragma unroll
         for (int u = 0; u < NT; ++u)
 #pragma unroll
           for (int y = 0; y < 2; ++y) {
-            float mx = fmaxf(s[u][y], s[u][2 + y]);
+            float mx = -INFINITY;
+#pragma unroll
+            for (int h = 0; h < SUB; ++h) mx = fmaxf(mx, fmaxf(s[h][u][y], s[h][u][2 + y]));
 #pragma unroll
             for (int x = 4; x < 32; x <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
             const float now = fminf(-mx * fr[u][y], from[u][y]);
@@ -611,134 +640,138 @@ __global__ void __launch_bounds__(NW * 32, 1)
           }
         shift();
       }
-      // As B operand of the values' product: slots of rows 0..7 and 8..15 of the tile's order (float16 outputs: and
-      // what their rounding left).
-      uint32_t pw[WP][NT][2];
 #pragma unroll
-      for (int u = 0; u < NT; ++u)
+      for (int h = 0; h < SUB; ++h) {
+        const uint32_t at_h = vt + 16 * h * REC;
+        // As B operand of the values' product: slots of rows 0..7 and 8..15 of the tile's order (float16 outputs: and
+        // what their rounding left).
+        uint32_t pw[WP][NT][2];
 #pragma unroll
-        for (int x = 0; x < 2; ++x) {
-          const float w0 = ex2(z[u][x][0]), w1 = ex2(z[u][x][1]);
-          l[u][0] += w0;
-          l[u][1] += w1;
-          if constexpr (FULL) {
-            float2 rest = make_float2(w0, w1);
+        for (int u = 0; u < NT; ++u)
 #pragma unroll
-            for (int y = 0; y < 3; ++y) pw[y][u][x] = transposed(next_piece(rest));
-            continue;
+          for (int x = 0; x < 2; ++x) {
+            const float w0 = ex2(z[h][u][x][0]), w1 = ex2(z[h][u][x][1]);
+            l[u][0] += w0;
+            l[u][1] += w1;
+            if constexpr (FULL) {
+              float2 rest = make_float2(w0, w1);
+#pragma unroll
+              for (int y = 0; y < 3; ++y) pw[y][u][x] = transposed(next_piece(rest));
+              continue;
+            }
+            const uint32_t both = pack16(w0, w1);
+            pw[0][u][x] = transposed(both);
+            if constexpr (HALVES) {
+              const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&both));
+              pw[1][u][x] = transposed(pack16(w0 - h.x, w1 - h.y));
+            }
           }
-          const uint32_t both = pack16(w0, w1);
-          pw[0][u][x] = transposed(both);
-          if constexpr (HALVES) {
-            const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&both));
-            pw[1][u][x] = transposed(pack16(w0 - h.x, w1 - h.y));
+        // ---- values
+        const uint32_t ra[4] = {at_h + va, at_h + vb, at_h + va + REC, at_h + vb + REC};
+        uint32_t vw[4][NB], pr[4][2];
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          if constexpr (NI == 4) {
+            load2(vw[x], ra[x] + g * 8);
+            load2(pr[x], ra[x] + 16 * NI + (g & 1) * 8);
+          } else if constexpr (NI == 3) {  // words 2 g, 2 g + 1 of twelve
+            const int w = min(2 * g, 10);
+            load2(vw[x], ra[x] + w * 4);
+            pr[x][0] = load1(ra[x] + 16 * NI + w % 3 * 4);
+            pr[x][1] = load1(ra[x] + 16 * NI + (w + 1) % 3 * 4);
+          } else {
+            const int w = NI == 2 ? g : g & 3;
+            vw[x][0] = load1(ra[x] + w * 4);
+            load2(pr[x], ra[x] + 16 * NI + w % NI * 8);
           }
         }
-      // ---- values
-      const uint32_t ra[4] = {vt + va, vt + vb, vt + va + REC, vt + vb + REC};
-      uint32_t vw[4][NB], pr[4][2];
-#pragma unroll
-      for (int x = 0; x < 4; ++x) {
-        if constexpr (NI == 4) {
-          load2(vw[x], ra[x] + g * 8);
-          load2(pr[x], ra[x] + 16 * NI + (g & 1) * 8);
-        } else if constexpr (NI == 3) {  // words 2 g, 2 g + 1 of twelve
-          const int w = min(2 * g, 10);
-          load2(vw[x], ra[x] + w * 4);
-          pr[x][0] = load1(ra[x] + 16 * NI + w % 3 * 4);
-          pr[x][1] = load1(ra[x] + 16 * NI + (w + 1) % 3 * 4);
-        } else {
-          const int w = NI == 2 ? g : g & 3;
-          vw[x][0] = load1(ra[x] + w * 4);
-          load2(pr[x], ra[x] + 16 * NI + w % NI * 8);
-        }
-      }
-      uint32_t sc[2][2], mi[2][2];  // [rows 0..7, 8..15][group]
-#pragma unroll
-      for (int x = 0; x < 2; ++x)
-#pragma unroll
-        for (int y = 0; y < 2; ++y) {
-          sc[x][y] = __byte_perm(pr[2 * x][y], pr[2 * x + 1][y], 0x5410);
-          mi[x][y] = __byte_perm(pr[2 * x][y], pr[2 * x + 1][y], 0x7632);
-        }
-      // A group that stands for NaN must not reach the rows that do not see its slot (0 * NaN): the
-      // product takes zeros in its place, and the rows that see it become NaN below.
-      bool hide = false;
-      uint32_t bad[2][2] = {{0u, 0u}, {0u, 0u}};
-      if (MULTI && !whole) {
-        uint32_t any = 0u;
+        uint32_t sc[2][2], mi[2][2];  // [rows 0..7, 8..15][group]
 #pragma unroll
         for (int x = 0; x < 2; ++x)
 #pragma unroll
           for (int y = 0; y < 2; ++y) {
-            const uint32_t lo = (sc[x][y] & 0x7c00u) == 0x7c00u || (mi[x][y] & 0x7c00u) == 0x7c00u ? 0xffffu : 0u;
-            const uint32_t hi = (sc[x][y] & 0x7c000000u) == 0x7c000000u || (mi[x][y] & 0x7c000000u) == 0x7c000000u ? 0xffff0000u : 0u;
-            bad[x][y] = lo | hi;
-            any |= bad[x][y];
-            sc[x][y] &= ~bad[x][y];
-            mi[x][y] &= ~bad[x][y];
+            sc[x][y] = __byte_perm(pr[2 * x][y], pr[2 * x + 1][y], 0x5410);
+            mi[x][y] = __byte_perm(pr[2 * x][y], pr[2 * x + 1][y], 0x7632);
           }
-        hide = __any_sync(0xffffffffu, any != 0u);
-      }
-      // The value of nibble j (0..3) of a 16-bit half, of two slots side by side.
-      auto value = [&](uint32_t w, int j, uint32_t scale, uint32_t mid) {
-        const uint32_t x = j & 2 ? w >> 8 : w;
-        const uint32_t c8 = j & 1 ? add16(and_or(x, k_odd, k_64), 0xd480d480u)      // 64 + c - 72
-                                  : add16(and_or(x, k_even, k_1024), 0xe408e408u);  // 1024 + c - 1032
-        return fma16(c8, scale, mid);
-      };
+        // A group that stands for NaN must not reach the rows that do not see its slot (0 * NaN): the
+        // product takes zeros in its place, and the rows that see it become NaN below.
+        bool hide = false;
+        uint32_t bad[2][2] = {{0u, 0u}, {0u, 0u}};
+        if (MULTI && !whole) {
+          uint32_t any = 0u;
 #pragma unroll
-      for (int b = 0; b < NB; ++b) {
-        const uint32_t l0 = __byte_perm(vw[0][b], vw[1][b], 0x5410), h0 = __byte_perm(vw[0][b], vw[1][b], 0x7632);
-        const uint32_t l1 = __byte_perm(vw[2][b], vw[3][b], 0x5410), h1 = __byte_perm(vw[2][b], vw[3][b], 0x7632);
+          for (int x = 0; x < 2; ++x)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int y = NI > 2 ? b : j >> 1;
-          if constexpr (FULL) {
-            uint32_t v[3][4];
-            pieces(l0, j, sc[0][y], mi[0][y], v[0][0], v[1][0], v[2][0]);
-            pieces(h0, j, sc[0][y], mi[0][y], v[0][1], v[1][1], v[2][1]);
-            pieces(l1, j, sc[1][y], mi[1][y], v[0][2], v[1][2], v[2][2]);
-            pieces(h1, j, sc[1][y], mi[1][y], v[0][3], v[1][3], v[2][3]);
-            // The smallest products first; those below 2^-24 of the whole are left out.
-#pragma unroll
-            for (int z = 2; z >= 0; --z)
-#pragma unroll
-              for (int x = z; x >= 0; --x)
-#pragma unroll
-                for (int u = 0; u < NT; ++u)
-                  mma_bf16(o[u][4 * b + j], v[x][0], v[x][1], v[x][2], v[x][3], pw[z - x][u][0], pw[z - x][u][1]);
-          } else {
-            const uint32_t a0 = value(l0, j, sc[0][y], mi[0][y]), a1 = value(h0, j, sc[0][y], mi[0][y]);
-            const uint32_t a2 = value(l1, j, sc[1][y], mi[1][y]), a3 = value(h1, j, sc[1][y], mi[1][y]);
-#pragma unroll
-            for (int z = 0; z < WP; ++z)
-#pragma unroll
-              for (int u = 0; u < NT; ++u) mma_add(o[u][4 * b + j], a0, a1, a2, a3, pw[z][u][0], pw[z][u][1]);
-          }
+            for (int y = 0; y < 2; ++y) {
+              const uint32_t lo = (sc[x][y] & 0x7c00u) == 0x7c00u || (mi[x][y] & 0x7c00u) == 0x7c00u ? 0xffffu : 0u;
+              const uint32_t hi = (sc[x][y] & 0x7c000000u) == 0x7c000000u || (mi[x][y] & 0x7c000000u) == 0x7c000000u ? 0xffff0000u : 0u;
+              bad[x][y] = lo | hi;
+              any |= bad[x][y];
+              sc[x][y] &= ~bad[x][y];
+              mi[x][y] &= ~bad[x][y];
+            }
+          hide = __any_sync(0xffffffffu, any != 0u);
         }
-      }
-      if (MULTI && hide) {
+        // The value of nibble j (0..3) of a 16-bit half, of two slots side by side.
+        auto value = [&](uint32_t w, int j, uint32_t scale, uint32_t mid) {
+          const uint32_t x = j & 2 ? w >> 8 : w;
+          const uint32_t c8 = j & 1 ? add16(and_or(x, k_odd, k_64), 0xd480d480u)      // 64 + c - 72
+                                    : add16(and_or(x, k_even, k_1024), 0xe408e408u);  // 1024 + c - 1032
+          return fma16(c8, scale, mid);
+        };
 #pragma unroll
-        for (int b = 0; b < NB; ++b)
+        for (int b = 0; b < NB; ++b) {
+          const uint32_t l0 = __byte_perm(vw[0][b], vw[1][b], 0x5410), h0 = __byte_perm(vw[0][b], vw[1][b], 0x7632);
+          const uint32_t l1 = __byte_perm(vw[2][b], vw[3][b], 0x5410), h1 = __byte_perm(vw[2][b], vw[3][b], 0x7632);
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             const int y = NI > 2 ? b : j >> 1;
-            const uint32_t one = FULL ? 0x3f803f80u : kOnes, x0 = bad[0][y] & one, x1 = bad[1][y] & one;
+            if constexpr (FULL) {
+              uint32_t v[3][4];
+              pieces(l0, j, sc[0][y], mi[0][y], v[0][0], v[1][0], v[2][0]);
+              pieces(h0, j, sc[0][y], mi[0][y], v[0][1], v[1][1], v[2][1]);
+              pieces(l1, j, sc[1][y], mi[1][y], v[0][2], v[1][2], v[2][2]);
+              pieces(h1, j, sc[1][y], mi[1][y], v[0][3], v[1][3], v[2][3]);
+              // The smallest products first; those below 2^-24 of the whole are left out.
 #pragma unroll
-            for (int u = 0; u < NT; ++u) {
-              float seen[4];
-              if constexpr (FULL) {
-                seen[0] = seen[1] = seen[2] = seen[3] = 0.f;
-                mma_bf16(seen, x0, x0, x1, x1, pw[0][u][0], pw[0][u][1]);
-              } else {
-                mma_new(seen, x0, x0, x1, x1, pw[0][u][0], pw[0][u][1]);
-              }
+              for (int z = 2; z >= 0; --z)
 #pragma unroll
-              for (int q = 0; q < 4; ++q)
-                if (seen[q] != 0.f) o[u][4 * b + j][q] = __int_as_float(0x7fc00000);
+                for (int x = z; x >= 0; --x)
+#pragma unroll
+                  for (int u = 0; u < NT; ++u)
+                    mma_bf16(o[u][4 * b + j], v[x][0], v[x][1], v[x][2], v[x][3], pw[z - x][u][0], pw[z - x][u][1]);
+            } else {
+              const uint32_t a0 = value(l0, j, sc[0][y], mi[0][y]), a1 = value(h0, j, sc[0][y], mi[0][y]);
+              const uint32_t a2 = value(l1, j, sc[1][y], mi[1][y]), a3 = value(h1, j, sc[1][y], mi[1][y]);
+#pragma unroll
+              for (int z = 0; z < WP; ++z)
+#pragma unroll
+                for (int u = 0; u < NT; ++u) mma_add(o[u][4 * b + j], a0, a1, a2, a3, pw[z][u][0], pw[z][u][1]);
             }
           }
+        }
+        if (MULTI && hide) {
+#pragma unroll
+          for (int b = 0; b < NB; ++b)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const int y = NI > 2 ? b : j >> 1;
+              const uint32_t one = FULL ? 0x3f803f80u : kOnes, x0 = bad[0][y] & one, x1 = bad[1][y] & one;
+#pragma unroll
+              for (int u = 0; u < NT; ++u) {
+                float seen[4];
+                if constexpr (FULL) {
+                  seen[0] = seen[1] = seen[2] = seen[3] = 0.f;
+                  mma_bf16(seen, x0, x0, x1, x1, pw[0][u][0], pw[0][u][1]);
+                } else {
+                  mma_new(seen, x0, x0, x1, x1, pw[0][u][0], pw[0][u][1]);
+                }
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+                  if (seen[q] != 0.f) o[u][4 * b + j][q] = __int_as_float(0x7fc00000);
+              }
+            }
+        }
       }
     }
     // The warp's results into shared memory.
@@ -766,7 +799,7 @@ __global__ void __launch_bounds__(NW * 32, 1)
         }
       }
     }
-    if (end < c1) {
+    if (more) {
       const bool row_ends = p.h + 1 == K;
       load_q(row_ends ? p.r + 1 : p.r, row_ends ? 0 : p.h + 1);
     }
@@ -816,16 +849,16 @@ __global__ void __launch_bounds__(NW * 32, 1)
       const int e = a.lengths ? a.lengths[p.r] : a.capacity, s = a.starts ? a.starts[p.r] : 0;
       a.status[p.r] = (e < 0 || e > a.capacity || s < 0 || s > max(e, 0)) ? 8 : 0;
     }
-    if (end < c1) make_q();  // (nobody reads the queries past the barriers above)
+    if (more) make_q();  // (nobody reads the queries past the barriers above)
     __syncthreads();
     last_shared = !alone;
-    if (end >= c1) break;
+    if (!more) break;
     // A unit that an earlier block began arrives at once: that block, which ends with it, mostly finds all there.
     if (!alone && tid == 0) sh_last[shared_parts - 1] = arrive_at(shared_part[shared_parts - 1]);
     p.k = 0;
     if (++p.h == K) {
       p.h = 0;
-      before += p.chunks;
+      before += p.chunks + between;
       p.row(a, p.r + 1);
     }
   }
@@ -913,20 +946,20 @@ __global__ void __launch_bounds__(NW * 32, 1)
   }
 }
 
-template <typename T, int NI, int NT, int NW, int RING, bool MULTI>
+template <typename T, int NI, int NT, int SUB, int NW, int RING, bool MULTI>
 cudaError_t record(const AttnArgs& a, int row_groups, cudaStream_t stream) {
-  constexpr size_t smem = (size_t)NW * RING * 2 * Form<NI>::TILE + sizeof(float) * NW * 8 * NT * 32 * NI;
-  const cudaError_t e = allow_smem<attn_record_kernel<T, NI, NT, NW, RING, MULTI>>(smem);
+  constexpr size_t smem = (size_t)NW * RING * 2 * Form<NI, SUB>::TILE + sizeof(float) * NW * 8 * NT * 32 * NI;
+  const cudaError_t e = allow_smem<attn_record_kernel<T, NI, NT, SUB, NW, RING, MULTI>>(smem);
   if (e != cudaSuccess) return e;
-  attn_record_kernel<T, NI, NT, NW, RING, MULTI><<<kTokenBlocks, NW * 32, smem, stream>>>(a, kTokenBlocks, row_groups);
+  attn_record_kernel<T, NI, NT, SUB, NW, RING, MULTI><<<kTokenBlocks, NW * 32, smem, stream>>>(a, kTokenBlocks, row_groups);
   return cudaGetLastError();
 }
 
 template <typename T, int NI, bool MULTI> cudaError_t record_rows(const AttnArgs& a, const RecordRows& x, cudaStream_t stream) {
   if constexpr (!std::is_same<T, float>::value) {
-    if (x.tiles == 2) return record<T, NI, 2, 8, 5, MULTI>(a, x.groups, stream);
+    if (x.tiles == 2) return record<T, NI, 2, 2, 8, 3, MULTI>(a, x.groups, stream);
   }
-  return record<T, NI, 1, 12, 4, MULTI>(a, x.groups, stream);
+  return record<T, NI, 1, 1, 12, 4, MULTI>(a, x.groups, stream);
 }
 
 template <typename T> cudaError_t record_any(const AttnArgs& a, const RecordRows& x, cudaStream_t stream) {
