@@ -231,6 +231,10 @@ __global__ void __launch_bounds__(NW * 32, 1)
     return reinterpret_cast<float4*>(outs) + (w * ROWS + m) * (OS / 4) + (c ^ (m >> 1 & 3) ^ (OS >= 128 ? c >> 2 & 4 : 0));
   };
 
+  // (Launched while the kernel before it ends; the next one may be, too.)
+  wait_before();
+  launch_dependents();
+
   // Chunks of all rows, every head of a row having as many: see sv_attention_token.cu.
   const int per = (a.rows + THREADS - 1) / THREADS, row0 = tid * per;
   int mine = 0;
@@ -951,8 +955,8 @@ cudaError_t record(const AttnArgs& a, int row_groups, cudaStream_t stream) {
   constexpr size_t smem = (size_t)NW * RING * 2 * Form<NI, SUB>::TILE + sizeof(float) * NW * 8 * NT * 32 * NI;
   const cudaError_t e = allow_smem<attn_record_kernel<T, NI, NT, SUB, NW, RING, MULTI>>(smem);
   if (e != cudaSuccess) return e;
-  attn_record_kernel<T, NI, NT, SUB, NW, RING, MULTI><<<kTokenBlocks, NW * 32, smem, stream>>>(a, kTokenBlocks, row_groups);
-  return cudaGetLastError();
+  return launch_after(true, attn_record_kernel<T, NI, NT, SUB, NW, RING, MULTI>, dim3(kTokenBlocks), NW * 32, smem, stream, a,
+                      kTokenBlocks, row_groups);
 }
 
 template <typename T, int NI, bool MULTI> cudaError_t record_rows(const AttnArgs& a, const RecordRows& x, cudaStream_t stream) {

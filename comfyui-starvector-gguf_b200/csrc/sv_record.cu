@@ -124,6 +124,8 @@ __device__ __forceinline__ Item item_at(int item, int units_log2, int slots_log2
 template <typename T, int LPS_LOG2>  // 2^LPS_LOG2 threads per slot
 __global__ void __launch_bounds__(NT) kv_quantize_kernel(const __grid_constant__ WriteArgs a, const int units_log2,
                                                          const int slots_log2) {
+  wait_before();  // (launched while the kernel before it ends; the next one may be, too)
+  launch_dependents();
   const int lane = threadIdx.x & ((1 << LPS_LOG2) - 1), y = lane & 1, i = lane >> 1;
   const Item it = item_at(threadIdx.x >> LPS_LOG2, units_log2, slots_log2, a.kv_heads, a.rows, a.tokens);
   int end = a.capacity, given = 0;
@@ -248,6 +250,8 @@ template <> __device__ __forceinline__ void store8<__nv_bfloat16>(__nv_bfloat16*
 template <typename T, int LPS_LOG2, int PER>
 __global__ void __launch_bounds__(NT) kv_dequantize_kernel(const __grid_constant__ ReadArgs a, const int units_log2,
                                                            const int slots_log2) {
+  wait_before();  // (launched while the kernel before it ends; the next one may be, too)
+  launch_dependents();
   const int lane = threadIdx.x & ((1 << LPS_LOG2) - 1), y = lane & 1, i = lane >> 1;
   Item it = item_at(threadIdx.x >> LPS_LOG2, units_log2, slots_log2, a.kv_heads, a.rows, a.tokens);
   if (PER > 1) it.i += (int)blockIdx.x * (PER - 1) << slots_log2;
@@ -328,8 +332,7 @@ template <typename T> cudaError_t write_records(const WriteArgs& a, cudaStream_t
   const int64_t units = (int64_t)a.rows * a.kv_heads;
   auto go = [&](auto kernel, int lps_log2) {
     const dim3 grid = grid_of(lps_log2, units, a.tokens, a.in[1] != nullptr, u, s);
-    kernel<<<grid, NT, 0, stream>>>(a, u, s);
-    return cudaGetLastError();
+    return launch_after(true, kernel, grid, NT, 0, stream, a, u, s);
   };
   if (a.dim > 64) return go(kv_quantize_kernel<T, 3>, 3);
   return a.dim > 32 ? go(kv_quantize_kernel<T, 2>, 2) : go(kv_quantize_kernel<T, 1>, 1);
@@ -343,11 +346,9 @@ template <typename T> cudaError_t read_records(const ReadArgs& a, cudaStream_t s
     dim3 grid = grid_of(lps_log2, units, a.tokens, a.out[1] != nullptr, u, s);
     if ((int64_t)grid.x * grid.y * grid.z >= 8 * 148) {
       grid.x = (grid.x + 3) / 4;
-      four<<<grid, NT, 0, stream>>>(a, u, s);
-    } else {
-      one<<<grid, NT, 0, stream>>>(a, u, s);
+      return launch_after(true, four, grid, NT, 0, stream, a, u, s);
     }
-    return cudaGetLastError();
+    return launch_after(true, one, grid, NT, 0, stream, a, u, s);
   };
   if (a.dim > 64) return go(kv_dequantize_kernel<T, 3, 1>, kv_dequantize_kernel<T, 3, 4>, 3);
   return a.dim > 32 ? go(kv_dequantize_kernel<T, 2, 1>, kv_dequantize_kernel<T, 2, 4>, 2)
