@@ -226,6 +226,8 @@ RecordPlan record_plan(const AttnArgs& a) {
   const int64_t nG = (int64_t)a.n * a.group, units = (int64_t)a.rows * a.kv_heads, all = units * nG;
   p.rows.tiles = nG <= 8 || a.dtype == SV_F32 ? 1 : 2;
   p.rows.groups = div_up(nG, 8 * p.rows.tiles);
+  const int64_t chunks = div_up(most_slots(a.capacity, a.window, a.sinks, a.n), 128) + 1;
+  p.rows.fits = chunks <= 16 && units * p.rows.groups * chunks <= kTokenBlocks;
   p.counters = SV_ATTENTION_ZERO_BYTES;
   p.o_bytes = up256((size_t)2 * kTokenBlocks * 8 * p.rows.tiles * record_dims(a.dim) * 4);
   p.ml_bytes = up256((size_t)2 * kTokenBlocks * 8 * p.rows.tiles * 8);

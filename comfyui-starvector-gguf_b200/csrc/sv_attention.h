@@ -208,9 +208,10 @@ cudaError_t launch_attn_status(const AttnArgs& a, cudaStream_t stream);
 cudaError_t launch_attn_tile(const AttnArgs& a, bool prefix, const TileSplit& split, cudaStream_t stream);
 cudaError_t launch_attn_token(const AttnArgs& a, int blocks, cudaStream_t stream);
 // How the kernel over 4-bit records takes a head's query rows: column tiles of eight per warp, groups of
-// so many rows as units of their own.
+// so many rows as units of their own; and whether tiles of 16 slots (not 32) let every chunk have its own block.
 struct RecordRows {
   int tiles, groups;
+  bool fits;
 };
 cudaError_t launch_attn_record(const AttnArgs& a, const RecordRows& rows, cudaStream_t stream);
 cudaError_t launch_weights16(const AttnArgs& a, cudaStream_t stream);

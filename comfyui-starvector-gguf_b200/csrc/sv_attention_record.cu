@@ -961,7 +961,11 @@ cudaError_t record(const AttnArgs& a, int row_groups, cudaStream_t stream) {
 
 template <typename T, int NI, bool MULTI> cudaError_t record_rows(const AttnArgs& a, const RecordRows& x, cudaStream_t stream) {
   if constexpr (!std::is_same<T, float>::value) {
-    if (x.tiles == 2) return record<T, NI, 2, 2, 8, 3, MULTI>(a, x.groups, stream);
+    // Tiles of 32 slots where blocks take many (679 cycles per 16 slots and scheduler, 798 with tiles of 16); of
+    // 16 where that gives each chunk of 128 slots a block, and a unit not more than 16 to be joined (two rows over 516 slots
+    // 10.7 us, 12.0 with 32; one row over 4096 slots 17.7 us, 14.2 with 32).
+    if (x.tiles == 2)
+      return x.fits ? record<T, NI, 2, 1, 8, 5, MULTI>(a, x.groups, stream) : record<T, NI, 2, 2, 8, 3, MULTI>(a, x.groups, stream);
   }
   return record<T, NI, 1, 1, 12, 4, MULTI>(a, x.groups, stream);
 }

@@ -5,7 +5,7 @@ drop-in generation loops.
 
 The decoder is a stand-in with random weights (no positions, no training), in the
 reference's decoder protocol (`prefill(embeddings, rows, capacity)` returns a decoding
-and the first logits; `step(tokens)`), with two kinds of cache:
+and the first logits; `step(tokens)`), with three kinds of cache:
 
   * beams: the prompt's keys and values are computed once and shared by all beams
     (prefix_attention); each beam keeps only its own tokens, and a beam step reorders
@@ -13,6 +13,9 @@ and the first logits; `step(tokens)`), with two kinds of cache:
   * one long sequence within a budget: each token's attention also accumulates every
     slot's weight (window_attention with `weights`), and when the cache is full the
     lightest slots leave it (kv_evict), so memory and time per token stay bounded.
+  * beams over a cache held in 4 bits: every token's keys and values are quantised as they come
+    (kv_quantize) and attended as they lie (quantized_attention); a beam step moves the records
+    (kv_reorder on the uint8 cache).
 
 The prompt itself runs through window_attention with a sliding window and sinks.
 """
@@ -121,11 +124,37 @@ class BudgetDecoding:
         return forward(self.w, self.w.embedding[tokens.reshape(-1)][:, None], attend)
 
 
-class Decoder:
-    """The reference's decoder protocol over either cache."""
+class QuantizedDecoding:
+    """Beams whose whole cache, the prompt's included, is held in 4 bits."""
 
-    def __init__(self, w, window=64, sinks=4, budget=None, slack=32):
+    def __init__(self, w, prompt, rows, capacity):
+        self.w, self.length = w, prompt[0][0].shape[1]
+        shape = (len(w.layers), rows, w.kv_heads, self.length + max(capacity, 1), sv.kv_record_bytes(w.head_dim))
+        self.keys = torch.zeros(shape, dtype=torch.uint8, device=w.device)
+        self.values = torch.zeros_like(self.keys)
+        for i, (k, v) in enumerate(prompt):
+            sv.kv_quantize(k.expand(rows, -1, -1, -1), v.expand(rows, -1, -1, -1), self.keys[i], self.values[i],
+                           self.length)
+
+    def step(self, tokens):
+        self.length += 1
+
+        def attend(i, q, k, v):
+            sv.kv_quantize(k, v, self.keys[i], self.values[i], self.length)
+            return sv.quantized_attention(q, self.keys[i], self.values[i], self.length)
+
+        return forward(self.w, self.w.embedding[tokens.reshape(-1)][:, None], attend)
+
+    def reorder_device(self, parents):
+        sv.kv_reorder(self.keys, self.values, parents, self.length)
+
+
+class Decoder:
+    """The reference's decoder protocol over any of the caches."""
+
+    def __init__(self, w, window=64, sinks=4, budget=None, slack=32, quantized=False):
         self.w, self.window, self.sinks, self.budget, self.slack = w, window, sinks, budget, slack
+        self.quantized = quantized
 
     def prefill(self, embeddings, rows, capacity):
         prompt = []
@@ -136,6 +165,8 @@ class Decoder:
 
         logits = forward(self.w, embeddings, attend)
         new = capacity - embeddings.shape[1]
+        if self.quantized:
+            return QuantizedDecoding(self.w, prompt, rows, new), logits.expand(rows, -1)
         if self.budget is None:
             return SharedPrefixDecoding(self.w, prompt, rows, new), logits.expand(rows, -1)
         return BudgetDecoding(self.w, prompt, self.budget + self.slack, self.budget), logits
@@ -154,6 +185,9 @@ def main():
     torch.manual_seed(0)
     tokens, why = rs._beam_sample(Decoder(w), prompt, a.tokens, 1.0, 0.9, a.beams, [], None, True, lambda step: None)
     print(f"{a.beams} beams behind a shared prompt of {a.prompt}: {len(tokens)} tokens ({why}), first {tokens[:8]}")
+    tokens, why = rs._beam_sample(Decoder(w, quantized=True), prompt, a.tokens, 1.0, 0.9, a.beams, [], None, True,
+                                  lambda step: None)
+    print(f"{a.beams} beams over a 4-bit cache: {len(tokens)} tokens ({why}), first {tokens[:8]}")
     tokens, why = rs._sample(Decoder(w, budget=128), prompt, a.tokens, 1.0, 0.9, [], None, True, lambda step: None)
     print(f"one sequence within 128 slots: {len(tokens)} tokens ({why}), first {tokens[:8]}")
 
