@@ -47,7 +47,7 @@ namespace {
 constexpr int kJoin = 16;      // parts per first-level group
 constexpr int kMaxFlat = 32;   // parts joined in one level
 constexpr float kSlack = 8.f;  // log2 by which a score may exceed its reference
-constexpr float kNever = -1e30f;  // a reference before the first score
+constexpr float kNever = -0x1.fp127f;  // a reference before the first score
 
 __device__ __forceinline__ float ex2(float x) {
   float y;

@@ -367,6 +367,17 @@ int check_records(const void* k, const void* v, int32_t rows, int32_t kv_heads, 
   return SV_OK;
 }
 
+// The bytes from the first entry of a strided array to behind its last.
+template <int D> int64_t span_of(int64_t entry, const int64_t (&sizes)[D], const int64_t (&strides)[D]) {
+  for (int d = 0; d < D; ++d) entry += (sizes[d] - 1) * strides[d];
+  return entry;
+}
+
+bool overlap(const void* a, int64_t a_bytes, const void* b, int64_t b_bytes) {
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+  return a && b && x < y + (uintptr_t)b_bytes && y < x + (uintptr_t)a_bytes;
+}
+
 }  // namespace
 
 cudaError_t launch_read_records(const ReadArgs& a, cudaStream_t stream) {
@@ -398,11 +409,17 @@ int sv_kv_quantize(const void* keys, const void* values, int32_t dtype, int32_t 
   for (int64_t s : {stride_row, stride_head, stride_token})
     if (s < 0 || s * e % 16) return SV_E_ALIGN;
   if (reinterpret_cast<uintptr_t>(keys) % 16 || reinterpret_cast<uintptr_t>(values) % 16) return SV_E_ALIGN;
-  // Every slot's record is written by its own threads.
-  if (!entries_apart<3>(record_bytes(head_dim), {rows, kv_heads, capacity},
-                        {cache_stride_row, cache_stride_head, cache_stride_slot}))
+  // Every slot's record is written by its own threads, the keys' and the values'.
+  const int64_t record = record_bytes(head_dim);
+  const intptr_t apart = reinterpret_cast<intptr_t>(cache_values) - reinterpret_cast<intptr_t>(cache_keys);
+  if (!entries_apart<4>(record, {rows, kv_heads, capacity, cache_values ? 2 : 1},
+                        {cache_stride_row, cache_stride_head, cache_stride_slot, apart < 0 ? -apart : apart}))
     return SV_E_SHAPE;
   if (tokens == 0) return SV_OK;
+  const int64_t in = span_of<3>(head_dim * e, {rows, kv_heads, tokens}, {stride_row * e, stride_head * e, stride_token * e});
+  const int64_t out = span_of<3>(record, {rows, kv_heads, capacity}, {cache_stride_row, cache_stride_head, cache_stride_slot});
+  for (const void* x : {keys, values})
+    if (overlap(x, in, cache_keys, out) || overlap(x, in, cache_values, out)) return SV_E_ARG;
   WriteArgs a = {{keys, values}, stride_row, stride_head, stride_token,
                  {static_cast<unsigned char*>(cache_keys), static_cast<unsigned char*>(cache_values)},
                  cache_stride_row, cache_stride_head, cache_stride_slot, lengths, out_status,
@@ -424,6 +441,12 @@ int sv_kv_dequantize(const void* cache_keys, const void* cache_values, int32_t r
                                cache_stride_head, cache_stride_slot);
   if (rc) return rc;
   if (reinterpret_cast<uintptr_t>(keys) % 16 || reinterpret_cast<uintptr_t>(values) % 16) return SV_E_ALIGN;
+  const int64_t in = span_of<3>(record_bytes(head_dim), {rows, kv_heads, capacity},
+                                {cache_stride_row, cache_stride_head, cache_stride_slot});
+  const int64_t out = (int64_t)rows * kv_heads * (tokens ? tokens : capacity) * head_dim * (dtype == SV_F32 ? 4 : 2);
+  for (const void* x : {cache_keys, cache_values})
+    if (overlap(x, in, keys, out) || overlap(x, in, values, out)) return SV_E_ARG;
+  if (overlap(keys, out, values, out)) return SV_E_ARG;
   ReadArgs a = {};
   a.cache[0] = static_cast<const unsigned char*>(cache_keys);
   a.cache[1] = static_cast<const unsigned char*>(cache_values);

@@ -517,8 +517,9 @@ int32_t sv_kv_record_bytes(int32_t head_dim);
  *   lengths  int32 [rows] or NULL (= capacity), the new tokens included; values outside [0,
  *          capacity] are clamped and reported as SV_ST_LENGTH
  *   out_status  int32 [rows] or NULL
- * values and cache_values may both be NULL.  rows * kv_heads <= 65535; capacity and tokens <=
- * 2^29; pointers and all strides in bytes multiples of 16.
+ * values and cache_values may both be NULL; the inputs do not overlap the caches (SV_E_ARG).  With tokens 0
+ * nothing is done.  rows * kv_heads <= 65535; capacity and tokens <= 2^29; pointers and all strides in
+ * bytes multiples of 16.
  */
 int sv_kv_quantize(const void* keys, const void* values, int32_t dtype, int32_t rows, int32_t kv_heads, int32_t tokens,
                    int32_t head_dim, int64_t stride_row, int64_t stride_head, int64_t stride_token, void* cache_keys,
@@ -529,8 +530,8 @@ int sv_kv_quantize(const void* keys, const void* values, int32_t dtype, int32_t 
  * Reads such a cache back: place i of keys / values [rows, kv_heads, places, head_dim]
  * (contiguous, of dtype) gets what slot i stands for (tokens 0: places = capacity), or with tokens > 0 that of
  * slot lengths[r] - tokens + i (places = tokens), rounded once to dtype; places without a slot of the row
- * (before 0, from lengths[r] on) become 0.  The rest as sv_kv_quantize.  The outputs must
- * not overlap the caches.
+ * (before 0, from lengths[r] on) become 0.  The rest as sv_kv_quantize; the outputs overlap neither the
+ * caches nor one another (SV_E_ARG).
  */
 int sv_kv_dequantize(const void* cache_keys, const void* cache_values, int32_t rows, int32_t kv_heads, int32_t head_dim,
                      int32_t capacity, int64_t cache_stride_row, int64_t cache_stride_head, int64_t cache_stride_slot,
@@ -540,8 +541,13 @@ int sv_kv_dequantize(const void* cache_keys, const void* cache_values, int32_t r
 /*
  * sv_window_attention over a cache held in 4 bits: the same of the values that the records
  * stand for.  cache_keys, cache_values as in sv_kv_dequantize; they hold records that
- * sv_kv_quantize made.  The workspace has
- * sv_quantized_attention_workspace_bytes(...) bytes; the rest as sv_window_attention.
+ * sv_kv_quantize made (what lies in slots that no query of the row sees is never used).  A group that
+ * stands for NaN makes NaN of what the queries that see its slot take from it, and of nothing else.  Scores are of the values' full precision
+ * (only with weights and many query rows 16-bit calls round keys and values to the inputs' type first); the values
+ * themselves are rounded once to float16 in 16-bit calls.  The workspace has
+ * sv_quantized_attention_workspace_bytes(...) bytes, of which the first SV_ATTENTION_ZERO_BYTES are zero
+ * before its first use; calls with many query rows (more than 64 per key/value head; float32: 32)
+ * keep plain values in it, up to 96 MB or one cache row's.  The rest as sv_window_attention.
  */
 size_t sv_quantized_attention_workspace_bytes(int32_t dtype, int32_t rows, int32_t tokens, int32_t heads,
                                               int32_t kv_heads, int32_t head_dim, int32_t capacity, int32_t window,

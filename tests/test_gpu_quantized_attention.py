@@ -186,6 +186,58 @@ def test_extreme_scores_and_scales(sv, dtype, n):
     check(got, want, tol)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n", [1, 40])
+def test_scale_of_zero_and_queries_that_are_not_finite(sv, dtype, n):
+    """A scale of zero weighs all slots alike; a query with NaN makes its own row NaN, no others."""
+    R, H, K, D, C = 2, 18, 2, 128, 333
+    q = rand((R, n, H, D), 27, dtype)
+    ck, cv = cache(sv, (R, K, C, D), 28), cache(sv, (R, K, C, D), 29)
+    lengths = i32([C, max(n, 100)])
+    k, v = decode(ck, D), decode(cv, D)
+    got = sv.quantized_attention(q, ck, cv, lengths, scale=0.0, window=200, sinks=2)
+    want, tol, _, _ = attention(q, k, v, lengths, None, 200, 2, 0.0)
+    check(got, want, tol, "zero")
+    q[:, n - 1, 3, 5] = torch.nan
+    want, tol, _, _ = attention(q.nan_to_num(0.0), k, v, lengths)
+    got = sv.quantized_attention(q, ck, cv, lengths)
+    assert torch.isnan(got[:, n - 1, 3]).all()
+    rest = torch.ones((n, H), dtype=torch.bool, device=DEV)
+    rest[n - 1, 3] = False
+    check(got[:, rest], want[:, rest], tol[:, rest], "others")
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("D", [64, 128])
+def test_many_rows_in_batches(sv, dtype, D):
+    """More cache rows than are turned into plain values at a time, and two at the end."""
+    R, n, H, K, C = 14, 70, 2, 2, 20000 if D == 128 else 40000
+    q = rand((R, n, H, D), 30, dtype)
+    ck, cv = cache(sv, (R, K, C, D), 31), cache(sv, (R, K, C, D), 32)
+    lengths = i32([C - 911 * r for r in range(R)])
+    status = i32([-1] * R)
+    got = sv.quantized_attention(q, ck, cv, lengths, window=300, sinks=4, status=status)
+    assert status.tolist() == [0] * R
+    for r in (0, 1, 6, R - 2, R - 1):
+        end = int(lengths[r])
+        k, v = decode(ck[r:r + 1, :, :end], D), decode(cv[r:r + 1, :, :end], D)
+        want, tol, _, _ = attention(q[r:r + 1], k, v, None, None, 300, 4)
+        check(got[r:r + 1], want, tol, f"row {r}")
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_long_units_and_many(sv, dtype):
+    """One unit in more parts than one block joins, and far more units than blocks."""
+    for R, H, K, D, C in ((1, 8, 1, 128, 40000), (1, 16, 1, 64, 70000), (90, 9, 3, 128, 700)):
+        q = rand((R, 1, H, D), 33, dtype)
+        ck, cv = cache(sv, (R, K, C, D), 34), cache(sv, (R, K, C, D), 35)
+        lengths = i32([max(1, C - 7 * r) for r in range(R)])
+        got = sv.quantized_attention(q, ck, cv, lengths)
+        want, tol, _, _ = attention(q, decode(ck, D), decode(cv, D), lengths)
+        check(got, want, tol, f"{R} rows")
+        assert torch.equal(got, sv.quantized_attention(q, ck, cv, lengths))
+
+
 def test_streams_and_graphs(sv):
     R, H, K, D, C = 4, 36, 4, 128, 600
     q = rand((R, 1, H, D), 19, torch.bfloat16)

@@ -226,6 +226,26 @@ def test_streams_and_graphs(sv):
             assert torch.equal(out[0][r, :, 2], decode(want[r, :, 0], D).to(DEV).to(torch.bfloat16))
 
 
+def test_offsets_past_32_bits(sv):
+    """Rows four gigabytes apart, the keys' and values' records interleaved."""
+    C, D = 300, 128
+    memory = torch.empty(((4 << 30) + 2 * C * record(D),), dtype=torch.uint8, device=DEV)
+    ck, cv = (memory.as_strided((2, 1, C, record(D)), (4 << 30, 0, 2 * record(D), 1), i * record(D)) for i in range(2))
+    k, v = rand((2, 1, C, D), 11, torch.bfloat16), rand((2, 1, C, D), 12, torch.bfloat16)
+    sv.kv_quantize(k, v, ck, cv)
+    a = sv.kv_dequantize(ck, cv, D)
+    q = rand((2, 1, 9, D), 13, torch.bfloat16)
+    b = sv.quantized_attention(q, ck, cv)
+    many = rand((2, 40, 9, D), 14, torch.bfloat16)
+    c = sv.quantized_attention(many, ck, cv)
+    dense = [x.contiguous() for x in (ck, cv)]
+    assert same_values(dense[0], encode(k.double().cpu().numpy()), D)
+    assert same_values(dense[1], encode(v.double().cpu().numpy()), D)
+    for got, want in zip(a, sv.kv_dequantize(*dense, D)):
+        assert torch.equal(got, want)
+    assert torch.equal(b, sv.quantized_attention(q, *dense)) and torch.equal(c, sv.quantized_attention(many, *dense))
+
+
 def test_refusals(sv):
     k = torch.zeros((2, 1, 4, 128), device=DEV, dtype=torch.float16)
     ck, cv = new_cache(2, 1, 8, 128), new_cache(2, 1, 8, 128)
@@ -241,6 +261,7 @@ def test_refusals(sv):
             (lambda: sv.kv_quantize(k, None, ck, None, 0), ValueError),
             (lambda: sv.kv_quantize(k, None, ck, None, i32([1, 2, 3])), ValueError),
             (lambda: sv.kv_quantize(k, k, ck, ck), RuntimeError),
+            (lambda: sv.kv_quantize(k[:, :, :3], k[:, :, :3], ck[:, :, :7], ck[:, :, 1:]), RuntimeError),
             (lambda: sv.kv_quantize(k, None, ck[:1].expand(2, 1, 8, 80), None), RuntimeError),
             (lambda: sv.kv_quantize(k, None, ck[:, :, :1].expand(2, 1, 8, 80), None), RuntimeError),
             (lambda: sv.kv_quantize(k.cpu(), None, ck, None), RuntimeError),
@@ -249,7 +270,8 @@ def test_refusals(sv):
             (lambda: sv.kv_dequantize(ck, cv, 128, tokens=-1), ValueError),
             (lambda: sv.kv_dequantize(ck, cv, 128, dtype=torch.float64), ValueError),
             (lambda: sv.kv_dequantize(ck, cv[:, :, :4], 128), ValueError),
-            (lambda: sv.kv_dequantize(ck, None, 128, out=(torch.zeros(3, device=DEV), None)), RuntimeError)]:
+            (lambda: sv.kv_dequantize(ck, None, 128, out=(torch.zeros(3, device=DEV), None)), RuntimeError),
+            (lambda: sv.kv_dequantize(ck, cv, 128, out=(k.new_zeros((2, 1, 8, 128)),) * 2), RuntimeError)]:
         with pytest.raises(error):
             bad()
     assert (ck == 0).all() and (cv == 0).all()

@@ -20,7 +20,8 @@ WRITE = dict(keys=16, values=32, dtype=1, rows=2, kv_heads=2, tokens=3, head_dim
     (dict(head_dim=136), -3), (dict(capacity=0), -3), (dict(capacity=2 ** 29 + 1), -3), (dict(tokens=2 ** 29 + 1), -3),
     (dict(rows=40000), -3), (dict(c_slot=64), -3), (dict(c_head=784), -3), (dict(c_row=800), -3), (dict(c_slot=0), -3),
     (dict(c_slot=-80), -3), (dict(c_slot=88), -5), (dict(keys=8), -5), (dict(s_tok=100), -5), (dict(s_head=-384), -5),
-    (dict(ck=4104), -5), (dict(tokens=0), 0),
+    (dict(ck=4104), -5), (dict(tokens=0), 0), (dict(cv=4096 + 80), -3), (dict(cv=4096 + 800), -3), (dict(keys=6000), -1),
+    (dict(values=66000), -1),
 ])
 def test_kv_quantize_rejects(sv, kw, code):
     assert call(sv._lib.lib().sv_kv_quantize, WRITE, kw) == code
@@ -33,7 +34,7 @@ READ = dict(ck=4096, cv=65536, rows=2, kv_heads=2, head_dim=128, capacity=10, c_
 @pytest.mark.parametrize("kw,code", [
     (dict(ck=None), -1), (dict(keys=None), -1), (dict(values=None), -1), (dict(cv=None), -1), (dict(values=16), -1),
     (dict(dtype=-1), -2), (dict(tokens=-1), -3), (dict(head_dim=0), -3), (dict(c_slot=0), -3), (dict(c_row=8), -5),
-    (dict(keys=24), -5),
+    (dict(keys=24), -5), (dict(keys=4112), -1), (dict(values=65536), -1), (dict(keys=64, values=1088), -1),
 ])
 def test_kv_dequantize_rejects(sv, kw, code):
     assert call(sv._lib.lib().sv_kv_dequantize, READ, kw) == code
