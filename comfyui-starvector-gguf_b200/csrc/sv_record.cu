@@ -43,21 +43,28 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   return r;
 }
 
-// x + e rounded to float16, where e in +-|x| 2^-21 is not known in f32: false where it decides.
+// x, which is off by up to three units in its last place, rounded to float16: false where those may decide (the 13
+// bits that are dropped are near their middle), and for float16's subnormals.
 __device__ __forceinline__ bool half_sure(float x, __half& h) {
   h = __float2half_rn(x);
-  const __half below = __float2half_rn(fmaf(x, -0x1p-21f, x)), above = __float2half_rn(fmaf(x, 0x1p-21f, x));
-  return __half_as_ushort(below) == __half_as_ushort(above);
+  const uint32_t bits = __float_as_uint(x);
+  return (bits & 0x1fffu) - (0x1000u - 8u) > 16u && (bits & 0x7fffffffu) >= 0x38800000u;
 }
 
-// The code next to q, which was computed as (x - mid) / scale to within 2^-17, less 8.
-__device__ __noinline__ float code_exactly(float x, float mid, float scale, float q) {
-  const float k = floorf(q);
-  const double border = (double)mid + ((double)k + 0.5) * (double)scale;  // exact: 11 bits and 16, 30 binades
-  const double v = x;
-  if (v > border) return k + 1.f;
-  if (v < border) return k;
-  return (int)k & 1 ? k + 1.f : k;
+__device__ __noinline__ bool above_exactly(float x, float mid, float scale, float half) {
+  return (double)x > (double)mid + (double)half * (double)scale;  // exact: 11 bits and 16, 30 binades
+}
+
+// The whole number next to q = (x - mid) / scale, which was computed to within 2^-17: of the two next to it the upper
+// one where x - mid is above (k + 1/2) scale, or equals it and the lower one is odd.  In f32 where that difference is exact
+// (float16 and bfloat16 mostly; borders themselves are frequent there: one in 2000 values), otherwise in f64.
+__device__ __forceinline__ float code_exactly(float x, float mid, float scale, float q) {
+  const float k = floorf(q), half = k + 0.5f, t = x - mid, u = half * scale;
+  const bool exact = fabsf(x) >= fabsf(mid) ? x - t == mid : t + mid == x;
+  const bool odd = (int)k & 1;
+  bool up = t > u || (t == u && odd);
+  if (!exact) up = above_exactly(x, mid, scale, half) || (odd && !above_exactly(-x, -mid, -scale, half));
+  return up ? k + 1.f : k;
 }
 
 // The smallest and the largest of eight values as they lie, NaN if one is.
@@ -79,15 +86,24 @@ __device__ __forceinline__ void extremes(const uint4& v, float& lo, float& hi, _
   lo = min_nan(__low2float(l), __high2float(l));
   hi = max_nan(__low2float(h), __high2float(h));
 }
-// Eight values in a thread: as loaded, their extremes, one by one.
+__device__ __forceinline__ float2 two_of(uint32_t w, __half) { return __half22float2(*reinterpret_cast<const __half2*>(&w)); }
+__device__ __forceinline__ float2 two_of(uint32_t w, __nv_bfloat16) {
+  return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+}
+
+// Eight values in a thread: as loaded, their extremes, as floats.
 template <typename T> struct Eight {
   uint4 v;
   __device__ __forceinline__ void load(const T* p) { v = __ldg(reinterpret_cast<const uint4*>(p)); }
   __device__ __forceinline__ void ends(float& lo, float& hi) const { extremes(v, lo, hi, T()); }
-  __device__ __forceinline__ float at(int k) const { return (float)reinterpret_cast<const T*>(&v)[k]; }
-  __device__ __forceinline__ void clamp() {  // (the bounds are exact in either type)
+  __device__ __forceinline__ void floats(float (&f)[8]) const {
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-    for (int k = 0; k < 8; ++k) reinterpret_cast<T*>(&v)[k] = from_float<T>(fminf(fmaxf(at(k), -kRecordMost), kRecordMost));
+    for (int k = 0; k < 4; ++k) {
+      const float2 two = two_of(w[k], T());
+      f[2 * k] = two.x;
+      f[2 * k + 1] = two.y;
+    }
   }
 };
 template <> struct Eight<float> {
@@ -97,22 +113,24 @@ template <> struct Eight<float> {
     v[1] = __ldg(reinterpret_cast<const float4*>(p) + 1);
   }
   __device__ __forceinline__ void ends(float& lo, float& hi) const { extremes(v, lo, hi); }
-  __device__ __forceinline__ float at(int k) const { return reinterpret_cast<const float*>(v)[k]; }
-  __device__ __forceinline__ void clamp() {
+  __device__ __forceinline__ void floats(float (&f)[8]) const {
+    const float w[8] = {v[0].x, v[0].y, v[0].z, v[0].w, v[1].x, v[1].y, v[1].z, v[1].w};
 #pragma unroll
-    for (int k = 0; k < 8; ++k) reinterpret_cast<float*>(v)[k] = fminf(fmaxf(at(k), -kRecordMost), kRecordMost);
+    for (int k = 0; k < 8; ++k) f[k] = w[k];
   }
 };
 
 // Where an item (one slot of one head, of keys or values) lies: blocks take slots of one
-// unit, or units whole where these have few slots.
+// unit (ONE: then everything but the slot is the same for the whole block), or units whole where these have few slots.
 struct Item {
   int r, h, i;
   bool in;
 };
-__device__ __forceinline__ Item item_at(int item, int units_log2, int slots_log2, int kv_heads, int rows, int tokens) {
+template <bool ONE, int LPS_LOG2>
+__device__ __forceinline__ Item item_at(int units_log2, int slots_log2, int kv_heads, int rows, int tokens) {
   // A block: 2^units_log2 units of 2^slots_log2 slots each.
-  const int unit = ((int)blockIdx.y << units_log2) + (item >> slots_log2);
+  if (ONE) units_log2 = 0, slots_log2 = 8 - LPS_LOG2;
+  const int item = threadIdx.x >> LPS_LOG2, unit = ((int)blockIdx.y << units_log2) + (ONE ? 0 : item >> slots_log2);
   Item x;
   x.r = unit / kv_heads;
   x.h = unit - x.r * kv_heads;
@@ -121,13 +139,13 @@ __device__ __forceinline__ Item item_at(int item, int units_log2, int slots_log2
   return x;
 }
 
-template <typename T, int LPS_LOG2>  // 2^LPS_LOG2 threads per slot
+template <typename T, int LPS_LOG2, bool ONE>  // 2^LPS_LOG2 threads per slot
 __global__ void __launch_bounds__(NT) kv_quantize_kernel(const __grid_constant__ WriteArgs a, const int units_log2,
                                                          const int slots_log2) {
   wait_before();  // (launched while the kernel before it ends; the next one may be, too)
   launch_dependents();
   const int lane = threadIdx.x & ((1 << LPS_LOG2) - 1), y = lane & 1, i = lane >> 1;
-  const Item it = item_at(threadIdx.x >> LPS_LOG2, units_log2, slots_log2, a.kv_heads, a.rows, a.tokens);
+  const Item it = item_at<ONE, LPS_LOG2>(units_log2, slots_log2, a.kv_heads, a.rows, a.tokens);
   int end = a.capacity, given = 0;
   if (it.in && a.lengths) {
     given = a.lengths[it.r];
@@ -137,7 +155,7 @@ __global__ void __launch_bounds__(NT) kv_quantize_kernel(const __grid_constant__
     a.status[it.r] = a.lengths && given != end ? SV_ST_LENGTH : 0;
   const int blocks = (a.dim + 31) >> 5, slot = end - a.tokens + it.i;
   const bool in = it.in && slot >= 0 && i < blocks;  // (the shuffles need all lanes)
-  const T* src = static_cast<const T*>(blockIdx.z ? a.in[1] : a.in[0]) + it.r * a.i_row + it.h * a.i_head + it.i * a.i_tok;
+  const T* src = static_cast<const T*>(blockIdx.z ? a.in[1] : a.in[0]) + (it.r * a.i_row + it.h * a.i_head) + it.i * a.i_tok;
   Eight<T> x[2];
   bool has[2];
 #pragma unroll
@@ -158,22 +176,15 @@ __global__ void __launch_bounds__(NT) kv_quantize_kernel(const __grid_constant__
     lo[0] = min_nan(lo[0], lo[1]);
     hi[0] = max_nan(hi[0], hi[1]);
   }
-  bool clamps = false;
 #pragma unroll
   for (int e = 0; e < (wide ? 1 : 2); ++e) {
     lo[e] = min_nan(lo[e], __shfl_xor_sync(0xffffffffu, lo[e], 1));
     hi[e] = max_nan(hi[e], __shfl_xor_sync(0xffffffffu, hi[e], 1));
-    clamps |= lo[e] <= hi[e] && (lo[e] < -kRecordMost || hi[e] > kRecordMost);
-  }
-  if (__any_sync(0xffffffffu, clamps)) {
-#pragma unroll
-    for (int e = 0; e < 2; ++e)
-      if (has[e]) x[e].clamp();
   }
   uint32_t word[2] = {0u, 0u};
   uint32_t pair[2] = {0u, 0u};
-  float scale = 0.f, mid = 0.f, inv = 0.f;
-  bool none = true;
+  float scale = 0.f, mid = 0.f, inv = 0.f, base = 0.f;
+  bool none = true, plain = true;
 #pragma unroll
   for (int e = 0; e < 2; ++e) {
     if (!e || !wide) {
@@ -187,6 +198,10 @@ __global__ void __launch_bounds__(NT) kv_quantize_kernel(const __grid_constant__
       if (!half_sure(fmaf(8.f, scale, l), m16)) m16 = __double2half((double)l + 8.0 * (double)scale);
       mid = __half2float(m16);
       inv = scale > 0.f ? __fdividef(1.f, scale) : 0.f;  // (to within two units in the last place)
+      base = -mid * inv;
+      // What is off from the whole number by rounding stays within 2^-17 in one step where mid is not many scales
+      // away; and no code leaves its range where the extremes' do not.
+      plain = fabsf(base) <= 32.f && fmaf(hi[e], inv, base) < 7.4f && fmaf(lo[e], inv, base) > -8.4f;
       pair[e] = none ? 0u : bad ? 0x7e007e00u : (uint32_t)__half_as_ushort(s16) | (uint32_t)__half_as_ushort(m16) << 16;
       none = none || bad;
     }
@@ -194,17 +209,27 @@ __global__ void __launch_bounds__(NT) kv_quantize_kernel(const __grid_constant__
       // The whole number next to q by adding 1.5 2^23 (and 8): its last bits are the code then.
       constexpr float kAdd = 12582912.f + 8.f;
       constexpr uint32_t kBits = 0x4b400000u;
-      float q[8], r[8], edge = 0.f;
+      float v[8], q[8], r[8], edge = 0.f;
+      x[e].floats(v);
+      if (!__all_sync(__activemask(), plain)) {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          v[k] = fminf(fmaxf(v[k], -kRecordMost), kRecordMost);
+          q[k] = fminf(fmaxf((v[k] - mid) * inv, -8.f), 7.f);
+        }
+      } else {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) q[k] = fmaf(v[k], inv, base);
+      }
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
-        q[k] = fminf(fmaxf((x[e].at(k) - mid) * inv, -8.f), 7.f);
         r[k] = q[k] + kAdd;
         edge = fmaxf(edge, fabsf(q[k] - (r[k] - kAdd)));
       }
       if (edge > 0.5f - 0x1p-16f) {
 #pragma unroll
         for (int k = 0; k < 8; ++k)
-          if (fabsf(q[k] - (r[k] - kAdd)) > 0.5f - 0x1p-16f) r[k] = code_exactly(x[e].at(k), mid, scale, q[k]) + kAdd;
+          if (fabsf(q[k] - (r[k] - kAdd)) > 0.5f - 0x1p-16f) r[k] = code_exactly(v[k], mid, scale, q[k]) + kAdd;
       }
       // Dimension 4 t + 2 a + b, t = 2 y + (k >> 2); the numbers' other bits are taken off the sum.
 #pragma unroll
@@ -214,7 +239,7 @@ __global__ void __launch_bounds__(NT) kv_quantize_kernel(const __grid_constant__
     }
   }
   if (!in) return;
-  unsigned char* rec = (blockIdx.z ? a.cache[1] : a.cache[0]) + it.r * a.row + it.h * a.head + (int64_t)slot * a.slot;
+  unsigned char* rec = (blockIdx.z ? a.cache[1] : a.cache[0]) + (it.r * a.row + it.h * a.head) + (int64_t)slot * a.slot;
   uint32_t* codes = reinterpret_cast<uint32_t*>(rec);
   codes[2 * y * blocks + i] = word[0];
   codes[(2 * y + 1) * blocks + i] = word[1];
@@ -253,7 +278,7 @@ __global__ void __launch_bounds__(NT) kv_dequantize_kernel(const __grid_constant
   wait_before();  // (launched while the kernel before it ends; the next one may be, too)
   launch_dependents();
   const int lane = threadIdx.x & ((1 << LPS_LOG2) - 1), y = lane & 1, i = lane >> 1;
-  Item it = item_at(threadIdx.x >> LPS_LOG2, units_log2, slots_log2, a.kv_heads, a.rows, a.tokens);
+  Item it = item_at<(PER > 1), LPS_LOG2>(units_log2, slots_log2, a.kv_heads, a.rows, a.tokens);
   if (PER > 1) it.i += (int)blockIdx.x * (PER - 1) << slots_log2;
   const int blocks = (a.dim + 31) >> 5;
   if (it.r >= a.rows || it.i >= a.tokens || i >= blocks) return;
@@ -330,12 +355,13 @@ dim3 grid_of(int lps_log2, int64_t units, int tokens, bool both, int& units_log2
 template <typename T> cudaError_t write_records(const WriteArgs& a, cudaStream_t stream) {
   int u, s;
   const int64_t units = (int64_t)a.rows * a.kv_heads;
-  auto go = [&](auto kernel, int lps_log2) {
+  auto go = [&](auto one, auto many, int lps_log2) {
     const dim3 grid = grid_of(lps_log2, units, a.tokens, a.in[1] != nullptr, u, s);
-    return launch_after(true, kernel, grid, NT, 0, stream, a, u, s);
+    return launch_after(true, u == 0 ? one : many, grid, NT, 0, stream, a, u, s);
   };
-  if (a.dim > 64) return go(kv_quantize_kernel<T, 3>, 3);
-  return a.dim > 32 ? go(kv_quantize_kernel<T, 2>, 2) : go(kv_quantize_kernel<T, 1>, 1);
+  if (a.dim > 64) return go(kv_quantize_kernel<T, 3, true>, kv_quantize_kernel<T, 3, false>, 3);
+  return a.dim > 32 ? go(kv_quantize_kernel<T, 2, true>, kv_quantize_kernel<T, 2, false>, 2)
+                    : go(kv_quantize_kernel<T, 1, true>, kv_quantize_kernel<T, 1, false>, 1);
 }
 
 template <typename T> cudaError_t read_records(const ReadArgs& a, cudaStream_t stream) {
@@ -344,7 +370,7 @@ template <typename T> cudaError_t read_records(const ReadArgs& a, cudaStream_t s
   auto go = [&](auto one, auto four, int lps_log2) {
     // Four slots a thread where that leaves two blocks per SM.
     dim3 grid = grid_of(lps_log2, units, a.tokens, a.out[1] != nullptr, u, s);
-    if ((int64_t)grid.x * grid.y * grid.z >= 8 * 148) {
+    if (u == 0 && (int64_t)grid.x * grid.y * grid.z >= 8 * 148) {
       grid.x = (grid.x + 3) / 4;
       return launch_after(true, four, grid, NT, 0, stream, a, u, s);
     }
