@@ -25,11 +25,13 @@
 // a group do not pay for sixteen; weights pass from the one to the other by a transposition
 // (movmatrix).
 //
-// What bounds it: the records' bytes; next to that the instructions that turn codes into
-// operands (about 270 per 16 slots and warp at eight rows; the memory's rate allows 450).  A warp
-// takes tiles of 16 slots through a ring in shared memory of its own (cp.async, zeros for
-// slots past the end): registers alone would keep too few bytes in flight, since 16 slots are
-// only 2560.  Rows of a tile are taken in an order in which neither the keys' nor the
+// What bounds it: the instructions that turn codes into operands, and the products.  128 dimensions, cycles of a
+// scheduler per 16 slots (the memory's rate allows 450): 524 to 540 with four query rows (5.3 to 5.5 TB/s of
+// records), 679 with nine, of which about 300 are the products' and 300 the integer instructions'.  64 rows of 36/4
+// heads over 4096 slots take 64 us (2.6 TB/s; floor 26 us), 8 rows over up to 16384 slots 28 us (floor 9.6), of
+// which start, units' ends and joins are a large part.
+// A warp takes tiles of 16 or 32 slots through a ring in shared memory of its own (cp.async, zeros for slots past
+// the end): registers alone would keep too few bytes in flight, since 16 slots are only 2560.  Rows of a tile are taken in an order in which neither the keys' nor the
 // values' reads meet in a bank (kSlot).
 //
 // Work split and joins as in sv_attention_token.cu: one list of chunks (a tile per warp) over all

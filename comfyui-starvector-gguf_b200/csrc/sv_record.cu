@@ -3,7 +3,9 @@
 // A group of threads takes one slot of one head: thread (i, y) of it block i's dimensions
 // 8 y .. 8 y + 7 and 16 + 8 y .. 16 + 8 y + 7, which are the words t = 2 y and 2 y + 1 of the
 // block.  Both kernels move each byte once; a warp's loads and stores cover whole
-// sectors.
+// sectors.  Reading is bound by memory (8 x 4096 slots of four heads of 128 in bfloat16: 16 us, floor 13.4; four
+// slots a thread where there are many, 19.5 us with one).  Writing is bound by its instructions (8192 tokens of four heads
+// in 9.3 us; one slot a thread: with four a call under a profiler took 17.5 us, 14.7 with one).
 //
 // Writing.  Of a group's finite values x, clamped to +-32768, with extremes lo, hi:
 //   scale = f16((hi - lo) / 15),  mid = f16(lo + 8 scale),

@@ -272,6 +272,42 @@ def test_streams_and_graphs(sv):
     assert torch.equal(eager, want)
 
 
+# Tokens, heads and key/value heads: single tokens, a draft in several groups of rows, and chunks past 64 rows.
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n,H,K", [(1, 36, 4), (1, 4, 4), (5, 36, 4), (40, 8, 2), (90, 36, 4)])
+def test_output_in_the_queries_place(sv, dtype, n, H, K):
+    """Outputs may take their own queries' place: many blocks share a unit (long rows) or blocks take many."""
+    for R, C in ((2, 6000), (40, 300)):
+        q = rand((R, n, H, 128), 40, dtype)
+        ck, cv = cache(sv, (R, K, C, 128), 41), cache(sv, (R, K, C, 128), 42)
+        lengths = i32(lengths_for(R, n, C))
+        want = sv.quantized_attention(q, ck, cv, lengths, window=C // 2, sinks=3)
+        for _ in range(3):
+            x = q.clone()
+            got = sv.quantized_attention(x, ck, cv, lengths, window=C // 2, sinks=3, out=x)
+            assert got.data_ptr() == x.data_ptr() and torch.equal(got, want)
+
+
+def test_calls_that_share_a_kept_workspace(sv):
+    """Calls of many sizes, types and kinds in turn on one stream give what each gives first: workspaces are kept by the
+    power of two of their size, and plain and 4-bit calls share them."""
+    calls = []
+    for i, (R, n, H, K, D, C, dtype) in enumerate([
+            (1, 1, 4, 1, 64, 40, torch.float16), (8, 1, 36, 4, 128, 3000, torch.bfloat16), (2, 90, 8, 2, 64, 700, torch.float16),
+            (600, 1, 8, 8, 64, 60, torch.bfloat16), (3, 5, 36, 4, 128, 900, torch.float32), (2, 50, 36, 4, 128, 300, torch.float32),
+            (4, 130, 36, 4, 128, 500, torch.bfloat16)]):
+        q, ck, cv = rand((R, n, H, D), 50 + i, dtype), cache(sv, (R, K, C, D), 60 + i), cache(sv, (R, K, C, D), 70 + i)
+        k, v = sv.kv_dequantize(ck, cv, D, dtype=dtype)
+        calls.append(lambda q=q, ck=ck, cv=cv: sv.quantized_attention(q, ck, cv))
+        calls.append(lambda q=q, k=k, v=v: sv.window_attention(q, k, v))
+        calls.append(lambda q=q, ck=ck, cv=cv, R=R, K=K, C=C: sv.quantized_attention(
+            q, ck, cv, weights=torch.zeros((R, K, C), device=DEV)))
+    want = [call() for call in calls]
+    for order in (range(len(calls)), reversed(range(len(calls))), [5 * i % len(calls) for i in range(len(calls))]):
+        for i in order:
+            assert torch.equal(calls[i](), want[i]), i
+
+
 def test_decode_loop(sv):
     """A few steps as a decoder takes them: write the token, attend, reorder, evict; against 64 bits."""
     L, R, H, K, D, C = 1, 3, 8, 2, 64, 40
