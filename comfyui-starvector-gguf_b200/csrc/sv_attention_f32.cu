@@ -267,6 +267,9 @@ __global__ void __launch_bounds__(NT, 1) attn_f32_kernel(const __grid_constant__
       for (int e = 0; e < TK; ++e) {
         const int from = (lane & 28) | (e >> 1), j = j0 + e;
         float w[2];
+        bool sees[2];  // (a weight may be zero)
+#pragma unroll
+        for (int y = 0; y < 2; ++y) sees[y] = prefix || slot_seen(a, sp.start, pos[y], low[y], j);
 #pragma unroll
         for (int y = 0; y < 2; ++y) w[y] = __shfl_sync(0xffffffffu, e & 1 ? s[2 * y + 1] : s[2 * y], from);
         if (j >= jend) break;
@@ -284,7 +287,7 @@ __global__ void __launch_bounds__(NT, 1) attn_f32_kernel(const __grid_constant__
             for (int k = 0; k < 4; ++k)
 #pragma unroll
               for (int y = 0; y < 2; ++y)
-                if (w[y] != 0.f && !isfinite(v[k])) o[4 * u + k][2 * y + x] = fmaf(w[y], v[k], o[4 * u + k][2 * y + x]);
+                if (sees[y] && !isfinite(v[k])) o[4 * u + k][2 * y + x] = fmaf(w[y], v[k], o[4 * u + k][2 * y + x]);
           }
       }
 #pragma unroll

@@ -757,20 +757,39 @@ __global__ void __launch_bounds__(NW * 32, 1)
           }
         }
         if (MULTI && hide) {
+          // Ones where a row sees a slot, in the weights' place: weights may be zero.
+          constexpr uint32_t one = FULL ? 0x3f803f80u : kOnes;
+          const int tile = tile0 + k * NW;
+          const bool in_a = tile < rt.ta;
+          const int j0 = (in_a ? rt.a0 + tile * TK : rt.b0 + (tile - rt.ta) * TK) + 16 * h, jend = in_a ? rt.a1 : rt.b1;
+          uint32_t sees[NT][2];
+#pragma unroll
+          for (int u = 0; u < NT; ++u)
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+              const int j = j0 + (x ? s1 : s0);
+              uint32_t both = 0u;
+#pragma unroll
+              for (int y = 0; y < 2; ++y) {
+                const int pos = pos_first + (m0 + 8 * u + 2 * t + y) / group;
+                if (j < jend && slot_seen(a, rt.start, pos, window_low(a, rt.start, pos), j)) both |= y ? one & 0xffff0000u : one & 0xffffu;
+              }
+              sees[u][x] = transposed(both);
+            }
 #pragma unroll
           for (int b = 0; b < NB; ++b)
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
               const int y = NI > 2 ? b : j >> 1;
-              const uint32_t one = FULL ? 0x3f803f80u : kOnes, x0 = bad[0][y] & one, x1 = bad[1][y] & one;
+              const uint32_t x0 = bad[0][y] & one, x1 = bad[1][y] & one;
 #pragma unroll
               for (int u = 0; u < NT; ++u) {
                 float seen[4];
                 if constexpr (FULL) {
                   seen[0] = seen[1] = seen[2] = seen[3] = 0.f;
-                  mma_bf16(seen, x0, x0, x1, x1, pw[0][u][0], pw[0][u][1]);
+                  mma_bf16(seen, x0, x0, x1, x1, sees[u][0], sees[u][1]);
                 } else {
-                  mma_new(seen, x0, x0, x1, x1, pw[0][u][0], pw[0][u][1]);
+                  mma_new(seen, x0, x0, x1, x1, sees[u][0], sees[u][1]);
                 }
 #pragma unroll
                 for (int q = 0; q < 4; ++q)

@@ -1,0 +1,52 @@
+"""quantized_attention where a small error of its own would show: structured inputs whose results follow from a few
+exact numbers.  Keys that are constant within a group are held exactly (scale 0), so scores are known.  Bounds count
+roundings: U of the output's type, half a step each; what a 16-bit call's tensor cores take is float16 (2^-11)."""
+import math
+
+import pytest
+import torch
+
+from _attention_ref import U, check
+from _records_ref import attention, decode, record
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+DTYPES = [torch.float32, torch.float16, torch.bfloat16]
+SHORT = [torch.float16, torch.bfloat16]
+
+
+def rand(shape, seed, dtype, scale=1.0):
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    return (scale * torch.randn(shape, generator=g, device=DEV)).to(dtype)
+
+
+def i32(values):
+    return torch.tensor(values, dtype=torch.int32, device=DEV)
+
+
+def records(sv, x):
+    c = torch.zeros(x.shape[:-1] + (record(x.shape[-1]),), dtype=torch.uint8, device=DEV)
+    sv.kv_quantize(x, None, c, None)
+    return c
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n", [2, 3, 6, 16, 90])
+@pytest.mark.parametrize("below", [5, 18, 40, 200])
+def test_nan_under_a_small_weight(sv, dtype, n, below):
+    """Values that stand for NaN make NaN of every query that sees their slot, however little it weighs there."""
+    R, H, K, D, C = 1, 4, 2, 64, 320
+    where = C - 2  # seen by the last two queries
+    q = torch.ones((R, n, H, D), dtype=dtype, device=DEV)
+    x, y = torch.zeros((R, K, C, D), device=DEV), rand((R, K, C, D), 1, torch.float32)
+    x[:, :, where] = -below / (D * D ** -0.5)
+    ck, clean = records(sv, x), records(sv, y)
+    y[:, 1, where, 20:24] = torch.nan  # dimensions 16..31
+    cv = records(sv, y)
+    for window in (0, 40):
+        want, tol, _, _ = attention(q, decode(ck, D), decode(clean, D), None, None, window, 2)
+        got = sv.quantized_attention(q, ck, cv, window=window, sinks=2)
+        assert torch.isnan(got[:, -2:, 2:, 16:32]).all()
+        nan = torch.zeros_like(got, dtype=torch.bool)
+        nan[:, -2:, 2:, 16:32] = True
+        check(got[~nan], want[~nan], tol[~nan], "the rest")
