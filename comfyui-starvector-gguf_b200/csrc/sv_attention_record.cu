@@ -18,7 +18,7 @@
 // Float32: queries in two float16 pieces, weights and values in three bfloat16 pieces each and the six products
 // that count.
 // The softmax as in sv_attention_token.cu: the reference moves only when a score exceeds it by
-// 2^8.
+// 2^8.  Weights are held to 2^-32 of the heaviest (kRaised).
 //
 // Both products are turned round, S^T = K Q^T and O^T = V^T P^T (mma.m16n8k16): slots and
 // dimensions fill the 16 rows, and the query rows take columns in eights, so that four heads of
@@ -49,6 +49,10 @@ namespace {
 constexpr int kJoin = 16;      // parts per first-level group
 constexpr int kMaxFlat = 32;   // parts joined in one level
 constexpr float kSlack = 8.f;  // log2 by which a score may exceed its reference
+// 16-bit calls: log2 of the weight that a new reference stands for, so that weights use float16's range up to 2^15 and
+// those down to 2^-32 of the reference do not vanish in it (with a reference of weight 1 a slot that outweighed 16384
+// others by 2^24.5 each lost or gained two fifths of their share).
+constexpr float kRaised = 7.f;
 constexpr float kNever = -0x1.fp127f;  // a reference before the first score
 
 __device__ __forceinline__ float ex2(float x) {
@@ -213,6 +217,7 @@ __global__ void __launch_bounds__(NW * 32, 1)
   constexpr int QP = FULL ? 2 : 1, WP = FULL ? 3 : HALVES ? 2 : 1;  // pieces of a query, of a weight
   constexpr bool KEEP_Q = NT * NW <= 16 && !FULL;                   // the queries' operands in registers
   constexpr uint32_t kOnes = 0x3c003c00u;
+  constexpr float kRaise = FULL ? 0.f : kRaised, kMove = kSlack + kRaise;
   // [NW][RING][keys, values of a tile], then [NW][ROWS][OS] floats.
   extern __shared__ __align__(16) unsigned char ring_bytes[];
   float* const outs = reinterpret_cast<float*>(ring_bytes + NW * RING * 2 * F::TILE);
@@ -624,7 +629,7 @@ __global__ void __launch_bounds__(NW * 32, 1)
       for (int h = 0; h < SUB; ++h)
 #pragma unroll
         for (int u = 0; u < NT; ++u) most = fmaxf(most, fmaxf(fmaxf(z[h][u][0][0], z[h][u][0][1]), fmaxf(z[h][u][1][0], z[h][u][1][1])));
-      if (__any_sync(0xffffffffu, most > kSlack)) {
+      if (__any_sync(0xffffffffu, most > kMove)) {
 #pragma unroll
         for (int u = 0; u < NT; ++u)
 #pragma unroll
@@ -634,7 +639,7 @@ __global__ void __launch_bounds__(NW * 32, 1)
             for (int h = 0; h < SUB; ++h) mx = fmaxf(mx, fmaxf(s[h][u][y], s[h][u][2 + y]));
 #pragma unroll
             for (int x = 4; x < 32; x <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
-            const float now = fminf(-mx * fr[u][y], from[u][y]);
+            const float now = fminf(kRaise - mx * fr[u][y], from[u][y]);
             const float by = now == from[u][y] ? 1.f : ex2(now - from[u][y]);
             from[u][y] = now;
             l[u][y] *= by;

@@ -191,6 +191,8 @@ __global__ void __launch_bounds__(NT, 1) attn_tile_kernel(const __grid_constant_
   using L = Layout<DC, SRC>;
   using H = std::conditional_t<SRC == kPlain, T, __half>;
   constexpr int RING = L::RING, STAGES = L::STAGES;
+  // Of a 4-bit cache: log2 of the weight that a new reference stands for, as in sv_attention_record.cu.
+  constexpr float kRaise = SRC == kPlain ? 0.f : 7.f;
   static_assert(!PAIRED || RING % 2 == 0, "a group's every other step alternates a barrier's phase");
   constexpr int LPR = DC * 8, RPI = 32 / LPR;  // lanes of a row's 16-byte vectors, rows per warp instruction
   extern __shared__ unsigned char dyn_raw[];
@@ -667,10 +669,10 @@ __global__ void __launch_bounds__(NT, 1) attn_tile_kernel(const __grid_constant_
           }
           // A NaN stays in the maximum, so that it makes the whole row NaN.
           const float top = max_nan(max_nan(mx[0], mx[1]), max_nan(mx[2], mx[3])) * scale;
-          const bool need = !(top <= ref + kSlack) && top != -INFINITY;
+          const bool need = !(top <= ref + (kSlack + kRaise)) && top != -INFINITY;
           if (__any_sync(0xffffffffu, need)) {
-            const float f = need ? ex2(ref - top) : 1.f;
-            if (need) ref = top;
+            const float f = need ? ex2(ref - (top - kRaise)) : 1.f;
+            if (need) ref = top - kRaise;
             l *= f;
             if (own > 0) {  // the product before must be in, and this step's waits for these weights
               constexpr int back = PAIRED ? 2 : 1;

@@ -544,7 +544,7 @@ int sv_kv_dequantize(const void* cache_keys, const void* cache_values, int32_t r
  * sv_kv_quantize made (what lies in slots that no query of the row sees is never used).  A group that
  * stands for NaN makes NaN of what the queries that see its slot take from it, and of nothing else.  Scores are of the values' full precision
  * (only with weights and many query rows 16-bit calls round keys and values to the inputs' type first); the values
- * themselves are rounded once to float16 in 16-bit calls.  The workspace has
+ * themselves are rounded once to float16 in 16-bit calls, whose weights are held to 2^-32 of the heaviest.  The workspace has
  * sv_quantized_attention_workspace_bytes(...) bytes, of which the first SV_ATTENTION_ZERO_BYTES are zero
  * before its first use; calls with many query rows (more than 64 per key/value head; float32: 32)
  * keep plain values in it, up to 96 MB or one cache row's.  The rest as sv_window_attention.

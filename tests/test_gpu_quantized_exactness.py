@@ -50,3 +50,26 @@ def test_nan_under_a_small_weight(sv, dtype, n, below):
         nan = torch.zeros_like(got, dtype=torch.bool)
         nan[:, -2:, 2:, 16:32] = True
         check(got[~nan], want[~nan], tol[~nan], "the rest")
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("R,n,H,K,D", [(150, 1, 4, 2, 64), (40, 1, 36, 4, 128), (20, 5, 16, 2, 64), (1, 1, 8, 1, 128),
+                                       (2, 100, 4, 2, 64), (1, 100, 9, 1, 128)])
+@pytest.mark.parametrize("below", [20.5, 24.5, 25.2])
+def test_many_light_slots_beside_a_heavy_one(sv, dtype, R, n, H, K, D, below):
+    """A first slot of value zero that outweighs each other slot by 2^below: the others' share is the output.  A
+    weight is held to 2^-32 of the heaviest (the 16-bit calls' operands: 2^-25 of what stands at 2^7), the rest is relative:
+    the weights' and the values' roundings, the output's, 2^-18 for scores of 25, and half a step of 1 for each of the
+    C / 4 weights at most that one thread adds to the heavy one."""
+    C = 16384 if R < 100 else 8192
+    x, y = torch.zeros((R, K, C, D), device=DEV, dtype=torch.float16), torch.ones((R, K, C, D), device=DEV, dtype=torch.float16)
+    x[:, :, 0], y[:, :, 0] = 1.0, 0.0
+    ck, cv = records(sv, x), records(sv, y)
+    q = torch.ones((R, n, H, D), dtype=dtype, device=DEV)
+    got = sv.quantized_attention(q, ck, cv, scale=below * math.log(2) / D)
+    light = torch.arange(C - n, C, dtype=torch.float64, device=DEV)
+    mass = light * 2.0 ** -below
+    want = (mass / (1 + mass))[None, :, None, None].expand_as(got)
+    relative = U[dtype] + 2.0 ** -18 + C / 4 * 2.0 ** -24 + (2 * 2.0 ** -11 if dtype != torch.float32 else 0.0)
+    tol = relative * want + (light * 2.0 ** -32 + 2.0 ** -25 if dtype != torch.float32 else light * 0)[None, :, None, None]
+    check(got, want, tol)
