@@ -444,10 +444,12 @@ __global__ void __launch_bounds__(NW * 32, 1)
     }
     const float high = __half2float(__float2half_rn(own));
     sh_qm[warp][lane] = make_uint2(pack16(-8.f * high, high), pack16(-8.f * (own - high), own - high));
-    // (Scores past f32's range stay within it by a smaller factor: any of them is the whole softmax.  A
-    // factor of zero would make NaN of hidden slots' -infinity.)
-    if (t == 0)
-      sh_fr[8 * warp + g] = fmaxf(fabsf(a.scale) * __uint_as_float((uint32_t)(min(ex, 230) + 10) << 23), 0x1p-126f);  // 2^(ex - 141 + 24)
+    // |scale| 2^(ex - 141 + 24).  (Past 2^112 a smaller factor: it keeps scores past f32's range within it, and any two
+    // that differ are 2^40 apart by then.  A factor of zero would make NaN of hidden slots' -infinity.)
+    if (t == 0) {
+      const float factor = fabsf(a.scale) * __uint_as_float((uint32_t)min(ex, 254) << 23) * 1024.f;
+      sh_fr[8 * warp + g] = fminf(fmaxf(factor, 0x1p-126f), 0x1p112f);
+    }
   };
 
   auto write_out = [&](int r, int head, int m, int d, float4 x, float L) {  // m: row of the head's nG

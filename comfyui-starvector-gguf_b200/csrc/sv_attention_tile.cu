@@ -301,9 +301,11 @@ __global__ void __launch_bounds__(NT, 1) attn_tile_kernel(const __grid_constant_
         const float up = copysignf(__uint_as_float((uint32_t)(268 - min(ex, 254)) << 23), a.scale);
         v[k] = make_uint4(Half16<H>::pack(x[0] * up, x[1] * up), Half16<H>::pack(x[2] * up, x[3] * up),
                           Half16<H>::pack(x[4] * up, x[5] * up), Half16<H>::pack(x[6] * up, x[7] * up));
-        // (Zero would make NaN of hidden slots' -infinity.)
+        // (Zero would make NaN of hidden slots' -infinity; past 2^89 scores could leave f32, and any two that differ are
+        // 2^41 apart by then.)
         if (my_vec == 0)
-          sh.row_scale[wg][my_row + k * RPI] = fmaxf(fabsf(a.scale) * __uint_as_float((uint32_t)(min(ex, 254) - 14) << 23), 0x1p-126f);
+          sh.row_scale[wg][my_row + k * RPI] =
+              fminf(fmaxf(fabsf(a.scale) * __uint_as_float((uint32_t)(min(ex, 254) - 14) << 23), 0x1p-126f), 0x1p89f);
       } else {
         v[k].x ^= flip, v[k].y ^= flip, v[k].z ^= flip, v[k].w ^= flip;
       }
@@ -934,8 +936,9 @@ static std::atomic<int32_t> test_head{0};
 cudaError_t launch_attn_tile(const AttnArgs& args, bool prefix, const TileSplit& split, cudaStream_t stream) {
   AttnArgs a = args;
   a.test_head = test_head.load(std::memory_order_relaxed) ? test_head.exchange(0) : 0;
-  // A scale of zero weighs all slots alike; a tiny one does so without 0 * inf at the mask.
-  if (fabsf(a.scale) < 1e-30f) a.scale = 1e-30f;
+  // A scale of zero weighs all slots alike; the least normal one does so without 0 * inf at the mask (kHalves: the
+  // rows' factors are kept from zero instead).
+  if (!(a.halves && a.dtype == 2) && fabsf(a.scale) < 0x1p-126f) a.scale = copysignf(0x1p-126f, a.scale);
   if (!encode_fn()) return cudaErrorNotSupported;
   Maps maps;
   memset(&maps, 0, sizeof maps);

@@ -73,3 +73,36 @@ def test_many_light_slots_beside_a_heavy_one(sv, dtype, R, n, H, K, D, below):
     relative = U[dtype] + 2.0 ** -18 + C / 4 * 2.0 ** -24 + (2 * 2.0 ** -11 if dtype != torch.float32 else 0.0)
     tol = relative * want + (light * 2.0 ** -32 + 2.0 ** -25 if dtype != torch.float32 else light * 0)[None, :, None, None]
     check(got, want, tol)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("n", [1, 4, 90])
+@pytest.mark.parametrize("up", [90, 100, 108, 113])
+def test_large_queries_under_a_small_scale(sv, dtype, n, up):
+    """Queries times 2^up under a scale times 2^-up are the same call."""
+    R, H, K, D, C = 2, 8, 2, 128, 500
+    q = rand((R, n, H, D), 2, dtype)
+    ck, cv = records(sv, rand((R, K, C, D), 3, dtype)), records(sv, rand((R, K, C, D), 4, dtype))
+    got = sv.quantized_attention(q * 2.0 ** up, ck, cv, scale=D ** -0.5 * 2.0 ** -up)
+    assert torch.equal(got, sv.quantized_attention(q, ck, cv, scale=D ** -0.5))
+
+
+@pytest.mark.parametrize("n", [1, 4, 90])
+def test_a_scale_of_zero_under_large_queries(sv, n):
+    """All slots weigh alike whatever the queries' size; a negative scale below float's range is as good as zero."""
+    R, H, K, D, C = 2, 8, 2, 128, 300
+    q = (rand((R, n, H, D), 2, torch.float32) * 2.0 ** 120).bfloat16()
+    ck, cv = records(sv, rand((R, K, C, D), 3, torch.float32)), records(sv, rand((R, K, C, D), 4, torch.float32))
+    want = sv.quantized_attention(torch.zeros_like(q), ck, cv)
+    assert torch.equal(sv.quantized_attention(q, ck, cv, scale=0.0), want)
+    assert torch.equal(sv.quantized_attention(rand(q.shape, 5, q.dtype), ck, cv, scale=-1e-60), want)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n", [1, 90])
+def test_window_attention_of_large_queries_under_a_small_scale(sv, dtype, n):
+    """Over a 16- or 32-bit cache too: queries and keys times powers of two under a scale that takes them back."""
+    R, H, K, D, C, up = 2, 8, 2, 64, 300, 0 if dtype == torch.float16 else 53
+    q, k, v = rand((R, n, H, D), 6, dtype), rand((R, K, C, D), 7, dtype), rand((R, K, C, D), 8, dtype)
+    got = sv.window_attention(q * 2.0 ** up, k * 2.0 ** up, v, scale=-0.125 * 4.0 ** -up)
+    assert torch.equal(got, sv.window_attention(q, k, v, scale=-0.125))
