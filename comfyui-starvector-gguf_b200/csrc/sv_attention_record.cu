@@ -434,13 +434,14 @@ __global__ void __launch_bounds__(NW * 32, 1)
         }
       }
     }
-    // Group t's sum, in the keys' units; in halves, for scale (times -8) and mid.
+    // Group t's sum, 2^10 above the keys' units (in theirs the halves would be float16's subnormals: scores off by 2^-15 of
+    // the largest query times the middles); in halves, for scale (times -8) and mid.
     float own = 0.f;
 #pragma unroll
     for (int k = 0; k < NG; ++k) {
       sum[k] += __shfl_xor_sync(0xffffffffu, sum[k], 1);
       sum[k] += __shfl_xor_sync(0xffffffffu, sum[k], 2);
-      if (k == t) own = sum[k] * (FULL ? 0x1p-14f : 0x1p-24f);  // (float32: clear of float16's subnormals)
+      if (k == t) own = sum[k] * 0x1p-14f;
     }
     const float high = __half2float(__float2half_rn(own));
     sh_qm[warp][lane] = make_uint2(pack16(-8.f * high, high), pack16(-8.f * (own - high), own - high));
@@ -559,10 +560,8 @@ __global__ void __launch_bounds__(NW * 32, 1)
         for (int u = 0; u < NT; ++u) {
           const uint2 q = KEEP_Q ? qm[u] : sh_qm[u][lane];
           mma_new(s[h][u], own[0], own[1], own[0], own[1], q.x, q.y);
-          if constexpr (FULL) {
 #pragma unroll
-            for (int y = 0; y < 4; ++y) s[h][u][y] *= 0x1p-10f;
-          }
+          for (int y = 0; y < 4; ++y) s[h][u][y] *= 0x1p-10f;
         }
 #pragma unroll
         for (int grp = 0; grp < NG; ++grp) {

@@ -106,3 +106,26 @@ def test_window_attention_of_large_queries_under_a_small_scale(sv, dtype, n):
     q, k, v = rand((R, n, H, D), 6, dtype), rand((R, K, C, D), 7, dtype), rand((R, K, C, D), 8, dtype)
     got = sv.window_attention(q * 2.0 ** up, k * 2.0 ** up, v, scale=-0.125 * 4.0 ** -up)
     assert torch.equal(got, sv.window_attention(q, k, v, scale=-0.125))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n,H,K,D", [(1, 4, 1, 128), (1, 16, 1, 96), (1, 9, 1, 64), (4, 8, 2, 128)])
+def test_scores_are_exact(sv, dtype, n, H, K, D):
+    """The weights (float32) of keys with middles up to 100 that cancel in the scores, under queries with one large
+    value a group and many 2^-10 of it: the groups' sums have to be exact.  The bound: 2^-20 of sum |q k| per score,
+    twice."""
+    R, C, G = 2, 400, 32 if D > 64 else 16
+    g = torch.Generator(device=DEV).manual_seed(5)
+    q = ((torch.rand((R, n, H, D), generator=g, device=DEV) * 2 - 1) * 2.0 ** -10).to(dtype)
+    q[..., ::G] = 1.0
+    a = (torch.rand((R, K, C, 1), generator=g, device=DEV) * 200 - 100)
+    x = torch.zeros((R, K, C, D), device=DEV)
+    x[..., :G], x[..., G:2 * G] = a, -a
+    x = x.half()
+    ck, cv = records(sv, x), records(sv, rand((R, K, C, D), 6, torch.float16))
+    assert torch.equal(decode(ck, D), x.double())
+    w = torch.zeros((R, K, C), device=DEV)
+    sv.quantized_attention(q, ck, cv, scale=1.0, weights=w)
+    _, _, want, _ = attention(q, x.double(), decode(cv, D), scale=1.0)
+    S = 2 * 100 * (1 + G * 2.0 ** -10)
+    check(w, want, want * (math.expm1(2 * 2.0 ** -20 * S) + 2.0 ** -19) + 1e-30)
