@@ -510,6 +510,7 @@ __global__ void __launch_bounds__(NW * 32, 1)
     const uint32_t va = slot_at(2 * t) * REC, vb = slot_at(2 * t + 1) * REC;  // rows 8..15: the slots behind them
     float fr[NT][2], from[NT][2];  // from: a row's reference, negative (far below any score before the first)
     float o[NT][MT][4], l[NT][2];
+    bool huge = false;  // a reference past 2^20, where the fused product's exactness would set its own maximum far off
     uint4 qb[KEEP_Q ? NT : 1][NI];
     uint2 qm[NT];
 #pragma unroll
@@ -615,7 +616,7 @@ __global__ void __launch_bounds__(NW * 32, 1)
       }
       // ---- weights, by what exceeds the reference; past the slack it moves
       float z[SUB][NT][2][2], most = -INFINITY;
-      auto shift = [&]() {
+      auto shift = [&](const bool fused) {
 #pragma unroll
         for (int h = 0; h < SUB; ++h)
 #pragma unroll
@@ -623,9 +624,12 @@ __global__ void __launch_bounds__(NW * 32, 1)
 #pragma unroll
             for (int x = 0; x < 2; ++x)
 #pragma unroll
-              for (int y = 0; y < 2; ++y) z[h][u][x][y] = fmaf(s[h][u][2 * x + y], fr[u][y], from[u][y]);
+              for (int y = 0; y < 2; ++y)
+                z[h][u][x][y] = fused ? fmaf(s[h][u][2 * x + y], fr[u][y], from[u][y])
+                                      : __fadd_rn(__fmul_rn(s[h][u][2 * x + y], fr[u][y]), from[u][y]);
       };
-      shift();
+      shift(true);
+      if (huge) shift(false);
 #pragma unroll
       for (int h = 0; h < SUB; ++h)
 #pragma unroll
@@ -640,9 +644,10 @@ __global__ void __launch_bounds__(NW * 32, 1)
             for (int h = 0; h < SUB; ++h) mx = fmaxf(mx, fmaxf(s[h][u][y], s[h][u][2 + y]));
 #pragma unroll
             for (int x = 4; x < 32; x <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
-            const float now = fminf(kRaise - mx * fr[u][y], from[u][y]);
+            const float now = fminf(kRaise - __fmul_rn(mx, fr[u][y]), from[u][y]);
             const float by = now == from[u][y] ? 1.f : ex2(now - from[u][y]);
             from[u][y] = now;
+            huge = huge || (fabsf(now) > 0x1p20f && now != -kNever);
             l[u][y] *= by;
 #pragma unroll
             for (int j = 0; j < MT; ++j) {
@@ -650,7 +655,9 @@ __global__ void __launch_bounds__(NW * 32, 1)
               o[u][j][2 + y] *= by;
             }
           }
-        shift();
+        huge = __any_sync(0xffffffffu, huge);
+        shift(true);
+        if (huge) shift(false);
       }
 #pragma unroll
       for (int h = 0; h < SUB; ++h) {

@@ -48,6 +48,7 @@ constexpr int kSMs = 148;
 constexpr int BM = 128, BN = 64;
 constexpr int kMostRing = 4;       // steps (64 slots) whose keys and values are held
 constexpr float kSlack = 8.f;
+constexpr float kHuge = 0x1p20f;  // references whose last place is no longer small beside the slack
 
 // kPlain: keys and values of the queries' type.  What a cache held in 4 bits stands for comes as float16:
 // kHalves: for bfloat16 queries, which become float16 too, each row times a power of two (they lose nothing, and the
@@ -671,7 +672,7 @@ __global__ void __launch_bounds__(NT, 1) attn_tile_kernel(const __grid_constant_
           }
           // A NaN stays in the maximum, so that it makes the whole row NaN.
           const float top = max_nan(max_nan(mx[0], mx[1]), max_nan(mx[2], mx[3])) * scale;
-          const bool need = !(top <= ref + (kSlack + kRaise)) && top != -INFINITY;
+          const bool need = !(fabsf(ref) > kHuge ? top - ref <= kSlack + kRaise : top <= ref + (kSlack + kRaise)) && top != -INFINITY;
           if (__any_sync(0xffffffffu, need)) {
             const float f = need ? ex2(ref - (top - kRaise)) : 1.f;
             if (need) ref = top - kRaise;
@@ -692,7 +693,14 @@ __global__ void __launch_bounds__(NT, 1) attn_tile_kernel(const __grid_constant_
           }
           // Nothing seen yet: weights of zero; a maximum of +inf: NaN, as inf - inf.
           const float at = ref == -INFINITY ? 0.f : (ref == INFINITY ? __int_as_float(0x7fc00000) : ref);
-          const uint64_t scale2 = pack2(scale, scale), at2 = pack2(-at, -at);
+          // Scores past kHuge are rounded as their maximum was: the fused product would set that maximum itself far off.
+          float by = scale;
+          if (fabsf(ref) > kHuge) {
+#pragma unroll
+            for (int c = 0; c < BN; ++c) s[c] *= scale;
+            by = 1.f;
+          }
+          const uint64_t scale2 = pack2(by, by), at2 = pack2(-at, -at);
           uint64_t sum[2] = {0, 0}, z[BN / 2];
 #pragma unroll
           for (int k = 0; k < BN / 2; ++k) z[k] = fma2(pack2(s[2 * k], s[2 * k + 1]), scale2, at2);

@@ -129,3 +129,39 @@ def test_scores_are_exact(sv, dtype, n, H, K, D):
     _, _, want, _ = attention(q, x.double(), decode(cv, D), scale=1.0)
     S = 2 * 100 * (1 + G * 2.0 ** -10)
     check(w, want, want * (math.expm1(2 * 2.0 ** -20 * S) + 2.0 ** -19) + 1e-30)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n", [1, 4, 12, 90])
+@pytest.mark.parametrize("size", [1000.0, 8000.0, 32000.0])
+@pytest.mark.parametrize("quantized", [True, False])
+def test_scores_far_past_the_whole_numbers_of_f32(sv, quantized, dtype, n, size):
+    """Scores of +-2^30 and more, of which one is the whole softmax (rows of one slot and of none among them).  Two
+    roundings: the weight's (and over records the value's) to float16 or the 16-bit cache's type, and the output's."""
+    R, H, K, D, C = 2, 8, 2, 128, 60 if n != 12 else 12
+    q = (rand((R, n, H, D), 7, torch.float32) * size).clamp(-60000, 60000).to(dtype)
+    ck = records(sv, (rand((R, K, C, D), 8, torch.float32) * size).clamp(-30000, 30000))
+    cv = records(sv, rand((R, K, C, D), 9, torch.float32))
+    k, v = decode(ck, D), decode(cv, D)
+    if quantized:
+        got = sv.quantized_attention(q, ck, cv)
+    else:
+        k, v = k.to(dtype), v.to(dtype)
+        got = sv.window_attention(q, k, v)
+        k, v = k.double(), v.double()
+    for r in range(R):
+        for i in range(n):
+            end = C - n + i + 1
+            if end < 1:
+                assert (got[r, i] == 0).all()
+                continue
+            s = q[r, i].double().view(K, H // K, D) @ k[r, :, :end].transpose(1, 2) * D ** -0.5
+            S = q[r, i].double().abs().view(K, H // K, D) @ k[r, :, :end].abs().transpose(1, 2) * D ** -0.5
+            top = s.topk(min(2, end), -1)
+            # The others are behind by more than twice the scores' own error.
+            clear = (top.values[..., 0] - top.values[..., -1] > 2.0 ** -9 * S.amax(-1) + 50) | (end == 1)
+            want = torch.stack([v[r, h][top.indices[h, :, 0]] for h in range(K)]).view(H, D)
+            off = (got[r, i].double() - want).abs()
+            ok = off <= (U[dtype] + (2 * 2.0 ** -11 if quantized else U[dtype])) * want.abs() + 2.0 ** -24
+            assert torch.isfinite(got[r, i]).all()
+            assert ok.view(K, H // K, D)[clear].all()
