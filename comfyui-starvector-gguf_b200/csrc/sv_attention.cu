@@ -213,7 +213,8 @@ struct RecordPlan {
   bool direct;
   RecordRows rows;
   size_t counters, o_bytes, ml_bytes, lse_bytes, score_bytes;  // direct
-  int32_t batch;                                               // otherwise: cache rows at a time,
+  int32_t batch;                                               // cache rows at a time (direct: whose scores are kept),
+  int32_t heads;                                               // direct: key/value heads at a time; otherwise all:
   int32_t halves, pairs;                                       // float16 values, the keys' in pairs;
   size_t before, array;                                        // bytes of the attention's own, of the keys or values
   size_t total() const {
@@ -223,7 +224,7 @@ struct RecordPlan {
 
 RecordPlan record_plan(const AttnArgs& a) {
   RecordPlan p = {};
-  const int64_t nG = (int64_t)a.n * a.group, units = (int64_t)a.rows * a.kv_heads, all = units * nG;
+  const int64_t nG = (int64_t)a.n * a.group, units = (int64_t)a.rows * a.kv_heads;
   p.rows.tiles = nG <= 8 || a.dtype == SV_F32 ? 1 : 2;
   p.rows.groups = div_up(nG, 8 * p.rows.tiles);
   const int64_t chunks = div_up(most_slots(a.capacity, a.window, a.sinks, a.n), 128) + 1;
@@ -231,12 +232,20 @@ RecordPlan record_plan(const AttnArgs& a) {
   p.counters = SV_ATTENTION_ZERO_BYTES;
   p.o_bytes = up256((size_t)2 * kTokenBlocks * 8 * p.rows.tiles * record_dims(a.dim) * 4);
   p.ml_bytes = up256((size_t)2 * kTokenBlocks * 8 * p.rows.tiles * 8);
-  p.lse_bytes = a.weights ? up256(all * 4) : 0;
-  p.score_bytes = a.weights ? up256(all * a.capacity * 4) : 0;
   // A unit's counter each, and chunks (of at least 128 slots) counted in 31 bits.
   p.direct = p.rows.groups <= kMostRecordGroups && units * p.rows.groups <= 65536 &&
-             units * p.rows.groups * (a.capacity / 128 + 8) < (int64_t)1 << 31 && p.score_bytes <= kMostScores;
-  if (!p.direct) {
+             units * p.rows.groups * (a.capacity / 128 + 8) < (int64_t)1 << 31;
+  p.heads = a.kv_heads;
+  if (p.direct) {
+    p.batch = a.rows;
+    if (a.weights) {  // as many rows, or of one row as many heads, as kMostScores holds
+      const int64_t unit = nG * a.capacity * 4, fit = std::max<int64_t>(kMostScores / unit, 1);
+      if (fit < units) p.batch = (int32_t)std::max<int64_t>(fit / a.kv_heads, 1);
+      p.heads = (int32_t)std::min<int64_t>(fit, a.kv_heads);
+      p.lse_bytes = up256((size_t)p.batch * p.heads * nG * 4);
+      p.score_bytes = up256((size_t)p.batch * p.heads * unit);
+    }
+  } else {
     p.halves = a.dtype != SV_F32 && !a.weights;  // (the accumulated weights' product takes keys of the queries' type)
     p.pairs = p.halves && a.dtype == SV_F16;
     const size_t row = (size_t)a.kv_heads * a.capacity * a.dim * (a.dtype == SV_F32 ? 4 : 2);
@@ -373,6 +382,20 @@ int sv_quantized_attention(const void* q, int32_t dtype, int32_t rows, int32_t t
   rc = check_pointers(a, scale);
   if (rc) return rc;
   if (!workspace || workspace_bytes < p.total()) return SV_E_WORKSPACE;
+  // The call's rows from r on, and key/value heads from h on (of records as they are).
+  const auto rows_from = [&](AttnArgs& b, int32_t r, int32_t h) {
+    const int64_t e = dtype == SV_F32 ? 4 : 2, head = (int64_t)h * a.group;
+    b.q = static_cast<const unsigned char*>(q) + (r * q_stride_row + head * q_stride_head) * e;
+    b.out = static_cast<unsigned char*>(out) + ((int64_t)r * tokens * heads + head) * head_dim * e;
+    if (p.direct) {
+      b.k = static_cast<const unsigned char*>(cache_keys) + r * cache_stride_row + h * cache_stride_head;
+      b.v = static_cast<const unsigned char*>(cache_values) + r * cache_stride_row + h * cache_stride_head;
+    }
+    b.lengths = lengths ? lengths + r : nullptr;
+    b.starts = starts ? starts + r : nullptr;
+    b.status = out_status ? out_status + r : nullptr;
+    b.weights = weights ? weights + r * weights_stride_row + h * weights_stride_head : nullptr;
+  };
   if (reinterpret_cast<uintptr_t>(workspace) % 16) return SV_E_ALIGN;
   if (p.direct) {
     auto take = [&](size_t bytes) {
@@ -385,8 +408,16 @@ int sv_quantized_attention(const void* q, int32_t dtype, int32_t rows, int32_t t
     a.part_ml = reinterpret_cast<float2*>(take(p.ml_bytes));
     a.lse = reinterpret_cast<float*>(take(p.lse_bytes));
     a.scores = reinterpret_cast<float*>(take(p.score_bytes));
-    if (launch_attn_record(a, p.rows, s) != cudaSuccess) return SV_E_CUDA;
-    return a.weights && launch_scores_weights(a, s) != cudaSuccess ? SV_E_CUDA : SV_OK;
+    for (int32_t r = 0; r < rows; r += p.batch)
+      for (int32_t h = 0; h < kv_heads; h += p.heads) {
+        AttnArgs b = a;
+        b.rows = std::min(p.batch, rows - r);
+        b.kv_heads = std::min(p.heads, kv_heads - h);
+        rows_from(b, r, h);
+        if (launch_attn_record(b, p.rows, s) != cudaSuccess) return SV_E_CUDA;
+        if (b.weights && launch_scores_weights(b, s) != cudaSuccess) return SV_E_CUDA;
+      }
+    return SV_OK;
   }
   ReadArgs x = {};
   x.row = cache_stride_row;
@@ -403,18 +434,14 @@ int sv_quantized_attention(const void* q, int32_t dtype, int32_t rows, int32_t t
   x.seen = tokens;
   x.window = a.window;
   x.sinks = a.sinks;
-  const int64_t e = dtype == SV_F32 ? 4 : 2;
   for (int32_t r = 0; r < rows; r += p.batch) {
     AttnArgs b = a;
     x.rows = b.rows = std::min(p.batch, rows - r);
     x.cache[0] = static_cast<const unsigned char*>(cache_keys) + r * cache_stride_row;
     x.cache[1] = static_cast<const unsigned char*>(cache_values) + r * cache_stride_row;
-    x.lengths = b.lengths = lengths ? lengths + r : nullptr;
-    x.starts = b.starts = starts ? starts + r : nullptr;
-    b.q = static_cast<const unsigned char*>(q) + r * q_stride_row * e;
-    b.out = static_cast<unsigned char*>(out) + (int64_t)r * tokens * heads * head_dim * e;
-    b.status = out_status ? out_status + r : nullptr;
-    b.weights = weights ? weights + r * weights_stride_row : nullptr;
+    rows_from(b, r, 0);
+    x.lengths = b.lengths;
+    x.starts = b.starts;
     if (launch_read_records(x, s) != cudaSuccess) return SV_E_CUDA;
     rc = run(b, workspace, p.before, s);
     if (rc) return rc;

@@ -165,3 +165,65 @@ def test_scores_far_past_the_whole_numbers_of_f32(sv, quantized, dtype, n, size)
             ok = off <= (U[dtype] + (2 * 2.0 ** -11 if quantized else U[dtype])) * want.abs() + 2.0 ** -24
             assert torch.isfinite(got[r, i]).all()
             assert ok.view(K, H // K, D)[clear].all()
+
+
+def two_keys(sv, D, fine):
+    """Records of two keys that stand for 1 +- a little: what lies below the last place of float16 at 1 (fine), or below
+    bfloat16's only; and by how much their sums over the dimensions differ."""
+    G = 32 if D > 64 else 16
+    x = torch.ones((1, 1, 2, D), dtype=torch.float64, device=DEV)
+    if fine:
+        s = 2.0 ** -14
+        x[:, :, 0], x[:, :, 1] = 1 + 7 * s, 1 - 8 * s
+        x[:, :, 0, ::G], x[:, :, 1, ::G] = 1 - 8 * s, 1 + 7 * s
+    else:
+        x[:, :, 0] = 1 + 3 * 2.0 ** -10
+    c = records(sv, x.float())
+    assert torch.equal(decode(c, D), x)
+    return c, (x[0, 0, 0].sum() - x[0, 0, 1].sum()).item()
+
+
+def alternating(sv, dtype, R, n, H, K, D, C, fine=True):
+    """Every second slot of half the weight's logarithm more: (q, scale, keys, values, shares [n], weights [n, C],
+    relative bound).  What the rounded keys would do instead: weigh all alike, a share of 0.5 for 0.62."""
+    two, apart = two_keys(sv, D, fine)
+    ck = two.expand(R, K, 2, two.shape[-1]).repeat(1, 1, C // 2, 1)
+    v = torch.zeros((1, 1, 2, D), device=DEV)
+    v[:, :, 0] = 1.0
+    cv = records(sv, v).expand(R, K, 2, two.shape[-1]).repeat(1, 1, C // 2, 1)
+    q = torch.full((R, n, H, D), 2.0, dtype=dtype, device=DEV)
+    scale = 0.25 / apart
+    j = torch.arange(C, device=DEV)
+    see = j <= torch.arange(C - n, C, device=DEV)[:, None]
+    e = torch.where(see, torch.where(j % 2 == 0, math.exp(0.5), 1.0).double(), 0.0)
+    p = e / e.sum(1, keepdim=True)
+    share = p[:, ::2].sum(1)
+    # Scores to 2^-20 of sum |q k| (about 2 D scale), twice; f32 sums of the slots that one thread adds.
+    bound = math.expm1(2 * 2.0 ** -20 * 2 * D * scale) + C / 4 * 2.0 ** -24 + 2.0 ** -18
+    return q, scale, ck, cv, share, p.sum(0), bound
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("R,n,H,K,D,C", [(40, 1, 36, 4, 128, 49152), (3, 5, 36, 4, 64, 131072), (1, 8, 32, 8, 64, 300000)])
+def test_more_scores_than_are_kept(sv, dtype, R, n, H, K, D, C):
+    """Accumulated weights of few query rows whose scores take more than 256 MB: cache rows, and heads of one row, in
+    turn, with keys as exact as below that."""
+    assert R * n * H * C * 4 > 1 << 28
+    q, scale, ck, cv, share, weights, bound = alternating(sv, dtype, R, n, H, K, D, C)
+    w = torch.zeros((R, K, C), device=DEV)
+    status = i32([-1] * R)
+    got = sv.quantized_attention(q, ck, cv, scale=scale, weights=w, status=status)
+    assert status.tolist() == [0] * R
+    roundings = U[dtype] + (2 * 2.0 ** -11 if dtype != torch.float32 else 0.0)
+    want = share[None, :, None, None].expand_as(got)
+    check(got, want, want * (bound + roundings))
+    check(w, (H // K * weights).expand_as(w), (H // K * weights * bound).expand_as(w), "weights")
+    # Other cache rows' queries and records reach a row: each on its own place.
+    if R > 1:
+        q[1], ck[1, 1:] = 0, ck[1, 1:].flip(1)
+        w.zero_()
+        again = sv.quantized_attention(q, ck, cv, scale=scale, weights=w)
+        assert torch.equal(again[0], got[0]) and torch.equal(again[2:], got[2:])
+        half = torch.arange(C - n + 1, C + 1, device=DEV)
+        half = ((half + 1) // 2 / half.double())[:, None, None].expand_as(again[1])
+        check(again[1], half, half * (bound + roundings), "a row of its own")
