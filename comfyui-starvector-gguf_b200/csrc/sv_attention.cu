@@ -215,10 +215,11 @@ struct RecordPlan {
   size_t counters, o_bytes, ml_bytes, lse_bytes, score_bytes;  // direct
   int32_t batch;                                               // cache rows at a time (direct: whose scores are kept),
   int32_t heads;                                               // direct: key/value heads at a time; otherwise all:
-  int32_t halves, pairs;                                       // float16 values, the keys' in pairs;
+  int32_t halves, pairs, bf16_pairs;                           // float16 values, the keys' in pairs, in bfloat16 too;
   size_t before, array;                                        // bytes of the attention's own, of the keys or values
+  int arrays() const { return 2 + pairs + 2 * bf16_pairs; }
   size_t total() const {
-    return direct ? counters + o_bytes + ml_bytes + lse_bytes + score_bytes : before + (pairs ? 3 : 2) * array;
+    return direct ? counters + o_bytes + ml_bytes + lse_bytes + score_bytes : before + arrays() * array;
   }
 };
 
@@ -246,10 +247,11 @@ RecordPlan record_plan(const AttnArgs& a) {
       p.score_bytes = up256((size_t)p.batch * p.heads * unit);
     }
   } else {
-    p.halves = a.dtype != SV_F32 && !a.weights;  // (the accumulated weights' product takes keys of the queries' type)
-    p.pairs = p.halves && a.dtype == SV_F16;
+    p.halves = a.dtype != SV_F32;
+    p.pairs = a.dtype == SV_F16;
+    p.bf16_pairs = a.dtype == SV_BF16 && a.weights;  // (the accumulated weights' product takes keys of the queries' type)
     const size_t row = (size_t)a.kv_heads * a.capacity * a.dim * (a.dtype == SV_F32 ? 4 : 2);
-    const size_t fit = kMostValues / ((p.pairs ? 3 : 2) * row);
+    const size_t fit = kMostValues / (p.arrays() * row);
     p.batch = fit >= (size_t)a.rows ? a.rows : fit > 1 ? (int32_t)fit : 1;
     p.array = up256(p.batch * row);
     static const char some = 0;
@@ -427,6 +429,10 @@ int sv_quantized_attention(const void* q, int32_t dtype, int32_t rows, int32_t t
   a.v = x.out[1] = w + p.before + p.array;
   a.halves = p.halves;
   a.k_low = x.low = p.pairs ? w + p.before + 2 * p.array : nullptr;
+  if (weights && p.halves) {
+    a.w_k = p.pairs ? a.k : w + p.before + 2 * p.array;
+    a.w_low = p.pairs ? a.k_low : w + p.before + 3 * p.array;
+  }
   x.dtype = p.halves ? SV_F16 : dtype;
   x.kv_heads = kv_heads;
   x.dim = head_dim;
@@ -443,6 +449,15 @@ int sv_quantized_attention(const void* q, int32_t dtype, int32_t rows, int32_t t
     x.lengths = b.lengths;
     x.starts = b.starts;
     if (launch_read_records(x, s) != cudaSuccess) return SV_E_CUDA;
+    if (p.bf16_pairs) {
+      ReadArgs z = x;
+      z.dtype = SV_BF16;
+      z.cache[1] = nullptr;
+      z.out[0] = const_cast<void*>(a.w_k);
+      z.out[1] = nullptr;
+      z.low = const_cast<void*>(a.w_low);
+      if (launch_read_records(z, s) != cudaSuccess) return SV_E_CUDA;
+    }
     rc = run(b, workspace, p.before, s);
     if (rc) return rc;
   }

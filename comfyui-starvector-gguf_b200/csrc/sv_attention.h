@@ -51,6 +51,7 @@ struct AttnArgs {
   int32_t p_splits, o_splits;  // o_splits 0: the own part is written directly
   int32_t w_splits;            // of the query rows, for the accumulated weights of calls with many
   const void* k_low;           // with halves and float16 queries: what the keys' rounding left, laid out as they are
+  const void *w_k, *w_low;     // with halves and weights: keys of the queries' type and what their rounding left, as above
   int32_t halves;              // keys and values are float16 whatever the queries are (values of a 4-bit cache)
   int32_t test_head;           // test hook: one plus the key/value head whose waits run out
 };

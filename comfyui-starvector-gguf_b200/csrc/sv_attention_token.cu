@@ -711,21 +711,26 @@ __global__ void __launch_bounds__(256) scores_weights_kernel(const __grid_consta
 // rows 8 at a time as the B operand, both straight from global memory as above; the
 // queries come from L1 for seven of a block's eight warps.  One warp owns its slots, so
 // the sum's order is fixed and no atomics are needed.  Bound by the products.
-template <typename T, int DC, bool FULL>
+// LOW: the keys of a 4-bit cache in two pieces of T.
+template <typename T, int DC, bool FULL, bool LOW>
 __global__ void __launch_bounds__(NT) attn_weights16_kernel(const __grid_constant__ AttnArgs a) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
   const int unit = blockIdx.y, h = unit % a.kv_heads, r = unit / a.kv_heads, nG = a.n * a.group, vecs = a.dim >> 3;
   const RowSpan sp = row_span(a, r);
   const int j0 = (blockIdx.x * NW + warp) * 16;
   if (j0 >= sp.end || j0 + 16 <= sp.start) return;
-  const T* kb = static_cast<const T*>(a.k) + r * a.kv_row + h * a.kv_head;
-  uint4 kf[2][2 * DC], qf[2 * DC], qn[2 * DC];
+  uint4 kf[2][2 * DC], kl[2][2 * DC], qf[2 * DC], qn[2 * DC];
+  auto load_k = [&](uint4(&to)[2][2 * DC], const void* from) {
+    const T* kb = static_cast<const T*>(from) + r * a.kv_row + h * a.kv_head;
 #pragma unroll
-  for (int x = 0; x < 2; ++x)
+    for (int x = 0; x < 2; ++x)
 #pragma unroll
-    for (int u = 0; u < 2 * DC; ++u)
-      kf[x][u] = load_stream(kb + (j0 + g + 8 * x) * a.kv_slot + (4 * u + t) * 8,
-                             j0 + g + 8 * x < sp.end && (FULL || 4 * u + t < vecs));
+      for (int u = 0; u < 2 * DC; ++u)
+        to[x][u] = load_stream(kb + (j0 + g + 8 * x) * a.kv_slot + (4 * u + t) * 8,
+                               j0 + g + 8 * x < sp.end && (FULL || 4 * u + t < vecs));
+  };
+  load_k(kf, LOW ? a.w_k : a.k);
+  if (LOW) load_k(kl, a.w_low);
   const int first_pos = sp.end - a.n;
   int m_first, m_end;
   weight_rows(a, sp, j0, 16, blockIdx.z, m_first, m_end);
@@ -763,6 +768,10 @@ __global__ void __launch_bounds__(NT) attn_weights16_kernel(const __grid_constan
     for (int u = 0; u < 2 * DC; ++u) {
       Mma<T>::run(c[0], kf[0][u].x, kf[1][u].x, kf[0][u].y, kf[1][u].y, qf[u].x, qf[u].y);
       Mma<T>::run(c[1], kf[0][u].z, kf[1][u].z, kf[0][u].w, kf[1][u].w, qf[u].z, qf[u].w);
+      if (LOW) {
+        Mma<T>::run(c[0], kl[0][u].x, kl[1][u].x, kl[0][u].y, kl[1][u].y, qf[u].x, qf[u].y);
+        Mma<T>::run(c[1], kl[0][u].z, kl[1][u].z, kl[0][u].w, kl[1][u].w, qf[u].z, qf[u].w);
+      }
     }
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
@@ -805,20 +814,21 @@ cudaError_t launch_attn_token(const AttnArgs& a, int blocks, cudaStream_t stream
   return a.dtype == 1 ? token_any<__half>(a, blocks, stream) : token_any<__nv_bfloat16>(a, blocks, stream);
 }
 
-template <typename T> cudaError_t weights16(const AttnArgs& a, cudaStream_t stream) {
+template <typename T, bool LOW> cudaError_t weights16(const AttnArgs& a, cudaStream_t stream) {
   const dim3 grid((unsigned)((a.capacity + NW * 16 - 1) / (NW * 16)), (unsigned)(a.rows * a.kv_heads),
                   (unsigned)a.w_splits);
   if (a.dim == 128)
-    attn_weights16_kernel<T, 2, true><<<grid, NT, 0, stream>>>(a);
+    attn_weights16_kernel<T, 2, true, LOW><<<grid, NT, 0, stream>>>(a);
   else if (a.dim > 64)
-    attn_weights16_kernel<T, 2, false><<<grid, NT, 0, stream>>>(a);
+    attn_weights16_kernel<T, 2, false, LOW><<<grid, NT, 0, stream>>>(a);
   else
-    attn_weights16_kernel<T, 1, false><<<grid, NT, 0, stream>>>(a);
+    attn_weights16_kernel<T, 1, false, LOW><<<grid, NT, 0, stream>>>(a);
   return cudaGetLastError();
 }
 
 cudaError_t launch_weights16(const AttnArgs& a, cudaStream_t stream) {
-  return a.dtype == 1 ? weights16<__half>(a, stream) : weights16<__nv_bfloat16>(a, stream);
+  if (a.w_low) return a.dtype == 1 ? weights16<__half, true>(a, stream) : weights16<__nv_bfloat16, true>(a, stream);
+  return a.dtype == 1 ? weights16<__half, false>(a, stream) : weights16<__nv_bfloat16, false>(a, stream);
 }
 
 cudaError_t launch_scores_weights(const AttnArgs& a, cudaStream_t stream) {

@@ -334,10 +334,10 @@ __global__ void __launch_bounds__(NT) kv_dequantize_kernel(const __grid_constant
       }
       T* to = out + ((int64_t)x << slots_log2) * a.dim + d;
       store8(to, v);
-      if constexpr (std::is_same<T, __half>::value) {
+      if constexpr (!std::is_same<T, float>::value) {
         if (a.low && blockIdx.z == 0) {
 #pragma unroll
-          for (int k = 0; k < 8; ++k) v[k] -= __half2float(__float2half_rn(v[k]));
+          for (int k = 0; k < 8; ++k) v[k] -= (float)from_float<T>(v[k]);
           store8(static_cast<T*>(a.low) + (to - static_cast<T*>(a.out[0])), v);
         }
       }

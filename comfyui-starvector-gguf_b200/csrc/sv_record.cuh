@@ -28,7 +28,7 @@ struct ReadArgs {
   const unsigned char* cache[2];  // keys, values (may be null)
   int64_t row, head, slot;        // strides in bytes
   void* out[2];                   // [rows][kv_heads][tokens][dim]
-  void* low;                      // with float16: what the keys' rounding left, rounded; or null
+  void* low;                      // with 16-bit types: what the keys' rounding left, rounded; or null
   const int32_t *lengths, *starts;
   int32_t* status;
   int32_t dtype, rows, kv_heads, dim, capacity;

@@ -542,12 +542,14 @@ int sv_kv_dequantize(const void* cache_keys, const void* cache_values, int32_t r
  * sv_window_attention over a cache held in 4 bits: the same of the values that the records
  * stand for.  cache_keys, cache_values as in sv_kv_dequantize; they hold records that
  * sv_kv_quantize made (what lies in slots that no query of the row sees is never used).  A group that
- * stands for NaN makes NaN of what the queries that see its slot take from it, and of nothing else.  Scores are of the values' full precision
- * (only with weights and many query rows 16-bit calls round keys and values to the inputs' type first); the values
- * themselves are rounded once to float16 in 16-bit calls, whose weights are held to 2^-32 of the heaviest.  The workspace has
- * sv_quantized_attention_workspace_bytes(...) bytes, of which the first SV_ATTENTION_ZERO_BYTES are zero
- * before its first use; calls with many query rows (more than 64 per key/value head; float32: 32)
- * keep plain values in it, up to 96 MB or one cache row's.  The rest as sv_window_attention.
+ * stands for NaN makes NaN of what the queries that see its slot take from it, and of nothing else.  Scores are of the
+ * values' full precision (float32 calls: of queries to 22 bits), but bfloat16 calls with many query rows (more than
+ * 64 per key/value head) round the keys once to float16.  The values are rounded once to float16 in 16-bit calls,
+ * whose weights are held to 2^-32 of the heaviest, and in bfloat16 calls rounded to float16's 11 bits.
+ * The workspace has sv_quantized_attention_workspace_bytes(...) bytes, of which the first SV_ATTENTION_ZERO_BYTES are
+ * zero before its first use; calls with many query rows (more than 64 per key/value head; float32: 32) keep plain
+ * values in it, up to 96 MB or one cache row's; with weights the others keep scores, up to 256 MB or one
+ * key/value head's.  The rest as sv_window_attention.
  */
 size_t sv_quantized_attention_workspace_bytes(int32_t dtype, int32_t rows, int32_t tokens, int32_t heads,
                                               int32_t kv_heads, int32_t head_dim, int32_t capacity, int32_t window,

@@ -227,3 +227,19 @@ def test_more_scores_than_are_kept(sv, dtype, R, n, H, K, D, C):
         half = torch.arange(C - n + 1, C + 1, device=DEV)
         half = ((half + 1) // 2 / half.double())[:, None, None].expand_as(again[1])
         check(again[1], half, half * (bound + roundings), "a row of its own")
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("R,n,H,K,D,C", [(2, 90, 8, 2, 64, 700), (1, 200, 16, 1, 128, 2000), (20, 70, 4, 4, 96, 20000),
+                                         (3, 33, 36, 4, 128, 34)])
+def test_weights_of_many_query_rows(sv, dtype, R, n, H, K, D, C):
+    """Accumulated weights change nothing of the outputs, and are those of keys that the inputs' type does not hold."""
+    q, scale, ck, cv, share, weights, bound = alternating(sv, dtype, R, n, H, K, D, C, fine=dtype != torch.bfloat16)
+    plain = sv.quantized_attention(q, ck, cv, scale=scale)
+    w = torch.zeros((R, K, C), device=DEV)
+    got = sv.quantized_attention(q, ck, cv, scale=scale, weights=w)
+    want = share[None, :, None, None].expand_as(got)
+    roundings = U[dtype] + (2 * 2.0 ** -11 if dtype != torch.float32 else 0.0)
+    check(plain, want, want * (bound + roundings))
+    check(got, want, want * (bound + roundings))
+    check(w, (H // K * weights).expand_as(w), (H // K * weights * bound).expand_as(w), "weights")
