@@ -186,7 +186,7 @@ __global__ void __launch_bounds__(NT) kv_quantize_kernel(const __grid_constant__
   uint32_t word[2] = {0u, 0u};
   uint32_t pair[2] = {0u, 0u};
   float scale = 0.f, mid = 0.f, inv = 0.f, base = 0.f;
-  bool none = true, plain = true;
+  bool none = true, all_plain = true;
 #pragma unroll
   for (int e = 0; e < 2; ++e) {
     if (!e || !wide) {
@@ -203,9 +203,10 @@ __global__ void __launch_bounds__(NT) kv_quantize_kernel(const __grid_constant__
       base = -mid * inv;
       // What is off from the whole number by rounding stays within 2^-17 in one step where mid is not many scales
       // away; and no code leaves its range where the extremes' do not.
-      plain = fabsf(base) <= 32.f && fmaf(hi[e], inv, base) < 7.4f && fmaf(lo[e], inv, base) > -8.4f;
+      const bool plain = fabsf(base) <= 32.f && fmaf(hi[e], inv, base) < 7.4f && fmaf(lo[e], inv, base) > -8.4f;
       pair[e] = none ? 0u : bad ? 0x7e007e00u : (uint32_t)__half_as_ushort(s16) | (uint32_t)__half_as_ushort(m16) << 16;
       none = none || bad;
+      all_plain = __all_sync(0xffffffffu, plain || none);
     }
     if (has[e] && !none) {
       // The whole number next to q by adding 1.5 2^23 (and 8): its last bits are the code then.
@@ -213,7 +214,7 @@ __global__ void __launch_bounds__(NT) kv_quantize_kernel(const __grid_constant__
       constexpr uint32_t kBits = 0x4b400000u;
       float v[8], q[8], r[8], edge = 0.f;
       x[e].floats(v);
-      if (!__all_sync(__activemask(), plain)) {
+      if (!all_plain) {
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
           v[k] = fminf(fmaxf(v[k], -kRecordMost), kRecordMost);
