@@ -53,6 +53,14 @@ __device__ __forceinline__ bool half_sure(float x, __half& h) {
   return (bits & 0x1fffu) - (0x1000u - 8u) > 16u && (bits & 0x7fffffffu) >= 0x38800000u;
 }
 
+// (h - l) / 15 rounded once to float16.  Where the difference does not fit 64 bits its last bit stands for the rest: on
+// neither side of a border of float16 (a fifteenth of which has 16 bits) does the quotient reach it then.
+__device__ __noinline__ __half fifteenth(float h, float l) {
+  double d = __dsub_rd((double)h, (double)l);
+  if (d != __dsub_ru((double)h, (double)l)) d = __longlong_as_double(__double_as_longlong(d) | 1);
+  return __double2half(d / 15.0);
+}
+
 __device__ __noinline__ bool above_exactly(float x, float mid, float scale, float half) {
   return (double)x > (double)mid + (double)half * (double)scale;  // exact: 11 bits and 16, 30 binades
 }
@@ -195,7 +203,7 @@ __global__ void __launch_bounds__(NT) kv_quantize_kernel(const __grid_constant__
       const bool bad = !none && !(lo[e] > -INFINITY && hi[e] < INFINITY);
       const float l = fminf(fmaxf(lo[e], -kRecordMost), kRecordMost), h = fminf(fmaxf(hi[e], -kRecordMost), kRecordMost);
       __half s16, m16;
-      if (!half_sure((h - l) * (1.f / 15.f), s16)) s16 = __double2half(((double)h - (double)l) / 15.0);
+      if (!half_sure((h - l) * (1.f / 15.f), s16)) s16 = fifteenth(h, l);
       scale = __half2float(s16);
       if (!half_sure(fmaf(8.f, scale, l), m16)) m16 = __double2half((double)l + 8.0 * (double)scale);
       mid = __half2float(m16);
