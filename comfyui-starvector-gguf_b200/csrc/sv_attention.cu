@@ -13,7 +13,11 @@ namespace {
 constexpr int kSMs = 148;
 constexpr int kMostPrefixSplits = 16;  // that the token kernel joins
 constexpr int kMostSlots = 1 << 29;    // sums of two slot numbers stay in 31 bits
-constexpr int kMostRecordGroups = 4;   // groups of query rows that the kernel over 4-bit records takes one by one
+// Groups of query rows that the kernel over 4-bit records takes one by one; more go through plain values.  16 units over
+// 4097 slots, bfloat16: 63 rows 71 us (four groups); 72 rows 94 us from plain values, 86 us in five groups; 90 rows 95 and
+// 101 us, 126 rows 96 and 131 us.  4 x 4 units over 16384 slots: 63 rows 61 us, 72 rows 107 and 72 us, 126 rows 107 and 106 us,
+// 189 rows 121 and 152 us.
+constexpr int kMostRecordGroups = 4;
 constexpr size_t kMostValues = (size_t)96 << 20;  // bytes of plain values of 4-bit records at a time: they stay in L2
 constexpr size_t kMostScores = (size_t)256 << 20;  // bytes of scores kept for the accumulated weights
 

@@ -1,8 +1,8 @@
 // sv_attention_record.cu -- attention of few query rows per key/value head over the
-// cache held in 4 bits (sv_record.cuh): single tokens and drafts, float16 / bfloat16, one
-// pass over the records at memory speed.
+// cache held in 4 bits (sv_record.cuh): single tokens and drafts.  A unit's records are read once; rows
+// past 16 of a head (float32: 8) are units of their own, up to four, each of which reads them again.
 //
-// Mathematics.  Row m of a unit (cache row r, key/value head h, eight to 32 of its query rows):
+// Mathematics.  Row m of a unit (cache row r, key/value head h, 8 or 16 of its query rows):
 // with a key's groups k_d = mid_g + scale_g (c_d - 8),
 //   q . k = sum_g scale_g (sum_{d in g} q_d c_d - 8 sum_{d in g} q_d) + sum_g mid_g sum_{d in g} q_d.
 // The codes are whole numbers below 16, which float16 holds exactly: a nibble masked out
@@ -11,7 +11,7 @@
 // tensor core takes it.  The queries are brought into float16's upper range by a power of two
 // per row, which loses nothing of a bfloat16.  The scales multiply the groups' sums in f32; the rest,
 // sum_g (mid_g - 8 scale_g) times the queries' group sums, is one product more, whose A operand is the
-// record's pairs as they lie (the group sums in two halves).  So scores are as exact as those of f32 keys.
+// record's pairs as they lie (the group sums in two halves, 22 bits).  So scores are as exact as those of f32 keys.
 // Values are formed in float16, v = scale (c - 8) + mid rounded once, and the weights rounded to
 // float16, for float16 outputs in two halves: one such rounding is about what the output's own adds (error of
 // one token's output 0.0003 against 64 bits, 0.0002 that of the output's rounding alone; with both 0.00032).
@@ -26,13 +26,13 @@
 // (movmatrix).
 //
 // What bounds it: the instructions that turn codes into operands, and the products.  128 dimensions, cycles of a
-// scheduler per 16 slots (the memory's rate allows 450): 524 to 540 with four query rows (5.3 to 5.5 TB/s of
-// records), 679 with nine, of which about 300 are the products' and 300 the integer instructions'.  64 rows of 36/4
-// heads over 4096 slots take 64 us (2.6 TB/s; floor 26 us), 8 rows over up to 16384 slots 28 us (floor 9.6), of
+// scheduler per 16 slots (the memory's rate allows 450): 532 with four query rows (5.4 TB/s of
+// records), 727 with nine, of which about 300 are the products' and 300 the integer instructions'.  64 rows of 36/4
+// heads over 4096 slots take 66 us (2.6 TB/s; floor 26 us), 8 rows over up to 16384 slots 29 us (floor 9.6), of
 // which start, units' ends and joins are a large part.
 // A warp takes tiles of 16 or 32 slots through a ring in shared memory of its own (cp.async, zeros for slots past
 // the end): registers alone would keep too few bytes in flight, since 16 slots are only 2560.  Rows of a tile are taken in an order in which neither the keys' nor the
-// values' reads meet in a bank (kSlot).
+// values' reads meet in a bank (slot_at).
 //
 // Work split and joins as in sv_attention_token.cu: one list of chunks (a tile per warp) over all
 // units, cut into equal parts, one per block; the last block to arrive joins a unit that
@@ -189,7 +189,7 @@ template <int TK> __device__ __noinline__ RowTiles row_tiles(const AttnArgs& a, 
 }
 
 // Empty places of the list behind every unit's chunks, where blocks take eight and more: what beginning and ending a
-// unit costs, so that blocks of many units get fewer chunks (64 rows over 4096 slots 64 us, 66 without: some blocks
+// unit costs, so that blocks of many units get fewer chunks (64 rows over 4096 slots 64 us, 66 without, when they came in: some blocks
 // worked 8 us longer).
 constexpr int kBetween = 2;
 
@@ -316,7 +316,7 @@ __global__ void __launch_bounds__(NW * 32, 1)
   // The place f by slots (the end of a unit, sinks, other strides), or none; then what comes after it.
   auto fetch_slots = [&]() {
     if (f_place >= c1) return;
-    const int tile = f.k * NW + warp, f_hi = f.rt.ta + (f.rt.b1 - f.rt.b0) / TK;
+    const int tile = f.k * NW + warp;
     const int64_t base = f.r * a.kv_row + (f.h / row_groups) * a.kv_head;
     if (tile < f.rt.tiles) {
       const bool in_a = tile < f.rt.ta;
@@ -995,7 +995,7 @@ cudaError_t record(const AttnArgs& a, int row_groups, cudaStream_t stream) {
 
 template <typename T, int NI, bool MULTI> cudaError_t record_rows(const AttnArgs& a, const RecordRows& x, cudaStream_t stream) {
   if constexpr (!std::is_same<T, float>::value) {
-    // Tiles of 32 slots where blocks take many (679 cycles per 16 slots and scheduler, 798 with tiles of 16); of
+    // Tiles of 32 slots where blocks take many (679 cycles per 16 slots and scheduler, 798 with tiles of 16, when they came in); of
     // 16 where that gives each chunk of 128 slots a block, and a unit not more than 16 to be joined (two rows over 516 slots
     // 10.7 us, 12.0 with 32; one row over 4096 slots 17.7 us, 14.2 with 32).
     if (x.tiles == 2)

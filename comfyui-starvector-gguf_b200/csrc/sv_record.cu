@@ -379,7 +379,8 @@ template <typename T> cudaError_t read_records(const ReadArgs& a, cudaStream_t s
   int u, s;
   const int64_t units = (int64_t)a.rows * a.kv_heads;
   auto go = [&](auto one, auto four, int lps_log2) {
-    // Four slots a thread where that leaves two blocks per SM.
+    // Four slots a thread where that leaves two blocks per SM (4 x 4096 slots of four heads of 128 in bfloat16 8.2 us, 10.9
+    // with one; of one head 2.1 with one, 2.75 with four; float32 gains nothing: 23.2 us for the former, 19.8 with one).
     dim3 grid = grid_of(lps_log2, units, a.tokens, a.out[1] != nullptr, u, s);
     if (u == 0 && (int64_t)grid.x * grid.y * grid.z >= 8 * 148) {
       grid.x = (grid.x + 3) / 4;

@@ -18,8 +18,6 @@ namespace sv {
 __host__ __device__ constexpr int record_dims(int dim) { return (dim + 31) / 32 * 32; }
 __host__ __device__ constexpr int record_codes(int dim) { return record_dims(dim) / 2; }
 __host__ __device__ constexpr int record_bytes(int dim) { return record_codes(dim) + 16; }
-// Dimensions of a pair, as a power of two.
-__host__ __device__ constexpr int record_group_log2(int dim) { return dim > 64 ? 5 : 4; }
 
 constexpr float kRecordMost = 32768.f;  // finite values beyond count as this: what they stand for stays in float16
 

@@ -7,8 +7,8 @@
 // exceptions as before).  Shapes and the history form are decided by the Python
 // wrappers (ops.py), which pass the same sizes and strides as the C signatures;
 // nothing here synchronises or allocates.  The cache operators (window_attention,
-// prefix_attention, quantized_attention, kv_quantize, kv_dequantize, kv_evict) are called once per layer or token, where each tensor
-// attribute read from Python counts: they look at the shapes here (ValueError where
+// prefix_attention, quantized_attention, kv_quantize, kv_dequantize, kv_evict) are called
+// once per layer or token, where each tensor attribute read from Python counts: they look at the shapes here (ValueError where
 // ops.py would raise one) and allocate their outputs, the attention functions also a
 // workspace kept per device, stream and size.
 #include <ATen/cuda/CUDAContext.h>
